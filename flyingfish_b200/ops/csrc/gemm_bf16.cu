@@ -15,6 +15,7 @@
 #include "ptx.cuh"
 #include "comm.cuh"
 #include "host_util.h"
+#include "launchers.h"
 
 namespace ff {
 
@@ -138,7 +139,22 @@ struct LinTail {
   const int* slots;
   __nv_bfloat16 *kcache, *vcache;
   int hq, hkv, rhalf, block_size, num_blocks;
+  // added to the FP32 sums of rows whose id is within [0, adapters): delta[row][column], pitch ldd (lora.cu)
+  const float* delta; const int* ids; int ldd, adapters;
 };
+
+// n (a multiple of 8) columns from `col` of a row's delta; N is a multiple of 8
+template <int n>
+__device__ __forceinline__ void add_delta(uint32_t* r, const float* drow, int col, int N) {
+#pragma unroll
+  for (int j = 0; j < n; j += 8)
+    if (col + j < N) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(drow + col + j)), y = __ldcg(reinterpret_cast<const float4*>(drow + col + j) + 1);
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[j + i] = __float_as_uint(__uint_as_float(r[j + i]) + v[i]);
+    }
+}
 
 constexpr int RS_STG_PITCH = 144, RS_STG_BYTES = 32 * RS_STG_PITCH;   // COMM 2 epilogue staging, per warp
 constexpr int COMM_PARTS = 4;       // a 128-row block is pushed (COMM 1) / reduced (COMM 2) in this many pieces
@@ -146,9 +162,12 @@ constexpr int COMM_PARTS = 4;       // a 128-row block is pushed (COMM 1) / redu
 // An epilogue thread's row of a finished tile: tensor memory -> registers -> global. row: row of the result, stored where `live`; col0: first
 // of the tile's `width` columns (a multiple of 32, of 128 with epi 1 and 3), N: columns (of the head), col_off: first column of the head. The PARTS
 // warps that share the row take turns with its groups of columns.
-template <int PARTS>
+template <int PARTS, bool DELTA>
 __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict__ Cout, int row, bool live, int ldc, int N, int epi, int col0,
                                                int width, size_t col_off, const LinTail& tail, int part, int* status) {
+  const float* drow = nullptr;
+  if constexpr (DELTA)
+    if (live && (unsigned)tail.ids[row] < (unsigned)tail.adapters) drow = tail.delta + (size_t)row * tail.ldd;
   if (epi == 1) {
     const int half = width / 2, out0 = col0 / 2;
     __nv_bfloat16* crow = reinterpret_cast<__nv_bfloat16*>(Cout) + (size_t)row * ldc + out0;
@@ -160,6 +179,7 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
       tmem_ld_x16(taddr + gc, g);
       tmem_ld_x16(taddr + gc + 64, u);
       tmem_ld_wait();
+      if (DELTA && drow != nullptr) { add_delta<16>(g, drow, col0 + gc, N); add_delta<16>(u, drow, col0 + gc + 64, N); }
       if (live) {
         uint32_t o[8];
 #pragma unroll
@@ -228,6 +248,7 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
         tmem_ld_x16(taddr + h0 + c, a);
         tmem_ld_x16(taddr + h0 + c + 64, b);
         tmem_ld_wait();
+        if (DELTA && drow != nullptr) { add_delta<16>(a, drow, col0 + h0 + c, N); add_delta<16>(b, drow, col0 + h0 + c + 64, N); }
         if (live) {
           __nv_bfloat16* cached = nullptr;
           if (blk >= 0 && head >= tail.hq) {
@@ -290,6 +311,7 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
       uint32_t r[32];
       tmem_ld_x32(taddr + c, r);
       tmem_ld_wait();
+      if (DELTA && drow != nullptr) add_delta<32>(r, drow, col0 + c, N);
       if (tail.bias != nullptr) {
         const int col = col0 + c;
         if (col + 32 <= N) {
@@ -360,7 +382,7 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
   }
 }
 
-template <int BN, int STAGES, int COMM>
+template <int BN, int STAGES, int COMM, bool DELTA = false>
 __global__ void __launch_bounds__(COMM == 2 ? 192 : 320, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1,
                  const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmB, void* __restrict__ Cout, int M, int N, int K, int ldc, int epi,
@@ -510,7 +532,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           tma_store_wait<0>();                              // every row of this tile has landed in the owner's slot
           asm volatile("fence.proxy.async;" ::: "memory");
       } else {
-        store_tile_row<COMM ? 1 : 2>(taddr, Cout, row, row < row_end, ldc, N, epi, tn * BN, BN, (size_t)head * ga.c_cols, tail, COMM ? 0 : (warp - 2) >> 2, status);
+        store_tile_row<COMM ? 1 : 2, DELTA>(taddr, Cout, row, row < row_end, ldc, N, epi, tn * BN, BN, (size_t)head * ga.c_cols, tail, COMM ? 0 : (warp - 2) >> 2, status);
       }
       tc_fence_before();
       __syncwarp();
@@ -676,7 +698,7 @@ __device__ __forceinline__ void pair_tile(const PairTiles& pt, int t, int tiles_
   else { tile_coords(t - n1, tiles_m, tiles_n2, tm, tn); col0 = pt.wide * pt.w1 + tn * pt.w2; width = pt.w2; }
 }
 
-template <int PARTS>
+template <int PARTS, bool DELTA>
 __global__ void __launch_bounds__(64 + 128 * PARTS, 1)
 gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmB2,
                       void* __restrict__ Cout, int M, int N, int K, int ldc, int epi, const PairTiles pt, int stages, int* status, LinTail tail) {
@@ -771,7 +793,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       if (!ok) break;
       tc_fence_after();
       const int row = (2 * tm + rank) * BM + q * 32 + lane;
-      store_tile_row<PARTS>(tmem_base + (uint32_t(q * 32) << 16) + acc * 256, Cout, row, row < M, ldc, N, epi, col0, width, 0, tail, (warp - 2) >> 2, status);
+      store_tile_row<PARTS, DELTA>(tmem_base + (uint32_t(q * 32) << 16) + acc * 256, Cout, row, row < M, ldc, N, epi, col0, width, 0, tail, (warp - 2) >> 2, status);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_leader(&bars.tmem_empty[acc]);
@@ -877,7 +899,8 @@ static int pair_launch(const CUtensorMap& tmA, const void* W, void* Y, int M, in
   const int stages = fit == 7 && K <= 1536 ? 6 : fit < PAIR_STAGES ? fit : PAIR_STAGES;
   constexpr int SMEM = PAIR_RING + 1024;
   const bool stores = (epi == 0 || epi == 2) && tail.bias == nullptr && tail.act == 0 && tail.mul == nullptr;
-  auto kern = stores ? gemm_bf16_pair_kernel<1> : gemm_bf16_pair_kernel<2>;
+  auto kern = tail.delta != nullptr ? (stores ? gemm_bf16_pair_kernel<1, true> : gemm_bf16_pair_kernel<2, true>)
+                                    : (stores ? gemm_bf16_pair_kernel<1, false> : gemm_bf16_pair_kernel<2, false>);
   if (int e = opt_in_smem(kern, SMEM)) return e;
   if (int e = launch_pdl(kern, dim3(grid), dim3(stores ? 192 : 320), SMEM, stream, 2, tmA, tmB1, tmB2, Y, M, N, K, ldy, epi, pt, stages, status, tail)) return e;
   return launch_result();
@@ -903,7 +926,7 @@ static int gemm_bf16_launch(const void* X, const void* W, void* Y, int M, int N,
     CUtensorMap tmB;
     if (int e = make_tmap_2d(&tmB, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, K, N, (uint64_t)ldw * 2, BK, BN)) return e;
     const int smem = STAGES * (BM + BN) * BK * 2 + 1024, tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-    auto kern = gemm_bf16_kernel<BN, STAGES, 0>;
+    auto kern = tail.delta != nullptr ? gemm_bf16_kernel<BN, STAGES, 0, true> : gemm_bf16_kernel<BN, STAGES, 0, false>;
     if (int e = opt_in_smem(kern, smem)) return e;
     kern<<<tiles < sm_count() ? tiles : sm_count(), 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, M, N, K, ldy, epi, status, CommArgs{}, GroupArgs{}, tail);
     return launch_result();
@@ -930,17 +953,25 @@ FF_EXPORT int ff_gemm_bf16_act(const void* X, const void* W, void* Y, int M, int
                           status, stream);
 }
 
+static int rope_tail(LinTail& tail, const QkvRope* r, int N) {
+  if (r == nullptr || r->hq <= 0 || r->hkv <= 0 || N != (r->hq + 2 * r->hkv) * 128 || r->rot_dim <= 0 || r->rot_dim > 128 || r->rot_dim % 2 ||
+      r->block_size <= 0 || r->num_blocks <= 0) return FF_HOST_BAD_SHAPE;
+  if (r->cos_sin == nullptr || r->slots == nullptr || (reinterpret_cast<uintptr_t>(r->cos_sin) & 7) ||
+      ((reinterpret_cast<uintptr_t>(r->kcache) | reinterpret_cast<uintptr_t>(r->vcache)) & 15)) return FF_HOST_BAD_ALIGN;
+  tail.cos_sin = reinterpret_cast<const float2*>(r->cos_sin); tail.slots = r->slots;
+  tail.kcache = static_cast<__nv_bfloat16*>(r->kcache); tail.vcache = static_cast<__nv_bfloat16*>(r->vcache);
+  tail.hq = r->hq; tail.hkv = r->hkv; tail.rhalf = r->rot_dim / 2; tail.block_size = r->block_size; tail.num_blocks = r->num_blocks;
+  return FF_HOST_OK;
+}
+
 // QKV product with rotary embedding and paged cache write in the epilogue (heads of 128, N = (hq + 2 hkv) * 128): the bits of ff_gemm_bf16 and
 // ff_rope_kv_paged. cos_sin: [M, rot_dim / 2] pairs from ff_rope_table; caches [blocks, hkv, block_size, 128]; negative slots are skipped.
 FF_EXPORT int ff_gemm_bf16_rope_kv(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, const float* cos_sin,
                                    const int* slots, void* kcache, void* vcache, int hq, int hkv, int rot_dim, int block_size, int num_blocks,
                                    int* status, cudaStream_t stream) {
-  if (hq <= 0 || hkv <= 0 || N != (hq + 2 * hkv) * 128 || rot_dim <= 0 || rot_dim > 128 || rot_dim % 2 || block_size <= 0 || num_blocks <= 0) return FF_HOST_BAD_SHAPE;
-  if (cos_sin == nullptr || slots == nullptr || (reinterpret_cast<uintptr_t>(cos_sin) & 7) || ((reinterpret_cast<uintptr_t>(kcache) | reinterpret_cast<uintptr_t>(vcache)) & 15)) return FF_HOST_BAD_ALIGN;
+  const QkvRope rope = {cos_sin, slots, kcache, vcache, hq, hkv, rot_dim, block_size, num_blocks};
   LinTail tail = {};
-  tail.cos_sin = reinterpret_cast<const float2*>(cos_sin); tail.slots = slots;
-  tail.kcache = static_cast<__nv_bfloat16*>(kcache); tail.vcache = static_cast<__nv_bfloat16*>(vcache);
-  tail.hq = hq; tail.hkv = hkv; tail.rhalf = rot_dim / 2; tail.block_size = block_size; tail.num_blocks = num_blocks;
+  if (int e = rope_tail(tail, &rope, N)) return e;
   return gemm_bf16_launch(X, W, Y, M, N, K, ldx, ldw, ldy, 3, tail, status, stream);
 }
 
@@ -953,6 +984,20 @@ FF_EXPORT int ff_gemm_bf16_gated(const void* X, const void* W, void* Y, int M, i
   tail.gate = gate;
   tail.limit = limit;
   return gemm_bf16_launch(X, W, Y, M, N, K, ldx, ldw, ldy, 1, tail, status, stream);
+}
+
+// Y = X Wᵀ + delta for the rows whose id lies within [0, adapters) (lora.cu), one rounding; epi 0, 1 or 3 (`rope`) as above. delta: FP32, pitch ldd,
+// N a multiple of 8.
+int ff_gemm_bf16_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, const float* delta, const int* ids, int ldd,
+                       int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status, cudaStream_t stream) {
+  if (delta == nullptr || ids == nullptr || N % 8 || ldd % 8 || ldd < N || (reinterpret_cast<uintptr_t>(delta) & 15)) return FF_HOST_BAD_ALIGN;
+  LinTail tail = {};
+  tail.gate = gate; tail.limit = limit;
+  tail.delta = delta; tail.ids = ids; tail.ldd = ldd; tail.adapters = adapters;
+  if (epi == 3) {
+    if (int e = rope_tail(tail, rope, N)) return e;
+  }
+  return gemm_bf16_launch(X, W, Y, M, N, K, ldx, ldw, ldy, epi, tail, status, stream);
 }
 
 // Block-diagonal product: for every head h, Y[:, h * c_cols + (0..N)] = X[:, h * a_cols + (0..K)] · W[h]ᵀ with W [heads * N, K]. Columns of

@@ -57,11 +57,32 @@ struct SkinnyTail {
   const __nv_bfloat16* bias; int act;
   const __nv_bfloat16* mul; const int* mul_rows; int ldm, mul_table;
   int gate; float limit;
+  // added to the FP32 sums of rows whose id is within [0, adapters): delta[row][column], pitch ldd, written by the kernel in front of this one
+  const float* delta; const int* ids; int ldd, adapters;
 };
 
+// eight columns of a row's delta, where it has one
+__device__ __forceinline__ void add_delta8(const SkinnyTail& tail, int t, int col, float (&v)[8]) {
+  if ((unsigned)tail.ids[t] >= (unsigned)tail.adapters) return;
+  const float4* d = reinterpret_cast<const float4*>(tail.delta + (size_t)t * tail.ldd + col);
+  const float4 x = __ldcg(d), y = __ldcg(d + 1);
+  v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+  v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+}
+
 // emit_pair with the choice of the gate
+template <bool DELTA>
 __device__ __forceinline__ void emit_gated(const SkinnyEpi& ep, const SkinnyTail& tail, __nv_bfloat16* __restrict__ Y, int N, int ldy, int t, int tile, int j8,
                                            const float* lo, const float* hi, int* status) {
+  if constexpr (DELTA) {
+    float dl[8], dh[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { dl[j] = lo[j]; dh[j] = hi[j]; }
+    add_delta8(tail, t, tile * 128 + j8 * 8, dl);           // N is a multiple of 128: whole tiles
+    add_delta8(tail, t, tile * 128 + 64 + j8 * 8, dh);
+    emit_gated<false>(ep, tail, Y, N, ldy, t, tile, j8, dl, dh, status);
+    return;
+  }
   if (tail.gate == 0) { emit_pair(ep, Y, N, ldy, t, tile, j8, lo, hi, status); return; }
   const int col = tile * 64 + j8 * 8;
   if (col >= N / 2) return;
@@ -74,7 +95,7 @@ __device__ __forceinline__ void emit_gated(const SkinnyEpi& ep, const SkinnyTail
 }
 
 // Where the final values of a tile go: Y, or (FUSE_AR) the arena slot of this rank on every rank.
-template <bool FUSE_AR>
+template <bool FUSE_AR, bool DELTA = false>
 struct TileSink {
   __nv_bfloat16* Y; int N, ldy; bool vec8;      // vec8: 16-byte stores of eight values are aligned
   SkinnyTail tail;
@@ -88,6 +109,7 @@ struct TileSink {
 #pragma unroll
     for (int j = 0; j < 8; ++j) a[j] = sums[j];
     if (!FUSE_AR) {
+      if constexpr (DELTA) add_delta8(tail, t, col, a);
       const int act = tail.act;
       if (tail.bias != nullptr) {
 #pragma unroll
@@ -253,7 +275,7 @@ __device__ __forceinline__ void allreduce_tile(const TileSink<true>& sink, int M
 
 // cl_size == 1: persistent stream-K over gridDim.x CTAs.  cl_size > 1: cluster split-K, cluster c
 // owns weight tile c, CTA r of it the k-blocks [kblocks*r/S, kblocks*(r+1)/S).
-template <bool FUSE_AR>
+template <bool FUSE_AR, bool DELTA>
 __global__ void __launch_bounds__(192, 2)
 gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                    __nv_bfloat16* __restrict__ Y, int M, int N, int K, int ldy, int ntok, int tile_rows, int stages,
@@ -320,7 +342,9 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   if (warp == 0) {
     if (elect_one()) {
       const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      pdl_wait();
+      // With a delta the kernel in front of this one has let it start only once everything before that kernel was done (lora.cu): X is there, and
+      // the weights stream while the delta is computed. The epilogue waits.
+      if (!DELTA) pdl_wait();
       FF_TL(status, KID_GEMM_SKINNY, 3);
       uint32_t it = 0; RingPos rp; bool ok = true;
       long long u = u0; Segment sg;
@@ -376,7 +400,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     if (e == 0) FF_TL(status, KID_GEMM_SKINNY, 7);
     int ar_epoch = 0;
     if (FUSE_AR) ar_epoch = ld_volatile(arena_epoch(ar)) + 1;
-    TileSink<FUSE_AR> sink;
+    TileSink<FUSE_AR, DELTA> sink;
     sink.Y = Y; sink.N = N; sink.ldy = ldy; sink.ar = ar; sink.parity = ar_epoch & 1;
     sink.tail = tail;
     sink.vec8 = FUSE_AR || ((ldy % 8 == 0) && ((reinterpret_cast<uintptr_t>(Y) & 15) == 0));
@@ -427,7 +451,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             if (t_own < M) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                emit_gated(ep, tail, Y, N, ldy, t_own, sg.tile, (c >> 3) + h, reinterpret_cast<const float*>(g) + 8 * h,
+                emit_gated<DELTA>(ep, tail, Y, N, ldy, t_own, sg.tile, (c >> 3) + h, reinterpret_cast<const float*>(g) + 8 * h,
                           reinterpret_cast<const float*>(u) + 8 * h, status);
             }
           }
@@ -530,7 +554,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 #pragma unroll
             for (int g = 0; g < 4; g += 2) {
               const int pr = i0 + 128 * (g >> 1);
-              if (pr < i_end) emit_gated(ep, tail, Y, N, ldy, pr >> 3, sg.tile, pr & 7, a8[g], a8[g + 1], status);
+              if (pr < i_end) emit_gated<DELTA>(ep, tail, Y, N, ldy, pr >> 3, sg.tile, pr & 7, a8[g], a8[g + 1], status);
             }
           } else {
 #pragma unroll
@@ -568,7 +592,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
               lo[0] += l0.x; lo[1] += l0.y; lo[2] += l0.z; lo[3] += l0.w; lo[4] += l1.x; lo[5] += l1.y; lo[6] += l1.z; lo[7] += l1.w;
               hi[0] += h0.x; hi[1] += h0.y; hi[2] += h0.z; hi[3] += h0.w; hi[4] += h1.x; hi[5] += h1.y; hi[6] += h1.z; hi[7] += h1.w;
             }
-            emit_gated(ep, tail, Y, N, ldy, crank + ti * cl_size, sg.tile, j8, lo, hi, status);
+            emit_gated<DELTA>(ep, tail, Y, N, ldy, crank + ti * cl_size, sg.tile, j8, lo, hi, status);
           }
         } else
         for (int i = e; i < rows * vpr; i += 128) {
@@ -652,7 +676,7 @@ static int skinny_max_clusters(int s) {
   if (s < 2 || s > 8) return 0;
   int* cached = cache[current_device()];
   if (cached[s] >= 0) return cached[s];
-  auto kern = gemm_skinny_kernel<false>;
+  auto kern = gemm_skinny_kernel<false, false>;
   if (opt_in_smem(kern, SK_SMEM_FULL + 1024)) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(s * 64); cfg.blockDim = dim3(192); cfg.dynamicSmemBytes = SK_SMEM_FULL + 1024;
@@ -892,13 +916,13 @@ static int gemm_skinny_launch(const void* X, const void* W, void* Y, int M, int 
   const int smem = cfg.pipe_off + cfg.stages * (ntok + cfg.tile_rows) * SBK * 2 + skinny_tail_slack(ntok, cfg.tile_rows) + 1024;
   __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(Y);
   if (arena == nullptr) {
-    auto kern = gemm_skinny_kernel<false>;
+    auto kern = tail.delta != nullptr ? gemm_skinny_kernel<false, true> : gemm_skinny_kernel<false, false>;
     r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
     PeerArena none = {};
     return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
                       cfg.stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail);
   }
-  auto kern = gemm_skinny_kernel<true>;
+  auto kern = gemm_skinny_kernel<true, false>;
   r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
   return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
                     cfg.stages, cl, cfg.pipe_off, scratch, counters, status, *arena, ep, tail);
@@ -956,6 +980,27 @@ FF_EXPORT int ff_gemm_skinny_rope_kv(const void* X, const void* W, void* Y, int 
   ep.kcache = static_cast<__nv_bfloat16*>(kcache); ep.vcache = static_cast<__nv_bfloat16*>(vcache);
   ep.hq = hq; ep.hkv = hkv; ep.rot_dim = rot_dim; ep.block_size = block_size; ep.num_blocks = num_blocks;
   return gemm_skinny_launch(X, W, Y, M, N, K, ldx, ldw, ldy, grid, scratch, counters, status, stream, nullptr, &ep);
+}
+
+// Y = X Wᵀ + delta for the rows whose id lies within [0, adapters) (lora.cu), one rounding. epi 0: plain, 1: gate / up with the activation (`gate`,
+// `limit`), 2: rotary embedding and cache write (`rope`). delta: FP32, pitch ldd (a multiple of 8, at least N rounded up to 8), written by a kernel
+// that was launched directly in front and that triggers its dependents behind its own wait. `grid` from ff_gemm_skinny_plan(_epi).
+int ff_gemm_skinny_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, int grid, float* scratch, int* counters,
+                         const float* delta, const int* ids, int ldd, int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status,
+                         cudaStream_t stream) {
+  if (delta == nullptr || ids == nullptr || ldd % 8 || ldd < (N + 7) / 8 * 8 || (reinterpret_cast<uintptr_t>(delta) & 15)) return FF_HOST_BAD_ALIGN;
+  SkinnyTail tail = {};
+  tail.gate = gate; tail.limit = limit;
+  tail.delta = delta; tail.ids = ids; tail.ldd = ldd; tail.adapters = adapters;
+  SkinnyEpi ep = {};
+  ep.mode = epi;
+  if (epi == 2) {
+    if (rope == nullptr || rope->hq <= 0 || rope->hkv <= 0 || N != (rope->hq + 2 * rope->hkv) * 128 || rope->rot_dim > 128 || rope->rot_dim % 2) return FF_HOST_BAD_SHAPE;
+    ep.cos_sin = reinterpret_cast<const float2*>(rope->cos_sin); ep.slots = rope->slots;
+    ep.kcache = static_cast<__nv_bfloat16*>(rope->kcache); ep.vcache = static_cast<__nv_bfloat16*>(rope->vcache);
+    ep.hq = rope->hq; ep.hkv = rope->hkv; ep.rot_dim = rope->rot_dim; ep.block_size = rope->block_size; ep.num_blocks = rope->num_blocks;
+  }
+  return gemm_skinny_launch(X, W, Y, M, N, K, ldx, ldw, ldy, grid, scratch, counters, status, stream, nullptr, epi ? &ep : nullptr, tail);
 }
 
 // Row-parallel projection fused with the tensor-parallel all-reduce (decode shapes, M <= 128):

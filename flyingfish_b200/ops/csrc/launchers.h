@@ -15,6 +15,19 @@ FF_EXPORT int ff_gemm_skinny_rope_kv(const void* X, const void* W, void* Y, int 
                                      const float* cos_sin, const int* slots, void* kcache, void* vcache, int hq, int hkv, int rot_dim, int block_size,
                                      int num_blocks, int* status, cudaStream_t stream);
 
+// rotary embedding and cache write of a QKV product with heads of 128 (cos_sin from ff_rope_table)
+struct QkvRope {
+  const float* cos_sin; const int* slots; void *kcache, *vcache;
+  int hq, hkv, rot_dim, block_size, num_blocks;
+};
+int ff_gemm_skinny_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, int grid, float* scratch, int* counters,
+                         const float* delta, const int* ids, int ldd, int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status,
+                         cudaStream_t stream);
+
+// gemm_bf16.cu
+int ff_gemm_bf16_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, const float* delta, const int* ids, int ldd,
+                       int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status, cudaStream_t stream);
+
 // attention_tc.cu
 FF_EXPORT int ff_attn_prefill_tc(const void* q, const void* kcache, const void* vcache, const int* block_table, const int* q_start, const int* q_lens,
                                  const int* ctx_lens, void* out, int batch, int total_rows, int max_q_len, int hq, int hkv, int dk, int dv, int ldq, int ldo,

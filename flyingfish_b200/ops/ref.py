@@ -355,6 +355,17 @@ def philox_uniform(n: int, seed: int, offset: int = 0) -> torch.Tensor:
     return torch.tensor(out[:n], dtype=F32)
 
 
+def linear_lora(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    """``x W^T`` plus every row's own ``scale (x A^T) B^T``; ids outside the stack: none."""
+    x32 = x.to(F32)
+    y = x32 @ w.to(F32).T
+    for i in range(a.shape[0]):
+        rows = torch.nonzero(ids == i).flatten()
+        if rows.numel():
+            y[rows] += (float(scale[i]) * (x32[rows] @ a[i].to(F32).T)) @ b[i].to(F32).T
+    return y.to(x.dtype)
+
+
 def sampling_probs(logits: torch.Tensor, temperature: float, top_k: int, top_p: float, rep_penalty: float = 1.0,
                    history: torch.Tensor | None = None) -> torch.Tensor:
     """Probabilities after repetition penalty, temperature, top-k and top-p for one row

@@ -1,0 +1,276 @@
+"""Adapters of many requests beside a projection: packing, refusals and the oracle on the CPU; the kernels against 64 bits on a GPU."""
+import pytest
+import torch
+
+from flyingfish_b200 import ops
+from flyingfish_b200.ops import lora_ops, ref
+from flyingfish_b200.ops.lib import KernelError
+
+BF16 = torch.bfloat16
+
+
+def _case(m, k, n, r, count, seed=0, device="cpu", dtype=BF16, pad=0):
+    g = torch.Generator().manual_seed(seed)
+    new = lambda *s: torch.randn(*s, generator=g)
+    x = torch.zeros(m, k + pad, dtype=dtype)
+    x[:, :k] = new(m, k)
+    ranks = torch.tensor([(r, max(r // 2, 1), 0, 5)[i % 4] if count > 1 else r for i in range(count)], dtype=torch.int32)
+    live = torch.arange(r)[None] < ranks[:, None]
+    a = (new(count, r, k) * k ** -0.5 * live[:, :, None]).to(dtype)
+    b = (new(count, n, r) * 0.1 * live[:, None]).to(dtype)
+    scale = torch.rand(count, generator=g) + 0.5
+    ids = torch.randint(-1, count, (m,), generator=g, dtype=torch.int32)
+    to = lambda t: t.to(device)
+    return to(x)[:, :k], to((new(n, k) * k ** -0.5).to(dtype)), lora_ops.AdapterStack(to(a), to(b), to(scale), to(ranks)), to(ids)
+
+
+def _exact(x, w, st, ids):
+    """(y, bound of a sum's error before the last rounding) in 64 bits. FP32 sums of 16-element instructions lose at most 2^-23 of the absolute sum per
+    instruction and per partial sum that is joined; t is held to 2^-17 of itself."""
+    x, w = x.double().cpu(), w.double().cpu()
+    k, r = x.shape[1], st.a.shape[1]
+    y, size = x @ w.T, (k / 16 + 64) * 2.0 ** -23 * (x.abs() @ w.abs().T)
+    for i in range(st.a.shape[0]):
+        rows = torch.nonzero(ids.cpu() == i).flatten()
+        if rows.numel():
+            a, b, s = st.a[i].double().cpu(), st.b[i].double().cpu(), float(st.scale[i])
+            y[rows] += s * (x[rows] @ a.T) @ b.T
+            size[rows] += ((k / 16 + r / 8 + 80) * 2.0 ** -23 + 2.0 ** -17) * s * (x[rows].abs() @ a.abs().T) @ b.abs().T
+    return y, size
+
+
+def _assert_near(got, y, size):
+    got = got.double().cpu()
+    off = (got - y).abs() - (size + (y.abs() + size) * 2.0 ** -8)
+    assert torch.isfinite(got).all() and off.max() <= 0, f"{off.max():.3g} over the bound"
+
+
+# ------------------------------------------------------------------------------------------
+# CPU
+# ------------------------------------------------------------------------------------------
+def test_oracle_is_the_formula():
+    x, w, st, ids = _case(37, 64, 48, 16, 5, dtype=torch.float32)
+    y = lora_ops.linear_lora(x, w, st, ids)
+    for r in range(37):
+        want = w.double() @ x[r].double()
+        if ids[r] >= 0:
+            i = int(ids[r])
+            want = want + float(st.scale[i]) * st.b[i].double() @ (st.a[i].double() @ x[r].double())
+        assert torch.allclose(y[r].double(), want, rtol=1e-5, atol=1e-5)
+
+
+def test_packed_parts_are_the_parts():
+    """A fused projection's stack gives each part's own result, side by side and interleaved; missing parts give none."""
+    g = torch.Generator().manual_seed(1)
+    k, cols = 64, [256, 64, 64]
+    mk = lambda c, r, s: (torch.randn(r, k, generator=g), torch.randn(c, r, generator=g), s)
+    adapters = [[mk(256, 8, 2.0), None, mk(64, 20, 2.0)], [mk(256, 3, 0.5), mk(64, 17, 0.25), mk(64, 3, 0.5)], [None, None, None]]
+    st = lora_ops.pack_stack(adapters, k, cols, "cpu", torch.float32)
+    assert st.a.shape == (3, 96, k) and st.ranks.tolist() == [96, 96, 0] and st.part_of.tolist() == [0, 0, 0, 0, 1, 2]
+    x = torch.randn(6, k, generator=g)
+    ids = torch.tensor([0, 1, 2, -1, 1, 0], dtype=torch.int32)
+    got = lora_ops.linear_lora(x, torch.zeros(384, k), st, ids)
+    for r, i in enumerate(ids.tolist()):
+        want = torch.cat([torch.zeros(c) if i < 0 or p is None else p[2] * (p[1] @ (p[0] @ x[r])) for p, c in zip(adapters[i], cols)])
+        assert torch.allclose(got[r], want, rtol=1e-4, atol=1e-4)
+    gate, up = mk(128, 8, 1.0), mk(128, 16, 1.0)
+    st = lora_ops.pack_stack([[gate, up]], k, [128, 128], "cpu", torch.float32, interleave=True)
+    got = lora_ops.linear_lora(x, torch.zeros(256, k), st, torch.zeros(6, dtype=torch.int32))
+    want = [torch.cat([p[1] @ (p[0] @ x[r]) for p in (gate, up)]) for r in range(6)]
+    want = torch.stack([ref.interleave_gate_up(v[:128, None], v[128:, None])[:, 0] for v in want])
+    assert torch.allclose(got, want, rtol=1e-4, atol=1e-4) and st.part_of.tolist() == [0, 1, 0, 1]
+    # b is zero where a part's columns do not look
+    for i, p in enumerate(st.part_of.tolist()):
+        for s in range(st.a.shape[1] // 16):
+            if s % st.parts != p:
+                assert not st.b[:, 64 * i: 64 * i + 64, 16 * s: 16 * s + 16].any()
+
+
+def test_refusals():
+    x, w, st, ids = _case(4, 64, 48, 16, 2)
+    bad = [(st._replace(a=st.a[:, :, :56]), ids), (st._replace(b=st.b[:, :40]), ids), (st._replace(scale=st.scale.double()), ids),
+           (st._replace(a=st.a[:, :8], b=st.b[:, :, :8]), ids), (st._replace(ranks=st.ranks.long()), ids), (st, ids.long()), (st, ids[:3]),
+           (st._replace(b=st.b.float()), ids), (st._replace(a=st.a.transpose(0, 1).contiguous().transpose(0, 1)), ids),
+           (st._replace(part_of=torch.zeros(0, dtype=torch.int32)), ids)]
+    for stack, i in bad:
+        with pytest.raises(KernelError):
+            lora_ops.linear_lora(x, w, stack, i)
+    part = (torch.randn(4, 64), torch.randn(48, 4), 1.0)
+    for adapters, cols in (([], [48]), ([[part, part]], [48]), ([[(part[0], part[1][:40], 1.0)]], [48]), ([[(part[0] * float("inf"), part[1], 1.0)]], [48]),
+                           ([[part, part]], [48, 48]), ([[(torch.zeros(1040, 64), torch.zeros(48, 1040), 1.0)]], [48])):
+        with pytest.raises(KernelError):
+            lora_ops.pack_stack(adapters, 64, cols, "cpu")
+
+
+def test_a_stack_without_rows():
+    x, w, st, ids = _case(0, 64, 48, 16, 2)
+    assert lora_ops.linear_lora(x, w, st, ids).shape == (0, 48)
+
+
+# ------------------------------------------------------------------------------------------
+# GPU
+# ------------------------------------------------------------------------------------------
+SIZES = [(1, 64, 64, 16, 1), (1, 4096, 1000, 32, 3), (2, 72, 8, 16, 2), (7, 2048, 520, 48, 9), (31, 520, 384, 16, 40), (33, 4096, 256, 64, 4),
+         (64, 1024, 4096, 16, 64), (100, 264, 200, 80, 7), (113, 512, 28672, 16, 5), (128, 4096, 6144, 16, 128), (128, 1032, 136, 256, 2),
+         (129, 64, 64, 16, 3), (200, 2048, 1000, 32, 200), (257, 136, 72, 48, 2), (300, 4096, 512, 128, 6), (1000, 1024, 2048, 16, 3), (1500, 512, 264, 64, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n,r,count", SIZES)
+def test_against_64_bits(cuda, m, k, n, r, count):
+    x, w, st, ids = _case(m, k, n, r, count, seed=m + n, device=cuda, pad=16 * (m % 3))
+    y, size = _exact(x, w, st, ids)
+    got = lora_ops.linear_lora(x, w, st, ids)
+    _assert_near(got, y, size)
+    bare = ids < 0
+    assert torch.equal(got[bare], ops.linear(x, w)[bare])               # rows without an adapter: the product's own bits
+    # requests of several rows each: tiles with one adapter, two, and none
+    runs = torch.sort(ids).values
+    y, size = _exact(x, w, st, runs)
+    _assert_near(lora_ops.linear_lora(x, w, st, runs), y, size)
+    wide = torch.zeros(m, n + 8, dtype=BF16, device=cuda)
+    assert torch.equal(lora_ops.linear_lora(x, w, st._replace(ranks=None), runs, out=wide[:, :n]), lora_ops.linear_lora(x, w, st, runs))
+    assert not wide[:, n:].any()
+    for i in (-1, count - 1):
+        same = torch.full_like(ids, i)
+        y, size = _exact(x, w, st, same)
+        _assert_near(lora_ops.linear_lora(x, w, st, same), y, size)
+    ops.check_status(cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [5, 64, 128, 300, 700])
+def test_a_row_does_not_depend_on_its_neighbours(cuda, m):
+    x, w, st, ids = _case(m, 1024, 768, 32, 6, seed=3, device=cuda)
+    whole = lora_ops.linear_lora(x, w, st, ids)
+    other = ids.clone()
+    other[1:] = torch.randint(-1, 6, (m - 1,), device=cuda, dtype=torch.int32)
+    assert torch.equal(lora_ops.linear_lora(x, w, st, other)[0], whole[0])
+    if m <= 128:
+        for row in (0, m // 2, m - 1):
+            assert torch.equal(lora_ops.linear_lora(x[row: row + 1], w, st, ids[row: row + 1])[0], whole[row])
+    # an adapter whose weights are not finite, and rows that are not, reach their own rows only
+    st.a[1, 0, 0], st.b[2, 5, 1] = float("inf"), float("nan")
+    x = x.clone()
+    x[m // 2] = float("inf")
+    got = lora_ops.linear_lora(x, w, st, ids)
+    fine = (ids != 1) & (ids != 2)
+    fine[m // 2] = False
+    assert torch.equal(got[fine], whole[fine])
+
+
+@pytest.mark.gpu
+def test_ids_past_the_stack_are_reported(cuda):
+    for m in (4, 200):
+        x, w, st, ids = _case(m, 128, 64, 16, 3, device=cuda)
+        ids[1] = 3
+        got = lora_ops.linear_lora(x, w, st, ids)
+        with pytest.raises(ops.DeviceStatusError):
+            ops.check_status(cuda)
+        assert torch.equal(got[1], ops.linear(x, w)[1])
+        ids[1] = -7
+        assert torch.equal(lora_ops.linear_lora(x, w, st, ids), got)
+        ops.check_status(cuda)
+        st.ranks[:] = 1000                                                   # ranks past the stack's are cut, negative ones are none
+        full = lora_ops.linear_lora(x, w, st, ids)
+        assert torch.equal(full, got)
+        st.ranks[:] = -5
+        assert torch.equal(lora_ops.linear_lora(x, w, st, ids), ops.linear(x, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 64, 128, 200, 600])
+def test_fused_projections(cuda, m):
+    """Gate and up with the activation, q / k / v with rotation and cache write: what the product and the separate kernels give."""
+    g = torch.Generator().manual_seed(m)
+    k, f, hq, hkv = 512, 384, 4, 2
+    new = lambda *s: torch.randn(*s, generator=g)
+    x = new(m, k).to(BF16).to(cuda)
+    ids = torch.randint(-1, 3, (m,), generator=g, dtype=torch.int32).to(cuda)
+    wgu = (new(2 * f, k) * k ** -0.5).to(BF16).to(cuda)
+    part = lambda c, r: ((new(r, k) * k ** -0.5).to(BF16), (new(c, r) * 0.2).to(BF16), 1.0)
+    gu = lora_ops.pack_stack([[part(f, 16), part(f, 8)], [part(f, 24), None], [None, part(f, 16)]], k, [f, f], cuda, interleave=True)
+    y, size = _exact(x, wgu, gu, ids)
+    _assert_near(lora_ops.linear_lora(x, wgu, gu, ids), y, size)
+    _assert_near(lora_ops.linear_lora(x, wgu, gu._replace(part_of=None), ids), y, size)
+    for mode, limit in ((0, 0.0), (3, 0.0), (5, 1.5), (1, 0.0)):
+        got = lora_ops.linear_swiglu_lora(x, wgu, gu, ids, mode=mode, limit=limit)
+        want = ops.silu_mul_interleaved(lora_ops.linear_lora(x, wgu, gu, ids), None, mode, limit).double()
+        # Either way rounds gate g, up u, the activation and the result to BF16 at most once each: with |act(g)| <= |g| and |act'| <= 1.2 that is at
+        # most 2^-8 |g| (|u| + 1) (1.2 + 1 + 1 + 1) for each of the two, second orders included in 9 for both
+        near = (y.abs() + 8 * size).view(m, f // 64, 2, 64)
+        bound = 2.0 ** -8 * 9 * (near[:, :, 0] * (near[:, :, 1] + 1)).reshape(m, f)
+        assert ((got.double() - want).abs().cpu() <= bound).all(), mode
+        assert torch.equal(got[ids < 0], ops.linear_swiglu(x, wgu, mode=mode, limit=limit)[ids < 0])
+    d, n = 128, (hq + 2 * hkv) * 128
+    wqkv = (new(n, k) * k ** -0.5).to(BF16).to(cuda)
+    qkv = lora_ops.pack_stack([[part(hq * d, 16), part(hkv * d, 8), part(hkv * d, 16)], [part(hq * d, 32), None, part(hkv * d, 4)], [None, None, None]], k,
+                              [hq * d, hkv * d, hkv * d], cuda)
+    positions = torch.arange(m, dtype=torch.int32, device=cuda)
+    slots = torch.randperm(16 * 64, generator=g)[:m].to(torch.int32).to(cuda)
+    slots[m // 2] = -1
+    caches = lambda: [torch.zeros(16, hkv, 64, d, dtype=BF16, device=cuda) for _ in range(2)]
+    kc, vc = caches()
+    got = lora_ops.linear_rope_kv_lora(x, wqkv, qkv, ids, positions, slots, kc, vc, hq, hkv, d, 1e4)
+    ka, va = caches()
+    apart = lora_ops.linear_lora(x, wqkv, qkv, ids)
+    ops.rope_kv_paged(apart, positions, slots, ka, va, hq, hkv, d, 1e4)
+    # the two products may split K differently: one rounding's difference, turned (two terms) and rounded three times
+    for one, two in ((got, apart), (kc, ka), (vc, va)):
+        bound = 2.0 ** -8 * 8 * two.double().abs().max()
+        assert ((one.double() - two.double()).abs() <= bound).all() and (one != two).double().mean() < 0.2
+    kb, vb = caches()
+    plain = ops.linear_rope_kv(x, wqkv, positions, slots, kb, vb, hq, hkv, d, 1e4)
+    assert torch.equal(got[ids < 0], plain[ids < 0])
+    ops.check_status(cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [8, 200])
+def test_captured_and_on_other_streams(cuda, m):
+    x, w, st, ids = _case(m, 512, 1024, 16, 8, seed=5, device=cuda)
+    x, w = x.clone(), w.clone()
+    first = lora_ops.linear_lora(x, w, st, ids)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        mid = lora_ops.linear_lora(x, w, st, ids)
+        out = lora_ops.linear_lora(mid[:, :512], w, st, ids)
+    for seed in (7, 8):
+        g = torch.Generator().manual_seed(seed)
+        x.copy_(torch.randn(m, 512, generator=g))
+        ids.copy_(torch.randint(-1, 8, (m,), generator=g, dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(out, lora_ops.linear_lora(lora_ops.linear_lora(x, w, st, ids)[:, :512], w, st, ids))
+    g = torch.Generator().manual_seed(5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = lora_ops.linear_lora(x, w, st, ids)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, lora_ops.linear_lora(x, w, st, ids)) and first.shape == other.shape
+    ops.check_status(cuda)
+
+
+@pytest.mark.gpu
+def test_prompts_in_portions(cuda, monkeypatch):
+    """Rows whose deltas do not fit the buffer are done in portions: the same bits."""
+    x, w, st, ids = _case(900, 256, 512, 32, 5, seed=9, device=cuda)
+    ids = torch.sort(ids).values
+    whole = lora_ops.linear_lora(x, w, st, ids)
+    monkeypatch.setattr(lora_ops, "DELTA_BYTES", 300 * 512 * 4)
+    assert torch.equal(lora_ops.linear_lora(x, w, st, ids), whole)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device(cuda):
+    x, w, st, ids = _case(4, 64, 48, 16, 2, device=cuda)
+    for args in ((x.float(), w, st, ids), (x, w.float(), st, ids), (x, w, st, ids.cpu()), (x, w, st._replace(scale=st.scale.cpu()), ids), (x, w[:, :56], st, ids)):
+        with pytest.raises(KernelError):
+            lora_ops.linear_lora(*args)
+    with pytest.raises(KernelError):
+        lora_ops.linear_lora(x, w, st, ids, out=torch.zeros(4, 40, dtype=BF16, device=cuda))
+    x, w, st, ids = _case(200, 64, 44, 16, 2, device=cuda)                   # prompts' products want columns in eights, as ops.linear does
+    with pytest.raises(KernelError):
+        lora_ops.linear_lora(x, w, st, ids)
+    ops.check_status(cuda)
