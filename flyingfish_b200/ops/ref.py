@@ -405,6 +405,46 @@ def sample_row(logits: torch.Tensor, temperature: float, top_k: int, top_p: floa
     return idx
 
 
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor | None, top_p: torch.Tensor | None,
+                  min_p: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Drawn ids (int32) and their probabilities (FP32), in 64 bits: a row's settings filter the order (logit down, id up) to a prefix and the lowest id
+    whose sum of kept weights passes the number times their sum is drawn."""
+    ids = torch.zeros(logits.shape[0], dtype=torch.int32)
+    probs = torch.zeros(logits.shape[0], dtype=F32)
+    for r in range(logits.shape[0]):
+        l = torch.nan_to_num(logits[r].double(), nan=-math.inf, posinf=math.inf, neginf=-math.inf)
+        top, t = l.max(), float(temperature[r])
+        if top == -math.inf:
+            continue
+        if not t > 0:
+            ids[r], probs[r] = int(torch.nonzero(l == top)[0]), 1.0
+            continue
+        away = torch.where(l == top, 0.0, (l - top) / t)
+        if t == math.inf:
+            away = torch.where(l == -math.inf, l, 0.0)
+        w = torch.exp(away)
+        order = torch.argsort(l, descending=True, stable=True)
+        n = l.numel()
+        k = 0 if top_k is None else int(top_k[r])
+        if k > 0:
+            n = min(n, k)
+        p = 1.0 if top_p is None else float(top_p[r])
+        if p < 1:
+            mass = torch.cumsum(w[order], 0)
+            n = min(n, int((mass < max(p, 0.0) * w.sum()).sum()) + 1)
+        m = 0.0 if min_p is None else float(min_p[r])
+        if m > 0:
+            n = min(n, int((away >= math.log(min(m, 1.0))).sum()))
+        kept = torch.zeros_like(w)
+        kept[order[:n]] = w[order[:n]]
+        sums = torch.cumsum(kept, 0)
+        u = float(uniforms[r])
+        u = min(u, 1.0 - 2.0 ** -24) if u > 0 else 0.0
+        at = min(int((sums <= u * sums[-1]).sum()), int(torch.nonzero(kept)[-1]))
+        ids[r], probs[r] = at, float(kept[at] / sums[-1])
+    return ids, probs
+
+
 # ------------------------------------------------------------------------------------------
 # MoE
 # ------------------------------------------------------------------------------------------

@@ -1,0 +1,52 @@
+"""Next tokens of a batch whose rows have settings of their own: temperature, top-k, top-p and min-p, drawn with a given random number per row. CUDA:
+``csrc/sample.cu``; CPU: the oracle in 64 bits. Settings and numbers are data on the device, so a captured step serves any mix of them, greedy
+rows included."""
+from __future__ import annotations
+
+from ctypes import c_longlong, c_void_p
+
+import torch
+
+from . import BF16, _count, _require, _rows2d, ref
+from .lib import check, kernels
+
+F32, I32 = torch.float32, torch.int32
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor | None = None,
+                  top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  probs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``logits`` [rows, vocab] BF16 or FP32; ``uniforms`` (in [0, 1)), ``temperature``, ``top_p``, ``min_p`` FP32 and ``top_k`` int32, one per row. Returns the
+    drawn ids (int32) and the probability each had among what was left to draw from (FP32).
+
+    Tokens are ordered by logit, the larger first, equal ones by id. A row keeps the least of: its first ``top_k`` tokens (all where that is 0 or less); the
+    smallest prefix whose mass reaches ``top_p`` of the whole mass of ``softmax(logits / temperature)`` (all from 1 on, one token at 0 or less); the tokens of
+    at least ``min_p`` times the largest probability (all at 0 or less, those of the largest from 1 on). Drawn is the lowest id whose sum of kept masses up to it
+    passes ``uniforms`` times their sum. ``temperature`` 0 or less: the lowest id of the largest logit, probability 1. NaN logits count as -inf, which is
+    never drawn, and +inf shares everything among its equals; a row of -inf gives id 0 with probability 0. Masses are those of 64-bit arithmetic; one
+    below 2^-1000 of the largest counts as none."""
+    rows, ld = _rows2d(logits)
+    vocab = logits.shape[1]
+    _require(logits.dtype in (BF16, F32) and vocab > 0, "sample_tokens: bf16 or fp32 logits")
+    _require(vocab < 1 << 31, "sample_tokens: ids are 32 bits wide")
+    dev = logits.device
+    for t, dtype, name in ((uniforms, F32, "uniforms"), (temperature, F32, "temperature"), (top_k, I32, "top_k"), (top_p, F32, "top_p"), (min_p, F32, "min_p"),
+                           (out, I32, "out"), (probs, F32, "probs")):
+        _require(t is None or (t.dtype == dtype and t.shape == (rows,) and t.is_contiguous() and t.device == dev),
+                 f"sample_tokens: {name} is one {dtype} per row on the logits' device")
+    if not logits.is_cuda:
+        ids, p = ref.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p)
+        return (ids if out is None else out.copy_(ids)), (p if probs is None else probs.copy_(p))
+    _require(dev.index == torch.cuda.current_device(), "sample_tokens: operands on another device than the current one")
+    if out is None:
+        out = torch.empty(rows, dtype=I32, device=dev)
+    if probs is None:
+        probs = torch.empty(rows, dtype=F32, device=dev)
+    if rows == 0:
+        return out, probs
+    at = lambda t: c_void_p(0 if t is None else t.data_ptr())
+    rc = kernels().ff_sample_tokens(at(logits), int(logits.dtype == F32), at(uniforms), at(temperature), at(top_k), at(top_p), at(min_p), at(out), at(probs),
+                                    rows, vocab, c_longlong(ld), c_void_p(torch.cuda.current_stream().cuda_stream))
+    check(rc, "ff_sample_tokens")
+    _count()
+    return out, probs

@@ -1,0 +1,219 @@
+"""Sampling with settings per row: the oracle's rules and the refusals on the CPU; the kernel's ids against 64 bits on a GPU."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from flyingfish_b200 import ops
+from flyingfish_b200.ops import sample_ops
+from flyingfish_b200.ops.lib import KernelError
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _row(logits, u, t, k, p, m):
+    """The definition for one row, in 64 bits, with sums that do not depend on an order (math.fsum where it decides little, numpy otherwise)."""
+    l = np.where(np.isnan(logits), -np.inf, logits)
+    top = l.max()
+    if top == -np.inf:
+        return 0, 0.0
+    if not t > 0:
+        return int(np.argmax(l)), 1.0
+    with np.errstate(invalid="ignore", over="ignore"):
+        away = np.where(l == top, 0.0, (l - top) / t)
+    w = np.exp(away)
+    order = np.lexsort((np.arange(len(l)), -l))
+    n = len(l) if k <= 0 else min(k, len(l))
+    if p < 1:
+        sums = np.cumsum(w[order])
+        n = min(n, int(np.searchsorted(sums, max(p, 0.0) * sums[-1], side="left")) + 1)
+    if m > 0:
+        n = min(n, int((away >= math.log(min(m, 1.0))).sum()))
+    ids = np.sort(order[:n])
+    sums = np.cumsum(w[ids])
+    u = min(u, 1 - 2.0 ** -24) if u > 0 else 0.0
+    at = min(int(np.searchsorted(sums, u * sums[-1], side="right")), int(np.nonzero(w[ids])[0][-1]))
+    return int(ids[at]), float(w[ids[at]] / sums[-1])
+
+
+def _want(logits, u, t, k, p, m):
+    l = logits.double().cpu().numpy()
+    get = lambda v, i, other: other if v is None else v[i].item()
+    rows = [_row(l[i], u[i].item(), t[i].item(), get(k, i, 0), get(p, i, 1.0), get(m, i, 0.0)) for i in range(len(l))]
+    return torch.tensor([r[0] for r in rows], dtype=torch.int32), torch.tensor([r[1] for r in rows], dtype=torch.float64)
+
+
+def _check(logits, u, t, k=None, p=None, m=None):
+    ids, probs = sample_ops.sample_tokens(logits, u, t, k, p, m)
+    want, want_p = _want(logits, u, t, k, p, m)
+    bad = torch.nonzero(ids.cpu() != want).flatten().tolist()
+    assert not bad, f"rows {bad[:5]}: {ids.cpu()[bad[:5]].tolist()} for {want[bad[:5]].tolist()}"
+    # rounded once from a quotient whose parts are held to a few 1e-13
+    assert ((probs.double().cpu() - want_p).abs() <= want_p * (2.0 ** -24 + 1e-11)).all()
+
+
+def _settings(rows, seed, device):
+    g = torch.Generator().manual_seed(seed)
+    pick = lambda options, dtype: torch.tensor(options, dtype=dtype)[torch.randint(len(options), (rows,), generator=g)]
+    t = pick([0.0, 0.3, 0.7, 1.0, 1.3, 2.0, 50.0], F32)
+    k = pick([0, 0, 1, 2, 20, 50, 1000, 10 ** 6], torch.int32)
+    p = pick([1.0, 1.0, 0.999, 0.9, 0.5, 0.1, 0.0], F32)
+    m = pick([0.0, 0.0, 0.0, 0.001, 0.05, 0.5, 1.0], F32)
+    return [v.to(device) for v in (torch.rand(rows, generator=g), t, k, p, m)]
+
+
+def _logits(kind, rows, vocab, dtype, seed, device):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, vocab, generator=g)
+    if kind == "peaked":
+        x = x * 2.5
+        x[torch.arange(rows)[:, None], torch.randint(vocab, (rows, 20), generator=g)] += 12 * torch.rand(rows, 20, generator=g)
+    elif kind == "equal":
+        x = torch.full((rows, vocab), 1.7)
+    elif kind == "steps":
+        x = torch.randint(0, 4, (rows, vocab), generator=g).float() * 0.5
+    elif kind == "masked":
+        x = torch.where(torch.rand(rows, vocab, generator=g) < 0.9, torch.tensor(float("-inf")), x * 3)
+    elif kind == "lowest":
+        x = torch.where(torch.rand(rows, vocab, generator=g) < 0.9, torch.finfo(dtype).min, x * 3)
+    elif kind == "tiny":
+        x = x * 1e-30
+    elif kind == "wide":
+        x = x * 200
+    return x.to(dtype).to(device)
+
+
+KINDS = ["normal", "peaked", "equal", "steps", "masked", "lowest", "tiny", "wide"]
+
+
+# ------------------------------------------------------------------------------------------
+# CPU
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+def test_oracle_against_the_definition(kind):
+    _check(_logits(kind, 24, 301, F32, 1, "cpu"), *_settings(24, 2, "cpu"))
+
+
+def test_rules():
+    l = torch.tensor([[0.0, 2.0, 2.0, 1.0]]).log_softmax(-1)
+    one = lambda u, t=1.0, k=0, p=1.0, m=0.0: sample_ops.sample_tokens(l, torch.tensor([u]), torch.tensor([t]), torch.tensor([k], dtype=torch.int32), torch.tensor([p]),
+                                                                       torch.tensor([m]))[0].item()
+    assert one(0.99, t=0.0) == 1 and one(0.99, k=1) == 1 and one(0.99, k=2) == 2 and one(0.49, k=2) == 1
+    assert one(0.99, p=0.0) == 1 and one(0.0) == 0 and one(0.999999) == 3 and one(0.6, m=1.0) == 2 and one(float("nan")) == 0 and one(2.0) == 3
+    none = sample_ops.sample_tokens(torch.full((1, 4), -math.inf), torch.tensor([0.5]), torch.tensor([1.0]))
+    assert none[0].item() == 0 and none[1].item() == 0
+    inf = torch.tensor([[1.0, math.inf, math.nan, math.inf]])
+    assert [sample_ops.sample_tokens(inf, torch.tensor([u]), torch.tensor([1.0]))[0].item() for u in (0.4, 0.6)] == [1, 3]
+
+
+def test_refusals():
+    l, v = torch.zeros(2, 8), torch.zeros(2)
+    for args in ((l.double(), v, v), (l, v.double(), v), (l, v[:1], v), (l, v, v, v), (l, v, v, None, v.int()), (l.t(), torch.zeros(8), torch.zeros(8)), (l[:, :0], v, v)):
+        with pytest.raises(KernelError):
+            sample_ops.sample_tokens(*args)
+    assert sample_ops.sample_tokens(l[:0], v[:0], v[:0])[0].shape == (0,)
+
+
+# ------------------------------------------------------------------------------------------
+# GPU
+# ------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (40, 301), (17, 4099), (64, 50257), (9, 128256)])
+def test_ids_of_64_bits(cuda, rows, vocab, kind, dtype):
+    _check(_logits(kind, rows, vocab, dtype, rows + vocab, cuda), *_settings(rows, vocab, cuda))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dtype", [(500, 1000, BF16), (300, 32000, F32), (150, 151936, BF16), (2, 600001, BF16), (3, 300007, F32), (120, 262144, BF16)])
+def test_many_rows_and_wide_rows(cuda, rows, vocab, dtype):
+    _check(_logits("peaked", rows, vocab, dtype, 5, cuda), *_settings(rows, 6, cuda))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["normal", "peaked", "steps", "equal"])
+def test_single_filters(cuda, kind):
+    """Each filter by itself, with the others absent; numbers next to 0 and 1."""
+    rows, vocab = 32, 20011
+    for dtype in (BF16, F32):
+        l = _logits(kind, rows, vocab, dtype, 11, cuda)
+        u, t, k, p, m = _settings(rows, 12, cuda)
+        t = t.clamp(min=0.5)
+        u[0], u[1], u[2], u[3] = 0.0, 1.0 - 2.0 ** -24, 2.0 ** -24, 0.5
+        for args in ((None, None, None), (k, None, None), (None, p, None), (None, None, m), (k, p, None)):
+            _check(l, u, t, *args)
+
+
+@pytest.mark.gpu
+def test_layouts_and_special_values(cuda):
+    rows, vocab = 12, 5003
+    base = torch.full((rows, vocab + 9), 1e4, dtype=BF16, device=cuda)
+    base[:, 3:3 + vocab] = _logits("peaked", rows, vocab, BF16, 1, cuda)
+    s = _settings(rows, 3, cuda)
+    _check(base[:, 3:3 + vocab], *s)                                     # rows that start off a 16-byte boundary, in a wider buffer
+    assert torch.equal(sample_ops.sample_tokens(base[:, 3:3 + vocab], *s)[0], sample_ops.sample_tokens(base[:, 3:3 + vocab].contiguous(), *s)[0])
+    for dtype in (BF16, F32):
+        l = _logits("peaked", rows, vocab, dtype, 2, cuda)
+        l[0], l[1, ::3], l[2, 7], l[3, 5], l[3, 4000] = -math.inf, math.nan, math.inf, math.inf, math.inf
+        l[4, 1:] = -math.inf
+        l[5] = math.nan
+        u, t, k, p, m = s
+        _check(l, u, torch.ones_like(t))
+        _check(l, u, torch.ones_like(t), k, p, m)
+        t = t.clone()
+        t[6], t[7], t[8] = -1.0, math.nan, 1e-40
+        p, m, u = p.clone(), m.clone(), u.clone()
+        p[9], m[9], m[10], u[11] = math.nan, math.nan, 7.0, math.nan
+        _check(l, u, t, k, p, m)
+        _check(l, u, torch.full_like(t, math.inf).fill_(1e30), k, p, m)
+
+
+@pytest.mark.gpu
+def test_frequencies(cuda):
+    """Numbers spread evenly over [0, 1) draw every token as often as its probability says: off by at most one."""
+    l = _logits("peaked", 1, 200, F32, 4, cuda)
+    n = 4096
+    u = (torch.arange(n, device=cuda) / n).float()
+    ids, _ = sample_ops.sample_tokens(l.expand(n, 200), u, torch.ones(n, device=cuda), torch.full((n,), 40, dtype=torch.int32, device=cuda))
+    top = torch.topk(l[0].double(), 40)
+    share = torch.zeros(200, dtype=torch.float64, device=cuda)
+    share[top.indices] = torch.softmax(top.values, 0)
+    seen = torch.bincount(ids.long(), minlength=200).double()
+    assert ((seen - share * n).abs() < 1.0 + 1e-6).all()
+
+
+@pytest.mark.gpu
+def test_captured_and_on_another_stream(cuda):
+    l = _logits("peaked", 33, 32003, BF16, 1, cuda)
+    s = _settings(33, 1, cuda)
+    sample_ops.sample_tokens(l, *s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ids, probs = sample_ops.sample_tokens(l, *s)
+    for seed in (2, 3):
+        l.copy_(_logits("normal", 33, 32003, BF16, seed, cuda))
+        for v, w in zip(s, _settings(33, seed, cuda)):
+            v.copy_(w)
+        graph.replay()
+        want, want_p = sample_ops.sample_tokens(l, *s)
+        assert torch.equal(ids, want) and torch.equal(probs, want_p)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = sample_ops.sample_tokens(l, *s)
+    here = sample_ops.sample_tokens(l, *s)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other[0], here[0]) and torch.equal(other[1], here[1])
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device(cuda):
+    l, v = torch.zeros(2, 8, device=cuda), torch.zeros(2, device=cuda)
+    with pytest.raises(KernelError):
+        sample_ops.sample_tokens(l, v.cpu(), v)
+    with pytest.raises(KernelError):
+        sample_ops.sample_tokens(torch.zeros(1, 2_000_000, device=cuda), v[:1], v[:1])       # more than a cluster's shared memory holds
+    ops.check_status(cuda)
