@@ -16,6 +16,8 @@
 #include "comm.cuh"
 #include "host_util.h"
 #include "launchers.h"
+#include "lora.cuh"
+#include <type_traits>
 
 namespace ff {
 
@@ -139,22 +141,7 @@ struct LinTail {
   const int* slots;
   __nv_bfloat16 *kcache, *vcache;
   int hq, hkv, rhalf, block_size, num_blocks;
-  // added to the FP32 sums of rows whose id is within [0, adapters): delta[row][column], pitch ldd (lora.cu)
-  const float* delta; const int* ids; int ldd, adapters;
 };
-
-// n (a multiple of 8) columns from `col` of a row's delta; N is a multiple of 8
-template <int n>
-__device__ __forceinline__ void add_delta(uint32_t* r, const float* drow, int col, int N) {
-#pragma unroll
-  for (int j = 0; j < n; j += 8)
-    if (col + j < N) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(drow + col + j)), y = __ldcg(reinterpret_cast<const float4*>(drow + col + j) + 1);
-      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r[j + i] = __float_as_uint(__uint_as_float(r[j + i]) + v[i]);
-    }
-}
 
 constexpr int RS_STG_PITCH = 144, RS_STG_BYTES = 32 * RS_STG_PITCH;   // COMM 2 epilogue staging, per warp
 constexpr int COMM_PARTS = 4;       // a 128-row block is pushed (COMM 1) / reduced (COMM 2) in this many pieces
@@ -162,12 +149,9 @@ constexpr int COMM_PARTS = 4;       // a 128-row block is pushed (COMM 1) / redu
 // An epilogue thread's row of a finished tile: tensor memory -> registers -> global. row: row of the result, stored where `live`; col0: first
 // of the tile's `width` columns (a multiple of 32, of 128 with epi 1 and 3), N: columns (of the head), col_off: first column of the head. The PARTS
 // warps that share the row take turns with its groups of columns.
-template <int PARTS, bool DELTA>
+template <int PARTS>
 __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict__ Cout, int row, bool live, int ldc, int N, int epi, int col0,
                                                int width, size_t col_off, const LinTail& tail, int part, int* status) {
-  const float* drow = nullptr;
-  if constexpr (DELTA)
-    if (live && (unsigned)tail.ids[row] < (unsigned)tail.adapters) drow = tail.delta + (size_t)row * tail.ldd;
   if (epi == 1) {
     const int half = width / 2, out0 = col0 / 2;
     __nv_bfloat16* crow = reinterpret_cast<__nv_bfloat16*>(Cout) + (size_t)row * ldc + out0;
@@ -179,7 +163,6 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
       tmem_ld_x16(taddr + gc, g);
       tmem_ld_x16(taddr + gc + 64, u);
       tmem_ld_wait();
-      if (DELTA && drow != nullptr) { add_delta<16>(g, drow, col0 + gc, N); add_delta<16>(u, drow, col0 + gc + 64, N); }
       if (live) {
         uint32_t o[8];
 #pragma unroll
@@ -248,7 +231,6 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
         tmem_ld_x16(taddr + h0 + c, a);
         tmem_ld_x16(taddr + h0 + c + 64, b);
         tmem_ld_wait();
-        if (DELTA && drow != nullptr) { add_delta<16>(a, drow, col0 + h0 + c, N); add_delta<16>(b, drow, col0 + h0 + c + 64, N); }
         if (live) {
           __nv_bfloat16* cached = nullptr;
           if (blk >= 0 && head >= tail.hq) {
@@ -311,7 +293,6 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
       uint32_t r[32];
       tmem_ld_x32(taddr + c, r);
       tmem_ld_wait();
-      if (DELTA && drow != nullptr) add_delta<32>(r, drow, col0 + c, N);
       if (tail.bias != nullptr) {
         const int col = col0 + c;
         if (col + 32 <= N) {
@@ -382,11 +363,11 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
   }
 }
 
-template <int BN, int STAGES, int COMM, bool DELTA = false>
+template <int BN, int STAGES, int COMM, bool LORA = false>
 __global__ void __launch_bounds__(COMM == 2 ? 192 : 320, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1,
                  const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmB, void* __restrict__ Cout, int M, int N, int K, int ldc, int epi,
-                 int* status, CommArgs ca, GroupArgs ga, LinTail tail) {
+                 int* status, CommArgs ca, GroupArgs ga, LinTail tail, const __grid_constant__ std::conditional_t<LORA, LoraDev, NoLora> lora) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PipeBars bars;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -415,7 +396,100 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const uint32_t tmem_base = bars.tmem_base;
   volatile int* abort_flag = &bars.abort_flag;
 
-  if (warp == 0) {
+  if constexpr (LORA) {
+    // dense problems only, by whole warps: as below, with the units of the adapters (lora.cuh) behind a tile's K blocks
+    if (warp < 2) {
+      constexpr uint32_t idesc = umma_idesc(1, 1, 0, 0, BM, BN);
+      constexpr int T_BYTES = BM * 32, UNIT_BYTES = 2 * T_BYTES + BN * 32;
+      const int tiles = tiles_m * tiles_n;
+      RowGroups<4> rows, next;
+      RingPos rp;
+      bool ok = true;
+      uint32_t tile_it = 0;
+      int tm, tn;
+      tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
+      rows.load(lora.a, tm * BM, M, lane, status);
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tile_it) {
+        tile_coords(t, tiles_m, tiles_n, tm, tn);
+        const bool more = t + (int)gridDim.x < tiles;
+        if (more) { int tm2, tn2; tile_coords(t + gridDim.x, tiles_m, tiles_n, tm2, tn2); next.load_ids(lora.a, tm2 * BM, M, lane); }
+        const int acc = tile_it & 1;
+        const uint32_t aph = (tile_it >> 1) & 1, d_tmem = tmem_base + acc * BN;
+        RingPos at = rp;
+        if (warp == 0) {
+          if (elect_one()) {
+            for (int kb = 0; kb < kblocks; ++kb, at.next(STAGES)) {
+              const int s = at.s;
+              if (!mbar_wait(&bars.empty[s], at.ph ^ 1, abort_flag, status, KID_GEMM_BF16, 1)) { ok = false; break; }
+              mbar_expect_tx(&bars.full[s], STAGE_BYTES);
+              uint8_t* sa = smem + s * STAGE_BYTES;
+              tma_load_2d(sa, &tmA, &bars.full[s], kb * BK, tm * BM);
+              tma_load_2d(sa + A_BYTES, &tmB, &bars.full[s], kb * BK, tn * BN);
+            }
+          }
+        } else if (elect_one()) {
+          ok = mbar_wait(&bars.tmem_empty[acc], aph ^ 1, abort_flag, status, KID_GEMM_BF16, 2);
+          tc_fence_after();
+          for (int kb = 0; kb < kblocks && ok; ++kb, at.next(STAGES)) {
+            const int s = at.s;
+            if (!mbar_wait(&bars.full[s], at.ph, abort_flag, status, KID_GEMM_BF16, 3)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * STAGE_BYTES);
+            const uint64_t da = umma_desc_sw128(sa, 16, 1024), db = umma_desc_sw128(sa + A_BYTES, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k) umma_f16(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            umma_commit(&bars.empty[s]);
+          }
+        }
+        rp.skip(kblocks, STAGES);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (more) next.load_steps(lora.a);
+        UnitWalk<4> walk(rows, lora_part(lora.a, tn * BN, BN, N), lora.a.parts, 0, 1);
+        UnitPair<4> p;
+        while (ok && p.next(walk)) {
+          const int s = rp.s;
+          uint8_t* sa = smem + s * STAGE_BYTES;
+          if (warp == 0) {
+            if (elect_one()) {
+              ok = mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_BF16, 1);
+              if (ok) {
+                mbar_expect_tx(&bars.full[s], p.n * UNIT_BYTES);
+                tma_load_2d(sa, &lora.t, &bars.full[s], p.step0 * 16, tm * BM);
+                tma_load_2d(sa + T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step0 * 16, tm * BM);
+                tma_load_2d(sa + A_BYTES, &lora.b, &bars.full[s], p.step0 * 16, p.adapter0 * N + tn * BN);
+                if (p.n == 2) {
+                  tma_load_2d(sa + 2 * T_BYTES, &lora.t, &bars.full[s], p.step1 * 16, tm * BM);
+                  tma_load_2d(sa + 3 * T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step1 * 16, tm * BM);
+                  tma_load_2d(sa + A_BYTES + BN * 32, &lora.b, &bars.full[s], p.step1 * 16, p.adapter1 * N + tn * BN);
+                }
+              }
+            }
+          } else if (elect_one()) {
+            ok = mbar_wait(&bars.full[s], rp.ph, abort_flag, status, KID_GEMM_BF16, 3);
+            if (ok) {
+              tc_fence_after();
+              const uint32_t a0 = smem_u32(sa);
+              const uint64_t db0 = umma_desc_sw32(a0 + A_BYTES), db1 = umma_desc_sw32(a0 + A_BYTES + BN * 32);
+              umma_f16_lanes(d_tmem, umma_desc_sw32(a0), db0, idesc, p.mine0);
+              umma_f16_lanes(d_tmem, umma_desc_sw32(a0 + T_BYTES), db0, idesc, p.mine0);
+              if (p.n == 2) {
+                umma_f16_lanes(d_tmem, umma_desc_sw32(a0 + 2 * T_BYTES), db1, idesc, p.mine1);
+                umma_f16_lanes(d_tmem, umma_desc_sw32(a0 + 3 * T_BYTES), db1, idesc, p.mine1);
+              }
+              umma_commit(&bars.empty[s]);
+            }
+          }
+          rp.next(STAGES);
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        if (warp == 1 && ok && elect_one()) umma_commit(&bars.tmem_full[acc]);
+        __syncwarp();
+        if (more) { next.vote(); rows = next; }
+      }
+    }
+  }
+  if (!LORA && warp == 0) {
     if (elect_one()) {
       tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB);
       uint32_t it = 0;
@@ -445,7 +519,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (!LORA && warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc = umma_idesc(1, 1, 0, 0, BM, BN);
       uint32_t it = 0, tile_it = 0;
@@ -475,7 +549,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (ok) umma_commit(&bars.tmem_full[acc]);
       }
     }
-  } else if (warp < (COMM ? 6 : 10)) {
+  } else if (warp >= 2 && warp < (COMM ? 6 : 10)) {
     // epilogue warps 2..5, without communication 2..9 in two per quarter; TMEM lane quarter = warp % 4
     const int q = warp & 3;
     const int e = (warp - 2) * 32 + lane;
@@ -532,7 +606,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           tma_store_wait<0>();                              // every row of this tile has landed in the owner's slot
           asm volatile("fence.proxy.async;" ::: "memory");
       } else {
-        store_tile_row<COMM ? 1 : 2, DELTA>(taddr, Cout, row, row < row_end, ldc, N, epi, tn * BN, BN, (size_t)head * ga.c_cols, tail, COMM ? 0 : (warp - 2) >> 2, status);
+        store_tile_row<COMM ? 1 : 2>(taddr, Cout, row, row < row_end, ldc, N, epi, tn * BN, BN, (size_t)head * ga.c_cols, tail, COMM ? 0 : (warp - 2) >> 2, status);
       }
       tc_fence_before();
       __syncwarp();
@@ -698,10 +772,11 @@ __device__ __forceinline__ void pair_tile(const PairTiles& pt, int t, int tiles_
   else { tile_coords(t - n1, tiles_m, tiles_n2, tm, tn); col0 = pt.wide * pt.w1 + tn * pt.w2; width = pt.w2; }
 }
 
-template <int PARTS, bool DELTA>
+template <int PARTS, bool LORA>
 __global__ void __launch_bounds__(64 + 128 * PARTS, 1)
 gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmB2,
-                      void* __restrict__ Cout, int M, int N, int K, int ldc, int epi, const PairTiles pt, int stages, int* status, LinTail tail) {
+                      void* __restrict__ Cout, int M, int N, int K, int ldc, int epi, const PairTiles pt, int stages, int* status, LinTail tail,
+                      const __grid_constant__ std::conditional_t<LORA, LoraDev, NoLora> lora) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PairBars bars;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -720,7 +795,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     bars.abort_flag = 0;
     mbar_fence_init();
   }
-  pdl_wait();
+  // With adapters the kernel in front (lora.cu) lets this one start only when it has its tensor memory and everything before it is done: X and the ids are
+  // there, and the wait stands in front of the first t.
+  if constexpr (!LORA) pdl_wait();
   // after the wait: no kernel of this stream that still has tensor memory to allocate can be running. All 512 columns, so that both
   // CTAs' accumulators have the same addresses.
   if (warp == 1) { tmem_alloc_pair(&bars.tmem_base, 512); tmem_relinquish_pair(); }
@@ -732,7 +809,109 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const uint32_t tmem_base = bars.tmem_base;
   volatile int* abort_flag = &bars.abort_flag;
 
-  if (warp == 0) {
+  if constexpr (LORA) {
+    // by whole warps: as below, with the units of the adapters (lora.cuh) behind a tile's K blocks
+    if (warp < 2) {
+      constexpr int T_BYTES = BM * 32;
+      const uint32_t idesc1 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w1), idesc2 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w2);
+      RowGroups<8> rows, next;
+      RingPos rp;
+      bool ok = true, waited = false;
+      uint32_t it = 0, tile_it = 0;
+      int tm, col0, width;
+      if (first < tiles) { pair_tile(pt, first, tiles_m, tiles_n2, tm, col0, width); rows.load(lora.a, 2 * tm * BM, M, lane, status); }
+      for (int t = first; t < tiles && ok; t += step, ++tile_it) {
+        const bool more = t + step < tiles;
+        if (more) { pair_tile(pt, t + step, tiles_m, tiles_n2, tm, col0, width); next.load_ids(lora.a, 2 * tm * BM, M, lane); }
+        pair_tile(pt, t, tiles_m, tiles_n2, tm, col0, width);
+        const bool wide = t < pt.wide * tiles_m;
+        const CUtensorMap* tmB = wide ? &tmB1 : &tmB2;
+        const CUtensorMap* tmU = wide ? &lora.b : &lora.b2;
+        const int acc = tile_it & 1, row = (2 * tm + rank) * BM, half = width >> 1;
+        const uint32_t aph = (tile_it >> 1) & 1, d_tmem = tmem_base + acc * 256, idesc = wide ? idesc1 : idesc2;
+        RingPos at = rp;
+        if (warp == 0) {
+          if (elect_one()) {
+            const uint32_t bytes = 2 * A_BYTES + width * BK * 2;
+            for (int kb = 0; kb < kblocks; ++kb, at.next(stages)) {
+              const int s = at.s;
+              if (!mbar_wait(&bars.empty[s], at.ph ^ 1, abort_flag, status, KID_GEMM_BF16, 5)) { ok = false; break; }
+              if (rank == 0) mbar_expect_tx(&bars.full[s], bytes);
+              uint8_t* sa = smem + s * stage_bytes;
+              tma_load_2d_pair(sa, &tmA, &bars.full[s], kb * BK, row);
+              tma_load_2d_pair(sa + A_BYTES, tmB, &bars.full[s], kb * BK, col0 + rank * half);
+            }
+          }
+        } else if (rank == 0 && elect_one()) {
+          ok = mbar_wait(&bars.tmem_empty[acc], aph ^ 1, abort_flag, status, KID_GEMM_BF16, 6);
+          tc_fence_after();
+          for (int kb = 0; kb < kblocks && ok; ++kb, at.next(stages)) {
+            const int s = at.s;
+            if (!mbar_wait(&bars.full[s], at.ph, abort_flag, status, KID_GEMM_BF16, 7)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * stage_bytes);
+            const uint64_t da = umma_desc_sw128(sa, 16, 1024), db = umma_desc_sw128(sa + A_BYTES, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k) umma_f16_pair(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            umma_commit_pair(&bars.empty[s]);
+          }
+        }
+        it += kblocks;
+        rp.skip(kblocks, stages);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (more) next.load_steps(lora.a);
+        UnitWalk<8> walk(rows, lora_part(lora.a, col0, width, N), lora.a.parts, 0, 1);
+        UnitPair<8> p;
+        while (ok && p.next(walk)) {
+          const int s = rp.s;
+          uint8_t* sa = smem + s * stage_bytes;
+          if (warp == 0) {
+            if (!waited) { pdl_wait(); waited = true; }
+            if (elect_one()) {
+              ok = mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_BF16, 5);
+              if (ok) {
+                if (rank == 0) mbar_expect_tx(&bars.full[s], p.n * (4 * T_BYTES + width * 32));
+                tma_load_2d_pair(sa, &lora.t, &bars.full[s], p.step0 * 16, row);
+                tma_load_2d_pair(sa + T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step0 * 16, row);
+                tma_load_2d_pair(sa + A_BYTES, tmU, &bars.full[s], p.step0 * 16, p.adapter0 * N + col0 + rank * half);
+                if (p.n == 2) {
+                  tma_load_2d_pair(sa + 2 * T_BYTES, &lora.t, &bars.full[s], p.step1 * 16, row);
+                  tma_load_2d_pair(sa + 3 * T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step1 * 16, row);
+                  tma_load_2d_pair(sa + A_BYTES + half * 32, tmU, &bars.full[s], p.step1 * 16, p.adapter1 * N + col0 + rank * half);
+                }
+              }
+            }
+          } else if (rank == 0 && elect_one()) {
+            ok = mbar_wait(&bars.full[s], rp.ph, abort_flag, status, KID_GEMM_BF16, 7);
+            if (ok) {
+              tc_fence_after();
+              const uint32_t a0 = smem_u32(sa);
+              const uint64_t db0 = umma_desc_sw32(a0 + A_BYTES), db1 = umma_desc_sw32(a0 + A_BYTES + half * 32);
+              umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0), db0, idesc, p.mine0);
+              umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0 + T_BYTES), db0, idesc, p.mine0);
+              if (p.n == 2) {
+                umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0 + 2 * T_BYTES), db1, idesc, p.mine1);
+                umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0 + 3 * T_BYTES), db1, idesc, p.mine1);
+              }
+              umma_commit_pair(&bars.empty[s]);
+            }
+          }
+          ++it;
+          rp.next(stages);
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        if (warp == 1 && rank == 0 && ok && elect_one()) umma_commit_pair(&bars.tmem_full[acc]);
+        __syncwarp();
+        if (more) { next.vote(); rows = next; }
+      }
+      // the last commits of the even CTA have arrived before this CTA leaves (see below)
+      if (warp == 0 && elect_one())
+        for (uint32_t i = it > (uint32_t)stages ? it - stages : 0; i < it && ok; ++i)
+          ok = mbar_wait(&bars.empty[i % stages], (i / stages) & 1, abort_flag, status, KID_GEMM_BF16, 9);
+    }
+  }
+  if (!LORA && warp == 0) {
     if (elect_one()) {
       uint32_t it = 0;
       RingPos rp;
@@ -756,7 +935,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (uint32_t i = it > (uint32_t)stages ? it - stages : 0; i < it && ok; ++i)
         ok = mbar_wait(&bars.empty[i % stages], (i / stages) & 1, abort_flag, status, KID_GEMM_BF16, 9);
     }
-  } else if (warp == 1) {
+  } else if (!LORA && warp == 1) {
     if (rank == 0 && elect_one()) {
       const uint32_t idesc1 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w1), idesc2 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w2);
       uint32_t tile_it = 0;
@@ -780,7 +959,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (ok) umma_commit_pair(&bars.tmem_full[acc]);
       }
     }
-  } else {
+  } else if (warp >= 2) {
     const int q = warp & 3;                            // TMEM lane quarter
     uint32_t tile_it = 0;
     bool ok = true;
@@ -793,7 +972,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       if (!ok) break;
       tc_fence_after();
       const int row = (2 * tm + rank) * BM + q * 32 + lane;
-      store_tile_row<PARTS, DELTA>(tmem_base + (uint32_t(q * 32) << 16) + acc * 256, Cout, row, row < M, ldc, N, epi, col0, width, 0, tail, (warp - 2) >> 2, status);
+      store_tile_row<PARTS>(tmem_base + (uint32_t(q * 32) << 16) + acc * 256, Cout, row, row < M, ldc, N, epi, col0, width, 0, tail, (warp - 2) >> 2, status);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_leader(&bars.tmem_empty[acc]);
@@ -887,7 +1066,7 @@ FF_EXPORT int ff_gemm_bf16_pair_tiles(int M, int N, int epi, int pairs, int* til
 }
 
 static int pair_launch(const CUtensorMap& tmA, const void* W, void* Y, int M, int N, int K, int ldw, int ldy, int epi, const PairTiles& pt,
-                       const LinTail& tail, int* status, cudaStream_t stream) {
+                       const LinTail& tail, int* status, cudaStream_t stream, LoraDev* dev, const LoraCall* lora) {
   const int pairs = sm_count() / 2, tiles_m = (M + 2 * BM - 1) / (2 * BM), rest = N - pt.wide * pt.w1;
   const int tiles = tiles_m * (pt.wide + (rest > 0 ? (rest + pt.w2 - 1) / pt.w2 : 0)), grid = 2 * (tiles < pairs ? tiles : pairs);
   CUtensorMap tmB1, tmB2;
@@ -899,17 +1078,22 @@ static int pair_launch(const CUtensorMap& tmA, const void* W, void* Y, int M, in
   const int stages = fit == 7 && K <= 1536 ? 6 : fit < PAIR_STAGES ? fit : PAIR_STAGES;
   constexpr int SMEM = PAIR_RING + 1024;
   const bool stores = (epi == 0 || epi == 2) && tail.bias == nullptr && tail.act == 0 && tail.mul == nullptr;
-  auto kern = tail.delta != nullptr ? (stores ? gemm_bf16_pair_kernel<1, true> : gemm_bf16_pair_kernel<2, true>)
-                                    : (stores ? gemm_bf16_pair_kernel<1, false> : gemm_bf16_pair_kernel<2, false>);
+  if (lora != nullptr) {
+    if (int e = lora_maps(*dev, lora->t, lora->b, M, N, BM, pt.w1 / 2, pt.w2 / 2)) return e;
+    auto kern = stores ? gemm_bf16_pair_kernel<1, true> : gemm_bf16_pair_kernel<2, true>;
+    if (int e = opt_in_smem(kern, SMEM)) return e;
+    return launch_pdl(kern, dim3(grid), dim3(stores ? 192 : 320), SMEM, stream, 2, tmA, tmB1, tmB2, Y, M, N, K, ldy, epi, pt, stages, status, tail, *dev);
+  }
+  auto kern = stores ? gemm_bf16_pair_kernel<1, false> : gemm_bf16_pair_kernel<2, false>;
   if (int e = opt_in_smem(kern, SMEM)) return e;
-  if (int e = launch_pdl(kern, dim3(grid), dim3(stores ? 192 : 320), SMEM, stream, 2, tmA, tmB1, tmB2, Y, M, N, K, ldy, epi, pt, stages, status, tail)) return e;
+  if (int e = launch_pdl(kern, dim3(grid), dim3(stores ? 192 : 320), SMEM, stream, 2, tmA, tmB1, tmB2, Y, M, N, K, ldy, epi, pt, stages, status, tail, NoLora{})) return e;
   return launch_result();
 }
 
 // Y[M,N] = X[M,K] · W[N,K]ᵀ. epi: 0 bf16 out, 1 fused SwiGLU (out has N/2 columns), 2 fp32 out.
 // ldx / ldw / ldy in elements. Returns 0 or an error code (see host_util.h).
 static int gemm_bf16_launch(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy,
-                            int epi, LinTail tail, int* status, cudaStream_t stream) {
+                            int epi, LinTail tail, int* status, cudaStream_t stream, const LoraCall* lora = nullptr) {
   if (M <= 0 || N <= 0 || K <= 0) return FF_HOST_BAD_SHAPE;
   if ((K % 8) || (ldx % 8) || (ldw % 8)) return FF_HOST_BAD_ALIGN;
   if (epi == 1 && (N % 256)) return FF_HOST_BAD_SHAPE;
@@ -919,6 +1103,8 @@ static int gemm_bf16_launch(const void* X, const void* W, void* Y, int M, int N,
   if (reinterpret_cast<uintptr_t>(Y) & 15) return FF_HOST_BAD_ALIGN;
   CUtensorMap tmA;
   if (int e = make_tmap_2d(&tmA, X, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, K, M, (uint64_t)ldx * 2, BK, BM)) return e;
+  LoraDev dev = {};
+  if (lora != nullptr) dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts};
   PairTiles pt;
   float waves;
   if (one_cta_tiles(M, N, K, epi, tail.gate != 0, pt, waves)) {
@@ -926,12 +1112,20 @@ static int gemm_bf16_launch(const void* X, const void* W, void* Y, int M, int N,
     CUtensorMap tmB;
     if (int e = make_tmap_2d(&tmB, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, K, N, (uint64_t)ldw * 2, BK, BN)) return e;
     const int smem = STAGES * (BM + BN) * BK * 2 + 1024, tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-    auto kern = tail.delta != nullptr ? gemm_bf16_kernel<BN, STAGES, 0, true> : gemm_bf16_kernel<BN, STAGES, 0, false>;
+    const int grid = tiles < sm_count() ? tiles : sm_count();
+    if (lora != nullptr) {
+      if (int e = lora_maps(dev, lora->t, lora->b, M, N, BM, BN, BN)) return e;
+      auto kern = gemm_bf16_kernel<BN, STAGES, 0, true>;
+      if (int e = opt_in_smem(kern, smem)) return e;
+      kern<<<grid, 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, M, N, K, ldy, epi, status, CommArgs{}, GroupArgs{}, tail, dev);
+      return launch_result();
+    }
+    auto kern = gemm_bf16_kernel<BN, STAGES, 0>;
     if (int e = opt_in_smem(kern, smem)) return e;
-    kern<<<tiles < sm_count() ? tiles : sm_count(), 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, M, N, K, ldy, epi, status, CommArgs{}, GroupArgs{}, tail);
+    kern<<<grid, 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, M, N, K, ldy, epi, status, CommArgs{}, GroupArgs{}, tail, NoLora{});
     return launch_result();
   }
-  return pair_launch(tmA, W, Y, M, N, K, ldw, ldy, epi, pt, tail, status, stream);
+  return pair_launch(tmA, W, Y, M, N, K, ldw, ldy, epi, pt, tail, status, stream, &dev, lora);
 }
 
 FF_EXPORT int ff_gemm_bf16(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy,
@@ -986,18 +1180,16 @@ FF_EXPORT int ff_gemm_bf16_gated(const void* X, const void* W, void* Y, int M, i
   return gemm_bf16_launch(X, W, Y, M, N, K, ldx, ldw, ldy, 1, tail, status, stream);
 }
 
-// Y = X Wᵀ + delta for the rows whose id lies within [0, adapters) (lora.cu), one rounding; epi 0, 1 or 3 (`rope`) as above. delta: FP32, pitch ldd,
-// N a multiple of 8.
-int ff_gemm_bf16_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, const float* delta, const int* ids, int ldd,
-                       int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status, cudaStream_t stream) {
-  if (delta == nullptr || ids == nullptr || N % 8 || ldd % 8 || ldd < N || (reinterpret_cast<uintptr_t>(delta) & 15)) return FF_HOST_BAD_ALIGN;
+// Y = X Wᵀ with the adapters of the rows (lora.cu) in the sums, rounded once; epi 0, 1 (activation `gate`, `limit`) or 3 (`rope`) as above. Launched directly behind
+// the kernel that writes lora->t, which triggers its dependents behind its own wait and with its tensor memory in hand.
+int ff_gemm_bf16_lora(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, const LoraCall* lora, int epi, int gate,
+                      float limit, const QkvRope* rope, int* status, cudaStream_t stream) {
   LinTail tail = {};
   tail.gate = gate; tail.limit = limit;
-  tail.delta = delta; tail.ids = ids; tail.ldd = ldd; tail.adapters = adapters;
   if (epi == 3) {
     if (int e = rope_tail(tail, rope, N)) return e;
   }
-  return gemm_bf16_launch(X, W, Y, M, N, K, ldx, ldw, ldy, epi, tail, status, stream);
+  return gemm_bf16_launch(X, W, Y, M, N, K, ldx, ldw, ldy, epi, tail, status, stream, lora);
 }
 
 // Block-diagonal product: for every head h, Y[:, h * c_cols + (0..N)] = X[:, h * a_cols + (0..K)] · W[h]ᵀ with W [heads * N, K]. Columns of
@@ -1022,7 +1214,7 @@ FF_EXPORT int ff_gemm_bf16_heads(const void* X, const void* W, void* Y, int M, i
   CommArgs none = {};
   GroupArgs ga = {};
   ga.heads = heads; ga.a_cols = a_cols; ga.c_cols = c_cols;
-  kern<<<grid, 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, M, N, K, ldy, 0, status, none, ga, LinTail{});
+  kern<<<grid, 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, M, N, K, ldy, 0, status, none, ga, LinTail{}, NoLora{});
   return launch_result();
 }
 
@@ -1050,7 +1242,7 @@ FF_EXPORT int ff_moe_grouped_gemm_tiled(const void* Xs, const void* W, void* Y, 
   GroupArgs ga = {seg_off, counts, E_local};
   LinTail tail = {};
   if (limit > 0.f) { tail.gate = 5; tail.limit = limit; }
-  kern<<<sm_count(), 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, capacity, Nw, K, ldy, epi, status, none, ga, tail);
+  kern<<<sm_count(), 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, capacity, Nw, K, ldy, epi, status, none, ga, tail, NoLora{});
   return launch_result();
 }
 
@@ -1100,7 +1292,7 @@ FF_EXPORT int ff_ag_gemm(const unsigned long long* ptrs, int rank, int world, lo
   r = opt_in_smem(kern, smem); if (r) return r;
   const int tiles = (M / BM) * ((N + BN - 1) / BN);
   const int grid = tiles < sm_count() ? tiles : sm_count();
-  kern<<<grid, 320, smem, stream>>>(tmA0, tmA1, tmX, tmB, Y, M, N, K, ldy, epi, status, ca, GroupArgs{}, LinTail{});
+  kern<<<grid, 320, smem, stream>>>(tmA0, tmA1, tmX, tmB, Y, M, N, K, ldy, epi, status, ca, GroupArgs{}, LinTail{}, NoLora{});
   return launch_result();
 }
 
@@ -1126,7 +1318,7 @@ FF_EXPORT int ff_gemm_rs(const unsigned long long* ptrs, int rank, int world, lo
   r = opt_in_smem(kern, smem); if (r) return r;
   const int tiles = (M / BM) * ((N + BN - 1) / BN);
   const int grid = tiles < sm_count() ? tiles : sm_count();
-  kern<<<grid, 192, smem, stream>>>(tmA, tmA, tmA, tmB, nullptr, M, N, K, N, 0, status, ca, GroupArgs{}, LinTail{});
+  kern<<<grid, 192, smem, stream>>>(tmA, tmA, tmA, tmB, nullptr, M, N, K, N, 0, status, ca, GroupArgs{}, LinTail{}, NoLora{});
   return launch_result();
 }
 

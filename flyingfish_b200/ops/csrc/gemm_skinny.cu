@@ -31,6 +31,8 @@
 #include <mutex>
 #include <vector>
 #include "skinny_common.cuh"
+#include "lora.cuh"
+#include <type_traits>
 
 static_assert(FF_SKINNY_MAX_ROWS == ff::STOK, "rows of a decode product");
 
@@ -57,32 +59,11 @@ struct SkinnyTail {
   const __nv_bfloat16* bias; int act;
   const __nv_bfloat16* mul; const int* mul_rows; int ldm, mul_table;
   int gate; float limit;
-  // added to the FP32 sums of rows whose id is within [0, adapters): delta[row][column], pitch ldd, written by the kernel in front of this one
-  const float* delta; const int* ids; int ldd, adapters;
 };
 
-// eight columns of a row's delta, where it has one
-__device__ __forceinline__ void add_delta8(const SkinnyTail& tail, int t, int col, float (&v)[8]) {
-  if ((unsigned)tail.ids[t] >= (unsigned)tail.adapters) return;
-  const float4* d = reinterpret_cast<const float4*>(tail.delta + (size_t)t * tail.ldd + col);
-  const float4 x = __ldcg(d), y = __ldcg(d + 1);
-  v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-  v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-}
-
 // emit_pair with the choice of the gate
-template <bool DELTA>
 __device__ __forceinline__ void emit_gated(const SkinnyEpi& ep, const SkinnyTail& tail, __nv_bfloat16* __restrict__ Y, int N, int ldy, int t, int tile, int j8,
                                            const float* lo, const float* hi, int* status) {
-  if constexpr (DELTA) {
-    float dl[8], dh[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { dl[j] = lo[j]; dh[j] = hi[j]; }
-    add_delta8(tail, t, tile * 128 + j8 * 8, dl);           // N is a multiple of 128: whole tiles
-    add_delta8(tail, t, tile * 128 + 64 + j8 * 8, dh);
-    emit_gated<false>(ep, tail, Y, N, ldy, t, tile, j8, dl, dh, status);
-    return;
-  }
   if (tail.gate == 0) { emit_pair(ep, Y, N, ldy, t, tile, j8, lo, hi, status); return; }
   const int col = tile * 64 + j8 * 8;
   if (col >= N / 2) return;
@@ -95,7 +76,7 @@ __device__ __forceinline__ void emit_gated(const SkinnyEpi& ep, const SkinnyTail
 }
 
 // Where the final values of a tile go: Y, or (FUSE_AR) the arena slot of this rank on every rank.
-template <bool FUSE_AR, bool DELTA = false>
+template <bool FUSE_AR>
 struct TileSink {
   __nv_bfloat16* Y; int N, ldy; bool vec8;      // vec8: 16-byte stores of eight values are aligned
   SkinnyTail tail;
@@ -109,7 +90,6 @@ struct TileSink {
 #pragma unroll
     for (int j = 0; j < 8; ++j) a[j] = sums[j];
     if (!FUSE_AR) {
-      if constexpr (DELTA) add_delta8(tail, t, col, a);
       const int act = tail.act;
       if (tail.bias != nullptr) {
 #pragma unroll
@@ -275,12 +255,12 @@ __device__ __forceinline__ void allreduce_tile(const TileSink<true>& sink, int M
 
 // cl_size == 1: persistent stream-K over gridDim.x CTAs.  cl_size > 1: cluster split-K, cluster c
 // owns weight tile c, CTA r of it the k-blocks [kblocks*r/S, kblocks*(r+1)/S).
-template <bool FUSE_AR, bool DELTA>
+template <bool FUSE_AR, bool LORA>
 __global__ void __launch_bounds__(192, 2)
 gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                    __nv_bfloat16* __restrict__ Y, int M, int N, int K, int ldy, int ntok, int tile_rows, int stages,
                    int cl_size, int pipe_off, float* __restrict__ scratch, int* __restrict__ counters, int* status,
-                   PeerArena ar, SkinnyEpi ep, const SkinnyTail tail) {
+                   PeerArena ar, SkinnyEpi ep, const SkinnyTail tail, const __grid_constant__ std::conditional_t<LORA, LoraDev, NoLora> lora) {
   pdl_trigger();
   if (cl_size > 1) cluster_arrive_relaxed();         // phase A: "this CTA runs" (waited on before the first remote store)
   if (threadIdx.x == 0) FF_TL(status, KID_GEMM_SKINNY, 0);
@@ -315,7 +295,8 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   // Thread 0 is the TMA producer. It initialises the barriers and at once requests the first `stages`
   // weight tiles (weights are written by no kernel, so this needs no wait on the preceding kernel),
   // while warp 1 allocates TMEM; the other roles meet it at the block barrier.
-  const uint32_t pre = (uint32_t)min((long long)stages, u1 - u0);
+  // With adapters the stages of their units stand behind a segment's, so no more than the first segment's weights come early.
+  const uint32_t pre = (uint32_t)min((long long)stages, LORA ? min(u1 - u0, (long long)(kblocks - (int)(u0 % kblocks))) : u1 - u0);
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmW); tma_prefetch_desc(&tmX);
     for (int i = 0; i < stages; ++i) { mbar_init(&bars.full[i], 1); mbar_init(&bars.empty[i], 1); }
@@ -339,12 +320,110 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   volatile int* abort_flag = &bars.abort_flag;
   if (threadIdx.x == 0) FF_TL(status, KID_GEMM_SKINNY, 1);
 
-  if (warp == 0) {
+  if constexpr (LORA) {
+    // As below, by whole warps: behind a segment's K blocks come the units of the adapters (lora.cuh). The kernel in front of this one (lora.cu) lets it
+    // start only once everything before that kernel is done: X and the ids are there, the weights stream while t is computed, and the
+    // wait stands in front of the first t.
+    if (warp < 2) {
+      RowGroups<4> rows;
+      rows.load(lora.a, 0, M, lane, status);
+      uint32_t it = 0, seg_it = 0; RingPos rp; bool ok = true, waited = false;
+      long long u = u0; Segment sg;
+      const uint32_t idesc = umma_idesc(1, 1, 0, 0, STOK, tile_rows);
+      const int t_bytes = ntok * 32, b_bytes = tile_rows * 32;
+      while (ok && next_segment(u, u1, kblocks, sg)) {
+        const int n = sg.kb1 - sg.kb0, acc = seg_it & 1;
+        const uint32_t aph = (seg_it >> 1) & 1, d_tmem = tmem_base + acc * tile_rows;
+        RingPos at = rp;
+        if (warp == 0) {
+          if (elect_one()) {
+            const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+            for (int kb = sg.kb0; kb < sg.kb1; ++kb, at.next(stages)) {
+              const int s = at.s;
+              uint8_t* sa = pipe + s * stage_bytes;
+              if (it + (kb - sg.kb0) >= pre) {
+                if (!mbar_wait(&bars.empty[s], at.ph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 1)) { ok = false; break; }
+                mbar_expect_tx(&bars.full[s], tx_bytes);
+                tma_load_2d_hint(sa + A_BYTES, &tmW, &bars.full[s], kb * SBK, sg.tile * tile_rows, pol_w);
+              }
+              tma_load_2d_hint(sa, &tmX, &bars.full[s], kb * SBK, 0, pol_x);
+            }
+          }
+        } else if (elect_one()) {
+          ok = mbar_wait(&bars.tmem_empty[acc], aph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 2);
+          tc_fence_after();
+          for (int kb = sg.kb0; kb < sg.kb1 && ok; ++kb, at.next(stages)) {
+            const int s = at.s;
+            if (!mbar_wait(&bars.full[s], at.ph, abort_flag, status, KID_GEMM_SKINNY, 3)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(pipe + s * stage_bytes);
+            const uint64_t da = umma_desc_sw128(sa, 16, 1024), db = umma_desc_sw128(sa + A_BYTES, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < SBK / 16; ++k) umma_f16(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.kb0) || k > 0);
+            umma_commit(&bars.empty[s]);
+          }
+        }
+        it += n;
+        rp.skip(n, stages);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // the units of this CTA's share of the tile
+        int share = crank, shares = clustered ? cl_size : 1;
+        if (!clustered && n < kblocks) {
+          const int c_first = unit_owner((long long)sg.tile * kblocks, total, G);
+          share = blockIdx.x - c_first;
+          shares = unit_owner((long long)(sg.tile + 1) * kblocks - 1, total, G) - c_first + 1;
+        }
+        UnitWalk<4> walk(rows, lora_part(lora.a, sg.tile * tile_rows, tile_rows, N), lora.a.parts, share, shares);
+        UnitPair<4> p;
+        while (ok && p.next(walk)) {
+          const int s = rp.s;
+          if (warp == 0) {
+            if (!waited) { pdl_wait(); waited = true; }
+            if (elect_one()) {
+              ok = it < (uint32_t)stages || mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 1);
+              if (ok) {
+                uint8_t* sa = pipe + s * stage_bytes;
+                mbar_expect_tx(&bars.full[s], p.n * (2 * t_bytes + b_bytes));
+                tma_load_2d(sa, &lora.t, &bars.full[s], p.step0 * 16, 0);
+                tma_load_2d(sa + t_bytes, &lora.t, &bars.full[s], lora.a.R + p.step0 * 16, 0);
+                tma_load_2d(sa + A_BYTES, &lora.b, &bars.full[s], p.step0 * 16, p.adapter0 * N + sg.tile * tile_rows);
+                if (p.n == 2) {
+                  tma_load_2d(sa + 2 * t_bytes, &lora.t, &bars.full[s], p.step1 * 16, 0);
+                  tma_load_2d(sa + 3 * t_bytes, &lora.t, &bars.full[s], lora.a.R + p.step1 * 16, 0);
+                  tma_load_2d(sa + A_BYTES + b_bytes, &lora.b, &bars.full[s], p.step1 * 16, p.adapter1 * N + sg.tile * tile_rows);
+                }
+              }
+            }
+          } else if (elect_one()) {
+            ok = mbar_wait(&bars.full[s], rp.ph, abort_flag, status, KID_GEMM_SKINNY, 3);
+            if (ok) {
+              tc_fence_after();
+              const uint32_t sa = smem_u32(pipe + s * stage_bytes);
+              const uint64_t db0 = umma_desc_sw32(sa + A_BYTES), db1 = umma_desc_sw32(sa + A_BYTES + b_bytes);
+              umma_f16_lanes(d_tmem, umma_desc_sw32(sa), db0, idesc, p.mine0);
+              umma_f16_lanes(d_tmem, umma_desc_sw32(sa + t_bytes), db0, idesc, p.mine0);
+              if (p.n == 2) {
+                umma_f16_lanes(d_tmem, umma_desc_sw32(sa + 2 * t_bytes), db1, idesc, p.mine1);
+                umma_f16_lanes(d_tmem, umma_desc_sw32(sa + 3 * t_bytes), db1, idesc, p.mine1);
+              }
+              umma_commit(&bars.empty[s]);
+            }
+          }
+          ++it;
+          rp.next(stages);
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        if (warp == 1 && ok && elect_one()) umma_commit(&bars.tmem_full[acc]);
+        __syncwarp();
+        ++seg_it;
+      }
+    }
+  }
+  if (!LORA && warp == 0) {
     if (elect_one()) {
       const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      // With a delta the kernel in front of this one has let it start only once everything before that kernel was done (lora.cu): X is there, and
-      // the weights stream while the delta is computed. The epilogue waits.
-      if (!DELTA) pdl_wait();
+      pdl_wait();
       FF_TL(status, KID_GEMM_SKINNY, 3);
       uint32_t it = 0; RingPos rp; bool ok = true;
       long long u = u0; Segment sg;
@@ -362,7 +441,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       }
       FF_TL(status, KID_GEMM_SKINNY, 4);
     }
-  } else if (warp == 1) {
+  } else if (!LORA && warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = umma_idesc(1, 1, 0, 0, STOK, tile_rows);
       uint32_t it = 0, seg_it = 0; RingPos rp; bool ok = true;
@@ -389,7 +468,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       }
       FF_TL(status, KID_GEMM_SKINNY, 6);
     }
-  } else {
+  } else if (warp >= 2) {
     // ---- epilogue warps 2..5 ; TMEM lane quarter = warp % 4 ; lane = token ----------------------
     const int q = warp & 3;
     const int t_own = q * 32 + lane;              // token row held by this thread's TMEM lane
@@ -400,7 +479,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     if (e == 0) FF_TL(status, KID_GEMM_SKINNY, 7);
     int ar_epoch = 0;
     if (FUSE_AR) ar_epoch = ld_volatile(arena_epoch(ar)) + 1;
-    TileSink<FUSE_AR, DELTA> sink;
+    TileSink<FUSE_AR> sink;
     sink.Y = Y; sink.N = N; sink.ldy = ldy; sink.ar = ar; sink.parity = ar_epoch & 1;
     sink.tail = tail;
     sink.vec8 = FUSE_AR || ((ldy % 8 == 0) && ((reinterpret_cast<uintptr_t>(Y) & 15) == 0));
@@ -451,7 +530,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             if (t_own < M) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                emit_gated<DELTA>(ep, tail, Y, N, ldy, t_own, sg.tile, (c >> 3) + h, reinterpret_cast<const float*>(g) + 8 * h,
+                emit_gated(ep, tail, Y, N, ldy, t_own, sg.tile, (c >> 3) + h, reinterpret_cast<const float*>(g) + 8 * h,
                           reinterpret_cast<const float*>(u) + 8 * h, status);
             }
           }
@@ -554,7 +633,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 #pragma unroll
             for (int g = 0; g < 4; g += 2) {
               const int pr = i0 + 128 * (g >> 1);
-              if (pr < i_end) emit_gated<DELTA>(ep, tail, Y, N, ldy, pr >> 3, sg.tile, pr & 7, a8[g], a8[g + 1], status);
+              if (pr < i_end) emit_gated(ep, tail, Y, N, ldy, pr >> 3, sg.tile, pr & 7, a8[g], a8[g + 1], status);
             }
           } else {
 #pragma unroll
@@ -592,7 +671,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
               lo[0] += l0.x; lo[1] += l0.y; lo[2] += l0.z; lo[3] += l0.w; lo[4] += l1.x; lo[5] += l1.y; lo[6] += l1.z; lo[7] += l1.w;
               hi[0] += h0.x; hi[1] += h0.y; hi[2] += h0.z; hi[3] += h0.w; hi[4] += h1.x; hi[5] += h1.y; hi[6] += h1.z; hi[7] += h1.w;
             }
-            emit_gated<DELTA>(ep, tail, Y, N, ldy, crank + ti * cl_size, sg.tile, j8, lo, hi, status);
+            emit_gated(ep, tail, Y, N, ldy, crank + ti * cl_size, sg.tile, j8, lo, hi, status);
           }
         } else
         for (int i = e; i < rows * vpr; i += 128) {
@@ -886,7 +965,7 @@ FF_EXPORT int ff_gemm_skinny_plan_epi(int M, int N, int K, int epi, long long* s
 
 static int gemm_skinny_launch(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy,
                               int grid, float* scratch, int* counters, int* status, cudaStream_t stream,
-                              const PeerArena* arena, const SkinnyEpi* epi = nullptr, const SkinnyTail& tail = SkinnyTail{}) {
+                              const PeerArena* arena, const SkinnyEpi* epi = nullptr, const SkinnyTail& tail = SkinnyTail{}, const LoraCall* lora = nullptr) {
   if (M <= 0 || N <= 0 || K <= 0) return FF_HOST_BAD_SHAPE;
   SkinnyEpi ep = {};
   if (epi != nullptr) {
@@ -915,17 +994,26 @@ static int gemm_skinny_launch(const void* X, const void* W, void* Y, int M, int 
   if (cfg.stages < 2) return FF_HOST_TOO_LARGE;
   const int smem = cfg.pipe_off + cfg.stages * (ntok + cfg.tile_rows) * SBK * 2 + skinny_tail_slack(ntok, cfg.tile_rows) + 1024;
   __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(Y);
-  if (arena == nullptr) {
-    auto kern = tail.delta != nullptr ? gemm_skinny_kernel<false, true> : gemm_skinny_kernel<false, false>;
+  const PeerArena none = {};
+  if (lora != nullptr) {
+    LoraDev dev = {};
+    dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts};
+    if (int e = lora_maps(dev, lora->t, lora->b, M, N, ntok, cfg.tile_rows, cfg.tile_rows)) return e;
+    auto kern = gemm_skinny_kernel<false, true>;
     r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
-    PeerArena none = {};
     return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
-                      cfg.stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail);
+                      cfg.stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail, dev);
+  }
+  if (arena == nullptr) {
+    auto kern = gemm_skinny_kernel<false, false>;
+    r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
+    return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
+                      cfg.stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail, NoLora{});
   }
   auto kern = gemm_skinny_kernel<true, false>;
   r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
   return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
-                    cfg.stages, cl, cfg.pipe_off, scratch, counters, status, *arena, ep, tail);
+                    cfg.stages, cl, cfg.pipe_off, scratch, counters, status, *arena, ep, tail, NoLora{});
 }
 
 // `grid` is the value returned by ff_gemm_skinny_plan for the same problem.
@@ -982,16 +1070,13 @@ FF_EXPORT int ff_gemm_skinny_rope_kv(const void* X, const void* W, void* Y, int 
   return gemm_skinny_launch(X, W, Y, M, N, K, ldx, ldw, ldy, grid, scratch, counters, status, stream, nullptr, &ep);
 }
 
-// Y = X Wᵀ + delta for the rows whose id lies within [0, adapters) (lora.cu), one rounding. epi 0: plain, 1: gate / up with the activation (`gate`,
-// `limit`), 2: rotary embedding and cache write (`rope`). delta: FP32, pitch ldd (a multiple of 8, at least N rounded up to 8), written by a kernel
-// that was launched directly in front and that triggers its dependents behind its own wait. `grid` from ff_gemm_skinny_plan(_epi).
-int ff_gemm_skinny_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, int grid, float* scratch, int* counters,
-                         const float* delta, const int* ids, int ldd, int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status,
-                         cudaStream_t stream) {
-  if (delta == nullptr || ids == nullptr || ldd % 8 || ldd < (N + 7) / 8 * 8 || (reinterpret_cast<uintptr_t>(delta) & 15)) return FF_HOST_BAD_ALIGN;
+// Y = X Wᵀ with the adapters of the rows (lora.cu) in the sums, rounded once. epi 0: plain, 1: gate / up with the activation (`gate`, `limit`), 2: rotary
+// embedding and cache write (`rope`). Launched directly behind the kernel that writes lora->t, which triggers its dependents behind its own
+// wait. `grid` from ff_gemm_skinny_plan(_epi).
+int ff_gemm_skinny_lora(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, int grid, float* scratch, int* counters,
+                        const LoraCall* lora, int epi, int gate, float limit, const QkvRope* rope, int* status, cudaStream_t stream) {
   SkinnyTail tail = {};
   tail.gate = gate; tail.limit = limit;
-  tail.delta = delta; tail.ids = ids; tail.ldd = ldd; tail.adapters = adapters;
   SkinnyEpi ep = {};
   ep.mode = epi;
   if (epi == 2) {
@@ -1000,7 +1085,7 @@ int ff_gemm_skinny_delta(const void* X, const void* W, void* Y, int M, int N, in
     ep.kcache = static_cast<__nv_bfloat16*>(rope->kcache); ep.vcache = static_cast<__nv_bfloat16*>(rope->vcache);
     ep.hq = rope->hq; ep.hkv = rope->hkv; ep.rot_dim = rope->rot_dim; ep.block_size = rope->block_size; ep.num_blocks = rope->num_blocks;
   }
-  return gemm_skinny_launch(X, W, Y, M, N, K, ldx, ldw, ldy, grid, scratch, counters, status, stream, nullptr, epi ? &ep : nullptr, tail);
+  return gemm_skinny_launch(X, W, Y, M, N, K, ldx, ldw, ldy, grid, scratch, counters, status, stream, nullptr, epi ? &ep : nullptr, tail, lora);
 }
 
 // Row-parallel projection fused with the tensor-parallel all-reduce (decode shapes, M <= 128):

@@ -40,24 +40,29 @@ inline EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
-// 2-D row-major tensor [outer, inner] with `row_bytes` pitch; box [box_outer, box_inner];
-// 128-byte swizzle when the box's inner extent is exactly 128 bytes, none otherwise.
+// 2-D row-major tensor [outer, inner] with `row_bytes` pitch; box [box_outer, box_inner], its inner extent at most the swizzle's width.
 inline int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dt, int elem_bytes,
                         uint64_t inner, uint64_t outer, uint64_t row_bytes, uint32_t box_inner,
-                        uint32_t box_outer, bool swizzle128 = true) {
+                        uint32_t box_outer, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return FF_HOST_NO_DRIVER;
   if ((reinterpret_cast<uintptr_t>(base) & 15) || (row_bytes & 15)) return FF_HOST_BAD_ALIGN;
-  if (box_inner * elem_bytes > 128 && swizzle128) return FF_HOST_BAD_SHAPE;
+  if ((swizzle == CU_TENSOR_MAP_SWIZZLE_128B && box_inner * elem_bytes > 128) || (swizzle == CU_TENSOR_MAP_SWIZZLE_32B && box_inner * elem_bytes > 32)) return FF_HOST_BAD_SHAPE;
   if (box_outer > 256 || box_inner > 256) return FF_HOST_BAD_SHAPE;
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+  CUresult r = fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FF_HOST_OK : FF_HOST_TMAP_FAIL;
+}
+// 128-byte swizzle, or none
+inline int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dt, int elem_bytes,
+                        uint64_t inner, uint64_t outer, uint64_t row_bytes, uint32_t box_inner,
+                        uint32_t box_outer, bool swizzle128 = true) {
+  return make_tmap_2d(out, base, dt, elem_bytes, inner, outer, row_bytes, box_inner, box_outer,
+                      swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // 3-D tensor [d2, d1, d0] (d0 innermost) with byte strides for d1 and d2.

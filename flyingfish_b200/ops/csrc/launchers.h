@@ -20,13 +20,18 @@ struct QkvRope {
   const float* cos_sin; const int* slots; void *kcache, *vcache;
   int hq, hkv, rot_dim, block_size, num_blocks;
 };
-int ff_gemm_skinny_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, int grid, float* scratch, int* counters,
-                         const float* delta, const int* ids, int ldd, int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status,
-                         cudaStream_t stream);
+// adapters of a product's rows (lora.cuh): t [M, 2R], b [adapters, N, R]
+struct LoraCall {
+  const void *t, *b;
+  const int *ids, *ranks, *part_of;
+  int adapters, R, parts;
+};
+int ff_gemm_skinny_lora(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, int grid, float* scratch, int* counters,
+                        const LoraCall* lora, int epi, int gate, float limit, const QkvRope* rope, int* status, cudaStream_t stream);
 
 // gemm_bf16.cu
-int ff_gemm_bf16_delta(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, const float* delta, const int* ids, int ldd,
-                       int adapters, int epi, int gate, float limit, const QkvRope* rope, int* status, cudaStream_t stream);
+int ff_gemm_bf16_lora(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, const LoraCall* lora, int epi, int gate,
+                      float limit, const QkvRope* rope, int* status, cudaStream_t stream);
 
 // attention_tc.cu
 FF_EXPORT int ff_attn_prefill_tc(const void* q, const void* kcache, const void* vcache, const int* block_table, const int* q_start, const int* q_lens,

@@ -138,6 +138,7 @@ struct RingPos {
   int s = 0;
   uint32_t ph = 0;
   __device__ __forceinline__ void next(int n) { if (++s == n) { s = 0; ph ^= 1; } }
+  __device__ __forceinline__ void skip(int by, int n) { s += by; ph ^= (s / n) & 1; s %= n; }
 };
 
 // ---------------------------------------------------------------------------------------

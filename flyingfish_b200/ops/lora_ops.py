@@ -16,7 +16,6 @@ from . import BF16, SKINNY_MAX_M, _count, _require, _rows2d, ref, rope_in_produc
 from .lib import KernelError, check, kernels, status_tensor
 
 MAX_RANK = 1024                  # rank rows of a stack, all parts of a fused projection together
-DELTA_BYTES = 256 << 20          # prompts are done in portions of rows whose 32-bit deltas take at most this much
 GATES = (0, 3, 5)                # gates that the products' epilogues know (ops.linear_swiglu)
 
 
@@ -79,9 +78,9 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
 
 
 class _Lora(ctypes.Structure):            # FfLora of csrc/lora.cu
-    _fields_ = [(n, c_void_p) for n in ("x", "w", "y", "a", "b", "scale", "ranks", "ids", "part_of", "t", "delta", "scratch", "counters", "status", "cos_sin",
+    _fields_ = [(n, c_void_p) for n in ("x", "w", "y", "a", "b", "scale", "ranks", "ids", "part_of", "t", "scratch", "counters", "status", "cos_sin",
                                         "slots", "kcache", "vcache")] + [("scratch_bytes", c_longlong), ("counter_bytes", c_longlong)] + \
-               [(n, c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "ldd", "delta_rows", "R", "adapters", "parts", "epi", "gate")] + [("limit", c_float)] + \
+               [(n, c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "R", "adapters", "parts", "epi", "gate")] + [("limit", c_float)] + \
                [(n, c_int) for n in ("hq", "hkv", "rot_dim", "block_size", "num_blocks")]
 
 
@@ -117,21 +116,15 @@ def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tenso
     _require(out.shape == (m, width) and out.stride(1) == 1 and out.dtype == BF16, "linear_lora: bad output tensor")
     if m == 0:
         return out
-    ldd = (n + 7) // 8 * 8
-    rows = m if m <= SKINNY_MAX_M else min(m, max(256, DELTA_BYTES // (4 * ldd) // 256 * 256))
-    # one buffer of its own per call: t (two BF16 words per value), then the deltas
-    head = (rows * r * 4 + 255) // 256 * 256
-    buf = torch.empty(head + rows * ldd * 4, dtype=torch.uint8, device=dev)
+    t = torch.empty(m, 2 * r, dtype=BF16, device=dev)         # of this call alone
     ws = workspace(dev)
-    at = buf.data_ptr()
     opt = lambda t: 0 if t is None else t.data_ptr()
     cs, slots, kc, vc, heads = rope if rope is not None else (None, None, None, None, (0, 0, 0, 0, 0))
     lib = kernels()
     for attempt in (0, 1):
-        form = _Lora(x.data_ptr(), w.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), opt(ranks), ids.data_ptr(), opt(part_of), at,
-                     at + head, ws.gemm_scratch.data_ptr(), ws.gemm_counters.data_ptr(), status_tensor(dev).data_ptr(), opt(cs), opt(slots), opt(kc), opt(vc),
-                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, m, n, k, ldx, ldw, out.stride(0), ldd, rows, r, count, parts, epi, gate, limit,
-                     *heads)
+        form = _Lora(x.data_ptr(), w.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), opt(ranks), ids.data_ptr(), opt(part_of), t.data_ptr(),
+                     ws.gemm_scratch.data_ptr(), ws.gemm_counters.data_ptr(), status_tensor(dev).data_ptr(), opt(cs), opt(slots), opt(kc), opt(vc),
+                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, m, n, k, ldx, ldw, out.stride(0), r, count, parts, epi, gate, limit, *heads)
         rc = lib.ff_linear_lora(ctypes.byref(form), c_void_p(torch.cuda.current_stream().cuda_stream))
         if rc != -5 or attempt or m > SKINNY_MAX_M:
             break
@@ -141,7 +134,7 @@ def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tenso
         ws.ensure("gemm_scratch", scratch_b.value // 4)
         _require(counter_b.value // 4 <= ws.gemm_counters.numel(), "linear_lora: too many column tiles for counters")
     check(rc, "ff_linear_lora")
-    _count(3 * ((m + rows - 1) // rows))
+    _count(2)
     return out
 
 

@@ -253,16 +253,6 @@ def test_captured_and_on_other_streams(cuda, m):
 
 
 @pytest.mark.gpu
-def test_prompts_in_portions(cuda, monkeypatch):
-    """Rows whose deltas do not fit the buffer are done in portions: the same bits."""
-    x, w, st, ids = _case(900, 256, 512, 32, 5, seed=9, device=cuda)
-    ids = torch.sort(ids).values
-    whole = lora_ops.linear_lora(x, w, st, ids)
-    monkeypatch.setattr(lora_ops, "DELTA_BYTES", 300 * 512 * 4)
-    assert torch.equal(lora_ops.linear_lora(x, w, st, ids), whole)
-
-
-@pytest.mark.gpu
 def test_refusals_on_the_device(cuda):
     x, w, st, ids = _case(4, 64, 48, 16, 2, device=cuda)
     for args in ((x.float(), w, st, ids), (x, w.float(), st, ids), (x, w, st, ids.cpu()), (x, w, st._replace(scale=st.scale.cpu()), ids), (x, w[:, :56], st, ids)):
