@@ -445,7 +445,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (more) next.load_steps(lora.a);
-        UnitWalk<4> walk(rows, lora_part(lora.a, tn * BN, BN, N), lora.a.parts, 0, 1);
+        UnitWalk<4> walk(rows, lora_part(lora.a, tn * BN, BN, N), lora.a.parts);
         UnitPair<4> p;
         while (ok && p.next(walk)) {
           const int s = rp.s;
@@ -861,7 +861,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (more) next.load_steps(lora.a);
-        UnitWalk<8> walk(rows, lora_part(lora.a, col0, width, N), lora.a.parts, 0, 1);
+        UnitWalk<8> walk(rows, lora_part(lora.a, col0, width, N), lora.a.parts);
         UnitPair<8> p;
         while (ok && p.next(walk)) {
           const int s = rp.s;

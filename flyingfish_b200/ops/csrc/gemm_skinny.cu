@@ -266,6 +266,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   if (threadIdx.x == 0) FF_TL(status, KID_GEMM_SKINNY, 0);
   extern __shared__ uint8_t smem_raw[];
   __shared__ SkinnyBars bars;
+  __shared__ std::conditional_t<LORA, LoraList, NoLora> lists;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // cluster mode: receive buffer [source CTA][owned row][tile_rows + SP_PAD] FP32 for the partials of this CTA's rows
   float* recv = reinterpret_cast<float*>(smem);
@@ -284,6 +285,9 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   const int G = gridDim.x;
   const bool clustered = cl_size > 1;
   const int crank = clustered ? (int)cluster_ctarank() : 0;
+  // adapters: t of a step (high, low) twice behind the ring
+  [[maybe_unused]] uint8_t* t_buf = pipe + stages * stage_bytes;
+  [[maybe_unused]] const int t_bytes = ntok * 32, unit_bytes = tile_rows * 32;
   long long u0, u1;
   if (clustered) {
     const long long base = (long long)(blockIdx.x / cl_size) * kblocks;
@@ -291,6 +295,13 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   } else {
     u0 = total * blockIdx.x / G; u1 = total * (blockIdx.x + 1) / G;
   }
+  // adapters: this CTA's place among those that share the K of a tile
+  [[maybe_unused]] auto share_of = [&](int tile) {
+    if (clustered) return LoraShare{crank, cl_size};
+    const int c_first = unit_owner((long long)tile * kblocks, total, G);
+    return LoraShare{(int)blockIdx.x - c_first, unit_owner((long long)(tile + 1) * kblocks - 1, total, G) - c_first + 1};
+  };
+  [[maybe_unused]] const int first_tile = (int)(u0 / kblocks);
 
   // Thread 0 is the TMA producer. It initialises the barriers and at once requests the first `stages`
   // weight tiles (weights are written by no kernel, so this needs no wait on the preceding kernel),
@@ -301,6 +312,10 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     tma_prefetch_desc(&tmW); tma_prefetch_desc(&tmX);
     for (int i = 0; i < stages; ++i) { mbar_init(&bars.full[i], 1); mbar_init(&bars.empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&bars.tmem_full[i], 1); mbar_init(&bars.tmem_empty[i], 4); }
+    if constexpr (LORA) {
+      mbar_init(&lists.listed, 4);
+      for (int i = 0; i < 2; ++i) { mbar_init(&lists.t_full[i], 1); mbar_init(&lists.t_empty[i], 1); }
+    }
     bars.abort_flag = 0; bars.flag_a = 0; bars.flag_b = 0;
     mbar_fence_init();
     const uint64_t pol_w = l2_policy_evict_first();
@@ -320,112 +335,14 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   volatile int* abort_flag = &bars.abort_flag;
   if (threadIdx.x == 0) FF_TL(status, KID_GEMM_SKINNY, 1);
 
-  if constexpr (LORA) {
-    // As below, by whole warps: behind a segment's K blocks come the units of the adapters (lora.cuh). The kernel in front of this one (lora.cu) lets it
-    // start only once everything before that kernel is done: X and the ids are there, the weights stream while t is computed, and the
-    // wait stands in front of the first t.
-    if (warp < 2) {
-      RowGroups<4> rows;
-      rows.load(lora.a, 0, M, lane, status);
-      uint32_t it = 0, seg_it = 0; RingPos rp; bool ok = true, waited = false;
-      long long u = u0; Segment sg;
-      const uint32_t idesc = umma_idesc(1, 1, 0, 0, STOK, tile_rows);
-      const int t_bytes = ntok * 32, b_bytes = tile_rows * 32;
-      while (ok && next_segment(u, u1, kblocks, sg)) {
-        const int n = sg.kb1 - sg.kb0, acc = seg_it & 1;
-        const uint32_t aph = (seg_it >> 1) & 1, d_tmem = tmem_base + acc * tile_rows;
-        RingPos at = rp;
-        if (warp == 0) {
-          if (elect_one()) {
-            const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-            for (int kb = sg.kb0; kb < sg.kb1; ++kb, at.next(stages)) {
-              const int s = at.s;
-              uint8_t* sa = pipe + s * stage_bytes;
-              if (it + (kb - sg.kb0) >= pre) {
-                if (!mbar_wait(&bars.empty[s], at.ph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 1)) { ok = false; break; }
-                mbar_expect_tx(&bars.full[s], tx_bytes);
-                tma_load_2d_hint(sa + A_BYTES, &tmW, &bars.full[s], kb * SBK, sg.tile * tile_rows, pol_w);
-              }
-              tma_load_2d_hint(sa, &tmX, &bars.full[s], kb * SBK, 0, pol_x);
-            }
-          }
-        } else if (elect_one()) {
-          ok = mbar_wait(&bars.tmem_empty[acc], aph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 2);
-          tc_fence_after();
-          for (int kb = sg.kb0; kb < sg.kb1 && ok; ++kb, at.next(stages)) {
-            const int s = at.s;
-            if (!mbar_wait(&bars.full[s], at.ph, abort_flag, status, KID_GEMM_SKINNY, 3)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t sa = smem_u32(pipe + s * stage_bytes);
-            const uint64_t da = umma_desc_sw128(sa, 16, 1024), db = umma_desc_sw128(sa + A_BYTES, 16, 1024);
-#pragma unroll
-            for (int k = 0; k < SBK / 16; ++k) umma_f16(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.kb0) || k > 0);
-            umma_commit(&bars.empty[s]);
-          }
-        }
-        it += n;
-        rp.skip(n, stages);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        // the units of this CTA's share of the tile
-        int share = crank, shares = clustered ? cl_size : 1;
-        if (!clustered && n < kblocks) {
-          const int c_first = unit_owner((long long)sg.tile * kblocks, total, G);
-          share = blockIdx.x - c_first;
-          shares = unit_owner((long long)(sg.tile + 1) * kblocks - 1, total, G) - c_first + 1;
-        }
-        UnitWalk<4> walk(rows, lora_part(lora.a, sg.tile * tile_rows, tile_rows, N), lora.a.parts, share, shares);
-        UnitPair<4> p;
-        while (ok && p.next(walk)) {
-          const int s = rp.s;
-          if (warp == 0) {
-            if (!waited) { pdl_wait(); waited = true; }
-            if (elect_one()) {
-              ok = it < (uint32_t)stages || mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 1);
-              if (ok) {
-                uint8_t* sa = pipe + s * stage_bytes;
-                mbar_expect_tx(&bars.full[s], p.n * (2 * t_bytes + b_bytes));
-                tma_load_2d(sa, &lora.t, &bars.full[s], p.step0 * 16, 0);
-                tma_load_2d(sa + t_bytes, &lora.t, &bars.full[s], lora.a.R + p.step0 * 16, 0);
-                tma_load_2d(sa + A_BYTES, &lora.b, &bars.full[s], p.step0 * 16, p.adapter0 * N + sg.tile * tile_rows);
-                if (p.n == 2) {
-                  tma_load_2d(sa + 2 * t_bytes, &lora.t, &bars.full[s], p.step1 * 16, 0);
-                  tma_load_2d(sa + 3 * t_bytes, &lora.t, &bars.full[s], lora.a.R + p.step1 * 16, 0);
-                  tma_load_2d(sa + A_BYTES + b_bytes, &lora.b, &bars.full[s], p.step1 * 16, p.adapter1 * N + sg.tile * tile_rows);
-                }
-              }
-            }
-          } else if (elect_one()) {
-            ok = mbar_wait(&bars.full[s], rp.ph, abort_flag, status, KID_GEMM_SKINNY, 3);
-            if (ok) {
-              tc_fence_after();
-              const uint32_t sa = smem_u32(pipe + s * stage_bytes);
-              const uint64_t db0 = umma_desc_sw32(sa + A_BYTES), db1 = umma_desc_sw32(sa + A_BYTES + b_bytes);
-              umma_f16_lanes(d_tmem, umma_desc_sw32(sa), db0, idesc, p.mine0);
-              umma_f16_lanes(d_tmem, umma_desc_sw32(sa + t_bytes), db0, idesc, p.mine0);
-              if (p.n == 2) {
-                umma_f16_lanes(d_tmem, umma_desc_sw32(sa + 2 * t_bytes), db1, idesc, p.mine1);
-                umma_f16_lanes(d_tmem, umma_desc_sw32(sa + 3 * t_bytes), db1, idesc, p.mine1);
-              }
-              umma_commit(&bars.empty[s]);
-            }
-          }
-          ++it;
-          rp.next(stages);
-          ok = __all_sync(0xffffffffu, ok);
-        }
-        if (warp == 1 && ok && elect_one()) umma_commit(&bars.tmem_full[acc]);
-        __syncwarp();
-        ++seg_it;
-      }
-    }
-  }
-  if (!LORA && warp == 0) {
+  if (warp == 0) {
     if (elect_one()) {
       const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      pdl_wait();
+      // With adapters the kernel in front of this one (lora.cu) lets it start only once everything before that kernel is done: X and the ids are there, the
+      // weights stream while t is computed, and the wait stands in front of the first t.
+      if constexpr (!LORA) pdl_wait();
       FF_TL(status, KID_GEMM_SKINNY, 3);
-      uint32_t it = 0; RingPos rp; bool ok = true;
+      uint32_t it = 0, t_it = 0; RingPos rp; bool ok = true, listed = false, waited = false;
       long long u = u0; Segment sg;
       while (ok && next_segment(u, u1, kblocks, sg)) {
         for (int kb = sg.kb0; kb < sg.kb1; ++kb, ++it, rp.next(stages)) {
@@ -438,13 +355,55 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
           }
           tma_load_2d_hint(sa, &tmX, &bars.full[s], kb * SBK, 0, pol_x);
         }
+        if constexpr (LORA) {
+          // units of the adapters (lora.cuh): up to four of one step in a stage, t of the step (high, low) in one of two buffers of its own. The first t waits
+          // for the kernel that writes it, behind as many units as the ring takes.
+          if (!ok) break;
+          if (!listed) ok = listed = mbar_wait(&lists.listed, 0, abort_flag, status, KID_GEMM_SKINNY, 5);
+          const int part = lora_part(lora.a, sg.tile * tile_rows, tile_rows, N), col0 = sg.tile * tile_rows;
+          const uint32_t (*hits)[4] = lists.hits[sg.kb0 == 0 && sg.kb1 == kblocks ? 0 : sg.tile == first_tile ? 1 : 2];
+          const int steps = lists.steps;
+          for (int step = part < 0 ? 0 : part; ok && step < steps; step += part < 0 ? 1 : lora.a.parts) {
+            const uint4 h = *reinterpret_cast<const uint4*>(hits[step]);
+            if ((h.x | h.y | h.z | h.w) == 0) continue;
+            auto load_t = [&]() {
+              if (!waited) { pdl_wait(); waited = true; }
+              const int tb = t_it & 1;
+              if (!mbar_wait(&lists.t_empty[tb], ((t_it >> 1) & 1) ^ 1, abort_flag, status, KID_GEMM_SKINNY, 6)) return false;
+              mbar_expect_tx(&lists.t_full[tb], 2 * t_bytes);
+              tma_load_2d(t_buf + tb * 2 * t_bytes, &lora.t, &lists.t_full[tb], step * 16, 0);
+              tma_load_2d(t_buf + (tb * 2 + 1) * t_bytes, &lora.t, &lists.t_full[tb], lora.a.R + step * 16, 0);
+              ++t_it;
+              return true;
+            };
+            bool t_due = !waited;
+            if (waited && !load_t()) { ok = false; break; }
+            int in_stage = 0;
+            uint32_t left[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              while (left[w] && ok) {
+                const int j = 32 * w + __ffs(left[w]) - 1, s = rp.s;
+                left[w] &= left[w] - 1;
+                if (in_stage == 0) {
+                  if (t_due && !mbar_try_wait(&bars.empty[s], rp.ph ^ 1)) { t_due = false; ok = load_t(); }
+                  if (!ok || !mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 1)) { ok = false; break; }
+                }
+                mbar_expect(&bars.full[s], unit_bytes);
+                tma_load_2d_hint(pipe + s * stage_bytes + A_BYTES + in_stage * unit_bytes, &lora.b, &bars.full[s], step * 16, lists.row[j] + col0, pol_w);
+                if (++in_stage == 4) { mbar_arrive(&bars.full[s]); in_stage = 0; ++it; rp.next(stages); }
+              }
+            if (ok && in_stage) { mbar_arrive(&bars.full[rp.s]); ++it; rp.next(stages); }
+            if (ok && t_due) ok = load_t();
+          }
+        }
       }
       FF_TL(status, KID_GEMM_SKINNY, 4);
     }
-  } else if (!LORA && warp == 1) {
+  } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = umma_idesc(1, 1, 0, 0, STOK, tile_rows);
-      uint32_t it = 0, seg_it = 0; RingPos rp; bool ok = true;
+      uint32_t it = 0, seg_it = 0, t_it = 0; RingPos rp; bool ok = true, listed = false;
       long long u = u0; Segment sg;
       while (ok && next_segment(u, u1, kblocks, sg)) {
         const int acc = seg_it & 1; const uint32_t aph = (seg_it >> 1) & 1;
@@ -463,18 +422,55 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
           for (int k = 0; k < SBK / 16; ++k) umma_f16(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.kb0) || k > 0);
           umma_commit(&bars.empty[s]);
         }
+        if constexpr (LORA) {
+          if (!ok) break;
+          if (!listed) ok = listed = mbar_wait(&lists.listed, 0, abort_flag, status, KID_GEMM_SKINNY, 5);
+          const int part = lora_part(lora.a, sg.tile * tile_rows, tile_rows, N);
+          const uint32_t (*hits)[4] = lists.hits[sg.kb0 == 0 && sg.kb1 == kblocks ? 0 : sg.tile == first_tile ? 1 : 2];
+          const int steps = lists.steps;
+          for (int step = part < 0 ? 0 : part; ok && step < steps; step += part < 0 ? 1 : lora.a.parts) {
+            const uint4 h = *reinterpret_cast<const uint4*>(hits[step]);
+            if ((h.x | h.y | h.z | h.w) == 0) continue;
+            const int tb = t_it & 1;
+            if (!mbar_wait(&lists.t_full[tb], (t_it >> 1) & 1, abort_flag, status, KID_GEMM_SKINNY, 7)) { ok = false; break; }
+            const uint32_t st = smem_u32(t_buf + tb * 2 * t_bytes);
+            const uint64_t dh = umma_desc_sw32(st), dl = umma_desc_sw32(st + t_bytes);
+            int in_stage = 0;
+            uint32_t left[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              while (left[w] && ok) {
+                const int j = 32 * w + __ffs(left[w]) - 1, s = rp.s;
+                left[w] &= left[w] - 1;
+                const uint4 m = *reinterpret_cast<const uint4*>(lists.mine[j]);
+                if (in_stage == 0) {
+                  ok = mbar_wait(&bars.full[s], rp.ph, abort_flag, status, KID_GEMM_SKINNY, 3);
+                  tc_fence_after();
+                  if (!ok) break;
+                }
+                const uint32_t mine[4] = {m.x, m.y, m.z, m.w};
+                const uint64_t db = umma_desc_sw32(smem_u32(pipe + s * stage_bytes + A_BYTES + in_stage * unit_bytes));
+                umma_f16_lanes(d_tmem, dh, db, idesc, mine);
+                umma_f16_lanes(d_tmem, dl, db, idesc, mine);
+                if (++in_stage == 4) { umma_commit(&bars.empty[s]); in_stage = 0; rp.next(stages); }
+              }
+            if (ok && in_stage) { umma_commit(&bars.empty[rp.s]); rp.next(stages); }
+            if (ok) { umma_commit(&lists.t_empty[tb]); ++t_it; }
+          }
+        }
         if (ok) umma_commit(&bars.tmem_full[acc]);
         ++seg_it;
       }
       FF_TL(status, KID_GEMM_SKINNY, 6);
     }
-  } else if (warp >= 2) {
+  } else {
     // ---- epilogue warps 2..5 ; TMEM lane quarter = warp % 4 ; lane = token ----------------------
     const int q = warp & 3;
     const int t_own = q * 32 + lane;              // token row held by this thread's TMEM lane
     const bool row_live = q * 32 < M;             // warp-uniform: this quarter holds real tokens
     const int e = (warp - 2) * 32 + lane;         // 0..127, cooperative index
     const int vpr = tile_rows / 8;                // 8-value vectors per tile row
+    if constexpr (LORA) lora_list(lists, lora.a, M, N, e, share_of(first_tile), share_of((int)((u1 - 1) / kblocks)), status);
     pdl_wait();                                   // scratch, counters, the arena and Y belong to earlier kernels until here
     if (e == 0) FF_TL(status, KID_GEMM_SKINNY, 7);
     int ar_epoch = 0;
@@ -999,9 +995,12 @@ static int gemm_skinny_launch(const void* X, const void* W, void* Y, int M, int 
     LoraDev dev = {};
     dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts};
     if (int e = lora_maps(dev, lora->t, lora->b, M, N, ntok, cfg.tile_rows, cfg.tile_rows)) return e;
+    // behind the ring: t of two steps (the instruction reads 128 rows of each word)
+    const int ring = cfg.pipe_off + cfg.stages * (ntok + cfg.tile_rows) * SBK * 2 + 1024, t_room = 3 * ntok * 32 + STOK * 32;
+    const int with_t = ring + t_room > smem ? ring + t_room : smem;
     auto kern = gemm_skinny_kernel<false, true>;
-    r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
-    return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
+    r = opt_in_smem(kern, SK_SMEM_FULL + 1024 + STOK * 128); if (r) return r;
+    return launch_pdl(kern, dim3(grid), dim3(192), with_t, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
                       cfg.stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail, dev);
   }
   if (arena == nullptr) {

@@ -55,9 +55,9 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     mbar_fence_init();
   }
   pdl_wait();
-  // Tensor memory behind the wait, as in gemm_bf16.cu: what is taken here is not in the way of a kernel that still has to take its own. The kernel behind this
-  // one may start once every CTA is past this point.
-  if (warp == 1) { tmem_alloc(&sh.tmem_base, tmem_cols); tmem_relinquish(); }
+  // Tensor memory behind the wait, as in gemm_bf16.cu: what is taken here is not in the way of a kernel that still has to take its own. With it in hand the
+  // kernel behind this one may start: it finds X and the ids done, takes its own and streams its weights meanwhile.
+  if (warp == 1) { tmem_alloc(&sh.tmem_base, tmem_cols); tmem_relinquish(); pdl_trigger(); }
   if (warp >= 2) {
     // distinct adapters of the tile and where their units lie in the tile's list, in the order of their first rows
     const int e = threadIdx.x - 64;
@@ -95,7 +95,6 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_trigger();
   const uint32_t tmem_base = sh.tmem_base;
   volatile int* abort_flag = &sh.abort_flag;
   const int units = sh.units;

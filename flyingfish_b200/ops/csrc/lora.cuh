@@ -4,8 +4,8 @@
 // A unit (adapter a, step s) is t[:, 16 s .. 16 s + 15] B_a[:, 16 s .. 16 s + 15]^T, accumulated behind the product's own K blocks into the same
 // FP32 sums, for the rows of the adapter only: a row of the tile is a lane of tensor memory, and the instruction's mask of lanes leaves the others' sums
 // alone, whatever t and B hold. So a tile takes any mix of adapters, a row without one gets the bits of the product alone, and what an adapter
-// holds (infinities included) reaches its own rows only. t is two BF16 words per value (high, low), so a unit is two instructions. Two units
-// share a stage of the ring: [high 0 | low 0 | high 1 | low 1] of t in the place of X, [B 0 | B 1] in the place of W, 32-byte swizzle.
+// holds (infinities included) reaches its own rows only. t is two BF16 words per value (high, low), so a unit is two instructions. Operands of 16
+// columns, 32-byte swizzle.
 #pragma once
 #include "ptx.cuh"
 #include "host_util.h"
@@ -59,19 +59,16 @@ struct RowGroups {
 };
 
 // Units of a tile in turn: adapters in the order of their first rows, their steps ascending. part >= 0: the tile's columns lie in that part of a fused
-// projection and see every parts-th step only. Of the `shares` CTAs that divide a tile's K, number `share` takes the units whose adapter + step leaves
-// that remainder: where a row's units go depends on nothing but its adapter.
+// projection and see every parts-th step only.
 template <int H>
 struct UnitWalk {
   RowGroups<H> rg;
   uint32_t mine[H];
-  int adapter, step = 0, steps = 0, first, by, share, shares;
-  __device__ __forceinline__ UnitWalk(const RowGroups<H>& all, int part, int parts, int share_, int shares_)
-      : rg(all), first(part < 0 ? 0 : part), by(part < 0 ? 1 : parts), share(share_), shares(shares_) {}
+  int adapter, step = 0, steps = 0, first, by;
+  __device__ __forceinline__ UnitWalk(const RowGroups<H>& all, int part, int parts) : rg(all), first(part < 0 ? 0 : part), by(part < 0 ? 1 : parts) {}
   __device__ __forceinline__ bool next() {
     while (true) {
-      for (; step < steps; step += by)
-        if (shares == 1 || (unsigned)(adapter + step) % (unsigned)shares == (unsigned)share) return true;
+      if (step < steps) return true;
       adapter = -1;
 #pragma unroll
       for (int h = 0; h < H; ++h)
@@ -88,7 +85,7 @@ struct UnitWalk {
   }
 };
 
-// One or two units of a stage.
+// One or two units of a stage: [high 0 | low 0 | high 1 | low 1] of t in the place of X, [B 0 | B 1] in the place of W.
 template <int H>
 struct UnitPair {
   int n, adapter0, step0, adapter1, step1;
@@ -107,6 +104,72 @@ struct UnitPair {
     return true;
   }
 };
+
+// Decode products: one tile of up to 128 rows, whose adapters are listed once per CTA in shared memory by the epilogue's 128 threads while the weights stream.
+// Units go step by step, so that t of a step is loaded once for all adapters; up to four of a step's units share a stage of the ring. The threads that
+// load and multiply walk lists of bits: one thread alone takes hundreds of cycles to find a unit among the adapters, a few to take the next bit
+// (64 rows with 64 adapters of rank 16, 6144 x 4096: 51 us with the search, LORA_AFTER with the bits).
+//
+// Where a tile's K is divided among CTAs, a hash of the adapter and the step say whose a unit is: where a row's units go, and with it the order of its
+// sums, depends on nothing but its adapter.
+constexpr int LORA_LIST = 128, LORA_STEPS = 64;
+struct LoraShare { int share, shares; };
+struct LoraList {
+  alignas(16) int id[LORA_LIST];
+  alignas(16) uint32_t mine[LORA_LIST][4];             // rows of the n-th adapter
+  alignas(16) uint32_t hits[3][LORA_STEPS][4];         // adapters with a unit of this step: of the whole tile, of this CTA's first and last share of a tile
+  int row[LORA_LIST];                                  // first row of the n-th adapter in the stacked B
+  int hash[LORA_LIST], most[LORA_LIST], index[LORA_LIST], warp_count[4], warp_steps[4];
+  int count, steps;                                    // adapters, most steps of one
+  alignas(8) uint64_t listed, t_full[2], t_empty[2];
+};
+
+// 128 threads, e = 0 .. 127; `listed` (4 arrivals) says that it is done.
+__device__ __forceinline__ void lora_list(LoraList& l, const LoraArgs& a, int M, int N, int e, LoraShare first_share, LoraShare last_share, int* status) {
+  const int warp = e >> 5, lane = e & 31;
+  int id = e < M ? a.ids[e] : -1;
+  if (id >= a.adapters) { if (blockIdx.x == 0) set_status(status, KID_LORA, FF_ERR_BOUNDS, e, id); id = -1; }
+  const int steps = id >= 0 ? lora_steps(a, id) : 0;
+  if (steps == 0) id = -1;
+  l.id[e] = id;
+  *reinterpret_cast<uint4*>(l.mine[e]) = make_uint4(0, 0, 0, 0);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  int first = e;
+  if (id >= 0)
+    for (int j = 0; j < first; j += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(&l.id[j]);
+      if (v.w == id) first = min(first, j + 3);
+      if (v.z == id) first = min(first, j + 2);
+      if (v.y == id) first = min(first, j + 1);
+      if (v.x == id) first = min(first, j);
+    }
+  const bool leads = id >= 0 && first == e;
+  const uint32_t vote = __ballot_sync(0xffffffffu, leads);
+  const int most = (int)__reduce_max_sync(0xffffffffu, (unsigned)steps);
+  if (lane == 0) { l.warp_count[warp] = __popc(vote); l.warp_steps[warp] = most; }
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  int at = __popc(vote & ((1u << lane) - 1));
+  for (int w = 0; w < warp; ++w) at += l.warp_count[w];
+  const int count = l.warp_count[0] + l.warp_count[1] + l.warp_count[2] + l.warp_count[3];
+  const int all_steps = max(max(l.warp_steps[0], l.warp_steps[1]), max(l.warp_steps[2], l.warp_steps[3]));
+  if (leads) { l.row[at] = id * N; l.hash[at] = (int)(((unsigned)id * 40503u) & 0xffffu); l.most[at] = steps; l.index[e] = at; }
+  if (e == 0) { l.count = count; l.steps = all_steps; }
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  const uint32_t same = __match_any_sync(0xffffffffu, id);
+  if (id >= 0 && lane == __ffs(same) - 1) l.mine[l.index[first]][warp] = same;
+  // thread e: the e-th adapter
+  const int mine = e < count ? l.most[e] : 0, hash = e < count ? l.hash[e] : 0;
+  int r0 = hash * first_share.shares >> 16, r1 = hash * last_share.shares >> 16;
+  for (int s = 0; s < all_steps; ++s) {
+    const uint32_t whole = __ballot_sync(0xffffffffu, s < mine);
+    const uint32_t one = __ballot_sync(0xffffffffu, s < mine && r0 == first_share.share), two = __ballot_sync(0xffffffffu, s < mine && r1 == last_share.share);
+    if (lane == 0) { l.hits[0][s][warp] = whole; l.hits[1][s][warp] = one; l.hits[2][s][warp] = two; }
+    if (++r0 == first_share.shares) r0 = 0;
+    if (++r1 == last_share.shares) r1 = 0;
+  }
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&l.listed);
+}
 
 // the part that all of the columns [col0, col0 + width) lie in, or -1
 __device__ __forceinline__ int lora_part(const LoraArgs& a, int col0, int width, int N) {
