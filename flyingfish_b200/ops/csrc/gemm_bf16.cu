@@ -363,11 +363,11 @@ __device__ __forceinline__ void store_tile_row(uint32_t taddr, void* __restrict_
   }
 }
 
-template <int BN, int STAGES, int COMM, bool LORA = false>
+template <int BN, int STAGES, int COMM, int BW = 0>
 __global__ void __launch_bounds__(COMM == 2 ? 192 : 320, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1,
                  const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmB, void* __restrict__ Cout, int M, int N, int K, int ldc, int epi,
-                 int* status, CommArgs ca, GroupArgs ga, LinTail tail, const __grid_constant__ std::conditional_t<LORA, LoraDev, NoLora> lora) {
+                 int* status, CommArgs ca, GroupArgs ga, LinTail tail, const __grid_constant__ std::conditional_t<BW != 0, LoraDev, NoLora> lora) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PipeBars bars;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -396,11 +396,11 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const uint32_t tmem_base = bars.tmem_base;
   volatile int* abort_flag = &bars.abort_flag;
 
-  if constexpr (LORA) {
+  if constexpr (BW != 0) {
     // dense problems only, by whole warps: as below, with the units of the adapters (lora.cuh) behind a tile's K blocks
     if (warp < 2) {
       constexpr uint32_t idesc = umma_idesc(1, 1, 0, 0, BM, BN);
-      constexpr int T_BYTES = BM * 32, UNIT_BYTES = 2 * T_BYTES + BN * 32;
+      constexpr int T_BYTES = BM * BW * 2, B_UNIT = BN * BW * 2, UNIT_BYTES = 2 * T_BYTES + B_UNIT;
       const int tiles = tiles_m * tiles_n;
       RowGroups<4> rows, next;
       RingPos rp;
@@ -447,7 +447,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (more) next.load_steps(lora.a);
         UnitWalk<4> walk(rows, lora_part(lora.a, tn * BN, BN, N), lora.a.parts);
         UnitPair<4> p;
-        while (ok && p.next(walk)) {
+        while (ok && p.next(walk, BW == 16)) {
           const int s = rp.s;
           uint8_t* sa = smem + s * STAGE_BYTES;
           if (warp == 0) {
@@ -455,13 +455,13 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               ok = mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_BF16, 1);
               if (ok) {
                 mbar_expect_tx(&bars.full[s], p.n * UNIT_BYTES);
-                tma_load_2d(sa, &lora.t, &bars.full[s], p.step0 * 16, tm * BM);
-                tma_load_2d(sa + T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step0 * 16, tm * BM);
-                tma_load_2d(sa + A_BYTES, &lora.b, &bars.full[s], p.step0 * 16, p.adapter0 * N + tn * BN);
+                tma_load_2d(sa, &lora.t, &bars.full[s], p.step0 * BW, tm * BM);
+                tma_load_2d(sa + T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step0 * BW, tm * BM);
+                tma_load_2d(sa + A_BYTES, &lora.b, &bars.full[s], p.step0 * BW, p.adapter0 * N + tn * BN);
                 if (p.n == 2) {
-                  tma_load_2d(sa + 2 * T_BYTES, &lora.t, &bars.full[s], p.step1 * 16, tm * BM);
-                  tma_load_2d(sa + 3 * T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step1 * 16, tm * BM);
-                  tma_load_2d(sa + A_BYTES + BN * 32, &lora.b, &bars.full[s], p.step1 * 16, p.adapter1 * N + tn * BN);
+                  tma_load_2d(sa + 2 * T_BYTES, &lora.t, &bars.full[s], p.step1 * BW, tm * BM);
+                  tma_load_2d(sa + 3 * T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step1 * BW, tm * BM);
+                  tma_load_2d(sa + A_BYTES + B_UNIT, &lora.b, &bars.full[s], p.step1 * BW, p.adapter1 * N + tn * BN);
                 }
               }
             }
@@ -470,13 +470,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (ok) {
               tc_fence_after();
               const uint32_t a0 = smem_u32(sa);
-              const uint64_t db0 = umma_desc_sw32(a0 + A_BYTES), db1 = umma_desc_sw32(a0 + A_BYTES + BN * 32);
-              umma_f16_lanes(d_tmem, umma_desc_sw32(a0), db0, idesc, p.mine0);
-              umma_f16_lanes(d_tmem, umma_desc_sw32(a0 + T_BYTES), db0, idesc, p.mine0);
-              if (p.n == 2) {
-                umma_f16_lanes(d_tmem, umma_desc_sw32(a0 + 2 * T_BYTES), db1, idesc, p.mine1);
-                umma_f16_lanes(d_tmem, umma_desc_sw32(a0 + 3 * T_BYTES), db1, idesc, p.mine1);
-              }
+              umma_unit<BW>(d_tmem, a0, a0 + T_BYTES, a0 + A_BYTES, idesc, p.mine0);
+              if (p.n == 2) umma_unit<BW>(d_tmem, a0 + 2 * T_BYTES, a0 + 3 * T_BYTES, a0 + A_BYTES + B_UNIT, idesc, p.mine1);
               umma_commit(&bars.empty[s]);
             }
           }
@@ -489,7 +484,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     }
   }
-  if (!LORA && warp == 0) {
+  if (BW == 0 && warp == 0) {
     if (elect_one()) {
       tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB);
       uint32_t it = 0;
@@ -519,7 +514,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
     }
-  } else if (!LORA && warp == 1) {
+  } else if (BW == 0 && warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc = umma_idesc(1, 1, 0, 0, BM, BN);
       uint32_t it = 0, tile_it = 0;
@@ -772,11 +767,11 @@ __device__ __forceinline__ void pair_tile(const PairTiles& pt, int t, int tiles_
   else { tile_coords(t - n1, tiles_m, tiles_n2, tm, tn); col0 = pt.wide * pt.w1 + tn * pt.w2; width = pt.w2; }
 }
 
-template <int PARTS, bool LORA>
+template <int PARTS, int BW>
 __global__ void __launch_bounds__(64 + 128 * PARTS, 1)
 gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmB2,
                       void* __restrict__ Cout, int M, int N, int K, int ldc, int epi, const PairTiles pt, int stages, int* status, LinTail tail,
-                      const __grid_constant__ std::conditional_t<LORA, LoraDev, NoLora> lora) {
+                      const __grid_constant__ std::conditional_t<BW != 0, LoraDev, NoLora> lora) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ PairBars bars;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -797,7 +792,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   }
   // With adapters the kernel in front (lora.cu) lets this one start only when it has its tensor memory and everything before it is done: X and the ids are
   // there, and the wait stands in front of the first t.
-  if constexpr (!LORA) pdl_wait();
+  if constexpr (BW == 0) pdl_wait();
   // after the wait: no kernel of this stream that still has tensor memory to allocate can be running. All 512 columns, so that both
   // CTAs' accumulators have the same addresses.
   if (warp == 1) { tmem_alloc_pair(&bars.tmem_base, 512); tmem_relinquish_pair(); }
@@ -809,10 +804,10 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const uint32_t tmem_base = bars.tmem_base;
   volatile int* abort_flag = &bars.abort_flag;
 
-  if constexpr (LORA) {
+  if constexpr (BW != 0) {
     // by whole warps: as below, with the units of the adapters (lora.cuh) behind a tile's K blocks
     if (warp < 2) {
-      constexpr int T_BYTES = BM * 32;
+      constexpr int T_BYTES = BM * BW * 2;
       const uint32_t idesc1 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w1), idesc2 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w2);
       RowGroups<8> rows, next;
       RingPos rp;
@@ -863,7 +858,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (more) next.load_steps(lora.a);
         UnitWalk<8> walk(rows, lora_part(lora.a, col0, width, N), lora.a.parts);
         UnitPair<8> p;
-        while (ok && p.next(walk)) {
+        while (ok && p.next(walk, BW == 16)) {
           const int s = rp.s;
           uint8_t* sa = smem + s * stage_bytes;
           if (warp == 0) {
@@ -871,14 +866,14 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             if (elect_one()) {
               ok = mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_BF16, 5);
               if (ok) {
-                if (rank == 0) mbar_expect_tx(&bars.full[s], p.n * (4 * T_BYTES + width * 32));
-                tma_load_2d_pair(sa, &lora.t, &bars.full[s], p.step0 * 16, row);
-                tma_load_2d_pair(sa + T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step0 * 16, row);
-                tma_load_2d_pair(sa + A_BYTES, tmU, &bars.full[s], p.step0 * 16, p.adapter0 * N + col0 + rank * half);
+                if (rank == 0) mbar_expect_tx(&bars.full[s], p.n * (4 * T_BYTES + width * BW * 2));
+                tma_load_2d_pair(sa, &lora.t, &bars.full[s], p.step0 * BW, row);
+                tma_load_2d_pair(sa + T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step0 * BW, row);
+                tma_load_2d_pair(sa + A_BYTES, tmU, &bars.full[s], p.step0 * BW, p.adapter0 * N + col0 + rank * half);
                 if (p.n == 2) {
-                  tma_load_2d_pair(sa + 2 * T_BYTES, &lora.t, &bars.full[s], p.step1 * 16, row);
-                  tma_load_2d_pair(sa + 3 * T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step1 * 16, row);
-                  tma_load_2d_pair(sa + A_BYTES + half * 32, tmU, &bars.full[s], p.step1 * 16, p.adapter1 * N + col0 + rank * half);
+                  tma_load_2d_pair(sa + 2 * T_BYTES, &lora.t, &bars.full[s], p.step1 * BW, row);
+                  tma_load_2d_pair(sa + 3 * T_BYTES, &lora.t, &bars.full[s], lora.a.R + p.step1 * BW, row);
+                  tma_load_2d_pair(sa + A_BYTES + half * BW * 2, tmU, &bars.full[s], p.step1 * BW, p.adapter1 * N + col0 + rank * half);
                 }
               }
             }
@@ -887,13 +882,8 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             if (ok) {
               tc_fence_after();
               const uint32_t a0 = smem_u32(sa);
-              const uint64_t db0 = umma_desc_sw32(a0 + A_BYTES), db1 = umma_desc_sw32(a0 + A_BYTES + half * 32);
-              umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0), db0, idesc, p.mine0);
-              umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0 + T_BYTES), db0, idesc, p.mine0);
-              if (p.n == 2) {
-                umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0 + 2 * T_BYTES), db1, idesc, p.mine1);
-                umma_f16_pair_lanes(d_tmem, umma_desc_sw32(a0 + 3 * T_BYTES), db1, idesc, p.mine1);
-              }
+              umma_unit_pair<BW>(d_tmem, a0, a0 + T_BYTES, a0 + A_BYTES, idesc, p.mine0);
+              if (p.n == 2) umma_unit_pair<BW>(d_tmem, a0 + 2 * T_BYTES, a0 + 3 * T_BYTES, a0 + A_BYTES + half * BW * 2, idesc, p.mine1);
               umma_commit_pair(&bars.empty[s]);
             }
           }
@@ -911,7 +901,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           ok = mbar_wait(&bars.empty[i % stages], (i / stages) & 1, abort_flag, status, KID_GEMM_BF16, 9);
     }
   }
-  if (!LORA && warp == 0) {
+  if (BW == 0 && warp == 0) {
     if (elect_one()) {
       uint32_t it = 0;
       RingPos rp;
@@ -935,7 +925,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (uint32_t i = it > (uint32_t)stages ? it - stages : 0; i < it && ok; ++i)
         ok = mbar_wait(&bars.empty[i % stages], (i / stages) & 1, abort_flag, status, KID_GEMM_BF16, 9);
     }
-  } else if (!LORA && warp == 1) {
+  } else if (BW == 0 && warp == 1) {
     if (rank == 0 && elect_one()) {
       const uint32_t idesc1 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w1), idesc2 = umma_idesc(1, 1, 0, 0, 2 * BM, pt.w2);
       uint32_t tile_it = 0;
@@ -1080,11 +1070,11 @@ static int pair_launch(const CUtensorMap& tmA, const void* W, void* Y, int M, in
   const bool stores = (epi == 0 || epi == 2) && tail.bias == nullptr && tail.act == 0 && tail.mul == nullptr;
   if (lora != nullptr) {
     if (int e = lora_maps(*dev, lora->t, lora->b, M, N, BM, pt.w1 / 2, pt.w2 / 2)) return e;
-    auto kern = stores ? gemm_bf16_pair_kernel<1, true> : gemm_bf16_pair_kernel<2, true>;
+    auto kern = lora->bw == 32 ? (stores ? gemm_bf16_pair_kernel<1, 32> : gemm_bf16_pair_kernel<2, 32>) : (stores ? gemm_bf16_pair_kernel<1, 16> : gemm_bf16_pair_kernel<2, 16>);
     if (int e = opt_in_smem(kern, SMEM)) return e;
     return launch_pdl(kern, dim3(grid), dim3(stores ? 192 : 320), SMEM, stream, 2, tmA, tmB1, tmB2, Y, M, N, K, ldy, epi, pt, stages, status, tail, *dev);
   }
-  auto kern = stores ? gemm_bf16_pair_kernel<1, false> : gemm_bf16_pair_kernel<2, false>;
+  auto kern = stores ? gemm_bf16_pair_kernel<1, 0> : gemm_bf16_pair_kernel<2, 0>;
   if (int e = opt_in_smem(kern, SMEM)) return e;
   if (int e = launch_pdl(kern, dim3(grid), dim3(stores ? 192 : 320), SMEM, stream, 2, tmA, tmB1, tmB2, Y, M, N, K, ldy, epi, pt, stages, status, tail, NoLora{})) return e;
   return launch_result();
@@ -1104,7 +1094,7 @@ static int gemm_bf16_launch(const void* X, const void* W, void* Y, int M, int N,
   CUtensorMap tmA;
   if (int e = make_tmap_2d(&tmA, X, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, K, M, (uint64_t)ldx * 2, BK, BM)) return e;
   LoraDev dev = {};
-  if (lora != nullptr) dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts};
+  if (lora != nullptr) dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts, lora->bw};
   PairTiles pt;
   float waves;
   if (one_cta_tiles(M, N, K, epi, tail.gate != 0, pt, waves)) {
@@ -1115,7 +1105,7 @@ static int gemm_bf16_launch(const void* X, const void* W, void* Y, int M, int N,
     const int grid = tiles < sm_count() ? tiles : sm_count();
     if (lora != nullptr) {
       if (int e = lora_maps(dev, lora->t, lora->b, M, N, BM, BN, BN)) return e;
-      auto kern = gemm_bf16_kernel<BN, STAGES, 0, true>;
+      auto kern = lora->bw == 32 ? gemm_bf16_kernel<BN, STAGES, 0, 32> : gemm_bf16_kernel<BN, STAGES, 0, 16>;
       if (int e = opt_in_smem(kern, smem)) return e;
       kern<<<grid, 320, smem, stream>>>(tmA, tmA, tmA, tmB, Y, M, N, K, ldy, epi, status, CommArgs{}, GroupArgs{}, tail, dev);
       return launch_result();

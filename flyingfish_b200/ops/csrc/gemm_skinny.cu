@@ -255,18 +255,18 @@ __device__ __forceinline__ void allreduce_tile(const TileSink<true>& sink, int M
 
 // cl_size == 1: persistent stream-K over gridDim.x CTAs.  cl_size > 1: cluster split-K, cluster c
 // owns weight tile c, CTA r of it the k-blocks [kblocks*r/S, kblocks*(r+1)/S).
-template <bool FUSE_AR, bool LORA>
+template <bool FUSE_AR, int BW>
 __global__ void __launch_bounds__(192, 2)
 gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                    __nv_bfloat16* __restrict__ Y, int M, int N, int K, int ldy, int ntok, int tile_rows, int stages,
                    int cl_size, int pipe_off, float* __restrict__ scratch, int* __restrict__ counters, int* status,
-                   PeerArena ar, SkinnyEpi ep, const SkinnyTail tail, const __grid_constant__ std::conditional_t<LORA, LoraDev, NoLora> lora) {
+                   PeerArena ar, SkinnyEpi ep, const SkinnyTail tail, const __grid_constant__ std::conditional_t<BW != 0, LoraDev, NoLora> lora) {
   pdl_trigger();
   if (cl_size > 1) cluster_arrive_relaxed();         // phase A: "this CTA runs" (waited on before the first remote store)
   if (threadIdx.x == 0) FF_TL(status, KID_GEMM_SKINNY, 0);
   extern __shared__ uint8_t smem_raw[];
   __shared__ SkinnyBars bars;
-  __shared__ std::conditional_t<LORA, LoraList, NoLora> lists;
+  __shared__ std::conditional_t<BW != 0, LoraList, NoLora> lists;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // cluster mode: receive buffer [source CTA][owned row][tile_rows + SP_PAD] FP32 for the partials of this CTA's rows
   float* recv = reinterpret_cast<float*>(smem);
@@ -287,7 +287,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   const int crank = clustered ? (int)cluster_ctarank() : 0;
   // adapters: t of a step (high, low) twice behind the ring
   [[maybe_unused]] uint8_t* t_buf = pipe + stages * stage_bytes;
-  [[maybe_unused]] const int t_bytes = ntok * 32, unit_bytes = tile_rows * 32;
+  [[maybe_unused]] const int t_bytes = ntok * BW * 2, unit_bytes = tile_rows * BW * 2;
   long long u0, u1;
   if (clustered) {
     const long long base = (long long)(blockIdx.x / cl_size) * kblocks;
@@ -307,12 +307,12 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   // weight tiles (weights are written by no kernel, so this needs no wait on the preceding kernel),
   // while warp 1 allocates TMEM; the other roles meet it at the block barrier.
   // With adapters the stages of their units stand behind a segment's, so no more than the first segment's weights come early.
-  const uint32_t pre = (uint32_t)min((long long)stages, LORA ? min(u1 - u0, (long long)(kblocks - (int)(u0 % kblocks))) : u1 - u0);
+  const uint32_t pre = (uint32_t)min((long long)stages, BW != 0 ? min(u1 - u0, (long long)(kblocks - (int)(u0 % kblocks))) : u1 - u0);
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmW); tma_prefetch_desc(&tmX);
     for (int i = 0; i < stages; ++i) { mbar_init(&bars.full[i], 1); mbar_init(&bars.empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&bars.tmem_full[i], 1); mbar_init(&bars.tmem_empty[i], 4); }
-    if constexpr (LORA) {
+    if constexpr (BW != 0) {
       mbar_init(&lists.listed, 4);
       for (int i = 0; i < 2; ++i) { mbar_init(&lists.t_full[i], 1); mbar_init(&lists.t_empty[i], 1); }
     }
@@ -340,7 +340,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
       // With adapters the kernel in front of this one (lora.cu) lets it start only once everything before that kernel is done: X and the ids are there, the
       // weights stream while t is computed, and the wait stands in front of the first t.
-      if constexpr (!LORA) pdl_wait();
+      if constexpr (BW == 0) pdl_wait();
       FF_TL(status, KID_GEMM_SKINNY, 3);
       uint32_t it = 0, t_it = 0; RingPos rp; bool ok = true, listed = false, waited = false;
       long long u = u0; Segment sg;
@@ -355,45 +355,49 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
           }
           tma_load_2d_hint(sa, &tmX, &bars.full[s], kb * SBK, 0, pol_x);
         }
-        if constexpr (LORA) {
-          // units of the adapters (lora.cuh): up to four of one step in a stage, t of the step (high, low) in one of two buffers of its own. The first t waits
-          // for the kernel that writes it, behind as many units as the ring takes.
+        if constexpr (BW != 0) {
+          // units of the adapters (lora.cuh), t of a step (high, low) in one of two buffers of its own. The first t waits for the kernel that writes it, behind as
+          // many units as the ring takes.
           if (!ok) break;
           if (!listed) ok = listed = mbar_wait(&lists.listed, 0, abort_flag, status, KID_GEMM_SKINNY, 5);
+          constexpr int UNITS = 64 / BW;
           const int part = lora_part(lora.a, sg.tile * tile_rows, tile_rows, N), col0 = sg.tile * tile_rows;
           const uint32_t (*hits)[4] = lists.hits[sg.kb0 == 0 && sg.kb1 == kblocks ? 0 : sg.tile == first_tile ? 1 : 2];
           const int steps = lists.steps;
           for (int step = part < 0 ? 0 : part; ok && step < steps; step += part < 0 ? 1 : lora.a.parts) {
             const uint4 h = *reinterpret_cast<const uint4*>(hits[step]);
             if ((h.x | h.y | h.z | h.w) == 0) continue;
+            // one buffer per step where there are two steps at most: t stays for the tiles to come
+            const int tb = steps <= 2 ? step : t_it & 1;
+            bool t_due = steps > 2 || !(t_it >> tb & 1);
             auto load_t = [&]() {
+              t_due = false;
               if (!waited) { pdl_wait(); waited = true; }
-              const int tb = t_it & 1;
-              if (!mbar_wait(&lists.t_empty[tb], ((t_it >> 1) & 1) ^ 1, abort_flag, status, KID_GEMM_SKINNY, 6)) return false;
+              if (steps > 2 && !mbar_wait(&lists.t_empty[tb], ((t_it >> 1) & 1) ^ 1, abort_flag, status, KID_GEMM_SKINNY, 6)) return false;
               mbar_expect_tx(&lists.t_full[tb], 2 * t_bytes);
-              tma_load_2d(t_buf + tb * 2 * t_bytes, &lora.t, &lists.t_full[tb], step * 16, 0);
-              tma_load_2d(t_buf + (tb * 2 + 1) * t_bytes, &lora.t, &lists.t_full[tb], lora.a.R + step * 16, 0);
-              ++t_it;
+              tma_load_2d(t_buf + tb * 2 * t_bytes, &lora.t, &lists.t_full[tb], step * BW, 0);
+              tma_load_2d(t_buf + (tb * 2 + 1) * t_bytes, &lora.t, &lists.t_full[tb], lora.a.R + step * BW, 0);
+              if (steps > 2) ++t_it; else t_it |= 1u << tb;
               return true;
             };
-            bool t_due = !waited;
-            if (waited && !load_t()) { ok = false; break; }
-            int in_stage = 0;
-            uint32_t left[4] = {h.x, h.y, h.z, h.w};
+            if (waited && t_due && !load_t()) { ok = false; break; }
+            for (int w = 0; w < 4 && ok; ++w) {
+              uint32_t left = hits[step][w];
+              while (left) {
+                const int n = min(UNITS, __popc(left)), s = rp.s;
+                int y[UNITS];
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              while (left[w] && ok) {
-                const int j = 32 * w + __ffs(left[w]) - 1, s = rp.s;
-                left[w] &= left[w] - 1;
-                if (in_stage == 0) {
-                  if (t_due && !mbar_try_wait(&bars.empty[s], rp.ph ^ 1)) { t_due = false; ok = load_t(); }
-                  if (!ok || !mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 1)) { ok = false; break; }
-                }
-                mbar_expect(&bars.full[s], unit_bytes);
-                tma_load_2d_hint(pipe + s * stage_bytes + A_BYTES + in_stage * unit_bytes, &lora.b, &bars.full[s], step * 16, lists.row[j] + col0, pol_w);
-                if (++in_stage == 4) { mbar_arrive(&bars.full[s]); in_stage = 0; ++it; rp.next(stages); }
+                for (int i = 0; i < UNITS; ++i) { y[i] = i < n ? lists.row[32 * w + __ffs(left) - 1] : 0; left &= left - 1; }
+                if (t_due && !mbar_try_wait(&bars.empty[s], rp.ph ^ 1)) ok = load_t();
+                if (!ok || !mbar_wait(&bars.empty[s], rp.ph ^ 1, abort_flag, status, KID_GEMM_SKINNY, 1)) { ok = false; break; }
+                mbar_expect_tx(&bars.full[s], n * unit_bytes);
+                uint8_t* sb = pipe + s * stage_bytes + A_BYTES;
+#pragma unroll
+                for (int i = 0; i < UNITS; ++i)
+                  if (i < n) tma_load_2d_hint(sb + i * unit_bytes, &lora.b, &bars.full[s], step * BW, y[i] + col0, pol_w);
+                ++it; rp.next(stages);
               }
-            if (ok && in_stage) { mbar_arrive(&bars.full[rp.s]); ++it; rp.next(stages); }
+            }
             if (ok && t_due) ok = load_t();
           }
         }
@@ -422,40 +426,41 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
           for (int k = 0; k < SBK / 16; ++k) umma_f16(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.kb0) || k > 0);
           umma_commit(&bars.empty[s]);
         }
-        if constexpr (LORA) {
+        if constexpr (BW != 0) {
           if (!ok) break;
           if (!listed) ok = listed = mbar_wait(&lists.listed, 0, abort_flag, status, KID_GEMM_SKINNY, 5);
+          constexpr int UNITS = 64 / BW;
           const int part = lora_part(lora.a, sg.tile * tile_rows, tile_rows, N);
           const uint32_t (*hits)[4] = lists.hits[sg.kb0 == 0 && sg.kb1 == kblocks ? 0 : sg.tile == first_tile ? 1 : 2];
           const int steps = lists.steps;
           for (int step = part < 0 ? 0 : part; ok && step < steps; step += part < 0 ? 1 : lora.a.parts) {
             const uint4 h = *reinterpret_cast<const uint4*>(hits[step]);
             if ((h.x | h.y | h.z | h.w) == 0) continue;
-            const int tb = t_it & 1;
-            if (!mbar_wait(&lists.t_full[tb], (t_it >> 1) & 1, abort_flag, status, KID_GEMM_SKINNY, 7)) { ok = false; break; }
+            const int tb = steps <= 2 ? step : t_it & 1;
+            if (!mbar_wait(&lists.t_full[tb], steps <= 2 ? 0 : (t_it >> 1) & 1, abort_flag, status, KID_GEMM_SKINNY, 7)) { ok = false; break; }
             const uint32_t st = smem_u32(t_buf + tb * 2 * t_bytes);
-            const uint64_t dh = umma_desc_sw32(st), dl = umma_desc_sw32(st + t_bytes);
-            int in_stage = 0;
-            uint32_t left[4] = {h.x, h.y, h.z, h.w};
+            for (int w = 0; w < 4 && ok; ++w) {
+              uint32_t left = hits[step][w];
+              while (left) {
+                const int n = min(UNITS, __popc(left)), s = rp.s;
+                uint4 m[UNITS];
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              while (left[w] && ok) {
-                const int j = 32 * w + __ffs(left[w]) - 1, s = rp.s;
-                left[w] &= left[w] - 1;
-                const uint4 m = *reinterpret_cast<const uint4*>(lists.mine[j]);
-                if (in_stage == 0) {
-                  ok = mbar_wait(&bars.full[s], rp.ph, abort_flag, status, KID_GEMM_SKINNY, 3);
-                  tc_fence_after();
-                  if (!ok) break;
+                for (int i = 0; i < UNITS; ++i) {
+                  m[i] = i < n ? *reinterpret_cast<const uint4*>(lists.mine[32 * w + __ffs(left) - 1]) : make_uint4(0, 0, 0, 0);
+                  left &= left - 1;
                 }
-                const uint32_t mine[4] = {m.x, m.y, m.z, m.w};
-                const uint64_t db = umma_desc_sw32(smem_u32(pipe + s * stage_bytes + A_BYTES + in_stage * unit_bytes));
-                umma_f16_lanes(d_tmem, dh, db, idesc, mine);
-                umma_f16_lanes(d_tmem, dl, db, idesc, mine);
-                if (++in_stage == 4) { umma_commit(&bars.empty[s]); in_stage = 0; rp.next(stages); }
+                ok = mbar_wait(&bars.full[s], rp.ph, abort_flag, status, KID_GEMM_SKINNY, 3);
+                tc_fence_after();
+                if (!ok) break;
+                const uint32_t sb = smem_u32(pipe + s * stage_bytes + A_BYTES);
+#pragma unroll
+                for (int i = 0; i < UNITS; ++i)
+                  if (i < n) umma_unit<BW>(d_tmem, st, st + t_bytes, sb + i * unit_bytes, idesc, {m[i].x, m[i].y, m[i].z, m[i].w});
+                umma_commit(&bars.empty[s]);
+                rp.next(stages);
               }
-            if (ok && in_stage) { umma_commit(&bars.empty[rp.s]); rp.next(stages); }
-            if (ok) { umma_commit(&lists.t_empty[tb]); ++t_it; }
+            }
+            if (ok && steps > 2) { umma_commit(&lists.t_empty[tb]); ++t_it; }
           }
         }
         if (ok) umma_commit(&bars.tmem_full[acc]);
@@ -470,7 +475,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     const bool row_live = q * 32 < M;             // warp-uniform: this quarter holds real tokens
     const int e = (warp - 2) * 32 + lane;         // 0..127, cooperative index
     const int vpr = tile_rows / 8;                // 8-value vectors per tile row
-    if constexpr (LORA) lora_list(lists, lora.a, M, N, e, share_of(first_tile), share_of((int)((u1 - 1) / kblocks)), status);
+    if constexpr (BW != 0) lora_list(lists, lora.a, M, N, e, share_of(first_tile), share_of((int)((u1 - 1) / kblocks)), status);
     pdl_wait();                                   // scratch, counters, the arena and Y belong to earlier kernels until here
     if (e == 0) FF_TL(status, KID_GEMM_SKINNY, 7);
     int ar_epoch = 0;
@@ -737,6 +742,7 @@ static int sk_smem_limit() {
   }
   return v;
 }
+constexpr int SK_LORA_SMEM = 216 * 1024;        // with adapters, next to the lists of their units
 constexpr int SK_SMEM_FULL = 200 * 1024;        // budget of a CTA that has its SM to itself (more than 64 tokens)
 // budget for a launch of M tokens: the split of a problem is chosen for 64 tokens under the small budget and kept for
 // every M (a row's bits must not depend on the batch it is computed in); only the pipeline depth follows M
@@ -751,7 +757,7 @@ static int skinny_max_clusters(int s) {
   if (s < 2 || s > 8) return 0;
   int* cached = cache[current_device()];
   if (cached[s] >= 0) return cached[s];
-  auto kern = gemm_skinny_kernel<false, false>;
+  auto kern = gemm_skinny_kernel<false, 0>;
   if (opt_in_smem(kern, SK_SMEM_FULL + 1024)) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(s * 64); cfg.blockDim = dim3(192); cfg.dynamicSmemBytes = SK_SMEM_FULL + 1024;
@@ -993,23 +999,26 @@ static int gemm_skinny_launch(const void* X, const void* W, void* Y, int M, int 
   const PeerArena none = {};
   if (lora != nullptr) {
     LoraDev dev = {};
-    dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts};
+    dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts, lora->bw};
     if (int e = lora_maps(dev, lora->t, lora->b, M, N, ntok, cfg.tile_rows, cfg.tile_rows)) return e;
-    // behind the ring: t of two steps (the instruction reads 128 rows of each word)
-    const int ring = cfg.pipe_off + cfg.stages * (ntok + cfg.tile_rows) * SBK * 2 + 1024, t_room = 3 * ntok * 32 + STOK * 32;
-    const int with_t = ring + t_room > smem ? ring + t_room : smem;
-    auto kern = gemm_skinny_kernel<false, true>;
-    r = opt_in_smem(kern, SK_SMEM_FULL + 1024 + STOK * 128); if (r) return r;
-    return launch_pdl(kern, dim3(grid), dim3(192), with_t, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
-                      cfg.stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail, dev);
+    // behind the ring: both words of t of two steps (the instruction reads 128 rows of each)
+    const int stage = (ntok + cfg.tile_rows) * SBK * 2, t_room = (3 * ntok + STOK) * lora->bw * 2, most = SK_LORA_SMEM - 1024 - cfg.pipe_off - t_room;
+    const int stages = cfg.stages * stage <= most ? cfg.stages : most / stage;
+    if (stages < 2) return FF_HOST_TOO_LARGE;
+    int bytes = cfg.pipe_off + stages * stage + 1024;
+    bytes += t_room > skinny_tail_slack(ntok, cfg.tile_rows) ? t_room : skinny_tail_slack(ntok, cfg.tile_rows);
+    auto kern = lora->bw == 32 ? gemm_skinny_kernel<false, 32> : gemm_skinny_kernel<false, 16>;
+    r = opt_in_smem(kern, SK_LORA_SMEM); if (r) return r;
+    return launch_pdl(kern, dim3(grid), dim3(192), bytes, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
+                      stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail, dev);
   }
   if (arena == nullptr) {
-    auto kern = gemm_skinny_kernel<false, false>;
+    auto kern = gemm_skinny_kernel<false, 0>;
     r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
     return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
                       cfg.stages, cl, cfg.pipe_off, scratch, counters, status, none, ep, tail, NoLora{});
   }
-  auto kern = gemm_skinny_kernel<true, false>;
+  auto kern = gemm_skinny_kernel<true, 0>;
   r = opt_in_smem(kern, SK_SMEM_FULL + 1024); if (r) return r;
   return launch_pdl(kern, dim3(grid), dim3(192), smem, stream, cl, tmX, tmW, y, M, N, K, ldy, ntok, cfg.tile_rows,
                     cfg.stages, cl, cfg.pipe_off, scratch, counters, status, *arena, ep, tail, NoLora{});

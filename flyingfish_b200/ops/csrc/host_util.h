@@ -47,7 +47,8 @@ inline int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType 
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return FF_HOST_NO_DRIVER;
   if ((reinterpret_cast<uintptr_t>(base) & 15) || (row_bytes & 15)) return FF_HOST_BAD_ALIGN;
-  if ((swizzle == CU_TENSOR_MAP_SWIZZLE_128B && box_inner * elem_bytes > 128) || (swizzle == CU_TENSOR_MAP_SWIZZLE_32B && box_inner * elem_bytes > 32)) return FF_HOST_BAD_SHAPE;
+  const uint32_t most = swizzle == CU_TENSOR_MAP_SWIZZLE_128B ? 128 : swizzle == CU_TENSOR_MAP_SWIZZLE_64B ? 64 : swizzle == CU_TENSOR_MAP_SWIZZLE_32B ? 32 : ~0u;
+  if (box_inner * elem_bytes > most) return FF_HOST_BAD_SHAPE;
   if (box_outer > 256 || box_inner > 256) return FF_HOST_BAD_SHAPE;
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_bytes};

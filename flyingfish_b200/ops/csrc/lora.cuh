@@ -1,11 +1,11 @@
 // What the products of gemm_skinny.cu and gemm_bf16.cu take to add low-rank adapters (lora.cu): the distinct adapters of a tile's rows as units of
-// 16 ranks, the tensor maps of t and B, and tensor instructions that leave out lanes.
+// BW = 16 or 32 ranks, the tensor maps of t and B, and tensor instructions that leave out lanes.
 //
-// A unit (adapter a, step s) is t[:, 16 s .. 16 s + 15] B_a[:, 16 s .. 16 s + 15]^T, accumulated behind the product's own K blocks into the same
-// FP32 sums, for the rows of the adapter only: a row of the tile is a lane of tensor memory, and the instruction's mask of lanes leaves the others' sums
+// A unit (adapter a, step s) is t[:, BW s ..] B_a[:, BW s ..]^T, BW columns of both, accumulated behind the product's own K blocks into the same FP32
+// sums, for the rows of the adapter only: a row of the tile is a lane of tensor memory, and the instruction's mask of lanes leaves the others' sums
 // alone, whatever t and B hold. So a tile takes any mix of adapters, a row without one gets the bits of the product alone, and what an adapter
-// holds (infinities included) reaches its own rows only. t is two BF16 words per value (high, low), so a unit is two instructions. Operands of 16
-// columns, 32-byte swizzle.
+// holds (infinities included) reaches its own rows only. t is two BF16 words per value (high, low), so 16 ranks are two instructions. Operands of BW
+// columns lie in shared memory with a swizzle of their width.
 #pragma once
 #include "ptx.cuh"
 #include "host_util.h"
@@ -14,7 +14,7 @@ namespace ff {
 
 struct LoraArgs {
   const int *ids, *ranks, *part_of;    // ranks, part_of: may be null
-  int adapters, R, parts;
+  int adapters, R, parts, bw;
 };
 
 struct LoraDev {                       // kernel parameter
@@ -25,7 +25,7 @@ struct NoLora {};
 
 __device__ __forceinline__ int lora_steps(const LoraArgs& a, int adapter) {
   const int r = a.ranks == nullptr ? a.R : min(max(a.ranks[adapter], 0), a.R);
-  return (r + 15) >> 4;
+  return (r + a.bw - 1) >> (a.bw == 32 ? 5 : 4);
 }
 
 // The rows row0 .. row0 + 32 H of a tile by adapter. Warp-wide; lane i looks after rows row0 + i + 32 h.
@@ -85,18 +85,18 @@ struct UnitWalk {
   }
 };
 
-// One or two units of a stage: [high 0 | low 0 | high 1 | low 1] of t in the place of X, [B 0 | B 1] in the place of W.
+// The units of a stage: [high 0 | low 0 | high 1 | low 1] of t in the place of X, [B 0 | B 1] in the place of W, one unit of 32 ranks or up to two of 16.
 template <int H>
 struct UnitPair {
   int n, adapter0, step0, adapter1, step1;
   uint32_t mine0[H], mine1[H];
-  __device__ __forceinline__ bool next(UnitWalk<H>& w) {
+  __device__ __forceinline__ bool next(UnitWalk<H>& w, bool two) {
     n = 0;
     if (!w.next()) return false;
     adapter0 = w.adapter; step0 = w.step; w.step += w.by; n = 1;
 #pragma unroll
     for (int h = 0; h < H; ++h) mine0[h] = w.mine[h];
-    if (w.next()) {
+    if (two && w.next()) {
       adapter1 = w.adapter; step1 = w.step; w.step += w.by; n = 2;
 #pragma unroll
       for (int h = 0; h < H; ++h) mine1[h] = w.mine[h];
@@ -106,9 +106,9 @@ struct UnitPair {
 };
 
 // Decode products: one tile of up to 128 rows, whose adapters are listed once per CTA in shared memory by the epilogue's 128 threads while the weights stream.
-// Units go step by step, so that t of a step is loaded once for all adapters; up to four of a step's units share a stage of the ring. The threads that
-// load and multiply walk lists of bits: one thread alone takes hundreds of cycles to find a unit among the adapters, a few to take the next bit
-// (64 rows with 64 adapters of rank 16, 6144 x 4096: 51 us with the search, LORA_AFTER with the bits).
+// Units go step by step, so that t of a step is loaded once for all adapters (once for all tiles where there are no more steps than buffers); up to 64 / BW of
+// a step's units share a stage of the ring. The threads that load and multiply walk lists of bits: one thread alone takes hundreds of cycles
+// to find a unit among the adapters (64 rows with 64 adapters of rank 16, 6144 x 4096: 51 us with the search, 33 with the bits).
 //
 // Where a tile's K is divided among CTAs, a hash of the adapter and the step say whose a unit is: where a row's units go, and with it the order of its
 // sums, depends on nothing but its adapter.
@@ -180,14 +180,16 @@ __device__ __forceinline__ int lora_part(const LoraArgs& a, int col0, int width,
   return p;
 }
 
-// K-major operand of 16 BF16 per row, 32-byte swizzle: rows of 32 bytes, groups of eight 256 bytes apart
-__device__ __forceinline__ uint64_t umma_desc_sw32(uint32_t smem_addr) {
+// K-major operand of BW BF16 per row, swizzle of the row's width: groups of eight rows 16 BW bytes apart
+template <int BW>
+__device__ __forceinline__ uint64_t umma_desc_narrow(uint32_t smem_addr) {
+  static_assert(BW == 16 || BW == 32);
   uint64_t d = 0;
   d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
   d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(256 >> 4) << 32;
+  d |= (uint64_t)BW << 32;
   d |= (uint64_t)1 << 46;
-  d |= (uint64_t)6 << 61;      // SWIZZLE_32B
+  d |= (uint64_t)(BW == 16 ? 6 : 4) << 61;      // SWIZZLE_32B, SWIZZLE_64B
   return d;
 }
 
@@ -206,12 +208,32 @@ __device__ __forceinline__ void umma_f16_pair_lanes(uint32_t d_tmem, uint64_t a_
       "r"(~mine[6]), "r"(~mine[7]) : "memory");
 }
 
-// tensor maps of t [M, 2R] (boxes of t_rows rows) and of B [adapters * N, R] (boxes of b_rows and b2_rows rows), 16 columns wide
+// a unit: both words of t (t_high, t_low) times B, in shared memory, for the lanes of `mine`
+template <int BW>
+__device__ __forceinline__ void umma_unit(uint32_t d_tmem, uint32_t t_high, uint32_t t_low, uint32_t b, uint32_t idesc, const uint32_t (&mine)[4]) {
+  const uint64_t h = umma_desc_narrow<BW>(t_high), l = umma_desc_narrow<BW>(t_low), w = umma_desc_narrow<BW>(b);
+#pragma unroll
+  for (int k = 0; k < BW / 16; ++k) umma_f16_lanes(d_tmem, h + 2 * k, w + 2 * k, idesc, mine);
+#pragma unroll
+  for (int k = 0; k < BW / 16; ++k) umma_f16_lanes(d_tmem, l + 2 * k, w + 2 * k, idesc, mine);
+}
+template <int BW>
+__device__ __forceinline__ void umma_unit_pair(uint32_t d_tmem, uint32_t t_high, uint32_t t_low, uint32_t b, uint32_t idesc, const uint32_t (&mine)[8]) {
+  const uint64_t h = umma_desc_narrow<BW>(t_high), l = umma_desc_narrow<BW>(t_low), w = umma_desc_narrow<BW>(b);
+#pragma unroll
+  for (int k = 0; k < BW / 16; ++k) umma_f16_pair_lanes(d_tmem, h + 2 * k, w + 2 * k, idesc, mine);
+#pragma unroll
+  for (int k = 0; k < BW / 16; ++k) umma_f16_pair_lanes(d_tmem, l + 2 * k, w + 2 * k, idesc, mine);
+}
+
+// tensor maps of t [M, 2R] (boxes of t_rows rows) and of B [adapters * N, R] (boxes of b_rows and b2_rows rows), bw columns wide
 inline int lora_maps(LoraDev& d, const void* t, const void* b, int M, int N, int t_rows, int b_rows, int b2_rows) {
   const uint64_t r = d.a.R;
-  if (int e = make_tmap_2d(&d.t, t, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 2 * r, M, 4 * r, 16, t_rows, CU_TENSOR_MAP_SWIZZLE_32B)) return e;
-  if (int e = make_tmap_2d(&d.b, b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r, (uint64_t)d.a.adapters * N, 2 * r, 16, b_rows, CU_TENSOR_MAP_SWIZZLE_32B)) return e;
-  return make_tmap_2d(&d.b2, b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r, (uint64_t)d.a.adapters * N, 2 * r, 16, b2_rows, CU_TENSOR_MAP_SWIZZLE_32B);
+  const CUtensorMapSwizzle sw = d.a.bw == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  if (int e = make_tmap_2d(&d.t, t, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 2 * r, M, 4 * r, d.a.bw, t_rows, sw)) return e;
+  if (int e = make_tmap_2d(&d.b, b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r, (uint64_t)d.a.adapters * N, 2 * r, d.a.bw, b_rows, sw)) return e;
+  if (b2_rows == b_rows) { d.b2 = d.b; return FF_HOST_OK; }
+  return make_tmap_2d(&d.b2, b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r, (uint64_t)d.a.adapters * N, 2 * r, d.a.bw, b2_rows, sw);
 }
 
 }  // namespace ff

@@ -22,14 +22,15 @@ GATES = (0, 3, 5)                # gates that the products' epilogues know (ops.
 class AdapterStack(NamedTuple):
     """The adapters of one projection ``[N, K]``. ``a`` [adapters, R, K] and ``b`` [adapters, N, R] are BF16, ``scale`` FP32 [adapters]; R is a multiple of
     16 and the rank rows behind an adapter's own are zero. ``ranks`` (int32 [adapters]) says how many rows that are, so that the rest is
-    not read. ``part_of`` (int32 [N / 64]) and ``parts`` describe a fused projection: its adapters' ranks come in steps of 16, step s belongs to part
-    ``s % parts``, and the 64 columns from ``64 i`` have non-zero ``b`` in the steps of part ``part_of[i]`` only."""
+    not read. ``part_of`` (int32 [N / 64]), ``parts`` and ``step`` describe a fused projection: its adapters' ranks come in steps of ``step`` (16 or 32), step s
+    belongs to part ``s % parts``, and the 64 columns from ``64 i`` have non-zero ``b`` in the steps of part ``part_of[i]`` only."""
     a: torch.Tensor
     b: torch.Tensor
     scale: torch.Tensor
     ranks: torch.Tensor | None = None
     part_of: torch.Tensor | None = None
     parts: int = 1
+    step: int = 16
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.a, self.b, self.scale, self.ranks, self.part_of) if t is not None)
@@ -45,8 +46,8 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
     _require(not interleave or (parts == 2 and columns[0] == columns[1] and columns[0] % 64 == 0), "pack_stack: two equal parts interleave")
     _require(parts == 1 or all(c % 64 == 0 for c in columns), "pack_stack: parts of whole 64 columns")
     most = max((e[0].shape[0] for p in adapters for e in p if e is not None), default=0)
-    step = max(16, (most + 15) // 16 * 16)
-    r = step * parts
+    step = 16 if most <= 16 else 32
+    r = max(1, (most + step - 1) // step) * step * parts
     _require(r <= MAX_RANK, f"pack_stack: ranks of {parts} parts of {most} exceed {MAX_RANK}")
     a = torch.zeros(len(adapters), r, k, dtype=dtype)
     b = torch.zeros(len(adapters), n, r, dtype=dtype)
@@ -61,11 +62,11 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
                 rank = pa.shape[0]
                 _require(pa.shape == (rank, k) and pb.shape == (columns[j], rank), f"pack_stack: adapter {i}: A [{rank}, {k}] and B [{columns[j]}, {rank}]")
                 _require(bool(torch.isfinite(pa).all()) and bool(torch.isfinite(pb).all()), f"pack_stack: adapter {i} holds infinities or NaN")
-                where = torch.tensor([(q // 16 * parts + j) * 16 + q % 16 for q in range(rank)], dtype=torch.long)
+                where = torch.tensor([(q // step * parts + j) * step + q % step for q in range(rank)], dtype=torch.long)
                 a[i, where] = pa.to("cpu", dtype)
                 pb = pb.to("cpu", torch.float32) if s != first else pb.to("cpu")
                 b[i, at: at + columns[j], where] = (pb if s == first else pb * (s / first)).to(dtype)
-                ranks[i] = max(int(ranks[i]), (rank + 15) // 16 * 16 * parts)
+                ranks[i] = max(int(ranks[i]), (rank + step - 1) // step * step * parts)
             at += columns[j]
     part_of = None
     if interleave:
@@ -74,19 +75,19 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
     elif parts > 1:
         part_of = torch.repeat_interleave(torch.arange(parts, dtype=torch.int32), torch.tensor([c // 64 for c in columns]))
     move = lambda t: None if t is None else t.to(device)
-    return AdapterStack(move(a), move(b), move(scale), move(ranks), move(part_of), parts)
+    return AdapterStack(move(a), move(b), move(scale), move(ranks), move(part_of), parts, step)
 
 
 class _Lora(ctypes.Structure):            # FfLora of csrc/lora.cu
     _fields_ = [(n, c_void_p) for n in ("x", "w", "y", "a", "b", "scale", "ranks", "ids", "part_of", "t", "scratch", "counters", "status", "cos_sin",
                                         "slots", "kcache", "vcache")] + [("scratch_bytes", c_longlong), ("counter_bytes", c_longlong)] + \
-               [(n, c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "R", "adapters", "parts", "epi", "gate")] + [("limit", c_float)] + \
+               [(n, c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "R", "adapters", "parts", "step", "epi", "gate")] + [("limit", c_float)] + \
                [(n, c_int) for n in ("hq", "hkv", "rot_dim", "block_size", "num_blocks")]
 
 
 def _check_stack(x: torch.Tensor, n: int, stack: AdapterStack, ids: torch.Tensor) -> tuple[int, int]:
     """(adapters, R) of a stack that fits the projection."""
-    a, b, scale, ranks, part_of, parts = stack
+    a, b, scale, ranks, part_of, parts, step = stack
     _require(a.dim() == 3 and b.dim() == 3 and a.shape[2] == x.shape[1], "adapters: A [adapters, R, K] of the projection's K")
     count, r = a.shape[0], a.shape[1]
     _require(b.shape == (count, n, r) and scale.shape == (count,), "adapters: B [adapters, N, R], a scale per adapter")
@@ -95,7 +96,8 @@ def _check_stack(x: torch.Tensor, n: int, stack: AdapterStack, ids: torch.Tensor
     _require(a.is_contiguous() and b.is_contiguous() and scale.is_contiguous(), "adapters: contiguous weights")
     _require(ids.dtype == torch.int32 and ids.shape == (x.shape[0],) and ids.is_contiguous(), "adapters: one int32 id per row")
     _require(ranks is None or (ranks.dtype == torch.int32 and ranks.shape == (count,) and ranks.is_contiguous()), "adapters: int32 ranks")
-    _require(part_of is None or (part_of.dtype == torch.int32 and part_of.numel() * 64 >= n and part_of.is_contiguous() and parts > 0), "adapters: int32 parts")
+    _require(part_of is None or (part_of.dtype == torch.int32 and part_of.numel() * 64 >= n and part_of.is_contiguous() and parts > 0 and step in (16, 32) and r % step == 0),
+             "adapters: int32 parts, ranks in whole steps")
     return count, r
 
 
@@ -108,7 +110,7 @@ def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tenso
     k = x.shape[1]
     _require(w.shape[1] == k, "linear_lora: inner dimensions differ")
     count, r = _check_stack(x, n, stack, ids)
-    a, b, scale, ranks, part_of, parts = stack
+    a, b, scale, ranks, part_of, parts, step = stack
     _require(dev.index == torch.cuda.current_device(), "linear_lora: operands on another device than the current one")
     _require(all(t is None or t.device == dev for t in (w, a, b, scale, ids, ranks, part_of, out)), "linear_lora: operands on several devices")
     if out is None:
@@ -124,7 +126,7 @@ def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tenso
     for attempt in (0, 1):
         form = _Lora(x.data_ptr(), w.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), opt(ranks), ids.data_ptr(), opt(part_of), t.data_ptr(),
                      ws.gemm_scratch.data_ptr(), ws.gemm_counters.data_ptr(), status_tensor(dev).data_ptr(), opt(cs), opt(slots), opt(kc), opt(vc),
-                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, m, n, k, ldx, ldw, out.stride(0), r, count, parts, epi, gate, limit, *heads)
+                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, m, n, k, ldx, ldw, out.stride(0), r, count, parts, step, epi, gate, limit, *heads)
         rc = lib.ff_linear_lora(ctypes.byref(form), c_void_p(torch.cuda.current_stream().cuda_stream))
         if rc != -5 or attempt or m > SKINNY_MAX_M:
             break

@@ -66,7 +66,7 @@ def test_packed_parts_are_the_parts():
     mk = lambda c, r, s: (torch.randn(r, k, generator=g), torch.randn(c, r, generator=g), s)
     adapters = [[mk(256, 8, 2.0), None, mk(64, 20, 2.0)], [mk(256, 3, 0.5), mk(64, 17, 0.25), mk(64, 3, 0.5)], [None, None, None]]
     st = lora_ops.pack_stack(adapters, k, cols, "cpu", torch.float32)
-    assert st.a.shape == (3, 96, k) and st.ranks.tolist() == [96, 96, 0] and st.part_of.tolist() == [0, 0, 0, 0, 1, 2]
+    assert st.a.shape == (3, 96, k) and st.step == 32 and st.ranks.tolist() == [96, 96, 0] and st.part_of.tolist() == [0, 0, 0, 0, 1, 2]
     x = torch.randn(6, k, generator=g)
     ids = torch.tensor([0, 1, 2, -1, 1, 0], dtype=torch.int32)
     got = lora_ops.linear_lora(x, torch.zeros(384, k), st, ids)
@@ -81,9 +81,9 @@ def test_packed_parts_are_the_parts():
     assert torch.allclose(got, want, rtol=1e-4, atol=1e-4) and st.part_of.tolist() == [0, 1, 0, 1]
     # b is zero where a part's columns do not look
     for i, p in enumerate(st.part_of.tolist()):
-        for s in range(st.a.shape[1] // 16):
+        for s in range(st.a.shape[1] // st.step):
             if s % st.parts != p:
-                assert not st.b[:, 64 * i: 64 * i + 64, 16 * s: 16 * s + 16].any()
+                assert not st.b[:, 64 * i: 64 * i + 64, st.step * s: st.step * (s + 1)].any()
 
 
 def test_refusals():
@@ -91,7 +91,7 @@ def test_refusals():
     bad = [(st._replace(a=st.a[:, :, :56]), ids), (st._replace(b=st.b[:, :40]), ids), (st._replace(scale=st.scale.double()), ids),
            (st._replace(a=st.a[:, :8], b=st.b[:, :, :8]), ids), (st._replace(ranks=st.ranks.long()), ids), (st, ids.long()), (st, ids[:3]),
            (st._replace(b=st.b.float()), ids), (st._replace(a=st.a.transpose(0, 1).contiguous().transpose(0, 1)), ids),
-           (st._replace(part_of=torch.zeros(0, dtype=torch.int32)), ids)]
+           (st._replace(part_of=torch.zeros(0, dtype=torch.int32)), ids), (st._replace(part_of=torch.zeros(1, dtype=torch.int32), step=32), ids)]
     for stack, i in bad:
         with pytest.raises(KernelError):
             lora_ops.linear_lora(x, w, stack, i)
