@@ -28,6 +28,7 @@
 #include "comm.cuh"
 #include "host_util.h"
 #include "launchers.h"
+#include <atomic>
 #include <mutex>
 #include <vector>
 #include "skinny_common.cuh"
@@ -742,7 +743,9 @@ static int sk_smem_limit() {
   }
   return v;
 }
-constexpr int SK_LORA_SMEM = 216 * 1024;        // with adapters, next to the lists of their units
+// With adapters: what a CTA may take next to the lists of their units, and up to 64 rows less, so that a CTA of the kernel that computes t fits beside it and
+// the weights stream meanwhile (64 rows, 8 adapters of rank 64, 6144 x 4096: 22.5 -> 20.0 us; 113 rows want the ring: 57.5 us with 216 KB, 59.8 with 180).
+constexpr int SK_LORA_SMEM = 216 * 1024, SK_LORA_SMEM_FEW = 180 * 1024;
 constexpr int SK_SMEM_FULL = 200 * 1024;        // budget of a CTA that has its SM to itself (more than 64 tokens)
 // budget for a launch of M tokens: the split of a problem is chosen for 64 tokens under the small budget and kept for
 // every M (a row's bits must not depend on the batch it is computed in); only the pipeline depth follows M
@@ -796,6 +799,7 @@ static int skinny_stages(int tile_rows, int reserved = 0, int ntok = 64, int lim
 struct SkinnyChoice { int N, K, epi, s, rows; };
 static std::mutex g_choice_mu;
 static std::vector<SkinnyChoice> g_choices;
+static std::atomic<int> g_choice_version{0};
 
 static bool skinny_choice(int N, int K, int epi, int* s, int* rows) {
   std::lock_guard<std::mutex> lk(g_choice_mu);
@@ -816,7 +820,7 @@ static void skinny_fit_cluster(SkinnyConfig& c, int M, int N, int epi) {
 }
 
 // epi != 0 (row-wise epilogue): tiles are exactly 128 rows.
-static SkinnyConfig skinny_config(int M, int N, int K, int epi = 0) {
+static SkinnyConfig skinny_decompose(int M, int N, int K, int epi) {
   const int kblocks = (K + SBK - 1) / SBK;
   static int env_s = -1, env_r = -1;
   if (env_s < 0) {
@@ -910,6 +914,17 @@ static SkinnyConfig skinny_config(int M, int N, int K, int epi = 0) {
   return best;
 }
 
+// A thread's last decompositions: one takes 1.6 to 2.8 us to find, and a product asks for it twice (plan and launch), a step of a model for the same few again
+// and again.
+static SkinnyConfig skinny_config(int M, int N, int K, int epi = 0) {
+  struct Entry { int M, N, K, epi, dev, version; SkinnyConfig cfg; };
+  static thread_local Entry memo[64] = {};
+  const int dev = current_device(), version = g_choice_version.load();
+  Entry& e = memo[(unsigned)(M * 31 + N * 7 + K * 3 + epi) % 64u];
+  if (e.M != M || e.N != N || e.K != K || e.epi != epi || e.dev != dev || e.version != version) e = Entry{M, N, K, epi, dev, version, skinny_decompose(M, N, K, epi)};
+  return e.cfg;
+}
+
 // Decomposition chosen for a problem: out = {cluster size, tile rows, tiles, pipeline stages, grid}.
 FF_EXPORT int ff_gemm_skinny_config(int M, int N, int K, int epi, int* out) {
   if (M <= 0 || M > STOK || N <= 0 || K <= 0 || out == nullptr) return FF_HOST_BAD_SHAPE;
@@ -929,6 +944,7 @@ FF_EXPORT int ff_gemm_skinny_set_choice(int N, int K, int epi, int s, int rows) 
   for (size_t i = 0; i < g_choices.size(); ++i)
     if (g_choices[i].N == N && g_choices[i].K == K && g_choices[i].epi == epi) { g_choices.erase(g_choices.begin() + i); break; }
   if (s > 0) g_choices.push_back({N, K, epi, s, rows});
+  ++g_choice_version;
   return 0;
 }
 
@@ -1002,7 +1018,7 @@ static int gemm_skinny_launch(const void* X, const void* W, void* Y, int M, int 
     dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts, lora->bw};
     if (int e = lora_maps(dev, lora->t, lora->b, M, N, ntok, cfg.tile_rows, cfg.tile_rows)) return e;
     // behind the ring: both words of t of two steps (the instruction reads 128 rows of each)
-    const int stage = (ntok + cfg.tile_rows) * SBK * 2, t_room = (3 * ntok + STOK) * lora->bw * 2, most = SK_LORA_SMEM - 1024 - cfg.pipe_off - t_room;
+    const int stage = (ntok + cfg.tile_rows) * SBK * 2, t_room = (3 * ntok + STOK) * lora->bw * 2, most = (M <= 64 ? SK_LORA_SMEM_FEW : SK_LORA_SMEM) - 1024 - cfg.pipe_off - t_room;
     const int stages = cfg.stages * stage <= most ? cfg.stages : most / stage;
     if (stages < 2) return FF_HOST_TOO_LARGE;
     int bytes = cfg.pipe_off + stages * stage + 1024;

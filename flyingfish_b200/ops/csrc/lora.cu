@@ -246,7 +246,8 @@ static int lora_shrink(const FfLora& c, int bw, cudaStream_t stream) {
   if (int e = make_tmap_2d(&tmX, c.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.K, c.M, (uint64_t)c.ldx * 2, 64, xrows)) return e;
   if (int e = make_tmap_2d(&tmA, c.a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.K, (uint64_t)c.adapters * c.R, (uint64_t)c.K * 2, 64, bw)) return e;
   const int stage = xrows * 128 + most * bw * 128, kb = ((c.K + 63) / 64 + LS_SPLIT - 1) / LS_SPLIT, recv = most * LS_SPLIT * 16 * bw * 4;
-  int stages = (108 * 1024 - recv) / stage;
+  // two CTAs on an SM for prompts; for decode rows so little that one fits beside a CTA of the product (7 rows, 4096 x 14336: 29.0 -> 24.6 us)
+  int stages = ((c.M > LS_ROWS ? 108 : 40) * 1024 - recv) / stage;
   stages = stages > LS_STAGES ? LS_STAGES : stages < 2 ? 2 : stages;
   stages = stages > kb ? (kb < 2 ? 2 : kb) : stages;
   // the instruction reads 128 rows of X, past the loaded ones into what lies behind them

@@ -101,9 +101,12 @@ def _check_stack(x: torch.Tensor, n: int, stack: AdapterStack, ids: torch.Tensor
     return count, r
 
 
+def _at(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tensor, out: torch.Tensor | None, width: int, epi: int, gate: int = 0,
          limit: float = 0.0, rope: tuple | None = None) -> torch.Tensor:
-    dev = x.device
     _require(isinstance(w, torch.Tensor) and x.dtype == w.dtype == BF16, "linear_lora: BF16 operands required on CUDA")
     m, ldx = _rows2d(x)
     n, ldw = _rows2d(w)
@@ -111,23 +114,27 @@ def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tenso
     _require(w.shape[1] == k, "linear_lora: inner dimensions differ")
     count, r = _check_stack(x, n, stack, ids)
     a, b, scale, ranks, part_of, parts, step = stack
-    _require(dev.index == torch.cuda.current_device(), "linear_lora: operands on another device than the current one")
-    _require(all(t is None or t.device == dev for t in (w, a, b, scale, ids, ranks, part_of, out)), "linear_lora: operands on several devices")
+    at = x.get_device()
+    _require(at == torch.cuda.current_device(), "linear_lora: operands on another device than the current one")
+    _require(at == w.get_device() == a.get_device() == b.get_device() == scale.get_device() == ids.get_device() and
+             (ranks is None or ranks.get_device() == at) and (part_of is None or part_of.get_device() == at) and (out is None or out.get_device() == at),
+             "linear_lora: operands on several devices")
     if out is None:
-        out = torch.empty(m, width, dtype=BF16, device=dev)
-    _require(out.shape == (m, width) and out.stride(1) == 1 and out.dtype == BF16, "linear_lora: bad output tensor")
+        out = x.new_empty(m, width)
+    else:
+        _require(out.shape == (m, width) and out.stride(1) == 1 and out.dtype == BF16, "linear_lora: bad output tensor")
     if m == 0:
         return out
-    t = torch.empty(m, 2 * r, dtype=BF16, device=dev)         # of this call alone
+    dev = x.device
+    t = x.new_empty(m, 2 * r)                       # of this call alone
     ws = workspace(dev)
-    opt = lambda t: 0 if t is None else t.data_ptr()
     cs, slots, kc, vc, heads = rope if rope is not None else (None, None, None, None, (0, 0, 0, 0, 0))
-    lib = kernels()
+    lib, stream = kernels(), c_void_p(torch._C._cuda_getCurrentRawStream(at))
     for attempt in (0, 1):
-        form = _Lora(x.data_ptr(), w.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), opt(ranks), ids.data_ptr(), opt(part_of), t.data_ptr(),
-                     ws.gemm_scratch.data_ptr(), ws.gemm_counters.data_ptr(), status_tensor(dev).data_ptr(), opt(cs), opt(slots), opt(kc), opt(vc),
+        form = _Lora(x.data_ptr(), w.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), _at(ranks), ids.data_ptr(), _at(part_of), t.data_ptr(),
+                     ws.gemm_scratch.data_ptr(), ws.gemm_counters.data_ptr(), status_tensor(dev).data_ptr(), _at(cs), _at(slots), _at(kc), _at(vc),
                      ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, m, n, k, ldx, ldw, out.stride(0), r, count, parts, step, epi, gate, limit, *heads)
-        rc = lib.ff_linear_lora(ctypes.byref(form), c_void_p(torch.cuda.current_stream().cuda_stream))
+        rc = lib.ff_linear_lora(ctypes.byref(form), stream)
         if rc != -5 or attempt or m > SKINNY_MAX_M:
             break
         scratch_b, counter_b = c_longlong(0), c_longlong(0)          # the product's scratch is too small: nothing was launched

@@ -3,12 +3,12 @@
 rows included."""
 from __future__ import annotations
 
-from ctypes import c_longlong, c_void_p
+from ctypes import c_int, c_longlong, c_void_p
 
 import torch
 
 from . import BF16, _count, _require, _rows2d, ref
-from .lib import check, kernels
+from .lib import KernelError, check, kernels
 
 F32, I32 = torch.float32, torch.int32
 
@@ -26,27 +26,46 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
     never drawn, and +inf shares everything among its equals; a row of -inf gives id 0 with probability 0. Masses are those of 64-bit arithmetic; one
     below 2^-1000 of the largest counts as none."""
     rows, ld = _rows2d(logits)
+    at = logits.get_device()
     vocab = logits.shape[1]
     _require(logits.dtype in (BF16, F32) and vocab > 0, "sample_tokens: bf16 or fp32 logits")
     _require(vocab < 1 << 31, "sample_tokens: ids are 32 bits wide")
-    dev = logits.device
     for t, dtype, name in ((uniforms, F32, "uniforms"), (temperature, F32, "temperature"), (top_k, I32, "top_k"), (top_p, F32, "top_p"), (min_p, F32, "min_p"),
                            (out, I32, "out"), (probs, F32, "probs")):
-        _require(t is None or (t.dtype == dtype and t.shape == (rows,) and t.is_contiguous() and t.device == dev),
-                 f"sample_tokens: {name} is one {dtype} per row on the logits' device")
+        if t is not None and not (t.dtype == dtype and t.dim() == 1 and t.shape[0] == rows and t.is_contiguous() and t.get_device() == at):
+            raise KernelError(f"sample_tokens: {name} is one {dtype} per row on the logits' device")
     if not logits.is_cuda:
         ids, p = ref.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p)
         return (ids if out is None else out.copy_(ids)), (p if probs is None else probs.copy_(p))
-    _require(dev.index == torch.cuda.current_device(), "sample_tokens: operands on another device than the current one")
+    _require(at == torch.cuda.current_device(), "sample_tokens: operands on another device than the current one")
     if out is None:
-        out = torch.empty(rows, dtype=I32, device=dev)
+        out = logits.new_empty(rows, dtype=I32)
     if probs is None:
-        probs = torch.empty(rows, dtype=F32, device=dev)
+        probs = logits.new_empty(rows, dtype=F32)
     if rows == 0:
         return out, probs
-    at = lambda t: c_void_p(0 if t is None else t.data_ptr())
-    rc = kernels().ff_sample_tokens(at(logits), int(logits.dtype == F32), at(uniforms), at(temperature), at(top_k), at(top_p), at(min_p), at(out), at(probs),
-                                    rows, vocab, c_longlong(ld), c_void_p(torch.cuda.current_stream().cuda_stream))
+    rc = _launcher()(logits.data_ptr(), logits.dtype == F32, uniforms.data_ptr(), temperature.data_ptr(), _at(top_k), _at(top_p), _at(min_p), out.data_ptr(),
+                     probs.data_ptr(), rows, vocab, ld, torch._C._cuda_getCurrentRawStream(at))
     check(rc, "ff_sample_tokens")
     _count()
     return out, probs
+
+
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+_typed = None
+
+
+def _launcher():
+    """``ff_sample_tokens`` with its argument types declared: plain numbers are converted by the call."""
+    global _typed
+    if _typed is None:
+        fn = kernels().ff_sample_tokens
+        if hasattr(fn, "argtypes"):                   # the checking build wraps the function
+            fn.argtypes = [c_void_p, c_int] + [c_void_p] * 7 + [c_int, c_int, c_longlong, c_void_p]
+            _typed = fn
+        else:
+            return lambda *v: fn(*(c_void_p(q) if i in (0, 2, 3, 4, 5, 6, 7, 8, 12) else c_longlong(q) if i == 11 else int(q) for i, q in enumerate(v)))
+    return _typed
