@@ -3,15 +3,20 @@
 //   w_i = exp((l_i - max l) / T), order: logit down, id up;  kept: the first n of the order, the least of what top-k, top-p (least n whose mass
 //   reaches P of the whole mass) and min-p (w_i >= min_p) leave, at least one;  drawn: lowest id whose sum of kept w up to it passes u times their sum.
 //
-// Ids are to be those of the formulas, so nothing that decides is rounded to 32 bits: w and its sums are FP64 (a row of 128 thousand flat tokens has
-// borders 8e-6 of the mass apart, and 32-bit sums move 128 thousand of them by 1e-7 each), the histograms' masses are integers of 30 bits below the
-// bin's scale, and where a border lies inside a bin its tokens are ranked one by one.
+// Ids are to be those of the formulas, so what decides is held in FP64: a row of 128 thousand flat tokens has borders 8e-6 of the mass apart, and
+// 32-bit sums move 128 thousand of them by 1e-7 each. Of the whole mass, tokens below 2^-24 of the largest are taken in FP32 with a compensated
+// exponent: together they are at most 1.6 % of it (V = 262144), so the mass is held to 4e-9 at worst and far better as their errors average.
 //
 // A cluster of C CTAs has a row: every CTA keeps its slice of the logits in shared memory, so that they come from memory once, and a warp a run of
-// consecutive ids of it. Steps, one cluster barrier each (values are pushed into every CTA's shared memory before it):
-//   max; sum of w (only for top-p); histogram of the candidates over (max - l) in 1/16 octave of w, merged in CTA 0, which finds the bin that holds the
-//   border; its tokens ranked in CTA 0 (bins of more than LIST tokens are divided by key first, ties of one key go by id); sums of kept w; the draw.
-// Candidates: w >= (1 - P) S / V, since what lies below has less than 1 - P of the mass; w >= min_p.
+// consecutive ids of it. Values cross by stores into the peers' shared memory in front of a cluster barrier. Steps:
+//   1 the largest logit;
+//   2 the mass, where top-p or the draw needs it, and a logit that at least k tokens reach, where top-k is on: of a CTA's threads' largest logits the n-th,
+//     n its share of k, the least over the CTAs;
+//   3 without top-k and top-p: the draw. Else the candidates -- logits at or above what top-k leaves, (1 - P) S / V (less has less than 1 - P of the
+//     mass) and min-p -- go to CTA 0, which sorts them, finds the border, sorts the kept ones by id and draws;
+//   4 more than SM_LIST candidates (flat rows): a histogram of the candidates' logits, masses in 14 bits, says in which bin the border lies, or two if it
+//     cannot tell; the mass above is summed in FP64 and the bin's tokens are sorted as in 3. A bin of more tokens is divided by key, ties of one key go by
+//     id. CTA 0 finds the warp that holds the draw, and that warp the token.
 //
 // NaN counts as -inf, -inf is never drawn, +inf shares everything among its equals; a row without anything gives id 0 with probability 0.
 #include "dtype_io.cuh"
@@ -20,7 +25,8 @@
 namespace ff {
 
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CLUSTER = 8;
-constexpr int SM_BINS = 1024, SM_LIST = 256, SM_TABLE = 64;
+constexpr int SM_BINS = 1024, SM_LIST = 1024, SM_SMALL = 256, SM_TABLE = 256, SM_PARTS = SM_CLUSTER * SM_WARPS;
+constexpr float SM_NEAR = -24.f, SM_FAR = -64.f;      // octaves below the largest: FP64 above the one, nothing below the other
 
 struct SampleArgs {
   const void* logits;
@@ -32,26 +38,33 @@ struct SampleArgs {
   int V, seg;                           // seg: ids per warp
 };
 
-struct SampleFound { int bin, count, reached; unsigned above; double mass_above; };
+struct SampleFound { int lo, hi, count, reached; unsigned above; };
 
 struct SampleShared {
-  double table[SM_TABLE];               // 2^(i / 64)
-  double gather[3][SM_CLUSTER];         // what every CTA of the cluster has pushed: by step
-  double warp_sum[SM_WARPS];
-  double scan_mass[SM_WARPS];
-  double list_w[SM_LIST], sorted_w[SM_LIST];
-  unsigned long long list[SM_LIST], sorted[SM_LIST];      // key << 32 | ~id
-  unsigned scan_count[SM_WARPS];
-  unsigned key_min[SM_CLUSTER], key_max[SM_CLUSTER];
-  unsigned ties[SM_CLUSTER];
-  unsigned warp_ties[SM_WARPS];
-  unsigned count[SM_BINS], high[SM_BINS], low[SM_BINS];               // this CTA's: tokens, mass in digits of 15 bits
-  unsigned all_count[SM_BINS], all_high[SM_BINS], all_low[SM_BINS];   // CTA 0: of the cluster, digits of 24 bits
-  SampleFound found;
-  unsigned border_key; int border_id;
-  int list_n;
+  double table[SM_TABLE];               // 2^(i / 256)
+  double mass[SM_CLUSTER];              // what every CTA of the cluster has pushed: the mass
+  double part[SM_PARTS];                // CTA 0, general path: every warp's kept mass in front of the border's bins
+  unsigned long long part_in[SM_PARTS]; // and within them, in units of 2^-50: whole numbers, so that the order of their sum does not matter
+  double warp_sum[SM_WARPS], scan_mass[SM_WARPS];
+  double total, from;
+  float top[SM_CLUSTER], cut[SM_CLUSTER], warp_top[SM_WARPS];
+  int candidates[SM_CLUSTER];
+  unsigned key_min[SM_CLUSTER], key_max[SM_CLUSTER], ties[SM_CLUSTER], first_id[SM_CLUSTER];
+  unsigned warp_ties[SM_WARPS], scan_count[SM_WARPS];
   unsigned reduce[2];
-  unsigned first_id[SM_CLUSTER];
+  SampleFound found;
+  unsigned border_key;
+  int border_id, list_n, at, owner;
+  union {
+    struct {                            // a list of tokens: key << 32 | ~id, and their weights
+      unsigned long long list[SM_LIST];
+      double w[SM_LIST];
+    };
+    struct {                            // histogram: this CTA's, and in CTA 0 the cluster's
+      unsigned count[SM_BINS], mass_of[SM_BINS];
+      unsigned all_count[SM_BINS], all_high[SM_BINS], all_low[SM_BINS];
+    };
+  };
 };
 
 __device__ __forceinline__ uint32_t sm_at(const void* p, int cta) { return dsmem_addr(smem_u32(p), (uint32_t)cta); }
@@ -59,9 +72,9 @@ __device__ __forceinline__ void push_u32(const void* p, int cta, unsigned v) { a
 __device__ __forceinline__ void push_f64(const void* p, int cta, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(sm_at(p, cta)), "d"(v) : "memory"); }
 __device__ __forceinline__ void push_u64(const void* p, int cta, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(sm_at(p, cta)), "l"(v) : "memory"); }
 __device__ __forceinline__ void push_add(const void* p, int cta, unsigned v) { asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(sm_at(p, cta)), "r"(v) : "memory"); }
-__device__ __forceinline__ unsigned push_next(const void* p, int cta) {
+__device__ __forceinline__ unsigned push_take(const void* p, int cta, unsigned n) {
   unsigned r;
-  asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(r) : "r"(sm_at(p, cta)) : "memory");
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(sm_at(p, cta)), "r"(n) : "memory");
   return r;
 }
 
@@ -72,6 +85,12 @@ template <typename T> __device__ __forceinline__ unsigned key_of(float x);
 template <> __device__ __forceinline__ unsigned key_of<float>(float x) { return order_key(x); }
 template <> __device__ __forceinline__ unsigned key_of<__nv_bfloat16>(float x) { return order_key(__float2bfloat16(x)); }
 
+template <typename T> __device__ __forceinline__ float logit_of(unsigned key);
+template <> __device__ __forceinline__ float logit_of<float>(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+template <> __device__ __forceinline__ float logit_of<__nv_bfloat16>(unsigned key) {
+  return __bfloat162float(__ushort_as_bfloat16((unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key)));
+}
+
 template <typename T> __device__ __forceinline__ void load_vec(const T* p, float* v);
 template <> __device__ __forceinline__ void load_vec<float>(const float* p, float* v) {
   const float4 u = *reinterpret_cast<const float4*>(p);
@@ -79,22 +98,23 @@ template <> __device__ __forceinline__ void load_vec<float>(const float* p, floa
 }
 template <> __device__ __forceinline__ void load_vec<__nv_bfloat16>(const __nv_bfloat16* p, float* v) { load8(p, *reinterpret_cast<float(*)[8]>(v)); }
 
-// 2^x for x <= 0, zero below 2^-1000: table of 2^(i / 64) and the Taylor polynomial of degree 4 for the rest |r| <= 1/128 (Tang, 1989); 4e-14 of the value
-__device__ __forceinline__ double exp2_table(double x, const double* table) {
-  if (!(x > -1000.0)) return 0.0;
-  const double big = 6755399441055744.0 / 64;             // 1.5 * 2^52 / 64: the sum's last bits count 64ths
-  const double s = x + big;
-  const int n = __double2loint(s);
-  const double r = x - (s - big);
-  constexpr double L = 0.693147180559945309417;
-  double p = fma(r, L * L * L * L / 24, L * L * L / 6);
-  p = fma(p, r, L * L / 2);
-  p = fma(p, r, L);
-  p = fma(p, r, 1.0);
-  p *= table[n & 63];
-  return __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
-}
+template <typename T> __device__ __forceinline__ void store_vec(T* p, const float* v);
+template <> __device__ __forceinline__ void store_vec<float>(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+template <> __device__ __forceinline__ void store_vec<__nv_bfloat16>(__nv_bfloat16* p, const float* v) { store8(p, *reinterpret_cast<const float(*)[8]>(v)); }
 
+// 2^x for -1000 < x <= 0: table of 2^(i / 256) and the Taylor polynomial of degree 3 for the rest |r| <= 1/512 (Tang, 1989); 1.4e-13 of the value
+__device__ __forceinline__ double exp2_table(double x, const double* table) {
+  constexpr double BIG = 6755399441055744.0 / 256;        // 1.5 * 2^52 / 256: the sum's last bits count 256ths
+  const double s = x + BIG;
+  const int n = __double2loint(s);
+  const double r = x - (s - BIG);
+  constexpr double L = 0.693147180559945309417;
+  double p = fma(r, L * L * L / 6, L * L / 2);
+  p = fma(p, r, L);
+  const double t = table[n & 255];
+  p = fma(p * r, t, t);
+  return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+}
 __device__ __forceinline__ double power_of_2(int n) { return __hiloint2double((1023 + n) << 20, 0); }      // -1022 <= n <= 1023
 
 __device__ __forceinline__ double warp_sum64(double v) {
@@ -113,26 +133,114 @@ __device__ __forceinline__ unsigned warp_scan_u32(unsigned v, int lane) {
   return v;
 }
 
-// A row as a CTA sees it: weights and bins of its logits.
+// a float as a double by moving its fields: a conversion takes four times as long as a sum. Zero becomes 6e-39, infinity 2^128.
+__device__ __forceinline__ double widen(float x) {
+  const unsigned b = __float_as_uint(x);
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
+__device__ __forceinline__ float ex2_approx(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// A row as a CTA sees it: weights and bins of its logits. The largest logit is finite (rows with +inf are rewritten first).
 struct SampleRow {
   float top;                            // the largest logit
-  double c;                             // log2(e) / T
+  double c, wide_top;                   // log2(e) / T
+  float ch, cl;                         // c in two words
   float bins;                           // bins per unit of logit
   const double* table;
+  // zero below 2^-1000
   __device__ __forceinline__ double weight(float l) const {
-    if (top == INFINITY) return l == INFINITY ? 1.0 : 0.0;
-    return l == -INFINITY ? 0.0 : exp2_table(((double)l - (double)top) * c, table);
+    const double x = (widen(l) - wide_top) * c;
+    return l > -INFINITY && x > -1000.0 ? exp2_table(x, table) : 0.0;
   }
+  // octaves of a logit against the largest
+  __device__ __forceinline__ float octaves(float l) const { return (l - top) * ch; }
   // never falls as l does: a difference and a product with a positive factor, each rounded, are monotone
   __device__ __forceinline__ int bin(float l) const {
-    if (top == INFINITY) return l == INFINITY ? 0 : SM_BINS - 1;
     const float x = (top - l) * bins;
     return x < (float)(SM_BINS - 1) ? (int)x : SM_BINS - 1;
   }
 };
 
+// Sum over the block's threads in front of this one; `all`: over all of them. Every thread calls.
+__device__ __forceinline__ double block_scan(double v, SampleShared& sh, int warp, int lane, double& all) {
+  const double in = warp_scan64(v, lane);
+  __syncthreads();
+  if (lane == 31) sh.scan_mass[warp] = in;
+  __syncthreads();
+  double before = in - v;
+  all = 0.0;
+#pragma unroll
+  for (int w = 0; w < SM_WARPS; ++w) { const double m = sh.scan_mass[w]; if (w < warp) before += m; all += m; }
+  return before;
+}
+
+// list[0 .. n2) in descending order, n2 a power of two
+__device__ __forceinline__ void sort_down(unsigned long long* list, int n2, int tid) {
+  for (int size = 2; size <= n2; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int i = tid; i < n2 / 2; i += SM_THREADS) {
+        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
+        const unsigned long long x = list[a], y = list[b];
+        if ((x < y) == ((a & size) == 0)) { list[a] = y; list[b] = x; }
+      }
+      // pairs up to 32 apart lie within a warp's own 64 entries
+      if (stride > 32 || (stride == 1 && size >= 64)) __syncthreads(); else __syncwarp();
+    }
+  __syncthreads();
+}
+
+// list[0 .. n) in descending order, entries distinct
+__device__ __forceinline__ void sort_list(SampleShared& sh, int n, int tid) {
+  int n2 = 1;
+  while (n2 < n) n2 <<= 1;
+  if (n2 <= SM_SMALL) {
+    // every entry counts the larger ones, several threads per entry
+    const int per = min(SM_THREADS / n2, 32), i = tid / per, at = tid % per;
+    const unsigned long long me = i < n ? sh.list[i] : 0;
+    int place = 0;
+    if (i < n) for (int j = at; j < n; j += per) place += sh.list[j] > me;
+    for (int o = per >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    __syncthreads();
+    if (i < n && at == 0) sh.list[place] = me;
+    __syncthreads();
+    return;
+  }
+  for (int i = n + tid; i < n2; i += SM_THREADS) sh.list[i] = 0;
+  __syncthreads();
+  sort_down(sh.list, n2, tid);
+}
+
+// The list's n tokens (n <= SM_LIST) in the order's order, with their weights; then the first of them at which the prefix ends: `above` tokens of mass
+// `mass_above` stand in front of the list. Returns how many of the list are kept, and their mass with mass_above in sh.total.
 template <typename T>
-__global__ void __launch_bounds__(SM_THREADS)
+__device__ __forceinline__ int find_border(SampleShared& sh, const SampleRow& r, int n, unsigned above, double mass_above, bool use_k, int k, bool use_p, double target,
+                                           int tid, int warp, int lane) {
+  if (tid == 0) sh.at = n - 1;
+  __syncthreads();
+  sort_list(sh, n, tid);
+  const int per = (n + SM_THREADS - 1) / SM_THREADS, first = min(n, tid * per), last = min(n, first + per);
+  double mine = 0.0;
+  for (int i = first; i < last; ++i) { const double w = r.weight(logit_of<T>((unsigned)(sh.list[i] >> 32))); sh.w[i] = w; mine += w; }
+  double all;
+  double m = mass_above + block_scan(mine, sh, warp, lane, all);
+  const double from = m;
+  for (int i = first; i < last; ++i) {
+    m += sh.w[i];
+    if ((use_k && above + i + 1 >= (unsigned)k) || (use_p && m >= target)) { atomicMin(&sh.at, i); break; }
+  }
+  __syncthreads();
+  const int at = sh.at;
+  if (at >= first && at < last) {
+    m = from;
+    for (int i = first; i <= at; ++i) m += sh.w[i];
+    sh.total = m;
+  }
+  __syncthreads();
+  return at + 1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SM_THREADS, 2)
 sample_tokens_kernel(const SampleArgs a) {
   constexpr int VEC = 16 / sizeof(T), STEP = 32 * VEC;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -146,60 +254,69 @@ sample_tokens_kernel(const SampleArgs a) {
   const int id0 = first + warp * a.seg;
   cluster_arrive_relaxed();                              // "this CTA runs": waited on before the first store into a peer
   pdl_trigger();
-  if (tid < SM_TABLE) sh.table[tid] = exp2(tid / 64.0);
-  for (int i = tid; i < SM_BINS; i += SM_THREADS) { sh.all_count[i] = 0; sh.all_high[i] = 0; sh.all_low[i] = 0; }
+  if (tid < SM_TABLE) sh.table[tid] = exp2(tid / 256.0);
   if (tid == 0) sh.list_n = 0;
   pdl_wait();
+  const float temp = a.temperature[row];
+  const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+  const float p = a.top_p != nullptr ? a.top_p[row] : 1.f, floor_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
+  float u = a.uniforms[row];
+  u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+  auto answer = [&](int id, float prob) { a.ids[row] = id; if (a.probs != nullptr) a.probs[row] = prob; };
 
-  // ---- logits into shared memory, their largest ----
-  float top = -INFINITY;
+  // ---- 1: logits into shared memory, their largest. Four loads of a thread are on their way at a time ----
+  float mine_top = -INFINITY;                            // of this thread's tokens
   const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-  for (int i = lane * VEC; i < a.seg; i += STEP) {
-    float v[VEC];
-    const int at = warp * a.seg + i;
-    if (vec && at + VEC <= have) {
-      load_vec<T>(src + at, v);
-    } else {
+  for (int i0 = lane * VEC; i0 < a.seg; i0 += 4 * STEP) {
+    float v[4][VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = at + e < have ? to_float(src[at + e]) : -INFINITY;
+    for (int g = 0; g < 4; ++g) {
+      const int i = i0 + g * STEP, at = warp * a.seg + i;
+      if (i < a.seg && vec && at + VEC <= have) {
+        load_vec<T>(src + at, v[g]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[g][e] = i < a.seg && at + e < have ? to_float(src[at + e]) : -INFINITY;
+      }
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (v[e] != v[e]) v[e] = -INFINITY;
-      from_float(mine + i + e, v[e]);
-      top = fmaxf(top, v[e]);
+    for (int g = 0; g < 4; ++g) {
+      const int i = i0 + g * STEP;
+      if (i >= a.seg) break;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) { if (v[g][e] != v[g][e]) v[g][e] = -INFINITY; mine_top = fmaxf(mine_top, v[g][e]); }
+      store_vec<T>(mine + i, v[g]);
     }
   }
-  top = warp_max(top);
-  if (lane == 0) sh.warp_sum[warp] = top;
+  {
+    const float m = warp_max(mine_top);
+    if (lane == 0) sh.warp_top[warp] = m;
+  }
   __syncwarp();
   cluster_wait();
   __syncthreads();
   if (tid < C) {
-    double m = sh.warp_sum[0];
-    for (int w = 1; w < SM_WARPS; ++w) m = fmax(m, sh.warp_sum[w]);
-    push_f64(&sh.gather[0][rank], tid, m);
+    float m = sh.warp_top[0];
+    for (int w = 1; w < SM_WARPS; ++w) m = fmaxf(m, sh.warp_top[w]);
+    push_u32(&sh.top[rank], tid, __float_as_uint(m));
   }
   cluster_sync_all();
   SampleRow r;
   r.table = sh.table;
-  {
-    double m = sh.gather[0][0];
-    for (int i = 1; i < C; ++i) m = fmax(m, sh.gather[0][i]);
-    r.top = (float)m;
-  }
-  const float temp = a.temperature[row];
+  r.top = sh.top[0];
+  for (int i = 1; i < C; ++i) r.top = fmaxf(r.top, sh.top[i]);
   const bool greedy = !(temp > 0.f);
   if (greedy || r.top == -INFINITY) {
     // the lowest id of the largest logit
     unsigned best = 0xffffffffu;
-    for (int i = lane * VEC; i < a.seg; i += STEP) {
-      float v[VEC];
-      load_vec<T>(mine + i, v);
+    if (mine_top == r.top)
+      for (int i = lane * VEC; i < a.seg; i += STEP) {
+        float v[VEC];
+        load_vec<T>(mine + i, v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (v[e] == r.top) best = min(best, (unsigned)(id0 + i + e));
-    }
+        for (int e = 0; e < VEC; ++e)
+          if (v[e] == r.top) best = min(best, (unsigned)(id0 + i + e));
+      }
     best = __reduce_min_sync(0xffffffffu, best);
     if (lane == 0) sh.warp_ties[warp] = best;
     __syncthreads();
@@ -211,342 +328,480 @@ sample_tokens_kernel(const SampleArgs a) {
     if (rank == 0 && tid == 0) {
       for (int i = 0; i < C; ++i) best = min(best, sh.first_id[i]);
       const bool none = r.top == -INFINITY;
-      a.ids[row] = none ? 0 : (int)best;
-      if (a.probs != nullptr) a.probs[row] = none ? 0.f : 1.f;
+      answer(none ? 0 : (int)best, none ? 0.f : 1.f);
     }
     return;
   }
+  if (r.top == INFINITY) {
+    // +inf stands for equal finite logits above all others'
+    for (int i = lane * VEC; i < a.seg; i += STEP)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) from_float(mine + i + e, to_float(mine[i + e]) == INFINITY ? 0.f : -INFINITY);
+    mine_top = mine_top == INFINITY ? 0.f : -INFINITY;
+    r.top = 0.f;
+  }
+  r.wide_top = widen(r.top);
   r.c = 1.4426950408889634074 / (double)temp;
+  r.ch = fminf((float)r.c, 1e30f);
+  r.cl = r.c < 1e30 ? (float)(r.c - (double)r.ch) : 0.f;
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
-  const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-  const float p = a.top_p != nullptr ? a.top_p[row] : 1.f, floor_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
   // min-p as a logit: rounded up, so that for 32-bit logits the comparison is the one with the unrounded value
   float least = -INFINITY;
-  if (floor_p > 0.f && temp < INFINITY) least = r.top == INFINITY ? INFINITY : fminf(r.top, __double2float_ru((double)r.top + (double)temp * log((double)fminf(floor_p, 1.f))));
+  if (floor_p > 0.f && temp < INFINITY) least = fminf(r.top, __double2float_ru((double)r.top + (double)temp * log((double)fminf(floor_p, 1.f))));
 
-  // kept: key > border_key, or equal and id <= border_id
-  unsigned border_key = 0;
-  int border_id = 0x7fffffff;
-  double target = 0.0;
-  float cut = least;
-  if (use_p) {
-    double s = 0.0;
-    for (int i = lane * VEC; i < a.seg; i += STEP) {
+  // The warp that holds the draw: the lowest of its ids at which the sum of kept weights, `from` in front of the warp, passes the goal.
+  auto walk = [&](double from, double goal, unsigned border_key, int border_id, double kept_all) {
+    int pick = -1, spare = -1;
+    double pick_w = 0.0, spare_w = 0.0;
+    for (int i0 = 0; i0 < a.seg && pick < 0; i0 += STEP) {
+      const int i = i0 + lane * VEC;
       float v[VEC];
       load_vec<T>(mine + i, v);
+      double w[VEC], sum = 0.0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s += r.weight(v[e]);
+      for (int e = 0; e < VEC; ++e) {
+        const unsigned key = key_of<T>(v[e]);
+        const bool kept = v[e] >= least && (key > border_key || (key == border_key && id0 + i + e <= border_id));
+        w[e] = kept ? r.weight(v[e]) : 0.0;
+        sum += w[e];
+      }
+      const double upto = warp_scan64(sum, lane);
+      double x = from + (upto - sum);
+      int got = -1, some = -1;
+      double got_w = 0.0, some_w = 0.0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        x += w[e];
+        if (w[e] > 0.0) {
+          some = id0 + i + e; some_w = w[e];
+          if (got < 0 && x > goal) { got = some; got_w = w[e]; }
+        }
+      }
+      const unsigned vote = __ballot_sync(0xffffffffu, got >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
+      if (vote) {
+        pick = __shfl_sync(0xffffffffu, got, __ffs(vote) - 1);
+        pick_w = __shfl_sync(0xffffffffu, got_w, __ffs(vote) - 1);
+      }
+      if (any) {
+        spare = __shfl_sync(0xffffffffu, some, 31 - __clz(any));
+        spare_w = __shfl_sync(0xffffffffu, some_w, 31 - __clz(any));
+      }
+      from += __shfl_sync(0xffffffffu, upto, 31);
     }
-    s = warp_sum64(s);
+    if (pick < 0) { pick = spare; pick_w = spare_w; }    // the sums' last bits left the goal behind the last token
+    if (lane == 0) answer(pick, (float)(pick_w / kept_all));
+  };
+
+  // ---- 2: the mass, and a logit that k tokens reach ----
+  float my_cut = INFINITY;
+  if (use_k) {
+    const int k_here = (int)(((long long)k * have + a.V - 1) / a.V);          // in proportion to the slice: k in all, or more
+    if (k_here > 0) {
+      // Of the threads' largest logits, by bins of 1/4 octave: those down to the bin in which the k_here-th lies are k_here at least.
+      if (tid < 256) sh.count[tid] = 0;
+      if (tid == 0) { sh.at = -1; sh.reduce[0] = 0xffffffffu; }
+      __syncthreads();
+      const int b = mine_top > -INFINITY ? min(r.bin(mine_top) >> 2, 255) : 256;
+      if (b < 256) atomicAdd(&sh.count[b], 1u);
+      __syncthreads();
+      if (warp == 0) {
+        unsigned c[8], sum = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { c[q] = sh.count[lane * 8 + q]; sum += c[q]; }
+        unsigned at = warp_scan_u32(sum, lane) - sum;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { if (at < (unsigned)k_here && at + c[q] >= (unsigned)k_here) sh.at = lane * 8 + q; at += c[q]; }
+      }
+      __syncthreads();
+      const unsigned key = __reduce_min_sync(0xffffffffu, b <= sh.at ? order_key(mine_top) : 0xffffffffu);
+      if (lane == 0) atomicMin(&sh.reduce[0], key);
+      __syncthreads();
+      my_cut = sh.at < 0 ? -INFINITY : logit_of<float>(sh.reduce[0]);
+    }
+  }
+  if (use_p || !use_k) {
+    double s = 0.0;
+    float tail = 0.f;
+    const float from = use_p ? -INFINITY : least;        // the draw's mass is that of the kept tokens
+    const float lean = 0.69314718f * r.cl;               // what the first word of c leaves out
+    if (mine_top >= from && r.octaves(mine_top) > SM_FAR)
+      for (int i = lane * VEC; i < a.seg; i += STEP) {
+        float v[VEC];
+        load_vec<T>(mine + i, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float d = v[e] - r.top, x = v[e] >= from ? d * r.ch : -INFINITY;
+          if (x > SM_NEAR) s += exp2_table((widen(v[e]) - r.wide_top) * r.c, sh.table);
+          else if (x > SM_FAR) tail = fmaf(ex2_approx(x), fmaf(lean, d, 1.f), tail);
+        }
+      }
+    s = warp_sum64(s + (double)tail);
     if (lane == 0) sh.warp_sum[warp] = s;
-    __syncthreads();
-    if (tid < C) {
-      s = sh.warp_sum[0];
-      for (int w = 1; w < SM_WARPS; ++w) s += sh.warp_sum[w];
-      push_f64(&sh.gather[1][rank], tid, s);
-    }
-    cluster_sync_all();
-    s = sh.gather[1][0];
-    for (int i = 1; i < C; ++i) s += sh.gather[1][i];
-    target = fmax((double)p, 0.0) * s;
-    if (r.top != INFINITY) {
+  }
+  __syncthreads();
+  if (tid < C) {
+    double s = 0.0;
+    if (use_p || !use_k) for (int w = 0; w < SM_WARPS; ++w) s += sh.warp_sum[w];
+    push_f64(&sh.mass[rank], tid, s);
+    push_u32(&sh.cut[rank], tid, __float_as_uint(my_cut));
+  }
+  cluster_sync_all();
+  double s = 0.0;
+  float k_cut = INFINITY;
+  for (int i = 0; i < C; ++i) { s += sh.mass[i]; k_cut = fminf(k_cut, sh.cut[i]); }
+
+  // kept: key > border_key, or equal and id <= border_id; of those only logits >= least
+  unsigned border_key = 0;
+  int border_id = 0x7fffffff;
+  double kept_all = s;                                   // mass of all kept tokens
+  if (use_k || use_p) {
+    // ---- 3: candidates ----
+    const double target = use_p ? fmax((double)p, 0.0) * s : 0.0;
+    float cut = fmaxf(least, use_k ? k_cut : -INFINITY);
+    if (use_p) {
       // borders lie at weights of (1 - P) S / V and more; a thousandth is left for the roundings
       const double away = log(0.999 * (1.0 - fmax((double)p, 0.0)) * s / a.V) * (double)temp;
       cut = fmaxf(cut, fminf(r.top, __double2float_rd((double)r.top + away)));
     }
-  }
-  if (use_k || use_p) {
-    // ---- the border ----
-    unsigned above = 0;
-    double mass_above = 0.0;
-    unsigned key_lo = 0, key_hi = 0xffffffffu, shift = 0;
-    int bin1 = -1;
-    for (int level = 0;; ++level) {
-      // level 0: bins of (top - l); then the keys within the chosen bin
-      __syncthreads();
-      for (int i = tid; i < SM_BINS; i += SM_THREADS) { sh.count[i] = 0; sh.high[i] = 0; sh.low[i] = 0; }
-      if (tid == 0) { sh.reduce[0] = 0xffffffffu; sh.reduce[1] = 0; }
-      __syncthreads();
-      if (level > 0) {
-        unsigned lo = 0xffffffffu, hi = 0;
-        for (int i = lane * VEC; i < a.seg; i += STEP) {
-          float v[VEC];
-          load_vec<T>(mine + i, v);
+    const bool some = mine_top >= cut && mine_top > -INFINITY;
+    int n = 0;
+    if (some)
+      for (int i = lane * VEC; i < a.seg; i += STEP) {
+        float v[VEC];
+        load_vec<T>(mine + i, v);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const unsigned key = key_of<T>(v[e]);
-            if (v[e] >= cut && r.bin(v[e]) == bin1 && key >= key_lo && key <= key_hi) { lo = min(lo, key); hi = max(hi, key); }
-          }
-        }
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        hi = __reduce_max_sync(0xffffffffu, hi);
-        if (lane == 0) { atomicMin(&sh.reduce[0], lo); atomicMax(&sh.reduce[1], hi); }
-        __syncthreads();
-        if (tid < C) { push_u32(&sh.key_min[rank], tid, sh.reduce[0]); push_u32(&sh.key_max[rank], tid, sh.reduce[1]); }
-        cluster_sync_all();
-        key_lo = sh.key_min[0]; key_hi = sh.key_max[0];
-        for (int i = 1; i < C; ++i) { key_lo = min(key_lo, sh.key_min[i]); key_hi = max(key_hi, sh.key_max[i]); }
-        if (key_lo == key_hi) break;                     // ties of one key
-        shift = 0;
-        while ((key_hi - key_lo) >> shift >= SM_BINS) ++shift;
+        for (int e = 0; e < VEC; ++e) n += v[e] >= cut && v[e] > -INFINITY;
       }
+    const int in_warp = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) sh.scan_count[warp] = in_warp;
+    __syncthreads();
+    int in_cta = 0;
+    for (int w = 0; w < SM_WARPS; ++w) in_cta += sh.scan_count[w];
+    // a CTA with more than its part of the list leaves the row to the general path
+    const int share = SM_LIST / C;
+    if (tid < C) push_u32(&sh.candidates[rank], tid, in_cta);
+    if (in_cta <= share && n > 0) {
+      const unsigned slot0 = push_take(&sh.list_n, 0, n);          // at most SM_LIST in all
+      unsigned slot = slot0;
+      for (int i = lane * VEC; i < a.seg; i += STEP) {
+        float v[VEC];
+        load_vec<T>(mine + i, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (v[e] >= cut && v[e] > -INFINITY) push_u64(&sh.list[slot++], 0, (unsigned long long)key_of<T>(v[e]) << 32 | (unsigned)~(id0 + i + e));
+      }
+    }
+    cluster_sync_all();
+    int all = 0, most = 0;
+    for (int i = 0; i < C; ++i) { all += sh.candidates[i]; most = max(most, sh.candidates[i]); }
+    if (most <= share) {
+      if (rank != 0) return;
+      const int kept = find_border<T>(sh, r, all, 0, 0.0, use_k, k, use_p, target, tid, warp, lane);
+      const double goal = (double)u * sh.total;
+      // the kept ones by id: ~id << 32 | place, descending
+      const int per_thread = (kept + SM_THREADS - 1) / SM_THREADS;
+      unsigned long long hold[SM_LIST / SM_THREADS];
+#pragma unroll
+      for (int q = 0; q < SM_LIST / SM_THREADS; ++q) {
+        const int i = tid + q * SM_THREADS;
+        hold[q] = i < kept ? (sh.list[i] << 32) | (unsigned)i : 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < SM_LIST / SM_THREADS; ++q) { const int i = tid + q * SM_THREADS; if (i < kept) sh.list[i] = hold[q]; }
+      if (tid == 0) { sh.at = 0x7fffffff; sh.list_n = -1; }
+      __syncthreads();
+      sort_list(sh, kept, tid);
+      const int f0 = min(kept, tid * per_thread), f1 = min(kept, f0 + per_thread);
+      double mass = 0.0, total;
+      for (int i = f0; i < f1; ++i) mass += sh.w[(unsigned)sh.list[i]];
+      double m = block_scan(mass, sh, warp, lane, total);
+      int last = -1;
+      for (int i = f0; i < f1; ++i) {
+        const double w = sh.w[(unsigned)sh.list[i]];
+        m += w;
+        if (w > 0.0) { last = i; if (m > goal) { atomicMin(&sh.at, i); break; } }
+      }
+      if (last >= 0) atomicMax(&sh.list_n, last);
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned long long x = sh.list[sh.at == 0x7fffffff ? sh.list_n : sh.at];          // the sums' last bits may leave the goal behind the last token
+        answer((int)~(unsigned)(x >> 32), (float)(sh.w[(unsigned)x] / sh.total));
+      }
+      return;
+    }
+    // ---- 4: the general path ----
+    // the bins divide the range of the candidates, where it is known
+    if (cut > -INFINITY && r.top - cut > 0.f) r.bins = fminf(r.bins * 64.f, (float)(SM_BINS - 1) / (r.top - cut));
+    const float per_bin = r.bins > 0.f ? r.ch / r.bins : 0.f;
+    __syncthreads();
+    for (int i = tid; i < SM_BINS; i += SM_THREADS) { sh.all_count[i] = 0; sh.all_high[i] = 0; sh.all_low[i] = 0; sh.count[i] = 0; sh.mass_of[i] = 0; }
+    if (tid == 0) sh.list_n = 0;
+    cluster_sync_all();                                  // CTA 0's sums are clear, the lists forgotten
+    if (some)
       for (int i = lane * VEC; i < a.seg; i += STEP) {
         float v[VEC];
         load_vec<T>(mine + i, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           if (!(v[e] >= cut) || v[e] == -INFINITY) continue;
-          int b = r.bin(v[e]);
-          const int b1 = b;
-          if (level > 0) {
-            const unsigned key = key_of<T>(v[e]);
-            if (b != bin1 || key < key_lo || key > key_hi) continue;
-            b = (int)((key_hi - key) >> shift);
+          const int b = r.bin(v[e]);
+          if (use_p) {
+            // in units of 2^-14 of the power of two above the bin's weights; 120 octaves and more below the largest weigh nothing
+            const float x = r.octaves(v[e]), up = floorf((float)b * per_bin);
+            if (up < 120.f) atomicAdd(&sh.mass_of[b], (unsigned)__float2int_rn(ex2_approx(x + up) * 16384.f));
           }
           atomicAdd(&sh.count[b], 1u);
-          if (use_p) {
-            // mass in units of 2^-30 of the power of two above the bin's weights
-            const double f = r.weight(v[e]) * power_of_2(30 + (b1 >> 4));
-            const unsigned u = (unsigned)(f + 0.5);
-            atomicAdd(&sh.high[b], u >> 15);
-            atomicAdd(&sh.low[b], u & 32767u);
-          }
         }
+      }
+    __syncthreads();
+    for (int i = tid; i < SM_BINS; i += SM_THREADS)
+      if (sh.count[i]) {
+        push_add(&sh.all_count[i], 0, sh.count[i]);
+        if (use_p) { push_add(&sh.all_high[i], 0, sh.mass_of[i] >> 16); push_add(&sh.all_low[i], 0, sh.mass_of[i] & 0xffffu); }
+      }
+    cluster_sync_all();
+    if (rank == 0) {
+      constexpr int PER = SM_BINS / SM_THREADS;
+      unsigned c[PER], c_sum = 0;
+      double m[PER], m_sum = 0.0;
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const int b = tid * PER + q;
+        const float up = floorf((float)b * per_bin);
+        c[q] = sh.all_count[b];
+        m[q] = use_p && up < 120.f ? ((double)sh.all_high[b] * 65536.0 + (double)sh.all_low[b]) * power_of_2(-14 - (int)up) : 0.0;
+        c_sum += c[q]; m_sum += m[q];
+        sh.all_count[b] = 0; sh.all_high[b] = 0; sh.all_low[b] = 0;
+      }
+      const unsigned c_in = warp_scan_u32(c_sum, lane);
+      if (lane == 31) sh.scan_count[warp] = c_in;
+      if (tid == 0) sh.found = SampleFound{SM_BINS, 0, 0, 0, 0};
+      double m_all;
+      double m_at = block_scan(m_sum, sh, warp, lane, m_all);
+      unsigned c_at = c_in - c_sum;
+      for (int w = 0; w < warp; ++w) c_at += sh.scan_count[w];
+      // The masses are within 1e-4 of themselves: in the first bin behind which the target may be reached, or in a later one up to the first behind which
+      // it surely is, lies the border.
+      const double lo_target = target * (1.0 - 1e-4), hi_target = target * (1.0 + 1e-4);
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const unsigned c_to = c_at + c[q];
+        const double m_to = m_at + m[q];
+        if (c[q]) {
+          const bool maybe = (use_k && c_to >= (unsigned)k) || (use_p && m_to >= lo_target), before = (use_k && c_at >= (unsigned)k) || (use_p && c_at > 0 && m_at >= lo_target);
+          const bool sure = (use_k && c_to >= (unsigned)k) || (use_p && m_to >= hi_target), sure_before = (use_k && c_at >= (unsigned)k) || (use_p && c_at > 0 && m_at >= hi_target);
+          if (maybe && !before) atomicMin(&sh.found.lo, tid * PER + q);
+          if (!sure_before && (sure || maybe)) atomicMax(&sh.found.hi, tid * PER + q);
+        }
+        c_at = c_to; m_at = m_to;
       }
       __syncthreads();
-      for (int i = tid; i < SM_BINS; i += SM_THREADS)
-        if (sh.count[i]) {
-          push_add(&sh.all_count[i], 0, sh.count[i]);
-          if (use_p) {
-            const unsigned long long v = ((unsigned long long)sh.high[i] << 15) + sh.low[i];
-            push_add(&sh.all_high[i], 0, (unsigned)(v >> 24));
-            push_add(&sh.all_low[i], 0, (unsigned)(v & 0xffffffu));
-          }
-        }
-      cluster_sync_all();
-      if (rank == 0) {
-        constexpr int PER = SM_BINS / SM_THREADS;
-        unsigned n[PER], n_sum = 0;
-        double m[PER], m_sum = 0.0;
+      const int lo = sh.found.lo, hi = sh.found.hi;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const int b = tid * PER + j, b1 = level ? bin1 : b;
-          n[j] = sh.all_count[b];
-          m[j] = use_p ? ((double)sh.all_high[b] * 16777216.0 + (double)sh.all_low[b]) * power_of_2(-30 - (b1 >> 4)) : 0.0;
-          n_sum += n[j]; m_sum += m[j];
-          sh.all_count[b] = 0; sh.all_high[b] = 0; sh.all_low[b] = 0;
-        }
-        const unsigned n_in = warp_scan_u32(n_sum, lane);
-        const double m_in = warp_scan64(m_sum, lane);
-        if (lane == 31) { sh.scan_count[warp] = n_in; sh.scan_mass[warp] = m_in; }
-        if (tid == 0) { sh.found.reached = 0; }
-        __syncthreads();
-        unsigned n_at = above + n_in - n_sum;
-        double m_at = mass_above + (m_in - m_sum);
-        for (int w = 0; w < warp; ++w) { n_at += sh.scan_count[w]; m_at += sh.scan_mass[w]; }
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          // the first bin behind which one of the two is reached; divided bins: rounding may leave it to the last of them
-          const bool before = (use_k && n_at >= (unsigned)k) || (use_p && n_at > 0 && m_at >= target);
-          const bool here = (use_k && n_at + n[j] >= (unsigned)k) || (use_p && n[j] > 0 && m_at + m[j] >= target);
-          if (n[j] && here && !before) { sh.found = SampleFound{tid * PER + j, (int)n[j], 1, n_at, m_at}; }
-          n_at += n[j]; m_at += m[j];
-        }
-        __syncthreads();
-        if (tid < C) {
-          const SampleFound f = sh.found;
-          push_u32(&sh.found.bin, tid, (unsigned)f.bin); push_u32(&sh.found.count, tid, (unsigned)f.count);
-          push_u32(&sh.found.reached, tid, (unsigned)f.reached); push_u32(&sh.found.above, tid, f.above);
-          push_f64(&sh.found.mass_above, tid, f.mass_above);
-        }
+      for (int q = PER - 1; q >= 0; --q) {
+        const int b = tid * PER + q;
+        c_at -= c[q];
+        if (b >= lo && b <= hi && c[q]) atomicAdd(&sh.found.count, (int)c[q]);
+        if (b == lo) sh.found.above = c_at;
       }
-      cluster_sync_all();
-      const SampleFound f = sh.found;
-      if (!f.reached) {
-        // level 0: no border among the candidates, min-p alone decides. A divided bin: rounding has left the border behind its last token, so the
-        // whole bin is kept
-        if (level > 0) border_key = key_lo;
-        key_lo = 1; key_hi = 0;                          // nothing left to rank
-        break;
+      __syncthreads();
+      if (tid > 0 && tid < C) {
+        push_u32(&sh.found.lo, tid, (unsigned)lo); push_u32(&sh.found.hi, tid, (unsigned)hi); push_u32(&sh.found.count, tid, (unsigned)sh.found.count);
+        push_u32(&sh.found.above, tid, sh.found.above);
       }
-      above = f.above; mass_above = f.mass_above;
-      if (level == 0) bin1 = f.bin;
-      else { key_hi -= (unsigned)f.bin << shift; key_lo = max(key_lo, key_hi - ((1u << shift) - 1)); }
-      if (f.count <= SM_LIST) break;
     }
-    if (key_lo == key_hi && sh.found.count > SM_LIST) {
-      // ---- ties of one key: as many of the lowest ids as are needed ----
-      unsigned n = 0;
-      for (int i = lane * VEC; i < a.seg; i += STEP) {
-        float v[VEC];
-        load_vec<T>(mine + i, v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) n += key_of<T>(v[e]) == key_lo && v[e] >= cut;
-      }
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == 0) sh.warp_ties[warp] = n;
-      __syncthreads();
-      unsigned in_cta = 0;
-      for (int w = 0; w < SM_WARPS; ++w) in_cta += sh.warp_ties[w];
-      if (tid < C) push_u32(&sh.ties[rank], tid, in_cta);
-      cluster_sync_all();
-      unsigned all = 0, before = 0;
-      for (int i = 0; i < C; ++i) { if (i < rank) before += sh.ties[i]; all += sh.ties[i]; }
-      unsigned want = all;
-      if (use_k) want = min(want, (unsigned)k - above);
-      if (use_p) {
-        const float l = sizeof(T) == 2 ? __bfloat162float(__ushort_as_bfloat16((unsigned short)(key_lo & 0x8000u ? key_lo & 0x7fffu : ~key_lo)))
-                                       : __uint_as_float(key_lo & 0x80000000u ? key_lo & 0x7fffffffu : ~key_lo);
-        const double need = ceil((target - mass_above) / r.weight(l));
-        if (need < (double)want) want = need < 1.0 ? 1u : (unsigned)need;
-      }
-      for (int w = 0; w < warp; ++w) before += sh.warp_ties[w];
-      if (want > before && want <= before + n) {         // this warp holds the last one
-        unsigned at = before;
-        for (int i = lane * VEC; i - lane * VEC < a.seg; i += STEP) {
-          float v[VEC];
-          unsigned here = 0;
-          load_vec<T>(mine + i, v);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) here += key_of<T>(v[e]) == key_lo && v[e] >= cut;
-          const unsigned upto = warp_scan_u32(here, lane);
-          unsigned seen = at + upto - here;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (key_of<T>(v[e]) == key_lo && v[e] >= cut && ++seen == want)
-              for (int t = 0; t < C; ++t) push_u32(&sh.border_id, t, (unsigned)(id0 + i + e));
-          at += __shfl_sync(0xffffffffu, upto, 31);
-        }
-      }
-      cluster_sync_all();
-      border_key = key_lo; border_id = sh.border_id;
-    } else if (key_lo <= key_hi) {
-      // ---- few tokens: ranked one by one in CTA 0 ----
+    cluster_sync_all();
+    // the border's bins; none: all candidates are kept, and lie in front of bin SM_BINS
+    const int lo = sh.found.lo, hi = sh.found.hi;
+    unsigned above = lo < SM_BINS ? sh.found.above : 0u;
+    unsigned key_lo = 0, key_hi = 0xffffffffu;
+    int left = lo < SM_BINS ? sh.found.count : 0;
+    bool ties = false;
+    // bins of too many tokens: their keys are divided by count alone, down to the key up to which k or the list's length lead; masses are met in FP64 below
+    auto inside = [&](float l, unsigned key) { const int b = r.bin(l); return l >= cut && l > -INFINITY && b >= lo && b <= hi && key >= key_lo && key <= key_hi; };
+    double mass_above = 0.0;
+    while (left > SM_LIST) {
+      unsigned kmin = 0xffffffffu, kmax = 0;
       for (int i = lane * VEC; i < a.seg; i += STEP) {
         float v[VEC];
         load_vec<T>(mine + i, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const unsigned key = key_of<T>(v[e]);
-          if (!(v[e] >= cut) || v[e] == -INFINITY || r.bin(v[e]) != bin1 || key < key_lo || key > key_hi) continue;
-          const unsigned slot = push_next(&sh.list_n, 0);
-          if (slot < SM_LIST) {
-            push_u64(&sh.list[slot], 0, (unsigned long long)key << 32 | (unsigned)~(id0 + i + e));
-            push_f64(&sh.list_w[slot], 0, use_p ? r.weight(v[e]) : 0.0);
+          if (inside(v[e], key)) { kmin = min(kmin, key); kmax = max(kmax, key); }
+        }
+      }
+      kmin = __reduce_min_sync(0xffffffffu, kmin);
+      kmax = __reduce_max_sync(0xffffffffu, kmax);
+      __syncthreads();
+      if (tid == 0) { sh.reduce[0] = 0xffffffffu; sh.reduce[1] = 0; }
+      __syncthreads();
+      if (lane == 0) { atomicMin(&sh.reduce[0], kmin); atomicMax(&sh.reduce[1], kmax); }
+      __syncthreads();
+      if (tid < C) { push_u32(&sh.key_min[rank], tid, sh.reduce[0]); push_u32(&sh.key_max[rank], tid, sh.reduce[1]); }
+      cluster_sync_all();
+      key_lo = sh.key_min[0]; key_hi = sh.key_max[0];
+      for (int i = 1; i < C; ++i) { key_lo = min(key_lo, sh.key_min[i]); key_hi = max(key_hi, sh.key_max[i]); }
+      if (key_lo == key_hi) { ties = true; break; }
+      // the upper half of the keys: how many, and what mass with all in front of them
+      const unsigned mid = key_lo + (key_hi - key_lo + 1) / 2;
+      unsigned n_up = 0;
+      double m = 0.0;
+      for (int i = lane * VEC; i < a.seg; i += STEP) {
+        float v[VEC];
+        load_vec<T>(mine + i, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const unsigned key = key_of<T>(v[e]);
+          const bool in = inside(v[e], key);
+          n_up += in && key >= mid;
+          const int b = r.bin(v[e]);
+          if (use_p && v[e] >= cut && v[e] > -INFINITY && (b < lo || (b <= hi && key >= mid))) m += r.weight(v[e]);
+        }
+      }
+      n_up = __reduce_add_sync(0xffffffffu, n_up);
+      m = warp_sum64(m);
+      if (lane == 0) { sh.warp_ties[warp] = n_up; sh.warp_sum[warp] = m; }
+      __syncthreads();
+      if (tid < C) {
+        double t = 0.0;
+        unsigned c = 0;
+        for (int w = 0; w < SM_WARPS; ++w) { t += sh.warp_sum[w]; c += sh.warp_ties[w]; }
+        push_f64(&sh.mass[rank], tid, t);
+        push_u32(&sh.ties[rank], tid, c);
+      }
+      cluster_sync_all();
+      double upper = 0.0;
+      int n_upper = 0;
+      for (int i = 0; i < C; ++i) { upper += sh.mass[i]; n_upper += (int)sh.ties[i]; }
+      // the border lies in the upper half if it is reached there
+      if ((use_k && above + n_upper >= (unsigned)k) || (use_p && n_upper > 0 && upper >= target)) { key_lo = mid; left = n_upper; }
+      else { key_hi = mid - 1; above += n_upper; left -= n_upper; }
+    }
+    // the mass in front of the border's bins (and keys) in FP64, warp by warp; the tokens among which it lies into CTA 0's list
+    double m = 0.0;
+    unsigned n_ties = 0;
+    __syncthreads();                                     // the histogram's place is the list's
+    if (some)
+      for (int i = lane * VEC; i < a.seg; i += STEP) {
+        float v[VEC];
+        load_vec<T>(mine + i, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (!(v[e] >= cut) || v[e] == -INFINITY) continue;
+          const int b = r.bin(v[e]);
+          if (b > hi && lo < SM_BINS) continue;
+          const unsigned key = key_of<T>(v[e]);
+          if (b < lo || key > key_hi) m += r.weight(v[e]);
+          else if (key >= key_lo) {
+            if (ties) ++n_ties;
+            else push_u64(&sh.list[push_take(&sh.list_n, 0, 1)], 0, (unsigned long long)key << 32 | (unsigned)~(id0 + i + e));
           }
         }
       }
-      cluster_sync_all();
-      if (rank == 0) {
-        const int n = min(sh.list_n, SM_LIST);
-        if (tid < n) {
-          const unsigned long long me = sh.list[tid];
-          int at = 0;
-          for (int j = 0; j < n; ++j) at += sh.list[j] > me;
-          sh.sorted[at] = me; sh.sorted_w[at] = sh.list_w[tid];
-        }
-        __syncthreads();
-        double w = tid < n ? sh.sorted_w[tid] : 0.0;
-        const double upto = warp_scan64(w, lane);
-        if (lane == 31) sh.scan_mass[warp] = upto;
-        __syncthreads();
-        double m = mass_above + upto;
-        for (int i = 0; i < warp; ++i) m += sh.scan_mass[i];
-        bool here = tid < n && ((use_k && above + tid + 1 >= (unsigned)k) || (use_p && m >= target));
-        here = here || tid == n - 1;
-        // the first of them
-        const unsigned vote = __ballot_sync(0xffffffffu, here);
-        if (lane == 0) sh.scan_count[warp] = vote ? (unsigned)(warp * 32 + __ffs(vote) - 1) : 0xffffffffu;
-        __syncthreads();
-        if (tid < C) {
-          unsigned at = 0xffffffffu;
-          for (int i = 0; i < SM_WARPS; ++i) at = min(at, sh.scan_count[i]);
-          const unsigned long long border = sh.sorted[at];
-          push_u32(&sh.border_key, tid, (unsigned)(border >> 32));
-          push_u32(&sh.border_id, tid, ~(unsigned)border);
+    m = warp_sum64(m);
+    n_ties = __reduce_add_sync(0xffffffffu, n_ties);
+    if (lane == 0) {
+      sh.warp_sum[warp] = m; sh.warp_ties[warp] = n_ties;
+      push_f64(&sh.part[rank * SM_WARPS + warp], 0, m);
+    }
+    __syncthreads();
+    if (tid < C) {
+      unsigned c = 0;
+      for (int w = 0; w < SM_WARPS; ++w) c += sh.warp_ties[w];
+      push_u32(&sh.ties[rank], tid, c);
+      if (ties) { double t = 0.0; for (int w = 0; w < SM_WARPS; ++w) t += sh.warp_sum[w]; push_f64(&sh.mass[rank], tid, t); }
+    }
+    cluster_sync_all();
+    if (ties) {
+      // ---- ties of one key: as many of the lowest ids as are needed ----
+      const double w_tie = r.weight(logit_of<T>(key_lo));
+      unsigned all_ties = 0, before = 0;
+      for (int i = 0; i < C; ++i) { if (i < rank) before += sh.ties[i]; all_ties += sh.ties[i]; mass_above += sh.mass[i]; }
+      unsigned want = all_ties;
+      if (use_k) want = min(want, (unsigned)k - above);
+      if (use_p) {
+        const double need = ceil((target - mass_above) / w_tie);
+        if (need < (double)want) want = need < 1.0 ? 1u : (unsigned)need;
+      }
+      for (int w = 0; w < warp; ++w) before += sh.warp_ties[w];
+      const unsigned taken = want <= before ? 0u : min(want - before, n_ties);
+      if (lane == 0) push_f64(&sh.part[rank * SM_WARPS + warp], 0, m + (double)taken * w_tie);
+      if (want > before && want <= before + n_ties) {    // this warp holds the last one
+        unsigned at = before;
+        for (int i = lane * VEC; i - lane * VEC < a.seg; i += STEP) {
+          float v[VEC];
+          unsigned here = 0;
+          load_vec<T>(mine + i, v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) here += inside(v[e], key_of<T>(v[e]));
+          const unsigned upto = warp_scan_u32(here, lane);
+          unsigned seen = at + upto - here;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (inside(v[e], key_of<T>(v[e])) && ++seen == want) push_u32(&sh.border_id, 0, (unsigned)(id0 + i + e));
+          at += __shfl_sync(0xffffffffu, upto, 31);
         }
       }
       cluster_sync_all();
-      border_key = sh.border_key; border_id = sh.border_id;
     }
+    if (rank == 0) {
+      // the border, every warp's kept mass, and whose the draw is
+      if (!ties && left > 0) {
+        double front = 0.0;
+        for (int i = tid; i < C * SM_WARPS; i += SM_THREADS) front += sh.part[i];
+        block_scan(front, sh, warp, lane, mass_above);
+        const int kept = find_border<T>(sh, r, left, above, mass_above, use_k, k, use_p, target, tid, warp, lane);
+        if (tid < SM_PARTS) sh.part_in[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < kept; i += SM_THREADS) atomicAdd(&sh.part_in[(int)~(unsigned)sh.list[i] / a.seg], (unsigned long long)(sh.w[i] * 1125899906842624.0));
+        __syncthreads();
+        if (tid < C * SM_WARPS) sh.part[tid] += (double)sh.part_in[tid] * (1.0 / 1125899906842624.0);
+        if (tid == 0) { sh.border_key = (unsigned)(sh.list[kept - 1] >> 32); sh.border_id = (int)~(unsigned)sh.list[kept - 1]; }
+      } else if (tid == 0) {
+        sh.border_key = ties ? key_lo : 0u;
+        if (!ties) sh.border_id = 0x7fffffff;
+      }
+      __syncthreads();
+      const double mine_part = tid < C * SM_WARPS ? sh.part[tid] : 0.0;
+      double all_parts;
+      const double from = block_scan(mine_part, sh, warp, lane, all_parts);
+      const double goal = (double)u * all_parts;
+      if (tid == 0) { sh.total = all_parts; sh.owner = -1; sh.at = -1; }
+      __syncthreads();
+      if (mine_part > 0.0) { atomicMax(&sh.owner, from <= goal ? tid : -1); }
+      __syncthreads();
+      const int owner = sh.owner;
+      if (tid == owner) sh.from = from;
+      __syncthreads();
+      if (tid > 0 && tid < C) {
+        push_u32(&sh.owner, tid, (unsigned)owner); push_u32(&sh.border_key, tid, sh.border_key); push_u32(&sh.border_id, tid, (unsigned)sh.border_id);
+        push_f64(&sh.from, tid, sh.from); push_f64(&sh.total, tid, sh.total);
+      }
+    }
+    cluster_sync_all();
+    border_key = sh.border_key; border_id = sh.border_id;
+    kept_all = sh.total;
+    if (sh.owner != rank * SM_WARPS + warp) return;
+    walk(sh.from, (double)u * kept_all, border_key, border_id, kept_all);
+    return;
   }
 
-  // ---- sums of the kept weights, and the draw ----
-  auto kept = [&](float l, int id) {
-    const unsigned key = key_of<T>(l);
-    return l >= least && (key > border_key || (key == border_key && id <= border_id));
-  };
-  double s = 0.0;
-  for (int i = lane * VEC; i < a.seg; i += STEP) {
-    float v[VEC];
-    load_vec<T>(mine + i, v);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (kept(v[e], id0 + i + e)) s += r.weight(v[e]);
-  }
-  s = warp_sum64(s);
-  __syncthreads();
-  if (lane == 0) sh.warp_sum[warp] = s;
-  __syncthreads();
-  if (tid < C) {
-    double t = sh.warp_sum[0];
-    for (int w = 1; w < SM_WARPS; ++w) t += sh.warp_sum[w];
-    push_f64(&sh.gather[2][rank], tid, t);
-  }
-  cluster_sync_all();
-  double all = 0.0, before = 0.0;
+  // ---- 3, without top-k and top-p: the draw from the warps' masses ----
+  double before = 0.0, all = 0.0;
   int last = 0;                                          // the last CTA that holds any of the mass
-  for (int i = 0; i < C; ++i) { if (i == rank) before = all; all += sh.gather[2][i]; if (sh.gather[2][i] > 0.0) last = i; }
-  float u = a.uniforms[row];
-  u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
-  const double goal = (double)u * all;
-  double after = before + sh.gather[2][rank];
-  if (!(goal >= before && (goal < after || rank == last) && sh.gather[2][rank] > 0.0)) return;
+  for (int i = 0; i < C; ++i) { if (i == rank) before = all; all += sh.mass[i]; if (sh.mass[i] > 0.0) last = i; }
+  const double goal = (double)u * all, after = before + sh.mass[rank];
+  if (!(goal >= before && (goal < after || rank == last) && sh.mass[rank] > 0.0)) return;
   // this CTA has it: the warp, then the token
   int last_warp = 0;
   double at = before, from = before;
   for (int w = 0; w < SM_WARPS; ++w) { if (w == warp) from = at; at += sh.warp_sum[w]; if (sh.warp_sum[w] > 0.0) last_warp = w; }
   const double mass = sh.warp_sum[warp];
-  // the warps' ends as every warp computes them: from + mass is the next one's `from`
   if (!(mass > 0.0 && goal >= from && (goal < from + mass || warp == last_warp))) return;
-  int pick = -1, spare = -1;
-  double pick_w = 0.0, spare_w = 0.0;
-  for (int i0 = 0; i0 < a.seg && pick < 0; i0 += STEP) {
-    const int i = i0 + lane * VEC;
-    float v[VEC];
-    load_vec<T>(mine + i, v);
-    double w[VEC], sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) { w[e] = kept(v[e], id0 + i + e) ? r.weight(v[e]) : 0.0; sum += w[e]; }
-    const double upto = warp_scan64(sum, lane);
-    double x = from + (upto - sum);
-    int got = -1, some = -1;
-    double got_w = 0.0, some_w = 0.0;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      x += w[e];
-      if (w[e] > 0.0) {
-        some = id0 + i + e; some_w = w[e];
-        if (got < 0 && x > goal) { got = some; got_w = w[e]; }
-      }
-    }
-    const unsigned vote = __ballot_sync(0xffffffffu, got >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
-    if (vote) {
-      pick = __shfl_sync(0xffffffffu, got, __ffs(vote) - 1);
-      pick_w = __shfl_sync(0xffffffffu, got_w, __ffs(vote) - 1);
-    }
-    if (any) {
-      spare = __shfl_sync(0xffffffffu, some, 31 - __clz(any));
-      spare_w = __shfl_sync(0xffffffffu, some_w, 31 - __clz(any));
-    }
-    from += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  if (pick < 0) { pick = spare; pick_w = spare_w; }      // the sums' last bits left the goal behind the last token
-  if (lane == 0) {
-    a.ids[row] = pick;
-    if (a.probs != nullptr) a.probs[row] = (float)(pick_w / all);
-  }
+  walk(from, goal, border_key, border_id, kept_all);
 }
 
 }  // namespace ff
@@ -557,8 +812,9 @@ static int sample_launch(const SampleArgs& args, int rows, cudaStream_t stream) 
   constexpr int STEP = 32 * (16 / (int)sizeof(T)), MOST = 227 * 1024;
   const int fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16;
   SampleArgs a = args;
-  int c = 8;
-  while (c > 1 && (long long)rows * c > 444 && (long long)(a.V + c / 2 - 1) / (c / 2) * sizeof(T) + fixed + 16 * STEP * sizeof(T) <= MOST) c /= 2;
+  auto fits = [&](int n) { return (long long)((a.V + n * SM_WARPS - 1) / (n * SM_WARPS) + STEP) * SM_WARPS * sizeof(T) + fixed <= MOST; };
+  int c = SM_CLUSTER;
+  while (c > 1 && (a.V < 4096 * c || rows * c > 2 * sm_count()) && fits(c / 2)) c /= 2;
   a.seg = (a.V + c * SM_WARPS - 1) / (c * SM_WARPS);
   a.seg = (a.seg + STEP - 1) / STEP * STEP;
   const long long smem = fixed + (long long)SM_WARPS * a.seg * sizeof(T);
