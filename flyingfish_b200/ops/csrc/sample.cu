@@ -16,7 +16,7 @@
 //     mass) and min-p -- go to CTA 0, which sorts them, finds the border, sorts the kept ones by id and draws;
 //   4 more than SM_LIST candidates (flat rows): a histogram of the candidates' logits, masses in 14 bits, says in which bin the border lies, or two if it
 //     cannot tell; the mass above is summed in FP64 and the bin's tokens are sorted as in 3. A bin of more tokens is divided by key, ties of one key go by
-//     id. CTA 0 finds the warp that holds the draw, and that warp the token.
+//     id. CTA 0 finds the warp whose run holds the draw, and that warp's CTA the token.
 //
 // NaN counts as -inf, -inf is never drawn, +inf shares everything among its equals; a row without anything gives id 0 with probability 0.
 #include "dtype_io.cuh"
@@ -55,6 +55,7 @@ struct SampleShared {
   SampleFound found;
   unsigned border_key;
   int border_id, list_n, at, owner;
+  double step_sum[32];                  // mass of each step of the run that holds the draw
   union {
     struct {                            // a list of tokens: key << 32 | ~id, and their weights
       unsigned long long list[SM_LIST];
@@ -350,47 +351,54 @@ sample_tokens_kernel(const SampleArgs a) {
   float least = -INFINITY;
   if (floor_p > 0.f && temp < INFINITY) least = fminf(r.top, __double2float_ru((double)r.top + (double)temp * log((double)fminf(floor_p, 1.f))));
 
-  // The warp that holds the draw: the lowest of its ids at which the sum of kept weights, `from` in front of the warp, passes the goal.
-  auto walk = [&](double from, double goal, unsigned border_key, int border_id, double kept_all) {
-    int pick = -1, spare = -1;
-    double pick_w = 0.0, spare_w = 0.0;
-    for (int i0 = 0; i0 < a.seg && pick < 0; i0 += STEP) {
-      const int i = i0 + lane * VEC;
+  // The draw within the run of ids of warp `owner` of this CTA, by all of its warps: the lowest id at which the sum of kept weights, `from` in front of
+  // the run, passes the goal. Shared memory holds runs of 28 steps at most; their sums first, then the step's tokens (48 rows of 128256: 30 us, 38 where
+  // one warp walks step by step).
+  auto walk = [&](int owner, double from, double goal, unsigned border_key, int border_id, double kept_all) {
+    const T* run = slice + owner * a.seg;
+    const int run_id = first + owner * a.seg, steps = a.seg / STEP;
+    auto weigh = [&](int step, double (&w)[VEC]) {
+      const int i = step * STEP + lane * VEC;
       float v[VEC];
-      load_vec<T>(mine + i, v);
-      double w[VEC], sum = 0.0;
+      load_vec<T>(run + i, v);
+      double sum = 0.0;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const unsigned key = key_of<T>(v[e]);
-        const bool kept = v[e] >= least && (key > border_key || (key == border_key && id0 + i + e <= border_id));
+        const bool kept = v[e] >= least && (key > border_key || (key == border_key && run_id + i + e <= border_id));
         w[e] = kept ? r.weight(v[e]) : 0.0;
         sum += w[e];
       }
-      const double upto = warp_scan64(sum, lane);
-      double x = from + (upto - sum);
-      int got = -1, some = -1;
-      double got_w = 0.0, some_w = 0.0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        x += w[e];
-        if (w[e] > 0.0) {
-          some = id0 + i + e; some_w = w[e];
-          if (got < 0 && x > goal) { got = some; got_w = w[e]; }
-        }
-      }
-      const unsigned vote = __ballot_sync(0xffffffffu, got >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
-      if (vote) {
-        pick = __shfl_sync(0xffffffffu, got, __ffs(vote) - 1);
-        pick_w = __shfl_sync(0xffffffffu, got_w, __ffs(vote) - 1);
-      }
-      if (any) {
-        spare = __shfl_sync(0xffffffffu, some, 31 - __clz(any));
-        spare_w = __shfl_sync(0xffffffffu, some_w, 31 - __clz(any));
-      }
-      from += __shfl_sync(0xffffffffu, upto, 31);
+      return sum;
+    };
+    double w[VEC];
+    for (int step = warp; step < steps; step += SM_WARPS) {
+      const double sum = warp_sum64(weigh(step, w));
+      if (lane == 0) sh.step_sum[step] = sum;
     }
-    if (pick < 0) { pick = spare; pick_w = spare_w; }    // the sums' last bits left the goal behind the last token
-    if (lane == 0) answer(pick, (float)(pick_w / kept_all));
+    __syncthreads();
+    if (warp != 0) return;
+    const double mine_sum = lane < steps ? sh.step_sum[lane] : 0.0, upto_step = warp_scan64(mine_sum, lane);
+    const unsigned starts = __ballot_sync(0xffffffffu, mine_sum > 0.0 && from + (upto_step - mine_sum) <= goal);
+    const unsigned any_step = __ballot_sync(0xffffffffu, mine_sum > 0.0);
+    const int step = starts ? 31 - __clz(starts) : __ffs(any_step) - 1;
+    const double before = from + __shfl_sync(0xffffffffu, upto_step - mine_sum, step);
+    const double sum = weigh(step, w);
+    const double upto = warp_scan64(sum, lane);
+    double x = before + (upto - sum);
+    int got = -1, some = -1;
+    double got_w = 0.0, some_w = 0.0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      x += w[e];
+      if (w[e] > 0.0) {
+        some = run_id + step * STEP + lane * VEC + e; some_w = w[e];
+        if (got < 0 && x > goal) { got = some; got_w = w[e]; }
+      }
+    }
+    // the first that passes; the sums' last bits may leave the goal behind the last token
+    const unsigned vote = __ballot_sync(0xffffffffu, got >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
+    if (vote ? lane == __ffs(vote) - 1 : lane == 31 - __clz(any)) answer(vote ? got : some, (float)((vote ? got_w : some_w) / kept_all));
   };
 
   // ---- 2: the mass, and a logit that k tokens reach ----
@@ -784,8 +792,8 @@ sample_tokens_kernel(const SampleArgs a) {
     cluster_sync_all();
     border_key = sh.border_key; border_id = sh.border_id;
     kept_all = sh.total;
-    if (sh.owner != rank * SM_WARPS + warp) return;
-    walk(sh.from, (double)u * kept_all, border_key, border_id, kept_all);
+    if (sh.owner / SM_WARPS != rank) return;
+    walk(sh.owner % SM_WARPS, sh.from, (double)u * kept_all, border_key, border_id, kept_all);
     return;
   }
 
@@ -796,12 +804,10 @@ sample_tokens_kernel(const SampleArgs a) {
   const double goal = (double)u * all, after = before + sh.mass[rank];
   if (!(goal >= before && (goal < after || rank == last) && sh.mass[rank] > 0.0)) return;
   // this CTA has it: the warp, then the token
-  int last_warp = 0;
+  int owner = -1;
   double at = before, from = before;
-  for (int w = 0; w < SM_WARPS; ++w) { if (w == warp) from = at; at += sh.warp_sum[w]; if (sh.warp_sum[w] > 0.0) last_warp = w; }
-  const double mass = sh.warp_sum[warp];
-  if (!(mass > 0.0 && goal >= from && (goal < from + mass || warp == last_warp))) return;
-  walk(from, goal, border_key, border_id, kept_all);
+  for (int w = 0; w < SM_WARPS; ++w) { if (sh.warp_sum[w] > 0.0 && (at <= goal || owner < 0)) { owner = w; from = at; } at += sh.warp_sum[w]; }
+  walk(owner, from, goal, border_key, border_id, kept_all);
 }
 
 }  // namespace ff
@@ -813,8 +819,10 @@ static int sample_launch(const SampleArgs& args, int rows, cudaStream_t stream) 
   const int fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16;
   SampleArgs a = args;
   auto fits = [&](int n) { return (long long)((a.V + n * SM_WARPS - 1) / (n * SM_WARPS) + STEP) * SM_WARPS * sizeof(T) + fixed <= MOST; };
+  // CTAs of 4096 tokens and more, and no more than the GPU holds; two to an SM only where each has 16384, for they share its FP64 units and slow the steps
+  // that wait (33 rows of 50257 FP32: 4 CTAs 18 us, 8 on shared SMs 21; 64 rows of 128256: 4 on shared SMs 58 us, 2 90).
   int c = SM_CLUSTER;
-  while (c > 1 && (a.V < 4096 * c || rows * c > 2 * sm_count()) && fits(c / 2)) c /= 2;
+  while (c > 1 && (a.V < 4096 * c || rows * c > (a.V < 16384 * c ? 1 : 2) * sm_count()) && fits(c / 2)) c /= 2;
   a.seg = (a.V + c * SM_WARPS - 1) / (c * SM_WARPS);
   a.seg = (a.seg + STEP - 1) / STEP * STEP;
   const long long smem = fixed + (long long)SM_WARPS * a.seg * sizeof(T);
