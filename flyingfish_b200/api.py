@@ -59,9 +59,10 @@ class Model:
     # -- construction ------------------------------------------------------------------------
     @classmethod
     def load(cls, model: "str | ModelSpec", settings: Settings | None = None, device: str | torch.device | None = None,
-             random_init: bool | None = None, seed: int = 0, comm=None, ep=None) -> "Model":
+             random_init: bool | None = None, seed: int = 0, comm=None, ep=None, adapters: "dict | None" = None) -> "Model":
         """Load a checkpoint directory, or a named shape with seeded random weights
-        (``random_init``; implied when ``model`` names a shape rather than a directory)."""
+        (``random_init``; implied when ``model`` names a shape rather than a directory). ``adapters``: low-rank adapters by name, each a directory
+        (``loaders.adapters.read_adapter``) or its entries; sequences choose one by its name."""
         t0 = time.perf_counter()
         settings = settings or Settings()
         if device is None:
@@ -159,12 +160,20 @@ class Model:
                     log_json("kernel_choices_applied", verbose_only=True, count=applied)
             except (OSError, ValueError, RuntimeError):
                 pass
-        plan = plan_engine(spec, settings, device, weights_bytes=weights.nbytes(), tp=tp.size)
+        stacks = None
+        if adapters:
+            from .loaders.adapters import AdapterError, build_adapters, read_adapter
+            if name in adapters:
+                raise AdapterError(f"adapter {name!r} has the model's name")
+            stacks = build_adapters(net, {n: a if isinstance(a, dict) else read_adapter(a) for n, a in adapters.items()})
+            log_json("adapters_loaded", verbose_only=True, names=stacks.names, bytes=stacks.nbytes())
+        plan = plan_engine(spec, settings, device, weights_bytes=weights.nbytes() + (0 if stacks is None else stacks.nbytes()), tp=tp.size)
         log_json("prefill_memory_plan", verbose_only=True, **plan.to_json())
         chunk = plan.prefill_chunk
         if ep is not None and getattr(ep, "arena", None) is not None and getattr(ep, "max_rows", 0) > 0:
             chunk = min(chunk, ep.max_rows)          # the expert-parallel receive buffers are sized for this many rows per call
         engine = Engine(net, spec, settings, plan.kv_blocks, device, max_prefill_rows=chunk)
+        engine.adapters = stacks
         m = cls(engine, spec, settings, tokenizer, name)
         if spec.extra.get("vision") and spec.extra["vision"].get("kind") == "minicpm":
             from .models.minicpm_vision import MiniCpmVisionSpec, MiniCpmVisionTower
@@ -194,12 +203,16 @@ class Model:
         self.engine.reset()
         self._seq = None
 
-    def prefill(self, ids: list[int]) -> int:
-        """Start a sequence with ``ids``; returns the first generated token."""
+    def prefill(self, ids: list[int], sampling=None, adapter: str | None = None) -> int:
+        """Start a sequence with ``ids``; returns the first generated token. ``sampling`` (``engine.sampling.Sampling``): how its tokens are drawn,
+        default the largest logit; ``adapter``: the loaded adapter that it goes through."""
         if self._seq is not None:
             self.engine.free_sequence(self._seq.seq_id)
             self._seq = None
         store = self.prefix_store()
+        if sampling is not None or adapter is not None:
+            store = None                   # stored prefixes hold the base model's keys and its greedy token
+            self._seq = self.engine.add_sequence(ids, sampling=sampling, adapter=adapter)
         if store is not None:
             self._seq = store.restore(self, ids)
         if self._seq is None:
@@ -260,24 +273,26 @@ class Model:
             raise RuntimeError(f"{len(positions)} image rows in the prompt for {embeds.shape[0]} rows from the tower")
         return out, positions, embeds
 
-    def prefill_multimodal(self, ids: list[int], images: list) -> int:
+    def prefill_multimodal(self, ids: list[int], images: list, sampling=None, adapter: str | None = None) -> int:
         """Like :meth:`prefill` for a prompt with one image placeholder token per image."""
         ids, positions, embeds = self.encode_images(ids, images)
         if self._seq is not None:
             self.engine.free_sequence(self._seq.seq_id)
-        self._seq = self.engine.add_sequence(ids, positions, embeds)
+        self._seq = self.engine.add_sequence(ids, positions, embeds, sampling=sampling, adapter=adapter)
         return self.engine.prefill([self._seq])[0]
 
     def decode(self) -> int:
-        """One greedy decode step for the current sequence."""
+        """One decode step for the current sequence."""
         assert self._seq is not None, "prefill first"
         return self.engine.decode([self._seq])[0]
 
     def capture(self) -> float:
-        """Capture the batch-1 decode graph ahead of time; returns milliseconds spent."""
+        """Capture the batch-1 decode graph of the current sequence's kind ahead of time; returns milliseconds spent."""
         t0 = time.perf_counter()
         if self.engine.use_graph:
-            self.engine.capture(1)
+            s = self._seq
+            kind = (s.adapter >= 0, s.draws is not None) if s is not None and s.special else ()
+            self.engine.capture(1, *kind)
         return (time.perf_counter() - t0) * 1e3
 
     def graph_decode(self) -> bool:
@@ -285,19 +300,19 @@ class Model:
 
     # -- generation --------------------------------------------------------------------------
     def generate_batch(self, prompts: list[list[int]], max_new_tokens: int, ignore_eos: bool = True,
-                       on_token=None) -> list[list[int]]:
-        return self.engine.generate(prompts, max_new_tokens, self.spec.eos_token_id, ignore_eos, on_token)
+                       on_token=None, sampling=None, adapter=None) -> list[list[int]]:
+        return self.engine.generate(prompts, max_new_tokens, self.spec.eos_token_id, ignore_eos, on_token, sampling, adapter)
 
 
 def generate_plain(model: Model, ids: list[int], count: int, ignore_eos: bool = False, graph: bool = True,
-                   on_token=None) -> GenerationOutput:
-    """Greedy loop: prefill -> optional graph capture -> decode until EOS or ``count`` tokens.
-    ``ids[0]`` of the result is the token emitted by prefill."""
+                   on_token=None, sampling=None, adapter: str | None = None) -> GenerationOutput:
+    """Plain loop: prefill -> optional graph capture -> decode until EOS or ``count`` tokens.
+    ``ids[0]`` of the result is the token emitted by prefill. Greedy unless ``sampling`` says otherwise."""
     eng = model.engine
     eng.use_graph = graph and eng.device.type == "cuda"
     sync = (lambda: torch.cuda.synchronize(eng.device)) if eng.device.type == "cuda" else (lambda: None)
     t0 = time.perf_counter()
-    first = model.prefill(ids)
+    first = model.prefill(ids, sampling, adapter) if sampling is not None or adapter is not None else model.prefill(ids)
     sync()
     t1 = time.perf_counter()
     out = [first]

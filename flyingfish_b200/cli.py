@@ -72,11 +72,19 @@ def _global_parser() -> argparse.ArgumentParser:
     g.add_argument("--diffusion-block", type=int, default=0, help="denoise the canvas in blocks of this many tokens")
     g.add_argument("--image", action="append", default=[],
                    help="PNG file for each image placeholder of the prompt (vision-language models)")
+    g.add_argument("--temperature", type=float, default=0.0, help="above 0: tokens are drawn, by --top-k, --top-p, --min-p and --sample-seed")
+    g.add_argument("--top-k", type=int, default=0)
+    g.add_argument("--top-p", type=float, default=1.0)
+    g.add_argument("--min-p", type=float, default=0.0)
+    g.add_argument("--sample-seed", type=int, default=0)
+    g.add_argument("--adapter", metavar="DIR", help="low-rank adapter that the prompt goes through (adapter_config.json + adapter_model.safetensors)")
 
     s = sub.add_parser("serve")
     s.add_argument("--port", type=int, default=8080)
     s.add_argument("--mtp", type=int, default=None, choices=range(0, 5))
-    s.add_argument("--allow-sampling", action="store_true")
+    s.add_argument("--allow-sampling", action="store_true", help="accept temperature / top_p / top_k / min_p / seed (default: greedy requests only)")
+    s.add_argument("--adapter", metavar="NAME=DIR", action="append", default=[],
+                   help="low-rank adapter that requests choose with \"model\": NAME (may be given several times)")
 
     b = sub.add_parser("bench")
     b.add_argument("--steps", type=int, default=256)
@@ -239,6 +247,53 @@ def check_flags(args) -> None:
         raise SystemExit("--spec-graph applies to --draft-model speculation")
     if args.prefix_cache and args.tp > 1:
         raise SystemExit("--prefix-cache with --tp is not supported")
+    if args.command in ("generate", "serve"):
+        _check_sampling(args)
+
+
+def _check_sampling(args) -> None:
+    adapters = adapters_from(args)
+    if args.command == "serve":
+        sampled = args.allow_sampling
+    else:
+        sampled = args.temperature > 0
+        if not sampled and (args.top_k or args.top_p != 1 or args.min_p or args.sample_seed):
+            raise SystemExit("--top-k, --top-p, --min-p and --sample-seed need --temperature above 0")
+        try:
+            sampling_from(args)
+        except ValueError as e:
+            raise SystemExit(str(e))
+    what = "adapters" if adapters else "sampling" if sampled else None
+    if what is None:
+        return
+    if args.draft_model or getattr(args, "mtp", None):
+        raise SystemExit(f"{what}: speculative decoding compares with the base model's greedy tokens")
+    if args.prefix_cache:
+        raise SystemExit(f"{what}: the prefix cache holds the base model's keys and its greedy token")
+    if args.tp > 1 and (adapters or args.command == "generate"):
+        raise SystemExit(f"{what} with --tp is not supported")
+
+
+def adapters_from(args) -> dict:
+    """Adapters by name: generate has one, serve those of its NAME=DIR flags."""
+    given = getattr(args, "adapter", None)
+    if not given:
+        return {}
+    if isinstance(given, str):
+        return {"adapter": given}
+    out = {}
+    for text in given:
+        name, eq, path = text.partition("=")
+        if not eq or not name or not path or name in out:
+            raise SystemExit(f"--adapter takes NAME=DIR with a name of its own, not {text!r}")
+        out[name] = path
+    return out
+
+
+def sampling_from(args):
+    from .engine.sampling import Sampling
+    s = Sampling(args.temperature, args.top_k, args.top_p, args.min_p, args.sample_seed)
+    return s if s.temperature > 0 else None
 
 
 def _world() -> tuple[int, int, int]:
@@ -259,6 +314,7 @@ def relaunch_tp(args, argv: list[str]) -> int | None:
 def _load(args):
     import torch
     from .api import Model
+    from .loaders.adapters import AdapterError
     from .utils.log import with_verbose
     if not args.model:
         raise SystemExit("--model (or FLYINGFISH_MODEL) is required before the subcommand")
@@ -282,7 +338,10 @@ def _load(args):
     else:
         device = "cpu" if args.cpu or not torch.cuda.is_available() else f"cuda:{args.device}"
     with with_verbose(args.verbose):
-        return Model.load(args.model, st, device=device, seed=args.seed, comm=comm)
+        try:
+            return Model.load(args.model, st, device=device, seed=args.seed, comm=comm, adapters=adapters_from(args) or None)
+        except AdapterError as e:
+            raise SystemExit(str(e))
 
 
 def cmd_generate(args) -> dict:
@@ -304,7 +363,10 @@ def cmd_generate(args) -> dict:
         from .utils.trace import Trace
         trace = Trace(device=str(model.engine.device), only_layer=args.trace_layer)
         model.engine.model.trace = trace
+    sampling, adapter = sampling_from(args), "adapter" if args.adapter else None
     if model.spec.arch == "diffusion_lm":
+        if sampling is not None or adapter is not None:
+            raise SystemExit("a masked-diffusion model takes neither sampling settings nor adapters")
         from .spec.diffusion import DiffusionTrace, diffusion_generate
         tr = DiffusionTrace()
         steps = args.diffusion_steps or max(1, args.max_new_tokens // 4)
@@ -312,10 +374,10 @@ def cmd_generate(args) -> dict:
         return {"mode": "diffusion", "tokens": toks, "text": tk.decode(toks), "passes": tr.passes}
     if args.image:
         from .serve.image import decode_png
-        first = model.prefill_multimodal(ids, [decode_png(Path(f).read_bytes()) for f in args.image])
+        first = model.prefill_multimodal(ids, [decode_png(Path(f).read_bytes()) for f in args.image], sampling, adapter)
         toks = [first] + [model.decode() for _ in range(args.max_new_tokens - 1)]
         return {"mode": "multimodal", "tokens": toks, "text": tk.decode(toks), "images": len(args.image)}
-    depth = resolve_mtp_depth(args.mtp, model.spec.mtp_layers > 0, model.spec.arch)
+    depth = resolve_mtp_depth(args.mtp, model.spec.mtp_layers > 0, model.spec.arch) if sampling is None and adapter is None else 0
     mode = "plain"
     extra = {}
     if args.draft_model:
@@ -343,10 +405,15 @@ def cmd_generate(args) -> dict:
         extra = {"mtp_depth": depth, "mtp_verify": out.extra.get("verify", "batched"),
                  "accepted_per_round": out.extra.get("accepted_per_round")}
     else:
-        out = generate_plain(model, ids, args.max_new_tokens, ignore_eos=args.ignore_eos, graph=args.graph)
+        out = generate_plain(model, ids, args.max_new_tokens, ignore_eos=args.ignore_eos, graph=args.graph, sampling=sampling, adapter=adapter)
+        if sampling is not None:
+            extra["sampling"] = {"temperature": sampling.temperature, "top_k": sampling.top_k, "top_p": sampling.top_p, "min_p": sampling.min_p,
+                                 "seed": sampling.seed}
+        if adapter is not None:
+            extra["adapter"] = args.adapter
         store = model.prefix_store()
         if store is not None:
-            extra = {"prefix_cache": {"hits": store.hits, "stored": store.stored, "dir": str(store.root)}}
+            extra["prefix_cache"] = {"hits": store.hits, "stored": store.stored, "dir": str(store.root)}
     if model.engine.kv.compact is not None:
         c = model.engine.kv.compact
         extra = dict(extra, kv={"format": "affine8", "recent": c.recent, **c.stats})

@@ -42,6 +42,14 @@ class BatchLayout:
         self.kv_start = o; o += self.max_batch if self.max_groups else 0
         self.groups = o; o += self.max_batch * self.max_groups
         self.total = o
+        # behind what every step uploads: adapters of the rows and the settings of the rows whose next token is drawn, for the steps that have any
+        self.adapter_ids = o; o += self.max_rows
+        self.uniforms = o; o += self.max_batch               # FP32, as are temperature, top_p and min_p
+        self.temperature = o; o += self.max_batch
+        self.top_k = o; o += self.max_batch
+        self.top_p = o; o += self.max_batch
+        self.min_p = o; o += self.max_batch
+        self.full = o
 
 
 class ForwardBatch:
@@ -51,11 +59,11 @@ class ForwardBatch:
         self.layout = layout
         self.device = torch.device(device)
         pin = self.device.type == "cuda" if pinned is None else pinned
-        pinned = torch.zeros(layout.total + 4 + layout.max_batch, dtype=torch.int32, pin_memory=pin)
-        self.host = pinned[: layout.total]
-        self.results = pinned[layout.total:]     # where the engine reads a step's device status (four words) and ids
+        pinned = torch.zeros(layout.full + 4 + layout.max_batch, dtype=torch.int32, pin_memory=pin)
+        self.host = pinned[: layout.full]
+        self.results = pinned[layout.full:]     # where the engine reads a step's device status (four words) and ids
         self._words = self.host.numpy()   # the same memory: a field is written in about a microsecond, through a tensor in four
-        self.dev = torch.zeros(layout.total, dtype=torch.int32, device=self.device)
+        self.dev = torch.zeros(layout.full, dtype=torch.int32, device=self.device)
         # host-side scalars of the current step
         self.batch = 0
         self.rows = 0
@@ -66,6 +74,8 @@ class ForwardBatch:
         self.max_ctx = 0
         self.n_logit_rows = 0
         self.use_tree_mask = False
+        self.adapters = None              # the model's adapters (``layers`` of stacks) where a row of the step has one
+        self.sampled = False              # the step's tokens are drawn, by the settings of the logit rows
         self._bt_sig: list = []           # block list last written to each block-table row of the host buffer
         self.key_pages: tuple | None = None   # what a model's layers derive once from this step's block lists; fill() drops it
 
@@ -87,6 +97,18 @@ class ForwardBatch:
     def ctx_lens(self) -> torch.Tensor: return self._v(self.layout.ctx_lens, self.batch)
     @property
     def logit_rows(self) -> torch.Tensor: return self._v(self.layout.logit_rows, self.n_logit_rows)
+    @property
+    def adapter_ids(self) -> torch.Tensor: return self._v(self.layout.adapter_ids, self.rows)
+    @property
+    def uniforms(self) -> torch.Tensor: return self._v(self.layout.uniforms, self.n_logit_rows).view(torch.float32)
+    @property
+    def temperature(self) -> torch.Tensor: return self._v(self.layout.temperature, self.n_logit_rows).view(torch.float32)
+    @property
+    def top_k(self) -> torch.Tensor: return self._v(self.layout.top_k, self.n_logit_rows)
+    @property
+    def top_p(self) -> torch.Tensor: return self._v(self.layout.top_p, self.n_logit_rows).view(torch.float32)
+    @property
+    def min_p(self) -> torch.Tensor: return self._v(self.layout.min_p, self.n_logit_rows).view(torch.float32)
     @property
     def block_table(self) -> torch.Tensor:
         L = self.layout
@@ -114,9 +136,11 @@ class ForwardBatch:
 
     # -- host fill -----------------------------------------------------------------------------
     def fill(self, *, ids, positions, slots, q_lens, ctx_lens, block_rows, logit_rows, is_decode: bool, nq: int = 1,
-             tree_mask=None, kv_start=None, group_rows=None, state_slots=None, singles: int = 0) -> None:
+             tree_mask=None, kv_start=None, group_rows=None, state_slots=None, singles: int = 0, adapters=None, adapter_ids=None,
+             draws=None) -> None:
         """Write one step's metadata into the pinned host buffer (lists of ints; ids, positions and slots also as int32 arrays, which
-        is what a prompt's thousands of rows take)."""
+        is what a prompt's thousands of rows take). ``adapters`` with ``adapter_ids`` (one per sequence, -1 for none; rows behind the sequences'
+        have none): the step reads them. ``draws``: per logit row None (the largest logit) or ``(engine.sampling.Draws, index of the new token)``."""
         L = self.layout
         h = self._words
         rows, batch = len(ids), len(q_lens)
@@ -167,6 +191,21 @@ class ForwardBatch:
                 if row:
                     assert len(row) <= L.max_groups
                     gt[i, : len(row)] = row
+        self.adapters = adapters
+        if adapters is not None:
+            h[L.adapter_ids: L.adapter_ids + rows] = -1
+            h[L.adapter_ids: L.adapter_ids + int(ql.sum())] = np.repeat(np.asarray(adapter_ids, dtype=np.int32), ql)
+        self.sampled = draws is not None
+        if draws is not None:
+            n = len(draws)
+            assert n == self.n_logit_rows and n <= L.max_batch, "one drawn token per sequence"
+            f = h.view(np.float32)
+            u, t, k, p, m = (a[o: o + n] for a, o in ((f, L.uniforms), (f, L.temperature), (h, L.top_k), (f, L.top_p), (f, L.min_p)))
+            u[:], t[:], k[:], p[:], m[:] = 0, 0, 0, 1, 0
+            for i, d in enumerate(draws):
+                if d is not None:
+                    u[i] = d[0].uniform(d[1])
+                    t[i], k[i], p[i], m[i] = d[0].row
         self.max_q_len = int(max(q_lens)) if batch else 0
         self.max_ctx = int(max(ctx_lens)) if batch else 0
         self.use_tree_mask = tree_mask is not None
@@ -174,9 +213,13 @@ class ForwardBatch:
             # 64 bits per row, bit 63 may be set
             h[L.tree_mask: L.tree_mask + 2 * rows] = np.array([m & (1 << 64) - 1 for m in tree_mask], dtype=np.uint64).view(np.int32)
 
+    def _used(self) -> int:
+        return self.layout.full if self.adapters is not None or self.sampled else self.layout.total
+
     def h2d_bytes(self) -> int:
-        return self.layout.total * 4
+        return self._used() * 4
 
     def upload(self) -> None:
-        """One host-to-device copy of the whole packed buffer."""
-        self.dev.copy_(self.host, non_blocking=True)
+        """One host-to-device copy of the packed buffer, adapters and settings included where the step has any."""
+        n = self._used()
+        self.dev[:n].copy_(self.host[:n], non_blocking=True)

@@ -20,9 +20,11 @@ import torch
 
 from .. import ops
 from ..config import ModelSpec, Settings
+from ..ops import sample_ops
 from ..utils.log import log_json
 from .batch import BatchLayout, ForwardBatch
 from .kv_cache import OutOfBlocks, PagedKVCache
+from .sampling import Draws, Sampling
 
 
 class EnginePoisoned(RuntimeError):
@@ -50,6 +52,12 @@ class Sequence:
     state_slot: int = -1               # slot of the per-sequence recurrent state (hybrid linear-attention models)
     mm_positions: list[int] | None = None      # prompt indices whose embedding row comes from ``mm_embeds``
     mm_embeds: torch.Tensor | None = None      # [len(mm_positions), hidden] (vision-tower output)
+    draws: Draws | None = None         # settings its tokens are drawn by; None: greedy
+    adapter: int = -1                  # index in the engine's adapters, -1 for none
+
+    @property
+    def special(self) -> bool:
+        return self.draws is not None or self.adapter >= 0
 
     @property
     def all_tokens(self) -> list[int]:
@@ -111,9 +119,11 @@ class Engine:
         self.mixed_batches = bool(getattr(model, "mixed_batches", False))
         self.prefill_batch = ForwardBatch(BatchLayout(self.max_batch, max(max_prefill_rows, self.max_batch),
                                                       self.max_blocks), self.device)
-        self.graphs: dict[tuple[int, int], _Graph] = {}
+        self.graphs: dict[tuple, _Graph] = {}
+        self.adapters = None               # loaders.adapters.AdapterSet of a model loaded with adapters
         self.eager_decode_batch: dict[int, ForwardBatch] = {}
         self.seqs: dict[int, Sequence] = {}
+        self._special = 0                  # live sequences with sampling settings or an adapter
         self._next_id = 0
         self.poisoned = False
         self.use_graph = settings.graph and self.device.type == "cuda"
@@ -134,17 +144,26 @@ class Engine:
 
     # -- sequence management ---------------------------------------------------------------
     def add_sequence(self, prompt: list[int], mm_positions: list[int] | None = None,
-                     mm_embeds: torch.Tensor | None = None) -> Sequence:
+                     mm_embeds: torch.Tensor | None = None, sampling: Sampling | None = None, adapter: str | None = None) -> Sequence:
         """``mm_positions`` / ``mm_embeds``: prompt indices whose embedding rows are supplied by the caller (the
-        vision tower's output for image placeholder tokens) instead of the embedding table."""
+        vision tower's output for image placeholder tokens) instead of the embedding table. ``sampling``: how the sequence's tokens are drawn (default:
+        the largest logit); ``adapter``: name of the low-rank adapter its rows go through."""
         self._check()
         if len(prompt) == 0:
             raise ValueError("empty prompt")
         if len(prompt) + 1 > self.settings.capacity:
             raise ValueError(f"prompt of {len(prompt)} tokens exceeds the KV capacity {self.settings.capacity}")
+        if sampling is not None and self.model.w.tp.size > 1:
+            raise ValueError("sampling is not available with tensor parallelism")
+        if adapter is not None and (self.adapters is None or adapter not in self.adapters.index):
+            raise ValueError(f"no adapter {adapter!r} is loaded")
         sid = self._next_id
         self._next_id += 1
         s = Sequence(sid, list(prompt))
+        if sampling is not None and sampling.temperature > 0:
+            s.draws = Draws(sampling)
+        if adapter is not None:
+            s.adapter = self.adapters.index[adapter]
         if mm_positions:
             if mm_embeds is None or mm_embeds.shape[0] != len(mm_positions) or mm_embeds.shape[1] != self.spec.hidden:
                 raise ValueError("mm_embeds must hold one hidden-sized row per mm position")
@@ -155,11 +174,14 @@ class Engine:
             s.state_slot = self.state_slots.pop()
             self.model.reset_state(s.state_slot)
         self.seqs[sid] = s
+        self._special += s.special
         self.kv.add_sequence(sid)
         return s
 
     def free_sequence(self, seq_id: int) -> None:
         s = self.seqs.pop(seq_id, None)
+        if s is not None:
+            self._special -= s.special
         if s is not None and self.state_slots is not None and s.state_slot >= 0:
             self.state_slots.append(s.state_slot)
             s.state_slot = -1
@@ -170,6 +192,7 @@ class Engine:
         for sid in list(self.kv.seqs):
             self.kv.free_sequence(sid)
         self.seqs.clear()
+        self._special = 0
         if self.state_slots is not None:
             self.state_slots = list(range(self.model.state_slot_count - 1))
         self.poisoned = False
@@ -273,12 +296,38 @@ class Engine:
         if need > self.kv.alloc.free_blocks:
             raise OutOfBlocks(f"step needs {need} KV blocks, {self.kv.alloc.free_blocks} free")
 
-    def _fill_spans(self, spans: list[Span], singles: int = 0) -> ForwardBatch:
+    def _extras(self, seqs: list[Sequence], draws: list | None) -> dict:
+        """What a batch is told of its sequences' adapters and, with ``draws`` (per logit row), of the rows that are drawn: nothing where there are none."""
+        extra = {}
+        if self.adapters is not None and any(s.adapter >= 0 for s in seqs):
+            extra = {"adapters": self.adapters, "adapter_ids": [s.adapter for s in seqs]}
+        if draws is not None and any(d is not None for d in draws):
+            extra["draws"] = draws
+        return extra
+
+    def _forward_ids(self, fb: ForwardBatch, **kw) -> torch.Tensor:
+        """The next token of every logit row: the largest logit, or drawn by the rows' settings."""
+        if not fb.sampled:
+            return self.model.forward(fb, self.kv, **kw)
+        lg = self.model.forward(fb, self.kv, return_logits=True, **kw)
+        if lg.dtype not in (torch.bfloat16, torch.float32):
+            lg = lg.float()
+        return sample_ops.sample_tokens(lg, fb.uniforms, fb.temperature, fb.top_k, fb.top_p, fb.min_p)[0]
+
+    @staticmethod
+    def _plain_only(seqs: list[Sequence], what: str) -> None:
+        """Refuse what compares with the base model's greedy tokens."""
+        if any(s.special for s in seqs):
+            raise ValueError(f"{what} is not available for a sequence with sampling settings or an adapter")
+
+    def _fill_spans(self, spans: list[Span], singles: int = 0, draw: bool = True) -> ForwardBatch:
         """Pack the spans row-wise into the prefill batch and upload it (reserves their KV rows; commits nothing). With
         ``singles``, that many spans at the end are one row each and take the decode attention."""
         self._need_blocks([(sp.seq.seq_id, len(sp.tokens)) for sp in spans])
         fb = self.prefill_batch
         ids, positions, slots, q_lens, ctx_lens, block_rows, logit_rows = [], [], [], [], [], [], []
+        draw = draw and self._special > 0
+        draws = [] if draw else None
         # thousands of prompt rows are listed as arrays (8000 rows: 4.4 ms as lists of ints, 0.6 ms); for a few dozen lists are quicker
         wide = sum(len(sp.tokens) for sp in spans) > 256
         row = 0
@@ -296,6 +345,10 @@ class Engine:
             ctx_lens.append(kvs.length + take)
             block_rows.append(kvs.blocks)
             logit_rows += [row + k for k in sp.want]
+            if draw:
+                d, end = sp.seq.draws, kvs.length + 1
+                # a portion that does not reach its prompt's end gives a token that nobody reads
+                draws += [(d, end + k) if d is not None and end + k >= len(sp.seq.prompt) else None for k in sp.want]
             row += take
         mult = getattr(self.model.comm, "size", 1) * 128 if getattr(self.model.comm, "fused", False) else 1
         if mult > 1 and row >= mult and (row + mult - 1) // mult * mult <= fb.layout.max_rows:
@@ -311,14 +364,14 @@ class Engine:
             ids, positions, slots = (np.concatenate(v) for v in (ids, positions, slots))
         fb.fill(ids=ids, positions=positions, slots=slots, q_lens=q_lens, ctx_lens=ctx_lens, block_rows=block_rows,
                 logit_rows=logit_rows, is_decode=False, state_slots=state_slots if self.state_slots is not None else None,
-                singles=singles)
+                singles=singles, **(self._extras([sp.seq for sp in spans], draws) if self._special else {}))
         fb.upload()
         fb.state_slots = state_slots
         return fb
 
     def _prefill_chunk(self, part: list[tuple[Sequence, int]]) -> list[int]:
         fb = self._fill_spans([Span(s, s.prompt[s.prefilled: s.prefilled + take], [take - 1]) for s, take in part])
-        toks = self._read_ids(self.model.forward(fb, self.kv, inputs_embeds=self._mm_embeds(part, fb, fb.rows)))
+        toks = self._read_ids(self._forward_ids(fb, inputs_embeds=self._mm_embeds(part, fb, fb.rows)))
         for s, take in part:
             self.kv.commit(s.seq_id, take)
             s.prefilled += take
@@ -327,13 +380,13 @@ class Engine:
 
     # -- mixed steps ---------------------------------------------------------------------------
     def _run_mixed(self, spans: list[Span], greedy: bool) -> torch.Tensor | None:
-        """One forward over prompt portions and single tokens together; returns the greedy ids (``greedy``) or the logits
-        of the wanted rows in the order of the spans, or None when no row is wanted. Commits every span."""
+        """One forward over prompt portions and single tokens together; returns the next tokens (``greedy``; drawn where a sequence says so) or
+        the logits of the wanted rows in the order of the spans, or None when no row is wanted. Commits every span."""
         order = sorted(range(len(spans)), key=lambda i: len(spans[i].tokens) == 1)         # portions first, stable
         packed = [spans[i] for i in order]
-        fb = self._fill_spans(packed, singles=sum(len(sp.tokens) == 1 for sp in packed))
+        fb = self._fill_spans(packed, singles=sum(len(sp.tokens) == 1 for sp in packed), draw=greedy)
         if fb.n_logit_rows:
-            out = self.model.forward(fb, self.kv, return_logits=not greedy)
+            out = self._forward_ids(fb) if greedy else self.model.forward(fb, self.kv, return_logits=True)
             # wanted rows came out in packed order: put them back into the order of the spans
             first = {}
             at = 0
@@ -402,7 +455,7 @@ class Engine:
             if all(len(sp.tokens) == 1 for sp in spans):
                 for sp in spans:
                     sp.seq.pending = sp.tokens[0]
-                _, logits, _ = self._launch_decode([sp.seq for sp in spans])
+                _, logits, _ = self._launch_decode([sp.seq for sp in spans], draw=False)
                 for sp in spans:
                     self.kv.commit(sp.seq.seq_id, 1)
                 rows = [i for i, sp in enumerate(spans) for _ in sp.want]
@@ -478,7 +531,7 @@ class Engine:
         return emb
 
     # -- decode ------------------------------------------------------------------------------
-    def _fill_decode(self, fb: ForwardBatch, seqs: list[Sequence], bucket: int) -> None:
+    def _fill_decode(self, fb: ForwardBatch, seqs: list[Sequence], bucket: int, extra: dict | None = None) -> None:
         # field by field: a loop over the sequences that appends to a list per field cost 1.5 us a sequence, this 0.4
         held, lens, new = self.kv.reserve_step([s.seq_id for s in seqs])
         n, pad = len(seqs), bucket - len(seqs)
@@ -494,9 +547,15 @@ class Engine:
         st = None
         if self.state_slots is not None:
             st = [s.state_slot for s in seqs] + [self.scratch_slot] * pad
+        if extra:
+            extra = dict(extra)
+            if "adapters" in extra:
+                extra["adapter_ids"] = extra["adapter_ids"] + [-1] * pad
+            if "draws" in extra:
+                extra["draws"] = extra["draws"] + [None] * pad
         fb.fill(ids=ids, positions=positions, slots=slots, q_lens=np.ones(bucket, np.int32), ctx_lens=ctx_lens, block_rows=block_rows,
                 logit_rows=range(bucket), is_decode=True, nq=1, kv_start=kv_start, group_rows=group_rows,
-                state_slots=st)
+                state_slots=st, **(extra or {}))
         fb.max_ctx = self.settings.capacity      # fixed launch geometry (graph-stable)
 
     def _decode_batch(self, bucket: int) -> ForwardBatch:
@@ -506,11 +565,12 @@ class Engine:
             self.eager_decode_batch[bucket] = fb
         return fb
 
-    def capture(self, bucket: int) -> _Graph:
+    def capture(self, bucket: int, adapters: bool = False, sampled: bool = False) -> _Graph:
         """Capture the decode step for a batch bucket: one eager warm-up on padding rows (which
         write no KV), then stream capture of the same step. A replay reads the step's metadata from the batch's device
-        buffer (``batch.dev``), which the caller has written, and leaves ids and logits in ``out`` and ``logits``."""
-        key = (bucket, 1)
+        buffer (``batch.dev``), which the caller has written, and leaves ids and logits in ``out`` and ``logits``. A step with ``adapters`` or drawn tokens
+        (``sampled``) is a graph of its own, which serves any mix of adapters and settings: they are metadata too."""
+        key = (bucket, 1, adapters, sampled) if adapters or sampled else (bucket, 1)
         g = self.graphs.get(key)
         if g is not None:
             return g
@@ -519,19 +579,20 @@ class Engine:
         fb = self._decode_batch(bucket)
         fb.fill(ids=[0] * bucket, positions=[0] * bucket, slots=[-1] * bucket, q_lens=[1] * bucket,
                 ctx_lens=[0] * bucket, block_rows=[[]] * bucket, logit_rows=list(range(bucket)), is_decode=True,
-                state_slots=[self.scratch_slot] * bucket if self.state_slots is not None else None)
+                state_slots=[self.scratch_slot] * bucket if self.state_slots is not None else None,
+                adapters=self.adapters if adapters else None, adapter_ids=[-1] * bucket, draws=[None] * bucket if sampled else None)
         fb.max_ctx = self.settings.capacity
         fb.upload()
         side = torch.cuda.Stream(self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
             for _ in range(2):
-                self.model.forward(fb, self.kv)
+                self._forward_ids(fb)
         torch.cuda.current_stream(self.device).wait_stream(side)
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            out = self.model.forward(fb, self.kv)
+            out = self._forward_ids(fb)
         g.graph, g.batch, g.out, g.logits = graph, fb, out, getattr(self.model, "last_logits", None)
         self.graphs[key] = g
         self.stats["captures"] += 1
@@ -544,23 +605,27 @@ class Engine:
             if held[s.seq_id].length >= cap:
                 raise OutOfBlocks(f"sequence {s.seq_id} reached the KV capacity {cap}")
 
-    def _launch_decode(self, seqs: list[Sequence]) -> tuple[torch.Tensor, torch.Tensor | None, ForwardBatch]:
+    def _launch_decode(self, seqs: list[Sequence], draw: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, ForwardBatch]:
         """Upload and launch the decode step of every sequence's pending token (a graph replay where graphs are on);
-        returns (greedy ids, logits, batch), all of the padded bucket. Commits nothing; the caller waits for the
-        device before it launches the next step, which writes the batch's pinned buffer."""
+        returns (next tokens, logits, batch), all of the padded bucket; without ``draw`` the tokens are the greedy ones. Commits nothing; the caller waits
+        for the device before it launches the next step, which writes the batch's pinned buffer."""
         bucket = bucket_for(len(seqs))
+        held = self.kv.seqs
+        extra = {}
+        if self._special:
+            extra = self._extras(seqs, [None if s.draws is None else (s.draws, held[s.seq_id].length + 1) for s in seqs] if draw else None)
         if self.use_graph and getattr(self.model, "expert_provider", None) is None:
-            g = self.capture(bucket)
+            g = self.capture(bucket, "adapters" in extra, "draws" in extra)
             fb = g.batch
-            self._fill_decode(fb, seqs, bucket)
+            self._fill_decode(fb, seqs, bucket, extra)
             fb.upload()
             g.graph.replay()
             self.stats["graph_replays"] += 1
             return g.out, g.logits, fb
         fb = self._decode_batch(bucket)
-        self._fill_decode(fb, seqs, bucket)
+        self._fill_decode(fb, seqs, bucket, extra)
         fb.upload()
-        out = self.model.forward(fb, self.kv)
+        out = self._forward_ids(fb)
         return out, getattr(self.model, "last_logits", None), fb
 
     def decode(self, seqs: list[Sequence]) -> list[int]:
@@ -669,6 +734,7 @@ class Engine:
         kernels/tree/meta.cu)."""
         self._check()
         self._no_compact("speculative verification")
+        self._plain_only(seqs, "speculative verification")
         if self.fail_next_step:
             self.fail_next_step = False
             self.poisoned = True
@@ -739,6 +805,7 @@ class Engine:
         committed length and are overwritten by whatever runs next."""
         self._check()
         self._no_compact("an uncommitted multi-row forward")
+        self._plain_only([seq], "an uncommitted multi-row forward")
         kvs = self.kv.seqs[seq.seq_id]
         n = len(tokens)
         sl = self.kv.reserve(seq.seq_id, n)
@@ -755,6 +822,7 @@ class Engine:
         token after every row."""
         self._check()
         self._no_compact("tree verification")
+        self._plain_only([seq], "tree verification")
         try:
             kvs = self.kv.seqs[seq.seq_id]
             n = len(tokens)
@@ -822,10 +890,22 @@ class Engine:
 
     # -- convenience ---------------------------------------------------------------------------
     def generate(self, prompts: list[list[int]], max_new_tokens: int, eos: int | None = None,
-                 ignore_eos: bool = True, on_token=None) -> list[list[int]]:
-        """Greedy generation for a batch of prompts; returns the generated ids per prompt
-        (``generated[0]`` is the token emitted by prefill, as in the reference's ``generate``)."""
-        seqs = [self.add_sequence(p) for p in prompts]
+                 ignore_eos: bool = True, on_token=None, sampling=None, adapter=None) -> list[list[int]]:
+        """Generation for a batch of prompts, greedy by default; returns the generated ids per prompt
+        (``generated[0]`` is the token emitted by prefill, as in the reference's ``generate``). ``sampling`` and ``adapter``: one for all
+        prompts, or a list of one (or None) per prompt."""
+        each = lambda v: list(v) if isinstance(v, (list, tuple)) else [v] * len(prompts)
+        how, whose = each(sampling), each(adapter)
+        if len(how) != len(prompts) or len(whose) != len(prompts):
+            raise ValueError("sampling and adapter: one for all prompts or one per prompt")
+        seqs = []
+        try:
+            for p, h, a in zip(prompts, how, whose):
+                seqs.append(self.add_sequence(p, sampling=h, adapter=a) if h is not None or a is not None else self.add_sequence(p))
+        except Exception:
+            for s in seqs:
+                self.free_sequence(s.seq_id)
+            raise
         try:
             self.prefill(seqs)
             if on_token:

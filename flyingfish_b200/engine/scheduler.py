@@ -44,6 +44,8 @@ class Request:
     images: list | None = None        # decoded images, one per image placeholder token of ``prompt``
     mm_positions: list[int] | None = None
     mm_embeds: object | None = None
+    sampling: object | None = None    # engine.sampling.Sampling; None: greedy
+    adapter: str | None = None        # name of a loaded low-rank adapter
 
     @property
     def ttft_ms(self) -> float | None:
@@ -73,6 +75,13 @@ class Scheduler:
         if len(req.prompt) + req.max_tokens > self.engine.settings.capacity:
             raise ValueError(f"prompt ({len(req.prompt)}) + max_tokens ({req.max_tokens}) exceeds the KV capacity "
                              f"{self.engine.settings.capacity}")
+        if req.adapter is not None:
+            loaded = getattr(self.engine, "adapters", None)
+            if loaded is None or req.adapter not in loaded.index:
+                raise ValueError(f"no adapter {req.adapter!r} is loaded")
+        if req.sampling is not None and getattr(getattr(getattr(self.engine, "model", None), "w", None), "tp", None) is not None \
+                and self.engine.model.w.tp.size > 1:
+            raise ValueError("sampling is not available with tensor parallelism")
         self.waiting.append(req)
         return req
 
@@ -120,10 +129,11 @@ class Scheduler:
             free -= need
             self.waiting.popleft()
             # a preempted request resumes by recomputing prompt + what it already produced
+            how = {k: v for k, v in (("sampling", req.sampling), ("adapter", req.adapter)) if v is not None}
             if req.mm_positions:
-                req.seq = self.engine.add_sequence(req.prompt + req.output, req.mm_positions, req.mm_embeds)
+                req.seq = self.engine.add_sequence(req.prompt + req.output, req.mm_positions, req.mm_embeds, **how)
             else:
-                req.seq = self.engine.add_sequence(req.prompt + req.output)
+                req.seq = self.engine.add_sequence(req.prompt + req.output, **how)
             req.state = "running"
             admitted.append(req)
             self.stats["admitted"] += 1

@@ -20,6 +20,7 @@ import torch
 
 from .. import ops
 from ..config import ModelSpec
+from ..ops import lora_ops
 from ..engine.batch import ForwardBatch
 from ..engine.kv_cache import PagedKVCache
 from .weights import ModelWeights
@@ -59,6 +60,7 @@ class DecoderModel:
         self.normed_sink: list | None = None      # when a list: every forward appends its final-normed rows
         self.last_logits: torch.Tensor | None = None   # logits of the latest forward (a captured step keeps its own)
         self._rope_cs: torch.Tensor | None = None  # per-forward cos/sin table of the fused QKV kernels
+        self._adapters: tuple | None = None        # per-forward (stacks of every layer, adapter id of every row), or None
         # encoders and diffusion language models attend in both directions inside a sequence; they run whole
         # sequences in one prefill chunk and never decode
         self.bidirectional = bool(self.spec.extra.get("bidirectional"))
@@ -66,10 +68,16 @@ class DecoderModel:
     # -- pieces ----------------------------------------------------------------------------
     def _attention(self, i: int, n: torch.Tensor, b: ForwardBatch, kv: PagedKVCache) -> torch.Tensor:
         lw, s = self.w.layers[i], self.spec
+        ad = self._adapters
+        stacks, rows = (None, None) if ad is None else (ad[0][i], ad[1])
+        lora = stacks is not None and stacks.qkv is not None
         if s.qk_norm:
-            qkv = ops.linear(n, lw.wqkv)
+            qkv = lora_ops.linear_lora(n, lw.wqkv, stacks.qkv, rows) if lora else ops.linear(n, lw.wqkv)
             ops.rope_kv_paged(qkv, b.positions, b.slots, kv.k[i], kv.v[i], self.hq, self.hkv, self.d, s.rope_theta,
                               q_norm=lw.q_norm, k_norm=lw.k_norm, eps=s.rms_eps)
+        elif lora:
+            qkv = lora_ops.linear_rope_kv_lora(n, lw.wqkv, stacks.qkv, rows, b.positions, b.slots, kv.k[i], kv.v[i], self.hq, self.hkv, self.d,
+                                               s.rope_theta, cos_sin=self._rope_cs)
         else:
             qkv = ops.linear_rope_kv(n, lw.wqkv, b.positions, b.slots, kv.k[i], kv.v[i], self.hq, self.hkv, self.d,
                                      s.rope_theta, cos_sin=self._rope_cs)
@@ -85,16 +93,28 @@ class DecoderModel:
                                  self.hq, self.hkv, self.d, self.scale, window=-1 if self.bidirectional else 0)
         if self.trace is not None:
             self.trace.record(f"layer.{i}.attn", a)
+        if stacks is not None and stacks.o is not None:
+            return lora_ops.linear_lora(a, lw.wo, stacks.o, rows)
         return self.comm.row_linear(a, lw.wo)
 
     def _ffn(self, i: int, n: torch.Tensor) -> torch.Tensor:
         lw = self.w.layers[i]
         if lw.router is not None:
             return moe_mod.moe_ffn(self, i, n)
-        if lw.wgu_interleaved:
+        ad = self._adapters
+        stacks, rows = (None, None) if ad is None else (ad[0][i], ad[1])
+        if stacks is not None and stacks.gu is not None:
+            if lw.wgu_interleaved and lw.wgu.shape[0] % 256 == 0:
+                hmid = lora_ops.linear_swiglu_lora(n, lw.wgu, stacks.gu, rows, mode=self.spec.swiglu_mode)
+            else:
+                gu = lora_ops.linear_lora(n, lw.wgu, stacks.gu, rows)
+                hmid = (ops.silu_mul_interleaved if lw.wgu_interleaved else ops.silu_mul)(gu, mode=self.spec.swiglu_mode)
+        elif lw.wgu_interleaved:
             hmid = ops.linear_swiglu(n, lw.wgu, mode=self.spec.swiglu_mode)
         else:
             hmid = ops.silu_mul(ops.linear(n, lw.wgu), mode=self.spec.swiglu_mode)
+        if stacks is not None and stacks.down is not None:
+            return lora_ops.linear_lora(hmid, lw.wdown, stacks.down, rows)
         return self.comm.row_linear(hmid, lw.wdown)
 
     # -- forward ---------------------------------------------------------------------------
@@ -105,6 +125,8 @@ class DecoderModel:
         next token's embedding and the previous hidden state)."""
         w, s = self.w, self.spec
         self._rope_cs = None
+        ad = getattr(b, "adapters", None)
+        self._adapters = None if ad is None else (ad.layers, b.adapter_ids)
         if inputs_embeds is None and self._sequence_parallel(b):
             return self._hidden_states_sp(b, kv)
         if self._chain_ok(b):
@@ -152,7 +174,7 @@ class DecoderModel:
         difference or slower (200 1662 / 1688)."""
         from ..ops import lib
         w, s, me = self.w, self.spec, type(self)
-        if b.is_decode or b.rows > STACK_MAX_ROWS or not b.positions.is_cuda or self.trace is not None or self.capture_taps or lib.DEBUG_CHECKS:
+        if self._adapters is not None or b.is_decode or b.rows > STACK_MAX_ROWS or not b.positions.is_cuda or self.trace is not None or self.capture_taps or lib.DEBUG_CHECKS:
             return None
         if me._attention is not DecoderModel._attention or me._ffn is not DecoderModel._ffn or type(self.comm) is not NoComm or type(w.layers) is not list:
             return None
@@ -173,7 +195,7 @@ class DecoderModel:
         s = self.spec
         if not (chain.ENABLED and b.is_decode and b.positions.is_cuda and b.rows <= chain.MAX_ROWS):
             return False
-        if getattr(b, "kv_start", None) is not None:
+        if getattr(b, "kv_start", None) is not None or self._adapters is not None:
             return False
         if getattr(self.comm, "size", 1) != 1 or self.trace is not None or self.capture_taps or s.qk_norm:
             return False

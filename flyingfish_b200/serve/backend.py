@@ -43,6 +43,8 @@ class Unavailable(RuntimeError):
 class Backend:
     """Thread-safe front of the engine thread."""
 
+    greedy_only = False            # requests with sampling settings or an adapter are refused
+
     def __init__(self, engine, eos_ids: tuple[int, ...] = (), max_inflight: int | None = None,
                  token_budget: int | None = None):
         self.engine = engine
@@ -68,7 +70,7 @@ class Backend:
 
     # -- called from the event loop thread --------------------------------------------------
     def add_request(self, prompt: list[int], max_tokens: int, ignore_eos: bool = False,
-                    images: list | None = None) -> tuple[Request, asyncio.Queue]:
+                    images: list | None = None, sampling=None, adapter: str | None = None) -> tuple[Request, asyncio.Queue]:
         if self.state == "unavailable":
             raise Unavailable("engine is unavailable after an earlier failure")
         with self._lock:
@@ -77,7 +79,7 @@ class Backend:
             loop = asyncio.get_running_loop()
             q: asyncio.Queue = asyncio.Queue()
             req = Request(prompt=prompt, max_tokens=max_tokens, eos_ids=self.eos_ids, ignore_eos=ignore_eos,
-                          images=images or None)
+                          images=images or None, sampling=sampling, adapter=adapter)
             req.on_tokens = self._on_tokens
             req.on_finish = self._on_finish
             self._inflight[req.req_id] = (req, q, loop)
@@ -162,7 +164,9 @@ class MtpBackend(Backend):
     """Server backend for ``ff serve --mtp N``: every request is generated by multi-token-prediction speculation
     (draft with the MTP head, verify with one multi-row target forward). Speculation rounds are per sequence, so
     admission is the reference's single slot (src/serve/mod.rs:41-59, ``run_mtp`` :144-161): a second request while
-    one runs is answered 409."""
+    one runs is answered 409. Drafts are compared with the base model's greedy tokens: a request has no sampling settings and no adapter."""
+
+    greedy_only = True
 
     def __init__(self, model, depth: int, eos_ids: tuple[int, ...] = ()):
         super().__init__(model.engine, eos_ids=eos_ids, max_inflight=1)

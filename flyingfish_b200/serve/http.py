@@ -10,8 +10,10 @@ chunk with ``finish_reason`` and ``data: [DONE]``. Too many requests in flight -
 reference answers 409 whenever one request is running; here the bound is the scheduler's
 in-flight limit). A client that disconnects aborts its request.
 
-``allow_sampling=True`` additionally accepts temperature / top_p / top_k (an extension; off by
-default so the validation matrix matches the reference).
+``allow_sampling=True`` additionally accepts temperature / top_p / top_k / min_p / seed (an extension; off by
+default so the validation matrix matches the reference): a temperature above 0 has the request's tokens drawn, each by settings and random numbers of
+its own request, so that a seed gives the same tokens whatever else the server runs. ``model`` may also name one of the adapters
+that the server was started with.
 """
 from __future__ import annotations
 
@@ -19,11 +21,13 @@ import asyncio
 import base64
 import itertools
 import json
+import secrets
 import time
 from typing import Any
 
 from aiohttp import web
 
+from ..engine.sampling import Sampling
 from ..loaders.tokenizer import Detok
 from .backend import Backend, Busy, EngineEvent, Unavailable
 
@@ -31,6 +35,7 @@ MAX_BODY = 128 * 1024 * 1024
 TEMPLATE_ROLES = ("system", "user", "assistant", "tool")
 COMMON_KEYS = {"temperature", "top_p", "top_k", "n", "logit_bias", "presence_penalty", "frequency_penalty",
                "max_tokens", "max_completion_tokens", "stop", "stream", "model"}
+SAMPLING_KEYS = {"min_p", "seed"}            # beside those of COMMON_KEYS, where sampling is allowed
 
 
 class HttpError(Exception):
@@ -56,20 +61,38 @@ def check_greedy(p: dict) -> None:
         raise bad_request("greedy only: top_p must be 1 or absent")
     if p.get("top_k") is not None:
         raise bad_request("greedy only: top_k is not supported")
+    check_plain(p, "greedy only: ")
+
+
+def check_plain(p: dict, why: str = "") -> None:
+    """Refuse what no request can ask for, sampled or not."""
     if p.get("n") is not None and p["n"] != 1:
-        raise bad_request("greedy only: n must be 1")
+        raise bad_request(f"{why}n must be 1")
     if p.get("logit_bias") is not None:
-        raise bad_request("greedy only: logit_bias is not supported")
+        raise bad_request(f"{why}logit_bias is not supported")
     for k in ("presence_penalty", "frequency_penalty"):
         if p.get(k) is not None and p[k] != 0:
-            raise bad_request(f"greedy only: {k} must be 0 or absent")
+            raise bad_request(f"{why}{k} must be 0 or absent")
     if p.get("stop") is not None:
         raise bad_request("stop sequences are not supported")
 
 
-def check_request(body: dict, allowed_extra: set[str], model_name: str) -> None:
+def resolve_sampling(p: dict) -> Sampling | None:
+    """A request's sampling settings; None for a greedy one (temperature 0 or absent). Without a seed the request gets one of its own."""
+    check_plain(p)
+    given = {k: p[k] for k in ("temperature", "top_k", "top_p", "min_p", "seed") if p.get(k) is not None}
+    if given.get("top_k") == -1:                 # "all tokens" in other servers' requests
+        given["top_k"] = 0
+    try:
+        s = Sampling(**{"temperature": 0, "seed": secrets.randbits(64), **given})
+    except ValueError as e:
+        raise bad_request(str(e))
+    return s if s.temperature > 0 else None
+
+
+def check_request(body: dict, allowed_extra: set[str], model_name: str, adapters=()) -> None:
     model = body.get("model")
-    if model is not None and model != model_name:
+    if model is not None and model != model_name and model not in adapters:
         raise HttpError(404, f"model {model!r} is not served; the loaded model is {model_name!r}",
                         code="model_not_found")
     for k, v in body.items():
@@ -90,7 +113,10 @@ def resolve_max_tokens(p: dict) -> int:
 
 class Server:
     def __init__(self, backend: Backend, tokenizer, model_name: str, chat_template: str | None = None,
-                 capacity: int = 4096, allow_sampling: bool = False, image_placeholder: str | None = None):
+                 capacity: int = 4096, allow_sampling: bool = False, image_placeholder: str | None = None, adapters: tuple[str, ...] = ()):
+        if backend.greedy_only and (allow_sampling or adapters):
+            raise ValueError("multi-token-prediction speculation serves greedy requests of the base model")
+        self.adapters = adapters               # names that a request's ``model`` may take beside the loaded model's
         self.backend, self.tk, self.model_name = backend, tokenizer, model_name
         self.capacity = capacity
         # text of the image placeholder token (vision-language models only); None refuses image parts
@@ -198,28 +224,35 @@ class Server:
             raise bad_request(f"prompt ({len(ids)} tokens) + max_tokens ({max_tokens}) exceeds the context capacity "
                               f"{self.capacity}")
 
+    def _settings(self, body: dict, allowed_extra: set[str]) -> Sampling | None:
+        """Checks the request's parameters; its sampling settings, or None where it is greedy."""
+        sampling = None
+        if self.allow_sampling:
+            sampling = resolve_sampling(body)
+            allowed_extra = allowed_extra | SAMPLING_KEYS
+        else:
+            check_greedy(body)
+        check_request(body, allowed_extra, self.model_name, self.adapters)
+        return sampling
+
     # -- handlers ------------------------------------------------------------------------------
     async def completions(self, request: web.Request) -> web.StreamResponse:
         try:
             body = await self._json(request)
-            if not self.allow_sampling:
-                check_greedy(body)
-            check_request(body, {"prompt"}, self.model_name)
+            sampling = self._settings(body, {"prompt"})
             max_tokens = resolve_max_tokens(body)
             if body.get("prompt") is None:
                 raise bad_request("prompt is required")
             ids = self._prompt_ids(body["prompt"])
             self._check_validity(ids, max_tokens)
-            return await self._respond(request, ids, max_tokens, bool(body.get("stream")), chat=False)
+            return await self._respond(request, ids, max_tokens, bool(body.get("stream")), chat=False, sampling=sampling, model=body.get("model"))
         except HttpError as e:
             return e.response()
 
     async def chat_completions(self, request: web.Request) -> web.StreamResponse:
         try:
             body = await self._json(request)
-            if not self.allow_sampling:
-                check_greedy(body)
-            check_request(body, {"messages", "chat_template_kwargs"}, self.model_name)
+            sampling = self._settings(body, {"messages", "chat_template_kwargs"})
             max_tokens = resolve_max_tokens(body)
             opts = body.get("chat_template_kwargs") or {}
             if not isinstance(opts, dict) or any(k != "enable_thinking" for k in opts):
@@ -232,7 +265,8 @@ class Server:
                 if sum(1 for t in ids if t == token) != len(images):
                     raise bad_request("the rendered prompt does not hold one image placeholder token per image")
             self._check_validity(ids, max_tokens)
-            return await self._respond(request, ids, max_tokens, bool(body.get("stream")), chat=True, images=images)
+            return await self._respond(request, ids, max_tokens, bool(body.get("stream")), chat=True, images=images, sampling=sampling,
+                                       model=body.get("model"))
         except HttpError as e:
             return e.response()
 
@@ -240,13 +274,15 @@ class Server:
         return f"{'chatcmpl' if chat else 'cmpl'}-{int(time.time())}-{next(self._seq)}"
 
     async def _respond(self, request: web.Request, ids: list[int], max_tokens: int, stream: bool,
-                       chat: bool, images: list | None = None) -> web.StreamResponse:
+                       chat: bool, images: list | None = None, sampling: Sampling | None = None,
+                       model: str | None = None) -> web.StreamResponse:
+        model = model or self.model_name
         rid = self._new_id(chat)
         created = int(time.time())
         if max_tokens == 0:
-            return web.json_response(self._final_body(rid, created, chat, "", "length", len(ids), 0))
+            return web.json_response(self._final_body(rid, created, chat, "", "length", len(ids), 0, model))
         try:
-            req, q = self.backend.add_request(ids, max_tokens, images=images)
+            req, q = self.backend.add_request(ids, max_tokens, images=images, **self._choices(sampling, model))
         except Busy as e:
             return HttpError(409, str(e), etype="server_busy").response()
         except Unavailable as e:
@@ -269,7 +305,7 @@ class Server:
                 self.backend.abort(req)
                 raise
             text += detok.flush()
-            return web.json_response(self._final_body(rid, created, chat, text, reason, len(ids), n_out))
+            return web.json_response(self._final_body(rid, created, chat, text, reason, len(ids), n_out, model))
         # ---- SSE ----
         resp = web.StreamResponse(status=200, headers={"Content-Type": "text/event-stream", "Cache-Control": "no-cache"})
         await resp.prepare(request)
@@ -289,7 +325,7 @@ class Server:
                 choice = {"index": 0, "delta": delta, "finish_reason": finish}
             else:
                 choice = {"index": 0, "text": delta_text or "", "finish_reason": finish}
-            return {"id": rid, "object": obj, "created": created, "model": self.model_name, "choices": [choice]}
+            return {"id": rid, "object": obj, "created": created, "model": model, "choices": [choice]}
 
         try:
             if chat:
@@ -316,12 +352,16 @@ class Server:
         await resp.write_eof()
         return resp
 
+    def _choices(self, sampling: Sampling | None, model: str) -> dict:
+        adapter = model if model in self.adapters and model != self.model_name else None
+        return {k: v for k, v in (("sampling", sampling), ("adapter", adapter)) if v is not None}
+
     def _strip_eos(self, toks: list[int]) -> list[int]:
         eos = set(self.backend.eos_ids)
         return [t for t in toks if t not in eos]
 
     def _final_body(self, rid: str, created: int, chat: bool, text: str, reason: str | None, n_prompt: int,
-                    n_out: int) -> dict:
+                    n_out: int, model: str) -> dict:
         usage = {"prompt_tokens": n_prompt, "completion_tokens": n_out, "total_tokens": n_prompt + n_out}
         if chat:
             choice = {"index": 0, "message": {"role": "assistant", "content": text}, "finish_reason": reason}
@@ -329,7 +369,7 @@ class Server:
         else:
             choice = {"index": 0, "text": text, "finish_reason": reason}
             obj = "text_completion"
-        return {"id": rid, "object": obj, "created": created, "model": self.model_name, "choices": [choice],
+        return {"id": rid, "object": obj, "created": created, "model": model, "choices": [choice],
                 "usage": usage}
 
 
@@ -350,7 +390,8 @@ def run(model, port: int = 8080, host: str = "127.0.0.1", allow_sampling: bool =
     if getattr(model, "vision", None) is not None:
         placeholder = tk.decode([int(model.spec.extra["image_token_id"])])
     server = Server(backend, tk, model.name, chat_template or getattr(tk, "chat_template", None),
-                    capacity=model.settings.capacity, allow_sampling=allow_sampling, image_placeholder=placeholder)
+                    capacity=model.settings.capacity, allow_sampling=allow_sampling, image_placeholder=placeholder,
+                    adapters=tuple(model.engine.adapters.names) if model.engine.adapters is not None else ())
     try:
         web.run_app(server.app(), host=host, port=port, print=None)
     finally:
