@@ -16,6 +16,8 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
+from .sampling import renew
+
 
 @dataclass
 class BatchLayout:
@@ -202,6 +204,7 @@ class ForwardBatch:
             f = h.view(np.float32)
             u, t, k, p, m = (a[o: o + n] for a, o in ((f, L.uniforms), (f, L.temperature), (h, L.top_k), (f, L.top_p), (f, L.min_p)))
             u[:], t[:], k[:], p[:], m[:] = 0, 0, 0, 1, 0
+            renew(draws)
             for i, d in enumerate(draws):
                 if d is not None:
                     u[i] = d[0].uniform(d[1])

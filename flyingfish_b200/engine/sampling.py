@@ -9,7 +9,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-BLOCK = 256                      # numbers made at a time: the rounds are array operations, so a block costs little more than one number
+BLOCK = 64                       # numbers made at a time: the rounds are array operations, so a block costs little more than one number
 
 
 @dataclass(frozen=True)
@@ -37,18 +37,22 @@ class Sampling:
             raise ValueError("seed must be a whole number of 64 bits")
 
 
-def philox_uniforms(seed: int, start: int, n: int) -> np.ndarray:
-    """Numbers ``start .. start + n`` of a seed, FP32 in [0, 1): number i is word ``i % 4`` of block ``i // 4``, its upper 24 bits."""
+def philox_uniforms(seed, start, n: int) -> np.ndarray:
+    """Numbers ``start .. start + n`` of a seed, FP32 in [0, 1): number i is word ``i % 4`` of block ``i // 4``, its upper 24 bits. With lists of seeds and
+    starts (all of one remainder by 4) a row for each."""
     lo32, shift = np.uint64(0xFFFFFFFF), np.uint64(32)
-    block = np.arange(start // 4, (start + n + 3) // 4, dtype=np.uint64)
+    seeds, starts = np.atleast_1d(np.asarray(seed, dtype=np.uint64)), np.atleast_1d(np.asarray(start, dtype=np.uint64))
+    skip = int(starts[0]) % 4
+    block = starts[:, None] // np.uint64(4) + np.arange((skip + n + 3) // 4, dtype=np.uint64)
     c0, c1, c2, c3 = block & lo32, block >> shift, np.zeros_like(block), np.zeros_like(block)
-    k0, k1 = seed & 0xFFFFFFFF, seed >> 32
+    k0, k1 = (seeds & lo32)[:, None], (seeds >> shift)[:, None]
     for _ in range(10):
         p0, p1 = np.uint64(0xD2511F53) * c0, np.uint64(0xCD9E8D57) * c2
-        c0, c1, c2, c3 = (p1 >> shift) ^ c1 ^ np.uint64(k0), p1 & lo32, (p0 >> shift) ^ c3 ^ np.uint64(k1), p0 & lo32
-        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
-    words = np.stack((c0, c1, c2, c3), axis=1).reshape(-1)[start % 4: start % 4 + n]
-    return ((words >> np.uint64(8)).astype(np.float64) * 2.0 ** -24).astype(np.float32)
+        c0, c1, c2, c3 = (p1 >> shift) ^ c1 ^ k0, p1 & lo32, (p0 >> shift) ^ c3 ^ k1, p0 & lo32
+        k0, k1 = (k0 + np.uint64(0x9E3779B9)) & lo32, (k1 + np.uint64(0xBB67AE85)) & lo32
+    words = np.stack((c0, c1, c2, c3), axis=2).reshape(len(seeds), -1)[:, skip: skip + n]
+    out = ((words >> np.uint64(8)).astype(np.float64) * 2.0 ** -24).astype(np.float32)
+    return out if np.ndim(seed) else out[0]
 
 
 class Draws:
@@ -62,6 +66,14 @@ class Draws:
 
     def uniform(self, index: int) -> float:
         if index // BLOCK != self._block:
-            self._block = index // BLOCK
-            self._numbers = philox_uniforms(self.settings.seed, self._block * BLOCK, BLOCK)
+            renew([(self, index)])
         return self._numbers[index % BLOCK]
+
+
+def renew(draws: "list[tuple[Draws, int] | None]") -> None:
+    """Makes the blocks that a step's ``(Draws, index of the new token)`` lack, all at once: 64 together take the host as long as one does, 0.2 ms."""
+    need = [(d, i // BLOCK) for d, i in (e for e in draws if e is not None) if i // BLOCK != d._block]
+    if need:
+        numbers = philox_uniforms([d.settings.seed for d, _ in need], [b * BLOCK for _, b in need], BLOCK)
+        for (d, b), row in zip(need, numbers):
+            d._block, d._numbers = b, row
