@@ -4,8 +4,7 @@
 //   reaches P of the whole mass) and min-p (w_i >= min_p) leave, at least one;  drawn: lowest id whose sum of kept w up to it passes u times their sum.
 //
 // Ids are to be those of the formulas, so what decides is held in FP64: a row of 128 thousand flat tokens has borders 8e-6 of the mass apart, and
-// 32-bit sums move 128 thousand of them by 1e-7 each. Of the whole mass, tokens below 2^-24 of the largest are taken in FP32 with a compensated
-// exponent: together they are at most 1.6 % of it (V = 262144), so the mass is held to 4e-9 at worst and far better as their errors average.
+// 32-bit sums move 128 thousand of them by 1e-7 each. Tokens below 2^-64 of the largest are left out of the whole mass: 2^-46 of it at V = 262144.
 //
 // A cluster of C CTAs has a row: every CTA keeps its slice of the logits in shared memory, so that they come from memory once, and a warp a run of
 // consecutive ids of it. Values cross by stores into the peers' shared memory in front of a cluster barrier. Steps:
@@ -25,8 +24,8 @@
 namespace ff {
 
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CLUSTER = 8;
-constexpr int SM_BINS = 1024, SM_LIST = 1024, SM_SMALL = 256, SM_TABLE = 256, SM_PARTS = SM_CLUSTER * SM_WARPS;
-constexpr float SM_NEAR = -24.f, SM_FAR = -64.f;      // octaves below the largest: FP64 above the one, nothing below the other
+constexpr int SM_BINS = 1024, SM_LIST = 1024, SM_SMALL = 256, SM_TABLE = 32, SM_COPIES = 16, SM_PARTS = SM_CLUSTER * SM_WARPS;
+constexpr float SM_FAR = -64.f;         // octaves below the largest that count for the mass
 
 struct SampleArgs {
   const void* logits;
@@ -41,7 +40,7 @@ struct SampleArgs {
 struct SampleFound { int lo, hi, count, reached; unsigned above; };
 
 struct SampleShared {
-  double table[SM_TABLE];               // 2^(i / 256)
+  double table[SM_TABLE * SM_COPIES];   // 2^(i / 32), every lane of a half warp its own
   double mass[SM_CLUSTER];              // what every CTA of the cluster has pushed: the mass
   double part[SM_PARTS];                // CTA 0, general path: every warp's kept mass in front of the border's bins
   unsigned long long part_in[SM_PARTS]; // and within them, in units of 2^-50: whole numbers, so that the order of their sum does not matter
@@ -103,18 +102,20 @@ template <typename T> __device__ __forceinline__ void store_vec(T* p, const floa
 template <> __device__ __forceinline__ void store_vec<float>(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 template <> __device__ __forceinline__ void store_vec<__nv_bfloat16>(__nv_bfloat16* p, const float* v) { store8(p, *reinterpret_cast<const float(*)[8]>(v)); }
 
-// 2^x for -1000 < x <= 0: table of 2^(i / 256) and the Taylor polynomial of degree 3 for the rest |r| <= 1/512 (Tang, 1989); 1.4e-13 of the value
-__device__ __forceinline__ double exp2_table(double x, const double* table) {
-  constexpr double BIG = 6755399441055744.0 / 256;        // 1.5 * 2^52 / 256: the sum's last bits count 256ths
-  const double s = x + BIG;
+// 2^(d c) for -1000 < d c <= 0: table of 2^(i / 32) and the Taylor polynomial of degree 4 for the rest |r| <= 1/64 (Tang, 1989); 1.2e-12 of the value. The
+// table lies in shared memory 16 times over, a copy for each lane of a half warp, so that a warp's loads meet no conflicts.
+__device__ __forceinline__ double exp2_table(double d, double c, const double* table) {
+  constexpr double BIG = 6755399441055744.0 / 32;         // 1.5 * 2^52 / 32: the sum's last bits count 32nds
+  const double s = fma(d, c, BIG);
   const int n = __double2loint(s);
-  const double r = x - (s - BIG);
+  const double r = fma(d, c, BIG - s);
   constexpr double L = 0.693147180559945309417;
-  double p = fma(r, L * L * L / 6, L * L / 2);
+  double p = fma(r, L * L * L * L / 24, L * L * L / 6);
+  p = fma(p, r, L * L / 2);
   p = fma(p, r, L);
-  const double t = table[n & 255];
+  const double t = table[(n & 31) * SM_COPIES];
   p = fma(p * r, t, t);
-  return __hiloint2double(__double2hiint(p) + ((n >> 8) << 20), __double2loint(p));
+  return __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
 }
 __device__ __forceinline__ double power_of_2(int n) { return __hiloint2double((1023 + n) << 20, 0); }      // -1022 <= n <= 1023
 
@@ -145,13 +146,13 @@ __device__ __forceinline__ float ex2_approx(float x) { float y; asm("ex2.approx.
 struct SampleRow {
   float top;                            // the largest logit
   double c, wide_top;                   // log2(e) / T
-  float ch, cl;                         // c in two words
+  float ch;                             // c rounded
   float bins;                           // bins per unit of logit
   const double* table;
   // zero below 2^-1000
   __device__ __forceinline__ double weight(float l) const {
-    const double x = (widen(l) - wide_top) * c;
-    return l > -INFINITY && x > -1000.0 ? exp2_table(x, table) : 0.0;
+    const double d = widen(l) - wide_top;
+    return l > -INFINITY && d * c > -1000.0 ? exp2_table(d, c, table) : 0.0;
   }
   // octaves of a logit against the largest
   __device__ __forceinline__ float octaves(float l) const { return (l - top) * ch; }
@@ -255,7 +256,8 @@ sample_tokens_kernel(const SampleArgs a) {
   const int id0 = first + warp * a.seg;
   cluster_arrive_relaxed();                              // "this CTA runs": waited on before the first store into a peer
   pdl_trigger();
-  if (tid < SM_TABLE) sh.table[tid] = exp2(tid / 256.0);
+  static_assert(SM_TABLE * SM_COPIES == SM_THREADS, "a thread per entry");
+  sh.table[tid] = exp2((tid / SM_COPIES) / (double)SM_TABLE);
   if (tid == 0) sh.list_n = 0;
   pdl_wait();
   const float temp = a.temperature[row];
@@ -303,7 +305,7 @@ sample_tokens_kernel(const SampleArgs a) {
   }
   cluster_sync_all();
   SampleRow r;
-  r.table = sh.table;
+  r.table = sh.table + lane % SM_COPIES;
   r.top = sh.top[0];
   for (int i = 1; i < C; ++i) r.top = fmaxf(r.top, sh.top[i]);
   const bool greedy = !(temp > 0.f);
@@ -344,7 +346,6 @@ sample_tokens_kernel(const SampleArgs a) {
   r.wide_top = widen(r.top);
   r.c = 1.4426950408889634074 / (double)temp;
   r.ch = fminf((float)r.c, 1e30f);
-  r.cl = r.c < 1e30 ? (float)(r.c - (double)r.ch) : 0.f;
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
   // min-p as a logit: rounded up, so that for 32-bit logits the comparison is the one with the unrounded value
@@ -429,22 +430,21 @@ sample_tokens_kernel(const SampleArgs a) {
     }
   }
   if (use_p || !use_k) {
+    // the draw's mass is that of the kept tokens; what is further than SM_FAR octaves below the largest is 1e-14 of the whole at most, all together
     double s = 0.0;
-    float tail = 0.f;
-    const float from = use_p ? -INFINITY : least;        // the draw's mass is that of the kept tokens
-    const float lean = 0.69314718f * r.cl;               // what the first word of c leaves out
-    if (mine_top >= from && r.octaves(mine_top) > SM_FAR)
+    const float from = fmaxf(fmaxf(use_p ? -INFINITY : least, r.ch > 0.f ? r.top + SM_FAR / r.ch : -INFINITY), -3.4028235e38f);
+    if (mine_top >= from)
       for (int i = lane * VEC; i < a.seg; i += STEP) {
         float v[VEC];
         load_vec<T>(mine + i, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float d = v[e] - r.top, x = v[e] >= from ? d * r.ch : -INFINITY;
-          if (x > SM_NEAR) s += exp2_table((widen(v[e]) - r.wide_top) * r.c, sh.table);
-          else if (x > SM_FAR) tail = fmaf(ex2_approx(x), fmaf(lean, d, 1.f), tail);
+          const bool in = v[e] >= from;
+          const double w = exp2_table(widen(in ? v[e] : r.top) - r.wide_top, r.c, r.table);
+          if (in) s += w;
         }
       }
-    s = warp_sum64(s + (double)tail);
+    s = warp_sum64(s);
     if (lane == 0) sh.warp_sum[warp] = s;
   }
   __syncthreads();
@@ -818,11 +818,12 @@ static int sample_launch(const SampleArgs& args, int rows, cudaStream_t stream) 
   constexpr int STEP = 32 * (16 / (int)sizeof(T)), MOST = 227 * 1024;
   const int fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16;
   SampleArgs a = args;
-  auto fits = [&](int n) { return (long long)((a.V + n * SM_WARPS - 1) / (n * SM_WARPS) + STEP) * SM_WARPS * sizeof(T) + fixed <= MOST; };
-  // CTAs of 4096 tokens and more, and no more than the GPU holds; two to an SM only where each has 16384, for they share its FP64 units and slow the steps
-  // that wait (33 rows of 50257 FP32: 4 CTAs 18 us, 8 on shared SMs 21; 64 rows of 128256: 4 on shared SMs 58 us, 2 90).
+  // CTAs of 2048 tokens and more where each has an SM, of 6144 where two share one or rows wait: a CTA has about 15 us of steps that wait, which two on an
+  // SM overlap (V = 50257, C = 8 / 4: 8 rows 21 / 26 us, 64 34 / 37; 33 rows top-k only 21 / 18). No more than 4 CTAs per SM in all, unless larger ones would
+  // leave one to an SM (256 rows BF16, C = 8 / 4 / 2: V = 32000 71 / 50 / 45 us, V = 128256 127 / 111 / 156).
+  auto smem_of = [&](int n) { return (long long)((a.V + n * SM_WARPS - 1) / (n * SM_WARPS) + STEP) * SM_WARPS * sizeof(T) + fixed; };
   int c = SM_CLUSTER;
-  while (c > 1 && (a.V < 4096 * c || rows * c > (a.V < 16384 * c ? 1 : 2) * sm_count()) && fits(c / 2)) c /= 2;
+  while (c > 1 && smem_of(c / 2) <= MOST && (a.V < (rows * c > sm_count() ? 6144 : 2048) * c || (rows * c > 4 * sm_count() && 2 * (smem_of(c / 2) + 1024) <= 228 * 1024))) c /= 2;
   a.seg = (a.V + c * SM_WARPS - 1) / (c * SM_WARPS);
   a.seg = (a.seg + STEP - 1) / STEP * STEP;
   const long long smem = fixed + (long long)SM_WARPS * a.seg * sizeof(T);
