@@ -43,7 +43,7 @@ struct SampleShared {
   double table[SM_TABLE * SM_COPIES];   // 2^(i / 32), every lane of a half warp its own
   double mass[SM_CLUSTER];              // what every CTA of the cluster has pushed: the mass
   double part[SM_PARTS];                // CTA 0, general path: every warp's kept mass in front of the border's bins
-  unsigned long long part_in[SM_PARTS]; // and within them, in units of 2^-50: whole numbers, so that the order of their sum does not matter
+  unsigned part_in[SM_PARTS][3];        // and within them, whole numbers of 2^-10, 2^-30 and 2^-50, so that the order of their sum does not matter
   double warp_sum[SM_WARPS], scan_mass[SM_WARPS];
   double total, from;
   float top[SM_CLUSTER], cut[SM_CLUSTER], warp_top[SM_WARPS];
@@ -177,9 +177,9 @@ __device__ __forceinline__ double block_scan(double v, SampleShared& sh, int war
   return before;
 }
 
-// list[0 .. n) in descending order, entries distinct. Few entries count the larger ones, several threads per entry; more are placed by bins of their upper
-// halves first and count within their bin (a bitonic sort in shared memory took 5.5 us for 458 entries and 9 for 750, this 2; by counting 256 take 1.5).
-__device__ __forceinline__ void sort_list(SampleShared& sh, int n, int tid, int warp, int lane) {
+// list[0 .. n) in descending order, entries distinct, their lower halves within `span` from `base` on. Few entries count the larger ones, several threads per
+// entry; more are placed by bins of both halves first, so that ties of one key spread over them, and count within their bin (a bitonic sort in shared memory took 5.5 us for 458 entries and 9 for 750, this 2; by counting 256 take 1.5).
+__device__ __forceinline__ void sort_list(SampleShared& sh, int n, unsigned span, unsigned base, int tid, int warp, int lane) {
   if (n <= SM_SMALL) {
     int n2 = 1;
     while (n2 < n) n2 <<= 1;
@@ -209,14 +209,20 @@ __device__ __forceinline__ void sort_list(SampleShared& sh, int n, int tid, int 
   high = __reduce_max_sync(0xffffffffu, high);
   if (lane == 0) { atomicMin(&sh.reduce[0], low); atomicMax(&sh.reduce[1], high); }
   __syncthreads();
-  high = sh.reduce[1];
-  const float scale = (float)(BINS - 1) / fmaxf((float)(high - sh.reduce[0]), 1.f);
+  // distances from the end of the highest key's range: whole numbers below 2^32 * 2^31
+  const unsigned lowest = sh.reduce[0];
+  const unsigned long long top = ((unsigned long long)(sh.reduce[1] - lowest) + 1) * span;
+  const float scale = (float)(BINS - 1) / (float)top;
   int bin[PER];
   unsigned slot[PER];
 #pragma unroll
   for (int q = 0; q < PER; ++q) {
-    bin[q] = min((int)((float)(high - (unsigned)(me[q] >> 32)) * scale), BINS - 1);
-    if (tid + q * SM_THREADS < n) slot[q] = atomicAdd(&sh.place[bin[q]], 1u);
+    bin[q] = 0;
+    if (tid + q * SM_THREADS < n) {
+      const unsigned long long at = (unsigned long long)((unsigned)(me[q] >> 32) - lowest) * span + ((unsigned)me[q] - base);
+      bin[q] = min((int)((float)(top - at) * scale), BINS - 1);
+      slot[q] = atomicAdd(&sh.place[bin[q]], 1u);
+    }
   }
   __syncthreads();
   unsigned c[PER], sum = 0;
@@ -253,10 +259,10 @@ __device__ __forceinline__ void sort_list(SampleShared& sh, int n, int tid, int 
 // `mass_above` stand in front of the list. Returns how many of the list are kept, and their mass with mass_above in sh.total.
 template <typename T>
 __device__ __forceinline__ int find_border(SampleShared& sh, const SampleRow& r, int n, unsigned above, double mass_above, bool use_k, int k, bool use_p, double target,
-                                           int tid, int warp, int lane) {
+                                           int V, int tid, int warp, int lane) {
   if (tid == 0) sh.at = n - 1;
   __syncthreads();
-  sort_list(sh, n, tid, warp, lane);
+  sort_list(sh, n, (unsigned)V, ~(unsigned)(V - 1), tid, warp, lane);
   const int per = (n + SM_THREADS - 1) / SM_THREADS, first = min(n, tid * per), last = min(n, first + per);
   double mine = 0.0;
   for (int i = first; i < last; ++i) { const double w = r.weight(logit_of<T>((unsigned)(sh.list[i] >> 32))); sh.w[i] = w; mine += w; }
@@ -385,6 +391,7 @@ sample_tokens_kernel(const SampleArgs a) {
   r.ch = fminf((float)r.c, 1e30f);
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
+  const float far = r.ch > 0.f ? r.top + SM_FAR / r.ch : -INFINITY;      // what lies lower is 1e-14 of the whole mass at most, all together
   // min-p as a logit: rounded up, so that for 32-bit logits the comparison is the one with the unrounded value
   float least = -INFINITY;
   if (floor_p > 0.f && temp < INFINITY) least = fminf(r.top, __double2float_ru((double)r.top + (double)temp * log((double)fminf(floor_p, 1.f))));
@@ -467,9 +474,9 @@ sample_tokens_kernel(const SampleArgs a) {
     }
   }
   if (use_p || !use_k) {
-    // the draw's mass is that of the kept tokens; what is further than SM_FAR octaves below the largest is 1e-14 of the whole at most, all together
+    // the draw's mass is that of the kept tokens
     double s = 0.0;
-    const float from = fmaxf(fmaxf(use_p ? -INFINITY : least, r.ch > 0.f ? r.top + SM_FAR / r.ch : -INFINITY), -3.4028235e38f);
+    const float from = fmaxf(fmaxf(use_p ? -INFINITY : least, far), -3.4028235e38f);
     if (mine_top >= from)
       for (int i = lane * VEC; i < a.seg; i += STEP) {
         float v[VEC];
@@ -542,7 +549,7 @@ sample_tokens_kernel(const SampleArgs a) {
     for (int i = 0; i < C; ++i) { all += sh.candidates[i]; most = max(most, sh.candidates[i]); }
     if (most <= share) {
       if (rank != 0) return;
-      const int kept = find_border<T>(sh, r, all, 0, 0.0, use_k, k, use_p, target, tid, warp, lane);
+      const int kept = find_border<T>(sh, r, all, 0, 0.0, use_k, k, use_p, target, a.V, tid, warp, lane);
       const double goal = (double)u * sh.total;
       // the kept ones by id: ~id << 32 | place, descending
       const int per_thread = (kept + SM_THREADS - 1) / SM_THREADS;
@@ -557,7 +564,7 @@ sample_tokens_kernel(const SampleArgs a) {
       for (int q = 0; q < SM_LIST / SM_THREADS; ++q) { const int i = tid + q * SM_THREADS; if (i < kept) sh.list[i] = hold[q]; }
       if (tid == 0) { sh.at = 0x7fffffff; sh.list_n = -1; }
       __syncthreads();
-      sort_list(sh, kept, tid, warp, lane);
+      sort_list(sh, kept, SM_LIST, 0u, tid, warp, lane);
       const int f0 = min(kept, tid * per_thread), f1 = min(kept, f0 + per_thread);
       double mass = 0.0, total;
       for (int i = f0; i < f1; ++i) mass += sh.w[(unsigned)sh.list[i]];
@@ -725,27 +732,43 @@ sample_tokens_kernel(const SampleArgs a) {
       if ((use_k && above + n_upper >= (unsigned)k) || (use_p && n_upper > 0 && upper >= target)) { key_lo = mid; left = n_upper; }
       else { key_hi = mid - 1; above += n_upper; left -= n_upper; }
     }
-    // the mass in front of the border's bins (and keys) in FP64, warp by warp; the tokens among which it lies into CTA 0's list
+    // the mass in front of the border's bins (and keys) in FP64, warp by warp, without branches; the tokens among which the border lies into CTA 0's list
     double m = 0.0;
     unsigned n_ties = 0;
+    // bins as numbers that r.bin rounds down: no number reaches the first one behind the last bin, nor NaN, which stands for it
+    const float lo_x = lo < SM_BINS ? (float)lo : __uint_as_float(0x7fffffffu), hi_x = hi < SM_BINS - 1 ? (float)(hi + 1) : __uint_as_float(0x7fffffffu);
+    const float cut_in = fmaxf(cut, -3.4028235e38f), heavy = fmaxf(cut_in, far);
+    auto at_border = [&](float l) {
+      const float x = (r.top - l) * r.bins;
+      const unsigned key = key_of<T>(l);
+      return l >= cut_in && x >= lo_x && !(x >= hi_x) && key >= key_lo && key <= key_hi;
+    };
     __syncthreads();                                     // the histogram's place is the list's
-    if (some)
+    if (some) {
       for (int i = lane * VEC; i < a.seg; i += STEP) {
         float v[VEC];
         load_vec<T>(mine + i, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          if (!(v[e] >= cut) || v[e] == -INFINITY) continue;
-          const int b = r.bin(v[e]);
-          if (b > hi && lo < SM_BINS) continue;
+          const float x = (r.top - v[e]) * r.bins;
           const unsigned key = key_of<T>(v[e]);
-          if (b < lo || key > key_hi) m += r.weight(v[e]);
-          else if (key >= key_lo) {
-            if (ties) ++n_ties;
-            else push_u64(&sh.list[push_take(&sh.list_n, 0, 1)], 0, (unsigned long long)key << 32 | (unsigned)~(id0 + i + e));
-          }
+          const bool until = !(x >= hi_x), front = !(x >= lo_x) || (until && key > key_hi), weighs = v[e] >= heavy;
+          const double w = exp2_table(widen(weighs ? v[e] : r.top) - r.wide_top, r.c, r.table);
+          if (weighs && front) m += w;
+          n_ties += v[e] >= cut_in && until && !front && key >= key_lo;
         }
       }
+      if (n_ties > 0 && !ties) {
+        unsigned slot = push_take(&sh.list_n, 0, n_ties);
+        for (int i = lane * VEC; i < a.seg; i += STEP) {
+          float v[VEC];
+          load_vec<T>(mine + i, v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (at_border(v[e])) push_u64(&sh.list[slot++], 0, (unsigned long long)key_of<T>(v[e]) << 32 | (unsigned)~(id0 + i + e));
+        }
+      }
+    }
     m = warp_sum64(m);
     n_ties = __reduce_add_sync(0xffffffffu, n_ties);
     if (lane == 0) {
@@ -798,12 +821,16 @@ sample_tokens_kernel(const SampleArgs a) {
         double front = 0.0;
         for (int i = tid; i < C * SM_WARPS; i += SM_THREADS) front += sh.part[i];
         block_scan(front, sh, warp, lane, mass_above);
-        const int kept = find_border<T>(sh, r, left, above, mass_above, use_k, k, use_p, target, tid, warp, lane);
-        if (tid < SM_PARTS) sh.part_in[tid] = 0;
+        const int kept = find_border<T>(sh, r, left, above, mass_above, use_k, k, use_p, target, a.V, tid, warp, lane);
+        if (tid < SM_PARTS) { sh.part_in[tid][0] = 0; sh.part_in[tid][1] = 0; sh.part_in[tid][2] = 0; }
         __syncthreads();
-        for (int i = tid; i < kept; i += SM_THREADS) atomicAdd(&sh.part_in[(int)~(unsigned)sh.list[i] / a.seg], (unsigned long long)(sh.w[i] * 1125899906842624.0));
+        for (int i = tid; i < kept; i += SM_THREADS) {
+          const unsigned long long w = (unsigned long long)(sh.w[i] * 1125899906842624.0);        // 2^50 and less
+          unsigned* part = sh.part_in[(int)~(unsigned)sh.list[i] / a.seg];
+          atomicAdd(part, (unsigned)(w >> 40)); atomicAdd(part + 1, (unsigned)(w >> 20) & 0xfffffu); atomicAdd(part + 2, (unsigned)w & 0xfffffu);
+        }
         __syncthreads();
-        if (tid < C * SM_WARPS) sh.part[tid] += (double)sh.part_in[tid] * (1.0 / 1125899906842624.0);
+        if (tid < C * SM_WARPS) sh.part[tid] += (((double)sh.part_in[tid][0] * 1048576.0 + sh.part_in[tid][1]) * 1048576.0 + sh.part_in[tid][2]) * (1.0 / 1125899906842624.0);
         if (tid == 0) { sh.border_key = (unsigned)(sh.list[kept - 1] >> 32); sh.border_id = (int)~(unsigned)sh.list[kept - 1]; }
       } else if (tid == 0) {
         sh.border_key = ties ? key_lo : 0u;
