@@ -270,7 +270,7 @@ def _check_sampling(args) -> None:
         raise SystemExit(f"{what}: speculative decoding compares with the base model's greedy tokens")
     if args.prefix_cache:
         raise SystemExit(f"{what}: the prefix cache holds the base model's keys and its greedy token")
-    if args.tp > 1 and (adapters or args.command == "generate"):
+    if args.tp > 1:
         raise SystemExit(f"{what} with --tp is not supported")
 
 

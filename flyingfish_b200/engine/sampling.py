@@ -4,7 +4,6 @@ The number for the token at index ``i`` of a sequence is a function of the reque
 so a request gives the same tokens whatever it is batched with, and goes on with the same numbers after it was preempted and recomputed."""
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -23,7 +22,7 @@ class Sampling:
     seed: int = 0
 
     def __post_init__(self) -> None:
-        number = lambda v: isinstance(v, (int, float)) and not isinstance(v, bool) and math.isfinite(v)
+        number = lambda v: isinstance(v, (int, float)) and not isinstance(v, bool)          # NaN is in no range
         whole = lambda v: isinstance(v, int) and not isinstance(v, bool)
         if not number(self.temperature) or not 0 <= self.temperature <= 1e6:
             raise ValueError("temperature must be a number from 0 to 1e6")

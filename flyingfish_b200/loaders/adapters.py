@@ -61,7 +61,8 @@ def _pattern(patterns: dict, module: str, default):
 
 def read_adapter(path: str | Path) -> Entries:
     """An adapter directory's matrices with their scales (``lora_alpha / r``, or over its root where the configuration says so). What this framework
-    has no place for -- other adapter kinds, trained biases, whole modules, embeddings -- is refused by name."""
+    has no place for -- other adapter kinds, trained biases, whole modules, embeddings -- is refused by name. The matrices keep the file's type here and are rounded
+    to the weights' when the stacks are built, as the products read them."""
     path = Path(path)
     config, weights = (path / f for f in FILES)
     if not config.is_file() or not weights.is_file():
@@ -74,11 +75,13 @@ def read_adapter(path: str | Path) -> Entries:
         raise AdapterError(f"{config}: not a LoRA adapter")
     if cfg.get("bias", "none") != "none" or cfg.get("modules_to_save"):
         raise AdapterError(f"{config}: trained biases and whole modules are not supported")
-    for key in ("use_dora", "fan_in_fan_out", "lora_bias", "use_qalora", "trainable_token_indices", "alora_invocation_tokens"):
+    for key in ("use_dora", "fan_in_fan_out", "lora_bias", "use_qalora", "trainable_token_indices", "alora_invocation_tokens", "layer_replication"):
         if cfg.get(key):
             raise AdapterError(f"{config}: {key} is not supported")
     alpha, root = cfg.get("lora_alpha", 8), bool(cfg.get("use_rslora"))
     alphas = cfg.get("alpha_pattern") or {}
+    if not isinstance(alphas, dict) or any(re.fullmatch(r"[\w.]+", k) is None for k in alphas):
+        raise AdapterError(f"{config}: alpha_pattern takes module paths or ends of them, not expressions")
     found: dict[tuple[int, str], dict] = {}
     f = SafetensorsFile(weights)
     for name in f.tensors:

@@ -45,6 +45,8 @@ class NoComm:
 
 
 class DecoderModel:
+    _adapters: tuple | None = None         # per-forward (stacks of every layer, adapter id of every row), or None
+
     def __init__(self, weights: ModelWeights, comm=None, trace=None):
         self.w = weights
         self.spec: ModelSpec = weights.spec
@@ -60,7 +62,6 @@ class DecoderModel:
         self.normed_sink: list | None = None      # when a list: every forward appends its final-normed rows
         self.last_logits: torch.Tensor | None = None   # logits of the latest forward (a captured step keeps its own)
         self._rope_cs: torch.Tensor | None = None  # per-forward cos/sin table of the fused QKV kernels
-        self._adapters: tuple | None = None        # per-forward (stacks of every layer, adapter id of every row), or None
         # encoders and diffusion language models attend in both directions inside a sequence; they run whole
         # sequences in one prefill chunk and never decode
         self.bidirectional = bool(self.spec.extra.get("bidirectional"))
@@ -104,11 +105,10 @@ class DecoderModel:
         ad = self._adapters
         stacks, rows = (None, None) if ad is None else (ad[0][i], ad[1])
         if stacks is not None and stacks.gu is not None:
-            if lw.wgu_interleaved and lw.wgu.shape[0] % 256 == 0:
+            if lw.wgu_interleaved:
                 hmid = lora_ops.linear_swiglu_lora(n, lw.wgu, stacks.gu, rows, mode=self.spec.swiglu_mode)
             else:
-                gu = lora_ops.linear_lora(n, lw.wgu, stacks.gu, rows)
-                hmid = (ops.silu_mul_interleaved if lw.wgu_interleaved else ops.silu_mul)(gu, mode=self.spec.swiglu_mode)
+                hmid = ops.silu_mul(lora_ops.linear_lora(n, lw.wgu, stacks.gu, rows), mode=self.spec.swiglu_mode)
         elif lw.wgu_interleaved:
             hmid = ops.linear_swiglu(n, lw.wgu, mode=self.spec.swiglu_mode)
         else:

@@ -4,7 +4,7 @@
 //   reaches P of the whole mass) and min-p (w_i >= min_p) leave, at least one;  drawn: lowest id whose sum of kept w up to it passes u times their sum.
 //
 // Ids are to be those of the formulas, so what decides is held in FP64: a row of 128 thousand flat tokens has borders 8e-6 of the mass apart, and
-// 32-bit sums move 128 thousand of them by 1e-7 each. Tokens below 2^-64 of the largest are left out of the whole mass: 2^-46 of it at V = 262144.
+// 32-bit sums move 128 thousand of them by 1e-7 each.
 //
 // A cluster of C CTAs has a row: every CTA keeps its slice of the logits in shared memory, so that they come from memory once, and a warp a run of
 // consecutive ids of it. Values cross by stores into the peers' shared memory in front of a cluster barrier. Steps:
@@ -25,7 +25,7 @@ namespace ff {
 
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CLUSTER = 8;
 constexpr int SM_BINS = 1024, SM_LIST = 1024, SM_SMALL = 128, SM_TABLE = 32, SM_COPIES = 16, SM_PARTS = SM_CLUSTER * SM_WARPS;
-constexpr float SM_FAR = -64.f;         // octaves below the largest that count for the mass
+constexpr float SM_FAR = -1000.f;       // octaves below the largest from which on a token weighs nothing
 
 struct SampleArgs {
   const void* logits;
@@ -153,7 +153,7 @@ struct SampleRow {
   // zero below 2^-1000
   __device__ __forceinline__ double weight(float l) const {
     const double d = widen(l) - wide_top;
-    return l > -INFINITY && d * c > -1000.0 ? exp2_table(d, c, table) : 0.0;
+    return l > -INFINITY && d * c > SM_FAR ? exp2_table(d, c, table) : 0.0;
   }
   // octaves of a logit against the largest
   __device__ __forceinline__ float octaves(float l) const { return (l - top) * ch; }
@@ -391,7 +391,7 @@ sample_tokens_kernel(const SampleArgs a) {
   r.ch = fminf((float)r.c, 1e30f);
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
-  const float far = r.ch > 0.f ? r.top + SM_FAR / r.ch : -INFINITY;      // what lies lower is 1e-14 of the whole mass at most, all together
+  const float far = r.ch > 0.f ? r.top + SM_FAR / r.ch : -INFINITY;
   // min-p as a logit: rounded up, so that for 32-bit logits the comparison is the one with the unrounded value
   float least = -INFINITY;
   if (floor_p > 0.f && temp < INFINITY) least = fminf(r.top, __double2float_ru((double)r.top + (double)temp * log((double)fminf(floor_p, 1.f))));
@@ -424,9 +424,10 @@ sample_tokens_kernel(const SampleArgs a) {
     __syncthreads();
     if (warp != 0) return;
     const double mine_sum = lane < steps ? sh.step_sum[lane] : 0.0, upto_step = warp_scan64(mine_sum, lane);
-    const unsigned starts = __ballot_sync(0xffffffffu, mine_sum > 0.0 && from + (upto_step - mine_sum) <= goal);
+    // the first step that passes, or the last one of any mass, as for tokens below
+    const unsigned ends = __ballot_sync(0xffffffffu, mine_sum > 0.0 && from + upto_step > goal);
     const unsigned any_step = __ballot_sync(0xffffffffu, mine_sum > 0.0);
-    const int step = starts ? 31 - __clz(starts) : __ffs(any_step) - 1;
+    const int step = ends ? __ffs(ends) - 1 : 31 - __clz(any_step);
     const double before = from + __shfl_sync(0xffffffffu, upto_step - mine_sum, step);
     const double sum = weigh(step, w);
     const double upto = warp_scan64(sum, lane);
@@ -825,7 +826,8 @@ sample_tokens_kernel(const SampleArgs a) {
         if (tid < SM_PARTS) { sh.part_in[tid][0] = 0; sh.part_in[tid][1] = 0; sh.part_in[tid][2] = 0; }
         __syncthreads();
         for (int i = tid; i < kept; i += SM_THREADS) {
-          const unsigned long long w = (unsigned long long)(sh.w[i] * 1125899906842624.0);        // 2^50 and less
+          // 2^50 and less; what weighs anything is at least a unit, so that its warp is seen to hold some
+          const unsigned long long w = max((unsigned long long)(sh.w[i] * 1125899906842624.0), sh.w[i] > 0.0 ? 1ull : 0ull);
           unsigned* part = sh.part_in[(int)~(unsigned)sh.list[i] / a.seg];
           atomicAdd(part, (unsigned)(w >> 40)); atomicAdd(part + 1, (unsigned)(w >> 20) & 0xfffffu); atomicAdd(part + 2, (unsigned)w & 0xfffffu);
         }
@@ -841,11 +843,12 @@ sample_tokens_kernel(const SampleArgs a) {
       double all_parts;
       const double from = block_scan(mine_part, sh, warp, lane, all_parts);
       const double goal = (double)u * all_parts;
-      if (tid == 0) { sh.total = all_parts; sh.owner = -1; sh.at = -1; }
+      if (tid == 0) { sh.total = all_parts; sh.owner = SM_PARTS; sh.at = 0; }
       __syncthreads();
-      if (mine_part > 0.0) { atomicMax(&sh.owner, from <= goal ? tid : -1); }
+      // the first warp whose end passes the goal; the sums' last bits may leave it behind the last one
+      if (mine_part > 0.0) { if (from + mine_part > goal) atomicMin(&sh.owner, tid); atomicMax(&sh.at, tid); }
       __syncthreads();
-      const int owner = sh.owner;
+      const int owner = min(sh.owner, sh.at);
       if (tid == owner) sh.from = from;
       __syncthreads();
       if (tid > 0 && tid < C) {

@@ -24,7 +24,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
     at least ``min_p`` times the largest probability (all at 0 or less, those of the largest from 1 on). Drawn is the lowest id whose sum of kept masses up to it
     passes ``uniforms`` times their sum. ``temperature`` 0 or less: the lowest id of the largest logit, probability 1. NaN logits count as -inf, which is
     never drawn, and +inf shares everything among its equals; a row of -inf gives id 0 with probability 0. Masses are those of 64-bit arithmetic; one
-    below 2^-1000 of the largest counts as none."""
+    below 2^-1000 of the largest counts as none. On a GPU a row lies in the shared memory of 8 multiprocessors: 380 thousand FP32 tokens or 760 thousand BF16
+    ones, and there are 65535 rows at most."""
     rows, ld = _rows2d(logits)
     at = logits.get_device()
     vocab = logits.shape[1]

@@ -76,7 +76,7 @@ def test_numbers_are_those_of_the_counter_based_generator(seed):
     assert [float(d.uniform(i)) for i in asked] == [float(philox_uniforms(seed, i, 1)[0]) for i in asked]
 
 
-@pytest.mark.parametrize("bad", [{"temperature": -1}, {"temperature": float("nan")}, {"temperature": "1"}, {"temperature": True}, {"top_k": -1},
+@pytest.mark.parametrize("bad", [{"temperature": -1}, {"temperature": float("nan")}, {"temperature": "1"}, {"temperature": True}, {"temperature": 10 ** 400}, {"top_k": -1},
                                  {"top_k": 1.5}, {"top_k": 1 << 31}, {"top_p": 0}, {"top_p": 1.01}, {"min_p": -0.1}, {"min_p": 2}, {"seed": -1},
                                  {"seed": 1 << 64}, {"seed": None}])
 def test_settings_are_checked(bad):
@@ -114,7 +114,7 @@ def test_an_adapter_directory_is_read(tmp_path):
 
 
 @pytest.mark.parametrize("config", [{"peft_type": "IA3"}, {"bias": "all"}, {"modules_to_save": ["lm_head"]}, {"use_dora": True}, {"fan_in_fan_out": True},
-                                    {"lora_alpha": "x"}, {"lora_alpha": float("inf")}])
+                                    {"lora_alpha": "x"}, {"lora_alpha": float("inf")}, {"alpha_pattern": {".*q_proj": 4}}, {"layer_replication": [[0, 2]]}])
 def test_adapter_kinds_without_a_place_are_refused(tmp_path, config):
     with pytest.raises(AdapterError):
         read_adapter(_write_adapter(tmp_path / "a", _entries(4, 1), config))

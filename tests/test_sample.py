@@ -49,8 +49,8 @@ def _check(logits, u, t, k=None, p=None, m=None):
     want, want_p = _want(logits, u, t, k, p, m)
     bad = torch.nonzero(ids.cpu() != want).flatten().tolist()
     assert not bad, f"rows {bad[:5]}: {ids.cpu()[bad[:5]].tolist()} for {want[bad[:5]].tolist()}"
-    # rounded once from a quotient whose parts are held to a few 1e-13
-    assert ((probs.double().cpu() - want_p).abs() <= want_p * (2.0 ** -24 + 1e-11)).all()
+    # rounded once from a quotient whose parts are held to a few 1e-12; below 2^-126 numbers lie 2^-149 apart, so half a step is 2^-150 whatever the value
+    assert ((probs.double().cpu() - want_p).abs() <= want_p * (2.0 ** -24 + 1e-11) + 2.0 ** -150).all()
 
 
 def _settings(rows, seed, device):
@@ -217,3 +217,26 @@ def test_refusals_on_the_device(cuda):
     with pytest.raises(KernelError):
         sample_ops.sample_tokens(torch.zeros(1, 2_000_000, device=cuda), v[:1], v[:1])       # more than a cluster's shared memory holds
     ops.check_status(cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["normal", "peaked", "steps"])
+def test_long_prefixes_at_extreme_temperatures(cuda, kind, dtype):
+    """Prefixes of more tokens than a list holds, whose last ones weigh nothing, next to nothing, or as much as the first."""
+    rows, vocab = 24, 30011
+    l = _logits(kind, rows, vocab, dtype, 21, cuda)
+    f = lambda v: torch.tensor([v[i % len(v)] for i in range(rows)], device=cuda)
+    for min_p in (None, f([0.0, 1e-30, 1e-3])):
+        for top_p in (None, f([0.9999999, 1.0])):
+            _check(l, f([0.0, 0.3, 0.99999, 0.7, 0.999999]), f([1e-6, 1e-3, 0.05, 1.0, 40.0, 1e6, 3e-39]), f([1500, 5000, 30010, 1025]).to(torch.int32), top_p, min_p)
+
+
+@pytest.mark.gpu
+def test_rows_that_no_shared_memory_holds_are_refused(cuda):
+    one = lambda: torch.zeros(1, device=cuda)
+    for vocab, dtype in ((786433, BF16), (393217, F32)):
+        with pytest.raises(KernelError):
+            sample_ops.sample_tokens(torch.zeros(1, vocab, dtype=dtype, device=cuda), one(), one())
+        ids, p = sample_ops.sample_tokens(torch.zeros(1, vocab - 1, dtype=dtype, device=cuda), one() + 0.5, one() + 1)
+        assert abs(int(ids[0]) - (vocab - 1) // 2) <= 1 and float(p[0]) == pytest.approx(1 / (vocab - 1), rel=1e-6)
