@@ -17,6 +17,7 @@ constexpr int LS_SPLIT = 8;          // CTAs of a cluster share K
 constexpr int LS_ROWS = 128;         // rows of a tile: lanes of tensor memory
 constexpr int LS_COLS = 256;         // most columns of the accumulator: units of BW rank rows of a pass
 constexpr int LS_STAGES = 8;         // most stages
+constexpr int LS_SMEM = 220 * 1024;  // most shared memory
 constexpr int LS_TABLE = 128;        // stacks of at most so many adapters have their ranks and scales read ahead of the ids
 
 struct alignas(16) ShrinkShared {
@@ -240,12 +241,16 @@ static int lora_shrink(const FfLora& c, int bw, cudaStream_t stream) {
   if (c.M > LS_ROWS) most = per < 64 / bw ? 64 / bw : per > 128 / bw ? 128 / bw : per;
   most = most > units ? units : most;
   most = most > LS_COLS / bw ? LS_COLS / bw : most;
+  // two stages and the partial sums have to fit an SM: 128 rows leave room for passes of 224 columns
+  auto stage_of = [&](int n) { return xrows * 128 + n * bw * 128; };
+  auto recv_of = [&](int n) { return n * LS_SPLIT * 16 * bw * 4; };
+  while (most > 1 && 1024 + 2 * stage_of(most) + recv_of(most) > LS_SMEM) --most;
   int passes = (units + most - 1) / most;
   passes = passes < lanes ? passes : lanes;
   CUtensorMap tmX, tmA;
   if (int e = make_tmap_2d(&tmX, c.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.K, c.M, (uint64_t)c.ldx * 2, 64, xrows)) return e;
   if (int e = make_tmap_2d(&tmA, c.a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.K, (uint64_t)c.adapters * c.R, (uint64_t)c.K * 2, 64, bw)) return e;
-  const int stage = xrows * 128 + most * bw * 128, kb = ((c.K + 63) / 64 + LS_SPLIT - 1) / LS_SPLIT, recv = most * LS_SPLIT * 16 * bw * 4;
+  const int stage = stage_of(most), kb = ((c.K + 63) / 64 + LS_SPLIT - 1) / LS_SPLIT, recv = recv_of(most);
   // two CTAs on an SM for prompts; for decode rows so little that one fits beside a CTA of the product (7 rows, 4096 x 14336: 29.0 -> 24.6 us)
   int stages = ((c.M > LS_ROWS ? 108 : 40) * 1024 - recv) / stage;
   stages = stages > LS_STAGES ? LS_STAGES : stages < 2 ? 2 : stages;
@@ -253,7 +258,7 @@ static int lora_shrink(const FfLora& c, int bw, cudaStream_t stream) {
   // the instruction reads 128 rows of X, past the loaded ones into what lies behind them
   const int slack = stage < LS_ROWS * 128 ? LS_ROWS * 128 - stage : 0, recv_off = stages * stage, smem = 1024 + recv_off + (recv > slack ? recv : slack);
   auto kern = bw == 32 ? lora_shrink_kernel<32> : lora_shrink_kernel<16>;
-  if (int e = opt_in_smem(kern, 220 * 1024)) return e;
+  if (int e = opt_in_smem(kern, LS_SMEM)) return e;
   const LoraArgs args = {c.ids, c.ranks, c.part_of, c.adapters, c.R, c.parts, bw};
   return launch_pdl(kern, dim3(LS_SPLIT, passes, tiles), dim3(192), smem, stream, LS_SPLIT, tmX, tmA, args, c.scale,
                     static_cast<__nv_bfloat16*>(c.t), c.M, c.K, xrows, most, stages, recv_off, c.status);

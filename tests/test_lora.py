@@ -139,6 +139,17 @@ def test_against_64_bits(cuda, m, k, n, r, count):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,r", [(128, 96), (120, 80), (97, 256), (128, 1024), (100, 1008), (300, 512)])
+def test_an_adapter_for_every_row(cuda, m, r):
+    """As many units as a tile can have: passes as wide as shared memory allows."""
+    x, w, st, _ = _case(m, 256, 192, r, m, seed=r, device=cuda)
+    ids = torch.arange(m, dtype=torch.int32, device=cuda).flip(0).contiguous()
+    y, size = _exact(x, w, st, ids)
+    _assert_near(lora_ops.linear_lora(x, w, st, ids), y, size)
+    ops.check_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [5, 64, 128, 300, 700])
 def test_a_row_does_not_depend_on_its_neighbours(cuda, m):
     x, w, st, ids = _case(m, 1024, 768, 32, 6, seed=3, device=cuda)
