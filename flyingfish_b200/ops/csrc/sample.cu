@@ -178,7 +178,8 @@ __device__ __forceinline__ double block_scan(double v, SampleShared& sh, int war
 }
 
 // list[0 .. n) in descending order, entries distinct, their lower halves within `span` from `base` on. Few entries count the larger ones, several threads per
-// entry; more are placed by bins of both halves first, so that ties of one key spread over them, and count within their bin (a bitonic sort in shared memory took 5.5 us for 458 entries and 9 for 750, this 2; by counting 256 take 1.5).
+// entry; more are placed by bins of both halves first, so that ties of one key spread over them, and count within their bin (a bitonic sort in
+// shared memory took 5.5 us for 458 entries and 8.5 for 750, this 1.5 and 3.5).
 __device__ __forceinline__ void sort_list(SampleShared& sh, int n, unsigned span, unsigned base, int tid, int warp, int lane) {
   if (n <= SM_SMALL) {
     int n2 = 1;
@@ -397,8 +398,8 @@ sample_tokens_kernel(const SampleArgs a) {
   if (floor_p > 0.f && temp < INFINITY) least = fminf(r.top, __double2float_ru((double)r.top + (double)temp * log((double)fminf(floor_p, 1.f))));
 
   // The draw within the run of ids of warp `owner` of this CTA, by all of its warps: the lowest id at which the sum of kept weights, `from` in front of
-  // the run, passes the goal. Shared memory holds runs of 28 steps at most; their sums first, then the step's tokens (48 rows of 128256: 30 us, 38 where
-  // one warp walks step by step).
+  // the run, passes the goal. Shared memory holds runs of 28 steps at most; their sums first, then the step's tokens (48 rows of 128256 7 us
+  // less than with one warp that walks step by step).
   auto walk = [&](int owner, double from, double goal, unsigned border_key, int border_id, double kept_all) {
     const T* run = slice + owner * a.seg;
     const int run_id = first + owner * a.seg, steps = a.seg / STEP;
@@ -885,12 +886,13 @@ static int sample_launch(const SampleArgs& args, int rows, cudaStream_t stream) 
   constexpr int STEP = 32 * (16 / (int)sizeof(T)), MOST = 227 * 1024;
   const int fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16;
   SampleArgs a = args;
-  // CTAs of 2048 tokens and more where each has an SM, of 6144 where two share one or rows wait: a CTA has about 15 us of steps that wait, which two on an
-  // SM overlap (V = 50257, C = 8 / 4: 8 rows 21 / 26 us, 64 34 / 37; 33 rows top-k only 21 / 18). No more than 4 CTAs per SM in all, unless larger ones would
-  // leave one to an SM (256 rows BF16, C = 8 / 4 / 2: V = 32000 71 / 50 / 45 us, V = 128256 127 / 111 / 156).
+  // As many CTAs of at least 2048 tokens as stand on the GPU at once, two to an SM: a CTA has about 15 us of steps that wait, so a second wave costs more
+  // than smaller CTAs save (64 rows of 128256, C = 8 in two waves / 4 in one: top-k, top-p and min-p together 37 / 29 us, top-p alone on flat rows 89 / 77; the other
+  // way round only where few of the rows are flat, 46 / 57; 64 rows of 50257 with top-k 24 / 16). CTAs so large that an SM holds one are no gain where
+  // rows wait anyway (256 rows of 128256, C = 4 / 2: 105 / 134).
   auto smem_of = [&](int n) { return (long long)((a.V + n * SM_WARPS - 1) / (n * SM_WARPS) + STEP) * SM_WARPS * sizeof(T) + fixed; };
   int c = SM_CLUSTER;
-  while (c > 1 && smem_of(c / 2) <= MOST && (a.V < (rows * c > sm_count() ? 6144 : 2048) * c || (rows * c > 4 * sm_count() && 2 * (smem_of(c / 2) + 1024) <= 228 * 1024))) c /= 2;
+  while (c > 1 && smem_of(c / 2) <= MOST && (a.V < 2048 * c || (rows * c > 2 * sm_count() && 2 * (smem_of(c / 2) + 1024) <= 228 * 1024))) c /= 2;
   a.seg = (a.V + c * SM_WARPS - 1) / (c * SM_WARPS);
   a.seg = (a.seg + STEP - 1) / STEP * STEP;
   const long long smem = fixed + (long long)SM_WARPS * a.seg * sizeof(T);
