@@ -99,9 +99,29 @@ template <> __device__ __forceinline__ void load_vec<float>(const float* p, floa
 }
 template <> __device__ __forceinline__ void load_vec<__nv_bfloat16>(const __nv_bfloat16* p, float* v) { load8(p, *reinterpret_cast<float(*)[8]>(v)); }
 
-template <typename T> __device__ __forceinline__ void store_vec(T* p, const float* v);
-template <> __device__ __forceinline__ void store_vec<float>(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-template <> __device__ __forceinline__ void store_vec<__nv_bfloat16>(__nv_bfloat16* p, const float* v) { store8(p, *reinterpret_cast<const float(*)[8]>(v)); }
+template <typename T> __device__ __forceinline__ uint4 pack_vec(const float* v);
+template <> __device__ __forceinline__ uint4 pack_vec<float>(const float* v) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <> __device__ __forceinline__ uint4 pack_vec<__nv_bfloat16>(const float* v) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// the largest of the numbers among 16 bytes at a time; NaN is none
+template <typename T> struct RunMax;
+template <> struct RunMax<float> {
+  float m = -INFINITY;
+  __device__ __forceinline__ void add(const uint4& v) {
+    m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+  }
+  __device__ __forceinline__ float get() const { return m; }
+};
+template <> struct RunMax<__nv_bfloat16> {
+  __nv_bfloat162 m = __floats2bfloat162_rn(-INFINITY, -INFINITY);
+  __device__ __forceinline__ static __nv_bfloat162 two(unsigned v) { return *reinterpret_cast<__nv_bfloat162*>(&v); }
+  __device__ __forceinline__ void add(const uint4& v) { m = __hmax2(m, __hmax2(__hmax2(two(v.x), two(v.y)), __hmax2(two(v.z), two(v.w)))); }
+  __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
 
 // 2^(d c) for -1000 < d c <= 0: table of 2^(i / 32) and the Taylor polynomial of degree 4 for the rest |r| <= 1/64 (Tang, 1989); 1.2e-12 of the value. The
 // table lies in shared memory 16 times over, a copy for each lane of a half warp, so that a warp's loads meet no conflicts.
@@ -137,9 +157,12 @@ __device__ __forceinline__ unsigned warp_scan_u32(unsigned v, int lane) {
 }
 
 // a float as a double by moving its fields: a conversion takes four times as long as a sum. Zero becomes 6e-39, infinity 2^128.
-__device__ __forceinline__ double widen(float x) {
-  const unsigned b = __float_as_uint(x);
-  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+__device__ __forceinline__ int widen_high(float x) { return (int)(((unsigned)(__float_as_int(x) >> 3) & 0x8fffffffu) + 0x38000000u); }
+__device__ __forceinline__ double widen(float x) { return __hiloint2double(widen_high(x), (int)(__float_as_uint(x) << 29)); }
+// x or, where not `in`, the value that `other` is the widened form of; BF16 values have nothing in the lower word
+template <typename T> __device__ __forceinline__ double widen_or(bool in, float x, double other) {
+  const int high = in ? widen_high(x) : __double2hiint(other);
+  return __hiloint2double(high, sizeof(T) == 2 ? 0 : in ? (int)(__float_as_uint(x) << 29) : __double2loint(other));
 }
 __device__ __forceinline__ float ex2_approx(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
@@ -311,30 +334,32 @@ sample_tokens_kernel(const SampleArgs a) {
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
   auto answer = [&](int id, float prob) { a.ids[row] = id; if (a.probs != nullptr) a.probs[row] = prob; };
 
-  // ---- 1: logits into shared memory, their largest. Four loads of a thread are on their way at a time ----
-  float mine_top = -INFINITY;                            // of this thread's tokens
+  // ---- 1: logits into shared memory, their largest. Four loads of a thread are on their way at a time. NaN stays: no comparison lets it through ----
+  RunMax<T> run_max;
   const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
   for (int i0 = lane * VEC; i0 < a.seg; i0 += 4 * STEP) {
-    float v[4][VEC];
+    uint4 v[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int i = i0 + g * STEP, at = warp * a.seg + i;
       if (i < a.seg && vec && at + VEC <= have) {
-        load_vec<T>(src + at, v[g]);
+        v[g] = *reinterpret_cast<const uint4*>(src + at);
       } else {
+        float f[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[g][e] = i < a.seg && at + e < have ? to_float(src[at + e]) : -INFINITY;
+        for (int e = 0; e < VEC; ++e) f[e] = i < a.seg && at + e < have ? to_float(src[at + e]) : -INFINITY;
+        v[g] = pack_vec<T>(f);
       }
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int i = i0 + g * STEP;
       if (i >= a.seg) break;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) { if (v[g][e] != v[g][e]) v[g][e] = -INFINITY; mine_top = fmaxf(mine_top, v[g][e]); }
-      store_vec<T>(mine + i, v[g]);
+      run_max.add(v[g]);
+      *reinterpret_cast<uint4*>(mine + i) = v[g];
     }
   }
+  float mine_top = run_max.get();                        // of this thread's tokens
   {
     const float m = warp_max(mine_top);
     if (lane == 0) sh.warp_top[warp] = m;
@@ -486,7 +511,7 @@ sample_tokens_kernel(const SampleArgs a) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const bool in = v[e] >= from;
-          const double w = exp2_table(widen(in ? v[e] : r.top) - r.wide_top, r.c, r.table);
+          const double w = exp2_table(widen_or<T>(in, v[e], r.wide_top) - r.wide_top, r.c, r.table);
           if (in) s += w;
         }
       }
@@ -755,7 +780,7 @@ sample_tokens_kernel(const SampleArgs a) {
           const float x = (r.top - v[e]) * r.bins;
           const unsigned key = key_of<T>(v[e]);
           const bool until = !(x >= hi_x), front = !(x >= lo_x) || (until && key > key_hi), weighs = v[e] >= heavy;
-          const double w = exp2_table(widen(weighs ? v[e] : r.top) - r.wide_top, r.c, r.table);
+          const double w = exp2_table(widen_or<T>(weighs, v[e], r.wide_top) - r.wide_top, r.c, r.table);
           if (weighs && front) m += w;
           n_ties += v[e] >= cut_in && until && !front && key >= key_lo;
         }
