@@ -45,7 +45,7 @@ struct SampleShared {
   double part[SM_PARTS];                // CTA 0, general path: every warp's kept mass in front of the border's bins
   unsigned part_in[SM_PARTS][3];        // and within them, whole numbers of 2^-10, 2^-30 and 2^-50, so that the order of their sum does not matter
   double warp_sum[SM_WARPS], scan_mass[SM_WARPS];
-  double total, from;
+  double total, from, c, below;
   float top[SM_CLUSTER], cut[SM_CLUSTER], warp_top[SM_WARPS];
   int candidates[SM_CLUSTER];
   unsigned key_min[SM_CLUSTER], key_max[SM_CLUSTER], ties[SM_CLUSTER], first_id[SM_CLUSTER];
@@ -323,8 +323,12 @@ sample_tokens_kernel(const SampleArgs a) {
   const int id0 = first + warp * a.seg;
   cluster_arrive_relaxed();                              // "this CTA runs": waited on before the first store into a peer
   pdl_trigger();
-  static_assert(SM_TABLE * SM_COPIES == SM_THREADS, "a thread per entry");
-  sh.table[tid] = exp2((tid / SM_COPIES) / (double)SM_TABLE);
+  // 64-bit functions are hundreds of instructions that every warp would repeat: one warp calls each (256 rows of 151936: 105 -> 103 us)
+  if (warp == 0) {
+    static_assert(SM_TABLE == 32, "a lane per entry");
+    const double t = exp2(lane / (double)SM_TABLE);
+    for (int j = 0; j < SM_COPIES; ++j) sh.table[lane * SM_COPIES + (lane + j) % SM_COPIES] = t;
+  }
   if (tid == 0) sh.list_n = 0;
   pdl_wait();
   const float temp = a.temperature[row];
@@ -332,6 +336,12 @@ sample_tokens_kernel(const SampleArgs a) {
   const float p = a.top_p != nullptr ? a.top_p[row] : 1.f, floor_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
   float u = a.uniforms[row];
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+  // min-p as a distance of logits: rounded up below, so that for 32-bit logits the comparison is the one with the unrounded value
+  const bool use_m = floor_p > 0.f && temp < INFINITY;
+  if (warp == 1 && temp > 0.f) {
+    const double c = 1.4426950408889634074 / (double)temp, below = use_m ? (double)temp * log((double)fminf(floor_p, 1.f)) : 0.0;
+    if (lane == 0) { sh.c = c; sh.below = below; }
+  }
   auto answer = [&](int id, float prob) { a.ids[row] = id; if (a.probs != nullptr) a.probs[row] = prob; };
 
   // ---- 1: logits into shared memory, their largest. Four loads of a thread are on their way at a time. NaN stays: no comparison lets it through ----
@@ -413,14 +423,12 @@ sample_tokens_kernel(const SampleArgs a) {
     r.top = 0.f;
   }
   r.wide_top = widen(r.top);
-  r.c = 1.4426950408889634074 / (double)temp;
+  r.c = sh.c;
   r.ch = fminf((float)r.c, 1e30f);
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
   const float far = r.ch > 0.f ? r.top + SM_FAR / r.ch : -INFINITY;
-  // min-p as a logit: rounded up, so that for 32-bit logits the comparison is the one with the unrounded value
-  float least = -INFINITY;
-  if (floor_p > 0.f && temp < INFINITY) least = fminf(r.top, __double2float_ru((double)r.top + (double)temp * log((double)fminf(floor_p, 1.f))));
+  const float least = use_m ? fminf(r.top, __double2float_ru((double)r.top + sh.below)) : -INFINITY;
 
   // The draw within the run of ids of warp `owner` of this CTA, by all of its warps: the lowest id at which the sum of kept weights, `from` in front of
   // the run, passes the goal. Shared memory holds runs of 28 steps at most; their sums first, then the step's tokens (48 rows of 128256 7 us
@@ -540,8 +548,12 @@ sample_tokens_kernel(const SampleArgs a) {
     float cut = fmaxf(least, use_k ? k_cut : -INFINITY);
     if (use_p) {
       // borders lie at weights of (1 - P) S / V and more; a thousandth is left for the roundings
-      const double away = log(0.999 * (1.0 - fmax((double)p, 0.0)) * s / a.V) * (double)temp;
-      cut = fmaxf(cut, fminf(r.top, __double2float_rd((double)r.top + away)));
+      if (warp == 0) {
+        const double away = log(0.999 * (1.0 - fmax((double)p, 0.0)) * s / a.V) * (double)temp;
+        if (lane == 0) sh.below = away;
+      }
+      __syncthreads();
+      cut = fmaxf(cut, fminf(r.top, __double2float_rd((double)r.top + sh.below)));
     }
     const bool some = mine_top >= cut && mine_top > -INFINITY;
     int n = 0;
@@ -555,8 +567,7 @@ sample_tokens_kernel(const SampleArgs a) {
     const int in_warp = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) sh.scan_count[warp] = in_warp;
     __syncthreads();
-    int in_cta = 0;
-    for (int w = 0; w < SM_WARPS; ++w) in_cta += sh.scan_count[w];
+    const int in_cta = __reduce_add_sync(0xffffffffu, lane < SM_WARPS ? sh.scan_count[lane] : 0u);
     // a CTA with more than its part of the list leaves the row to the general path
     const int share = SM_LIST / C;
     if (tid < C) push_u32(&sh.candidates[rank], tid, in_cta);
@@ -576,6 +587,36 @@ sample_tokens_kernel(const SampleArgs a) {
     for (int i = 0; i < C; ++i) { all += sh.candidates[i]; most = max(most, sh.candidates[i]); }
     if (most <= share) {
       if (rank != 0) return;
+      if (all <= 32) {
+        // few candidates, what peaked distributions leave: one warp without a barrier, a token per lane
+        if (warp != 0) return;
+        const bool here = lane < all;
+        const unsigned long long entry = here ? sh.list[lane] : 0;
+        const double weight = here ? r.weight(logit_of<T>((unsigned)(entry >> 32))) : 0.0;
+        int place = 0;
+        for (int j = 0; j < all; ++j) place += sh.list[j] > entry;
+        __syncwarp();
+        if (here) { sh.list[place] = entry; sh.w[place] = weight; }
+        __syncwarp();
+        double w = here ? sh.w[lane] : 0.0;
+        const double upto = warp_scan64(w, lane);
+        const unsigned ends = __ballot_sync(0xffffffffu, here && ((use_k && lane + 1 >= k) || (use_p && upto >= target)));
+        const int last_kept = ends ? __ffs(ends) - 1 : all - 1;
+        const double total = __shfl_sync(0xffffffffu, upto, last_kept), goal = (double)u * total;
+        // the kept ones by id
+        const unsigned id = here ? ~(unsigned)sh.list[lane] : 0u;
+        const bool kept = lane <= last_kept;
+        place = 0;
+        for (int j = 0; j <= last_kept; ++j) place += ~(unsigned)sh.list[j] < id;
+        __syncwarp();
+        if (kept) { sh.list[place] = id; sh.w[place] = w; }
+        __syncwarp();
+        w = kept ? sh.w[lane] : 0.0;
+        const double m = warp_scan64(w, lane);
+        const unsigned pass = __ballot_sync(0xffffffffu, w > 0.0 && m > goal), some_w = __ballot_sync(0xffffffffu, w > 0.0);
+        if (lane == (pass ? __ffs(pass) - 1 : 31 - __clz(some_w))) answer((int)sh.list[lane], (float)(w / total));          // the sums' last bits may leave the goal behind the last token
+        return;
+      }
       const int kept = find_border<T>(sh, r, all, 0, 0.0, use_k, k, use_p, target, a.V, tid, warp, lane);
       const double goal = (double)u * sh.total;
       // the kept ones by id: ~id << 32 | place, descending
