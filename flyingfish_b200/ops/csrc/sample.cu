@@ -158,16 +158,12 @@ __device__ __forceinline__ unsigned warp_scan_u32(unsigned v, int lane) {
 
 // a float as a double by moving its fields: a conversion takes four times as long as a sum. Zero becomes 6e-39, infinity 2^128.
 __device__ __forceinline__ int widen_high(float x) { return (int)(((unsigned)(__float_as_int(x) >> 3) & 0x8fffffffu) + 0x38000000u); }
-__device__ __forceinline__ double widen(float x) { return __hiloint2double(widen_high(x), (int)(__float_as_uint(x) << 29)); }
-// x or, where not `in`, the value that `other` is the widened form of; BF16 values have nothing in the lower word
-template <typename T> __device__ __forceinline__ double widen_or(bool in, float x, double other) {
-  const int high = in ? widen_high(x) : __double2hiint(other);
-  return __hiloint2double(high, sizeof(T) == 2 ? 0 : in ? (int)(__float_as_uint(x) << 29) : __double2loint(other));
-}
+// BF16 values have nothing in the lower word
+template <typename T> __device__ __forceinline__ double widen(float x) { return __hiloint2double(widen_high(x), sizeof(T) == 2 ? 0 : (int)(__float_as_uint(x) << 29)); }
 __device__ __forceinline__ float ex2_approx(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // A row as a CTA sees it: weights and bins of its logits. The largest logit is finite (rows with +inf are rewritten first).
-struct SampleRow {
+template <typename T> struct SampleRow {
   float top;                            // the largest logit
   double c, wide_top;                   // log2(e) / T
   float ch;                             // c rounded
@@ -175,7 +171,7 @@ struct SampleRow {
   const double* table;
   // zero below 2^-1000
   __device__ __forceinline__ double weight(float l) const {
-    const double d = widen(l) - wide_top;
+    const double d = widen<T>(l) - wide_top;
     return l > -INFINITY && d * c > SM_FAR ? exp2_table(d, c, table) : 0.0;
   }
   // octaves of a logit against the largest
@@ -282,7 +278,7 @@ __device__ __forceinline__ void sort_list(SampleShared& sh, int n, unsigned span
 // The list's n tokens (n <= SM_LIST) in the order's order, with their weights; then the first of them at which the prefix ends: `above` tokens of mass
 // `mass_above` stand in front of the list. Returns how many of the list are kept, and their mass with mass_above in sh.total.
 template <typename T>
-__device__ __forceinline__ int find_border(SampleShared& sh, const SampleRow& r, int n, unsigned above, double mass_above, bool use_k, int k, bool use_p, double target,
+__device__ __forceinline__ int find_border(SampleShared& sh, const SampleRow<T>& r, int n, unsigned above, double mass_above, bool use_k, int k, bool use_p, double target,
                                            int V, int tid, int warp, int lane) {
   if (tid == 0) sh.at = n - 1;
   __syncthreads();
@@ -383,7 +379,7 @@ sample_tokens_kernel(const SampleArgs a) {
     push_u32(&sh.top[rank], tid, __float_as_uint(m));
   }
   cluster_sync_all();
-  SampleRow r;
+  SampleRow<T> r;
   r.table = sh.table + lane % SM_COPIES;
   r.top = sh.top[0];
   for (int i = 1; i < C; ++i) r.top = fmaxf(r.top, sh.top[i]);
@@ -422,7 +418,7 @@ sample_tokens_kernel(const SampleArgs a) {
     mine_top = mine_top == INFINITY ? 0.f : -INFINITY;
     r.top = 0.f;
   }
-  r.wide_top = widen(r.top);
+  r.wide_top = widen<T>(r.top);
   r.c = sh.c;
   r.ch = fminf((float)r.c, 1e30f);
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
@@ -518,9 +514,9 @@ sample_tokens_kernel(const SampleArgs a) {
         load_vec<T>(mine + i, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const bool in = v[e] >= from;
-          const double w = exp2_table(widen_or<T>(in, v[e], r.wide_top) - r.wide_top, r.c, r.table);
-          if (in) s += w;
+          // what lies below gives some number or other, which is not added
+          const double w = exp2_table(widen<T>(v[e]) - r.wide_top, r.c, r.table);
+          s = v[e] >= from ? s + w : s;
         }
       }
     s = warp_sum64(s);
@@ -821,8 +817,8 @@ sample_tokens_kernel(const SampleArgs a) {
           const float x = (r.top - v[e]) * r.bins;
           const unsigned key = key_of<T>(v[e]);
           const bool until = !(x >= hi_x), front = !(x >= lo_x) || (until && key > key_hi), weighs = v[e] >= heavy;
-          const double w = exp2_table(widen_or<T>(weighs, v[e], r.wide_top) - r.wide_top, r.c, r.table);
-          if (weighs && front) m += w;
+          const double w = exp2_table(widen<T>(v[e]) - r.wide_top, r.c, r.table);
+          m = weighs && front ? m + w : m;
           n_ties += v[e] >= cut_in && until && !front && key >= key_lo;
         }
       }
