@@ -552,9 +552,12 @@ sample_tokens_kernel(const SampleArgs a) {
       cut = fmaxf(cut, fminf(r.top, __double2float_rd((double)r.top + sh.below)));
     }
     const bool some = mine_top >= cut && mine_top > -INFINITY;
+    // 16 bytes of which none is a candidate are seen by their largest
+    auto none_in = [&](int i) { RunMax<T> chunk; chunk.add(*reinterpret_cast<const uint4*>(mine + i)); return !(chunk.get() >= cut); };
     int n = 0;
     if (some)
       for (int i = lane * VEC; i < a.seg; i += STEP) {
+        if (none_in(i)) continue;
         float v[VEC];
         load_vec<T>(mine + i, v);
 #pragma unroll
@@ -571,6 +574,7 @@ sample_tokens_kernel(const SampleArgs a) {
       const unsigned slot0 = push_take(&sh.list_n, 0, n);          // at most SM_LIST in all
       unsigned slot = slot0;
       for (int i = lane * VEC; i < a.seg; i += STEP) {
+        if (none_in(i)) continue;
         float v[VEC];
         load_vec<T>(mine + i, v);
 #pragma unroll
