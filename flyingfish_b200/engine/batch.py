@@ -62,10 +62,12 @@ class ForwardBatch:
         self.device = torch.device(device)
         pin = self.device.type == "cuda" if pinned is None else pinned
         pinned = torch.zeros(layout.full + 4 + layout.max_batch, dtype=torch.int32, pin_memory=pin)
-        self.host = pinned[: layout.full]
+        self._host_all = pinned[: layout.full]
+        self.host = pinned[: layout.total]       # what every step uploads
         self.results = pinned[layout.full:]     # where the engine reads a step's device status (four words) and ids
-        self._words = self.host.numpy()   # the same memory: a field is written in about a microsecond, through a tensor in four
-        self.dev = torch.zeros(layout.full, dtype=torch.int32, device=self.device)
+        self._words = self._host_all.numpy()   # the same memory: a field is written in about a microsecond, through a tensor in four
+        self._dev_all = torch.zeros(layout.full, dtype=torch.int32, device=self.device)
+        self.dev = self._dev_all[: layout.total]
         # host-side scalars of the current step
         self.batch = 0
         self.rows = 0
@@ -83,7 +85,7 @@ class ForwardBatch:
 
     # -- device views (fixed addresses) ------------------------------------------------------
     def _v(self, off: int, n: int) -> torch.Tensor:
-        return self.dev[off: off + n]
+        return self._dev_all[off: off + n]
 
     @property
     def ids(self) -> torch.Tensor: return self._v(self.layout.ids, self.rows)
@@ -225,4 +227,4 @@ class ForwardBatch:
     def upload(self) -> None:
         """One host-to-device copy of the packed buffer, adapters and settings included where the step has any."""
         n = self._used()
-        self.dev[:n].copy_(self.host[:n], non_blocking=True)
+        self._dev_all[:n].copy_(self._host_all[:n], non_blocking=True)

@@ -17,6 +17,10 @@
 //     cannot tell; the mass above is summed in FP64 and the bin's tokens are sorted as in 3. A bin of more tokens is divided by key, ties of one key go by
 //     id. CTA 0 finds the warp whose run holds the draw, and that warp's CTA the token.
 //
+// What bounds it: dependent steps, each with a barrier of the cluster, in small batches (one flat row of 128256: 25 us, 33 rows of 50257 with top-k 17);
+// issue slots in large ones (256 rows of 151936 with top-k, top-p and min-p: 87 us, 57 % of the slots, FP64 pipe 27 %, 0.9 TB/s). Why shared memory: the
+// logits are looked at three to six times. Why FP64 and no compensated FP32: an SM has half as many FP64 lanes, and pairs of words take more than twice the operations.
+//
 // NaN counts as -inf, -inf is never drawn, +inf shares everything among its equals; a row without anything gives id 0 with probability 0.
 #include "dtype_io.cuh"
 #include "host_util.h"

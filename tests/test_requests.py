@@ -90,6 +90,7 @@ def test_a_plain_step_uploads_what_it_did():
     seqs = [eng.add_sequence([1, 2, 3 + i]) for i in range(3)]
     eng.prefill(seqs)
     eng.decode(seqs)
+    assert fb.host.numel() == fb.dev.numel() == fb.layout.total          # whoever stages plain steps by hand copies these whole
     assert fb.h2d_bytes() == 4 * fb.layout.total < 4 * fb.layout.full and fb.adapters is None and not fb.sampled
     s = eng.add_sequence([1, 2, 9], adapter="poet", sampling=Sampling(0.5))
     eng.prefill([s])
