@@ -83,12 +83,9 @@ __device__ __forceinline__ unsigned push_take(const void* p, int cta, unsigned n
   return r;
 }
 
-// keys that order as the logits do
-__device__ __forceinline__ unsigned order_key(float x) { const unsigned b = __float_as_uint(x); return b & 0x80000000u ? ~b : b | 0x80000000u; }
-__device__ __forceinline__ unsigned order_key(__nv_bfloat16 x) { const unsigned b = __bfloat16_as_ushort(x); return b & 0x8000u ? 0xffffu & ~b : b | 0x8000u; }
-template <typename T> __device__ __forceinline__ unsigned key_of(float x);
-template <> __device__ __forceinline__ unsigned key_of<float>(float x) { return order_key(x); }
-template <> __device__ __forceinline__ unsigned key_of<__nv_bfloat16>(float x) { return order_key(__float2bfloat16(x)); }
+// keys that order as the logits do, zeros of both signs as one: BF16 values have the upper half of an FP32 key
+__device__ __forceinline__ unsigned order_key(float x) { const unsigned b = __float_as_uint(x + 0.f); return b & 0x80000000u ? ~b : b | 0x80000000u; }
+template <typename T> __device__ __forceinline__ unsigned key_of(float x) { return order_key(x) >> (sizeof(T) == 2 ? 16 : 0); }
 
 template <typename T> __device__ __forceinline__ float logit_of(unsigned key);
 template <> __device__ __forceinline__ float logit_of<float>(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }

@@ -240,3 +240,45 @@ def test_rows_that_no_shared_memory_holds_are_refused(cuda):
             sample_ops.sample_tokens(torch.zeros(1, vocab, dtype=dtype, device=cuda), one(), one())
         ids, p = sample_ops.sample_tokens(torch.zeros(1, vocab - 1, dtype=dtype, device=cuda), one() + 0.5, one() + 1)
         assert abs(int(ids[0]) - (vocab - 1) // 2) <= 1 and float(p[0]) == pytest.approx(1 / (vocab - 1), rel=1e-6)
+
+
+def _zeros(rows, vocab, dtype, device):
+    """Zeros of both signs among smaller logits."""
+    g = torch.Generator().manual_seed(rows)
+    pick = torch.randint(0, 4, (rows, vocab), generator=g)
+    return torch.tensor([0.0, -0.0, -2.0, -0.5])[pick].to(dtype).to(device)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_zeros_of_both_signs_are_equal_for_the_oracle(dtype):
+    l = torch.tensor([[-0.0, 0.0, -0.0, -1.0]], dtype=dtype)
+    one = lambda u, k: sample_ops.sample_tokens(l, torch.tensor([u]), torch.tensor([1.0]), torch.tensor([k], dtype=torch.int32))[0].item()
+    assert one(0.9, 1) == 0 and one(0.9, 2) == 1 and one(0.9, 3) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [4, 301, 50257])
+def test_zeros_of_both_signs_are_equal(cuda, vocab, dtype):
+    rows = 24
+    l = _zeros(rows, vocab, dtype, cuda)
+    f = lambda v, t=F32: torch.tensor([v[i % len(v)] for i in range(rows)], dtype=t, device=cuda)
+    u, t = f([0.1, 0.5, 0.99, 0.0, 0.999]), f([1.0, 0.5])
+    for k in (f([1, 2, 3, 5, 100, vocab // 3 + 1], torch.int32), None):
+        for p in (f([0.3, 0.05, 0.9, 0.6]), None):
+            ids, _ = sample_ops.sample_tokens(l, u, t, k, p)
+            want, _ = _want(l, u, t, k, p, None)
+            for r in torch.nonzero(ids.cpu() != want).flatten().tolist():
+                # Weights 1, w, 1, w and the number 0.5: the half of the mass ends with a token, and 0.5 (2 + 2 w) against 1 + w is decided by the last bit of either sum.
+                # Sums of n weights in 64 bits are off by n 2^-53 of themselves at most: within that the draw may fall on either side.
+                low, high = sorted((int(ids[r]), int(want[r])))
+                w = torch.exp((l[r].double().cpu() - l[r].double().cpu().max()) / float(t[r]))
+                order = torch.argsort(l[r].double().cpu(), descending=True, stable=True)
+                n = vocab if k is None else min(vocab, int(k[r]))
+                if p is not None:
+                    n = min(n, int((torch.cumsum(w[order], 0) < float(p[r]) * w.sum()).sum()) + 1)
+                kept = torch.zeros_like(w)
+                kept[order[:n]] = w[order[:n]]
+                sums = torch.cumsum(kept, 0)
+                assert kept[low] > 0 and kept[high] > 0 and not kept[low + 1: high].any(), (r, low, high)
+                assert abs(sums[low] - float(u[r]) * sums[-1]) <= vocab * 2.0 ** -52 * sums[-1], (r, low, high)
