@@ -41,7 +41,7 @@ struct SampleArgs {
   int V, seg;                           // seg: ids per warp
 };
 
-struct SampleFound { int lo, hi, count, reached; unsigned above; };
+struct SampleFound { int lo, hi, count; unsigned above; };
 
 struct SampleShared {
   double table[SM_TABLE * SM_COPIES];   // 2^(i / 32), every lane of a half warp its own
@@ -698,7 +698,7 @@ sample_tokens_kernel(const SampleArgs a) {
       }
       const unsigned c_in = warp_scan_u32(c_sum, lane);
       if (lane == 31) sh.scan_count[warp] = c_in;
-      if (tid == 0) sh.found = SampleFound{SM_BINS, 0, 0, 0, 0};
+      if (tid == 0) sh.found = SampleFound{SM_BINS, 0, 0, 0};
       double m_all;
       double m_at = block_scan(m_sum, sh, warp, lane, m_all);
       unsigned c_at = c_in - c_sum;

@@ -3,7 +3,8 @@ that adapter, rounded once. The rows of a batch have an adapter each or none; wh
 any mix. CUDA: ``csrc/lora.cu`` (BF16, FP32 sums) with the products of ``csrc/gemm_skinny.cu`` and ``csrc/gemm_bf16.cu``; CPU: FP32 oracle.
 
 The adapters of one projection form an :class:`AdapterStack` (:func:`pack_stack` builds one, once). A stack's weights are taken to be finite
-where they are within an adapter's rank; what is not reaches the rows of that adapter only."""
+where they are within an adapter's rank; what is not reaches the rows of that adapter only. As with ``ops.linear``, weights (a stack's among them) may be
+read ahead of what the stream still holds, and calls of up to 128 rows use the device's workspace: one stream at a time, or a ``SideLane``."""
 from __future__ import annotations
 
 import ctypes
