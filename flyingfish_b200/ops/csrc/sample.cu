@@ -170,11 +170,8 @@ template <typename T> struct SampleRow {
   float ch;                             // c rounded
   float bins;                           // bins per unit of logit
   const double* table;
-  // zero below 2^-1000
-  __device__ __forceinline__ double weight(float l) const {
-    const double d = widen<T>(l) - wide_top;
-    return l > -INFINITY && d * c > SM_FAR ? exp2_table(d, c, table) : 0.0;
-  }
+  float far;                            // least logit that weighs anything
+  __device__ __forceinline__ double weight(float l) const { return l >= far ? exp2_table(widen<T>(l) - wide_top, c, table) : 0.0; }
   // octaves of a logit against the largest
   __device__ __forceinline__ float octaves(float l) const { return (l - top) * ch; }
   // never falls as l does: a difference and a product with a positive factor, each rounded, are monotone
@@ -424,7 +421,7 @@ sample_tokens_kernel(const SampleArgs a) {
   r.ch = fminf((float)r.c, 1e30f);
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
-  const float far = r.ch > 0.f ? r.top + SM_FAR / r.ch : -INFINITY;
+  r.far = fmaxf(r.ch > 0.f ? __fadd_ru(r.top, SM_FAR / r.ch) : -INFINITY, -3.4028235e38f);      // rounded up: the next number below may lie thousands of octaves lower
   const float least = use_m ? fminf(r.top, __double2float_ru((double)r.top + sh.below)) : -INFINITY;
 
   // The draw within the run of ids of warp `owner` of this CTA, by all of its warps: the lowest id at which the sum of kept weights, `from` in front of
@@ -508,7 +505,7 @@ sample_tokens_kernel(const SampleArgs a) {
   if (use_p || !use_k) {
     // the draw's mass is that of the kept tokens
     double s = 0.0;
-    const float from = fmaxf(fmaxf(use_p ? -INFINITY : least, far), -3.4028235e38f);
+    const float from = fmaxf(use_p ? -INFINITY : least, r.far);
     if (mine_top >= from)
       for (int i = lane * VEC; i < a.seg; i += STEP) {
         float v[VEC];
@@ -806,7 +803,7 @@ sample_tokens_kernel(const SampleArgs a) {
     unsigned n_ties = 0;
     // bins as numbers that r.bin rounds down: no number reaches the first one behind the last bin, nor NaN, which stands for it
     const float lo_x = lo < SM_BINS ? (float)lo : __uint_as_float(0x7fffffffu), hi_x = hi < SM_BINS - 1 ? (float)(hi + 1) : __uint_as_float(0x7fffffffu);
-    const float cut_in = fmaxf(cut, -3.4028235e38f), heavy = fmaxf(cut_in, far);
+    const float cut_in = fmaxf(cut, -3.4028235e38f), heavy = fmaxf(cut_in, r.far);
     auto at_border = [&](float l) {
       const float x = (r.top - l) * r.bins;
       const unsigned key = key_of<T>(l);

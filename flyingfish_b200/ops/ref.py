@@ -422,7 +422,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
         away = torch.where(l == top, 0.0, (l - top) / t)
         if t == math.inf:
             away = torch.where(l == -math.inf, l, 0.0)
-        w = torch.exp(away)
+        w = torch.where(away < -1000.0 * math.log(2.0), 0.0, torch.exp(away))          # what is less counts as none
         order = torch.argsort(l, descending=True, stable=True)
         n = l.numel()
         k = 0 if top_k is None else int(top_k[r])

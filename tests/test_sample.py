@@ -22,7 +22,7 @@ def _row(logits, u, t, k, p, m):
         return int(np.argmax(l)), 1.0
     with np.errstate(invalid="ignore", over="ignore"):
         away = np.where(l == top, 0.0, (l - top) / t)
-    w = np.exp(away)
+    w = np.where(away < -1000 * math.log(2.0), 0.0, np.exp(away))          # a mass below 2^-1000 of the largest counts as none, by the operator's definition
     order = np.lexsort((np.arange(len(l)), -l))
     n = len(l) if k <= 0 else min(k, len(l))
     if p < 1:
@@ -282,3 +282,23 @@ def test_zeros_of_both_signs_are_equal(cuda, vocab, dtype):
                 sums = torch.cumsum(kept, 0)
                 assert kept[low] > 0 and kept[high] > 0 and not kept[low + 1: high].any(), (r, low, high)
                 assert abs(sums[low] - float(u[r]) * sums[-1]) <= vocab * 2.0 ** -52 * sums[-1], (r, low, high)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("top", [25.0, 3e4, -7.5, 1e-3])
+def test_neighbouring_numbers_at_temperatures_that_part_them(cuda, top, dtype):
+    """Logits a step or a few below the largest, at temperatures where a step is from less than an octave to thousands of them."""
+    rows, vocab = 30, 5003
+    start = torch.tensor(top, dtype=dtype)
+    steps = [start]
+    for _ in range(6):
+        steps.append(torch.nextafter(steps[-1], torch.tensor(-float("inf"), dtype=dtype)))
+    gap = float(steps[0]) - float(steps[1])
+    g = torch.Generator().manual_seed(3)
+    l = torch.stack(steps)[torch.randint(0, 7, (rows, vocab), generator=g)].to(cuda)
+    f = lambda v, t=F32: torch.tensor([v[i % len(v)] for i in range(rows)], dtype=t, device=cuda)
+    t = f([gap * s for s in (1e-6, 1e-4, 4e-4, 7e-4, 1.1e-3, 1.44e-3, 1.6e-3, 3e-3, 0.1, 3.0)])
+    u = f([0.0, 0.3, 0.999, 0.7, 0.9999999])
+    for k, p in ((None, None), (f([3000, 700, 20], torch.int32), None), (None, f([0.9, 0.4])), (f([3000, 700, 20], torch.int32), f([0.9, 0.4]))):
+        _check(l, u, t, k, p)
