@@ -842,11 +842,14 @@ sample_tokens_kernel(const SampleArgs a) {
       push_f64(&sh.part[rank * SM_WARPS + warp], 0, m);
     }
     __syncthreads();
-    if (tid < C) {
+    if (ties && tid < C) {
+      // Counts and masses have places of their CTA's that the division by keys pushed to as well. Only after its end by ties has a barrier of the cluster passed
+      // since they were read there; after its other end a peer may still be reading them.
+      double t = 0.0;
       unsigned c = 0;
-      for (int w = 0; w < SM_WARPS; ++w) c += sh.warp_ties[w];
+      for (int w = 0; w < SM_WARPS; ++w) { t += sh.warp_sum[w]; c += sh.warp_ties[w]; }
       push_u32(&sh.ties[rank], tid, c);
-      if (ties) { double t = 0.0; for (int w = 0; w < SM_WARPS; ++w) t += sh.warp_sum[w]; push_f64(&sh.mass[rank], tid, t); }
+      push_f64(&sh.mass[rank], tid, t);
     }
     cluster_sync_all();
     if (ties) {

@@ -302,3 +302,23 @@ def test_neighbouring_numbers_at_temperatures_that_part_them(cuda, top, dtype):
     u = f([0.0, 0.3, 0.999, 0.7, 0.9999999])
     for k, p in ((None, None), (f([3000, 700, 20], torch.int32), None), (None, f([0.9, 0.4])), (f([3000, 700, 20], torch.int32), f([0.9, 0.4]))):
         _check(l, u, t, k, p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(24, 4099), (140, 4099), (24, 9001), (9, 20011), (3, 128256)])
+def test_borders_in_a_bin_of_many_tokens(cuda, rows, vocab, dtype):
+    """One large logit far above thousands within a thousandth of one another: the border's bin holds them all, and is divided by key until a list holds what is left (FP32:
+    thousands of keys) or one key is (BF16: a few). All CTAs of a row have to come to the same keys, each time."""
+    g = torch.Generator().manual_seed(rows + vocab)
+    l = torch.rand(rows, vocab, generator=g) * (1e-3 if dtype == F32 else 0.05) + 1.0
+    l[torch.arange(rows), torch.randint(vocab, (rows,), generator=g)] = 31.0
+    l = l.to(dtype).to(cuda)
+    f = lambda v, t=F32: torch.tensor([v[i % len(v)] for i in range(rows)], dtype=t, device=cuda)
+    u, t, k, p = torch.rand(rows, generator=g).to(cuda), f([50.0, 20.0, 100.0]), f([1500, vocab // 2, vocab - 1100, 2600], torch.int32), f([0.9, 0.55, 0.3])
+    for args in ((k, None), (None, p), (k, p)):
+        _check(l, u, t, *args)
+        first = sample_ops.sample_tokens(l, u, t, *args)
+        for _ in range(30):
+            again = sample_ops.sample_tokens(l, u, t, *args)
+            assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
