@@ -325,7 +325,7 @@ sample_tokens_kernel(const SampleArgs a) {
   }
   if (tid == 0) sh.list_n = 0;
   pdl_wait();
-  const float temp = a.temperature[row];
+  float temp = a.temperature[row];
   const int k = a.top_k != nullptr ? a.top_k[row] : 0;
   const float p = a.top_p != nullptr ? a.top_p[row] : 1.f, floor_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
   float u = a.uniforms[row];
@@ -416,13 +416,24 @@ sample_tokens_kernel(const SampleArgs a) {
     mine_top = mine_top == INFINITY ? 0.f : -INFINITY;
     r.top = 0.f;
   }
-  r.wide_top = widen<T>(r.top);
+  double below = sh.below;
   r.c = sh.c;
+  if (temp < 0x1p-80f && fabsf(r.top) < 0x1p-40f) {
+    // Logits and temperature times 2^90 draw as before, and then no zero and no subnormal logit is nearer to the largest than widen() tells apart; what this takes to
+    // -inf weighs nothing. Above 2^-40 numbers lie 2^-64 and more apart, so that at these temperatures only the largest logit weighs anything.
+    constexpr float UP = 0x1p90f;
+    for (int i = lane * VEC; i < a.seg; i += STEP)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) from_float(mine + i + e, to_float(mine[i + e]) * UP);
+    mine_top *= UP; r.top *= UP; temp *= UP;
+    r.c *= 1.0 / UP; below *= UP;
+  }
+  r.wide_top = widen<T>(r.top);
   r.ch = fminf((float)r.c, 1e30f);
   r.bins = fminf((float)(r.c * 16.0), 1e30f);
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
   r.far = fmaxf(r.ch > 0.f ? __fadd_ru(r.top, SM_FAR / r.ch) : -INFINITY, -3.4028235e38f);      // rounded up: the next number below may lie thousands of octaves lower
-  const float least = use_m ? fminf(r.top, __double2float_ru((double)r.top + sh.below)) : -INFINITY;
+  const float least = use_m ? fminf(r.top, __double2float_ru((double)r.top + below)) : -INFINITY;
 
   // The draw within the run of ids of warp `owner` of this CTA, by all of its warps: the lowest id at which the sum of kept weights, `from` in front of
   // the run, passes the goal. Shared memory holds runs of 28 steps at most; their sums first, then the step's tokens (48 rows of 128256 7 us

@@ -322,3 +322,37 @@ def test_borders_in_a_bin_of_many_tokens(cuda, rows, vocab, dtype):
         for _ in range(30):
             again = sample_ops.sample_tokens(l, u, t, *args)
             assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
+def _nearly_zero(rows, vocab, dtype, device):
+    """Logits from 1e-28 down to subnormal ones, by rows, with zeros of both signs, values far below and masked ones among them."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=g, dtype=torch.float64) * torch.tensor([1e-28, 1e-33, 1e-38, 1e-40, 1e-42, 0.0], dtype=torch.float64)[torch.arange(rows) % 6][:, None]
+    what = torch.randint(0, 20, (rows, vocab), generator=g)
+    for i, v in enumerate((0.0, -0.0, -1.0, -3e38, -math.inf)):
+        x[what == i] = v
+    x[torch.arange(rows) % 5 == 4, 7] = math.nan
+    return x.to(F32).to(dtype).to(device)
+
+
+def _freezing(rows, device):
+    f = lambda v, t=F32: torch.tensor([v[i % len(v)] for i in range(rows)], dtype=t, device=device)
+    return (f([0.0, 0.3, 0.999, 0.7, 0.9999999]), f([1e-25, 1e-29, 3e-31, 1e-35, 1e-40, 2e-42, 1e-45]),
+            ((None, None, None), (f([40, 3, 2000], torch.int32), None, None), (None, f([0.9, 0.4]), None), (f([3000, 900, 20], torch.int32), f([0.97, 0.4]), f([0.0, 0.2, 1e-9]))))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_temperatures_next_to_zero_for_the_oracle(dtype):
+    u, t, settings = _freezing(42, "cpu")
+    for args in settings:
+        _check(_nearly_zero(42, 301, dtype, "cpu"), u, t, *args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [301, 5003, 60013])
+def test_temperatures_next_to_zero(cuda, vocab, dtype):
+    """Logits whose differences such temperatures still part: what is 2^-1000 of the largest counts as none, what is more has its weight."""
+    u, t, settings = _freezing(42, cuda)
+    for args in settings:
+        _check(_nearly_zero(42, vocab, dtype, cuda), u, t, *args)
