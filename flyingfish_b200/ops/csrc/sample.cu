@@ -167,16 +167,18 @@ __device__ __forceinline__ float ex2_approx(float x) { float y; asm("ex2.approx.
 template <typename T> struct SampleRow {
   float top;                            // the largest logit
   double c, wide_top;                   // log2(e) / T
-  float ch;                             // c rounded
-  float bins;                           // bins per unit of logit
+  float half_top, ch, bins;             // half the largest logit; twice c, rounded; bins per two units of logit
   const double* table;
   float far;                            // least logit that weighs anything
   __device__ __forceinline__ double weight(float l) const { return l >= far ? exp2_table(widen<T>(l) - wide_top, c, table) : 0.0; }
+  // half of what the largest logit is above l: a whole difference may be infinite, and infinity has no place in bins, nor octaves where c is zero
+  __device__ __forceinline__ float half_down(float l) const { return fmaf(l, -0.5f, half_top); }
   // octaves of a logit against the largest
-  __device__ __forceinline__ float octaves(float l) const { return (l - top) * ch; }
-  // never falls as l does: a difference and a product with a positive factor, each rounded, are monotone
+  __device__ __forceinline__ float octaves(float l) const { return half_down(l) * -ch; }
+  // never falls as l does: a difference and a product with a factor that is not negative, each rounded, are monotone
+  __device__ __forceinline__ float place(float l) const { return half_down(l) * bins; }
   __device__ __forceinline__ int bin(float l) const {
-    const float x = (top - l) * bins;
+    const float x = place(l);
     return x < (float)(SM_BINS - 1) ? (int)x : SM_BINS - 1;
   }
 };
@@ -429,10 +431,11 @@ sample_tokens_kernel(const SampleArgs a) {
     r.c *= 1.0 / UP; below *= UP;
   }
   r.wide_top = widen<T>(r.top);
-  r.ch = fminf((float)r.c, 1e30f);
-  r.bins = fminf((float)(r.c * 16.0), 1e30f);
+  r.half_top = 0.5f * r.top;
+  r.ch = fminf((float)(r.c * 2.0), 2e30f);
+  r.bins = fminf((float)(r.c * 32.0), 2e30f);
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
-  r.far = fmaxf(r.ch > 0.f ? __fadd_ru(r.top, SM_FAR / r.ch) : -INFINITY, -3.4028235e38f);      // rounded up: the next number below may lie thousands of octaves lower
+  r.far = fmaxf(r.ch > 0.f ? __fadd_ru(r.top, 2.f * SM_FAR / r.ch) : -INFINITY, -3.4028235e38f);      // rounded up: the next number below may lie thousands of octaves lower
   const float least = use_m ? fminf(r.top, __double2float_ru((double)r.top + below)) : -INFINITY;
 
   // The draw within the run of ids of warp `owner` of this CTA, by all of its warps: the lowest id at which the sum of kept weights, `from` in front of
@@ -662,7 +665,7 @@ sample_tokens_kernel(const SampleArgs a) {
     }
     // ---- 4: the general path ----
     // the bins divide the range of the candidates, where it is known
-    if (cut > -INFINITY && r.top - cut > 0.f) r.bins = fminf(r.bins * 64.f, (float)(SM_BINS - 1) / (r.top - cut));
+    if (cut > -INFINITY && r.half_down(cut) > 0.f) r.bins = fminf(r.bins * 64.f, (float)(SM_BINS - 1) / r.half_down(cut));
     const float per_bin = r.bins > 0.f ? r.ch / r.bins : 0.f;
     __syncthreads();
     for (int i = tid; i < SM_BINS; i += SM_THREADS) { sh.all_count[i] = 0; sh.all_high[i] = 0; sh.all_low[i] = 0; sh.count[i] = 0; sh.mass_of[i] = 0; }
@@ -816,7 +819,7 @@ sample_tokens_kernel(const SampleArgs a) {
     const float lo_x = lo < SM_BINS ? (float)lo : __uint_as_float(0x7fffffffu), hi_x = hi < SM_BINS - 1 ? (float)(hi + 1) : __uint_as_float(0x7fffffffu);
     const float cut_in = fmaxf(cut, -3.4028235e38f), heavy = fmaxf(cut_in, r.far);
     auto at_border = [&](float l) {
-      const float x = (r.top - l) * r.bins;
+      const float x = r.place(l);
       const unsigned key = key_of<T>(l);
       return l >= cut_in && x >= lo_x && !(x >= hi_x) && key >= key_lo && key <= key_hi;
     };
@@ -827,7 +830,7 @@ sample_tokens_kernel(const SampleArgs a) {
         load_vec<T>(mine + i, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float x = (r.top - v[e]) * r.bins;
+          const float x = r.place(v[e]);
           const unsigned key = key_of<T>(v[e]);
           const bool until = !(x >= hi_x), front = !(x >= lo_x) || (until && key > key_hi), weighs = v[e] >= heavy;
           const double w = exp2_table(widen<T>(v[e]) - r.wide_top, r.c, r.table);

@@ -356,3 +356,31 @@ def test_temperatures_next_to_zero(cuda, vocab, dtype):
     u, t, settings = _freezing(42, cuda)
     for args in settings:
         _check(_nearly_zero(42, vocab, dtype, cuda), u, t, *args)
+
+
+def _far_apart(rows, vocab, dtype, device):
+    """Logits whose distance from the largest passes the largest number of their type, and infinite temperatures, which make them all alike."""
+    g = torch.Generator().manual_seed(vocab + rows)
+    low = torch.finfo(dtype).min
+    x = torch.randn(rows, vocab, generator=g).clamp(-3, 3) * 1e38
+    x = torch.where(torch.rand(rows, vocab, generator=g) < torch.tensor([0.9, 0.1, 0.5])[torch.arange(rows) % 3][:, None], torch.tensor(low), x)
+    f = lambda v, t=F32: torch.tensor([v[i % len(v)] for i in range(rows)], dtype=t, device=device)
+    t = f([math.inf, 1e38, 1.0, 3e38, 1e36, math.inf, 1e30])
+    k, p = f([1500, vocab // 2, vocab - 40, 3001, 30], torch.int32), f([0.9, 0.6, 0.31])
+    return x.to(dtype).to(device), f([0.3, 0.0, 0.777, 0.9999]), t, ((None, None, None), (k, None, None), (None, p, None), (k, p, f([0.0, 0.01, 0.2, 0.0])))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_logits_far_apart_for_the_oracle(dtype):
+    l, u, t, settings = _far_apart(24, 5003, dtype, "cpu")
+    for args in settings:
+        _check(l, u, t, *args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [5003, 30011])
+def test_logits_far_apart(cuda, vocab, dtype):
+    l, u, t, settings = _far_apart(24, vocab, dtype, cuda)
+    for args in settings:
+        _check(l, u, t, *args)
