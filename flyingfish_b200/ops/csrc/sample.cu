@@ -29,6 +29,7 @@ namespace ff {
 
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CLUSTER = 8;
 constexpr int SM_BINS = 1024, SM_LIST = 1024, SM_SMALL = 128, SM_TABLE = 32, SM_COPIES = 16, SM_PARTS = SM_CLUSTER * SM_WARPS;
+constexpr int SM_MOST_SMEM = 227 * 1024, SM_STEP_BYTES = 512, SM_MOST_STEPS = 32;        // most steps of a warp's run: one per lane where the draw looks for the step
 constexpr float SM_FAR = -1000.f;       // octaves below the largest from which on a token weighs nothing
 
 struct SampleArgs {
@@ -58,7 +59,7 @@ struct SampleShared {
   SampleFound found;
   unsigned border_key;
   int border_id, list_n, at, owner;
-  double step_sum[32];                  // mass of each step of the run that holds the draw
+  double step_sum[SM_MOST_STEPS];       // mass of each step of the run that holds the draw
   union {
     struct {                            // a list of tokens: key << 32 | ~id, and their weights; where the bins of a sort begin
       unsigned long long list[SM_LIST];
@@ -439,7 +440,7 @@ sample_tokens_kernel(const SampleArgs a) {
   const float least = use_m ? fminf(r.top, __double2float_ru((double)r.top + below)) : -INFINITY;
 
   // The draw within the run of ids of warp `owner` of this CTA, by all of its warps: the lowest id at which the sum of kept weights, `from` in front of
-  // the run, passes the goal. Shared memory holds runs of 28 steps at most; their sums first, then the step's tokens (48 rows of 128256 7 us
+  // the run, passes the goal. Shared memory holds runs of 24 steps at most; their sums first, then the step's tokens (48 rows of 128256 7 us
   // less than with one warp that walks step by step).
   auto walk = [&](int owner, double from, double goal, unsigned border_key, int border_id, double kept_all) {
     const T* run = slice + owner * a.seg;
@@ -964,7 +965,8 @@ using namespace ff;
 
 template <typename T>
 static int sample_launch(const SampleArgs& args, int rows, cudaStream_t stream) {
-  constexpr int STEP = 32 * (16 / (int)sizeof(T)), MOST = 227 * 1024;
+  constexpr int STEP = SM_STEP_BYTES / (int)sizeof(T), MOST = SM_MOST_SMEM;
+  static_assert((MOST - (int)sizeof(SampleShared)) / (SM_WARPS * SM_STEP_BYTES) <= SM_MOST_STEPS, "a run's steps have a lane each");
   const int fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16;
   SampleArgs a = args;
   // As many CTAs of at least 2048 tokens as stand on the GPU at once, two to an SM: a CTA has about 15 us of steps that wait, so a second wave costs more
