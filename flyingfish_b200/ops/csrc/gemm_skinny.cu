@@ -262,7 +262,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                    __nv_bfloat16* __restrict__ Y, int M, int N, int K, int ldy, int ntok, int tile_rows, int stages,
                    int cl_size, int pipe_off, float* __restrict__ scratch, int* __restrict__ counters, int* status,
                    PeerArena ar, SkinnyEpi ep, const SkinnyTail tail, const __grid_constant__ std::conditional_t<BW != 0, LoraDev, NoLora> lora) {
-  pdl_trigger();
+  if constexpr (BW == 0) pdl_trigger();
   if (cl_size > 1) cluster_arrive_relaxed();         // phase A: "this CTA runs" (waited on before the first remote store)
   if (threadIdx.x == 0) FF_TL(status, KID_GEMM_SKINNY, 0);
   extern __shared__ uint8_t smem_raw[];
@@ -328,7 +328,9 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       }
     FF_TL(status, KID_GEMM_SKINNY, 2);
   }
-  if (warp == 1) { tmem_alloc(&bars.tmem_base, tmem_cols); tmem_relinquish(); }
+  // With adapters the kernel in front (lora.cu) may still hold tensor memory here, and a kernel behind may take its own before its wait: this one's dependents
+  // start only when it has what it needs.
+  if (warp == 1) { tmem_alloc(&bars.tmem_base, tmem_cols); tmem_relinquish(); if constexpr (BW != 0) pdl_trigger(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
