@@ -790,9 +790,10 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     bars.abort_flag = 0;
     mbar_fence_init();
   }
-  // With adapters the kernel in front (lora.cu) lets this one start only when it has its tensor memory and everything before it is done: X and the ids are
-  // there, and the wait stands in front of the first t.
+  // With adapters the kernel in front (lora.cu) lets this one start only when it has its tensor memory and everything before it is done; X and the ids are there,
+  // and the wait stands in front of the first t.
   if constexpr (BW == 0) pdl_wait();
+  else if (threadIdx.x == 64) lora_see_ready(lora.a);
   // after the wait: no kernel of this stream that still has tensor memory to allocate can be running. All 512 columns, so that both
   // CTAs' accumulators have the same addresses.
   if (warp == 1) { tmem_alloc_pair(&bars.tmem_base, 512); tmem_relinquish_pair(); }
@@ -828,6 +829,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (warp == 0) {
           if (elect_one()) {
             const uint32_t bytes = 2 * A_BYTES + width * BK * 2;
+            lora_ready_for_tma();
             for (int kb = 0; kb < kblocks; ++kb, at.next(stages)) {
               const int s = at.s;
               if (!mbar_wait(&bars.empty[s], at.ph ^ 1, abort_flag, status, KID_GEMM_BF16, 5)) { ok = false; break; }
@@ -894,6 +896,12 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (warp == 1 && rank == 0 && ok && elect_one()) umma_commit_pair(&bars.tmem_full[acc]);
         __syncwarp();
         if (more) { next.vote(); rows = next; }
+      }
+      if (warp == 0) {
+        // also where no tile had a unit: the kernel behind takes the end of this one for the end of all before it
+        if (!waited) pdl_wait();
+        if (lane == 0) lora_clear_ready(lora.a);
+        __syncwarp();
       }
       // the last commits of the even CTA have arrived before this CTA leaves (see below)
       if (warp == 0 && elect_one())
@@ -1094,7 +1102,7 @@ static int gemm_bf16_launch(const void* X, const void* W, void* Y, int M, int N,
   CUtensorMap tmA;
   if (int e = make_tmap_2d(&tmA, X, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, K, M, (uint64_t)ldx * 2, BK, BM)) return e;
   LoraDev dev = {};
-  if (lora != nullptr) dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts, lora->bw};
+  if (lora != nullptr) dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts, lora->bw, lora->ready, lora->call};
   PairTiles pt;
   float waves;
   if (one_cta_tiles(M, N, K, epi, tail.gate != 0, pt, waves)) {

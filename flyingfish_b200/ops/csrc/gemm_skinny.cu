@@ -328,6 +328,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       }
     FF_TL(status, KID_GEMM_SKINNY, 2);
   }
+  if constexpr (BW != 0) { if (threadIdx.x == 64) lora_see_ready(lora.a); }
   // With adapters the kernel in front (lora.cu) may still hold tensor memory here, and a kernel behind may take its own before its wait: this one's dependents
   // start only when it has what it needs.
   if (warp == 1) { tmem_alloc(&bars.tmem_base, tmem_cols); tmem_relinquish(); if constexpr (BW != 0) pdl_trigger(); }
@@ -341,9 +342,8 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   if (warp == 0) {
     if (elect_one()) {
       const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      // With adapters the kernel in front of this one (lora.cu) lets it start only once everything before that kernel is done: X and the ids are there, the
-      // weights stream while t is computed, and the wait stands in front of the first t.
       if constexpr (BW == 0) pdl_wait();
+      else lora_ready_for_tma();                       // X is there, the wait stands in front of the first t
       FF_TL(status, KID_GEMM_SKINNY, 3);
       uint32_t it = 0, t_it = 0; RingPos rp; bool ok = true, listed = false, waited = false;
       long long u = u0; Segment sg;
@@ -480,6 +480,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     const int vpr = tile_rows / 8;                // 8-value vectors per tile row
     if constexpr (BW != 0) lora_list(lists, lora.a, M, N, e, share_of(first_tile), share_of((int)((u1 - 1) / kblocks)), status);
     pdl_wait();                                   // scratch, counters, the arena and Y belong to earlier kernels until here
+    if constexpr (BW != 0) { if (e == 0) lora_clear_ready(lora.a); }
     if (e == 0) FF_TL(status, KID_GEMM_SKINNY, 7);
     int ar_epoch = 0;
     if (FUSE_AR) ar_epoch = ld_volatile(arena_epoch(ar)) + 1;
@@ -1017,7 +1018,7 @@ static int gemm_skinny_launch(const void* X, const void* W, void* Y, int M, int 
   const PeerArena none = {};
   if (lora != nullptr) {
     LoraDev dev = {};
-    dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts, lora->bw};
+    dev.a = {lora->ids, lora->ranks, lora->part_of, lora->adapters, lora->R, lora->parts, lora->bw, lora->ready, lora->call};
     if (int e = lora_maps(dev, lora->t, lora->b, M, N, ntok, cfg.tile_rows, cfg.tile_rows)) return e;
     // behind the ring: both words of t of two steps (the instruction reads 128 rows of each)
     const int stage = (ntok + cfg.tile_rows) * SBK * 2, t_room = (3 * ntok + STOK) * lora->bw * 2, most = (M <= 64 ? SK_LORA_SMEM_FEW : SK_LORA_SMEM) - 1024 - cfg.pipe_off - t_room;

@@ -25,6 +25,7 @@ struct LoraCall {
   const void *t, *b;
   const int *ids, *ranks, *part_of;
   int adapters, R, parts, bw;          // bw: ranks of a step, 16 or 32
+  unsigned long long *ready, call;     // the word behind t, and the number of the call
 };
 int ff_gemm_skinny_lora(const void* X, const void* W, void* Y, int M, int N, int K, int ldx, int ldw, int ldy, int grid, float* scratch, int* counters,
                         const LoraCall* lora, int epi, int gate, float limit, const QkvRope* rope, int* status, cudaStream_t stream);

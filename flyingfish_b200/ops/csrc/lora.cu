@@ -65,8 +65,13 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   if (warp >= 2 && e < a.adapters && table) { sh.step_table[e] = lora_steps(a, e); sh.scale_table[e] = scale[e]; }
   pdl_wait();
   // Tensor memory behind the wait, as in gemm_bf16.cu: what is taken here is not in the way of a kernel that still has to take its own. With it in hand the
-  // kernel behind this one may start: it finds X and the ids done, takes its own and streams its weights meanwhile.
-  if (warp == 1) { tmem_alloc(&sh.tmem_base, tmem_cols); tmem_relinquish(); pdl_trigger(); }
+  // kernel behind this one may start: it is told that X and the ids are done, takes its own and streams its weights meanwhile.
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem_base, tmem_cols); tmem_relinquish();
+    if (lane == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) lora_set_ready(a);
+    __syncwarp();
+    pdl_trigger();
+  }
   if (warp >= 2) {
     // distinct adapters of the tile and where their units lie in the tile's list, in the order of their first rows
     int id = row0 + e < M ? a.ids[row0 + e] : -1;
@@ -219,17 +224,19 @@ struct FfLora {
   const void *a, *b;
   const float* scale;
   const int *ranks, *ids, *part_of;
-  void* t;                             // [M, 2R] BF16
+  void* t;                             // [M, 2R] BF16, and a word of 64 bits
   float* scratch;                      // scratch and counters of the decode product
   int *counters, *status;
   const float* cos_sin;
   const int* slots;
   void *kcache, *vcache;
-  long long scratch_bytes, counter_bytes;
+  long long scratch_bytes, counter_bytes, call;          // call: a number that no other call has
   int M, N, K, ldx, ldw, ldy, R, adapters, parts, step, epi, gate;          // step: ranks of a step of a fused projection
   float limit;
   int hq, hkv, rot_dim, block_size, num_blocks;
 };
+
+static unsigned long long* lora_word(const FfLora& c) { return reinterpret_cast<unsigned long long*>(static_cast<__nv_bfloat16*>(c.t) + (size_t)c.M * 2 * c.R); }
 
 static int lora_shrink(const FfLora& c, int bw, cudaStream_t stream) {
   const int tiles = (c.M + LS_ROWS - 1) / LS_ROWS, xrows = c.M < LS_ROWS ? (c.M + 15) / 16 * 16 : LS_ROWS, per = c.R / bw;
@@ -259,7 +266,7 @@ static int lora_shrink(const FfLora& c, int bw, cudaStream_t stream) {
   const int slack = stage < LS_ROWS * 128 ? LS_ROWS * 128 - stage : 0, recv_off = stages * stage, smem = 1024 + recv_off + (recv > slack ? recv : slack);
   auto kern = bw == 32 ? lora_shrink_kernel<32> : lora_shrink_kernel<16>;
   if (int e = opt_in_smem(kern, LS_SMEM)) return e;
-  const LoraArgs args = {c.ids, c.ranks, c.part_of, c.adapters, c.R, c.parts, bw};
+  const LoraArgs args = {c.ids, c.ranks, c.part_of, c.adapters, c.R, c.parts, bw, lora_word(c), (unsigned long long)c.call};
   return launch_pdl(kern, dim3(LS_SPLIT, passes, tiles), dim3(192), smem, stream, LS_SPLIT, tmX, tmA, args, c.scale,
                     static_cast<__nv_bfloat16*>(c.t), c.M, c.K, xrows, most, stages, recv_off, c.status);
 }
@@ -280,7 +287,7 @@ FF_EXPORT int ff_linear_lora(const FfLora* p, cudaStream_t stream) {
   const QkvRope rope = {c.cos_sin, c.slots, c.kcache, c.vcache, c.hq, c.hkv, c.rot_dim, c.block_size, c.num_blocks};
   // units of 32 ranks are one copy where two of 16 are two; a stack of 16 has no more, and the steps of a fused projection are given
   const int bw = c.part_of != nullptr ? c.step : c.R % 32 ? 16 : 32;
-  const LoraCall lora = {c.t, c.b, c.ids, c.ranks, c.part_of, c.adapters, c.R, c.parts, bw};
+  const LoraCall lora = {c.t, c.b, c.ids, c.ranks, c.part_of, c.adapters, c.R, c.parts, bw, lora_word(c), (unsigned long long)c.call};
   if (c.M > FF_SKINNY_MAX_ROWS) {
     if (c.N % 8 || c.ldy % 8 || (reinterpret_cast<uintptr_t>(c.y) & 15)) return FF_HOST_BAD_ALIGN;       // before anything is launched
     if (int e = lora_shrink(c, bw, stream)) return e;

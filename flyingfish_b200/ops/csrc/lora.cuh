@@ -15,6 +15,7 @@ namespace ff {
 struct LoraArgs {
   const int *ids, *ranks, *part_of;    // ranks, part_of: may be null
   int adapters, R, parts, bw;
+  unsigned long long *ready, call;     // where the call's number says that X and the ids are there
 };
 
 struct LoraDev {                       // kernel parameter
@@ -22,6 +23,21 @@ struct LoraDev {                       // kernel parameter
   LoraArgs a;
 };
 struct NoLora {};
+
+// What lies in front of a call -- X, the ids, tables of angles -- may reach the product before t does: the shrink waits for it, writes the call's number to
+// `ready`, and only then lets the product start. A product that finds the number there has what it stands for (release and acquire, on the GPU) and puts its
+// wait for the shrink in front of the first t; one that does not waits at once. Nobody polls. The word lies behind t and holds anything before a call: numbers
+// are 63 bits, of a process's own, and the product's first CTA takes its call's away again, so that a replay does not find the number of the one before.
+__device__ __forceinline__ void lora_set_ready(const LoraArgs& a) { asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(a.ready), "l"(a.call) : "memory"); }
+__device__ __forceinline__ void lora_see_ready(const LoraArgs& a) {
+  unsigned long long v;
+  asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(a.ready) : "memory");
+  if (v != a.call) pdl_wait();
+}
+// in front of loads by the TMA engine of what lora_see_ready() stands for
+__device__ __forceinline__ void lora_ready_for_tma() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
+// one thread, behind a wait of its own; a CTA that looks later waits
+__device__ __forceinline__ void lora_clear_ready(const LoraArgs& a) { if (blockIdx.x == 0) *a.ready = 0; }
 
 __device__ __forceinline__ int lora_steps(const LoraArgs& a, int adapter) {
   const int r = a.ranks == nullptr ? a.R : min(max(a.ranks[adapter], 0), a.R);

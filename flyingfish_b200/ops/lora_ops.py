@@ -8,6 +8,8 @@ read ahead of what the stream still holds, and calls of up to 128 rows use the d
 from __future__ import annotations
 
 import ctypes
+import itertools
+import os
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import NamedTuple
 
@@ -16,6 +18,7 @@ import torch
 from . import BF16, SKINNY_MAX_M, _count, _require, _rows2d, ref, rope_in_product, rope_kv_paged, rope_table, silu_mul_interleaved, workspace
 from .lib import KernelError, check, kernels, status_tensor
 
+_calls = itertools.count(int.from_bytes(os.urandom(8), "little") | 1 << 62)          # numbers of calls: what a word of memory does not hold by chance
 MAX_RANK = 1024                  # rank rows of a stack, all parts of a fused projection together
 GATES = (0, 3, 5)                # gates that the products' epilogues know (ops.linear_swiglu)
 
@@ -81,7 +84,7 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
 
 class _Lora(ctypes.Structure):            # FfLora of csrc/lora.cu
     _fields_ = [(n, c_void_p) for n in ("x", "w", "y", "a", "b", "scale", "ranks", "ids", "part_of", "t", "scratch", "counters", "status", "cos_sin",
-                                        "slots", "kcache", "vcache")] + [("scratch_bytes", c_longlong), ("counter_bytes", c_longlong)] + \
+                                        "slots", "kcache", "vcache")] + [("scratch_bytes", c_longlong), ("counter_bytes", c_longlong), ("call", c_longlong)] + \
                [(n, c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "R", "adapters", "parts", "step", "epi", "gate")] + [("limit", c_float)] + \
                [(n, c_int) for n in ("hq", "hkv", "rot_dim", "block_size", "num_blocks")]
 
@@ -127,14 +130,14 @@ def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tenso
     if m == 0:
         return out
     dev = x.device
-    t = x.new_empty(m, 2 * r)                       # of this call alone
+    t, call = x.new_empty(m * 2 * r + 4), next(_calls) & (1 << 63) - 1          # of this call alone
     ws = workspace(dev)
     cs, slots, kc, vc, heads = rope if rope is not None else (None, None, None, None, (0, 0, 0, 0, 0))
     lib, stream = kernels(), c_void_p(torch._C._cuda_getCurrentRawStream(at))
     for attempt in (0, 1):
         form = _Lora(x.data_ptr(), w.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), _at(ranks), ids.data_ptr(), _at(part_of), t.data_ptr(),
                      ws.gemm_scratch.data_ptr(), ws.gemm_counters.data_ptr(), status_tensor(dev).data_ptr(), _at(cs), _at(slots), _at(kc), _at(vc),
-                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, m, n, k, ldx, ldw, out.stride(0), r, count, parts, step, epi, gate, limit, *heads)
+                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, call, m, n, k, ldx, ldw, out.stride(0), r, count, parts, step, epi, gate, limit, *heads)
         rc = lib.ff_linear_lora(ctypes.byref(form), stream)
         if rc != -5 or attempt or m > SKINNY_MAX_M:
             break

@@ -275,3 +275,51 @@ def test_refusals_on_the_device(cuda):
     with pytest.raises(KernelError):
         lora_ops.linear_lora(x, w, st, ids)
     ops.check_status(cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 7, 64, 113, 200, 300, 600])
+def test_inputs_written_just_before(cuda, m):
+    """X and the ids come from kernels that end just before the call, over and over into the same memory, eagerly and replayed: every call reads its own. Some calls
+    have rows without adapters only, or a stack none of whose live steps has columns."""
+    k, n, count = 1024, 1536, 5
+    _, w, st, _ = _case(m, k, n, 32, count, seed=m, device=cuda)
+    blind = st._replace(part_of=torch.ones(n // 64, dtype=torch.int32, device=cuda), parts=2, step=16, ranks=torch.full_like(st.ranks, 16))
+    g = torch.Generator().manual_seed(m)
+    rounds = 24
+    raw = torch.randn(rounds, m, k, generator=g).to(BF16).to(cuda)
+    who = torch.randint(-1, count, (rounds, m), generator=g, dtype=torch.int32)
+    who[::5] = -1
+    who = who.to(cuda)
+    gain = torch.ones(k, dtype=BF16, device=cuda)
+    stacks = [blind if i % 7 == 3 else st for i in range(rounds)]
+    want = []
+    for i in range(rounds):
+        x = ops.rmsnorm(raw[i], gain, 1e-6)
+        torch.cuda.synchronize()
+        want.append(lora_ops.linear_lora(x, w, stacks[i], who[i]))
+        torch.cuda.synchronize()
+    x, ids = torch.empty(m, k, dtype=BF16, device=cuda), torch.empty(m, dtype=torch.int32, device=cuda)
+
+    def run():
+        out = []
+        for i in range(rounds):
+            ids.copy_(who[i])
+            x.copy_(ops.rmsnorm(raw[i], gain, 1e-6))
+            out.append(lora_ops.linear_lora(ops.rmsnorm(x, gain, 0.0) if i % 2 else x, w, stacks[i], ids))
+            x.fill_(float("nan"))                        # behind the call
+            ids.fill_(0)
+        return out
+    again = [lora_ops.linear_lora(ops.rmsnorm(ops.rmsnorm(raw[i], gain, 1e-6), gain, 0.0), w, stacks[i], who[i]) if i % 2 else want[i] for i in range(rounds)]
+    torch.cuda.synchronize()
+    for i, y in enumerate(run()):
+        assert torch.equal(y, again[i]), i
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(3):
+        graph.replay()
+        for i, y in enumerate(out):
+            assert torch.equal(y, again[i]), i
+    ops.check_status(cuda)
