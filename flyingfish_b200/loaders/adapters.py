@@ -118,9 +118,9 @@ def _one_part(entries: list, columns: list[int]) -> list:
         at = 0
         for (pa, pb, scale), c in have:
             first = sum(columns[:c])
-            b[first: first + columns[c], at: at + pa.shape[0]] = pb.float() * scale
+            b[first: first + columns[c], at: at + pa.shape[0]] = pb.float()
             at += pa.shape[0]
-        out.append([(a, b, 1.0)])
+        out.append([(a, b, torch.cat([torch.full((p[0].shape[0],), float(p[2])) for p, _ in have]))])
     return out
 
 

@@ -1,6 +1,6 @@
 // Low-rank adapters of many requests beside a shared projection:  Y[M,N] = X W^T + delta,  delta_r = B_a (s_a A_a x_r)  for the
 // adapter a = ids[r] of row r, no delta where ids[r] is negative. A stack holds the adapters of one projection: A [adapters, R, K],
-// B [adapters, N, R], scales and ranks (rank rows behind an adapter's own are zero and not read). R is a multiple of 16.
+// B [adapters, N, R], scales (of an adapter, or of each of its rank rows) and ranks (rank rows behind an adapter's own are zero and not read). R is a multiple of 16.
 //
 //   lora_shrink_kernel (here)   t_r = s_a A_a x_r: [M, 2R], every value as two BF16 words, t = high + low
 //   the product with W          gemm_skinny.cu, gemm_bf16.cu: B_a t_r is accumulated behind the product's own K blocks (lora.cuh), one rounding at the end
@@ -39,7 +39,7 @@ struct alignas(16) ShrinkShared {
 // ascending order. blockIdx.y: passes y, y + gridDim.y, ... over the tile's units.
 template <int BW>
 __global__ void __launch_bounds__(192)
-lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const LoraArgs a, const float* __restrict__ scale,
+lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const LoraArgs a, const float* __restrict__ scale, int scales,
                    __nv_bfloat16* __restrict__ t, int M, int K, int xrows, int most, int stages, int recv_off, int* status) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ ShrinkShared sh;
@@ -62,7 +62,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
   }
   const int e = threadIdx.x - 64;
   const bool table = a.adapters <= LS_TABLE;
-  if (warp >= 2 && e < a.adapters && table) { sh.step_table[e] = lora_steps(a, e); sh.scale_table[e] = scale[e]; }
+  if (warp >= 2 && e < a.adapters && table) { sh.step_table[e] = lora_steps(a, e); sh.scale_table[e] = scales ? 0.f : scale[e]; }
   pdl_wait();
   // Tensor memory behind the wait, as in gemm_bf16.cu: what is taken here is not in the way of a kernel that still has to take its own. With it in hand the
   // kernel behind this one may start: it is told that X and the ids are done, takes its own and streams its weights meanwhile.
@@ -79,7 +79,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     sh.id[e] = id;
     int steps = 0;
     float f = 0.f;
-    if (!table && id >= 0) { steps = lora_steps(a, id); f = scale[id]; }
+    if (!table && id >= 0) { steps = lora_steps(a, id); f = scales ? 0.f : scale[id]; }
     asm volatile("bar.sync 1, 128;" ::: "memory");
     if (table && id >= 0) { steps = sh.step_table[id]; f = sh.scale_table[id]; }
     int first = e;
@@ -192,11 +192,13 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         const float4 x = *reinterpret_cast<const float4*>(recv + ((j * LS_SPLIT + c) * 16 + (row >> 3)) * BW + 4 * quad);
         v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
       }
-      const float f = sh.scale[row];
+      float f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = scales ? scale[(size_t)sh.id[row] * a.R + BW * step + 4 * quad + k] : sh.scale[row];
       float low[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[k] *= f;
+        v[k] *= f[k];
         const float h = __bfloat162float(__float2bfloat16(v[k]));
         low[k] = isinf(h) ? 0.f : v[k] - h;              // an infinite first word has no second: infinity less infinity would be NaN
       }
@@ -231,7 +233,7 @@ struct FfLora {
   const int* slots;
   void *kcache, *vcache;
   long long scratch_bytes, counter_bytes, call;          // call: a number that no other call has
-  int M, N, K, ldx, ldw, ldy, R, adapters, parts, step, epi, gate;          // step: ranks of a step of a fused projection
+  int M, N, K, ldx, ldw, ldy, R, adapters, parts, step, epi, gate, scales;  // step: ranks of a step of a fused projection; scales: 1 with a scale per rank row
   float limit;
   int hq, hkv, rot_dim, block_size, num_blocks;
 };
@@ -267,7 +269,7 @@ static int lora_shrink(const FfLora& c, int bw, cudaStream_t stream) {
   auto kern = bw == 32 ? lora_shrink_kernel<32> : lora_shrink_kernel<16>;
   if (int e = opt_in_smem(kern, LS_SMEM)) return e;
   const LoraArgs args = {c.ids, c.ranks, c.part_of, c.adapters, c.R, c.parts, bw, lora_word(c), (unsigned long long)c.call};
-  return launch_pdl(kern, dim3(LS_SPLIT, passes, tiles), dim3(192), smem, stream, LS_SPLIT, tmX, tmA, args, c.scale,
+  return launch_pdl(kern, dim3(LS_SPLIT, passes, tiles), dim3(192), smem, stream, LS_SPLIT, tmX, tmA, args, c.scale, c.scales,
                     static_cast<__nv_bfloat16*>(c.t), c.M, c.K, xrows, most, stages, recv_off, c.status);
 }
 

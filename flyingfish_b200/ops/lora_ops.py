@@ -24,8 +24,8 @@ GATES = (0, 3, 5)                # gates that the products' epilogues know (ops.
 
 
 class AdapterStack(NamedTuple):
-    """The adapters of one projection ``[N, K]``. ``a`` [adapters, R, K] and ``b`` [adapters, N, R] are BF16, ``scale`` FP32 [adapters]; R is a multiple of
-    16 and the rank rows behind an adapter's own are zero. ``ranks`` (int32 [adapters]) says how many rows that are, so that the rest is
+    """The adapters of one projection ``[N, K]``. ``a`` [adapters, R, K] and ``b`` [adapters, N, R] are BF16, ``scale`` FP32 [adapters], or [adapters, R]
+    where an adapter's rank rows have scales of their own; R is a multiple of 16 and the rank rows behind an adapter's own are zero. ``ranks`` (int32 [adapters]) says how many rows that are, so that the rest is
     not read. ``part_of`` (int32 [N / 64]), ``parts`` and ``step`` describe a fused projection: its adapters' ranks come in steps of ``step`` (16 or 32), step s
     belongs to part ``s % parts``, and the 64 columns from ``64 i`` have non-zero ``b`` in the steps of part ``part_of[i]`` only."""
     a: torch.Tensor
@@ -44,7 +44,7 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
                dtype: torch.dtype = BF16, interleave: bool = False) -> AdapterStack:
     """``adapters``: for every adapter one entry per part of the projection (one part, or those of a fused one, ``columns`` wide each): ``(A [r, K],
     B [columns, r], scale)`` or None where the adapter leaves the part alone. ``interleave``: two parts whose columns lie in turns of 64 (gate and up).
-    An adapter's scale goes with its parts: parts of different scales share the first one, the others' ``B`` takes the quotient."""
+    A part's scale is a number, or a tensor of one per rank. Neither matrix takes a scale into itself: with different ones the stack has a scale per rank row."""
     parts, n = len(columns), sum(columns)
     _require(bool(adapters) and all(len(p) == parts for p in adapters), "pack_stack: an entry per part for every adapter")
     _require(not interleave or (parts == 2 and columns[0] == columns[1] and columns[0] % 64 == 0), "pack_stack: two equal parts interleave")
@@ -56,22 +56,25 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
     a = torch.zeros(len(adapters), r, k, dtype=dtype)
     b = torch.zeros(len(adapters), n, r, dtype=dtype)
     scale, ranks = torch.ones(len(adapters)), torch.zeros(len(adapters), dtype=torch.int32)
+    scales, alike = torch.ones(len(adapters), r), True           # alike: every adapter's parts have one scale
     for i, entry in enumerate(adapters):
-        first = next((e[2] for e in entry if e is not None and e[2] != 0), 1.0)
-        scale[i] = first
-        at = 0
+        at, own = 0, []
         for j, part in enumerate(entry):
             if part is not None:
                 pa, pb, s = part
                 rank = pa.shape[0]
                 _require(pa.shape == (rank, k) and pb.shape == (columns[j], rank), f"pack_stack: adapter {i}: A [{rank}, {k}] and B [{columns[j]}, {rank}]")
+                pa, pb = pa.to("cpu", dtype), pb.to("cpu", dtype)
                 _require(bool(torch.isfinite(pa).all()) and bool(torch.isfinite(pb).all()), f"pack_stack: adapter {i} holds infinities or NaN")
                 where = torch.tensor([(q // step * parts + j) * step + q % step for q in range(rank)], dtype=torch.long)
-                a[i, where] = pa.to("cpu", dtype)
-                pb = pb.to("cpu", torch.float32) if s != first else pb.to("cpu")
-                b[i, at: at + columns[j], where] = (pb if s == first else pb * (s / first)).to(dtype)
+                a[i, where], b[i, at: at + columns[j], where] = pa, pb
+                scales[i, where] = torch.as_tensor(s, dtype=torch.float32)
+                own.append(scales[i, where])
                 ranks[i] = max(int(ranks[i]), (rank + step - 1) // step * step * parts)
             at += columns[j]
+        own = torch.cat([*own, torch.empty(0)])
+        if own.numel():
+            scale[i], alike = own[0], alike and bool((own == own[0]).all())
     part_of = None
     if interleave:
         b = b.view(len(adapters), 2, n // 128, 64, r).transpose(1, 2).reshape(len(adapters), n, r).contiguous()
@@ -79,13 +82,13 @@ def pack_stack(adapters: list[list[tuple[torch.Tensor, torch.Tensor, float] | No
     elif parts > 1:
         part_of = torch.repeat_interleave(torch.arange(parts, dtype=torch.int32), torch.tensor([c // 64 for c in columns]))
     move = lambda t: None if t is None else t.to(device)
-    return AdapterStack(move(a), move(b), move(scale), move(ranks), move(part_of), parts, step)
+    return AdapterStack(move(a), move(b), move(scale if alike else scales), move(ranks), move(part_of), parts, step)
 
 
 class _Lora(ctypes.Structure):            # FfLora of csrc/lora.cu
     _fields_ = [(n, c_void_p) for n in ("x", "w", "y", "a", "b", "scale", "ranks", "ids", "part_of", "t", "scratch", "counters", "status", "cos_sin",
                                         "slots", "kcache", "vcache")] + [("scratch_bytes", c_longlong), ("counter_bytes", c_longlong), ("call", c_longlong)] + \
-               [(n, c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "R", "adapters", "parts", "step", "epi", "gate")] + [("limit", c_float)] + \
+               [(n, c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "R", "adapters", "parts", "step", "epi", "gate", "scales")] + [("limit", c_float)] + \
                [(n, c_int) for n in ("hq", "hkv", "rot_dim", "block_size", "num_blocks")]
 
 
@@ -94,7 +97,7 @@ def _check_stack(x: torch.Tensor, n: int, stack: AdapterStack, ids: torch.Tensor
     a, b, scale, ranks, part_of, parts, step = stack
     _require(a.dim() == 3 and b.dim() == 3 and a.shape[2] == x.shape[1], "adapters: A [adapters, R, K] of the projection's K")
     count, r = a.shape[0], a.shape[1]
-    _require(b.shape == (count, n, r) and scale.shape == (count,), "adapters: B [adapters, N, R], a scale per adapter")
+    _require(b.shape == (count, n, r) and scale.shape in ((count,), (count, r)), "adapters: B [adapters, N, R], a scale per adapter or rank row")
     _require(count > 0 and 0 < r <= MAX_RANK and r % 16 == 0, f"adapters: R is a multiple of 16, at most {MAX_RANK}")
     _require(a.dtype == b.dtype == x.dtype and scale.dtype == torch.float32, "adapters: weights of the operands' type, FP32 scales")
     _require(a.is_contiguous() and b.is_contiguous() and scale.is_contiguous(), "adapters: contiguous weights")
@@ -137,7 +140,7 @@ def _run(x: torch.Tensor, w: torch.Tensor, stack: AdapterStack, ids: torch.Tenso
     for attempt in (0, 1):
         form = _Lora(x.data_ptr(), w.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), _at(ranks), ids.data_ptr(), _at(part_of), t.data_ptr(),
                      ws.gemm_scratch.data_ptr(), ws.gemm_counters.data_ptr(), status_tensor(dev).data_ptr(), _at(cs), _at(slots), _at(kc), _at(vc),
-                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, call, m, n, k, ldx, ldw, out.stride(0), r, count, parts, step, epi, gate, limit, *heads)
+                     ws.gemm_scratch.numel() * 4, ws.gemm_counters.numel() * 4, call, m, n, k, ldx, ldw, out.stride(0), r, count, parts, step, epi, gate, scale.dim() - 1, limit, *heads)
         rc = lib.ff_linear_lora(ctypes.byref(form), stream)
         if rc != -5 or attempt or m > SKINNY_MAX_M:
             break

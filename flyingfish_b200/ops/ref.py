@@ -362,7 +362,7 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tens
     for i in range(a.shape[0]):
         rows = torch.nonzero(ids == i).flatten()
         if rows.numel():
-            y[rows] += (float(scale[i]) * (x32[rows] @ a[i].to(F32).T)) @ b[i].to(F32).T
+            y[rows] += (scale[i].to(F32) * (x32[rows] @ a[i].to(F32).T)) @ b[i].to(F32).T
     return y.to(x.dtype)
 
 

@@ -323,3 +323,56 @@ def test_inputs_written_just_before(cuda, m):
         for i, y in enumerate(out):
             assert torch.equal(y, again[i]), i
     ops.check_status(cuda)
+
+
+def _parts_of_several_scales(k, cols, scales, device, seed=0):
+    """One adapter of rank 1 per scale set, whose A picks element 3 of x."""
+    g = torch.Generator().manual_seed(seed)
+    pick = torch.zeros(1, k)
+    pick[0, 3] = 1.0
+    return [[None if s is None else (pick.to(BF16), torch.randn(c, 1, generator=g).to(BF16), s) for c, s in zip(cols, row)] for row in scales]
+
+
+def test_no_matrix_takes_a_scale_into_itself():
+    cols, scales = [128, 64, 64], [(1.0, 41 / 32, 0.7), (0.3, 0.3, None), (None, None, None), (0.0, 2.0, 1e-3)]
+    parts = _parts_of_several_scales(64, cols, scales, "cpu")
+    for stack, one in ((lora_ops.pack_stack(parts, 64, cols, "cpu"), False), (lora_ops.pack_stack(parts[1:3], 64, cols, "cpu"), True)):
+        assert stack.scale.shape == ((2,) if one else (4, stack.a.shape[1]))
+        for i, row in enumerate(parts[1:3] if one else parts):
+            at = 0
+            for j, p in enumerate(row):
+                if p is not None:
+                    assert torch.equal(stack.b[i, at: at + cols[j], j * stack.step], p[1][:, 0])
+                    s = stack.scale[i] if one else stack.scale[i, j * stack.step]
+                    assert float(s) == pytest.approx(p[2], rel=2.0 ** -24)
+                at += cols[j]
+    from flyingfish_b200.loaders.adapters import _one_part
+    small = [[(torch.ones(1, 8, dtype=BF16), torch.tensor([[1.1], [0.3]]).to(BF16), s) for s in row] for row in ((0.7, 0.9), (0.7, 0.7))]
+    stack = lora_ops.pack_stack(_one_part(small, [2, 2]), 8, [4], "cpu")
+    assert torch.equal(stack.b[:, :2, 0], stack.b[:, 2:, 1]) and torch.equal(stack.b[0, :2, 0], small[0][0][1][:, 0])
+    assert stack.scale[0, :2].tolist() == torch.tensor([0.7, 0.9]).tolist() and stack.scale[1, :2].tolist() == torch.tensor([0.7, 0.7]).tolist()
+    with pytest.raises(KernelError):                     # what BF16 has no number for
+        lora_ops.pack_stack([[(torch.full((1, 8), 3.4e38), torch.ones(2, 1), 1.0)]], 8, [2], "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 128, 200, 600])
+@pytest.mark.parametrize("adapters", [3, 200])
+def test_scales_of_parts_cost_no_rounding(cuda, m, adapters):
+    """Rank-1 adapters of one element x, so that a delta is B s x with 8 + 6 + 8 bits: rounded once, it is within half a step of BF16 (and what FP32 sums of the two
+    words of t leave, 2^-22 of itself). B rounded with its scale first would be off by up to a whole step."""
+    k, cols = 64, [256, 128, 128]
+    sets = [(1.0, 41 / 32, 25 / 32), (37 / 32, 1.0, None), (0.5, 0.5, 0.5)]
+    stack = lora_ops.pack_stack(_parts_of_several_scales(k, cols, [sets[i % 3] for i in range(adapters)], cuda, m), k, cols, cuda)
+    assert stack.scale.dim() == 2
+    g = torch.Generator().manual_seed(m)
+    x = torch.randn(m, k, generator=g).to(BF16).to(cuda)
+    ids = torch.randint(-1, adapters, (m,), generator=g, dtype=torch.int32).to(cuda)
+    got = lora_ops.linear_lora(x, torch.zeros(sum(cols), k, dtype=BF16, device=cuda), stack, ids).double()
+    a, b, s = stack.a.double(), stack.b.double(), stack.scale.double()
+    safe = ids.long().clamp(min=0)
+    t = s[safe] * torch.einsum("mk,mrk->mr", x.double(), a[safe])
+    want = torch.einsum("mr,mnr->mn", t, b[safe]) * (ids >= 0)[:, None]
+    step = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=1e-30))) - 7)
+    assert ((got - want).abs() <= step / 2 * (1 + 2.0 ** -12)).all()
+    ops.check_status(cuda)
