@@ -19,7 +19,8 @@ from .safetensors_io import SafetensorsFile
 
 PROJECTIONS = {"self_attn": ("q_proj", "k_proj", "v_proj", "o_proj"), "mlp": ("gate_proj", "up_proj", "down_proj")}
 FILES = ("adapter_config.json", "adapter_model.safetensors")
-_NAME = re.compile(r"(?:^|\.)layers\.(\d+)\.(self_attn|mlp)\.(\w+)\.lora_([AB])(?:\.default)?\.weight$")
+# a decoder's own layers: not those of a tower that a larger model has beside it, whose names end alike
+_NAME = re.compile(r"^(?:base_model\.)?(?:model\.|language_model\.)*layers\.(\d+)\.(self_attn|mlp)\.(\w+)\.lora_([AB])(?:\.default)?\.weight$")
 
 Entries = dict[tuple[int, str], tuple[torch.Tensor, torch.Tensor, float]]      # (layer, projection) -> A [r, K], B [N, r], scale
 
@@ -90,7 +91,10 @@ def read_adapter(path: str | Path) -> Entries:
             raise AdapterError(f"{weights.name}: {name} changes none of the decoder's projections")
         layer, proj, side = int(m.group(1)), m.group(3), m.group(4)
         module = name[: name.index(".lora_")]
-        found.setdefault((layer, proj), {"module": module.removeprefix("base_model.model.")})[side] = f.tensor(name).clone()
+        entry = found.setdefault((layer, proj), {"module": module.removeprefix("base_model.model.")})
+        if side in entry:
+            raise AdapterError(f"{weights.name}: {name} is a second lora_{side} of layer {layer} {proj}")
+        entry[side] = f.tensor(name).clone()
     entries: Entries = {}
     for (layer, proj), e in found.items():
         if "A" not in e or "B" not in e or e["A"].dim() != 2 or e["B"].dim() != 2 or e["A"].shape[0] != e["B"].shape[1] or e["A"].shape[0] == 0:

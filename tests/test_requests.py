@@ -143,6 +143,28 @@ def test_broken_adapters_are_refused(tmp_path):
             build_adapters(net, {"x": {at: entry}})
 
 
+@pytest.mark.parametrize("prefix", ["base_model.model.vision_tower.encoder", "model.visual.transformer", "encoder", "model.language_model.visual"])
+def test_matrices_of_another_tower_are_refused(tmp_path, prefix):
+    with pytest.raises(AdapterError, match="none of the decoder"):
+        read_adapter(_write_adapter(tmp_path / "a", _entries(4, 1), names=prefix + ".layers.{l}.{m}.{p}.lora_{s}.weight"))
+
+
+@pytest.mark.parametrize("prefix", ["base_model.model.model", "base_model.model.model.language_model", "language_model.model", "model"])
+def test_a_decoders_names_are_known_with_what_stands_before_them(tmp_path, prefix):
+    got = read_adapter(_write_adapter(tmp_path / "a", _entries(4, 1), names=prefix + ".layers.{l}.{m}.{p}.lora_{s}.weight"))
+    assert set(got) == set(_entries(4, 1))
+
+
+def test_a_matrix_named_twice_is_refused(tmp_path):
+    path = tmp_path / "a"
+    path.mkdir()
+    (path / "adapter_config.json").write_text("{}")
+    a, b, _ = _entries(4, 1)[0, "q_proj"]
+    save_safetensors(path / "adapter_model.safetensors", {f"{p}layers.0.self_attn.q_proj.lora_{s}.weight": t for p in ("model.", "base_model.model.model.") for s, t in (("A", a), ("B", b))})
+    with pytest.raises(AdapterError, match="second"):
+        read_adapter(path)
+
+
 @pytest.mark.parametrize("shape", ["tiny-hybrid", "deepseek-v3-tiny"])
 def test_models_without_the_plain_projections_are_refused(shape):
     with pytest.raises(AdapterError):
