@@ -18,6 +18,7 @@ from ..ops import lora_ops
 from .safetensors_io import SafetensorsFile
 
 PROJECTIONS = {"self_attn": ("q_proj", "k_proj", "v_proj", "o_proj"), "mlp": ("gate_proj", "up_proj", "down_proj")}
+REBASED = ("pissa", "olora", "corda", "loftq")          # initialisations that leave the model without what the adapter begins with
 FILES = ("adapter_config.json", "adapter_model.safetensors")
 # a decoder's own layers: not those of a tower that a larger model has beside it, whose names end alike
 _NAME = re.compile(r"^(?:base_model\.)?(?:model\.|language_model\.)*layers\.(\d+)\.(self_attn|mlp)\.(\w+)\.lora_([AB])(?:\.default)?\.weight$")
@@ -79,6 +80,9 @@ def read_adapter(path: str | Path) -> Entries:
     for key in ("use_dora", "fan_in_fan_out", "lora_bias", "use_qalora", "trainable_token_indices", "alora_invocation_tokens", "layer_replication"):
         if cfg.get(key):
             raise AdapterError(f"{config}: {key} is not supported")
+    init = cfg.get("init_lora_weights")
+    if isinstance(init, str) and init.lower().startswith(REBASED):
+        raise AdapterError(f"{config}: adapters that begin as {init} take a part of the model's weights into themselves; convert them to plain ones first")
     alpha, root = cfg.get("lora_alpha", 8), bool(cfg.get("use_rslora"))
     alphas = cfg.get("alpha_pattern") or {}
     if not isinstance(alphas, dict) or any(re.fullmatch(r"[\w.]+", k) is None for k in alphas):

@@ -121,6 +121,14 @@ def test_adapter_kinds_without_a_place_are_refused(tmp_path, config):
         read_adapter(_write_adapter(tmp_path / "a", _entries(4, 1), config))
 
 
+@pytest.mark.parametrize("init", ["pissa", "pissa_niter_16", "olora", "CorDA", "loftq"])
+def test_adapters_of_a_changed_base_are_refused(tmp_path, init):
+    with pytest.raises(AdapterError, match="convert"):
+        read_adapter(_write_adapter(tmp_path / "a", _entries(4, 1), {"init_lora_weights": init}))
+    assert read_adapter(_write_adapter(tmp_path / "b", _entries(4, 1), {"init_lora_weights": True}))
+    assert read_adapter(_write_adapter(tmp_path / "c", _entries(4, 1), {"init_lora_weights": "gaussian"}))
+
+
 def test_broken_adapters_are_refused(tmp_path):
     with pytest.raises(AdapterError):
         read_adapter(tmp_path)
