@@ -88,7 +88,10 @@ def read_adapter(path: str | Path) -> Entries:
     if not isinstance(alphas, dict) or any(re.fullmatch(r"[\w.]+", k) is None for k in alphas):
         raise AdapterError(f"{config}: alpha_pattern takes module paths or ends of them, not expressions")
     found: dict[tuple[int, str], dict] = {}
-    f = SafetensorsFile(weights)
+    try:
+        f = SafetensorsFile(weights)
+    except (OSError, ValueError) as e:
+        raise AdapterError(f"{weights}: {e}")
     for name in f.tensors:
         m = _NAME.search(name)
         if m is None or m.group(3) not in PROJECTIONS[m.group(2)]:

@@ -163,6 +163,16 @@ def test_a_decoders_names_are_known_with_what_stands_before_them(tmp_path, prefi
     assert set(got) == set(_entries(4, 1))
 
 
+@pytest.mark.parametrize("data", [b"", b"1234567", b"\xff" * 64, (8).to_bytes(8, "little") + b"nonsense"])
+def test_files_that_hold_no_matrices_are_refused(tmp_path, data):
+    (tmp_path / "adapter_config.json").write_text("{}")
+    (tmp_path / "adapter_model.safetensors").write_bytes(data)
+    with pytest.raises(AdapterError, match="adapter_model"):
+        read_adapter(tmp_path)
+    with pytest.raises(SystemExit):
+        cli.main(["--model", "tiny-llama", "--cpu", "generate", "--tokens", "1", "--max-new-tokens", "1", "--adapter", str(tmp_path)])
+
+
 def test_a_matrix_named_twice_is_refused(tmp_path):
     path = tmp_path / "a"
     path.mkdir()
