@@ -73,6 +73,8 @@ class Backend:
                     images: list | None = None, sampling=None, adapter: str | None = None) -> tuple[Request, asyncio.Queue]:
         if self.state == "unavailable":
             raise Unavailable("engine is unavailable after an earlier failure")
+        if self.greedy_only and (adapter is not None or sampling is not None and sampling.temperature > 0):
+            raise ValueError("multi-token-prediction speculation serves greedy requests of the base model")
         with self._lock:
             if len(self._inflight) >= self.max_inflight:
                 raise Busy("busy: too many requests in flight")

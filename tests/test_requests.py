@@ -421,6 +421,19 @@ def test_speculation_serves_greedy_requests_only():
             Server(backend, ByteTokenizer(m.spec.vocab), "x", None, **kw)
 
 
+def test_speculation_takes_no_other_request():
+    backend = MtpBackend(Model.load("deepseek-v3-tiny", Settings(capacity=128, max_batch=2), device="cpu"), 1)
+
+    async def add(**kw):
+        return backend.add_request([1, 2, 3], 4, **kw)
+    for kw in ({"sampling": Sampling(0.5)}, {"adapter": "x"}):
+        with pytest.raises(ValueError, match="greedy"):
+            asyncio.run(add(**kw))
+    assert not backend._inflight
+    req, _ = asyncio.run(add(sampling=Sampling(0.0)))
+    assert req.prompt == [1, 2, 3]
+
+
 def test_the_command_line_draws_and_adapts(tmp_path, capsys):
     where = str(_write_adapter(tmp_path / "poet", _entries(8, 1)))
 
