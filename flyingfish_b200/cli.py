@@ -82,7 +82,8 @@ def _global_parser() -> argparse.ArgumentParser:
     s = sub.add_parser("serve")
     s.add_argument("--port", type=int, default=8080)
     s.add_argument("--mtp", type=int, default=None, choices=range(0, 5))
-    s.add_argument("--allow-sampling", action="store_true", help="accept temperature / top_p / top_k / min_p / seed (default: greedy requests only)")
+    s.add_argument("--allow-sampling", action="store_true", help="accept temperature / top_p / top_k / min_p / seed (default: greedy requests only); top_p is a share of the whole softmax, "
+                   "whatever top_k leaves of it; not with --mtp or --tp")
     s.add_argument("--adapter", metavar="NAME=DIR", action="append", default=[],
                    help="low-rank adapter that requests choose with \"model\": NAME (may be given several times)")
 

@@ -1,7 +1,8 @@
 """Sampling settings of a request and the random numbers its tokens are drawn with.
 
 The number for the token at index ``i`` of a sequence is a function of the request's seed and ``i`` alone (counter-based Philox4x32-10, Salmon et al. 2011),
-so a request gives the same tokens whatever it is batched with, and goes on with the same numbers after it was preempted and recomputed."""
+so a request draws with the same numbers whatever it is batched with, and goes on with them after it was preempted and recomputed. Its tokens are the same wherever its
+logits are: rows keep their bits beside others in products of up to 128 rows, while a step of more rows, or a prompt in other portions, may sum in another order."""
 from __future__ import annotations
 
 from dataclasses import dataclass

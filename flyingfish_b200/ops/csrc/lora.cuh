@@ -124,7 +124,7 @@ struct UnitPair {
 // Decode products: one tile of up to 128 rows, whose adapters are listed once per CTA in shared memory by the epilogue's 128 threads while the weights stream.
 // Units go step by step, so that t of a step is loaded once for all adapters (once for all tiles where there are no more steps than buffers); up to 64 / BW of
 // a step's units share a stage of the ring. The threads that load and multiply walk lists of bits: one thread alone takes hundreds of cycles
-// to find a unit among the adapters (64 rows with 64 adapters of rank 16, 6144 x 4096: 51 us with the search, 33 with the bits).
+// to find a unit among the adapters (64 rows with 64 adapters of rank 16, 6144 x 4096: 56 us with the search, 33.5 with the bits).
 //
 // Where a tile's K is divided among CTAs, a hash of the adapter and the step say whose a unit is: where a row's units go, and with it the order of its
 // sums, depends on nothing but its adapter.

@@ -4,7 +4,8 @@
 //   reaches P of the whole mass) and min-p (w_i >= min_p) leave, at least one;  drawn: lowest id whose sum of kept w up to it passes u times their sum.
 //
 // Ids are to be those of the formulas, so what decides is held in FP64: a row of 128 thousand flat tokens has borders 8e-6 of the mass apart, and
-// 32-bit sums move 128 thousand of them by 1e-7 each.
+// 32-bit sums move 128 thousand of them by 1e-7 each. Less than FP64 has are the weights (1.2e-12 of themselves, exp2_table) and, where a list is joined with
+// the masses in front of it, the list's (multiples of 2^-50 of the largest weight): a millionth of the distance of those borders.
 //
 // A cluster of C CTAs has a row: every CTA keeps its slice of the logits in shared memory, so that they come from memory once, and a warp a run of
 // consecutive ids of it. Values cross by stores into the peers' shared memory in front of a cluster barrier. Steps:

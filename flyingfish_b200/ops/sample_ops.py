@@ -23,8 +23,10 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
     smallest prefix whose mass reaches ``top_p`` of the whole mass of ``softmax(logits / temperature)`` (all from 1 on, one token at 0 or less); the tokens of
     at least ``min_p`` times the largest probability (all at 0 or less, those of the largest from 1 on). Drawn is the lowest id whose sum of kept masses up to it
     passes ``uniforms`` times their sum. ``temperature`` 0 or less: the lowest id of the largest logit, probability 1. NaN logits count as -inf, which is
-    never drawn, and +inf shares everything among its equals; a row of -inf gives id 0 with probability 0. Masses are those of 64-bit arithmetic; one
-    below 2^-1000 of the largest counts as none. On a GPU a row lies in the shared memory of 8 multiprocessors: 380 thousand FP32 tokens or 760 thousand BF16
+    never drawn, and +inf shares everything among its equals; a row of -inf gives id 0 with probability 0. On a GPU masses are sums in 64 bits of weights that
+    are held to 1.2e-12 of themselves, so the ids are the definition's unless a border lies within a few 1e-12 of the mass from where a token begins or ends; a
+    weight below 2^-1000 of the largest counts as none, everywhere. The settings do not follow one another: ``top_p`` is a share of the mass before ``top_k`` and ``min_p``
+    cut anything off. On a GPU a row lies in the shared memory of 8 multiprocessors: 380 thousand FP32 tokens or 760 thousand BF16
     ones, and there are 65535 rows at most."""
     rows, ld = _rows2d(logits)
     at = logits.get_device()

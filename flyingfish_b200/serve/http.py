@@ -12,8 +12,10 @@ in-flight limit). A client that disconnects aborts its request.
 
 ``allow_sampling=True`` additionally accepts temperature / top_p / top_k / min_p / seed (an extension; off by
 default so the validation matrix matches the reference): a temperature above 0 has the request's tokens drawn, each by settings and random numbers of
-its own request, so that a seed gives the same tokens whatever else the server runs. ``model`` may also name one of the adapters
-that the server was started with.
+its own request, so that a seed draws with the same numbers whatever else the server runs (``engine/sampling.py``). ``top_p`` is a share of the whole
+softmax: it does not renormalise behind ``top_k``, as servers that apply one filter after another do. ``seed`` is a whole number from 0 below 2^64. What no request can
+have -- ``n`` other than 1, ``logit_bias``, penalties, ``stop`` -- is answered 400 with and without the option, and the option itself starts only where tokens can be drawn: not beside
+multi-token-prediction speculation, not with tensor parallelism. ``model`` may also name one of the adapters that the server was started with.
 """
 from __future__ import annotations
 
