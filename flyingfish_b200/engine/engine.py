@@ -153,7 +153,7 @@ class Engine:
             raise ValueError("empty prompt")
         if len(prompt) + 1 > self.settings.capacity:
             raise ValueError(f"prompt of {len(prompt)} tokens exceeds the KV capacity {self.settings.capacity}")
-        if sampling is not None and self.model.w.tp.size > 1:
+        if sampling is not None and sampling.temperature > 0 and self.model.w.tp.size > 1:
             raise ValueError("sampling is not available with tensor parallelism")
         if adapter is not None and (self.adapters is None or adapter not in self.adapters.index):
             raise ValueError(f"no adapter {adapter!r} is loaded")

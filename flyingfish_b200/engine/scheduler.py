@@ -79,7 +79,7 @@ class Scheduler:
             loaded = getattr(self.engine, "adapters", None)
             if loaded is None or req.adapter not in loaded.index:
                 raise ValueError(f"no adapter {req.adapter!r} is loaded")
-        if req.sampling is not None and getattr(getattr(getattr(self.engine, "model", None), "w", None), "tp", None) is not None \
+        if req.sampling is not None and req.sampling.temperature > 0 and getattr(getattr(getattr(self.engine, "model", None), "w", None), "tp", None) is not None \
                 and self.engine.model.w.tp.size > 1:
             raise ValueError("sampling is not available with tensor parallelism")
         self.waiting.append(req)

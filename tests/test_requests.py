@@ -354,6 +354,19 @@ def test_what_compares_with_greedy_tokens_refuses_such_sequences():
 # ------------------------------------------------------------------------------------------
 # server and command line
 # ------------------------------------------------------------------------------------------
+def test_greedy_settings_ask_for_nothing():
+    """Temperature 0 is the plain path, with tensor parallelism too."""
+    eng = _load().engine
+    tp = eng.model.w.tp
+    try:
+        eng.model.w.tp = TPInfo(0, 2)
+        s = eng.add_sequence([1, 2], sampling=Sampling(0))
+        assert s.draws is None and not s.special
+        assert Scheduler(eng).submit(Request(prompt=[1], max_tokens=1, sampling=Sampling(0.0))).sampling.temperature == 0
+    finally:
+        eng.model.w.tp = tp
+
+
 class Numbers(ByteTokenizer):
     """Ids as text, so that answers show the tokens."""
 
