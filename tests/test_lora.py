@@ -376,3 +376,20 @@ def test_scales_of_parts_cost_no_rounding(cuda, m, adapters):
     step = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=1e-30))) - 7)
     assert ((got - want).abs() <= step / 2 * (1 + 2.0 ** -12)).all()
     ops.check_status(cuda)
+
+
+@pytest.mark.gpu
+def test_prompts_on_two_streams_at_once(cuda):
+    """Calls of more than 128 rows share nothing: each has its own t and its own word behind it."""
+    cases = [_case(m, 1024, 1536, 32, 5, seed=m, device=cuda) for m in (300, 200, 700)]
+    want = [lora_ops.linear_lora(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[] for _ in cases]
+    for _ in range(20):
+        for s, c, out in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                out.append(lora_ops.linear_lora(*c))
+    torch.cuda.synchronize()
+    for out, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in out)
+    ops.check_status(cuda)

@@ -384,3 +384,18 @@ def test_logits_far_apart(cuda, vocab, dtype):
     l, u, t, settings = _far_apart(24, vocab, dtype, cuda)
     for args in settings:
         _check(l, u, t, *args)
+
+
+@pytest.mark.gpu
+def test_batches_on_two_streams_at_once(cuda):
+    cases = [(_logits(kind, rows, 32003, BF16, 1, cuda), *_settings(rows, rows, cuda)) for kind, rows in (("normal", 40), ("peaked", 100))]
+    want = [sample_ops.sample_tokens(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[] for _ in cases]
+    for _ in range(20):
+        for s, c, out in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                out.append(sample_ops.sample_tokens(*c))
+    torch.cuda.synchronize()
+    for out, w in zip(got, want):
+        assert all(torch.equal(o[0], w[0]) and torch.equal(o[1], w[1]) for o in out)
