@@ -1,0 +1,31 @@
+// Pages of a key / value cache that is held in 4 bits. A page is 64 tokens of one head of D = 64 or 128 elements; groups of 32
+// neighbouring elements of a token share two BF16 numbers (scale, lo), an element stands for code * scale + lo:
+//   lo = the group's least element, scale = RN_bf16((greatest - lo) / 15), code = RN_even((x - lo) / scale) in 0 .. 15
+// (real numbers, one rounding each; scale and codes are 0 where the scale would be below the least normal BF16 number).
+// 5 bits an element, 160 bytes a token and head of 128 for keys and values together where BF16 has 512.
+//
+// Layout of a page: 64 rows of D / 2 bytes of codes, then [64 tokens][D / 32] pairs (scale, lo). Element d = 32 j + 8 u + e:
+//   keys    nibble e / 2 + 4 (e & 1) of 32-bit word u D / 32 + j of the token's row. Lane (g, t) of a warp reads words t D / 32 .. of the rows of two
+//           tokens as its A fragments of mma.sync m16n8k16 (tokens x elements); masking a word at nibble i and i + 4 gives elements
+//           8 t + 2 i and 8 t + 2 i + 1 of a group, in that order, as the queries are in memory.
+//   values  nibble e / 2 of 16-bit unit j of chunk 2 u + (e & 1) (D / 16 bytes). Lane (g, t) reads chunk g of tokens 4 t .. 4 t + 3 as its fragments of
+//           (elements x tokens). Rows and chunks are moved so that no two lanes of such a read meet a bank: token k lies at row
+//           k ^ (k >> 3 & 1) with chunk c at c ^ 4 (k >> 2 & 1) for D = 128, at row k ^ (k >> 2 & 3) for D = 64.
+#pragma once
+#include "ptx.cuh"
+
+namespace ff {
+
+constexpr int KV4_PAGE = 64;
+__host__ __device__ constexpr int kv4_code_bytes(int dim) { return KV4_PAGE * dim / 2; }
+__host__ __device__ constexpr int kv4_page_bytes(int dim) { return KV4_PAGE * (dim / 2 + dim / 8); }
+
+// byte of 16-bit unit j of chunk c of token k's values
+template <int D>
+__device__ __forceinline__ int kv4_value_at(int k, int c, int j) {
+  const int row = D == 128 ? k ^ ((k >> 3) & 1) : k ^ ((k >> 2) & 3);
+  if (D == 128) c ^= ((k >> 2) & 1) << 2;
+  return row * (D / 2) + c * (D / 16) + 2 * j;
+}
+
+}  // namespace ff

@@ -1,0 +1,396 @@
+"""The 4-bit key / value cache: pages written and read back bit for bit, attention over them against the definition in 64 bits, copied pages, and what the
+operators refuse.
+
+Tolerances: a rounding to BF16 is off by 2^-8 of the value at most, and "2^-8" below is that. Where the bounds leave FP32 arithmetic
+aside they add 2^-14 of the sum of the terms' magnitudes: a few hundred roundings of 2^-24 and the exponential's."""
+import math
+
+import pytest
+import torch
+
+from flyingfish_b200 import ops
+from flyingfish_b200.ops import KernelError, kv4_ops, lib
+from flyingfish_b200.ops.kv4_ops import PAGE
+
+BF16 = torch.bfloat16
+E = 2.0 ** -8
+
+
+# ------------------------------------------------------------------------------------------
+# helpers
+# ------------------------------------------------------------------------------------------
+def _rows(rows, width, seed, pad=0):
+    gen = torch.Generator().manual_seed(seed)
+    gain = torch.exp(torch.randn(1, width, generator=gen))
+    x = torch.randn(rows, width, generator=gen) * gain + torch.randn(1, width, generator=gen)
+    wide = torch.full((rows, width + pad), 7.0, dtype=BF16)
+    wide[:, :width] = x.to(BF16)
+    return wide[:, :width]
+
+
+def _turn(rows, n, seed):
+    angle = torch.rand(rows, n, generator=torch.Generator().manual_seed(seed)) * 6.28
+    return torch.stack([torch.cos(angle), torch.sin(angle)], dim=-1).to(BF16).float().contiguous()
+
+
+def _cache(lens, hkv, dim, seed, device, width=None, fill=0xFF):
+    """Pages of sequences of given lengths, written row by row behind pages that hold no numbers (every byte ``fill``: a NaN in 16 bits), with the pages in any
+    order: (kpages, vpages, table, keys, values in 64 bits per sequence)."""
+    gen = torch.Generator().manual_seed(seed)
+    need = [-(-c // PAGE) for c in lens]
+    blocks = sum(need) + 2
+    order = torch.randperm(blocks, generator=gen)
+    table = torch.zeros(len(lens), width or max(max(need), 1), dtype=torch.int32)
+    pages = [torch.full((blocks, hkv, kv4_ops.page_bytes(dim)), fill, dtype=torch.uint8) for _ in range(2)]
+    at, slots = 0, []
+    for i, (n, c) in enumerate(zip(need, lens)):
+        table[i, :n] = order[at: at + n]
+        at += n
+        p = torch.arange(c)
+        slots.append(table[i].long()[p // PAGE] * PAGE + p % PAGE if c else torch.zeros(0, dtype=torch.long))
+    slots = torch.cat(slots)
+    kv = _rows(len(slots), 2 * hkv * dim, seed + 1)
+    for part, p, keys in ((kv[:, : hkv * dim], pages[0], True), (kv[:, hkv * dim:], pages[1], False)):
+        byte, shift = kv4_ops._places(dim, keys)
+        code, scale, lo = kv4_ops.quantise(part.reshape(-1, hkv, dim))
+        blk, k = slots // PAGE, slots % PAGE
+        nib = torch.zeros(blocks, hkv, PAGE * dim // 2, 2, dtype=torch.uint8)
+        flat = byte[k] * 2 + shift[k] // 4                                     # [rows, dim]
+        nib.flatten(2).index_put_((blk[:, None, None], torch.arange(hkv)[None, :, None], flat[:, None, :].expand(-1, hkv, -1)), code)
+        p[:, :, : PAGE * dim // 2] = nib[..., 0] | nib[..., 1] << 4
+        st = p[:, :, PAGE * dim // 2:].clone().view(BF16).view(blocks, hkv, PAGE, dim // 32, 2)
+        st[blk, :, k] = torch.stack([scale, lo], dim=-1)
+        p[:, :, PAGE * dim // 2:] = st.flatten(2).view(torch.uint8)
+    return pages[0].to(device), pages[1].to(device), table.to(device)
+
+
+def _definition(q, kpages, vpages, table, spans, hq, hkv, dim, scale, rounded=False):
+    """Per row and head: the attention in 64 bits, the sum of p |v| and of p (v - lo). ``rounded``: of keys and values that are rounded to BF16."""
+    g = hq // hkv
+    res, mag, off = (torch.zeros(q.shape[0], hq, dim, dtype=torch.float64) for _ in range(3))
+    for b, (at, n, ctx) in enumerate(spans):
+        if ctx <= 0 or n == 0:
+            continue
+        pages = table[b, : -(-ctx // PAGE)].long().cpu()
+        k, v = (kv4_ops.page_values(p.cpu()[pages], dim, keys).double().transpose(0, 1).reshape(hkv, -1, dim)[:, :ctx] for p, keys in ((kpages, True), (vpages, False)))
+        lo = v.unflatten(-1, (-1, 32)).amin(-1, keepdim=True).expand(-1, -1, -1, 32).flatten(-2)
+        if rounded:
+            k, v = k.to(BF16).double(), v.to(BF16).double()
+        x = q[at: at + n, : hq * dim].double().cpu().view(n, hkv, g, dim)
+        score = torch.einsum("nhgd,hkd->nhgk", x, k) * scale
+        score.masked_fill_((torch.arange(ctx)[None, :] > torch.arange(ctx - n, ctx)[:, None])[:, None, None], -math.inf)
+        p = torch.softmax(score, dim=-1)
+        res[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v).reshape(n, hq, dim)
+        mag[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v.abs()).reshape(n, hq, dim)
+        off[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v - lo).reshape(n, hq, dim)
+    return [t.view(q.shape[0], hq * dim) for t in (res, mag, off)]
+
+
+def _status_of(fn):
+    ops.read_status()
+    fn()
+    torch.cuda.synchronize()
+    return ops.read_status()[0]
+
+
+# ------------------------------------------------------------------------------------------
+# format
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("keys", [True, False])
+def test_every_code_has_a_place_of_its_own(dim, keys):
+    byte, shift = kv4_ops._places(dim, keys)
+    at = (byte * 2 + shift // 4).flatten()
+    assert at.unique().numel() == PAGE * dim and int(byte.max()) == PAGE * dim // 2 - 1
+    assert kv4_ops.page_bytes(dim) == PAGE * dim // 2 + PAGE * dim // 32 * 4
+
+
+def test_quantised_elements_are_off_by_half_a_step():
+    x = _rows(50, 128, 3)
+    code, scale, lo = kv4_ops.quantise(x)
+    value = code.double() * scale.double().repeat_interleave(32, -1) + lo.double().repeat_interleave(32, -1)
+    # half a step; the rounded scale moves the greatest element by 15 x 2^-8 of a step
+    assert bool(((value - x.double()).abs() <= scale.double().repeat_interleave(32, -1) * (0.5 + 15 * E)).all())
+    assert int(code.max()) == 15 and int(code.min()) == 0
+    same = kv4_ops.quantise(torch.full((1, 64), 3.25, dtype=BF16))
+    assert not same[0].any() and not same[1].any() and bool((same[2] == 3.25).all())
+
+
+@pytest.mark.parametrize("dim,hq,hkv,rows", [(64, 4, 2, 70), (128, 3, 1, 5)])
+def test_written_rows_are_read_back_cpu(dim, hq, hkv, rows):
+    qkv, slots = _rows(rows, (hq + 2 * hkv) * dim, 5), torch.randperm(3 * PAGE)[:rows].to(torch.int32)
+    slots[1] = -1
+    kp, vp = (kv4_ops.new_pages(3, hkv, dim, "cpu") for _ in range(2))
+    q = kv4_ops.write_kv4(qkv, slots, kp, vp, hq, hkv, dim)
+    assert q.data_ptr() == qkv.data_ptr() and torch.equal(q, qkv[:, : hq * dim])
+    k, v = kv4_ops.read_kv4(kp, vp, slots, dim)
+    x = qkv.view(rows, -1, dim)
+    for got, want in ((k, x[:, hq: hq + hkv]), (v, x[:, hq + hkv:])):
+        code, scale, lo = kv4_ops.quantise(want)
+        val = (code.double() * scale.double().repeat_interleave(32, -1) + lo.double().repeat_interleave(32, -1))
+        val[1] = 0
+        assert bool(((got.double() - val).abs() <= val.abs() * E).all()) and not got[1].any()
+
+
+def test_what_the_operators_refuse():
+    hq, hkv, dim = 4, 2, 64
+    kp, vp = (kv4_ops.new_pages(2, hkv, dim, "cpu") for _ in range(2))
+    qkv, slots = _rows(3, (hq + 2 * hkv) * dim, 1), torch.arange(3, dtype=torch.int32)
+    write = lambda **kw: kv4_ops.write_kv4(**{**dict(qkv=qkv, slots=slots, kpages=kp, vpages=vp, hq=hq, hkv=hkv, dim=dim), **kw})
+    bad = qkv.clone(); bad[1, hq * dim] = float("nan")
+    huge = qkv.clone(); huge[1, -1] = 2.0 ** 121
+    for kw in (dict(dim=96), dict(qkv=qkv.float()), dict(slots=slots.long()), dict(slots=slots[:2]), dict(kpages=kp[:, :1]), dict(kpages=kp.transpose(0, 1)),
+               dict(vpages=vp[:1]), dict(hq=5), dict(cos_sin=_turn(3, 33, 1)), dict(cos_sin=_turn(2, 32, 1)), dict(cos_sin=_turn(3, 32, 1).double()),
+               dict(q_norm=torch.ones(dim, dtype=BF16)), dict(q_norm=torch.ones(dim), k_norm=torch.ones(dim)), dict(qkv=bad), dict(qkv=huge),
+               dict(slots=slots + 2 * PAGE - 2)):
+        with pytest.raises(KernelError):
+            write(**kw)
+    with pytest.raises(KernelError):
+        kv4_ops.read_kv4(kp, vp, slots + 2 * PAGE, dim)
+    q, table, ctx = qkv[:, : hq * dim], torch.zeros(3, 1, dtype=torch.int32), torch.tensor([3, 1, 0], dtype=torch.int32)
+    decode = lambda **kw: kv4_ops.attn_decode_kv4(**{**dict(q=q, kpages=kp, vpages=vp, block_table=table, ctx_lens=ctx, hq=hq, hkv=hkv, dim=dim, scale=0.1), **kw})
+    decode()
+    for kw in (dict(hq=3), dict(nq=2), dict(scale=0.0), dict(block_table=table.long()), dict(block_table=table - 1), dict(block_table=table + 2), dict(ctx_lens=ctx + 64),
+               dict(ctx_lens=ctx.long()), dict(q=q.float()), dict(out=torch.empty(3, hq * dim)), dict(dim=128)):
+        with pytest.raises(KernelError):
+            decode(**kw)
+    one = torch.tensor([0], dtype=torch.int32)
+    with pytest.raises(KernelError):
+        kv4_ops.attn_prefill_kv4(q, kp, vp, table, one, one, ctx, 3, hq, hkv, dim, 0.1)
+    t = torch.zeros(4, 16, dtype=torch.uint8)
+    for src, dst in (([0], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0], [4]), ([-1], [2]), ([0, 1], [2])):
+        with pytest.raises(KernelError):
+            kv4_ops.copy_pages([t], src, dst)
+
+
+def test_attention_of_empty_and_short_sequences_cpu():
+    hq, hkv, dim, lens = 4, 2, 64, [0, 1, 64, 65, 130]
+    kp, vp, table = _cache(lens, hkv, dim, 3, "cpu")
+    q = _rows(5, hq * dim, 9)
+    got = kv4_ops.attn_decode_kv4(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32), hq, hkv, dim, 0.125)
+    want, mag, _ = _definition(q, kp, vp, table, [(i, 1, c) for i, c in enumerate(lens)], hq, hkv, dim, 0.125)
+    assert not got[0].any() and bool(((got.double() - want).abs() <= want.abs() * E + mag * 2.0 ** -14).all())
+
+
+def test_copied_pages_cpu():
+    a, b = torch.randn(5, 2, 8), torch.randint(256, (5, 16), dtype=torch.uint8)
+    wa, wb = a.clone(), b.clone()
+    kv4_ops.copy_pages([a, b], [0, 3, 0], [1, 2, 4])
+    wa[1], wa[2], wa[4] = wa[0], wa[3], wa[0]
+    wb[1], wb[2], wb[4] = wb[0], wb[3], wb[0]
+    assert torch.equal(a, wa) and torch.equal(b, wb)
+
+
+# ------------------------------------------------------------------------------------------
+# kernels
+# ------------------------------------------------------------------------------------------
+WRITES = [(64, 4, 2, 1, 0, 32), (128, 32, 8, 61, 8, 64), (128, 7, 1, 130, 24, 20), (64, 28, 4, 200, 0, 32), (128, 1, 1, 3, 0, None), (64, 3, 3, 77, 8, 7)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,hq,hkv,rows,pad,turned", WRITES)
+def test_written_pages_are_the_oracles(dim, hq, hkv, rows, pad, turned):
+    qkv = _rows(rows, (hq + 2 * hkv) * dim, rows, pad)
+    # groups of one value, of a span below the least normal number, of a great offset with a small span, and of far apart magnitudes
+    head = qkv[:, hq * dim:]
+    head[0, :32] = 1.5
+    head[0, 32:64] = torch.tensor([1e-38, 2e-38] * 16).to(BF16)
+    head[-1, :32] = (100 + torch.arange(32) * 0.5).to(BF16)
+    head[-1, 32:64] = torch.logspace(-20, 20, 32).to(BF16)
+    blocks = -(-rows // PAGE) + 1
+    slots = torch.randperm(blocks * PAGE, generator=torch.Generator().manual_seed(1))[:rows].to(torch.int32)
+    if rows > 2:
+        slots[1] = -1
+    turn = None if turned is None else _turn(rows, turned, 2)
+    want_pages = [torch.full((blocks, hkv, kv4_ops.page_bytes(dim)), 0xA5, dtype=torch.uint8) for _ in range(2)]
+    pages = [p.cuda() for p in want_pages]
+    want = kv4_ops.write_kv4(qkv, slots, *want_pages, hq, hkv, dim, turn)
+    dev = torch.full((rows, qkv.shape[1] + pad), 7.0, dtype=BF16, device="cuda")
+    dev[:, : qkv.shape[1]] = qkv
+    got = kv4_ops.write_kv4(dev[:, : qkv.shape[1]], slots.cuda(), *pages, hq, hkv, dim, None if turn is None else turn.cuda())
+    assert torch.equal(got.cpu(), want)
+    for p, w in zip(pages, want_pages):
+        assert torch.equal(p.cpu(), w)
+    k, v = kv4_ops.read_kv4(*pages, slots.cuda(), dim)
+    wk, wv = kv4_ops.read_kv4(*want_pages, slots, dim)
+    assert torch.equal(k.cpu(), wk) and torch.equal(v.cpu(), wv)
+    assert ops.read_status()[0] == 0
+
+
+@pytest.mark.gpu
+def test_head_norms_before_the_turn():
+    dim, hq, hkv, rows = 128, 4, 2, 33
+    qkv, turn, slots = _rows(rows, (hq + 2 * hkv) * dim, 4).cuda(), _turn(rows, 64, 5).cuda(), torch.arange(rows, dtype=torch.int32).cuda()
+    w = [torch.rand(dim, generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i in (6, 7)]
+    pages = [kv4_ops.new_pages(1, hkv, dim, "cuda") for _ in range(2)]
+    got = kv4_ops.write_kv4(qkv, slots, *pages, hq, hkv, dim, turn, *w, 1e-6)
+    # the BF16 cache's kernel, normed and turned the same way
+    cache = [torch.zeros(1, hkv, PAGE, dim, dtype=BF16, device="cuda") for _ in range(2)]
+    packed = qkv.clone()
+    cpu = [t.cpu() for t in (qkv, slots, *w)]
+    x = cpu[0].view(rows, -1, dim).double()
+    rms = lambda t, g: t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-6) * g.double()
+    normed = torch.cat([rms(x[:, :hq], cpu[2]), rms(x[:, hq: hq + hkv], cpu[3])], dim=1)
+    c, s = (turn.cpu().double()[:, None, :, i] for i in (0, 1))
+    a, b = normed[..., :64], normed[..., 64:]
+    exact = torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+    # four roundings to BF16: the norm's two inputs', their products', the sum's
+    tol = 2 * E * (torch.cat([a.abs() + b.abs()] * 2, dim=-1)) + E * exact.abs() + 2.0 ** -14
+    assert bool(((got.cpu().double().view(rows, hq, dim) - exact[:, :hq]).abs() <= tol[:, :hq]).all())
+    k, v = kv4_ops.read_kv4(*pages, slots, dim)
+    span = exact[:, hq:].unflatten(-1, (-1, 32))
+    step = ((span.amax(-1) - span.amin(-1)) / 15).repeat_interleave(32, -1)
+    wide = tol[:, hq:].unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1)       # the group's ends move too
+    assert bool(((k.cpu().double() - exact[:, hq:]).abs() <= step * 0.55 + 4 * wide).all())
+    del cache, packed
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf"), 2.0 ** 121])
+def test_numbers_that_are_not_finite_raise_the_status(what):
+    dim, hq, hkv = 128, 2, 2
+    qkv = _rows(3, (hq + 2 * hkv) * dim, 4)
+    qkv[1, hq * dim + 5] = what
+    pages = [kv4_ops.new_pages(1, hkv, dim, "cuda") for _ in range(2)]
+    slots = torch.arange(3, dtype=torch.int32).cuda()
+    assert _status_of(lambda: kv4_ops.write_kv4(qkv.cuda(), slots, *pages, hq, hkv, dim)) == 4
+    k, _ = kv4_ops.read_kv4(*pages, slots, dim)
+    assert not k[1, 0, :32].any() and bool(k[1, 0, 32:].any()) and bool(torch.isfinite(k.float()).all())
+    # padding rows hold anything
+    qkv[1] = what
+    assert _status_of(lambda: kv4_ops.write_kv4(qkv.cuda(), torch.tensor([0, -1, 2], dtype=torch.int32).cuda(), *pages, hq, hkv, dim)) == 0
+
+
+@pytest.mark.gpu
+def test_slots_and_pages_outside_the_cache_raise_the_status():
+    dim, hq, hkv = 64, 2, 2
+    pages = [kv4_ops.new_pages(2, hkv, dim, "cuda") for _ in range(2)]
+    qkv, i32 = _rows(1, (hq + 2 * hkv) * dim, 4).cuda(), lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    assert _status_of(lambda: kv4_ops.write_kv4(qkv, i32(128), *pages, hq, hkv, dim)) == 3
+    assert not pages[0].any() and not pages[1].any()
+    assert _status_of(lambda: kv4_ops.read_kv4(*pages, i32(128), dim)) == 3
+    for table, ctx in ((2, 5), (-1, 5), (0, 65)):
+        assert _status_of(lambda: kv4_ops.attn_decode_kv4(qkv, *pages, i32(table).view(1, 1), i32(ctx), hq, hkv, dim, 0.1)) == 3
+        assert _status_of(lambda: kv4_ops.attn_prefill_kv4(qkv, *pages, i32(table).view(1, 1), i32(0), i32(1), i32(ctx), 1, hq, hkv, dim, 0.1)) == 3
+
+
+def _close(got, want, mag, off, rounded=False):
+    """Few rows: p scale is rounded (2^-8 of p (v - lo)) and the result. Prompts in tiles (``rounded``, against keys and values that are rounded to BF16):
+    p is rounded (2^-8 of p |v|) and the result."""
+    tol = want.abs() * E + (mag if rounded else off) * E + mag * 2.0 ** -14
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"{float((err / tol.clamp_min(1e-30)).max())} of the tolerance"
+
+
+DECODES = [(128, 32, 8, 1, [900]), (128, 32, 8, 1, [0, 1, 63, 64, 65, 128, 777]), (64, 28, 4, 1, [5, 0, 300, 1000]), (128, 8, 8, 1, [129, 40]), (128, 7, 1, 3, [3, 200, 0, 517]),
+           (128, 64, 4, 5, [700, 5, 66]), (64, 16, 1, 8, [8, 2000]), (64, 2, 2, 2, [2, 64, 66]), (128, 64, 8, 1, [20000]), (128, 5, 1, 4, [4100, 70])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,hq,hkv,nq,lens", DECODES)
+def test_decoded_rows_over_4_bit_pages(dim, hq, hkv, nq, lens):
+    kp, vp, table = _cache(lens, hkv, dim, len(lens) + nq, "cuda", width=-(-max(lens) // PAGE) + 3)
+    q = _rows(len(lens) * nq, (hq + 2 * hkv) * dim, 11).cuda()
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    scale = 1 / math.sqrt(dim)
+    got = kv4_ops.attn_decode_kv4(q, kp, vp, table, ctx, hq, hkv, dim, scale, nq=nq)
+    again = kv4_ops.attn_decode_kv4(q, kp, vp, table, ctx, hq, hkv, dim, scale, nq=nq)
+    assert torch.equal(got, again) and ops.read_status()[0] == 0
+    want, mag, off = _definition(q, kp, vp, table, [(i * nq, nq, c) for i, c in enumerate(lens)], hq, hkv, dim, scale)
+    _close(got, want, mag, off)
+    for i, c in enumerate(lens):
+        if c == 0:
+            assert not got[i * nq: (i + 1) * nq].any()
+
+
+PROMPTS = [(128, 32, 8, [(37, 0)]), (128, 8, 2, [(1, 0), (64, 0), (65, 3), (0, 0), (130, 300)]), (64, 28, 4, [(200, 0), (3, 1000)]), (128, 4, 4, [(129, 127)]), (64, 8, 1, [(257, 64), (1, 63)]),
+           (128, 16, 2, [(700, 0)])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,hq,hkv,spans", PROMPTS)
+def test_prompts_over_4_bit_pages(dim, hq, hkv, spans):
+    lens = [n + past for n, past in spans]
+    kp, vp, table = _cache(lens, hkv, dim, 3 + len(spans), "cuda")
+    rows = sum(n for n, _ in spans) + 5                                     # two rows in front and three behind belong to nobody
+    q = _rows(rows, (hq + 2 * hkv) * dim, 12).cuda()
+    starts, at = [], 2
+    for n, _ in spans:
+        starts.append(at)
+        at += n
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    out = torch.full((rows, hq * dim + 8), 3.0, dtype=BF16, device="cuda")[:, : hq * dim]
+    scale = 1 / math.sqrt(dim)
+    got = kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(starts), i32([n for n, _ in spans]), i32(lens), max(n for n, _ in spans), hq, hkv, dim, scale, out=out)
+    assert got.data_ptr() == out.data_ptr() and bool((out[:2] == 3).all()) and bool((out[at:] == 3).all()) and ops.read_status()[0] == 0
+    tiles = kv4_ops.prompt_in_tiles(max(n for n, _ in spans), hq, hkv)
+    want = _definition(q, kp, vp, table, [(s, n, c) for s, (n, _), c in zip(starts, spans, lens)], hq, hkv, dim, scale, rounded=tiles)
+    _close(got[2: at], *(t[2: at] for t in want), rounded=tiles)
+
+
+@pytest.mark.gpu
+def test_copied_pages_of_many_tensors():
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    made = lambda i: torch.randint(256, (700, 16 * (1 + i % 5)), generator=gen, device="cuda", dtype=torch.uint8) if i % 2 else torch.randn(700, 3, 8, generator=gen, device="cuda").to(BF16)
+    tensors = [made(i) for i in range(165)] + [kv4_ops.new_pages(700, 2, 128, "cuda").random_(0, 256, generator=gen)]
+    ids = torch.randperm(700, generator=torch.Generator().manual_seed(1)).tolist()
+    src, dst = ids[:300], ids[300: 600]
+    src[5] = src[4]                                                         # one page to two places
+    want = [t.clone() for t in tensors]
+    for t in want:
+        t[torch.tensor(dst).cuda()] = t[torch.tensor(src).cuda()]
+    kv4_ops.copy_pages(tensors, src, dst)
+    assert all(torch.equal(a, b) for a, b in zip(tensors, want))
+
+
+@pytest.mark.gpu
+def test_a_step_on_another_stream_and_in_graphs():
+    """Write, attend and copy: on a stream of their own, and as two captured graphs that are replayed at the same time over new rows."""
+    dim, hq, hkv, lens = 128, 8, 2, [130, 700, 64]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+
+    def made(seed):
+        kp, vp, table = _cache(lens, hkv, dim, seed, "cuda")
+        slot = [int(table[i, (c - 1) // PAGE]) * PAGE + (c - 1) % PAGE for i, c in enumerate(lens)]
+        nobodys = sorted(set(range(kp.shape[0])) - {int(table[i, p]) for i, c in enumerate(lens) for p in range(-(-c // PAGE))})
+        return kp, vp, table, _rows(3, (hq + 2 * hkv) * dim, seed).cuda(), i32(slot), _turn(3, 64, seed).cuda(), nobodys
+
+    def step(kp, vp, table, qkv, slots, turn, nobodys):
+        q = kv4_ops.write_kv4(qkv, slots, kp, vp, hq, hkv, dim, turn)
+        a = kv4_ops.attn_decode_kv4(q, kp, vp, table, ctx, hq, hkv, dim, 0.09)
+        kv4_ops.copy_pages([kp, vp], nobodys[:1], nobodys[1:])
+        return a
+
+    fresh = lambda st: [v.clone() if torch.is_tensor(v) else v for v in st]
+    ctx = i32(lens)
+    states = [made(s) for s in (1, 2)]
+    want = [step(*fresh(st)) for st in states]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(*fresh(states[0]))
+    side.synchronize()
+    assert torch.equal(got, want[0])
+    graphs, outs, bufs = [], [], []
+    for st in states:
+        buf = fresh(st)
+        step(*fresh(st))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(*buf)
+        graphs.append(g); outs.append(out); bufs.append(buf)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    # other rows and lengths in the captured buffers
+    bufs[0][3].copy_(bufs[1][3])
+    want = step(*fresh(bufs[0]))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and ops.read_status()[0] == 0
