@@ -1,0 +1,359 @@
+// Prompts over the 4-bit key / value cache on the 5th-generation tensor cores (layout and format: kv4.cuh).
+//
+// The rows of a sequence times the query heads of one kv head are flattened (row c: query c / G, head c % G of the group), and a CTA has two tiles of 128 of
+// them over one kv head: both read the same keys and values, so a page is turned into BF16 once for 256 rows. Per page j of 64 tokens:
+//   four warps    load codes and (scale, lo) a page ahead into registers and write keys and values code * scale + lo, rounded to BF16 once, as
+//                 128-byte-swizzled tiles (rounding keys and values is this kernel's choice: the tensor core's operands are BF16)
+//   one thread    S_i(j + 1) = Q_i K^T for both tiles, then O_i += P_i V; S, P and O live in tensor memory (P over the S that it came from)
+//   two x 4 warps soft-max of a tile, a thread per row: running maximum and sum in FP32 in the base-2 domain; O is rescaled only when the maximum has moved
+//                 by more than 2^8 (the stale one stays exact: P and the sum share it)
+// S(j + 1) of a tile waits for its P V (j - 1), whose P it overwrites; the other tile's products run meanwhile.
+// Every wait is bounded; a time-out records FF_ERR_TIMEOUT, and all roles leave through the abort flag.
+#include "kv4.cuh"
+#include "host_util.h"
+
+namespace ff {
+
+constexpr int KVT_M = 128, KVT_N = KV4_PAGE, KVT_STAGES = 3;
+constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 1;      // warps 0-7 soft-max, 8-11 tiles, 12 products
+constexpr float KVT_MOVED = 8.0f;                                                    // log2 units
+template <int D> constexpr int kvt_smem() { return 2 * KVT_M * D * 2 + 2 * KVT_STAGES * KVT_N * D * 2 + 1024; }
+
+struct alignas(8) KvtBars {
+  uint64_t q_full[2], k_full[KVT_STAGES], k_empty[KVT_STAGES], v_full[KVT_STAGES], v_empty[KVT_STAGES], s_full[2][2], p_full[2][2], pv_done[2][2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __forceinline__ float kvt_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// nibbles at bits s and s + 16 times scale plus lo, one rounding (128 + n is a BF16 number, the difference is exact)
+__device__ __forceinline__ uint32_t kvt_value(uint32_t w, int s, uint32_t scale2, uint32_t lo2) {
+  uint32_t n = ((w >> s) & 0x000f000fu) | 0x43004300u, r;
+  asm("{\n\t.reg .b32 t;\n\tadd.rn.bf16x2 t, %1, %2;\n\tfma.rn.bf16x2 %0, t, %3, %4;\n\t}" : "=r"(r) : "r"(n), "r"(0xc300c300u), "r"(scale2), "r"(lo2));
+  return r;
+}
+__device__ __forceinline__ uint32_t kvt_prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+  return r;
+}
+
+// One lane's share of a page: a 16-byte (D = 128) or 8-byte piece of two tokens' keys and values, and their (scale, lo).
+template <int D>
+struct KvtPiece {
+  uint32_t kc[2][D / 32], ks[2][D / 32], vc[2][D / 32], vs[2][D / 32];
+};
+template <int D>
+__device__ __forceinline__ void kvt_load(uint32_t (&dst)[D / 32], const uint8_t* src) {
+  if (D == 128) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+    dst[0] = v.x; dst[1] = v.y; dst[D / 32 - 2] = v.z; dst[D / 32 - 1] = v.w;
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+    dst[0] = v.x; dst[1] = v.y;
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(32 * KVT_WARPS, 1)
+kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ block_table,
+                 const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, int hq, int hkv,
+                 long long ldq, long long ldo, int max_blocks, int num_blocks, float scale_log2, int* status) {
+  constexpr int NG = D / 32, PB = kv4_page_bytes(D), TILE = KVT_N * D * 2, QTILE = KVT_M * D * 2;
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.z, kvh = blockIdx.y, G = hq / hkv;
+  const int n = q_lens[b];
+  const int c0 = (int)(gridDim.x - 1 - blockIdx.x) * 2 * KVT_M;          // late rows see the most keys: they start first
+  const int rows = n * G - c0;                                            // of this CTA and behind it
+  if (rows <= 0) return;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ KvtBars bars;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* const sQ = smem;
+  uint8_t* const sK = smem + 2 * QTILE;
+  uint8_t* const sV = sK + KVT_STAGES * TILE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int two = rows > KVT_M ? 2 : 1;                                   // tiles of this CTA
+  int ctx = ctx_lens[b];
+  if (ctx > max_blocks * KV4_PAGE) {
+    if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, ctx);
+    ctx = max_blocks * KV4_PAGE;
+  }
+  const int past = ctx - n, row0 = q_start[b];
+  const int seen = past + (c0 + min(rows, 2 * KVT_M) - 1) / G + 1;        // keys that the last row sees
+  const int tiles = (max(seen, 0) + KVT_N - 1) / KVT_N;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.q_full[i], 4);
+      for (int k = 0; k < 2; ++k) { mbar_init(&bars.s_full[i][k], 1); mbar_init(&bars.p_full[i][k], 4); mbar_init(&bars.pv_done[i][k], 1); }
+    }
+    for (int i = 0; i < KVT_STAGES; ++i) {
+      mbar_init(&bars.k_full[i], KVT_FILL); mbar_init(&bars.k_empty[i], 1); mbar_init(&bars.v_full[i], KVT_FILL); mbar_init(&bars.v_empty[i], 1);
+    }
+    bars.abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == KVT_SOFT + KVT_FILL) { tmem_alloc(&bars.tmem_base, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // S buffer k of tile i: columns 128 i + 64 k, its P over the first 32 of them; O of tile i: columns 256 + 128 i
+  const uint32_t tmem = bars.tmem_base;
+  volatile int* const abort_flag = &bars.abort_flag;
+
+  if (warp >= KVT_SOFT && warp < KVT_SOFT + KVT_FILL) {
+    // ================================ tiles of keys and values ================================
+    // piece p of a page: token p / 4 ... the eight lanes of a store have eight tokens, whose swizzled chunks lie in different banks
+    const int w = warp - KVT_SOFT, key0 = w * 8 + (lane & 7), u = lane >> 3;            // tokens key0 and key0 + 32, chunk u of each group
+    bool bad = false;
+    auto block_of = [&](int j) -> int {
+      if (j >= tiles) return 0;
+      const int blk = block_table[(size_t)b * max_blocks + j];
+      if (blk < 0 || blk >= num_blocks) { bad = true; return 0; }
+      return blk;
+    };
+    auto load = [&](KvtPiece<D>& x, int blk) {
+      const size_t at = ((size_t)blk * hkv + kvh) * PB;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = key0 + 32 * i;
+        kvt_load<D>(x.kc[i], kpages + at + key * (D / 2) + u * (D / 8));
+        kvt_load<D>(x.vc[i], vpages + at + kv4_value_at<D>(key, 2 * u, 0));
+        kvt_load<D>(x.ks[i], kpages + at + kv4_code_bytes(D) + key * (D / 8));
+        kvt_load<D>(x.vs[i], vpages + at + kv4_code_bytes(D) + key * (D / 8));
+      }
+    };
+    KvtPiece<D> cur;
+    if (tiles > 0) load(cur, block_of(0));
+    int next_block = block_of(1);
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      KvtPiece<D> nxt;
+      if (j + 1 < tiles) load(nxt, next_block);
+      next_block = block_of(j + 2);
+      const int st = j % KVT_STAGES;
+      const uint32_t ph = (j / KVT_STAGES) & 1;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint64_t* const full = part ? &bars.v_full[st] : &bars.k_full[st];
+        if (!mbar_wait(part ? &bars.v_empty[st] : &bars.k_empty[st], ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 41 + part)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* const tile = (part ? sV : sK) + st * TILE;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int key = key0 + 32 * i;
+          const bool dead = j * KVT_N + key >= ctx;              // behind the sequence: whatever the page holds there is no number
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            uint32_t stat = part ? cur.vs[i][g] : cur.ks[i][g];
+            if (dead) stat = 0u;
+            const uint32_t scale2 = kvt_prmt(stat, stat, 0x1010u), lo2 = kvt_prmt(stat, stat, 0x3232u);
+            // values: 16-bit unit g of two chunks, the even elements and the odd ones
+            const uint32_t word = part ? kvt_prmt(cur.vc[i][g / 2], cur.vc[i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : cur.kc[i][g];
+            const uint4 v = make_uint4(kvt_value(word, 0, scale2, lo2), kvt_value(word, 4, scale2, lo2), kvt_value(word, 8, scale2, lo2), kvt_value(word, 12, scale2, lo2));
+            const int c = 4 * g + u;                             // 16-byte chunk of the row: 64-element block c / 8
+            *reinterpret_cast<uint4*>(tile + (c >> 3) * (KVT_N * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = v;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
+      }
+      if (!ok) break;
+      if (j + 1 < tiles) cur = nxt;
+    }
+    if (bad) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
+  } else if (warp == KVT_SOFT + KVT_FILL) {
+    // ================================ products ================================
+    if (elect_one() && tiles > 0) {
+      const uint32_t idesc_s = umma_idesc(1, 1, 0, 0, KVT_M, KVT_N), idesc_o = umma_idesc(1, 1, 0, 1, KVT_M, D);
+      const uint32_t q_addr = smem_u32(sQ);
+      bool ok = true;
+      for (int i = 0; i < two && ok; ++i) ok = mbar_wait(&bars.q_full[i], 0, abort_flag, status, KID_ATTN_PREFILL, 43);
+      auto issue_s = [&](int j) -> bool {
+        const int st = j % KVT_STAGES;
+        if (!mbar_wait(&bars.k_full[st], (j / KVT_STAGES) & 1, abort_flag, status, KID_ATTN_PREFILL, 44)) return false;
+        tc_fence_after();
+        const uint32_t k_addr = smem_u32(sK + st * TILE);
+        for (int i = 0; i < two; ++i) {
+          // the buffer holds the P of page j - 2
+          if (j >= 2 && !mbar_wait(&bars.pv_done[i][j & 1], ((j >> 1) & 1) ^ 1, abort_flag, status, KID_ATTN_PREFILL, 50)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16(tmem + 128 * i + 64 * (j & 1), umma_desc_sw128(q_addr + i * QTILE + (k >> 2) * (KVT_M * 128) + (k & 3) * 32, 16, 1024),
+                     umma_desc_sw128(k_addr + (k >> 2) * (KVT_N * 128) + (k & 3) * 32, 16, 1024), idesc_s, k != 0);
+          umma_commit(&bars.s_full[i][j & 1]);
+        }
+        umma_commit(&bars.k_empty[st]);
+        return true;
+      };
+      if (ok) ok = issue_s(0);
+      for (int j = 0; j < tiles && ok; ++j) {
+        if (j + 1 < tiles && !issue_s(j + 1)) { ok = false; break; }
+        const int st = j % KVT_STAGES;
+        if (!mbar_wait(&bars.v_full[st], (j / KVT_STAGES) & 1, abort_flag, status, KID_ATTN_PREFILL, 45)) { ok = false; break; }
+        const uint32_t v_addr = smem_u32(sV + st * TILE);
+        for (int i = 0; i < two; ++i) {
+          if (!mbar_wait(&bars.p_full[i][j & 1], (j >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 46)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < KVT_N / 16; ++k)
+            umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 64 * (j & 1) + k * 8, umma_desc_sw128(v_addr + k * 2048, KVT_N * 128, 1024), idesc_o, (j > 0) || (k != 0));
+          umma_commit(&bars.pv_done[i][j & 1]);
+        }
+        if (ok) umma_commit(&bars.v_empty[st]);
+      }
+    }
+  } else {
+    // ================================ soft-max ================================
+    const int i = warp >> 2, row = (warp & 3) * 32 + lane;               // tile, row = lane of tensor memory
+    if (i < two) {
+      const int c = c0 + i * KVT_M + row;
+      const bool live = c < n * G;
+      const int qi = live ? c / G : 0, head = kvh * G + (live ? c - qi * G : 0);
+      {
+        const uint4* src = reinterpret_cast<const uint4*>(q + (size_t)(row0 + qi) * ldq + (size_t)head * D);
+        uint8_t* dst = sQ + i * QTILE + row * 128;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          const uint4 v = live ? src[k] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + (k >> 3) * (KVT_M * 128) + (((k & 7) ^ (row & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_full[i]);
+      }
+      const int hi = live ? past + qi : -1;
+      const int all = past + (c0 + i * KVT_M) / G;                       // keys up to here are seen by every row of the tile
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t tmem_o = tmem + 256 + 128 * i + lanes;
+      float m_ref = -INFINITY;
+      float l0 = 0.f, l1 = 0.f;
+      bool ok = true;
+      for (int j = 0; j < tiles; ++j) {
+        const uint32_t s_addr = tmem + 128 * i + 64 * (j & 1) + lanes;
+        if (!mbar_wait(&bars.s_full[i][j & 1], (j >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 47)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        float s[KVT_N];
+        {
+          uint32_t r[KVT_N];
+          tmem_ld_x32(s_addr, r);
+          tmem_ld_x32(s_addr + 32, r + 32);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < KVT_N; ++k) s[k] = __uint_as_float(r[k]);
+        }
+        if (j * KVT_N + KVT_N - 1 > all) {
+#pragma unroll
+          for (int k = 0; k < KVT_N; ++k) s[k] = j * KVT_N + k <= hi ? s[k] : -INFINITY;
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < KVT_N; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
+        float alpha = 1.f;
+        bool need = false;
+        if (mx > m_ref + KVT_MOVED || (m_ref == -INFINITY && mx > -INFINITY)) {
+          alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
+          m_ref = mx;
+          need = j > 0;
+        }
+        if (__any_sync(0xffffffffu, need)) {
+          // O is rescaled in place: the P V before has to be complete (the rare path)
+          if (!mbar_wait(&bars.pv_done[i][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 48)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < D; k += 16) {
+            uint32_t r[16];
+            tmem_ld_x16(tmem_o + k, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+            tmem_st_x16(tmem_o + k, r);
+          }
+          tmem_st_wait();
+        }
+        const float mr = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t scale2 = f2_pack(scale_log2, scale_log2), off2 = f2_pack(-mr, -mr);
+        uint64_t sum = f2_pack(l0 * alpha, l1 * alpha);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float a, e;
+            f2_unpack(f2_fma(f2_pack(s[32 * h + 2 * k], s[32 * h + 2 * k + 1]), scale2, off2), a, e);
+            a = kvt_ex2(a); e = kvt_ex2(e);
+            pk[k] = pack_bf16x2(a, e);
+            sum = f2_add(sum, f2_pack(a, e));
+          }
+          tmem_st_x16(s_addr + 16 * h, pk);
+        }
+        f2_unpack(sum, l0, l1);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_full[i][j & 1]);
+      }
+      if (ok && tiles > 0 && !mbar_wait(&bars.pv_done[i][(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 49)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tc_fence_after();
+        const float l = l0 + l1, inv = l > 0.f ? 1.f / l : 0.f;
+        __nv_bfloat16* dst = out + (size_t)(row0 + qi) * ldo + (size_t)head * D;
+#pragma unroll
+        for (int k = 0; k < D; k += 16) {
+          uint32_t r[16];
+          if (tiles > 0) { tmem_ld_x16(tmem_o + k, r); tmem_ld_wait(); }
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = l > 0.f ? pack_bf16x2(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv) : 0u;
+          if (live) {
+            reinterpret_cast<uint4*>(dst + k)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<uint4*>(dst + k)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (bars.abort_flag) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  if (warp == KVT_SOFT + KVT_FILL) { __syncwarp(); tc_fence_after(); tmem_dealloc(bars.tmem_base, 512); }
+}
+
+}  // namespace ff
+using namespace ff;
+
+// As ff_kv4_attn_rows with ranges of rows; out rows of whole 16 bytes.
+FF_EXPORT int ff_kv4_attn_tiles(const void* q, const void* kpages, const void* vpages, const int* block_table, const int* q_start, const int* q_lens,
+                                const int* ctx_lens, void* out, int batch, int max_q_len, int hq, int hkv, int dim, long long ldq, long long ldo, int max_blocks,
+                                int num_blocks, float scale, int* status, cudaStream_t s) {
+  if (batch <= 0 || batch > 65535 || max_q_len <= 0 || hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0) return FF_HOST_BAD_SHAPE;
+  if (!(scale > 0.f) || !q_start || !q_lens || !ctx_lens) return FF_HOST_BAD_SHAPE;
+  if (ldq % 8 || ldo % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages) | reinterpret_cast<uintptr_t>(out)) & 15))
+    return FF_HOST_BAD_ALIGN;
+  const long long rows = (long long)max_q_len * (hq / hkv);
+  if (rows > 0x7fffff00ll) return FF_HOST_TOO_LARGE;
+  auto kern = dim == 128 ? kv4_tiles_kernel<128> : kv4_tiles_kernel<64>;
+  const int bytes = dim == 128 ? kvt_smem<128>() : kvt_smem<64>();
+  if (int r = opt_in_smem(kern, bytes)) return r;
+  return launch_pdl(kern, dim3((unsigned)((rows + 2 * KVT_M - 1) / (2 * KVT_M)), hkv, batch), dim3(32 * KVT_WARPS), bytes, s, 0, (const __nv_bfloat16*)q,
+                    (const uint8_t*)kpages, (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, hq, hkv, ldq, ldo, max_blocks, num_blocks,
+                    scale * 1.4426950408889634f, status);
+}

@@ -260,7 +260,7 @@ def attn_decode_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
 
 def prompt_in_tiles(max_q_len: int, hq: int, hkv: int) -> bool:
     """Whether :func:`attn_prefill_kv4` over so many rows takes the kernel whose keys and values are BF16 tiles in shared memory."""
-    return False
+    return max_q_len * (hq // hkv) > 64
 
 
 def attn_prefill_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor, q_lens: torch.Tensor,
@@ -272,11 +272,19 @@ def attn_prefill_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     _check_ints("attn_prefill_kv4", batch, q_start, q_lens)
     _check_device("attn_prefill_kv4", q, q_start, q_lens)
     _require(0 < max_q_len, "attn_prefill_kv4: at least one row")
+    _require(out is None or not out.is_cuda or (out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0), "attn_prefill_kv4: output rows aligned to 16 bytes")
     if not q.is_cuda:
         return _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq, hkv, dim, scale, out)
     if out is None:
         out = torch.empty(rows, hq * dim, dtype=BF16, device=q.device)
     if batch == 0 or rows == 0:
+        return out
+    if prompt_in_tiles(max_q_len, hq, hkv):
+        rc = kernels().ff_kv4_attn_tiles(ptr(q), ptr(kpages), ptr(vpages), ptr(block_table), ptr(q_start), ptr(q_lens), ptr(ctx_lens), ptr(out), batch, max_q_len,
+                                         hq, hkv, dim, c_longlong(ldq), c_longlong(out.stride(0)), block_table.shape[1], blocks, c_float(scale),
+                                         ptr(status_tensor(q.device)), stream_ptr())
+        check(rc, "ff_kv4_attn_tiles")
+        _count()
         return out
     rc = kernels().ff_kv4_attn_rows(ptr(q), ptr(kpages), ptr(vpages), ptr(block_table), ptr(q_start), ptr(q_lens), ptr(ctx_lens), ptr(out), None, batch, max_q_len,
                                     hq, hkv, dim, c_longlong(ldq), c_longlong(out.stride(0)), block_table.shape[1], blocks, 1, c_float(scale),
