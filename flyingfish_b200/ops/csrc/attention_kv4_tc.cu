@@ -2,8 +2,8 @@
 //
 // The rows of a sequence times the query heads of one kv head are flattened (row c: query c / G, head c % G of the group), and a CTA has two tiles of 128 of
 // them over one kv head: both read the same keys and values, so a page is turned into BF16 once for 256 rows. Per page j of 64 tokens:
-//   four warps    load codes and (scale, lo) a page ahead into registers and write keys and values code * scale + lo, rounded to BF16 once, as
-//                 128-byte-swizzled tiles (rounding keys and values is this kernel's choice: the tensor core's operands are BF16)
+//   one thread    fetches the page by bulk copies, three pages ahead
+//   four warps    write keys and values code * scale + lo, rounded to BF16 once, as 128-byte-swizzled tiles (rounding keys and values is this kernel's choice: the tensor core's operands are BF16)
 //   one thread    S_i(j + 1) = Q_i K^T for both tiles, then O_i += P_i V; S, P and O live in tensor memory (P over the S that it came from)
 //   two x 4 warps soft-max of a tile, a thread per row: running maximum and sum in FP32 in the base-2 domain; O is rescaled only when the maximum has moved
 //                 by more than 2^8 (the stale one stays exact: P and the sum share it)
@@ -15,12 +15,13 @@
 namespace ff {
 
 constexpr int KVT_M = 128, KVT_N = KV4_PAGE, KVT_STAGES = 3;
-constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 1;      // warps 0-7 soft-max, 8-11 tiles, 12 products
+constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 2;      // warps 0-7 soft-max, 8-11 tiles, 12 products, 13 pages
+constexpr int KVT_PAGES = 3;                                                         // pages on their way or being turned into tiles
 constexpr float KVT_MOVED = 8.0f;                                                    // log2 units
-template <int D> constexpr int kvt_smem() { return 2 * KVT_M * D * 2 + 2 * KVT_STAGES * KVT_N * D * 2 + 1024; }
+template <int D> constexpr int kvt_smem() { return 2 * KVT_M * D * 2 + 2 * KVT_STAGES * KVT_N * D * 2 + KVT_PAGES * 2 * kv4_page_bytes(D) + 1024; }
 
 struct alignas(8) KvtBars {
-  uint64_t q_full[2], k_full[KVT_STAGES], k_empty[KVT_STAGES], v_full[KVT_STAGES], v_empty[KVT_STAGES], s_full[2][2], p_full[2][2], pv_done[2][2];
+  uint64_t q_full[2], k_full[KVT_STAGES], k_empty[KVT_STAGES], v_full[KVT_STAGES], v_empty[KVT_STAGES], s_full[2][2], p_full[2][2], pv_done[2][2], p_in[KVT_PAGES], p_out[KVT_PAGES];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -42,20 +43,19 @@ __device__ __forceinline__ uint32_t kvt_prmt(uint32_t a, uint32_t b, uint32_t se
   return r;
 }
 
-// One lane's share of a page: a 16-byte (D = 128) or 8-byte piece of two tokens' keys and values, and their (scale, lo).
-template <int D>
-struct KvtPiece {
-  uint32_t kc[2][D / 32], ks[2][D / 32], vc[2][D / 32], vs[2][D / 32];
-};
 template <int D>
 __device__ __forceinline__ void kvt_load(uint32_t (&dst)[D / 32], const uint8_t* src) {
   if (D == 128) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+    const uint4 v = *reinterpret_cast<const uint4*>(src);
     dst[0] = v.x; dst[1] = v.y; dst[D / 32 - 2] = v.z; dst[D / 32 - 1] = v.w;
   } else {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+    const uint2 v = *reinterpret_cast<const uint2*>(src);
     dst[0] = v.x; dst[1] = v.y;
   }
+}
+__device__ __forceinline__ void kvt_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
 template <int D>
@@ -77,6 +77,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
   uint8_t* const sQ = smem;
   uint8_t* const sK = smem + 2 * QTILE;
   uint8_t* const sV = sK + KVT_STAGES * TILE;
+  uint8_t* const sP = sV + KVT_STAGES * TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int two = rows > KVT_M ? 2 : 1;                                   // tiles of this CTA
   int ctx = ctx_lens[b];
@@ -96,6 +97,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
     for (int i = 0; i < KVT_STAGES; ++i) {
       mbar_init(&bars.k_full[i], KVT_FILL); mbar_init(&bars.k_empty[i], 1); mbar_init(&bars.v_full[i], KVT_FILL); mbar_init(&bars.v_empty[i], 1);
     }
+    for (int i = 0; i < KVT_PAGES; ++i) { mbar_init(&bars.p_in[i], 1); mbar_init(&bars.p_out[i], KVT_FILL); }
     bars.abort_flag = 0;
     mbar_fence_init();
   }
@@ -109,107 +111,116 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
 
   if (warp >= KVT_SOFT && warp < KVT_SOFT + KVT_FILL) {
     // ================================ tiles of keys and values ================================
-    // piece p of a page: token p / 4 ... the eight lanes of a store have eight tokens, whose swizzled chunks lie in different banks
-    const int w = warp - KVT_SOFT, key0 = w * 8 + (lane & 7), u = lane >> 3;            // tokens key0 and key0 + 32, chunk u of each group
-    bool bad = false;
-    auto block_of = [&](int j) -> int {
-      if (j >= tiles) return 0;
-      const int blk = block_table[(size_t)b * max_blocks + j];
-      if (blk < 0 || blk >= num_blocks) { bad = true; return 0; }
-      return blk;
-    };
-    auto load = [&](KvtPiece<D>& x, int blk) {
-      const size_t at = ((size_t)blk * hkv + kvh) * PB;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = key0 + 32 * i;
-        kvt_load<D>(x.kc[i], kpages + at + key * (D / 2) + u * (D / 8));
-        kvt_load<D>(x.vc[i], vpages + at + kv4_value_at<D>(key, 2 * u, 0));
-        kvt_load<D>(x.ks[i], kpages + at + kv4_code_bytes(D) + key * (D / 8));
-        kvt_load<D>(x.vs[i], vpages + at + kv4_code_bytes(D) + key * (D / 8));
-      }
-    };
-    KvtPiece<D> cur;
-    if (tiles > 0) load(cur, block_of(0));
-    int next_block = block_of(1);
+    // tokens key and key + 32, chunk u of each of their groups: the eight lanes of a store have eight tokens, whose swizzled chunks lie in different banks
+    const int key0 = (warp - KVT_SOFT) * 8 + (lane & 7), u = lane >> 3;
+    RingPos pr, tr;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      KvtPiece<D> nxt;
-      if (j + 1 < tiles) load(nxt, next_block);
-      next_block = block_of(j + 2);
-      const int st = j % KVT_STAGES;
-      const uint32_t ph = (j / KVT_STAGES) & 1;
+      if (!mbar_wait(&bars.p_in[pr.s], pr.ph, abort_flag, status, KID_ATTN_PREFILL, 40)) ok = false;
+      const uint8_t* const page = sP + pr.s * 2 * PB;
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        uint64_t* const full = part ? &bars.v_full[st] : &bars.k_full[st];
-        if (!mbar_wait(part ? &bars.v_empty[st] : &bars.k_empty[st], ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 41 + part)) ok = false;
+        if (!mbar_wait(part ? &bars.v_empty[tr.s] : &bars.k_empty[tr.s], tr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 41 + part)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint8_t* const tile = (part ? sV : sK) + st * TILE;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int key = key0 + 32 * i;
-          const bool dead = j * KVT_N + key >= ctx;              // behind the sequence: whatever the page holds there is no number
+          uint32_t code[NG], stat[NG];
+          kvt_load<D>(code, page + part * PB + (part ? kv4_value_at<D>(key, 2 * u, 0) : key * (D / 2) + u * (D / 8)));
+          kvt_load<D>(stat, page + part * PB + kv4_code_bytes(D) + key * (D / 8));
+          if (j * KVT_N + key >= ctx) {                          // behind the sequence: whatever the page holds there is no number
+#pragma unroll
+            for (int g = 0; g < NG; ++g) stat[g] = 0u;
+          }
+          uint8_t* const row = (part ? sV : sK) + tr.s * TILE + key * 128;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            uint32_t stat = part ? cur.vs[i][g] : cur.ks[i][g];
-            if (dead) stat = 0u;
-            const uint32_t scale2 = kvt_prmt(stat, stat, 0x1010u), lo2 = kvt_prmt(stat, stat, 0x3232u);
+            const uint32_t scale2 = kvt_prmt(stat[g], stat[g], 0x1010u), lo2 = kvt_prmt(stat[g], stat[g], 0x3232u);
             // values: 16-bit unit g of two chunks, the even elements and the odd ones
-            const uint32_t word = part ? kvt_prmt(cur.vc[i][g / 2], cur.vc[i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : cur.kc[i][g];
+            const uint32_t word = part ? kvt_prmt(code[g / 2], code[NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[g];
             const uint4 v = make_uint4(kvt_value(word, 0, scale2, lo2), kvt_value(word, 4, scale2, lo2), kvt_value(word, 8, scale2, lo2), kvt_value(word, 12, scale2, lo2));
             const int c = 4 * g + u;                             // 16-byte chunk of the row: 64-element block c / 8
-            *reinterpret_cast<uint4*>(tile + (c >> 3) * (KVT_N * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = v;
+            *reinterpret_cast<uint4*>(row + (c >> 3) * (KVT_N * 128) + (((c & 7) ^ (key & 7)) << 4)) = v;
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(full);
+        if (lane == 0) mbar_arrive(part ? &bars.v_full[tr.s] : &bars.k_full[tr.s]);
       }
       if (!ok) break;
-      if (j + 1 < tiles) cur = nxt;
+      if (lane == 0) mbar_arrive(&bars.p_out[pr.s]);
+      pr.next(KVT_PAGES);
+      tr.next(KVT_STAGES);
     }
-    if (bad) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
+  } else if (warp == KVT_SOFT + KVT_FILL + 1) {
+    // ================================ pages ================================
+    if (elect_one()) {
+      bool bad = false;
+      RingPos pr;
+      int blk = tiles > 0 ? block_table[(size_t)b * max_blocks] : 0;
+      for (int j = 0; j < tiles; ++j) {
+        const int next = j + 1 < tiles ? block_table[(size_t)b * max_blocks + j + 1] : 0;
+        if (blk < 0 || blk >= num_blocks) { bad = true; blk = 0; }
+        const size_t at = ((size_t)blk * hkv + kvh) * PB;
+        if (!mbar_wait(&bars.p_out[pr.s], pr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 39)) break;
+        mbar_expect_tx(&bars.p_in[pr.s], 2 * PB);
+        kvt_bulk_load(sP + pr.s * 2 * PB, kpages + at, PB, &bars.p_in[pr.s]);
+        kvt_bulk_load(sP + pr.s * 2 * PB + PB, vpages + at, PB, &bars.p_in[pr.s]);
+        pr.next(KVT_PAGES);
+        blk = next;
+      }
+      if (bad) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
+    }
   } else if (warp == KVT_SOFT + KVT_FILL) {
     // ================================ products ================================
     if (elect_one() && tiles > 0) {
       const uint32_t idesc_s = umma_idesc(1, 1, 0, 0, KVT_M, KVT_N), idesc_o = umma_idesc(1, 1, 0, 1, KVT_M, D);
-      const uint32_t q_addr = smem_u32(sQ);
+      // descriptors differ by byte offsets / 16 in their low bits
+      const uint64_t qd = umma_desc_sw128(smem_u32(sQ), 16, 1024), kd = umma_desc_sw128(smem_u32(sK), 16, 1024), vd = umma_desc_sw128(smem_u32(sV), KVT_N * 128, 1024);
       bool ok = true;
       for (int i = 0; i < two && ok; ++i) ok = mbar_wait(&bars.q_full[i], 0, abort_flag, status, KID_ATTN_PREFILL, 43);
+      RingPos kr, vr;
       auto issue_s = [&](int j) -> bool {
-        const int st = j % KVT_STAGES;
-        if (!mbar_wait(&bars.k_full[st], (j / KVT_STAGES) & 1, abort_flag, status, KID_ATTN_PREFILL, 44)) return false;
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(sK + st * TILE);
-        for (int i = 0; i < two; ++i) {
-          // the buffer holds the P of page j - 2
-          if (j >= 2 && !mbar_wait(&bars.pv_done[i][j & 1], ((j >> 1) & 1) ^ 1, abort_flag, status, KID_ATTN_PREFILL, 50)) return false;
-          tc_fence_after();
+        if (!mbar_wait(&bars.k_full[kr.s], kr.ph, abort_flag, status, KID_ATTN_PREFILL, 44)) return false;
+        const uint64_t d = kd + (uint32_t)(kr.s * (TILE >> 4));
+        const uint32_t s0 = tmem + 64 * (j & 1), before = ((j >> 1) & 1) ^ 1;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_f16(tmem + 128 * i + 64 * (j & 1), umma_desc_sw128(q_addr + i * QTILE + (k >> 2) * (KVT_M * 128) + (k & 3) * 32, 16, 1024),
-                     umma_desc_sw128(k_addr + (k >> 2) * (KVT_N * 128) + (k & 3) * 32, 16, 1024), idesc_s, k != 0);
-          umma_commit(&bars.s_full[i][j & 1]);
+        for (int i = 0; i < 2; ++i) {
+          if (i < two) {
+            // the buffer holds the P of page j - 2
+            if (j >= 2 && !mbar_wait(&bars.pv_done[i][j & 1], before, abort_flag, status, KID_ATTN_PREFILL, 50)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_f16(s0 + 128 * i, qd + (uint32_t)((i * QTILE + (k >> 2) * (KVT_M * 128) + (k & 3) * 32) >> 4), d + (uint32_t)(((k >> 2) * (KVT_N * 128) + (k & 3) * 32) >> 4),
+                       idesc_s, k != 0);
+            umma_commit(&bars.s_full[i][j & 1]);
+          }
         }
-        umma_commit(&bars.k_empty[st]);
+        umma_commit(&bars.k_empty[kr.s]);
+        kr.next(KVT_STAGES);
         return true;
       };
       if (ok) ok = issue_s(0);
       for (int j = 0; j < tiles && ok; ++j) {
         if (j + 1 < tiles && !issue_s(j + 1)) { ok = false; break; }
-        const int st = j % KVT_STAGES;
-        if (!mbar_wait(&bars.v_full[st], (j / KVT_STAGES) & 1, abort_flag, status, KID_ATTN_PREFILL, 45)) { ok = false; break; }
-        const uint32_t v_addr = smem_u32(sV + st * TILE);
-        for (int i = 0; i < two; ++i) {
-          if (!mbar_wait(&bars.p_full[i][j & 1], (j >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 46)) { ok = false; break; }
-          tc_fence_after();
+        if (!mbar_wait(&bars.v_full[vr.s], vr.ph, abort_flag, status, KID_ATTN_PREFILL, 45)) { ok = false; break; }
+        const uint64_t d = vd + (uint32_t)(vr.s * (TILE >> 4));
+        const uint32_t p0 = tmem + 64 * (j & 1), mine = (j >> 1) & 1;
 #pragma unroll
-          for (int k = 0; k < KVT_N / 16; ++k)
-            umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 64 * (j & 1) + k * 8, umma_desc_sw128(v_addr + k * 2048, KVT_N * 128, 1024), idesc_o, (j > 0) || (k != 0));
-          umma_commit(&bars.pv_done[i][j & 1]);
+        for (int i = 0; i < 2; ++i) {
+          if (i < two && ok) {
+            if (!mbar_wait(&bars.p_full[i][j & 1], mine, abort_flag, status, KID_ATTN_PREFILL, 46)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < KVT_N / 16; ++k)
+              umma_f16_ts(tmem + 256 + 128 * i, p0 + 128 * i + k * 8, d + (uint32_t)((k * 2048) >> 4), idesc_o, (j > 0) || (k != 0));
+            umma_commit(&bars.pv_done[i][j & 1]);
+          }
         }
-        if (ok) umma_commit(&bars.v_empty[st]);
+        if (ok) umma_commit(&bars.v_empty[vr.s]);
+        vr.next(KVT_STAGES);
       }
     }
   } else {
