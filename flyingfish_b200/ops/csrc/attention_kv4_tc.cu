@@ -1,12 +1,15 @@
 // Prompts over the 4-bit key / value cache on the 5th-generation tensor cores (layout and format: kv4.cuh).
 //
 // The rows of a sequence times the query heads of one kv head are flattened (row c: query c / G, head c % G of the group), and a CTA has two tiles of 128 of
-// them over one kv head: both read the same keys and values, so a page is turned into BF16 once for 256 rows. Per page j of 64 tokens:
+// them over one kv head: both read the same keys and values, so a page is turned into FP16 once for 256 rows. Per page j of 64 tokens:
 //   one thread    fetches the page by bulk copies, three pages ahead
-//   four warps    write keys and values code * scale + lo, rounded to BF16 once, as 128-byte-swizzled tiles (rounding keys and values is this kernel's choice: the tensor core's operands are BF16)
+//   four warps    write keys and values code * scale + lo, rounded once, as 128-byte-swizzled tiles
 //   one thread    S_i(j + 1) = Q_i K^T for both tiles, then O_i += P_i V; S, P and O live in tensor memory (P over the S that it came from)
 //   two x 4 warps soft-max of a tile, a thread per row: running maximum and sum in FP32 in the base-2 domain; O is rescaled only when the maximum has moved
 //                 by more than 2^8 (the stale one stays exact: P and the sum share it)
+// All operands are FP16, this kernel's choice of a rounding: keys, values and weights keep 11 bits where BF16 has 8 (outputs 0.0017 off in the root mean square,
+// as a single rounding of the result is; 0.0035 with BF16 operands). The cache's elements are at most 2^15, so they fit; a scale or lo below 2^-14 is off by
+// 2^-25, an element by 2^-20 then. Queries are divided by a power of two per row, which the soft-max's scale takes back.
 // S(j + 1) of a tile waits for its P V (j - 1), whose P it overwrites; the other tile's products run meanwhile.
 // Every wait is bounded; a time-out records FF_ERR_TIMEOUT, and all roles leave through the abort flag.
 #include "kv4.cuh"
@@ -31,10 +34,15 @@ __device__ __forceinline__ float kvt_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// nibbles at bits s and s + 16 times scale plus lo, one rounding (128 + n is a BF16 number, the difference is exact)
+// nibbles at bits s and s + 16 times scale plus lo as FP16, one rounding (1024 + n is an FP16 number, the difference is exact)
 __device__ __forceinline__ uint32_t kvt_value(uint32_t w, int s, uint32_t scale2, uint32_t lo2) {
-  uint32_t n = ((w >> s) & 0x000f000fu) | 0x43004300u, r;
-  asm("{\n\t.reg .b32 t;\n\tadd.rn.bf16x2 t, %1, %2;\n\tfma.rn.bf16x2 %0, t, %3, %4;\n\t}" : "=r"(r) : "r"(n), "r"(0xc300c300u), "r"(scale2), "r"(lo2));
+  uint32_t n = ((w >> s) & 0x000f000fu) | 0x64006400u, r;
+  asm("{\n\t.reg .b32 t;\n\tadd.rn.f16x2 t, %1, %2;\n\tfma.rn.f16x2 %0, t, %3, %4;\n\t}" : "=r"(r) : "r"(n), "r"(0xe400e400u), "r"(scale2), "r"(lo2));
+  return r;
+}
+__device__ __forceinline__ uint32_t kvt_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 __device__ __forceinline__ uint32_t kvt_prmt(uint32_t a, uint32_t b, uint32_t sel) {
@@ -44,14 +52,9 @@ __device__ __forceinline__ uint32_t kvt_prmt(uint32_t a, uint32_t b, uint32_t se
 }
 
 template <int D>
-__device__ __forceinline__ void kvt_load(uint32_t (&dst)[D / 32], const uint8_t* src) {
-  if (D == 128) {
-    const uint4 v = *reinterpret_cast<const uint4*>(src);
-    dst[0] = v.x; dst[1] = v.y; dst[D / 32 - 2] = v.z; dst[D / 32 - 1] = v.w;
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(src);
-    dst[0] = v.x; dst[1] = v.y;
-  }
+__device__ __forceinline__ void kvt_load(uint32_t (&dst)[D / 32], uint32_t src) {
+  if (D == 128) kv4_lds(src, dst[0], dst[1], dst[D / 32 - 2], dst[D / 32 - 1]);
+  else kv4_lds(src, dst[0], dst[1]);
 }
 __device__ __forceinline__ void kvt_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -117,7 +120,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       if (!mbar_wait(&bars.p_in[pr.s], pr.ph, abort_flag, status, KID_ATTN_PREFILL, 40)) ok = false;
-      const uint8_t* const page = sP + pr.s * 2 * PB;
+      const uint32_t page = smem_u32(sP) + pr.s * 2 * PB;
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
         if (!mbar_wait(part ? &bars.v_empty[tr.s] : &bars.k_empty[tr.s], tr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 41 + part)) ok = false;
@@ -133,15 +136,15 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
 #pragma unroll
             for (int g = 0; g < NG; ++g) stat[g] = 0u;
           }
-          uint8_t* const row = (part ? sV : sK) + tr.s * TILE + key * 128;
+          const uint32_t row = smem_u32(part ? sV : sK) + tr.s * TILE + key * 128;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const uint32_t scale2 = kvt_prmt(stat[g], stat[g], 0x1010u), lo2 = kvt_prmt(stat[g], stat[g], 0x3232u);
+            const float2 sl = unpack_bf16x2(stat[g]);
+            const uint32_t scale2 = kvt_f16x2(sl.x, sl.x), lo2 = kvt_f16x2(sl.y, sl.y);
             // values: 16-bit unit g of two chunks, the even elements and the odd ones
             const uint32_t word = part ? kvt_prmt(code[g / 2], code[NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[g];
-            const uint4 v = make_uint4(kvt_value(word, 0, scale2, lo2), kvt_value(word, 4, scale2, lo2), kvt_value(word, 8, scale2, lo2), kvt_value(word, 12, scale2, lo2));
             const int c = 4 * g + u;                             // 16-byte chunk of the row: 64-element block c / 8
-            *reinterpret_cast<uint4*>(row + (c >> 3) * (KVT_N * 128) + (((c & 7) ^ (key & 7)) << 4)) = v;
+            kv4_sts(row + (c >> 3) * (KVT_N * 128) + (((c & 7) ^ (key & 7)) << 4), kvt_value(word, 0, scale2, lo2), kvt_value(word, 4, scale2, lo2), kvt_value(word, 8, scale2, lo2), kvt_value(word, 12, scale2, lo2));
           }
         }
         fence_proxy_async_smem();
@@ -175,7 +178,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
   } else if (warp == KVT_SOFT + KVT_FILL) {
     // ================================ products ================================
     if (elect_one() && tiles > 0) {
-      const uint32_t idesc_s = umma_idesc(1, 1, 0, 0, KVT_M, KVT_N), idesc_o = umma_idesc(1, 1, 0, 1, KVT_M, D);
+      const uint32_t idesc_s = umma_idesc(0, 0, 0, 0, KVT_M, KVT_N), idesc_o = umma_idesc(0, 0, 0, 1, KVT_M, D);
       // descriptors differ by byte offsets / 16 in their low bits
       const uint64_t qd = umma_desc_sw128(smem_u32(sQ), 16, 1024), kd = umma_desc_sw128(smem_u32(sK), 16, 1024), vd = umma_desc_sw128(smem_u32(sV), KVT_N * 128, 1024);
       bool ok = true;
@@ -230,13 +233,29 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       const int c = c0 + i * KVT_M + row;
       const bool live = c < n * G;
       const int qi = live ? c / G : 0, head = kvh * G + (live ? c - qi * G : 0);
+      float row_scale = scale_log2;
       {
+        // The row as FP16, divided by the power of two of its greatest element: exact, but for elements below 2^-14 of that.
+        uint32_t w[D / 2];
         const uint4* src = reinterpret_cast<const uint4*>(q + (size_t)(row0 + qi) * ldq + (size_t)head * D);
-        uint8_t* dst = sQ + i * QTILE + row * 128;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) {
           const uint4 v = live ? src[k] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + (k >> 3) * (KVT_M * 128) + (((k & 7) ^ (row & 7)) << 4)) = v;
+          w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
+        }
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 2; ++k) { const float2 v = unpack_bf16x2(w[k]); most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))); }
+        const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);          // 2^(e - 127), and its inverse
+        const float up = __uint_as_float(e << 23), down = __uint_as_float((254u - e) << 23);
+        row_scale *= up;
+        const uint32_t dst = smem_u32(sQ) + i * QTILE + row * 128;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          uint32_t x[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) { const float2 v = unpack_bf16x2(w[4 * k + z]); x[z] = kvt_f16x2(v.x * down, v.y * down); }
+          kv4_sts(dst + (k >> 3) * (KVT_M * 128) + (((k & 7) ^ (row & 7)) << 4), x[0], x[1], x[2], x[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -271,7 +290,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int k = 0; k < KVT_N; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * row_scale;
         float alpha = 1.f;
         bool need = false;
         if (mx > m_ref + KVT_MOVED || (m_ref == -INFINITY && mx > -INFINITY)) {
@@ -297,7 +316,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           tmem_st_wait();
         }
         const float mr = m_ref == -INFINITY ? 0.f : m_ref;
-        const uint64_t scale2 = f2_pack(scale_log2, scale_log2), off2 = f2_pack(-mr, -mr);
+        const uint64_t scale2 = f2_pack(row_scale, row_scale), off2 = f2_pack(-mr, -mr);
         uint64_t sum = f2_pack(l0 * alpha, l1 * alpha);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -307,7 +326,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
             float a, e;
             f2_unpack(f2_fma(f2_pack(s[32 * h + 2 * k], s[32 * h + 2 * k + 1]), scale2, off2), a, e);
             a = kvt_ex2(a); e = kvt_ex2(e);
-            pk[k] = pack_bf16x2(a, e);
+            pk[k] = kvt_f16x2(a, e);
             sum = f2_add(sum, f2_pack(a, e));
           }
           tmem_st_x16(s_addr + 16 * h, pk);

@@ -15,7 +15,7 @@ __device__ __forceinline__ float kv4_bf16_of_double(double x) {
 }
 
 // Codes of a lane's 8 elements and the (scale, lo) of their group, which four neighbouring lanes hold together. Every lane of the warp takes part.
-// ok: the group is finite and of magnitude 2^120 at most, so that no difference of elements overflows; otherwise everything is 0.
+// ok: the group is finite and of magnitude 2^15 at most (FP16 holds what it stands for); otherwise everything is 0.
 // A code comes from an FP32 quotient that is off by less than 3e-6; only where it lies within 1e-4 of a border between two codes is it taken in FP64.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t& stats, bool& ok) {
   float lo = x[0], hi = x[0], big = 0.f;
@@ -30,7 +30,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t& 
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
   }
-  ok = big <= 1.329227995784916e36f;                         // 2^120
+  ok = big <= 32768.f;
   float scale = ok ? kv4_bf16_of_double(((double)hi - (double)lo) / 15.0) : 0.f;
   if (scale < 1.1754943508222875e-38f) scale = 0.f;          // 2^-126
   if (!ok) lo = 0.f;

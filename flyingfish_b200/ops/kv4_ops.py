@@ -22,6 +22,7 @@ from .lib import KernelError, check, kernels, ptr, status_tensor, stream_ptr
 PAGE = 64
 GROUP = 32
 DIMS = (64, 128)
+MOST = 2.0 ** 15                  # greatest magnitude of an element: FP16 holds it
 
 
 def page_bytes(dim: int) -> int:
@@ -119,7 +120,7 @@ def write_kv4(qkv: torch.Tensor, slots: torch.Tensor, kpages: torch.Tensor, vpag
     first n elements of a head's halves turn), keys and values are written to ``slots`` (int32; page * 64 + place, below 0: not written). Returns the queries
     [rows, hq * dim]; ``qkv`` itself stays as it is (without ``cos_sin`` and norms the result is a view of it). ``q_norm`` / ``k_norm`` ([dim] BF16, given
     together): heads are RMS-normed with them and ``eps`` first. Rounds as ``ops.rope_kv_paged`` does. No two rows have the same slot. Keys and values that are
-    not finite, or of magnitude above 2^120, raise the device status and are stored as zeros."""
+    not finite, or of magnitude above 2^15, raise the device status, and their group of 32 is stored as zeros."""
     rows, ld = _rows2d(qkv)
     blocks = _check_pages("write_kv4", kpages, vpages, hkv, dim)
     _require(hq > 0 and hkv > 0 and qkv.shape[1] >= (hq + 2 * hkv) * dim and qkv.dtype == BF16, "write_kv4: packed BF16 rows")
@@ -149,7 +150,7 @@ def write_kv4(qkv: torch.Tensor, slots: torch.Tensor, kpages: torch.Tensor, vpag
         k, v = turned[:, hq:], x[:, hq + hkv:]
         live = slots >= 0
         _require(bool((slots[live] < blocks * PAGE).all()), "write_kv4: a slot behind the last page")
-        _require(all(bool((t[live].float().abs() <= 2.0 ** 120).all()) for t in (k, v)), "write_kv4: keys and values must be finite")
+        _require(all(bool((t[live].float().abs() <= MOST).all()) for t in (k, v)), "write_kv4: keys and values must be finite and at most 2^15")
         _write_rows(kpages, k, slots, dim, True)
         _write_rows(vpages, v, slots, dim, False)
         return qkv[:, : hq * dim] if plain else turned[:, :hq].reshape(rows, hq * dim)
@@ -259,7 +260,7 @@ def attn_decode_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
 
 
 def prompt_in_tiles(max_q_len: int, hq: int, hkv: int) -> bool:
-    """Whether :func:`attn_prefill_kv4` over so many rows takes the kernel whose keys and values are BF16 tiles in shared memory."""
+    """Whether :func:`attn_prefill_kv4` over so many rows takes the kernel whose keys and values are FP16 tiles in shared memory."""
     return max_q_len * (hq // hkv) > 64
 
 

@@ -65,9 +65,9 @@ def _cache(lens, hkv, dim, seed, device, width=None, fill=0xFF):
 
 
 def _definition(q, kpages, vpages, table, spans, hq, hkv, dim, scale, rounded=False):
-    """Per row and head: the attention in 64 bits, the sum of p |v| and of p (v - lo). ``rounded``: of keys and values that are rounded to BF16."""
+    """Per row and head: the attention in 64 bits, the sum of p |v|, of p (v - lo) and of |v| of the visible keys. ``rounded``: of keys and values that are rounded to FP16."""
     g = hq // hkv
-    res, mag, off = (torch.zeros(q.shape[0], hq, dim, dtype=torch.float64) for _ in range(3))
+    res, mag, off, tot = (torch.zeros(q.shape[0], hq, dim, dtype=torch.float64) for _ in range(4))
     for b, (at, n, ctx) in enumerate(spans):
         if ctx <= 0 or n == 0:
             continue
@@ -75,7 +75,7 @@ def _definition(q, kpages, vpages, table, spans, hq, hkv, dim, scale, rounded=Fa
         k, v = (kv4_ops.page_values(p.cpu()[pages], dim, keys).double().transpose(0, 1).reshape(hkv, -1, dim)[:, :ctx] for p, keys in ((kpages, True), (vpages, False)))
         lo = v.unflatten(-1, (-1, 32)).amin(-1, keepdim=True).expand(-1, -1, -1, 32).flatten(-2)
         if rounded:
-            k, v = k.to(BF16).double(), v.to(BF16).double()
+            k, v = k.half().double(), v.half().double()
         x = q[at: at + n, : hq * dim].double().cpu().view(n, hkv, g, dim)
         score = torch.einsum("nhgd,hkd->nhgk", x, k) * scale
         score.masked_fill_((torch.arange(ctx)[None, :] > torch.arange(ctx - n, ctx)[:, None])[:, None, None], -math.inf)
@@ -83,7 +83,8 @@ def _definition(q, kpages, vpages, table, spans, hq, hkv, dim, scale, rounded=Fa
         res[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v).reshape(n, hq, dim)
         mag[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v.abs()).reshape(n, hq, dim)
         off[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v - lo).reshape(n, hq, dim)
-    return [t.view(q.shape[0], hq * dim) for t in (res, mag, off)]
+        tot[at: at + n] = v.abs().sum(1).repeat_interleave(g, dim=0)
+    return [t.view(q.shape[0], hq * dim) for t in (res, mag, off, tot)]
 
 
 def _status_of(fn):
@@ -138,7 +139,7 @@ def test_what_the_operators_refuse():
     qkv, slots = _rows(3, (hq + 2 * hkv) * dim, 1), torch.arange(3, dtype=torch.int32)
     write = lambda **kw: kv4_ops.write_kv4(**{**dict(qkv=qkv, slots=slots, kpages=kp, vpages=vp, hq=hq, hkv=hkv, dim=dim), **kw})
     bad = qkv.clone(); bad[1, hq * dim] = float("nan")
-    huge = qkv.clone(); huge[1, -1] = 2.0 ** 121
+    huge = qkv.clone(); huge[1, -1] = 2.0 ** 15 * 1.01
     for kw in (dict(dim=96), dict(qkv=qkv.float()), dict(slots=slots.long()), dict(slots=slots[:2]), dict(kpages=kp[:, :1]), dict(kpages=kp.transpose(0, 1)),
                dict(vpages=vp[:1]), dict(hq=5), dict(cos_sin=_turn(3, 33, 1)), dict(cos_sin=_turn(2, 32, 1)), dict(cos_sin=_turn(3, 32, 1).double()),
                dict(q_norm=torch.ones(dim, dtype=BF16)), dict(q_norm=torch.ones(dim), k_norm=torch.ones(dim)), dict(qkv=bad), dict(qkv=huge),
@@ -168,7 +169,7 @@ def test_attention_of_empty_and_short_sequences_cpu():
     kp, vp, table = _cache(lens, hkv, dim, 3, "cpu")
     q = _rows(5, hq * dim, 9)
     got = kv4_ops.attn_decode_kv4(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32), hq, hkv, dim, 0.125)
-    want, mag, _ = _definition(q, kp, vp, table, [(i, 1, c) for i, c in enumerate(lens)], hq, hkv, dim, 0.125)
+    want, mag, _, _ = _definition(q, kp, vp, table, [(i, 1, c) for i, c in enumerate(lens)], hq, hkv, dim, 0.125)
     assert not got[0].any() and bool(((got.double() - want).abs() <= want.abs() * E + mag * 2.0 ** -14).all())
 
 
@@ -196,7 +197,7 @@ def test_written_pages_are_the_oracles(dim, hq, hkv, rows, pad, turned):
     head[0, :32] = 1.5
     head[0, 32:64] = torch.tensor([1e-38, 2e-38] * 16).to(BF16)
     head[-1, :32] = (100 + torch.arange(32) * 0.5).to(BF16)
-    head[-1, 32:64] = torch.logspace(-20, 20, 32).to(BF16)
+    head[-1, 32:64] = torch.logspace(-20, 4.5, 32).to(BF16)
     blocks = -(-rows // PAGE) + 1
     slots = torch.randperm(blocks * PAGE, generator=torch.Generator().manual_seed(1))[:rows].to(torch.int32)
     if rows > 2:
@@ -246,7 +247,7 @@ def test_head_norms_before_the_turn():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf"), 2.0 ** 121])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf"), 2.0 ** 15 * 1.01])
 def test_numbers_that_are_not_finite_raise_the_status(what):
     dim, hq, hkv = 128, 2, 2
     qkv = _rows(3, (hq + 2 * hkv) * dim, 4)
@@ -274,10 +275,11 @@ def test_slots_and_pages_outside_the_cache_raise_the_status():
         assert _status_of(lambda: kv4_ops.attn_prefill_kv4(qkv, *pages, i32(table).view(1, 1), i32(0), i32(1), i32(ctx), 1, hq, hkv, dim, 0.1)) == 3
 
 
-def _close(got, want, mag, off, rounded=False):
-    """Few rows: p scale is rounded (2^-8 of p (v - lo)) and the result. Prompts in tiles (``rounded``, against keys and values that are rounded to BF16):
-    p is rounded (2^-8 of p |v|) and the result."""
-    tol = want.abs() * E + (mag if rounded else off) * E + mag * 2.0 ** -14
+def _close(got, want, mag, off, tot, rounded=False):
+    """Few rows: p scale is rounded to BF16 (2^-8 of p (v - lo)) and the result. Prompts in tiles (``rounded``, against keys and values that are rounded to
+    FP16): p is rounded to FP16 (2^-11 of p |v|, and 2^-25 where it is below 2^-14), the result to BF16; where a value's last FP32 bit decides its FP16
+    rounding, 2^-11 of p |v| more; a scale or lo below 2^-14 is off by 2^-25, and so is what they give: 17 x 2^-25 with a code of 15."""
+    tol = want.abs() * E + (mag * 2.0 ** -10 + 2.0 ** -20 + tot * 2.0 ** -25 if rounded else off * E) + mag * 2.0 ** -14
     err = (got.cpu().double() - want).abs()
     assert bool((err <= tol).all()), f"{float((err / tol.clamp_min(1e-30)).max())} of the tolerance"
 
@@ -296,8 +298,8 @@ def test_decoded_rows_over_4_bit_pages(dim, hq, hkv, nq, lens):
     got = kv4_ops.attn_decode_kv4(q, kp, vp, table, ctx, hq, hkv, dim, scale, nq=nq)
     again = kv4_ops.attn_decode_kv4(q, kp, vp, table, ctx, hq, hkv, dim, scale, nq=nq)
     assert torch.equal(got, again) and ops.read_status()[0] == 0
-    want, mag, off = _definition(q, kp, vp, table, [(i * nq, nq, c) for i, c in enumerate(lens)], hq, hkv, dim, scale)
-    _close(got, want, mag, off)
+    want, mag, off, tot = _definition(q, kp, vp, table, [(i * nq, nq, c) for i, c in enumerate(lens)], hq, hkv, dim, scale)
+    _close(got, want, mag, off, tot)
     for i, c in enumerate(lens):
         if c == 0:
             assert not got[i * nq: (i + 1) * nq].any()
