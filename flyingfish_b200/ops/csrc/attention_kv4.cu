@@ -5,7 +5,7 @@
 
 namespace ff {
 
-constexpr float KV4_NEG = -3.0e38f;
+constexpr float KV4_NONE = -3.0e38f;       // running maximum of a row that has seen no key
 
 __device__ __forceinline__ uint32_t kv4_prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t r;
@@ -18,99 +18,153 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t a) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
-// nibbles at bits 4 i and 4 i + 16 as BF16 numbers: 128 + n is a BF16 number with n in its last bits, the difference is exact
-__device__ __forceinline__ uint32_t kv4_codes(uint32_t w, int shift) {
-  uint32_t v = ((w >> shift) & 0x000f000fu) | 0x43004300u;
-  const uint32_t m = 0xc300c300u;
+__device__ __forceinline__ uint32_t kv4_f16x2(float lo, float hi) {
   uint32_t r;
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(m));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+__device__ __forceinline__ float kv4_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void kv4_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void kv4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ float kv4_low(uint32_t w) { return __uint_as_float(w << 16); }              // BF16 in the lower / upper half
+__device__ __forceinline__ float kv4_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+template <int NG>
+__device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
+  if constexpr (NG == 4) kv4_lds(src, dst[0], dst[1], dst[2], dst[3]);
+  else kv4_lds(src, dst[0], dst[1]);
+}
 
 // Rows of queries, a few per sequence (one in a decode step): the rows of one sequence times the query heads of one kv head are the columns of
 //   S^T [keys x columns] = K Q^T        O^T [elements x columns] = V^T P^T
-// so that the cache is the 16-row operand of mma.sync m16n8k16 and 8 columns are enough to fill an instruction. Codes 0 .. 15 go into the products as
-// they are; with the groups j of 32 elements
+// so that the cache is the 16-row operand of mma.sync m16n8k16 and 8 columns are enough to fill an instruction. Codes go into the products as they are,
 //   S = sum_j scale_j (q_j . n_j) + lo_j sum(q_j)          O_j = sum_k (p_k scale_kj) n_kj + sum_k p_k lo_kj
-// scale and lo of the keys meet the scores in FP32, those of the values the probabilities (p scale is what is rounded to BF16).
-// A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, with its own ring of stages that bulk copies fill, its own running
-// maximum, sum and O. The warps' results meet in shared memory, those of several CTAs (splits) in kv4_merge_kernel.
-constexpr int KV4_WARPS = 4, KV4_STAGES = 2;
+// for groups j of 32 elements. A code at bits 0 .. 3 of a 16-bit half is the FP16 number n 2^-24, at bits 4 .. 7 n 2^-20 (both subnormal, so exact and linear):
+// four pairs of codes are four masks and one shift, and nothing has to be subtracted. The powers of two go into the queries (every other pair of elements, and
+// a power per column that brings its greatest element to 2^14) and out of the results. Rounded to FP16 is p scale, 11 bits; sums, maxima, scale and lo are FP32,
+// and sum(q_j) is three BF16 parts of a product of its own, whose A operand is lo as it is.
+// A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, fetched by bulk copies into its ring of three slots (keys, values, next keys),
+// with its own running maximum, sum and O. The warps' results meet in shared memory, those of several CTAs (splits) in kv4_merge_kernel.
+constexpr int KV4_WARPS = 4, KV4_SLOTS = 3;
 template <int D, int NT>
 constexpr int kv4_smem() {
-  const int ring = KV4_WARPS * KV4_STAGES * 2 * kv4_page_bytes(D), merge = KV4_WARPS * NT * 8 * (D + 2) * 4;
+  const int ring = KV4_WARPS * KV4_SLOTS * kv4_page_bytes(D), merge = KV4_WARPS * NT * 8 * (D + 2) * 4;
   return ring > merge ? ring : merge;
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * KV4_WARPS)
+__global__ void __launch_bounds__(32 * KV4_WARPS, NT == 1 ? 3 : 2)
 kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ block_table,
                 const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out,
                 float* __restrict__ part_o, float2* __restrict__ part_ml, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks,
                 int nsplit, float scale_log2, int* status) {
-  constexpr int NG = D / 32, PB = kv4_page_bytes(D), ROW = D / 2;
+  constexpr int NG = D / 32, PB = kv4_page_bytes(D), ROW = D / 2, STAT = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[KV4_WARPS][KV4_STAGES];
+  __shared__ uint64_t full[KV4_WARPS][KV4_SLOTS];
   pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (threadIdx.x < KV4_WARPS * KV4_SLOTS) mbar_init(&full[threadIdx.x / KV4_SLOTS][threadIdx.x % KV4_SLOTS], 1);
+  mbar_fence_init();
+  __syncthreads();
   pdl_wait();
   const int split = blockIdx.x, kvh = blockIdx.y % hkv, ct = blockIdx.y / hkv, b = blockIdx.z;
   const int G = hq / hkv;
   const int n = q_lens ? q_lens[b] : nq, row0 = q_start ? q_start[b] : b * nq;
+  int ctx = ctx_lens[b];
   const int columns = n * G - ct * NT * 8;                      // of this CTA and behind it
   if (columns <= 0) return;
-  int ctx = ctx_lens[b];
-  if (ctx > max_blocks * KV4_PAGE) {                            // more keys than the table has pages
-    if (threadIdx.x == 0) set_status(status, KID_ATTN_DECODE, FF_ERR_BOUNDS, b, ctx);
-    ctx = max_blocks * KV4_PAGE;
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  // keys that the last of this CTA's columns sees
-  const int seen = min(ctx, ctx - n + (ct * NT * 8 + min(columns, NT * 8) - 1) / G + 1);
-  const int pages = (max(seen, 0) + KV4_PAGE - 1) / KV4_PAGE;
-  const int per = (pages + nsplit - 1) / nsplit;
-  const int p0 = split * per, p1 = min(pages, p0 + per);
-  if (threadIdx.x < KV4_WARPS * KV4_STAGES) mbar_init(&full[threadIdx.x / KV4_STAGES][threadIdx.x % KV4_STAGES], 1);
-  mbar_fence_init();
-  __syncthreads();
-
-  bool bad = false;
-  uint8_t* const ring = smem + warp * (KV4_STAGES * 2 * PB);
-  auto issue = [&](int p, int st) {
-    int blk = block_table[(size_t)b * max_blocks + p];
-    if (blk < 0 || blk >= num_blocks) { bad = true; blk = 0; }
-    const size_t at = ((size_t)blk * hkv + kvh) * PB;
-    mbar_expect_tx(&full[warp][st], 2 * PB);
-    kv4_bulk_load(ring + st * 2 * PB, kpages + at, PB, &full[warp][st]);
-    kv4_bulk_load(ring + st * 2 * PB + PB, vpages + at, PB, &full[warp][st]);
-  };
-  if (lane == 0)
-    for (int i = 0; i < KV4_STAGES; ++i)
-      if (p0 + warp + i * KV4_WARPS < p1) issue(p0 + warp + i * KV4_WARPS, i);
-
-  // queries of this thread's column of B fragments (column g of every 8), sums of the groups of columns 2 t and 2 t + 1
-  uint32_t qf[NT][NG][2][2];
-  float qs[NT][NG][2];
-  int lim[NT][2];
+  // queries of this thread's column of B fragments (column g of every 8): 8 elements of each group
+  uint4 qv[NT][NG];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int c = ct * NT * 8 + nt * 8 + g;
     const bool live = nt * 8 + g < columns;
     const __nv_bfloat16* src = q + (size_t)(row0 + (live ? c / G : 0)) * ldq + (size_t)(kvh * G + (live ? c % G : 0)) * D;
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (live) v = *reinterpret_cast<const uint4*>(src + 32 * j + 8 * t);
-      qf[nt][j][0][0] = v.x; qf[nt][j][0][1] = v.y; qf[nt][j][1][0] = v.z; qf[nt][j][1][1] = v.w;
-      const float2 a = unpack_bf16x2(v.x), e = unpack_bf16x2(v.y), f = unpack_bf16x2(v.z), h = unpack_bf16x2(v.w);
-      float s = ((a.x + a.y) + (e.x + e.y)) + ((f.x + f.y) + (h.x + h.y));
-      s += __shfl_xor_sync(0xffffffffu, s, 1); s += __shfl_xor_sync(0xffffffffu, s, 2);
-      qs[nt][j][0] = __shfl_sync(0xffffffffu, s, 8 * t);        // column 2 t is held by lanes of g = 2 t
-      qs[nt][j][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+    for (int j = 0; j < NG; ++j) qv[nt][j] = live ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
+  }
+  if (ctx > max_blocks * KV4_PAGE) {                            // more keys than the table has pages
+    if (threadIdx.x == 0) set_status(status, KID_ATTN_DECODE, FF_ERR_BOUNDS, b, ctx);
+    ctx = max_blocks * KV4_PAGE;
+  }
+  // keys that the last of this CTA's columns sees; its pages are shared evenly by the splits and, one after the other, by the warps
+  const int seen = min(ctx, ctx - n + (ct * NT * 8 + min(columns, NT * 8) - 1) / G + 1);
+  const int pages = (max(seen, 0) + KV4_PAGE - 1) / KV4_PAGE;
+  const int per = (pages + nsplit - 1) / nsplit;
+  const int p0 = split * per + warp, p1 = min(pages, split * per + per);
+  const int mine = p1 > p0 ? (p1 - p0 + KV4_WARPS - 1) / KV4_WARPS : 0;
+
+  // numbers of this warp's pages: a lane each, 32 ahead
+  bool bad = false;
+  auto numbers = [&](int first) -> int {
+    const int p = p0 + (first + lane) * KV4_WARPS;
+    if (p >= p1) return 0;
+    const int blk = block_table[(size_t)b * max_blocks + p];
+    if (blk < 0 || blk >= num_blocks) { bad = true; return 0; }
+    return blk;
+  };
+  int ids = numbers(0), ids_next = mine > 32 ? numbers(32) : 0;
+  uint8_t* const ring = smem + warp * (KV4_SLOTS * PB);
+  auto issue = [&](int i) {                                     // item i: keys (even) or values of page i / 2; the whole warp
+    const int blk = __shfl_sync(0xffffffffu, ids, (i >> 1) & 31);
+    if (lane == 0) {
+      const int slot = i % KV4_SLOTS;
+      mbar_expect_tx(&full[warp][slot], PB);
+      kv4_bulk_load(ring + slot * PB, ((i & 1) ? vpages : kpages) + ((size_t)blk * hkv + kvh) * PB, PB, &full[warp][slot]);
     }
+  };
+#pragma unroll
+  for (int i = 0; i < KV4_SLOTS; ++i)
+    if (i < 2 * mine) issue(i);
+
+  uint32_t qf[NT][NG][2][2], qb[NT][2];
+  float cf[NT][2];
+  int lim[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const uint32_t w[4] = {qv[nt][j].x, qv[nt][j].y, qv[nt][j].z, qv[nt][j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(kv4_low(w[i])), fabsf(kv4_high(w[i]))));
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1)); most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // 2^(14 - exponent) of the column's greatest element, and 2^24 over it (zero columns: any; the exponents are kept where both are normal numbers)
+    const int ex = min(max((int)(__float_as_uint(most) >> 23), 20), 244);
+    const float gain = __uint_as_float((uint32_t)(min(254 + 14 - ex, 254)) << 23), back = __uint_as_float((uint32_t)(254 - min(254 + 14 - ex, 254) + 24) << 23);
+    float part[3] = {0.f, 0.f, 0.f};                            // of the group that this lane has in the product with lo
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const uint32_t w[4] = {qv[nt][j].x, qv[nt][j].y, qv[nt][j].z, qv[nt][j].w};
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = kv4_low(w[i]) * gain, y = kv4_high(w[i]) * gain;
+        s += x + y;
+        qf[nt][j][i >> 1][i & 1] = (i & 1) ? kv4_f16x2(x * 0.0625f, y * 0.0625f) : kv4_f16x2(x, y);
+      }
+      s += __shfl_xor_sync(0xffffffffu, s, 1); s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (j == t) {
+        s *= 5.9604644775390625e-8f;                            // 2^-24
+        part[0] = __bfloat162float(__float2bfloat16(s));
+        part[1] = __bfloat162float(__float2bfloat16(s - part[0]));
+        part[2] = s - part[0] - part[1];
+      }
+    }
+    qb[nt][0] = pack_bf16x2(part[0], part[1]); qb[nt][1] = pack_bf16x2(part[2], 0.f);
+    const float f = scale_log2 * back;
+    cf[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);             // column 2 t is held by lanes of g = 2 t
+    cf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
     for (int e = 0; e < 2; ++e) lim[nt][e] = nt * 8 + 2 * t + e < columns ? ctx - n + (ct * NT * 8 + nt * 8 + 2 * t + e) / G : -1;
   }
@@ -119,7 +173,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   float o[NT][NG][2][4], ol[NT][NG][2], m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = KV4_NEG; l[nt][0] = l[nt][1] = 0.f;
+    m[nt][0] = m[nt][1] = KV4_NONE; l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       ol[nt][j][0] = ol[nt][j][1] = 0.f;
@@ -128,108 +182,124 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     }
   }
 
+  // row r of a 16-key tile is key 4 (r / 2) + r % 2, two more from r = 8 on: a thread's four columns of P^T are then its keys 4 t .. 4 t + 3
+  const int kg = 4 * (g >> 1) + (g & 1);
+  const uint32_t ring_at = smem_u32(ring);
   bool ok = true;
-  int it = 0;
-  for (int p = p0 + warp; p < p1; p += KV4_WARPS, ++it) {
-    const int st = it % KV4_STAGES;
-    if (!mbar_wait(&full[warp][st], (it / KV4_STAGES) & 1, nullptr, status, KID_ATTN_DECODE, 41)) { ok = false; break; }
-    const uint8_t* sk = ring + st * 2 * PB;
-    const uint8_t* sv = sk + PB;
+  RingPos pos;
+  for (int w = 0; w < mine; ++w) {
+    const int p = p0 + w * KV4_WARPS;
     const bool whole = p * KV4_PAGE + KV4_PAGE - 1 <= all;
+    if (!mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 41)) { ok = false; break; }
     float s[4][NT][4];
-    // row r of a 16-key tile is key 4 (r / 2) + r % 2, two more from r = 8 on: a thread's four columns of P^T are then its keys 4 t .. 4 t + 3
-    const int kg = 4 * (g >> 1) + (g & 1);
+    {
+      const uint32_t sk = ring_at + pos.s * PB;
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      uint32_t kw[2][NG];
-      uint32_t ks[2][NG];
+      for (int mt = 0; mt < 4; ++mt) {
+        uint32_t kw[2][NG], ks[2][NG], la[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int key = mt * 16 + kg + 2 * r;
-        if (NG == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(sk + key * ROW + t * 16);
-          kw[r][0] = v.x; kw[r][1] = v.y; kw[r][NG - 2] = v.z; kw[r][NG - 1] = v.w;
-          const uint4 f = *reinterpret_cast<const uint4*>(sk + kv4_code_bytes(D) + key * 16);
-          ks[r][0] = f.x; ks[r][1] = f.y; ks[r][NG - 2] = f.z; ks[r][NG - 1] = f.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(sk + key * ROW + t * 8);
-          kw[r][0] = v.x; kw[r][1] = v.y;
-          const uint2 f = *reinterpret_cast<const uint2*>(sk + kv4_code_bytes(D) + key * 8);
-          ks[r][0] = f.x; ks[r][1] = f.y;
+        for (int r = 0; r < 2; ++r) {
+          const int key = mt * 16 + kg + 2 * r;
+          kv4_words<NG>(kw[r], sk + key * ROW + t * (D / 8));
+          kv4_words<NG>(ks[r], sk + kv4_code_bytes(D) + key * STAT);
+          // lo of group t, twice
+          uint32_t st = ks[r][0];
+#pragma unroll
+          for (int j = 1; j < NG; ++j) st = t == j ? ks[r][j] : st;
+          la[r] = t < NG ? kv4_prmt(st, st, 0x3232u) : 0u;
         }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        float acc[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-          const uint32_t a[4] = {kv4_codes(kw[0][j], 8 * k2), kv4_codes(kw[1][j], 8 * k2), kv4_codes(kw[0][j], 8 * k2 + 4), kv4_codes(kw[1][j], 8 * k2 + 4)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) ms_mma(acc[nt], a, qf[nt][j][k2][0], qf[nt][j][k2][1]);
-        }
-        const float2 f0 = unpack_bf16x2(ks[0][j]), f1 = unpack_bf16x2(ks[1][j]);
+        const uint32_t al[4] = {la[0], la[1], la[0], la[1]};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          s[mt][nt][0] = fmaf(f0.x, acc[nt][0], fmaf(f0.y, qs[nt][j][0], s[mt][nt][0]));
-          s[mt][nt][1] = fmaf(f0.x, acc[nt][1], fmaf(f0.y, qs[nt][j][1], s[mt][nt][1]));
-          s[mt][nt][2] = fmaf(f1.x, acc[nt][2], fmaf(f1.y, qs[nt][j][0], s[mt][nt][2]));
-          s[mt][nt][3] = fmaf(f1.x, acc[nt][3], fmaf(f1.y, qs[nt][j][1], s[mt][nt][3]));
+          s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+          ms_mma(s[mt][nt], al, qb[nt][0], qb[nt][1]);
+        }
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          float acc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+          uint32_t w0 = kw[0][j], w1 = kw[1][j];
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const uint32_t a[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) kv4_mma(acc[nt], a, qf[nt][j][k2][0], qf[nt][j][k2][1]);
+            w0 >>= 8; w1 >>= 8;
+          }
+          const float f0 = kv4_low(ks[0][j]), f1 = kv4_low(ks[1][j]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            s[mt][nt][0] = fmaf(f0, acc[nt][0], s[mt][nt][0]);
+            s[mt][nt][1] = fmaf(f0, acc[nt][1], s[mt][nt][1]);
+            s[mt][nt][2] = fmaf(f1, acc[nt][2], s[mt][nt][2]);
+            s[mt][nt][3] = fmaf(f1, acc[nt][3], s[mt][nt][3]);
+          }
         }
       }
     }
-    // masks, running maxima of columns 2 t and 2 t + 1 (in raw units: the scale is positive)
+    __syncwarp();                                               // the slot is read
+    if (2 * w + KV4_SLOTS < 2 * mine) {                         // values of the next page
+      issue(2 * w + KV4_SLOTS);
+      if (((w + 2) & 31) == 0) { ids = ids_next; ids_next = w + 34 < mine ? numbers(w + 34) : 0; }
+    }
+    pos.next(KV4_SLOTS);
+    // masks, running maxima of columns 2 t and 2 t + 1, weights times 8 (their sum has the factor too)
+    float alpha[NT][2];
+    bool moved = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float mx = KV4_NEG;
+        float mx = -INFINITY;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             float& v = s[mt][nt][2 * r + e];
-            v *= scale_log2;
-            if (!whole && p * KV4_PAGE + mt * 16 + kg + 2 * r > lim[nt][e]) v = KV4_NEG;
+            if (!whole && p * KV4_PAGE + mt * 16 + kg + 2 * r > lim[nt][e]) v = -INFINITY;
             mx = fmaxf(mx, v);
           }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m[nt][e], mx), alpha = exp2f(m[nt][e] - mn);
+        const float mn = fmaxf(m[nt][e], mx * cf[nt][e]);
+        alpha[nt][e] = kv4_ex2(m[nt][e] - mn);
+        moved = moved || mn != m[nt][e];
         m[nt][e] = mn;
-        l[nt][e] *= alpha;
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          ol[nt][j][e] *= alpha;
-#pragma unroll
-          for (int a = 0; a < 2; ++a) { o[nt][j][a][e] *= alpha; o[nt][j][a][2 + e] *= alpha; }
-        }
+        const float off = 3.0f - mn;
+        float sum = 0.f;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             float& v = s[mt][nt][2 * r + e];
-            v = v <= KV4_NEG ? 0.f : exp2f(v - mn);
-            l[nt][e] += v;
+            v = kv4_ex2(fmaf(v, cf[nt][e], off));
+            sum += v;
           }
+        l[nt][e] = fmaf(l[nt][e], alpha[nt][e], sum);
       }
     }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            ol[nt][j][e] *= alpha[nt][e];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) { o[nt][j][a][e] *= alpha[nt][e]; o[nt][j][a][2 + e] *= alpha[nt][e]; }
+          }
+    }
+    if (!mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 42)) { ok = false; break; }
+    const uint32_t sv = ring_at + pos.s * PB;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       uint32_t vs[2][NG];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int key = mt * 16 + kg + 2 * r;
-        if (NG == 4) {
-          const uint4 f = *reinterpret_cast<const uint4*>(sv + kv4_code_bytes(D) + key * 16);
-          vs[r][0] = f.x; vs[r][1] = f.y; vs[r][NG - 2] = f.z; vs[r][NG - 1] = f.w;
-        } else {
-          const uint2 f = *reinterpret_cast<const uint2*>(sv + kv4_code_bytes(D) + key * 8);
-          vs[r][0] = f.x; vs[r][1] = f.y;
-        }
+        kv4_words<NG>(vs[r], sv + kv4_code_bytes(D) + key * STAT);
         // tokens behind the sequence: whatever a page holds there (their probabilities are 0)
         if (!whole && p * KV4_PAGE + key >= ctx) {
 #pragma unroll
@@ -239,37 +309,35 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       uint32_t vw[4][NG / 2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* at = sv + kv4_value_at<D>(mt * 16 + 4 * t + i, g, 0);
-        if (NG == 4) {
-          const uint2 v = *reinterpret_cast<const uint2*>(at);
-          vw[i][0] = v.x; vw[i][NG / 2 - 1] = v.y;
-        } else {
-          vw[i][0] = *reinterpret_cast<const uint32_t*>(at);
-        }
+        const uint32_t at = sv + kv4_value_at<D>(mt * 16 + 4 * t + i, g, 0);
+        if constexpr (NG == 4) kv4_lds(at, vw[i][0], vw[i][1]);
+        else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(vw[i][0]) : "r"(at) : "memory");
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-        const uint32_t x01 = kv4_prmt(vw[0][j / 2], vw[1][j / 2], sel), x23 = kv4_prmt(vw[2][j / 2], vw[3][j / 2], sel);
-        const float2 f0 = unpack_bf16x2(vs[0][j]), f1 = unpack_bf16x2(vs[1][j]);
+        uint32_t x01 = kv4_prmt(vw[0][j / 2], vw[1][j / 2], sel), x23 = kv4_prmt(vw[2][j / 2], vw[3][j / 2], sel);
+        const float f0 = kv4_low(vs[0][j]), f1 = kv4_low(vs[1][j]), h0 = kv4_high(vs[0][j]), h1 = kv4_high(vs[1][j]);
         uint32_t bf[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          bf[nt][0] = kv4_transpose(pack_bf16x2(s[mt][nt][0] * f0.x, s[mt][nt][1] * f0.x));
-          bf[nt][1] = kv4_transpose(pack_bf16x2(s[mt][nt][2] * f1.x, s[mt][nt][3] * f1.x));
-          ol[nt][j][0] = fmaf(s[mt][nt][0], f0.y, fmaf(s[mt][nt][2], f1.y, ol[nt][j][0]));
-          ol[nt][j][1] = fmaf(s[mt][nt][1], f0.y, fmaf(s[mt][nt][3], f1.y, ol[nt][j][1]));
+          bf[nt][0] = kv4_transpose(kv4_f16x2(s[mt][nt][0] * f0, s[mt][nt][1] * f0));
+          bf[nt][1] = kv4_transpose(kv4_f16x2(s[mt][nt][2] * f1, s[mt][nt][3] * f1));
+          ol[nt][j][0] = fmaf(s[mt][nt][0], h0, fmaf(s[mt][nt][2], h1, ol[nt][j][0]));
+          ol[nt][j][1] = fmaf(s[mt][nt][1], h0, fmaf(s[mt][nt][3], h1, ol[nt][j][1]));
         }
 #pragma unroll
         for (int a2 = 0; a2 < 2; ++a2) {
-          const uint32_t a[4] = {kv4_codes(x01, 8 * a2), kv4_codes(x01, 8 * a2 + 4), kv4_codes(x23, 8 * a2), kv4_codes(x23, 8 * a2 + 4)};
+          const uint32_t a[4] = {x01 & 0x000f000fu, x01 & 0x00f000f0u, x23 & 0x000f000fu, x23 & 0x00f000f0u};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) ms_mma(o[nt][j][a2], a, bf[nt][0], bf[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) kv4_mma(o[nt][j][a2], a, bf[nt][0], bf[nt][1]);
+          x01 >>= 8; x23 >>= 8;
         }
       }
     }
-    __syncwarp();                                               // the stage is read
-    if (lane == 0 && p + KV4_STAGES * KV4_WARPS < p1) issue(p + KV4_STAGES * KV4_WARPS, st);
+    __syncwarp();
+    if (2 * w + 1 + KV4_SLOTS < 2 * mine) issue(2 * w + 1 + KV4_SLOTS);      // keys of the page after the next
+    pos.next(KV4_SLOTS);
   }
   if (bad) set_status(status, KID_ATTN_DECODE, FF_ERR_BOUNDS, b, split);
   if (!ok) {                                                    // a copy that never came: give those in flight time to end
@@ -294,13 +362,13 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
         add += __shfl_xor_sync(0xffffffffu, add, 4); add += __shfl_xor_sync(0xffffffffu, add, 8); add += __shfl_xor_sync(0xffffffffu, add, 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i)                             // nibble i of lane g's unit: element 32 j + 8 (g / 2) + 2 i + g % 2
-          so[(warp * NT * 8 + col) * D + 32 * j + 8 * (g >> 1) + 2 * i + (g & 1)] = o[nt][j][i >> 1][2 * (i & 1) + e] + add;
+          so[(warp * NT * 8 + col) * D + 32 * j + 8 * (g >> 1) + 2 * i + (g & 1)] = fmaf(o[nt][j][i >> 1][2 * (i & 1) + e], (i & 1) ? 1048576.f : 16777216.f, add);
       }
     }
   __syncthreads();
   for (int i = threadIdx.x; i < min(columns, NT * 8) * D; i += 32 * KV4_WARPS) {
     const int col = i / D, d = i - col * D;
-    float M = KV4_NEG, L = 0.f, acc = 0.f;
+    float M = KV4_NONE, L = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < KV4_WARPS; ++w) M = fmaxf(M, sml[(w * NT * 8 + col) * 2]);
 #pragma unroll
@@ -327,7 +395,7 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
   pdl_trigger();
   pdl_wait();
   const size_t pr = (size_t)blockIdx.x * nsplit;
-  float M = KV4_NEG, L = 0.f, acc = 0.f;
+  float M = KV4_NONE, L = 0.f, acc = 0.f;
   for (int s = 0; s < nsplit; ++s) M = fmaxf(M, part_ml[pr + s].x);
   for (int s = 0; s < nsplit; ++s) {
     const float2 v = part_ml[pr + s];
