@@ -202,11 +202,13 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
           const int key = mt * 16 + kg + 2 * r;
           kv4_words<NG>(kw[r], sk + key * ROW + t * (D / 8));
           kv4_words<NG>(ks[r], sk + kv4_code_bytes(D) + key * STAT);
-          // lo of group t, twice
-          uint32_t st = ks[r][0];
-#pragma unroll
-          for (int j = 1; j < NG; ++j) st = t == j ? ks[r][j] : st;
-          la[r] = t < NG ? kv4_prmt(st, st, 0x3232u) : 0u;
+          // lo of group t, twice (with two groups the other lanes' queries are zero, but what they would read may be no number)
+          la[r] = 0u;
+          if (NG == 4 || t < NG) {
+            uint32_t st;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(st) : "r"(sk + kv4_code_bytes(D) + key * STAT + 4 * t) : "memory");
+            la[r] = kv4_prmt(st, st, 0x3232u);
+          }
         }
         const uint32_t al[4] = {la[0], la[1], la[0], la[1]};
 #pragma unroll
@@ -244,7 +246,17 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       if (((w + 2) & 31) == 0) { ids = ids_next; ids_next = w + 34 < mine ? numbers(w + 34) : 0; }
     }
     pos.next(KV4_SLOTS);
-    // masks, running maxima of columns 2 t and 2 t + 1, weights times 8 (their sum has the factor too)
+    if (!whole) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (p * KV4_PAGE + mt * 16 + kg + 2 * (r >> 1) > lim[nt][r & 1]) s[mt][nt][r] = -INFINITY;
+      __syncwarp();                                             // (a branch of its own: the selects are not worth their place in every other page)
+    }
+    // running maxima of columns 2 t and 2 t + 1, weights times 8 (their sum has the factor too)
     float alpha[NT][2];
     bool moved = false;
 #pragma unroll
@@ -255,11 +267,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float& v = s[mt][nt][2 * r + e];
-            if (!whole && p * KV4_PAGE + mt * 16 + kg + 2 * r > lim[nt][e]) v = -INFINITY;
-            mx = fmaxf(mx, v);
-          }
+          for (int r = 0; r < 2; ++r) mx = fmaxf(mx, s[mt][nt][2 * r + e]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float mn = fmaxf(m[nt][e], mx * cf[nt][e]);
@@ -293,6 +301,12 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     }
     if (!mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 42)) { ok = false; break; }
     const uint32_t sv = ring_at + pos.s * PB;
+    if (p * KV4_PAGE + KV4_PAGE > ctx) {
+      // tokens behind the sequence: whatever the page holds there is no number, and 0 times it would not be 0 (this is the warp's last page)
+      for (int i = max(0, ctx - p * KV4_PAGE) * NG + lane; i < KV4_PAGE * NG; i += 32)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(sv + kv4_code_bytes(D) + 4 * i), "r"(0u) : "memory");
+      __syncwarp();
+    }
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       uint32_t vs[2][NG];
@@ -300,11 +314,6 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       for (int r = 0; r < 2; ++r) {
         const int key = mt * 16 + kg + 2 * r;
         kv4_words<NG>(vs[r], sv + kv4_code_bytes(D) + key * STAT);
-        // tokens behind the sequence: whatever a page holds there (their probabilities are 0)
-        if (!whole && p * KV4_PAGE + key >= ctx) {
-#pragma unroll
-          for (int j = 0; j < NG; ++j) vs[r][j] = 0u;
-        }
       }
       uint32_t vw[4][NG / 2];
 #pragma unroll
@@ -414,7 +423,7 @@ using namespace ff;
 FF_EXPORT int ff_kv4_attn_plan(int batch, int hq, int hkv, int nq, int dim, int max_ctx, long long* floats) {
   const int columns = nq * (hq / hkv), pages = (max_ctx + KV4_PAGE - 1) / KV4_PAGE;
   const long long ctas = (long long)batch * hkv * ((columns + 15) / 16);
-  long long nsplit = (2ll * sm_count() * 2 + ctas - 1) / ctas;
+  long long nsplit = (3ll * sm_count()) / ctas;
   const long long most = (pages + KV4_WARPS - 1) / KV4_WARPS;
   if (nsplit > most) nsplit = most;
   if (nsplit > 128) nsplit = 128;
