@@ -51,22 +51,23 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 // for groups j of 32 elements. A code at bits 0 .. 3 of a 16-bit half is the FP16 number n 2^-24, at bits 4 .. 7 n 2^-20 (both subnormal, so exact and linear):
 // four pairs of codes are four masks and one shift, and nothing has to be subtracted. The powers of two go into the queries (every other pair of elements, and
 // a power per column that brings its greatest element to 2^14) and out of the results. Rounded to FP16 is p scale, 11 bits; sums, maxima, scale and lo are FP32,
-// and sum(q_j) is three BF16 parts of a product of its own, whose A operand is lo as it is.
-// A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, fetched by bulk copies into its ring of three slots (keys, values, next keys),
+// and sum(q_j) is three BF16 parts of a product of its own, whose A operand is lo as it is. The sums of p lo are a product too, with both rounded to FP16
+// (lo, a BF16 number of at most 2^15, is one unless it is below 2^-14).
+// A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, fetched by bulk copies into its two slots (keys, values),
 // with its own running maximum, sum and O. The warps' results meet in shared memory, those of several CTAs (splits) in kv4_merge_kernel.
-constexpr int KV4_WARPS = 4, KV4_SLOTS = 3;
+constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;
 template <int D, int NT>
 constexpr int kv4_smem() {
-  const int ring = KV4_WARPS * KV4_SLOTS * kv4_page_bytes(D), merge = KV4_WARPS * NT * 8 * (D + 2) * 4;
+  const int ring = KV4_WARPS * KV4_SLOTS * kv4_page_bytes(D), merge = KV4_WARPS * NT * 8 * (D + D / 32 + 2) * 4;
   return ring > merge ? ring : merge;
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * KV4_WARPS, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(32 * KV4_WARPS, NT == 1 ? 4 : 2)
 kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ block_table,
                 const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out,
                 float* __restrict__ part_o, float2* __restrict__ part_ml, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks,
-                int nsplit, float scale_log2, int* status) {
+                int nsplit, uint32_t per_group, float scale_log2, int* status) {
   constexpr int NG = D / 32, PB = kv4_page_bytes(D), ROW = D / 2, STAT = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[KV4_WARPS][KV4_SLOTS];
@@ -78,6 +79,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   pdl_wait();
   const int split = blockIdx.x, kvh = blockIdx.y % hkv, ct = blockIdx.y / hkv, b = blockIdx.z;
   const int G = hq / hkv;
+  auto group_of = [&](int c) -> int { return per_group ? (int)__umulhi((uint32_t)c, per_group) : c; };      // c / G
   const int n = q_lens ? q_lens[b] : nq, row0 = q_start ? q_start[b] : b * nq;
   int ctx = ctx_lens[b];
   const int columns = n * G - ct * NT * 8;                      // of this CTA and behind it
@@ -88,7 +90,8 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   for (int nt = 0; nt < NT; ++nt) {
     const int c = ct * NT * 8 + nt * 8 + g;
     const bool live = nt * 8 + g < columns;
-    const __nv_bfloat16* src = q + (size_t)(row0 + (live ? c / G : 0)) * ldq + (size_t)(kvh * G + (live ? c % G : 0)) * D;
+    const int qi = live ? group_of(c) : 0;
+    const __nv_bfloat16* src = q + (size_t)(row0 + qi) * ldq + (size_t)(kvh * G + (live ? c - qi * G : 0)) * D;
 #pragma unroll
     for (int j = 0; j < NG; ++j) qv[nt][j] = live ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
   }
@@ -97,7 +100,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     ctx = max_blocks * KV4_PAGE;
   }
   // keys that the last of this CTA's columns sees; its pages are shared evenly by the splits and, one after the other, by the warps
-  const int seen = min(ctx, ctx - n + (ct * NT * 8 + min(columns, NT * 8) - 1) / G + 1);
+  const int seen = min(ctx, ctx - n + group_of(ct * NT * 8 + min(columns, NT * 8) - 1) + 1);
   const int pages = (max(seen, 0) + KV4_PAGE - 1) / KV4_PAGE;
   const int per = (pages + nsplit - 1) / nsplit;
   const int p0 = split * per + warp, p1 = min(pages, split * per + per);
@@ -166,17 +169,17 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     cf[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);             // column 2 t is held by lanes of g = 2 t
     cf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) lim[nt][e] = nt * 8 + 2 * t + e < columns ? ctx - n + (ct * NT * 8 + nt * 8 + 2 * t + e) / G : -1;
+    for (int e = 0; e < 2; ++e) lim[nt][e] = nt * 8 + 2 * t + e < columns ? ctx - n + group_of(ct * NT * 8 + nt * 8 + 2 * t + e) : -1;
   }
-  const int all = ctx - n + ct * NT * 8 / G;                    // keys up to here are seen by every column
+  const int all = ctx - n + group_of(ct * NT * 8);                    // keys up to here are seen by every column
 
-  float o[NT][NG][2][4], ol[NT][NG][2], m[NT][2], l[NT][2];
+  float o[NT][NG][2][4], ol[NT][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt][0] = m[nt][1] = KV4_NONE; l[nt][0] = l[nt][1] = 0.f;
+    ol[nt][0] = ol[nt][1] = ol[nt][2] = ol[nt][3] = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      ol[nt][j][0] = ol[nt][j][1] = 0.f;
 #pragma unroll
       for (int a = 0; a < 2; ++a) o[nt][j][a][0] = o[nt][j][a][1] = o[nt][j][a][2] = o[nt][j][a][3] = 0.f;
     }
@@ -241,9 +244,9 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       }
     }
     __syncwarp();                                               // the slot is read
-    if (2 * w + KV4_SLOTS < 2 * mine) {                         // values of the next page
-      issue(2 * w + KV4_SLOTS);
-      if (((w + 2) & 31) == 0) { ids = ids_next; ids_next = w + 34 < mine ? numbers(w + 34) : 0; }
+    if (w + 1 < mine) {                                         // keys of the next page
+      if (((w + 1) & 31) == 0) { ids = ids_next; ids_next = numbers(w + 33); }
+      issue(2 * w + 2);
     }
     pos.next(KV4_SLOTS);
     if (!whole) {
@@ -291,13 +294,13 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e) {
+          ol[nt][e] *= alpha[nt][e];
 #pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            ol[nt][j][e] *= alpha[nt][e];
+          for (int j = 0; j < NG; ++j)
 #pragma unroll
             for (int a = 0; a < 2; ++a) { o[nt][j][a][e] *= alpha[nt][e]; o[nt][j][a][2 + e] *= alpha[nt][e]; }
-          }
+        }
     }
     if (!mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 42)) { ok = false; break; }
     const uint32_t sv = ring_at + pos.s * PB;
@@ -315,6 +318,17 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
         const int key = mt * 16 + kg + 2 * r;
         kv4_words<NG>(vs[r], sv + kv4_code_bytes(D) + key * STAT);
       }
+      {
+        // rows of A: lo of group g % NG (rows 8 .. 15: nothing)
+        uint32_t st[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(st[i]) : "r"(sv + kv4_code_bytes(D) + (mt * 16 + 4 * t + i) * STAT + 4 * (g & (NG - 1))) : "memory");
+        const uint32_t a[4] = {kv4_f16x2(kv4_high(st[0]), kv4_high(st[1])), 0u, kv4_f16x2(kv4_high(st[2]), kv4_high(st[3])), 0u};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          kv4_mma(ol[nt], a, kv4_transpose(kv4_f16x2(s[mt][nt][0], s[mt][nt][1])), kv4_transpose(kv4_f16x2(s[mt][nt][2], s[mt][nt][3])));
+      }
       uint32_t vw[4][NG / 2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -326,14 +340,12 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       for (int j = 0; j < NG; ++j) {
         const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
         uint32_t x01 = kv4_prmt(vw[0][j / 2], vw[1][j / 2], sel), x23 = kv4_prmt(vw[2][j / 2], vw[3][j / 2], sel);
-        const float f0 = kv4_low(vs[0][j]), f1 = kv4_low(vs[1][j]), h0 = kv4_high(vs[0][j]), h1 = kv4_high(vs[1][j]);
+        const float f0 = kv4_low(vs[0][j]), f1 = kv4_low(vs[1][j]);
         uint32_t bf[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           bf[nt][0] = kv4_transpose(kv4_f16x2(s[mt][nt][0] * f0, s[mt][nt][1] * f0));
           bf[nt][1] = kv4_transpose(kv4_f16x2(s[mt][nt][2] * f1, s[mt][nt][3] * f1));
-          ol[nt][j][0] = fmaf(s[mt][nt][0], h0, fmaf(s[mt][nt][2], h1, ol[nt][j][0]));
-          ol[nt][j][1] = fmaf(s[mt][nt][1], h0, fmaf(s[mt][nt][3], h1, ol[nt][j][1]));
         }
 #pragma unroll
         for (int a2 = 0; a2 < 2; ++a2) {
@@ -345,7 +357,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       }
     }
     __syncwarp();
-    if (2 * w + 1 + KV4_SLOTS < 2 * mine) issue(2 * w + 1 + KV4_SLOTS);      // keys of the page after the next
+    if (w + 1 < mine) issue(2 * w + 3);                         // its values
     pos.next(KV4_SLOTS);
   }
   if (bad) set_status(status, KID_ATTN_DECODE, FF_ERR_BOUNDS, b, split);
@@ -355,8 +367,9 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   }
   __syncthreads();                                              // the rings are free
 
-  float* const so = reinterpret_cast<float*>(smem);             // [warp][column][D], then [warp][column][2]
+  float* const so = reinterpret_cast<float*>(smem);             // [warp][column][D], then [warp][column][2], then [warp][column][NG]
   float* const sml = so + KV4_WARPS * NT * 8 * D;
+  float* const sol = sml + KV4_WARPS * NT * 8 * 2;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -365,14 +378,12 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4); l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
       if (g == 0) { sml[(warp * NT * 8 + col) * 2] = m[nt][e]; sml[(warp * NT * 8 + col) * 2 + 1] = l[nt][e]; }
+      if (g < NG) sol[(warp * NT * 8 + col) * NG + g] = ol[nt][e];
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        float add = ol[nt][j][e];
-        add += __shfl_xor_sync(0xffffffffu, add, 4); add += __shfl_xor_sync(0xffffffffu, add, 8); add += __shfl_xor_sync(0xffffffffu, add, 16);
+      for (int j = 0; j < NG; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i)                             // nibble i of lane g's unit: element 32 j + 8 (g / 2) + 2 i + g % 2
-          so[(warp * NT * 8 + col) * D + 32 * j + 8 * (g >> 1) + 2 * i + (g & 1)] = fmaf(o[nt][j][i >> 1][2 * (i & 1) + e], (i & 1) ? 1048576.f : 16777216.f, add);
-      }
+          so[(warp * NT * 8 + col) * D + 32 * j + 8 * (g >> 1) + 2 * i + (g & 1)] = o[nt][j][i >> 1][2 * (i & 1) + e] * ((i & 1) ? 1048576.f : 16777216.f);
     }
   __syncthreads();
   for (int i = threadIdx.x; i < min(columns, NT * 8) * D; i += 32 * KV4_WARPS) {
@@ -384,9 +395,9 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     for (int w = 0; w < KV4_WARPS; ++w) {
       const float sc = exp2f(sml[(w * NT * 8 + col) * 2] - M);
       L += sml[(w * NT * 8 + col) * 2 + 1] * sc;
-      acc += so[(w * NT * 8 + col) * D + d] * sc;
+      acc += (so[(w * NT * 8 + col) * D + d] + sol[(w * NT * 8 + col) * NG + (d >> 5)]) * sc;
     }
-    const int c = ct * NT * 8 + col, qi = c / G, head = kvh * G + c % G;
+    const int c = ct * NT * 8 + col, qi = group_of(c), head = kvh * G + c - qi * G;
     if (nsplit == 1) {
       out[(size_t)(row0 + qi) * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
     } else {
@@ -422,8 +433,8 @@ using namespace ff;
 // Splits that ff_kv4_attn_rows takes for such a launch, and the floats of scratch it needs for them (0 for one split).
 FF_EXPORT int ff_kv4_attn_plan(int batch, int hq, int hkv, int nq, int dim, int max_ctx, long long* floats) {
   const int columns = nq * (hq / hkv), pages = (max_ctx + KV4_PAGE - 1) / KV4_PAGE;
-  const long long ctas = (long long)batch * hkv * ((columns + 15) / 16);
-  long long nsplit = (3ll * sm_count()) / ctas;
+  const long long ctas = (long long)batch * hkv * (columns > 8 ? (columns + 15) / 16 : 1);
+  long long nsplit = ((columns > 8 ? 2ll : 4ll) * sm_count()) / ctas;
   const long long most = (pages + KV4_WARPS - 1) / KV4_WARPS;
   if (nsplit > most) nsplit = most;
   if (nsplit > 128) nsplit = 128;
@@ -451,7 +462,7 @@ FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vp
   float2* ml = nsplit > 1 ? reinterpret_cast<float2*>(scratch + rows * hq * nsplit * dim) : nullptr;
   if (int r = launch_pdl(kern, dim3(nsplit, (unsigned)tiles, batch), dim3(32 * KV4_WARPS), bytes, s, 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
                          (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, scratch, ml, nq, hq, hkv, ldq, ldo, max_blocks,
-                         num_blocks, nsplit, scale * 1.4426950408889634f, status)) return r;
+                         num_blocks, nsplit, hq == hkv ? 0u : (uint32_t)((0x100000000ull + hq / hkv - 1) / (hq / hkv)), scale * 1.4426950408889634f, status)) return r;
   if (nsplit == 1) return FF_HOST_OK;
   return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(rows * hq)), dim3(dim), 0, s, 0, (const float*)scratch,
                     (const float2*)ml, (__nv_bfloat16*)out, hq, ldo, nsplit);
