@@ -38,6 +38,16 @@ __device__ __forceinline__ void kv4_bulk_load(void* dst, const void* src, uint32
 }
 __device__ __forceinline__ float kv4_low(uint32_t w) { return __uint_as_float(w << 16); }              // BF16 in the lower / upper half
 __device__ __forceinline__ float kv4_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ float kv4_peer(const float* p, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(dsmem_addr(smem_u32(p), (uint32_t)rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 kv4_peer2(const float* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(dsmem_addr(smem_u32(p), (uint32_t)rank)) : "memory");
+  return v;
+}
 template <int NG>
 __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
   if constexpr (NG == 4) kv4_lds(src, dst[0], dst[1], dst[2], dst[3]);
@@ -54,11 +64,12 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 // and sum(q_j) is three BF16 parts of a product of its own, whose A operand is lo as it is. The sums of p lo are a product too, with both rounded to FP16
 // (lo, a BF16 number of at most 2^15, is one unless it is below 2^-14).
 // A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, fetched by bulk copies into its two slots (keys, values),
-// with its own running maximum, sum and O. The warps' results meet in shared memory, those of several CTAs (splits) in kv4_merge_kernel.
+// with its own running maximum, sum and O. The warps' results meet in shared memory, those of up to eight CTAs (splits) in that of
+// their cluster, those of more in kv4_merge_kernel.
 constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;
 template <int D, int NT>
 constexpr int kv4_smem() {
-  const int ring = KV4_WARPS * KV4_SLOTS * kv4_page_bytes(D), merge = KV4_WARPS * NT * 8 * (D + D / 32 + 2) * 4;
+  const int ring = KV4_WARPS * KV4_SLOTS * kv4_page_bytes(D), merge = (KV4_WARPS * (D + D / 32 + 2) + D + 2) * NT * 8 * 4;
   return ring > merge ? ring : merge;
 }
 
@@ -367,9 +378,12 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   }
   __syncthreads();                                              // the rings are free
 
-  float* const so = reinterpret_cast<float*>(smem);             // [warp][column][D], then [warp][column][2], then [warp][column][NG]
+  float* const so = reinterpret_cast<float*>(smem);             // [warp][column][D], then [warp][column][2], [warp][column][NG]; this CTA's [column][D], [column][2]
   float* const sml = so + KV4_WARPS * NT * 8 * D;
   float* const sol = sml + KV4_WARPS * NT * 8 * 2;
+  float* const mo = sol + KV4_WARPS * NT * 8 * NG;
+  float* const mml = mo + NT * 8 * D;
+  const bool cluster = nsplit > 1 && part_o == nullptr;         // the splits are a cluster and join in shared memory
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -400,37 +414,94 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     const int c = ct * NT * 8 + col, qi = group_of(c), head = kvh * G + c - qi * G;
     if (nsplit == 1) {
       out[(size_t)(row0 + qi) * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+    } else if (cluster) {
+      mo[i] = acc;
+      if (d == 0) { mml[2 * col] = M; mml[2 * col + 1] = L; }
     } else {
       const size_t pr = ((size_t)(row0 + qi) * hq + head) * nsplit + split;
       part_o[pr * D + d] = acc;
       if (d == 0) part_ml[pr] = make_float2(M, L);
     }
   }
+  if (cluster) {
+    cluster_sync_all();
+    for (int i = split * 32 * KV4_WARPS + threadIdx.x; i < min(columns, NT * 8) * D; i += nsplit * 32 * KV4_WARPS) {
+      const int col = i / D, d = i - col * D;
+      float2 ml[8];
+      float M = KV4_NONE, L = 0.f, acc = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < nsplit) { ml[r] = kv4_peer2(mml + 2 * col, r); M = fmaxf(M, ml[r].x); }
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < nsplit) {
+          const float sc = kv4_ex2(ml[r].x - M);
+          L = fmaf(ml[r].y, sc, L);
+          acc = fmaf(kv4_peer(mo + i, r), sc, acc);
+        }
+      const int c = ct * NT * 8 + col, qi = group_of(c), head = kvh * G + c - qi * G;
+      out[(size_t)(row0 + qi) * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+    }
+    cluster_sync_all();                                         // no CTA leaves while its shared memory is read
+  }
 }
 
-// Splits of one (row, head) joined; D threads each.
+// More than eight splits of one (row, head) joined: four warps take every fourth split, a lane D / 32 elements, four splits on their way at once (one after the
+// other, 74 splits of a single sequence took as long as the attention itself).
 template <int D>
-__global__ void __launch_bounds__(D)
+__global__ void __launch_bounds__(128)
 kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, __nv_bfloat16* __restrict__ out, int hq, long long ldo, int nsplit) {
+  constexpr int E = D / 32;
+  __shared__ float sacc[4][D];
   pdl_trigger();
   pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t pr = (size_t)blockIdx.x * nsplit;
-  float M = KV4_NONE, L = 0.f, acc = 0.f;
-  for (int s = 0; s < nsplit; ++s) M = fmaxf(M, part_ml[pr + s].x);
-  for (int s = 0; s < nsplit; ++s) {
-    const float2 v = part_ml[pr + s];
-    const float sc = exp2f(v.x - M);
-    L += v.y * sc;
-    acc += part_o[(pr + s) * D + threadIdx.x] * sc;
+  float2 ml[4];                                                 // of splits lane, lane + 32, ... (at most 128)
+  float M = KV4_NONE, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ml[i] = lane + 32 * i < nsplit ? part_ml[pr + lane + 32 * i] : make_float2(KV4_NONE, 0.f);
+    M = fmaxf(M, ml[i].x);
   }
-  const int row = blockIdx.x / hq, head = blockIdx.x - row * hq;
-  out[(size_t)row * ldo + (size_t)head * D + threadIdx.x] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+  M = warp_max(M);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { ml[i].x = kv4_ex2(ml[i].x - M); L = fmaf(ml[i].y, ml[i].x, L); }
+  L = warp_sum(L);
+  float acc[E];
+#pragma unroll
+  for (int k = 0; k < E; ++k) acc[k] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    for (int s = 32 * i + warp; s < min(nsplit, 32 * i + 32); s += 16) {
+      float v[4][E], sc[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int at = s + 4 * u;
+        sc[u] = __shfl_sync(0xffffffffu, ml[i].x, at & 31);
+        if (at >= min(nsplit, 32 * i + 32)) sc[u] = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[u][k] = sc[u] > 0.f ? part_o[(pr + at) * D + lane + 32 * k] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] = fmaf(v[u][k], sc[u], acc[k]);
+    }
+#pragma unroll
+  for (int k = 0; k < E; ++k) sacc[warp][lane + 32 * k] = acc[k];
+  __syncthreads();
+  const int d = threadIdx.x, row = blockIdx.x / hq, head = blockIdx.x - row * hq;
+  if (d < D) {
+    const float o = (sacc[0][d] + sacc[1][d]) + (sacc[2][d] + sacc[3][d]);
+    out[(size_t)row * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? o / L : 0.f);
+  }
 }
 
 }  // namespace ff
 using namespace ff;
 
-// Splits that ff_kv4_attn_rows takes for such a launch, and the floats of scratch it needs for them (0 for one split).
+// Splits that ff_kv4_attn_rows takes for such a launch, and the floats of scratch it needs for them (none up to eight).
 FF_EXPORT int ff_kv4_attn_plan(int batch, int hq, int hkv, int nq, int dim, int max_ctx, long long* floats) {
   const int columns = nq * (hq / hkv), pages = (max_ctx + KV4_PAGE - 1) / KV4_PAGE;
   const long long ctas = (long long)batch * hkv * (columns > 8 ? (columns + 15) / 16 : 1);
@@ -439,17 +510,17 @@ FF_EXPORT int ff_kv4_attn_plan(int batch, int hq, int hkv, int nq, int dim, int 
   if (nsplit > most) nsplit = most;
   if (nsplit > 128) nsplit = 128;
   if (nsplit < 1) nsplit = 1;
-  if (floats) *floats = nsplit > 1 ? (long long)batch * nq * hq * nsplit * (dim + 2) : 0;
+  if (floats) *floats = nsplit > 8 ? (long long)batch * nq * hq * nsplit * (dim + 2) : 0;
   return (int)nsplit;
 }
 
 // q rows [.., ldq] with head h at column h dim; sequence b has rows q_start[b] .. + q_lens[b], or nq rows from b nq on where those are null (only then may
-// there be splits); ctx_lens[b] keys are seen by the last of them. Rows of no keys are zero.
+// there be more than eight splits); ctx_lens[b] keys are seen by the last of them. Rows of no keys are zero.
 FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vpages, const int* block_table, const int* q_start, const int* q_lens,
                                const int* ctx_lens, void* out, float* scratch, int batch, int nq, int hq, int hkv, int dim, long long ldq, long long ldo,
                                int max_blocks, int num_blocks, int nsplit, float scale, int* status, cudaStream_t s) {
   if (batch <= 0 || batch > 65535 || nq <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0) return FF_HOST_BAD_SHAPE;
-  if (!(scale > 0.f) || nsplit < 1 || (q_start == nullptr) != (q_lens == nullptr) || (nsplit > 1 && (scratch == nullptr || q_start != nullptr))) return FF_HOST_BAD_SHAPE;
+  if (!(scale > 0.f) || nsplit < 1 || nsplit > 128 || (q_start == nullptr) != (q_lens == nullptr) || (nsplit > 8 && (scratch == nullptr || q_start != nullptr))) return FF_HOST_BAD_SHAPE;
   if (ldq % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages)) & 15)) return FF_HOST_BAD_ALIGN;
   const int columns = nq * (hq / hkv);
   const bool wide = columns > 8;
@@ -459,11 +530,11 @@ FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vp
   const int bytes = dim == 128 ? (wide ? kv4_smem<128, 2>() : kv4_smem<128, 1>()) : (wide ? kv4_smem<64, 2>() : kv4_smem<64, 1>());
   if (int r = opt_in_smem(kern, bytes)) return r;
   const long long rows = (long long)batch * nq;                 // with splits
-  float2* ml = nsplit > 1 ? reinterpret_cast<float2*>(scratch + rows * hq * nsplit * dim) : nullptr;
-  if (int r = launch_pdl(kern, dim3(nsplit, (unsigned)tiles, batch), dim3(32 * KV4_WARPS), bytes, s, 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
-                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, scratch, ml, nq, hq, hkv, ldq, ldo, max_blocks,
+  float2* ml = nsplit > 8 ? reinterpret_cast<float2*>(scratch + rows * hq * nsplit * dim) : nullptr;
+  if (int r = launch_pdl(kern, dim3(nsplit, (unsigned)tiles, batch), dim3(32 * KV4_WARPS), bytes, s, nsplit <= 8 ? nsplit : 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
+                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, nsplit > 8 ? scratch : (float*)nullptr, ml, nq, hq, hkv, ldq, ldo, max_blocks,
                          num_blocks, nsplit, hq == hkv ? 0u : (uint32_t)((0x100000000ull + hq / hkv - 1) / (hq / hkv)), scale * 1.4426950408889634f, status)) return r;
-  if (nsplit == 1) return FF_HOST_OK;
-  return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(rows * hq)), dim3(dim), 0, s, 0, (const float*)scratch,
+  if (nsplit <= 8) return FF_HOST_OK;
+  return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(rows * hq)), dim3(128), 0, s, 0, (const float*)scratch,
                     (const float2*)ml, (__nv_bfloat16*)out, hq, ldo, nsplit);
 }

@@ -251,11 +251,11 @@ def attn_decode_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     lib = kernels()
     floats = c_longlong(0)
     nsplit = lib.ff_kv4_attn_plan(batch, hq, hkv, nq, dim, min(max_ctx or width * PAGE, width * PAGE), ctypes.byref(floats))
-    scratch = torch.empty(floats.value, dtype=torch.float32, device=q.device) if nsplit > 1 else None
+    scratch = torch.empty(floats.value, dtype=torch.float32, device=q.device) if floats.value else None
     rc = lib.ff_kv4_attn_rows(ptr(q), ptr(kpages), ptr(vpages), ptr(block_table), None, None, ptr(ctx_lens), ptr(out), ptr(scratch), batch, nq, hq, hkv, dim,
                               c_longlong(ldq), c_longlong(out.stride(0)), width, blocks, nsplit, c_float(scale), ptr(status_tensor(q.device)), stream_ptr())
     check(rc, "ff_kv4_attn_rows")
-    _count(1 if nsplit == 1 else 2)
+    _count(1 if scratch is None else 2)
     return out
 
 
