@@ -1,6 +1,7 @@
 // Attention over the 4-bit key / value cache (layout and format: kv4.cuh).
 #include "kv4.cuh"
 #include "host_util.h"
+#include "launchers.h"
 #include "mma_sync.cuh"
 
 namespace ff {
@@ -450,13 +451,17 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
 // other, 74 splits of a single sequence took as long as the attention itself).
 template <int D>
 __global__ void __launch_bounds__(128)
-kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, __nv_bfloat16* __restrict__ out, int hq, long long ldo, int nsplit) {
+kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int* __restrict__ q_start, const int* __restrict__ q_lens,
+                 __nv_bfloat16* __restrict__ out, int nq, int hq, long long ldo, int nsplit) {
   constexpr int E = D / 32;
   __shared__ float sacc[4][D];
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const size_t pr = (size_t)blockIdx.x * nsplit;
+  const int b = blockIdx.y, qi = blockIdx.x / hq, head = blockIdx.x - qi * hq;
+  if (q_lens != nullptr && qi >= q_lens[b]) return;
+  const int row = (q_start ? q_start[b] : b * nq) + qi;
+  const size_t pr = ((size_t)row * hq + head) * nsplit;
   float2 ml[4];                                                 // of splits lane, lane + 32, ... (at most 128)
   float M = KV4_NONE, L = 0.f;
 #pragma unroll
@@ -491,7 +496,7 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
 #pragma unroll
   for (int k = 0; k < E; ++k) sacc[warp][lane + 32 * k] = acc[k];
   __syncthreads();
-  const int d = threadIdx.x, row = blockIdx.x / hq, head = blockIdx.x - row * hq;
+  const int d = threadIdx.x;
   if (d < D) {
     const float o = (sacc[0][d] + sacc[1][d]) + (sacc[2][d] + sacc[3][d]);
     out[(size_t)row * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? o / L : 0.f);
@@ -512,6 +517,13 @@ FF_EXPORT int ff_kv4_attn_plan(int batch, int hq, int hkv, int nq, int dim, int 
   if (nsplit < 1) nsplit = 1;
   if (floats) *floats = nsplit > 8 ? (long long)batch * nq * hq * nsplit * (dim + 2) : 0;
   return (int)nsplit;
+}
+
+int kv4_merge(const float* part_o, const float2* part_ml, const int* q_start, const int* q_lens, void* out, int batch, int nq, int hq, int dim, long long ldo,
+              int nsplit, cudaStream_t s) {
+  if ((long long)nq * hq > 0x7fffffffll) return FF_HOST_TOO_LARGE;
+  return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(nq * hq), batch), dim3(128), 0, s, 0, part_o, part_ml, q_start, q_lens,
+                    (__nv_bfloat16*)out, nq, hq, ldo, nsplit);
 }
 
 // q rows [.., ldq] with head h at column h dim; sequence b has rows q_start[b] .. + q_lens[b], or nq rows from b nq on where those are null (only then may
@@ -535,6 +547,5 @@ FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vp
                          (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, nsplit > 8 ? scratch : (float*)nullptr, ml, nq, hq, hkv, ldq, ldo, max_blocks,
                          num_blocks, nsplit, hq == hkv ? 0u : (uint32_t)((0x100000000ull + hq / hkv - 1) / (hq / hkv)), scale * 1.4426950408889634f, status)) return r;
   if (nsplit <= 8) return FF_HOST_OK;
-  return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(rows * hq)), dim3(128), 0, s, 0, (const float*)scratch,
-                    (const float2*)ml, (__nv_bfloat16*)out, hq, ldo, nsplit);
+  return kv4_merge(scratch, ml, nullptr, nullptr, out, batch, nq, hq, dim, ldo, nsplit, s);
 }

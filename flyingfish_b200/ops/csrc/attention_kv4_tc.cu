@@ -14,6 +14,7 @@
 // Every wait is bounded; a time-out records FF_ERR_TIMEOUT, and all roles leave through the abort flag.
 #include "kv4.cuh"
 #include "host_util.h"
+#include "launchers.h"
 
 namespace ff {
 
@@ -64,14 +65,16 @@ __device__ __forceinline__ void kvt_bulk_load(void* dst, const void* src, uint32
 template <int D>
 __global__ void __launch_bounds__(32 * KVT_WARPS, 1)
 kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ block_table,
-                 const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, int hq, int hkv,
-                 long long ldq, long long ldo, int max_blocks, int num_blocks, float scale_log2, int* status) {
+                 const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out,
+                 float* __restrict__ part_o, float2* __restrict__ part_ml, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks, int nsplit,
+                 float scale_log2, int* status) {
   constexpr int NG = D / 32, PB = kv4_page_bytes(D), TILE = KVT_N * D * 2, QTILE = KVT_M * D * 2;
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.z, kvh = blockIdx.y, G = hq / hkv;
-  const int n = q_lens[b];
-  const int c0 = (int)(gridDim.x - 1 - blockIdx.x) * 2 * KVT_M;          // late rows see the most keys: they start first
+  const int n = q_lens ? q_lens[b] : nq;
+  const int split = blockIdx.x % nsplit;
+  const int c0 = (int)((gridDim.x - 1 - blockIdx.x) / nsplit) * 2 * KVT_M;          // late rows see the most keys: they start first
   const int rows = n * G - c0;                                            // of this CTA and behind it
   if (rows <= 0) return;
   extern __shared__ uint8_t smem_raw[];
@@ -88,9 +91,10 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
     if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, ctx);
     ctx = max_blocks * KV4_PAGE;
   }
-  const int past = ctx - n, row0 = q_start[b];
+  const int past = ctx - n, row0 = q_start ? q_start[b] : b * nq;
   const int seen = past + (c0 + min(rows, 2 * KVT_M) - 1) / G + 1;        // keys that the last row sees
-  const int tiles = (max(seen, 0) + KVT_N - 1) / KVT_N;
+  const int pages = (max(seen, 0) + KVT_N - 1) / KVT_N, per = (pages + nsplit - 1) / nsplit;
+  const int first = split * per, tiles = max(0, min(pages, first + per) - first);    // pages of this split
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -132,7 +136,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           uint32_t code[NG], stat[NG];
           kvt_load<D>(code, page + part * PB + (part ? kv4_value_at<D>(key, 2 * u, 0) : key * (D / 2) + u * (D / 8)));
           kvt_load<D>(stat, page + part * PB + kv4_code_bytes(D) + key * (D / 8));
-          if (j * KVT_N + key >= ctx) {                          // behind the sequence: whatever the page holds there is no number
+          if ((first + j) * KVT_N + key >= ctx) {                          // behind the sequence: whatever the page holds there is no number
 #pragma unroll
             for (int g = 0; g < NG; ++g) stat[g] = 0u;
           }
@@ -161,9 +165,9 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
     if (elect_one()) {
       bool bad = false;
       RingPos pr;
-      int blk = tiles > 0 ? block_table[(size_t)b * max_blocks] : 0;
+      int blk = tiles > 0 ? block_table[(size_t)b * max_blocks + first] : 0;
       for (int j = 0; j < tiles; ++j) {
-        const int next = j + 1 < tiles ? block_table[(size_t)b * max_blocks + j + 1] : 0;
+        const int next = j + 1 < tiles ? block_table[(size_t)b * max_blocks + first + j + 1] : 0;
         if (blk < 0 || blk >= num_blocks) { bad = true; blk = 0; }
         const size_t at = ((size_t)blk * hkv + kvh) * PB;
         if (!mbar_wait(&bars.p_out[pr.s], pr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 39)) break;
@@ -283,9 +287,9 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
 #pragma unroll
           for (int k = 0; k < KVT_N; ++k) s[k] = __uint_as_float(r[k]);
         }
-        if (j * KVT_N + KVT_N - 1 > all) {
+        if ((first + j) * KVT_N + KVT_N - 1 > all) {
 #pragma unroll
-          for (int k = 0; k < KVT_N; ++k) s[k] = j * KVT_N + k <= hi ? s[k] : -INFINITY;
+          for (int k = 0; k < KVT_N; ++k) s[k] = (first + j) * KVT_N + k <= hi ? s[k] : -INFINITY;
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -343,17 +347,25 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         tc_fence_after();
         const float l = l0 + l1, inv = l > 0.f ? 1.f / l : 0.f;
         __nv_bfloat16* dst = out + (size_t)(row0 + qi) * ldo + (size_t)head * D;
+        const size_t pr = ((size_t)(row0 + qi) * hq + head) * nsplit + split;
+        if (nsplit > 1 && live) part_ml[pr] = make_float2(m_ref == -INFINITY ? -3.0e38f : m_ref, l);
 #pragma unroll
         for (int k = 0; k < D; k += 16) {
           uint32_t r[16];
           if (tiles > 0) { tmem_ld_x16(tmem_o + k, r); tmem_ld_wait(); }
+          if (!live) continue;
+          if (nsplit > 1) {
+            if (l > 0.f) {                                       // (the merge does not read what has no weight)
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part_o + pr * D + k + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+            }
+            continue;
+          }
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = l > 0.f ? pack_bf16x2(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv) : 0u;
-          if (live) {
-            reinterpret_cast<uint4*>(dst + k)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            reinterpret_cast<uint4*>(dst + k)[1] = make_uint4(o[4], o[5], o[6], o[7]);
-          }
+          reinterpret_cast<uint4*>(dst + k)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          reinterpret_cast<uint4*>(dst + k)[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }
       }
     }
@@ -370,20 +382,39 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
 }  // namespace ff
 using namespace ff;
 
-// As ff_kv4_attn_rows with ranges of rows; out rows of whole 16 bytes.
+// Splits of ff_kv4_attn_tiles, and the floats of scratch it needs for them. rows: of the whole call, at most max_q_len per sequence. One CTA stands on an SM;
+// where there are fewer than SMs the keys are split, down to four pages each: for one round of CTAs, or three where half of the SMs would do without (their
+// contexts differ: 96 CTAs of up to 62 pages 66 us, in three splits 61).
+FF_EXPORT int ff_kv4_tiles_plan(int batch, int rows, int max_q_len, int hq, int hkv, int dim, int max_ctx, long long* floats) {
+  const long long G = hq / hkv, each = ((long long)max_q_len * G + 2 * KVT_M - 1) / (2 * KVT_M), some = ((long long)rows * G + 2 * KVT_M - 1) / (2 * KVT_M);
+  const long long ctas = hkv * (batch * each < batch + some ? batch * each : batch + some);
+  const long long most = (max_ctx + 4 * KVT_N - 1) / (4 * KVT_N);
+  long long nsplit = ctas <= 0 ? 1 : 2 * ctas <= sm_count() ? sm_count() / ctas : ctas < sm_count() ? 3 : 1;
+  if (nsplit > most) nsplit = most;
+  if (nsplit > 128) nsplit = 128;
+  if (nsplit < 1) nsplit = 1;
+  if (floats) *floats = nsplit > 1 ? (long long)rows * hq * nsplit * (dim + 2) : 0;
+  return (int)nsplit;
+}
+
+// As ff_kv4_attn_rows; out rows of whole 16 bytes. rows: of q and out.
 FF_EXPORT int ff_kv4_attn_tiles(const void* q, const void* kpages, const void* vpages, const int* block_table, const int* q_start, const int* q_lens,
-                                const int* ctx_lens, void* out, int batch, int max_q_len, int hq, int hkv, int dim, long long ldq, long long ldo, int max_blocks,
-                                int num_blocks, float scale, int* status, cudaStream_t s) {
-  if (batch <= 0 || batch > 65535 || max_q_len <= 0 || hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0) return FF_HOST_BAD_SHAPE;
-  if (!(scale > 0.f) || !q_start || !q_lens || !ctx_lens) return FF_HOST_BAD_SHAPE;
-  if (ldq % 8 || ldo % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages) | reinterpret_cast<uintptr_t>(out)) & 15))
+                                const int* ctx_lens, void* out, float* scratch, int batch, int rows, int max_q_len, int hq, int hkv, int dim, long long ldq, long long ldo,
+                                int max_blocks, int num_blocks, int nsplit, float scale, int* status, cudaStream_t s) {
+  if (batch <= 0 || batch > 65535 || rows <= 0 || max_q_len <= 0 || hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0)
+    return FF_HOST_BAD_SHAPE;
+  if (!(scale > 0.f) || (q_start == nullptr) != (q_lens == nullptr) || !ctx_lens || nsplit < 1 || nsplit > 128 || (nsplit > 1 && scratch == nullptr)) return FF_HOST_BAD_SHAPE;
+  if (ldq % 8 || ldo % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages) | reinterpret_cast<uintptr_t>(out) |
+                              reinterpret_cast<uintptr_t>(scratch)) & 15))
     return FF_HOST_BAD_ALIGN;
-  const long long rows = (long long)max_q_len * (hq / hkv);
-  if (rows > 0x7fffff00ll) return FF_HOST_TOO_LARGE;
+  const long long columns = (long long)max_q_len * (hq / hkv), grid = (columns + 2 * KVT_M - 1) / (2 * KVT_M) * nsplit;
+  if (columns > 0x7fffff00ll || grid > 0x7fffffffll) return FF_HOST_TOO_LARGE;
   auto kern = dim == 128 ? kv4_tiles_kernel<128> : kv4_tiles_kernel<64>;
   const int bytes = dim == 128 ? kvt_smem<128>() : kvt_smem<64>();
   if (int r = opt_in_smem(kern, bytes)) return r;
-  return launch_pdl(kern, dim3((unsigned)((rows + 2 * KVT_M - 1) / (2 * KVT_M)), hkv, batch), dim3(32 * KVT_WARPS), bytes, s, 0, (const __nv_bfloat16*)q,
-                    (const uint8_t*)kpages, (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, hq, hkv, ldq, ldo, max_blocks, num_blocks,
-                    scale * 1.4426950408889634f, status);
+  float2* ml = nsplit > 1 ? reinterpret_cast<float2*>(scratch + (long long)rows * hq * nsplit * dim) : nullptr;
+  if (int r = launch_pdl(kern, dim3((unsigned)grid, hkv, batch), dim3(32 * KVT_WARPS), bytes, s, 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
+                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, scratch, ml, max_q_len, hq, hkv, ldq, ldo, max_blocks,
+                         num_blocks, nsplit, scale * 1.4426950408889634f, status)) return r;
+  return nsplit == 1 ? FF_HOST_OK : kv4_merge(scratch, ml, q_start, q_lens, out, batch, max_q_len, hq, dim, ldo, nsplit, s);
 }

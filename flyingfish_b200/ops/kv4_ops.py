@@ -12,12 +12,12 @@ be current, also one that is captured, as long as the tensors are on the current
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_longlong
+from ctypes import c_longlong
 
 import torch
 
-from . import BF16, _count, _require, _rows2d, ref
-from .lib import KernelError, check, kernels, ptr, status_tensor, stream_ptr
+from . import BF16, _count, _require, ref
+from .lib import KernelError, check, kernels, status_tensor
 
 PAGE = 64
 GROUP = 32
@@ -55,7 +55,7 @@ def _places(dim: int, keys: bool) -> tuple[torch.Tensor, torch.Tensor]:
 def quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Codes [..., dim] and (scale, lo) [..., dim / 32] of finite elements [..., dim], in 64 bits."""
     g = x.double().unflatten(-1, (-1, GROUP))
-    lo, hi = g.amin(-1), g.amax(-1)
+    lo, hi = g.amin(-1) + 0.0, g.amax(-1)                             # (no negative zero)
     m, e = torch.frexp((hi - lo) / 15)
     scale = torch.ldexp(torch.round(m * 256) / 256, e)
     scale = torch.where(scale < 2.0 ** -126, 0.0, scale)
@@ -91,24 +91,49 @@ def _write_rows(pages: torch.Tensor, rows: torch.Tensor, slots: torch.Tensor, di
 # ------------------------------------------------------------------------------------------
 # arguments
 # ------------------------------------------------------------------------------------------
+# (plain ifs: a decode step makes these checks for every layer, and a message per check that holds costs more than the check)
 def _check_pages(what: str, kpages: torch.Tensor, vpages: torch.Tensor, hkv: int, dim: int) -> int:
-    _require(dim in DIMS, f"{what}: heads of 64 or 128 elements")
-    for t in (kpages, vpages):
-        _require(t.dtype == torch.uint8 and t.dim() == 3 and t.is_contiguous() and t.shape[1] == hkv and t.shape[2] == page_bytes(dim),
-                 f"{what}: pages are uint8 [blocks, kv heads, page_bytes(dim)]")
-    _require(kpages.shape[0] == vpages.shape[0] > 0, f"{what}: as many pages of keys as of values")
-    return kpages.shape[0]
+    if dim not in DIMS or hkv <= 0:
+        raise KernelError(f"{what}: heads of 64 or 128 elements")
+    shape = kpages.shape
+    if kpages.dtype != torch.uint8 or vpages.dtype != torch.uint8 or vpages.shape != shape or not kpages.is_contiguous() or not vpages.is_contiguous() \
+            or len(shape) != 3 or shape[0] == 0 or shape[1] != hkv or shape[2] != PAGE * (dim // 2 + dim // 8):
+        raise KernelError(f"{what}: pages of keys and of values are uint8 [blocks, kv heads, page_bytes(dim)]")
+    return shape[0]
 
 
 def _check_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
-    _require(all(t is None or t.device == first.device for t in others), f"{what}: tensors on one device")
-    if first.is_cuda:
-        _require(first.device.index == torch.cuda.current_device(), f"{what}: tensors on the current device")
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise KernelError(f"{what}: tensors on one device")
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on the current device")
 
 
 def _check_ints(what: str, n: int, *tensors: torch.Tensor) -> None:
     for t in tensors:
-        _require(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n, f"{what}: int32 metadata, one number each")
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
+            raise KernelError(f"{what}: int32 metadata, one number each")
+
+
+_bound: ctypes.CDLL | None = None
+
+
+def _lib() -> ctypes.CDLL:
+    """The kernels with the types of these launchers' arguments, so that numbers are passed as they are."""
+    global _bound
+    if _bound is None:
+        lib = kernels()
+        raw = getattr(lib, "_lib", lib)                                # (the checking build counts launches in front of it)
+        p, i, n, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+        raw.ff_kv4_write.argtypes = [p, p, p, p, p, i, p, p, f, p, i, i, i, i, n, i, p, p]
+        raw.ff_kv4_read.argtypes = [p, p, p, p, p, i, i, i, i, p, p]
+        raw.ff_kv4_attn_rows.argtypes = [p, p, p, p, p, p, p, p, p, i, i, i, i, i, n, n, i, i, i, f, p, p]
+        raw.ff_kv4_attn_tiles.argtypes = [p, p, p, p, p, p, p, p, p, i, i, i, i, i, i, n, n, i, i, i, f, p, p]
+        raw.ff_copy_pages.argtypes = [p, p, i, p, p, i, p]
+        _bound = lib
+    return _bound
 
 
 # ------------------------------------------------------------------------------------------
@@ -116,15 +141,17 @@ def _check_ints(what: str, n: int, *tensors: torch.Tensor) -> None:
 # ------------------------------------------------------------------------------------------
 def write_kv4(qkv: torch.Tensor, slots: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, hq: int, hkv: int, dim: int,
               cos_sin: torch.Tensor | None = None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 0.0) -> torch.Tensor:
-    """Packed BF16 rows ``[q heads | k heads | v heads]``: queries and keys are turned by ``cos_sin`` (``ops.rope_table``; float32 [rows, n, 2], the
-    first n elements of a head's halves turn), keys and values are written to ``slots`` (int32; page * 64 + place, below 0: not written). Returns the queries
+    """Packed BF16 rows ``[q heads | k heads | v heads]``: queries and keys are turned by ``cos_sin`` (``ops.rope_table``; float32 [rows, n, 2] of
+    BF16 numbers, others are rounded to BF16; the first n elements of a head's halves turn), keys and values are written to ``slots`` (int32; page * 64 + place, below 0: not written). Returns the queries
     [rows, hq * dim]; ``qkv`` itself stays as it is (without ``cos_sin`` and norms the result is a view of it). ``q_norm`` / ``k_norm`` ([dim] BF16, given
     together): heads are RMS-normed with them and ``eps`` first. Rounds as ``ops.rope_kv_paged`` does. No two rows have the same slot. Keys and values that are
     not finite, or of magnitude above 2^15, raise the device status, and their group of 32 is stored as zeros."""
-    rows, ld = _rows2d(qkv)
     blocks = _check_pages("write_kv4", kpages, vpages, hkv, dim)
-    _require(hq > 0 and hkv > 0 and qkv.shape[1] >= (hq + 2 * hkv) * dim and qkv.dtype == BF16, "write_kv4: packed BF16 rows")
-    _require((q_norm is None) == (k_norm is None), "write_kv4: both head norms or none")
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.dtype != BF16 or hq <= 0 or qkv.shape[1] < (hq + 2 * hkv) * dim:
+        raise KernelError("write_kv4: packed BF16 rows with unit inner stride")
+    rows, ld = qkv.shape[0], qkv.stride(0)
+    if (q_norm is None) != (k_norm is None):
+        raise KernelError("write_kv4: both head norms or none")
     _check_ints("write_kv4", rows, slots)
     if cos_sin is not None:
         _require(cos_sin.dtype == torch.float32 and cos_sin.dim() == 3 and cos_sin.shape[0] == rows and 0 < cos_sin.shape[1] <= dim // 2 and cos_sin.shape[2] == 2
@@ -141,7 +168,7 @@ def write_kv4(qkv: torch.Tensor, slots: torch.Tensor, kpages: torch.Tensor, vpag
         if cos_sin is not None:
             n, half = cos_sin.shape[1], dim // 2
             r16 = lambda t: t.to(BF16).float()
-            c, s = cos_sin[:, None, :, 0], cos_sin[:, None, :, 1]
+            c, s = r16(cos_sin[:, None, :, 0]), r16(cos_sin[:, None, :, 1])
             turned = turned.float().clone()
             a, b = turned[..., :n].clone(), turned[..., half: half + n].clone()
             turned[..., :n] = r16(r16(a * c) - r16(b * s))
@@ -154,13 +181,15 @@ def write_kv4(qkv: torch.Tensor, slots: torch.Tensor, kpages: torch.Tensor, vpag
         _write_rows(kpages, k, slots, dim, True)
         _write_rows(vpages, v, slots, dim, False)
         return qkv[:, : hq * dim] if plain else turned[:, :hq].reshape(rows, hq * dim)
-    _require(kpages.data_ptr() % 16 == 0 and vpages.data_ptr() % 16 == 0 and qkv.data_ptr() % 16 == 0 and ld % 8 == 0, "write_kv4: rows and pages aligned to 16 bytes")
+    if (kpages.data_ptr() | vpages.data_ptr() | qkv.data_ptr()) % 16 or ld % 8:
+        raise KernelError("write_kv4: rows and pages aligned to 16 bytes")
     q = qkv[:, : hq * dim] if plain else torch.empty(rows, hq * dim, dtype=BF16, device=qkv.device)
     if rows == 0:
         return q
-    rc = kernels().ff_kv4_write(ptr(qkv), ptr(slots), ptr(kpages), ptr(vpages), ptr(cos_sin), 0 if cos_sin is None else cos_sin.shape[1], ptr(q_norm), ptr(k_norm),
-                                c_float(eps), ptr(None if plain else q), rows, hq, hkv, dim, c_longlong(ld), blocks, ptr(status_tensor(qkv.device)), stream_ptr())
-    check(rc, "ff_kv4_write")
+    at = lambda t: None if t is None else t.data_ptr()
+    check(_lib().ff_kv4_write(qkv.data_ptr(), slots.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), at(cos_sin), 0 if cos_sin is None else cos_sin.shape[1], at(q_norm),
+                              at(k_norm), eps, None if plain else q.data_ptr(), rows, hq, hkv, dim, ld, blocks, status_tensor(qkv.device).data_ptr(),
+                              torch.cuda.current_stream().cuda_stream), "ff_kv4_write")
     _count()
     return q
 
@@ -177,11 +206,12 @@ def read_kv4(kpages: torch.Tensor, vpages: torch.Tensor, slots: torch.Tensor, di
         at = slots.long().clamp(min=0)
         out = [page_values(p[at // PAGE], dim, keys)[torch.arange(rows), :, at % PAGE] for p, keys in ((kpages, True), (vpages, False))]
         return tuple(torch.where((slots >= 0)[:, None, None], t, 0.0).to(BF16) for t in out)
-    _require(kpages.data_ptr() % 16 == 0 and vpages.data_ptr() % 16 == 0, "read_kv4: pages aligned to 16 bytes")
+    if (kpages.data_ptr() | vpages.data_ptr()) % 16:
+        raise KernelError("read_kv4: pages aligned to 16 bytes")
     k, v = (torch.empty(rows, hkv, dim, dtype=BF16, device=kpages.device) for _ in range(2))
     if rows:
-        check(kernels().ff_kv4_read(ptr(kpages), ptr(vpages), ptr(slots), ptr(k), ptr(v), rows, hkv, dim, blocks, ptr(status_tensor(kpages.device)), stream_ptr()),
-              "ff_kv4_read")
+        check(_lib().ff_kv4_read(kpages.data_ptr(), vpages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), rows, hkv, dim, blocks,
+                                 status_tensor(kpages.device).data_ptr(), torch.cuda.current_stream().cuda_stream), "ff_kv4_read")
         _count()
     return k, v
 
@@ -189,21 +219,27 @@ def read_kv4(kpages: torch.Tensor, vpages: torch.Tensor, slots: torch.Tensor, di
 # ------------------------------------------------------------------------------------------
 # attention
 # ------------------------------------------------------------------------------------------
-def _check_attention(what: str, q, kpages, vpages, block_table, ctx_lens, hq, hkv, dim, scale, out) -> tuple[int, int, int]:
-    rows, ldq = _rows2d(q)
+def _check_attention(what, q, kpages, vpages, block_table, ctx_lens, hq, hkv, dim, scale, out) -> tuple[int, int]:
     blocks = _check_pages(what, kpages, vpages, hkv, dim)
-    _require(hkv > 0 and hq % hkv == 0 and hq > 0, f"{what}: a whole number of query heads per kv head")
-    _require(q.dtype == BF16 and q.shape[1] >= hq * dim, f"{what}: BF16 queries")
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[1] > 0, f"{what}: int32 block table")
-    _require(block_table.shape[1] < 1 << 25, f"{what}: positions of 31 bits")
+    if q.dim() != 2 or q.stride(1) != 1 or q.dtype != BF16 or q.shape[1] < hq * dim:
+        raise KernelError(f"{what}: BF16 rows of queries with unit inner stride")
+    if hq <= 0 or hq % hkv:
+        raise KernelError(f"{what}: a whole number of query heads per kv head")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous() or not 0 < block_table.shape[1] < 1 << 25:
+        raise KernelError(f"{what}: int32 block table, positions of 31 bits")
     _check_ints(what, block_table.shape[0], ctx_lens)
-    _require(scale > 0, f"{what}: a positive scale")
+    if not 0 < scale < float("inf"):
+        raise KernelError(f"{what}: a positive scale")
     _check_device(what, q, kpages, vpages, block_table, ctx_lens, out)
-    if out is not None:
-        _require(out.shape == (rows, hq * dim) and out.dtype == BF16 and out.stride(1) == 1, f"{what}: output BF16 [rows, hq * dim]")
+    if out is not None and (out.shape != (q.shape[0], hq * dim) or out.dtype != BF16 or out.stride(1) != 1):
+        raise KernelError(f"{what}: output BF16 [rows, hq * dim]")
+    ldq = q.stride(0)
     if q.is_cuda:
-        _require(q.data_ptr() % 16 == 0 and ldq % 8 == 0 and kpages.data_ptr() % 16 == 0 and vpages.data_ptr() % 16 == 0, f"{what}: rows and pages aligned to 16 bytes")
-    return rows, ldq, blocks
+        if (q.data_ptr() | kpages.data_ptr() | vpages.data_ptr()) % 16 or ldq % 8:
+            raise KernelError(f"{what}: rows and pages aligned to 16 bytes")
+        if out is not None and (out.data_ptr() % 16 or out.stride(0) % 8):
+            raise KernelError(f"{what}: output rows aligned to 16 bytes")
+    return ldq, blocks
 
 
 def _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq, hkv, dim, scale, out):
@@ -233,66 +269,67 @@ def _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq
     return out
 
 
+def in_tiles(max_q_len: int, hq: int, hkv: int) -> bool:
+    """Whether attention of so many rows per sequence takes the kernel for prompts: FP16 tiles in shared memory for tcgen05 products of 128 rows, where
+    the other one multiplies 8 or 16 rows by codes as they are. A sequence's rows times the query heads of a kv head are what counts."""
+    return max_q_len * (hq // hkv) > 32
+
+
+def _attention(q, ldq, kpages, vpages, blocks, block_table, q_start, q_lens, ctx_lens, nq, hq, hkv, dim, scale, max_ctx, out):
+    batch, width, rows = block_table.shape[0], block_table.shape[1], q.shape[0]
+    if out is None:
+        out = torch.empty(rows, hq * dim, dtype=BF16, device=q.device)
+    if batch == 0 or rows == 0:
+        return out
+    lib, floats = _lib(), c_longlong(0)
+    most = width * PAGE if max_ctx is None else min(max_ctx, width * PAGE)
+    tiles = in_tiles(nq, hq, hkv)
+    if tiles:
+        nsplit = lib.ff_kv4_tiles_plan(batch, rows, nq, hq, hkv, dim, most, ctypes.byref(floats))
+    else:
+        nsplit = lib.ff_kv4_attn_plan(batch, hq, hkv, nq, dim, most, ctypes.byref(floats))
+        if q_start is not None and nsplit > 8:
+            nsplit, floats.value = 8, 0
+    scratch = torch.empty(floats.value, dtype=torch.float32, device=q.device) if floats.value else None
+    tail = (hq, hkv, dim, ldq, out.stride(0), width, blocks, nsplit, scale, status_tensor(q.device).data_ptr(), torch.cuda.current_stream().cuda_stream)
+    head = (q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), None if q_start is None else q_start.data_ptr(),
+            None if q_lens is None else q_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), None if scratch is None else scratch.data_ptr(), batch)
+    if tiles:
+        check(lib.ff_kv4_attn_tiles(*head, rows, nq, *tail), "ff_kv4_attn_tiles")
+    else:
+        check(lib.ff_kv4_attn_rows(*head, nq, *tail), "ff_kv4_attn_rows")
+    _count(1 if scratch is None else 2)
+    return out
+
+
 def attn_decode_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tensor, ctx_lens: torch.Tensor, hq: int, hkv: int, dim: int,
                     scale: float, nq: int = 1, max_ctx: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of ``nq`` rows per sequence over 4-bit pages: ``q`` holds ``batch * nq`` BF16 rows (head h at columns ``h * dim``; it may be the packed rows),
     ``ctx_lens[b]`` counts the keys that the last of them sees, each row before it one less. Sequences of no keys give zeros. ``max_ctx``: most keys of a
     sequence (default: what the block table has room for); fixes how the work is split, and with it the result's last bits. Returns ``[batch * nq, hq * dim]``."""
-    rows, ldq, blocks = _check_attention("attn_decode_kv4", q, kpages, vpages, block_table, ctx_lens, hq, hkv, dim, scale, out)
+    ldq, blocks = _check_attention("attn_decode_kv4", q, kpages, vpages, block_table, ctx_lens, hq, hkv, dim, scale, out)
     batch = block_table.shape[0]
-    _require(nq > 0 and rows == batch * nq, "attn_decode_kv4: q rows must equal batch * nq")
+    if nq <= 0 or q.shape[0] != batch * nq:
+        raise KernelError("attn_decode_kv4: q rows must equal batch * nq")
     if not q.is_cuda:
         return _attention_ref(q, kpages, vpages, block_table, torch.arange(batch) * nq, [nq] * batch, ctx_lens, hq, hkv, dim, scale, out)
-    if out is None:
-        out = torch.empty(rows, hq * dim, dtype=BF16, device=q.device)
-    if batch == 0:
-        return out
-    width = block_table.shape[1]
-    lib = kernels()
-    floats = c_longlong(0)
-    nsplit = lib.ff_kv4_attn_plan(batch, hq, hkv, nq, dim, min(max_ctx or width * PAGE, width * PAGE), ctypes.byref(floats))
-    scratch = torch.empty(floats.value, dtype=torch.float32, device=q.device) if floats.value else None
-    rc = lib.ff_kv4_attn_rows(ptr(q), ptr(kpages), ptr(vpages), ptr(block_table), None, None, ptr(ctx_lens), ptr(out), ptr(scratch), batch, nq, hq, hkv, dim,
-                              c_longlong(ldq), c_longlong(out.stride(0)), width, blocks, nsplit, c_float(scale), ptr(status_tensor(q.device)), stream_ptr())
-    check(rc, "ff_kv4_attn_rows")
-    _count(1 if scratch is None else 2)
-    return out
-
-
-def prompt_in_tiles(max_q_len: int, hq: int, hkv: int) -> bool:
-    """Whether :func:`attn_prefill_kv4` over so many rows takes the kernel whose keys and values are FP16 tiles in shared memory."""
-    return max_q_len * (hq // hkv) > 64
+    return _attention(q, ldq, kpages, vpages, blocks, block_table, None, None, ctx_lens, nq, hq, hkv, dim, scale, max_ctx, out)
 
 
 def attn_prefill_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor, q_lens: torch.Tensor,
-                     ctx_lens: torch.Tensor, max_q_len: int, hq: int, hkv: int, dim: int, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+                     ctx_lens: torch.Tensor, max_q_len: int, hq: int, hkv: int, dim: int, scale: float, max_ctx: int | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed rows over 4-bit pages: sequence b has the ``q_lens[b]`` rows from ``q_start[b]`` on (at most ``max_q_len``), the last of which
-    sees ``ctx_lens[b]`` keys. Rows that belong to no sequence stay as they are in ``out`` (undefined without one). Returns ``[rows, hq * dim]``."""
-    rows, ldq, blocks = _check_attention("attn_prefill_kv4", q, kpages, vpages, block_table, ctx_lens, hq, hkv, dim, scale, out)
-    batch = block_table.shape[0]
-    _check_ints("attn_prefill_kv4", batch, q_start, q_lens)
+    sees ``ctx_lens[b]`` keys. Rows that belong to no sequence stay as they are in ``out`` (undefined without one). ``max_ctx`` as in :func:`attn_decode_kv4`.
+    Returns ``[rows, hq * dim]``."""
+    ldq, blocks = _check_attention("attn_prefill_kv4", q, kpages, vpages, block_table, ctx_lens, hq, hkv, dim, scale, out)
+    _check_ints("attn_prefill_kv4", block_table.shape[0], q_start, q_lens)
     _check_device("attn_prefill_kv4", q, q_start, q_lens)
-    _require(0 < max_q_len, "attn_prefill_kv4: at least one row")
-    _require(out is None or not out.is_cuda or (out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0), "attn_prefill_kv4: output rows aligned to 16 bytes")
+    if max_q_len <= 0:
+        raise KernelError("attn_prefill_kv4: at least one row")
     if not q.is_cuda:
         return _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq, hkv, dim, scale, out)
-    if out is None:
-        out = torch.empty(rows, hq * dim, dtype=BF16, device=q.device)
-    if batch == 0 or rows == 0:
-        return out
-    if prompt_in_tiles(max_q_len, hq, hkv):
-        rc = kernels().ff_kv4_attn_tiles(ptr(q), ptr(kpages), ptr(vpages), ptr(block_table), ptr(q_start), ptr(q_lens), ptr(ctx_lens), ptr(out), batch, max_q_len,
-                                         hq, hkv, dim, c_longlong(ldq), c_longlong(out.stride(0)), block_table.shape[1], blocks, c_float(scale),
-                                         ptr(status_tensor(q.device)), stream_ptr())
-        check(rc, "ff_kv4_attn_tiles")
-        _count()
-        return out
-    rc = kernels().ff_kv4_attn_rows(ptr(q), ptr(kpages), ptr(vpages), ptr(block_table), ptr(q_start), ptr(q_lens), ptr(ctx_lens), ptr(out), None, batch, max_q_len,
-                                    hq, hkv, dim, c_longlong(ldq), c_longlong(out.stride(0)), block_table.shape[1], blocks, 1, c_float(scale),
-                                    ptr(status_tensor(q.device)), stream_ptr())
-    check(rc, "ff_kv4_attn_rows")
-    _count()
-    return out
+    return _attention(q, ldq, kpages, vpages, blocks, block_table, q_start, q_lens, ctx_lens, max_q_len, hq, hkv, dim, scale, max_ctx, out)
 
 
 # ------------------------------------------------------------------------------------------
@@ -302,24 +339,31 @@ def copy_pages(tensors: list[torch.Tensor], src: list[int], dst: list[int]) -> N
     """In every tensor (first dimension: pages; any type, widths may differ) page ``dst[i]`` becomes a copy of page ``src[i]``, in place. No page is
     written twice, and none that is written is read: those calls are refused. Keys and values of all layers go in one launch."""
     pairs = len(src)
-    _require(len(dst) == pairs, "copy_pages: as many sources as destinations")
-    _require(len(set(dst)) == pairs and not set(dst) & set(src), "copy_pages: a page that is written is neither read nor written again")
+    written = set(dst)
+    if len(dst) != pairs or len(written) != pairs or not written.isdisjoint(src):
+        raise KernelError("copy_pages: as many sources as destinations, and a page that is written is neither read nor written again")
     if pairs == 0 or not tensors:
         return
-    first = tensors[0]
+    where, least, most = tensors[0].get_device(), min(min(src), min(dst)), max(max(src), max(dst))
+    base, size = [], []
     for t in tensors:
-        _require(t.dim() > 0 and t.is_contiguous() and t.device == first.device, "copy_pages: contiguous tensors on one device")
-        _require(min(min(src), min(dst)) >= 0 and max(max(src), max(dst)) < t.shape[0], "copy_pages: a page outside the cache")
-    if not first.is_cuda:
+        n = t.shape[0] if t.dim() else 0
+        if least < 0 or most >= n:
+            raise KernelError("copy_pages: a page outside the cache")
+        if t.get_device() != where or not t.is_contiguous():
+            raise KernelError("copy_pages: contiguous tensors on one device")
+        base.append(t.data_ptr())
+        size.append(t.nbytes // n)
+    if where < 0:
         a, b = torch.tensor(src), torch.tensor(dst)
         for t in tensors:
             t[b] = t[a]
         return
-    _check_device("copy_pages", first)
-    size = [t[0].numel() * t.element_size() for t in tensors]
-    _require(all(n > 0 and n % 16 == 0 and t.data_ptr() % 16 == 0 for n, t in zip(size, tensors)), "copy_pages: pages of whole 16 bytes")
-    n = len(tensors)
-    base = (ctypes.c_ulonglong * n)(*[t.data_ptr() for t in tensors])
-    rc = kernels().ff_copy_pages(base, (c_longlong * n)(*size), n, (ctypes.c_int * pairs)(*src), (ctypes.c_int * pairs)(*dst), pairs, stream_ptr())
-    check(rc, "ff_copy_pages")
+    if where != torch.cuda.current_device():
+        raise KernelError("copy_pages: tensors on the current device")
+    if any(v <= 0 or v % 16 for v in size) or any(v % 16 for v in base):
+        raise KernelError("copy_pages: pages of whole 16 bytes")
+    n = len(base)
+    check(_lib().ff_copy_pages((ctypes.c_ulonglong * n)(*base), (c_longlong * n)(*size), n, (ctypes.c_int * pairs)(*src), (ctypes.c_int * pairs)(*dst), pairs,
+                               torch.cuda.current_stream().cuda_stream), "ff_copy_pages")
     _count(-(-n // 160) * -(-pairs // 256))

@@ -65,7 +65,7 @@ def _cache(lens, hkv, dim, seed, device, width=None, fill=0xFF):
 
 
 def _definition(q, kpages, vpages, table, spans, hq, hkv, dim, scale, rounded=False):
-    """Per row and head: the attention in 64 bits, the sum of p |v|, of p (v - lo) and of |v| of the visible keys. ``rounded``: of keys and values that are rounded to FP16."""
+    """Per row and head: the attention in 64 bits, the sum of p |v|, of p (v - lo) and, over the keys, of |v| + 2. ``rounded``: of keys and values that are rounded to FP16."""
     g = hq // hkv
     res, mag, off, tot = (torch.zeros(q.shape[0], hq, dim, dtype=torch.float64) for _ in range(4))
     for b, (at, n, ctx) in enumerate(spans):
@@ -83,7 +83,7 @@ def _definition(q, kpages, vpages, table, spans, hq, hkv, dim, scale, rounded=Fa
         res[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v).reshape(n, hq, dim)
         mag[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v.abs()).reshape(n, hq, dim)
         off[at: at + n] = torch.einsum("nhgk,hkd->nhgd", p, v - lo).reshape(n, hq, dim)
-        tot[at: at + n] = v.abs().sum(1).repeat_interleave(g, dim=0)
+        tot[at: at + n] = (v.abs() + 2).sum(1).repeat_interleave(g, dim=0)
     return [t.view(q.shape[0], hq * dim) for t in (res, mag, off, tot)]
 
 
@@ -276,10 +276,11 @@ def test_slots_and_pages_outside_the_cache_raise_the_status():
 
 
 def _close(got, want, mag, off, tot, rounded=False):
-    """Few rows: p scale is rounded to BF16 (2^-8 of p (v - lo)) and the result. Prompts in tiles (``rounded``, against keys and values that are rounded to
+    """Few rows: p scale and p are rounded to FP16 (2^-11 of p (v - lo) and of p |lo|, the latter at most p (v - lo) + p |v|), p, 8 p scale and lo below 2^-14
+    by 2^-25 (a code of 15 makes that less than 2^-24 a key), the result to BF16. Prompts in tiles (``rounded``, against keys and values that are rounded to
     FP16): p is rounded to FP16 (2^-11 of p |v|, and 2^-25 where it is below 2^-14), the result to BF16; where a value's last FP32 bit decides its FP16
     rounding, 2^-11 of p |v| more; a scale or lo below 2^-14 is off by 2^-25, and so is what they give: 17 x 2^-25 with a code of 15."""
-    tol = want.abs() * E + (mag * 2.0 ** -10 + 2.0 ** -20 + tot * 2.0 ** -25 if rounded else off * E) + mag * 2.0 ** -14
+    tol = want.abs() * E + (mag * 2.0 ** -10 if rounded else (2 * off + mag) * 2.0 ** -11) + 2.0 ** -20 + tot * 2.0 ** -25 + mag * 2.0 ** -14
     err = (got.cpu().double() - want).abs()
     assert bool((err <= tol).all()), f"{float((err / tol.clamp_min(1e-30)).max())} of the tolerance"
 
@@ -298,8 +299,9 @@ def test_decoded_rows_over_4_bit_pages(dim, hq, hkv, nq, lens):
     got = kv4_ops.attn_decode_kv4(q, kp, vp, table, ctx, hq, hkv, dim, scale, nq=nq)
     again = kv4_ops.attn_decode_kv4(q, kp, vp, table, ctx, hq, hkv, dim, scale, nq=nq)
     assert torch.equal(got, again) and ops.read_status()[0] == 0
-    want, mag, off, tot = _definition(q, kp, vp, table, [(i * nq, nq, c) for i, c in enumerate(lens)], hq, hkv, dim, scale)
-    _close(got, want, mag, off, tot)
+    tiles = kv4_ops.in_tiles(nq, hq, hkv)
+    want = _definition(q, kp, vp, table, [(i * nq, nq, c) for i, c in enumerate(lens)], hq, hkv, dim, scale, rounded=tiles)
+    _close(got, *want, rounded=tiles)
     for i, c in enumerate(lens):
         if c == 0:
             assert not got[i * nq: (i + 1) * nq].any()
@@ -325,7 +327,7 @@ def test_prompts_over_4_bit_pages(dim, hq, hkv, spans):
     scale = 1 / math.sqrt(dim)
     got = kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(starts), i32([n for n, _ in spans]), i32(lens), max(n for n, _ in spans), hq, hkv, dim, scale, out=out)
     assert got.data_ptr() == out.data_ptr() and bool((out[:2] == 3).all()) and bool((out[at:] == 3).all()) and ops.read_status()[0] == 0
-    tiles = kv4_ops.prompt_in_tiles(max(n for n, _ in spans), hq, hkv)
+    tiles = kv4_ops.in_tiles(max(n for n, _ in spans), hq, hkv)
     want = _definition(q, kp, vp, table, [(s, n, c) for s, (n, _), c in zip(starts, spans, lens)], hq, hkv, dim, scale, rounded=tiles)
     _close(got[2: at], *(t[2: at] for t in want), rounded=tiles)
 
