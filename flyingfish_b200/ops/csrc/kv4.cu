@@ -21,7 +21,7 @@ __device__ __forceinline__ uint32_t kv4_max2(uint32_t a, uint32_t b) { uint32_t 
 
 // Codes of a lane's 8 elements (w: BF16 pairs) and the (scale, lo) of their group, which four neighbouring lanes hold together. Every lane of the warp takes part.
 // ok: the group is finite and of magnitude 2^15 at most (FP16 holds what it stands for); otherwise everything is 0.
-// A code comes from an FP32 quotient that is off by less than 3e-6; only where it lies within 1e-4 of a border between two codes is it taken in FP64.
+// A code comes from an FP32 quotient that is off by less than 3e-6; only where one lies within 1e-4 of a border between two codes are they taken in FP64.
 __device__ __forceinline__ uint32_t kv4_quantise(const uint32_t (&w)[4], uint32_t& stats, bool& ok) {
   uint32_t mn = kv4_min2(kv4_min2(w[0], w[1]), kv4_min2(w[2], w[3])), mx = kv4_max2(kv4_max2(w[0], w[1]), kv4_max2(w[2], w[3]));
 #pragma unroll
@@ -33,20 +33,32 @@ __device__ __forceinline__ uint32_t kv4_quantise(const uint32_t (&w)[4], uint32_
   float lo = __uint_as_float(mn << 16) + 0.f;                    // (no negative zero)
   const float hi = __uint_as_float(mx << 16);
   ok = lo >= -32768.f && hi <= 32768.f;                          // false where one of them is no number
-  float scale = ok ? kv4_bf16_of_double(((double)hi - (double)lo) / 15.0) : 0.f;
+  // the scale: an FP32 quotient, off by less than 2^-22 of it, whose rounding to BF16 is in doubt only next to the middle between two BF16 numbers
+  float scale = __fmul_rn(__fsub_rn(hi, lo), 0.0666666667f);
+  const uint32_t low = __float_as_uint(scale) & 0xffffu;
+  if (low - 0x7ff0u <= 0x20u) scale = kv4_bf16_of_double(((double)hi - (double)lo) / 15.0);
+  else scale = kv4_bf16r(scale);
+  if (!ok) { scale = 0.f; lo = 0.f; }
   if (scale < 1.1754943508222875e-38f) scale = 0.f;              // 2^-126
-  if (!ok) lo = 0.f;
   stats = pack_bf16x2(scale, lo);
-  uint32_t word = 0;
-  if (scale > 0.f) {
-    const float inv = __frcp_rn(scale);
+  if (!(scale > 0.f)) return 0u;
+  // codes: q + 3 2^22 has the integer next to q in its last bits, of which those of a word are summed; what the upper bits add is known
+  const float inv = __frcp_rn(scale);
+  uint32_t word = 0u - (0x4b400000u + 0xb4000000u + 0x40000000u);
+  bool doubt = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    const float q = __fmul_rn(__fsub_rn(x, lo), inv), r = __fadd_rn(q, 12582912.f);
+    doubt = doubt || fabsf(__fsub_rn(q, __fsub_rn(r, 12582912.f))) > 0.4999f;
+    word += __float_as_uint(r) << (4 * (e / 2 + 4 * (e & 1)));
+  }
+  if (doubt) {
+    word = 0u;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-      const float q = __fmul_rn(__fsub_rn(x, lo), inv);
-      int c = __float2int_rn(q);
-      if (fabsf(fabsf(q - (float)c) - 0.5f) < 1e-4f) c = __double2int_rn(((double)x - (double)lo) / (double)scale);
-      word |= (uint32_t)min(15, c) << (4 * (e / 2 + 4 * (e & 1)));
+      word |= (uint32_t)min(15, __double2int_rn(((double)x - (double)lo) / (double)scale)) << (4 * (e / 2 + 4 * (e & 1)));
     }
   }
   return word;
@@ -54,97 +66,114 @@ __device__ __forceinline__ uint32_t kv4_quantise(const uint32_t (&w)[4], uint32_
 
 // Rows of packed queries, keys and values: queries and keys are RMS-normed per head (NORM) and turned (a table of cosines and sines), queries go to
 // qout, keys and values into the pages of the row's slot. A head is D / 8 lanes with 8 elements each, so a turn's partner is half a head's lanes
-// away and a group of 32 elements is 4 lanes; such a set of lanes walks heads of one row with the row's cosines and sines in registers, four heads on their way at
+// away and a group of 32 elements is 4 lanes; such a set of lanes walks heads of a row with the row's cosines and sines in registers, five heads on their way at
 // once. Norm and turn round as the BF16 cache's kernel does: every product and sum to BF16 (packed instructions; a sum of two BF16 numbers that FP32 does not
 // hold has a term too small to matter). Bound by DRAM; few rows are spread over CTAs by heads.
-constexpr int WRITE_THREADS = 256, WRITE_HEADS = 4;
+constexpr int WRITE_THREADS = 256, WRITE_HEADS = 5;
 template <int D, bool NORM>
-__global__ void __launch_bounds__(WRITE_THREADS)
+__global__ void __launch_bounds__(WRITE_THREADS, 4)
 kv4_write_kernel(const __nv_bfloat16* __restrict__ qkv, const int* __restrict__ slots, uint8_t* __restrict__ kpages, uint8_t* __restrict__ vpages,
                  const float2* __restrict__ cos_sin, int rhalf, const __nv_bfloat16* __restrict__ q_weight, const __nv_bfloat16* __restrict__ k_weight,
-                 float eps, __nv_bfloat16* __restrict__ qout, int hq, int hkv, long long ld, int num_blocks, int* status) {
+                 float eps, __nv_bfloat16* __restrict__ qout, int rows, int hq, int hkv, long long ld, int num_blocks, int* status) {
   pdl_trigger();
   pdl_wait();
   constexpr int LANES = D / 8, SETS = WRITE_THREADS / LANES;
-  const int c = threadIdx.x & (LANES - 1), row = blockIdx.x;
+  const int c = threadIdx.x & (LANES - 1);
   const int first = qout == nullptr ? hq : 0, heads = hq + 2 * hkv;               // nothing to do for queries?
-  const int slot = slots[row];
-  const int block = slot / KV4_PAGE, k = slot - block * KV4_PAGE;
-  if (slot >= 0 && block >= num_blocks && threadIdx.x == 0) set_status(status, KID_KV, FF_ERR_BOUNDS, row, slot);
-  const bool store = slot >= 0 && block < num_blocks, upper = c >= LANES / 2, turn = cos_sin != nullptr;
-  uint32_t cs[4], sn[4];
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int slot = slots[row];
+    const int block = slot / KV4_PAGE, k = slot - block * KV4_PAGE;
+    if (slot >= 0 && block >= num_blocks && threadIdx.x == 0) set_status(status, KID_KV, FF_ERR_BOUNDS, row, slot);
+    const bool store = slot >= 0 && block < num_blocks, upper = c >= LANES / 2, turn = cos_sin != nullptr;
+    uint32_t cs[4], sn[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { cs[i] = 0x3f803f80u; sn[i] = 0u; }
-  if (turn) {
-    // elements of a head's halves from rhalf on stay: cosine 1, sine 0 would give x + 0, which is x but for a zero's sign
-    const int k0 = (c & (LANES / 2 - 1)) * 8;
-    float x[8], y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 t = k0 + i < rhalf ? cos_sin[(size_t)row * rhalf + k0 + i] : make_float2(1.f, 0.f);
-      x[i] = t.x; y[i] = upper ? t.y : -t.y;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { cs[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]); sn[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]); }
-  }
-  const int stays = rhalf - (c & (LANES / 2 - 1)) * 8;                             // elements of the lane from here on do not turn
-  const int set = blockIdx.y * SETS + threadIdx.x / LANES, step = gridDim.y * SETS;
-  for (int base = first + set; base - set < heads; base += WRITE_HEADS * step) {   // the same number of rounds for every lane of a warp
-    uint4 v[WRITE_HEADS];
-#pragma unroll
-    for (int u = 0; u < WRITE_HEADS; ++u) {
-      const int head = base + u * step;
-      v[u] = make_uint4(0, 0, 0, 0);
-      if (head < heads) v[u] = reinterpret_cast<const uint4*>(qkv + (size_t)row * ld + (size_t)head * D)[c];
-    }
-#pragma unroll
-    for (int u = 0; u < WRITE_HEADS; ++u) {
-      const int head = base + u * step;
-      if (base - set + u * step >= heads) break;                                   // (for all lanes)
-      const int part = head < hq ? 0 : (head < hq + hkv ? 1 : 2);
-      const bool live = head < heads;
-      uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-      if (NORM) {
-        float x[8], ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { const float2 p = unpack_bf16x2(w[i]); x[2 * i] = p.x; x[2 * i + 1] = p.y; ss += p.x * p.x + p.y * p.y; }
-#pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (part < 2) {
-          const float rstd = rsqrtf(ss / (float)D + eps);
-          const uint4 g = __ldg(reinterpret_cast<const uint4*>(part == 0 ? q_weight : k_weight) + c);
-          const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { const float2 p = unpack_bf16x2(gw[i]); w[i] = pack_bf16x2(x[2 * i] * rstd * p.x, x[2 * i + 1] * rstd * p.y); }
-        }
-      }
-      if (turn) {
+    for (int i = 0; i < 4; ++i) { cs[i] = 0x3f803f80u; sn[i] = 0u; }
+    if (turn) {
+      // elements of a head's halves from rhalf on stay: cosine 1, sine 0 would give x + 0, which is x but for a zero's sign
+      const int k0 = (c & (LANES / 2 - 1)) * 8;
+      float x[8], y[8];
+      const float2* table = cos_sin + (size_t)row * rhalf + k0;
+      if (k0 + 8 <= rhalf && (rhalf & 1) == 0) {                     // (even rows of a 16-byte aligned table)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], LANES / 2);
-          const uint32_t t = kv4_add2(kv4_mul2(w[i], cs[i]), kv4_mul2(other, sn[i]));
-          const uint32_t keep = 2 * i >= stays ? 0xffffffffu : 2 * i + 1 >= stays ? 0xffff0000u : 0u;
-          if (part < 2) w[i] = (t & ~keep) | (w[i] & keep);
+          const float4 t = reinterpret_cast<const float4*>(table)[i];
+          x[2 * i] = t.x; y[2 * i] = t.y; x[2 * i + 1] = t.z; y[2 * i + 1] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 t = k0 + i < rhalf ? table[i] : make_float2(1.f, 0.f);
+          x[i] = t.x; y[i] = t.y;
         }
       }
-      if (part == 0 && live && qout != nullptr) reinterpret_cast<uint4*>(qout + ((size_t)row * hq + head) * D)[c] = make_uint4(w[0], w[1], w[2], w[3]);
-      const bool mine = part > 0 && live && store;
-      if (__any_sync(0xffffffffu, mine)) {
-        uint32_t stats;
-        bool ok;
-        const uint32_t word = kv4_quantise(w, stats, ok);
-        if (mine) {
-          if (!ok && (c & 3) == 0) set_status(status, KID_KV, FF_ERR_NONFINITE, row, head);
-          const int h = head - (part == 1 ? hq : hq + hkv);
-          uint8_t* page = (part == 1 ? kpages : vpages) + ((size_t)block * hkv + h) * kv4_page_bytes(D);
-          const int j = c >> 2, y = c & 3;
-          if (part == 1) {
-            reinterpret_cast<uint32_t*>(page + k * (D / 2))[y * (D / 32) + j] = word;
-          } else {
-            *reinterpret_cast<uint16_t*>(page + kv4_value_at<D>(k, 2 * y, j)) = (uint16_t)(word & 0xffffu);
-            *reinterpret_cast<uint16_t*>(page + kv4_value_at<D>(k, 2 * y + 1, j)) = (uint16_t)(word >> 16);
+      if (!upper) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = -y[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { cs[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]); sn[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]); }
+    }
+    const int stays = rhalf - (c & (LANES / 2 - 1)) * 8;                             // elements of the lane from here on do not turn
+    const __nv_bfloat16* const in = qkv + (size_t)row * ld + c * 8;
+    __nv_bfloat16* const qo = qout + (size_t)row * hq * D + c * 8;
+    const int set = blockIdx.y * SETS + threadIdx.x / LANES, step = gridDim.y * SETS;
+    for (int base = first + set; base - set < heads; base += WRITE_HEADS * step) {   // the same number of rounds for every lane of a warp
+      uint4 v[WRITE_HEADS];
+#pragma unroll
+      for (int u = 0; u < WRITE_HEADS; ++u) {
+        const int head = base + u * step;
+        v[u] = make_uint4(0, 0, 0, 0);
+        if (head < heads) v[u] = *reinterpret_cast<const uint4*>(in + head * D);
+      }
+#pragma unroll
+      for (int u = 0; u < WRITE_HEADS; ++u) {
+        const int head = base + u * step;
+        if (base - set + u * step >= heads) break;                                   // (for all lanes)
+        const int part = head < hq ? 0 : (head < hq + hkv ? 1 : 2);
+        const bool live = head < heads;
+        uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        if (NORM) {
+          float x[8], ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { const float2 p = unpack_bf16x2(w[i]); x[2 * i] = p.x; x[2 * i + 1] = p.y; ss += p.x * p.x + p.y * p.y; }
+#pragma unroll
+          for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (part < 2) {
+            const float rstd = rsqrtf(ss / (float)D + eps);
+            const uint4 g = __ldg(reinterpret_cast<const uint4*>(part == 0 ? q_weight : k_weight) + c);
+            const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { const float2 p = unpack_bf16x2(gw[i]); w[i] = pack_bf16x2(x[2 * i] * rstd * p.x, x[2 * i + 1] * rstd * p.y); }
           }
-          if (y == 0) reinterpret_cast<uint32_t*>(page + kv4_code_bytes(D))[k * (D / 32) + j] = stats;
+        }
+        if (turn) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], LANES / 2);
+            const uint32_t t = kv4_add2(kv4_mul2(w[i], cs[i]), kv4_mul2(other, sn[i]));
+            const uint32_t keep = 2 * i >= stays ? 0xffffffffu : 2 * i + 1 >= stays ? 0xffff0000u : 0u;
+            if (part < 2) w[i] = (t & ~keep) | (w[i] & keep);
+          }
+        }
+        if (part == 0 && live && qout != nullptr) *reinterpret_cast<uint4*>(qo + head * D) = make_uint4(w[0], w[1], w[2], w[3]);
+        const bool mine = part > 0 && live && store;
+        if (__any_sync(0xffffffffu, mine)) {
+          uint32_t stats;
+          bool ok;
+          const uint32_t word = kv4_quantise(w, stats, ok);
+          if (mine) {
+            if (!ok && (c & 3) == 0) set_status(status, KID_KV, FF_ERR_NONFINITE, row, head);
+            const int h = head - (part == 1 ? hq : hq + hkv);
+            uint8_t* page = (part == 1 ? kpages : vpages) + ((size_t)block * hkv + h) * kv4_page_bytes(D);
+            const int j = c >> 2, y = c & 3;
+            if (part == 1) {
+              reinterpret_cast<uint32_t*>(page + k * (D / 2))[y * (D / 32) + j] = word;
+            } else {
+              *reinterpret_cast<uint16_t*>(page + kv4_value_at<D>(k, 2 * y, j)) = (uint16_t)(word & 0xffffu);
+              *reinterpret_cast<uint16_t*>(page + kv4_value_at<D>(k, 2 * y + 1, j)) = (uint16_t)(word >> 16);
+            }
+            if (y == 0) reinterpret_cast<uint32_t*>(page + kv4_code_bytes(D))[k * (D / 32) + j] = stats;
+          }
         }
       }
     }
@@ -223,16 +252,16 @@ FF_EXPORT int ff_kv4_write(const void* qkv, const int* slots, void* kpages, void
   if (ld < (long long)(hq + 2 * hkv) * dim || rhalf < 0 || rhalf > dim / 2) return FF_HOST_BAD_SHAPE;
   if ((q_weight == nullptr) != (k_weight == nullptr) || (qout == nullptr && (cos_sin != nullptr || q_weight != nullptr))) return FF_HOST_BAD_SHAPE;
   if (ld % 8 || ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages) | reinterpret_cast<uintptr_t>(qout) |
-                  reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight)) & 15) || (reinterpret_cast<uintptr_t>(cos_sin) & 7))
+                  reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight)) & 15) || (reinterpret_cast<uintptr_t>(cos_sin) & 15))
     return FF_HOST_BAD_ALIGN;
   const int sets = WRITE_THREADS / (dim / 8), heads = (qout == nullptr ? 0 : hq) + 2 * hkv;
-  // few rows: a CTA for every set of heads that its lanes take at once; many: four rounds' heads in one, whose loads are on their way together
+  // few rows: a CTA for every set of heads that its lanes take at once; many: a row's heads in one, whose loads are on their way together
   const int at_once = rows >= 4 * sm_count() ? sets * WRITE_HEADS : sets, y = (heads + at_once - 1) / at_once;
   if (y > 65535) return FF_HOST_TOO_LARGE;
   auto kern = q_weight ? (dim == 128 ? kv4_write_kernel<128, true> : kv4_write_kernel<64, true>)
                        : (dim == 128 ? kv4_write_kernel<128, false> : kv4_write_kernel<64, false>);
-  return launch_pdl(kern, dim3((unsigned)rows, y), dim3(WRITE_THREADS), 0, s, 0, (const __nv_bfloat16*)qkv, slots, (uint8_t*)kpages, (uint8_t*)vpages, (const float2*)cos_sin,
-                    rhalf, (const __nv_bfloat16*)q_weight, (const __nv_bfloat16*)k_weight, eps, (__nv_bfloat16*)qout, hq, hkv, ld, num_blocks, status);
+  return launch_pdl(kern, dim3((unsigned)(rows < 16 * sm_count() ? rows : 16 * sm_count()), y), dim3(WRITE_THREADS), 0, s, 0, (const __nv_bfloat16*)qkv, slots, (uint8_t*)kpages, (uint8_t*)vpages, (const float2*)cos_sin,
+                    rhalf, (const __nv_bfloat16*)q_weight, (const __nv_bfloat16*)k_weight, eps, (__nv_bfloat16*)qout, rows, hq, hkv, ld, num_blocks, status);
 }
 
 FF_EXPORT int ff_kv4_read(const void* kpages, const void* vpages, const int* slots, void* kout, void* vout, int rows, int hkv, int dim, int num_blocks,

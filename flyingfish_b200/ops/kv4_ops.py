@@ -107,7 +107,7 @@ def _check_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) 
     for t in others:
         if t is not None and t.device != device:
             raise KernelError(f"{what}: tensors on one device")
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
+    if device.type == "cuda" and device.index != _device():
         raise KernelError(f"{what}: tensors on the current device")
 
 
@@ -115,6 +115,19 @@ def _check_ints(what: str, n: int, *tensors: torch.Tensor) -> None:
     for t in tensors:
         if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
             raise KernelError(f"{what}: int32 metadata, one number each")
+
+
+# The current stream's handle and the current device as numbers: what torch.cuda.current_stream().cuda_stream and torch.cuda.current_device() give, without the 5 us
+# of a stream object.
+_raw_stream, _raw_device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+
+
+def _device() -> int:
+    return torch.cuda.current_device() if _raw_device is None else _raw_device()
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(_device())
 
 
 _bound: ctypes.CDLL | None = None
@@ -155,7 +168,7 @@ def write_kv4(qkv: torch.Tensor, slots: torch.Tensor, kpages: torch.Tensor, vpag
     _check_ints("write_kv4", rows, slots)
     if cos_sin is not None:
         _require(cos_sin.dtype == torch.float32 and cos_sin.dim() == 3 and cos_sin.shape[0] == rows and 0 < cos_sin.shape[1] <= dim // 2 and cos_sin.shape[2] == 2
-                 and cos_sin.is_contiguous(), "write_kv4: cosines and sines float32 [rows, n, 2]")
+                 and cos_sin.is_contiguous() and cos_sin.data_ptr() % 16 == 0, "write_kv4: cosines and sines float32 [rows, n, 2], aligned to 16 bytes")
     for w in (q_norm, k_norm):
         _require(w is None or (w.dtype == BF16 and w.numel() == dim and w.is_contiguous()), "write_kv4: head norms BF16 [dim]")
     _check_device("write_kv4", qkv, slots, kpages, vpages, cos_sin, q_norm, k_norm)
@@ -189,7 +202,7 @@ def write_kv4(qkv: torch.Tensor, slots: torch.Tensor, kpages: torch.Tensor, vpag
     at = lambda t: None if t is None else t.data_ptr()
     check(_lib().ff_kv4_write(qkv.data_ptr(), slots.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), at(cos_sin), 0 if cos_sin is None else cos_sin.shape[1], at(q_norm),
                               at(k_norm), eps, None if plain else q.data_ptr(), rows, hq, hkv, dim, ld, blocks, status_tensor(qkv.device).data_ptr(),
-                              torch.cuda.current_stream().cuda_stream), "ff_kv4_write")
+                              _stream()), "ff_kv4_write")
     _count()
     return q
 
@@ -211,7 +224,7 @@ def read_kv4(kpages: torch.Tensor, vpages: torch.Tensor, slots: torch.Tensor, di
     k, v = (torch.empty(rows, hkv, dim, dtype=BF16, device=kpages.device) for _ in range(2))
     if rows:
         check(_lib().ff_kv4_read(kpages.data_ptr(), vpages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), rows, hkv, dim, blocks,
-                                 status_tensor(kpages.device).data_ptr(), torch.cuda.current_stream().cuda_stream), "ff_kv4_read")
+                                 status_tensor(kpages.device).data_ptr(), _stream()), "ff_kv4_read")
         _count()
     return k, v
 
@@ -291,7 +304,7 @@ def _attention(q, ldq, kpages, vpages, blocks, block_table, q_start, q_lens, ctx
         if q_start is not None and nsplit > 8:
             nsplit, floats.value = 8, 0
     scratch = torch.empty(floats.value, dtype=torch.float32, device=q.device) if floats.value else None
-    tail = (hq, hkv, dim, ldq, out.stride(0), width, blocks, nsplit, scale, status_tensor(q.device).data_ptr(), torch.cuda.current_stream().cuda_stream)
+    tail = (hq, hkv, dim, ldq, out.stride(0), width, blocks, nsplit, scale, status_tensor(q.device).data_ptr(), _stream())
     head = (q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), None if q_start is None else q_start.data_ptr(),
             None if q_lens is None else q_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), None if scratch is None else scratch.data_ptr(), batch)
     if tiles:
@@ -359,11 +372,11 @@ def copy_pages(tensors: list[torch.Tensor], src: list[int], dst: list[int]) -> N
         for t in tensors:
             t[b] = t[a]
         return
-    if where != torch.cuda.current_device():
+    if where != _device():
         raise KernelError("copy_pages: tensors on the current device")
     if any(v <= 0 or v % 16 for v in size) or any(v % 16 for v in base):
         raise KernelError("copy_pages: pages of whole 16 bytes")
     n = len(base)
     check(_lib().ff_copy_pages((ctypes.c_ulonglong * n)(*base), (c_longlong * n)(*size), n, (ctypes.c_int * pairs)(*src), (ctypes.c_int * pairs)(*dst), pairs,
-                               torch.cuda.current_stream().cuda_stream), "ff_copy_pages")
+                               _stream()), "ff_copy_pages")
     _count(-(-n // 160) * -(-pairs // 256))
