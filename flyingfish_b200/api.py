@@ -303,6 +303,10 @@ class Model:
                        on_token=None, sampling=None, adapter=None) -> list[list[int]]:
         return self.engine.generate(prompts, max_new_tokens, self.spec.eos_token_id, ignore_eos, on_token, sampling, adapter)
 
+    def generate_samples(self, prompt: list[int], settings: list, max_new_tokens: int, ignore_eos: bool = True, adapter: str | None = None) -> list[list[int]]:
+        """Continuations of one prompt by a list of ``engine.sampling.Sampling``: the prompt is computed once, its cache blocks are shared."""
+        return self.engine.sample(prompt, settings, max_new_tokens, None if ignore_eos else self.spec.eos_token_id, adapter)
+
 
 def generate_plain(model: Model, ids: list[int], count: int, ignore_eos: bool = False, graph: bool = True,
                    on_token=None, sampling=None, adapter: str | None = None) -> GenerationOutput:

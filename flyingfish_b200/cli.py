@@ -42,7 +42,8 @@ def _global_parser() -> argparse.ArgumentParser:
     p.add_argument("--spec-budget", choices=["chain", "tree16", "tree32", "tree64"], default="chain")
     p.add_argument("--spec-graph", type=lambda s: s.lower() != "false", default=True)
     p.add_argument("--prefix-cache", type=lambda s: s.lower() == "true", default=False)
-    p.add_argument("--kv-format", choices=["bf16", "affine8"], default="bf16")
+    p.add_argument("--kv-format", choices=["bf16", "affine8", "affine4"], default="bf16",
+                   help="affine8: groups older than the newest tokens as 8-bit codes; affine4: 4-bit pages throughout")
     p.add_argument("--kv-recent", type=int, default=2048, help="affine8: newest tokens kept in BF16 (older 128-token groups are sealed)")
     p.add_argument("--runtime-dir", default=os.environ.get("FLYINGFISH_RUNTIME_DIR"))
     p.add_argument("--dram-gb-s", type=float, default=6550.0)
@@ -220,7 +221,9 @@ def resolve_mtp_depth(requested: int | None, has_mtp: bool, arch: str) -> int:
 
 def check_flags(args) -> None:
     """Every flag either changes behaviour or is refused: nothing is parsed and then ignored."""
-    if args.kv_format != "bf16":
+    if args.kv_format == "affine4" and (args.spec_budget != "chain" or args.command in DSPARK_TOOLS + ("verify-spec", "bench-spec", "profile-spec")):
+        raise SystemExit("--kv-format affine4 does not combine with tree verification (rows of 4-bit pages are not moved)")
+    if args.kv_format == "affine8":
         # the sealed 8-bit store is read by plain decode steps only
         if args.draft_model or args.prefix_cache or args.command in DSPARK_TOOLS + ("verify-spec", "bench-spec", "profile-spec") \
                 or (args.command == "serve" and getattr(args, "mtp", None) not in (None, 0)):
@@ -415,6 +418,8 @@ def cmd_generate(args) -> dict:
         store = model.prefix_store()
         if store is not None:
             extra["prefix_cache"] = {"hits": store.hits, "stored": store.stored, "dir": str(store.root)}
+    if model.engine.kv.kv_format == "affine4":
+        extra = dict(extra, kv={"format": "affine4", "block_bytes": sum(t[0].numel() for t in model.engine.kv.k + model.engine.kv.v)})
     if model.engine.kv.compact is not None:
         c = model.engine.kv.compact
         extra = dict(extra, kv={"format": "affine8", "recent": c.recent, **c.stats})

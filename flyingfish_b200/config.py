@@ -1097,7 +1097,7 @@ class Settings:
     spec_budget: str = "chain"            # chain | tree16 | tree32 | tree64
     spec_graph: bool = True
     prefix_cache: bool = False
-    kv_format: str = "bf16"               # bf16 | affine8
+    kv_format: str = "bf16"               # bf16 | affine8 (older groups as 8-bit codes) | affine4 (4-bit pages)
     kv_recent: int = 2048                 # affine8: tokens behind the newest that stay BF16 (groups older than that are sealed)
     runtime_dir: str | None = None
     dram_gb_s: float = 6550.0             # roofline denominators (measured on the target box)

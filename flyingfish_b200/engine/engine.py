@@ -20,6 +20,7 @@ import torch
 
 from .. import ops
 from ..config import ModelSpec, Settings
+from ..models.decoder import DecoderModel
 from ..ops import sample_ops
 from ..utils.log import log_json
 from .batch import BatchLayout, ForwardBatch
@@ -31,6 +32,7 @@ class EnginePoisoned(RuntimeError):
     pass
 
 
+AFFINE4_NEEDS = "--kv-format affine4 needs a causal BF16 GQA decoder with heads of 64 or 128 and 64-token blocks"
 DECODE_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
 
 
@@ -97,7 +99,7 @@ class Engine:
             self.kv = PagedKVCache(spec.layers, 1, 8, num_blocks, settings.kv_block, dtype, self.device, v_head_dim=0)
         else:
             self.kv = PagedKVCache(spec.layers, hkv, spec.head_dim, num_blocks, settings.kv_block, dtype, self.device,
-                                   geometry=spec.kv_geometry())
+                                   geometry=spec.kv_geometry(), kv_format=self._kv_format(model, spec, settings, dtype))
         # 8-bit store behind the block cache: groups that leave the recent window are sealed after every step
         self.max_groups = 0
         if settings.kv_format == "affine8":
@@ -108,6 +110,8 @@ class Engine:
             self.kv.compact = CompactKV(spec.layers, hkv, spec.head_dim, max(num_blocks // 2, 1), self.device,
                                         recent=settings.kv_recent)
             self.max_groups = max(settings.capacity // 128, 1)
+        if settings.kv_format == "affine4" and self.kv.kv_format != "affine4":
+            raise ValueError(AFFINE4_NEEDS)
         self.max_blocks = (settings.capacity + settings.kv_block - 1) // settings.kv_block
         self.max_batch = max(settings.max_batch, 1)
         self.max_prefill_rows = max_prefill_rows
@@ -142,7 +146,46 @@ class Engine:
                       "captures": 0, "h2d_bytes": 0, "d2h_bytes": 0}
         self.fail_next_step = False      # host-side fault injection hook for tests
 
+    @staticmethod
+    def _kv_format(model, spec: ModelSpec, settings: Settings, dtype: torch.dtype) -> str:
+        """The block cache's format; refuses 4-bit pages where the model's attention does not read them."""
+        if settings.kv_format != "affine4":
+            return "bf16"
+        if type(model)._attention is not DecoderModel._attention or type(model).hidden_states is not DecoderModel.hidden_states or model.bidirectional \
+                or spec.layer_specs is not None or spec.head_dim not in (64, 128) or settings.kv_block != 64 or dtype != torch.bfloat16:
+            raise ValueError(AFFINE4_NEEDS)
+        return "affine4"
+
     # -- sequence management ---------------------------------------------------------------
+    def fork(self, seq: Sequence, sampling: Sampling | None = None, again: bool = False) -> Sequence:
+        """A second sequence that goes on from where ``seq`` stands, sharing its cache blocks (the block it is inside of is copied). ``sampling``: settings of its own
+        (default: those of ``seq``, whose random numbers it then draws too). ``again``: it goes on from the end of the prompt instead and chooses its first token
+        itself: the last prompt token is computed once more by its :meth:`prefill`. The prompt of ``seq`` has to be complete."""
+        self._check()
+        if self.state_slots is not None or getattr(self.model, "owns_token_state", False):
+            raise ValueError("sequences of a model with state of its own are not forked")
+        if self.kv.compact is not None:
+            raise ValueError("sequences with sealed 8-bit groups are not forked")
+        if self.seqs.get(seq.seq_id) is not seq or seq.prefilled < len(seq.prompt):
+            raise ValueError("a live sequence is forked once its prompt is complete")
+        if again and self.whole_prompt:
+            raise ValueError("this model computes a prompt only as a whole")
+        if sampling is not None and sampling.temperature > 0 and self.model.w.tp.size > 1:
+            raise ValueError("sampling is not available with tensor parallelism")
+        sid = self._next_id
+        self.kv.fork(seq.seq_id, sid, len(seq.prompt) - 1 if again else None)
+        self._next_id += 1
+        s = Sequence(sid, list(seq.prompt), adapter=seq.adapter, mm_positions=seq.mm_positions, mm_embeds=seq.mm_embeds)
+        s.prefilled = len(seq.prompt) - 1 if again else seq.prefilled
+        if not again:
+            s.output, s.pending, s.finished = list(seq.output), seq.pending, seq.finished
+        settings = sampling if sampling is not None else seq.draws.settings if seq.draws is not None else None
+        if settings is not None and settings.temperature > 0:
+            s.draws = Draws(settings)
+        self.seqs[sid] = s
+        self._special += s.special
+        return s
+
     def add_sequence(self, prompt: list[int], mm_positions: list[int] | None = None,
                      mm_embeds: torch.Tensor | None = None, sampling: Sampling | None = None, adapter: str | None = None) -> Sequence:
         """``mm_positions`` / ``mm_embeds``: prompt indices whose embedding rows are supplied by the caller (the
@@ -822,6 +865,8 @@ class Engine:
         token after every row."""
         self._check()
         self._no_compact("tree verification")
+        if self.kv.kv_format == "affine4":
+            raise ValueError("tree verification is not available with --kv-format affine4")
         self._plain_only([seq], "tree verification")
         try:
             kvs = self.kv.seqs[seq.seq_id]
@@ -889,6 +934,28 @@ class Engine:
                 raise ops.DeviceStatusError(*code)
 
     # -- convenience ---------------------------------------------------------------------------
+    def sample(self, prompt: list[int], settings: list[Sampling], max_new_tokens: int, eos: int | None = None, adapter: str | None = None) -> list[list[int]]:
+        """Continuations of one prompt, one per entry of ``settings``, drawn side by side: the prompt is computed once and its cache blocks are shared. A
+        continuation ends after ``eos`` or ``max_new_tokens``."""
+        if not settings:
+            return []
+        seqs = [self.add_sequence(prompt, sampling=settings[0], adapter=adapter)]
+        try:
+            self.prefill(seqs)
+            for h in settings[1:]:
+                seqs.append(self.fork(seqs[0], h, again=True))
+            if len(seqs) > 1:
+                self.prefill(seqs[1:])
+            live = seqs
+            while True:
+                live = [s for s in live if len(s.output) < max_new_tokens and (eos is None or s.output[-1] != eos)]
+                if not live:
+                    return [list(s.output) for s in seqs]
+                self.decode(live)
+        finally:
+            for s in seqs:
+                self.free_sequence(s.seq_id)
+
     def generate(self, prompts: list[list[int]], max_new_tokens: int, eos: int | None = None,
                  ignore_eos: bool = True, on_token=None, sampling=None, adapter=None) -> list[list[int]]:
         """Generation for a batch of prompts, greedy by default; returns the generated ids per prompt

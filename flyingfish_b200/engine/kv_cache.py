@@ -10,6 +10,10 @@ and speculative rows can be rolled back by truncating a sequence's length.
 The device tensors are zero-initialised: attention tiles always read whole 64-token blocks and
 multiply masked probabilities (exact zeros) with whatever the tail of the last block holds, so
 that tail must be finite.
+
+A sequence can be forked: the fork shares its whole blocks and gets a copy of the block it is inside of. Blocks that are shared
+are never written: a sequence that comes to stand inside one (it was taken back) gets a copy before its next row.
+With the format ``affine4`` the blocks are the 4-bit pages of ``ops.kv4_ops``.
 """
 from __future__ import annotations
 
@@ -30,6 +34,7 @@ class BlockAllocator:
         self.num_blocks = num_blocks
         self._free = list(range(num_blocks - 1, -1, -1))
         self._ref = [0] * num_blocks
+        self.shared = 0                      # blocks of more than one owner
 
     @property
     def free_blocks(self) -> int:
@@ -45,10 +50,12 @@ class BlockAllocator:
     def share(self, block: int) -> None:
         assert self._ref[block] > 0, "sharing a free block"
         self._ref[block] += 1
+        self.shared += self._ref[block] == 2
 
     def release(self, block: int) -> None:
         assert self._ref[block] > 0, "double free of a KV block"
         self._ref[block] -= 1
+        self.shared -= self._ref[block] == 1
         if self._ref[block] == 0:
             self._free.append(block)
 
@@ -69,9 +76,10 @@ class PagedKVCache:
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, num_blocks: int, block_size: int = 64,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cpu",
-                 v_head_dim: int | None = None, geometry: list[tuple[int, int, int]] | None = None):
+                 v_head_dim: int | None = None, geometry: list[tuple[int, int, int]] | None = None, kv_format: str = "bf16"):
         """``geometry``: (kv heads, key width, value width) per layer, for models whose layers differ; otherwise every
-        layer has ``kv_heads`` heads of ``head_dim`` (values: ``v_head_dim``)."""
+        layer has ``kv_heads`` heads of ``head_dim`` (values: ``v_head_dim``). ``kv_format`` ``affine4``: 4-bit pages (64-token blocks, heads of
+        64 or 128); other formats keep blocks of ``dtype``."""
         self.layers, self.kv_heads, self.head_dim = layers, kv_heads, head_dim
         self.block_size, self.num_blocks = block_size, num_blocks
         self.device = torch.device(device)
@@ -80,6 +88,11 @@ class PagedKVCache:
         assert len(self.geometry) == layers, "one cache geometry per layer"
         self.uniform = all(g == self.geometry[0] for g in self.geometry)
         zeros = lambda h, d: torch.zeros(num_blocks, h, block_size, d, dtype=dtype, device=self.device) if d > 0 else None
+        self.kv_format = "affine4" if kv_format == "affine4" else "bf16"
+        if self.kv_format == "affine4":
+            from ..ops import kv4_ops
+            assert block_size == kv4_ops.PAGE and all(dk == dv for _, dk, dv in self.geometry), "4-bit pages: 64-token blocks, keys as wide as values"
+            zeros = lambda h, d: kv4_ops.new_pages(num_blocks, h, d, self.device)
         self.k = [zeros(h, dk) for h, dk, _ in self.geometry]
         self.v = [zeros(h, dv) for h, _, dv in self.geometry]
         self.alloc = BlockAllocator(num_blocks)
@@ -112,7 +125,30 @@ class PagedKVCache:
         s = self.seqs[seq_id]
         total = s.length + new_tokens
         need = (total + self.block_size - 1) // self.block_size
-        return max(0, need - len(s.blocks))
+        return max(0, need - len(s.blocks)) + (1 if new_tokens > 0 and self.alloc.shared and self._inside_shared(s) else 0)
+
+    def _inside_shared(self, s: SequenceKV) -> bool:
+        """Whether the sequence's next row would go into a block that is not its own alone."""
+        at = s.length // self.block_size
+        return s.length % self.block_size != 0 and s.blocks[at] >= 0 and self.alloc.refcount(s.blocks[at]) > 1
+
+    def _own(self, seqs: list[SequenceKV]) -> None:
+        """Copies of the shared blocks that these sequences stand inside of (the blocks have been counted)."""
+        src, dst = [], []
+        for s in seqs:
+            if self._inside_shared(s):
+                at = s.length // self.block_size
+                src.append(s.blocks[at])
+                dst.append(self.alloc.alloc())
+                self.alloc.release(src[-1])
+                s.blocks[at] = dst[-1]
+        if src:
+            self.copy_blocks(src, dst)
+
+    def copy_blocks(self, src: list[int], dst: list[int]) -> None:
+        """Blocks ``src`` copied to blocks ``dst``, keys and values of every layer (``kv4_ops.copy_pages``: one launch)."""
+        from ..ops import kv4_ops
+        kv4_ops.copy_pages([t for pair in zip(self.k, self.v) for t in pair if t is not None], src, dst)
 
     def reserve(self, seq_id: int, new_tokens: int, list_slots: bool = True) -> list[int]:
         """Make room for ``new_tokens`` more tokens and return their slots
@@ -121,7 +157,9 @@ class PagedKVCache:
         need = self.blocks_needed(seq_id, new_tokens)
         if need > self.alloc.free_blocks:
             raise OutOfBlocks(f"sequence {seq_id} needs {need} blocks, {self.alloc.free_blocks} free")
-        for _ in range(need):
+        if self.alloc.shared and new_tokens > 0:
+            self._own([s])
+        for _ in range((s.length + new_tokens + self.block_size - 1) // self.block_size - len(s.blocks)):
             s.blocks.append(self.alloc.alloc())
         if not list_slots:
             return []
@@ -142,9 +180,12 @@ class PagedKVCache:
         the tokens' slots (int32)."""
         held, bs = [self.seqs[i] for i in seq_ids], self.block_size
         short = [s for s in held if s.length >= len(s.blocks) * bs]
-        need = sum(self.blocks_needed(s.seq_id, 1) for s in short)
+        inside = [s for s in held if self._inside_shared(s)] if self.alloc.shared else []
+        need = sum(self.blocks_needed(s.seq_id, 1) for s in short) + len(inside)
         if need > self.alloc.free_blocks:
             raise OutOfBlocks(f"step needs {need} KV blocks, {self.alloc.free_blocks} free")
+        if inside:
+            self._own(inside)
         for s in short:
             self.reserve(s.seq_id, 1, list_slots=False)
         at = np.array([s.length for s in held], dtype=np.int32)
@@ -176,6 +217,30 @@ class PagedKVCache:
         dst.length = tokens
         return dst
 
+    def fork(self, src_id: int, dst_id: int, length: int | None = None) -> SequenceKV:
+        """New sequence with the first ``length`` committed tokens of ``src`` (default: all): whole blocks are shared, of the block that ``length`` is inside
+        of it gets a copy. The two go on apart."""
+        src = self.seqs[src_id]
+        length = src.length if length is None else length
+        if self.compact is not None:
+            raise ValueError("sequences with sealed 8-bit groups are not forked")
+        if not 0 <= length <= src.length:
+            raise ValueError(f"sequence {src_id} has {src.length} committed tokens")
+        if dst_id in self.seqs:
+            raise ValueError(f"sequence {dst_id} exists")
+        whole, rest = divmod(length, self.block_size)
+        if rest and not self.alloc.free_blocks:
+            raise OutOfBlocks("no KV block is free for the fork's last one")
+        dst = self.add_sequence(dst_id)
+        for b in src.blocks[:whole]:
+            self.alloc.share(b)
+            dst.blocks.append(b)
+        if rest:
+            dst.blocks.append(self.alloc.alloc())
+            self.copy_blocks([src.blocks[whole]], [dst.blocks[whole]])
+        dst.length = length
+        return dst
+
     def block_row(self, seq_id: int, width: int) -> list[int]:
         blocks = self.seqs[seq_id].blocks
         assert len(blocks) <= width, "block table too narrow for the sequence"
@@ -188,6 +253,8 @@ class PagedKVCache:
         ``tree_kv_gather`` / ``tree_kv_scatter``, kernels/tree/meta.cu)."""
         if not src_positions:
             return
+        if self.kv_format == "affine4":
+            raise ValueError("rows of 4-bit pages are not moved")
         s = self.seqs[seq_id]
         bs = self.block_size
         dev = self.device

@@ -5,7 +5,7 @@ boundary, ring slots, compact block sizes).
 
 The attention kernels of this engine read BF16 pages; ``Affine8Store`` is the compact store behind them:
 ``seal`` packs every group that has left the recent window, ``materialise`` rebuilds BF16 rows for a token
-range (used when a sequence is paged back in or handed to another rank)."""
+range (used when a sequence is paged back in or handed to another rank). ``affine4`` is a format of the paged cache's blocks themselves (``ops.kv4_ops``)."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -14,7 +14,7 @@ import torch
 
 SINK_TOKENS, RECENT_TOKENS, GROUP_TOKENS, TENTATIVE_TOKENS = 64, 2048, 128, 5   # tentative = most rows one verify step appends
 RING_TOKENS = SINK_TOKENS + RECENT_TOKENS + GROUP_TOKENS - 1 + TENTATIVE_TOKENS
-TAGS = {"bf16": "BF16", "affine8": "UINT8_KC128_VT_F32_S64_R2048_MUL_ADD_BF16_RNE_V1"}
+TAGS = {"bf16": "BF16", "affine8": "UINT8_KC128_VT_F32_S64_R2048_MUL_ADD_BF16_RNE_V1", "affine4": "UINT4_G32_BF16_SCALE_LO_V1"}
 
 
 def from_tag(tag: str) -> str:
@@ -61,6 +61,11 @@ def layout(fmt: str, capacity: int, heads: int, dim: int) -> KvLayout:
         codes = heads * capacity * dim
         k_stats = heads * -(-capacity // GROUP_TOKENS) * dim * 2
         v_stats = heads * capacity * 2
+    elif fmt == "affine4":                                # all of it codes: nothing stays BF16 but (scale, lo) of every 32 elements
+        if dim not in (64, 128):
+            raise ValueError("4-bit pages hold heads of 64 or 128 elements")
+        pages = -(-capacity // 64) * heads
+        return KvLayout(capacity, 0, 0, pages * 32 * dim, pages * 2 * dim, pages * 2 * dim, pages * 80 * dim)
     else:
         raise ValueError(f"unknown KV format {fmt}")
     ring_elements = heads * ring * dim
@@ -75,6 +80,8 @@ def block_bytes(fmt: str, start: int, tokens: int, prefix: int, heads: int, dim:
         raise ValueError("KV block outside prefix")
     if fmt == "bf16":
         return heads * tokens * dim * 4
+    if fmt == "affine4":                                  # whole pages
+        return (-(-end // 64) - start // 64) * heads * 80 * dim
     if start % GROUP_TOKENS:
         raise ValueError("compact KV block must start on a 128-token group")
     sealed = sealed_until(prefix)

@@ -20,7 +20,7 @@ import torch
 
 from .. import ops
 from ..config import ModelSpec
-from ..ops import lora_ops
+from ..ops import kv4_ops, lora_ops
 from ..engine.batch import ForwardBatch
 from ..engine.kv_cache import PagedKVCache
 from .weights import ModelWeights
@@ -72,6 +72,17 @@ class DecoderModel:
         ad = self._adapters
         stacks, rows = (None, None) if ad is None else (ad[0][i], ad[1])
         lora = stacks is not None and stacks.qkv is not None
+        if kv.kv_format == "affine4":
+            # 4-bit pages: turned queries come back, keys and values are written as codes and read as such
+            qkv = lora_ops.linear_lora(n, lw.wqkv, stacks.qkv, rows) if lora else ops.linear(n, lw.wqkv)
+            q = kv4_ops.write_kv4(qkv, b.slots, kv.k[i], kv.v[i], self.hq, self.hkv, self.d, self._rope_cs, lw.q_norm if s.qk_norm else None,
+                                  lw.k_norm if s.qk_norm else None, s.rms_eps)
+            if b.is_decode:
+                a = kv4_ops.attn_decode_kv4(q, kv.k[i], kv.v[i], b.block_table, b.ctx_lens, self.hq, self.hkv, self.d, self.scale, nq=b.nq, max_ctx=b.max_ctx)
+            else:
+                a = kv4_ops.attn_prefill_kv4(q, kv.k[i], kv.v[i], b.block_table, b.q_start, b.q_lens, b.ctx_lens, b.max_q_len, self.hq, self.hkv, self.d,
+                                             self.scale, max_ctx=b.max_ctx)
+            return self._attention_out(i, a, stacks, rows)
         if s.qk_norm:
             qkv = lora_ops.linear_lora(n, lw.wqkv, stacks.qkv, rows) if lora else ops.linear(n, lw.wqkv)
             ops.rope_kv_paged(qkv, b.positions, b.slots, kv.k[i], kv.v[i], self.hq, self.hkv, self.d, s.rope_theta,
@@ -92,11 +103,14 @@ class DecoderModel:
         else:
             a = ops.attn_prefill(qkv, kv.k[i], kv.v[i], b.block_table, b.q_start, b.q_lens, b.ctx_lens, b.max_q_len,
                                  self.hq, self.hkv, self.d, self.scale, window=-1 if self.bidirectional else 0)
+        return self._attention_out(i, a, stacks, rows)
+
+    def _attention_out(self, i: int, a: torch.Tensor, stacks, rows) -> torch.Tensor:
         if self.trace is not None:
             self.trace.record(f"layer.{i}.attn", a)
         if stacks is not None and stacks.o is not None:
-            return lora_ops.linear_lora(a, lw.wo, stacks.o, rows)
-        return self.comm.row_linear(a, lw.wo)
+            return lora_ops.linear_lora(a, self.w.layers[i].wo, stacks.o, rows)
+        return self.comm.row_linear(a, self.w.layers[i].wo)
 
     def _ffn(self, i: int, n: torch.Tensor) -> torch.Tensor:
         lw = self.w.layers[i]
@@ -127,11 +141,14 @@ class DecoderModel:
         self._rope_cs = None
         ad = getattr(b, "adapters", None)
         self._adapters = None if ad is None else (ad.layers, b.adapter_ids)
-        if inputs_embeds is None and self._sequence_parallel(b):
+        packed = kv.kv_format == "affine4"         # these pages are written and read by kernels of their own (``_attention``)
+        if not packed and inputs_embeds is None and self._sequence_parallel(b):
             return self._hidden_states_sp(b, kv)
-        if self._chain_ok(b):
+        if not packed and self._chain_ok(b):
             return self._hidden_states_chain(b, kv, inputs_embeds)
-        if b.positions.is_cuda and self.d == 128 and not s.qk_norm and \
+        if packed:
+            self._rope_cs = ops.rope_table(b.positions, self.d, s.rope_theta)
+        elif b.positions.is_cuda and self.d == 128 and not s.qk_norm and \
                 (b.positions.shape[0] <= ops.SKINNY_MAX_M or
                  (type(self)._attention is DecoderModel._attention and type(w.layers[0].wqkv) is torch.Tensor and
                   ops.rope_in_product(b.positions.shape[0], *w.layers[0].wqkv.shape))):
@@ -144,7 +161,7 @@ class DecoderModel:
             n = ops.rmsnorm(x, w.layers[0].input_ln, s.rms_eps)
         if self.trace is not None:
             self.trace.record("embed", x)
-        stack = self._stack_layers(b, kv)
+        stack = None if packed else self._stack_layers(b, kv)
         done = 0 if stack is None else ops.dense_stack(
             x, n, stack, b.positions, b.slots, b.block_table, b.q_start, b.q_lens, b.ctx_lens, b.max_q_len, self.hq, self.hkv, w.layers[0].wdown.shape[1],
             self.scale, s.rms_eps, s.rope_theta, -1 if self.bidirectional else 0, self._rope_cs)

@@ -114,7 +114,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   // keys that the last of this CTA's columns sees; its pages are shared evenly by the splits and, one after the other, by the warps
   const int seen = min(ctx, ctx - n + group_of(ct * NT * 8 + min(columns, NT * 8) - 1) + 1);
   const int pages = (max(seen, 0) + KV4_PAGE - 1) / KV4_PAGE;
-  const int per = (pages + nsplit - 1) / nsplit;
+  const int per = max((pages + nsplit - 1) / nsplit, KV4_WARPS);       // a page for every warp at least: a launch for long contexts may meet a short one
   const int p0 = split * per + warp, p1 = min(pages, split * per + per);
   const int mine = p1 > p0 ? (p1 - p0 + KV4_WARPS - 1) / KV4_WARPS : 0;
 

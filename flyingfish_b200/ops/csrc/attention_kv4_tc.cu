@@ -93,7 +93,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
   }
   const int past = ctx - n, row0 = q_start ? q_start[b] : b * nq;
   const int seen = past + (c0 + min(rows, 2 * KVT_M) - 1) / G + 1;        // keys that the last row sees
-  const int pages = (max(seen, 0) + KVT_N - 1) / KVT_N, per = (pages + nsplit - 1) / nsplit;
+  const int pages = (max(seen, 0) + KVT_N - 1) / KVT_N, per = max((pages + nsplit - 1) / nsplit, 4);
   const int first = split * per, tiles = max(0, min(pages, first + per) - first);    // pages of this split
 
   if (threadIdx.x == 0) {

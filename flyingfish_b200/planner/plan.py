@@ -120,6 +120,8 @@ def plan_memory(spec: ModelSpec, settings: Settings, info: DeviceInfo, weights_b
         block_bytes = max(settings.kv_block * spec.elem_bytes * sum(h * (dk + dv) for h, dk, dv in spec.kv_geometry()), 1)
     else:
         block_bytes = spec.layers * hkv * settings.kv_block * spec.head_dim * 2 * 2
+        if settings.kv_format == "affine4":
+            block_bytes = block_bytes * 5 // 16          # 4 bits and two BF16 numbers per 32 elements
     blocks_per_seq = (settings.capacity + settings.kv_block - 1) // settings.kv_block
     # one sequence of `capacity` tokens must always fit next to a minimal chunk
     min_need = blocks_per_seq * block_bytes + ATTENTION_TILE * row_bytes

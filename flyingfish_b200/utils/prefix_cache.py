@@ -71,6 +71,9 @@ def save_prefix(model, seq, directory: str | Path) -> Path:
         for tag, cache in (("k", eng.kv.k[l]), ("v", eng.kv.v[l])):
             if cache is None:
                 continue
+            if eng.kv.kv_format == "affine4":          # whole pages as they are; what lies behind the prefix is never read
+                tensors[f"layer.{l}.{tag}"] = cache[blocks].cpu()
+                continue
             rows = cache[blocks].permute(1, 0, 2, 3).reshape(cache.shape[1], -1, cache.shape[3])[:, :n]
             tensors[f"layer.{l}.{tag}"] = rows.contiguous().cpu()
     save_safetensors(d / "kv.safetensors", tensors)
@@ -117,6 +120,10 @@ def restore_prefix(model, directory: str | Path, limit: int | None = None):
         for l in range(eng.kv.layers):
             for tag, cache in (("k", eng.kv.k[l]), ("v", eng.kv.v[l])):
                 if cache is None:
+                    continue
+                if eng.kv.kv_format == "affine4":
+                    at = torch.tensor(kvs.blocks[: (n + bs - 1) // bs], device=eng.device)
+                    cache[at] = f.tensor(f"layer.{l}.{tag}")[: at.numel()].to(eng.device)
                     continue
                 rows = f.tensor(f"layer.{l}.{tag}")[:, :n].to(eng.device)   # [heads, n, dim]
                 cache[blk, :, off, :] = rows.permute(1, 0, 2).to(cache.dtype)

@@ -1,0 +1,250 @@
+"""``--kv-format affine4``: the engine over 4-bit pages (prompts, decoding, drafts verified, graphs, forks, stored prefixes), and forks over every cache format."""
+import pytest
+import torch
+
+from flyingfish_b200 import cli
+from flyingfish_b200.api import Model
+from flyingfish_b200.config import Settings
+from flyingfish_b200.engine.kv_cache import OutOfBlocks, PagedKVCache
+from flyingfish_b200.engine.sampling import Sampling
+from flyingfish_b200.engine import kv_format as kf
+from flyingfish_b200.ops import kv4_ops
+from flyingfish_b200.utils.prefix_cache import PrefixError, restore_prefix, save_prefix
+
+
+def _prompt(n, seed=11):
+    return torch.randint(0, 2048, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def _load(device, kv_format="affine4", shape="tiny-llama", capacity=512, **kw):
+    return Model.load(shape, Settings(capacity=capacity, max_batch=4, graph=kw.pop("graph", False), kv_format=kv_format, **kw), device=device, seed=0)
+
+
+def test_planned_blocks_are_five_sixteenths_as_large():
+    a, b = kf.layout("bf16", 640, 2, 128), kf.layout("affine4", 640, 2, 128)
+    assert b.bytes * 16 == a.bytes * 5 and kf.from_tag(kf.TAGS["affine4"]) == "affine4"
+    assert kf.block_bytes("affine4", 0, 65, 65, 2, 128) == 2 * 2 * kv4_ops.page_bytes(128) * 2
+    kv = PagedKVCache(2, 2, 128, 5, kv_format="affine4")
+    assert kv.k[0].dtype == torch.uint8 and kv.k[0].shape == (5, 2, kv4_ops.page_bytes(128))
+    with pytest.raises(ValueError):
+        kf.layout("affine4", 64, 2, 96)
+
+
+def test_what_the_engine_refuses():
+    for shape in ("tiny-embed", "tiny-gemma", "flint-tiny", "tiny-hybrid"):
+        with pytest.raises(ValueError, match="affine4"):
+            _load("cpu", shape=shape)
+    with pytest.raises(ValueError, match="affine4"):
+        _load("cpu", dtype="fp32")
+    with pytest.raises(ValueError, match="affine4"):
+        _load("cpu", kv_block=32)
+    m = _load("cpu")
+    seq = m.engine.add_sequence(_prompt(5))
+    with pytest.raises(ValueError, match="prompt is complete"):
+        m.engine.fork(seq)
+    m.engine.prefill([seq])
+    with pytest.raises(ValueError, match="tree"):
+        m.engine.verify_tree(seq, [seq.pending], [0], [1])
+    base = ["--model", "tiny-llama", "--cpu", "--kv-format", "affine4"]
+    with pytest.raises(SystemExit):
+        cli.main(base + ["--draft-model", "tiny-llama", "--spec-budget", "tree16", "generate", "--tokens", "1,2"])
+    other = _load("cpu", kv_format="affine8")
+    seq = other.engine.add_sequence(_prompt(5))
+    other.engine.prefill([seq])
+    with pytest.raises(ValueError, match="8-bit"):
+        other.engine.fork(seq)
+    with pytest.raises(ValueError, match="8-bit"):
+        other.engine.kv.fork(seq.seq_id, 99)
+
+
+@pytest.mark.parametrize("shape", ["tiny-llama", "tiny-moe"])
+def test_a_model_goes_on_over_4_bit_pages_cpu(shape):
+    """4-bit keys and values perturb the logits; what is exact: portions of a prompt and single tokens read the same codes."""
+    m = _load("cpu", shape=shape, dtype="bf16")
+    ids = [i % 1024 for i in _prompt(150)]
+    whole = m.engine.generate([ids], 6)[0]
+    m.reset()
+    seq = m.engine.add_sequence(ids)
+    first = m.engine.prefill([seq], chunk=37)[0]
+    parts = [first] + [m.engine.decode([seq])[0] for _ in range(5)]
+    assert len(whole) == 6 and whole[0] == parts[0]
+    kv = m.engine.kv
+    used = kv.seqs[seq.seq_id].blocks
+    assert kv.seqs[seq.seq_id].length == 155 and bool(kv.k[0][used[0]].any())
+    m.engine.free_sequence(seq.seq_id)
+    assert kv.alloc.free_blocks == kv.num_blocks
+
+
+def test_verified_drafts_read_the_same_pages_cpu():
+    m = _load("cpu")
+    ids = _prompt(70)
+    want = m.engine.generate([ids], 5)[0]
+    seq = m.engine.add_sequence(ids)
+    m.engine.prefill([seq])
+    got = m.engine.verify([seq], [want[1:4]])[0]
+    assert got[:4] == want[1:5]
+    m.engine.commit_verified(seq, got, 3)
+    assert m.engine.kv.seqs[seq.seq_id].length == 74
+
+
+@pytest.mark.parametrize("kv_format", ["bf16", "affine4"])
+@pytest.mark.parametrize("n", [64, 100, 129])
+def test_a_fork_goes_on_alone_cpu(kv_format, n):
+    m = _load("cpu", kv_format=kv_format)
+    eng, ids = m.engine, _prompt(n)
+    want = eng.generate([ids], 8)[0]
+    a = eng.add_sequence(ids)
+    eng.prefill([a])
+    eng.decode([a]); eng.decode([a])
+    b = eng.fork(a)
+    assert b.output == a.output and b.pending == a.pending and eng.kv.seqs[b.seq_id].length == n + 2
+    shared = (n + 2) // 64
+    ka, kb = eng.kv.seqs[a.seq_id].blocks, eng.kv.seqs[b.seq_id].blocks
+    assert ka[:shared] == kb[:shared] and (len(kb) == shared or kb[shared] != ka[shared]) and eng.kv.alloc.shared == shared
+    # the fork alone, then the first one: each as if it were the only one
+    for _ in range(5):
+        eng.decode([b])
+    assert b.output == want and a.output == want[:3]
+    for _ in range(5):
+        eng.decode([a])
+    assert a.output == want
+    # taken back into a shared block: its next row goes into a copy
+    if shared:
+        eng.kv.truncate(b.seq_id, 30)
+        before = [t[ka[0]].clone() for t in eng.kv.k]
+        assert eng.kv.blocks_needed(b.seq_id, 1) == 1
+        b.pending = 5
+        eng.decode([b])
+        assert kb[0] != ka[0] and all(torch.equal(t[ka[0]], w) for t, w in zip(eng.kv.k, before))
+    for s in (a, b):
+        eng.free_sequence(s.seq_id)
+    assert eng.kv.alloc.free_blocks == eng.kv.num_blocks and eng.kv.alloc.shared == 0
+
+
+def test_forks_of_a_full_cache_are_refused():
+    kv = PagedKVCache(1, 1, 64, 3, kv_format="affine4")
+    kv.add_sequence(0)
+    kv.reserve(0, 130); kv.commit(0, 130)
+    with pytest.raises(OutOfBlocks):
+        kv.fork(0, 1)
+    assert 1 not in kv.seqs and kv.alloc.shared == 0
+    kv.fork(0, 1, 128)
+    with pytest.raises(ValueError):
+        kv.fork(0, 1)
+    with pytest.raises(ValueError):
+        kv.fork(0, 2, 131)
+    kv.truncate(1, 70)
+    with pytest.raises(OutOfBlocks):
+        kv.reserve(1, 1)
+    with pytest.raises(OutOfBlocks):
+        kv.reserve_step([0, 1])
+    kv.free_sequence(0)
+    kv.reserve(1, 1)
+
+
+def test_samples_of_one_prompt_are_those_of_separate_requests_cpu():
+    m = _load("cpu")
+    ids = _prompt(90)
+    how = [Sampling(temperature=0.9, seed=s) for s in (3, 4, 5)]
+    got = m.generate_samples(ids, how, 6)
+    apart = [m.engine.generate([ids], 6, sampling=h)[0] for h in how]
+    assert got == apart and m.engine.kv.alloc.free_blocks == m.engine.kv.num_blocks
+    assert m.generate_samples(ids, [Sampling(temperature=0)] * 2, 4) == [m.engine.generate([ids], 4)[0]] * 2
+    assert m.generate_samples(ids, [], 4) == []
+
+
+def test_stored_prefixes_are_the_pages(tmp_path):
+    m = _load("cpu")
+    ids = _prompt(100)
+    want = m.engine.generate([ids], 5)[0]
+    seq = m.engine.add_sequence(ids[:66])
+    m.engine.prefill([seq])
+    pages = m.engine.kv.k[0][m.engine.kv.seqs[seq.seq_id].blocks].clone()
+    pkg = save_prefix(m, seq, tmp_path / "pfx")
+    m.reset()
+    seq = restore_prefix(m, pkg)
+    assert torch.equal(m.engine.kv.k[0][m.engine.kv.seqs[seq.seq_id].blocks], pages)
+    seq.prompt = ids
+    assert [m.engine.prefill([seq])[0]] + [m.engine.decode([seq])[0] for _ in range(4)] == want
+    with pytest.raises(PrefixError, match="different"):
+        restore_prefix(_load("cpu", kv_format="bf16"), pkg)
+
+
+def test_cli_generates_over_4_bit_pages(capsys):
+    import json
+    args = ["--model", "tiny-llama", "--cpu", "--capacity", "256", "--kv-format", "affine4", "generate", "--tokens", "5,6,7,8,9", "--max-new-tokens", "4", "--ignore-eos"]
+    assert cli.main(args) in (0, None)
+    out = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert out["kv"]["format"] == "affine4" and len(out["generated_ids"]) == 4
+
+
+# ------------------------------------------------------------------------------------------
+# on the device
+# ------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_model_goes_on_over_4_bit_pages(graph):
+    """Against the same model on the CPU: logits of a prompt within the two paths' roundings, and the same pages but for codes next to a border."""
+    m, c = _load("cuda", graph=graph, capacity=1024), _load("cpu", capacity=1024)
+    prompts = [_prompt(300), _prompt(5, 12), _prompt(64, 13)]
+    seqs = [m.engine.add_sequence(p) for p in prompts]
+    m.engine.prefill(seqs)
+    for _ in range(70):
+        m.engine.decode(seqs)
+    ref = c.engine.add_sequence(prompts[0])
+    c.engine.prefill([ref])
+    kg, kc = m.engine.kv, c.engine.kv
+    slots = lambda kv, s, n: torch.tensor([kv.seqs[s.seq_id].blocks[p // 64] * 64 + p % 64 for p in range(n)], dtype=torch.int32)
+    a = kv4_ops.read_kv4(kg.k[0], kg.v[0], slots(kg, seqs[0], 300).cuda(), m.engine.model.d)
+    b = kv4_ops.read_kv4(kc.k[0], kc.v[0], slots(kc, ref, 300), m.engine.model.d)
+    for x, y in zip(a, b):
+        # the first layer's keys and values: sums of another order, and a code's step (1 / 15 of a group's span) where that crosses a border
+        x, y = x.cpu().double(), y.double()
+        span = y.unflatten(-1, (-1, 32))
+        step = ((span.amax(-1) - span.amin(-1)) / 15).repeat_interleave(32, -1)
+        assert bool(((x - y).abs() <= 1.1 * step + 0.02 * y.abs().amax()).all()) and float((x - y).norm() / y.norm()) < 0.02
+    assert all(len(s.output) == 71 for s in seqs)
+    for s in seqs:
+        m.engine.free_sequence(s.seq_id)
+    assert kg.alloc.free_blocks == kg.num_blocks
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_format", ["bf16", "affine4"])
+def test_forks_and_samples(kv_format):
+    """A fork's tokens are those of the sequence it left, whatever else runs; samples of one prompt draw as separate requests do."""
+    m = _load("cuda", kv_format=kv_format, graph=True, capacity=1024)
+    eng, ids = m.engine, _prompt(200)
+    want = eng.generate([ids], 40)[0]
+    a = eng.add_sequence(ids)
+    eng.prefill([a])
+    for _ in range(9):
+        eng.decode([a])
+    forks = [eng.fork(a) for _ in range(3)]
+    pages = [[t[eng.kv.seqs[s.seq_id].blocks].cpu() for t in eng.kv.k + eng.kv.v] for s in [a] + forks]
+    for other in pages[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(pages[0], other))
+    for _ in range(30):
+        eng.decode([a] + forks)
+    assert all(f.output == a.output for f in forks) and a.output[:10] == want[:10]
+    for s in [a] + forks:
+        eng.free_sequence(s.seq_id)
+    how = [Sampling(temperature=0.9, top_p=0.9, seed=s) for s in (3, 4, 5)]
+    got = m.generate_samples(ids, how, 12)
+    apart = [eng.generate([ids], 12, sampling=h)[0] for h in how]
+    assert [g[0] for g in got[:1]] == [x[0] for x in apart[:1]] and all(len(g) == 12 for g in got)
+    assert eng.kv.alloc.free_blocks == eng.kv.num_blocks
+
+
+@pytest.mark.gpu
+def test_verified_drafts_read_the_same_pages():
+    m = _load("cuda", graph=True, capacity=1024)
+    ids = _prompt(130)
+    want = m.engine.generate([ids], 5)[0]
+    seq = m.engine.add_sequence(ids)
+    m.engine.prefill([seq])
+    got = m.engine.verify([seq], [want[1:4]])[0]
+    # verified rows are multiplied eight at a time, single ones alone: equal up to near ties, which random weights give now and then
+    assert got[0] == want[1] and len(got) == 4
+    m.engine.commit_verified(seq, got[:1], 0)
+    assert m.engine.kv.seqs[seq.seq_id].length == 131
