@@ -67,7 +67,7 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 // A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, fetched by bulk copies into its two slots (keys, values),
 // with its own running maximum, sum and O. The warps' results meet in shared memory, those of up to eight CTAs (splits) in that of
 // their cluster, those of more in kv4_merge_kernel.
-constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;
+constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;      // (a warp for every group of a head at least)
 template <int D, int NT>
 constexpr int kv4_smem() {
   const int ring = KV4_WARPS * KV4_SLOTS * kv4_page_bytes(D), merge = (KV4_WARPS * (D + D / 32 + 2) + D + 2) * NT * 8 * 4;
@@ -83,6 +83,8 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   constexpr int NG = D / 32, PB = kv4_page_bytes(D), ROW = D / 2, STAT = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[KV4_WARPS][KV4_SLOTS];
+  __shared__ uint4 sq[NT][NG][32];
+  __shared__ float ssum[NT][NG][8];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (threadIdx.x < KV4_WARPS * KV4_SLOTS) mbar_init(&full[threadIdx.x / KV4_SLOTS][threadIdx.x % KV4_SLOTS], 1);
@@ -141,7 +143,8 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   for (int i = 0; i < KV4_SLOTS; ++i)
     if (i < 2 * mine) issue(i);
 
-  uint32_t qf[NT][NG][2][2], qb[NT][2];
+  // B fragments of the queries: the warps make those of a group each and share them; in registers they are only while a page's keys are multiplied
+  uint32_t qb[NT][2];
   float cf[NT][2];
   int lim[NT][2];
 #pragma unroll
@@ -157,31 +160,34 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     // 2^(14 - exponent) of the column's greatest element, and 2^24 over it (zero columns: any; the exponents are kept where both are normal numbers)
     const int ex = min(max((int)(__float_as_uint(most) >> 23), 20), 244);
     const float gain = __uint_as_float((uint32_t)(min(254 + 14 - ex, 254)) << 23), back = __uint_as_float((uint32_t)(254 - min(254 + 14 - ex, 254) + 24) << 23);
-    float part[3] = {0.f, 0.f, 0.f};                            // of the group that this lane has in the product with lo
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
+      if (j != warp) continue;
       const uint32_t w[4] = {qv[nt][j].x, qv[nt][j].y, qv[nt][j].z, qv[nt][j].w};
+      uint32_t f[4];
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float x = kv4_low(w[i]) * gain, y = kv4_high(w[i]) * gain;
         s += x + y;
-        qf[nt][j][i >> 1][i & 1] = (i & 1) ? kv4_f16x2(x * 0.0625f, y * 0.0625f) : kv4_f16x2(x, y);
+        f[i] = (i & 1) ? kv4_f16x2(x * 0.0625f, y * 0.0625f) : kv4_f16x2(x, y);
       }
       s += __shfl_xor_sync(0xffffffffu, s, 1); s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (j == t) {
-        s *= 5.9604644775390625e-8f;                            // 2^-24
-        part[0] = __bfloat162float(__float2bfloat16(s));
-        part[1] = __bfloat162float(__float2bfloat16(s - part[0]));
-        part[2] = s - part[0] - part[1];
-      }
+      sq[nt][j][lane] = make_uint4(f[0], f[1], f[2], f[3]);
+      if (t == 0) ssum[nt][j][g] = s * 5.9604644775390625e-8f;                       // 2^-24
     }
-    qb[nt][0] = pack_bf16x2(part[0], part[1]); qb[nt][1] = pack_bf16x2(part[2], 0.f);
     const float f = scale_log2 * back;
     cf[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);             // column 2 t is held by lanes of g = 2 t
     cf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
     for (int e = 0; e < 2; ++e) lim[nt][e] = nt * 8 + 2 * t + e < columns ? ctx - n + group_of(ct * NT * 8 + nt * 8 + 2 * t + e) : -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    // sum(q) of the group that this lane has in the product with lo, in three parts
+    const float s = t < NG ? ssum[nt][t & (NG - 1)][g] : 0.f, a = __bfloat162float(__float2bfloat16(s)), c = __bfloat162float(__float2bfloat16(s - a));
+    qb[nt][0] = pack_bf16x2(a, c); qb[nt][1] = pack_bf16x2(s - a - c, 0.f);
   }
   const int all = ctx - n + group_of(ct * NT * 8);                    // keys up to here are seen by every column
 
@@ -209,6 +215,11 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     float s[4][NT][4];
     {
       const uint32_t sk = ring_at + pos.s * PB;
+      uint32_t qf[NT][NG][2][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < NG; ++j) kv4_lds(smem_u32(&sq[nt][j][lane]), qf[nt][j][0][0], qf[nt][j][0][1], qf[nt][j][1][0], qf[nt][j][1][1]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         uint32_t kw[2][NG], ks[2][NG], la[2];
