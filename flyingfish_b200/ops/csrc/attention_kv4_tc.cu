@@ -4,7 +4,8 @@
 // them over one kv head: both read the same keys and values, so a page is turned into FP16 once for 256 rows. Per page j of 64 tokens:
 //   one thread    fetches the page by bulk copies, three pages ahead
 //   four warps    write keys and values code * scale + lo, rounded once, as 128-byte-swizzled tiles
-//   one thread    S_i(j + 1) = Q_i K^T for both tiles, then O_i += P_i V; S, P and O live in tensor memory (P over the S that it came from)
+//   two threads   one for a tile i: S_i(j + 1) = Q_i K^T, then O_i += P_i V; S, P and O live in tensor memory (P over the S that it came from). (One thread for both
+//                 spends 1400 cycles a page on issuing and on barriers, as long as the products take.)
 //   two x 4 warps soft-max of a tile, a thread per row: running maximum and sum in FP32 in the base-2 domain; O is rescaled only when the maximum has moved
 //                 by more than 2^8 (the stale one stays exact: P and the sum share it)
 // All operands are FP16, this kernel's choice of a rounding: keys, values and weights keep 11 bits where BF16 has 8 (outputs 0.0017 off in the root mean square,
@@ -19,7 +20,7 @@
 namespace ff {
 
 constexpr int KVT_M = 128, KVT_N = KV4_PAGE, KVT_STAGES = 3;
-constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 2;      // warps 0-7 soft-max, 8-11 tiles, 12 products, 13 pages
+constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 3;      // warps 0-7 soft-max, 8-11 tiles, 12 and 14 products, 13 pages
 constexpr int KVT_PAGES = 3;                                                         // pages on their way or being turned into tiles
 constexpr float KVT_MOVED = 8.0f;                                                    // log2 units
 template <int D> constexpr int kvt_smem() { return 2 * KVT_M * D * 2 + 2 * KVT_STAGES * KVT_N * D * 2 + KVT_PAGES * 2 * kv4_page_bytes(D) + 1024; }
@@ -102,7 +103,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       for (int k = 0; k < 2; ++k) { mbar_init(&bars.s_full[i][k], 1); mbar_init(&bars.p_full[i][k], 4); mbar_init(&bars.pv_done[i][k], 1); }
     }
     for (int i = 0; i < KVT_STAGES; ++i) {
-      mbar_init(&bars.k_full[i], KVT_FILL); mbar_init(&bars.k_empty[i], 1); mbar_init(&bars.v_full[i], KVT_FILL); mbar_init(&bars.v_empty[i], 1);
+      mbar_init(&bars.k_full[i], KVT_FILL); mbar_init(&bars.k_empty[i], two); mbar_init(&bars.v_full[i], KVT_FILL); mbar_init(&bars.v_empty[i], two);
     }
     for (int i = 0; i < KVT_PAGES; ++i) { mbar_init(&bars.p_in[i], 1); mbar_init(&bars.p_out[i], KVT_FILL); }
     bars.abort_flag = 0;
@@ -130,25 +131,34 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         if (!mbar_wait(part ? &bars.v_empty[tr.s] : &bars.k_empty[tr.s], tr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 41 + part)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        uint32_t code[2][NG], stat[2][NG];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int key = key0 + 32 * i;
-          uint32_t code[NG], stat[NG];
-          kvt_load<D>(code, page + part * PB + (part ? kv4_value_at<D>(key, 2 * u, 0) : key * (D / 2) + u * (D / 8)));
-          kvt_load<D>(stat, page + part * PB + kv4_code_bytes(D) + key * (D / 8));
-          if ((first + j) * KVT_N + key >= ctx) {                          // behind the sequence: whatever the page holds there is no number
+          kvt_load<D>(code[i], page + part * PB + (part ? kv4_value_at<D>(key, 2 * u, 0) : key * (D / 2) + u * (D / 8)));
+          kvt_load<D>(stat[i], page + part * PB + kv4_code_bytes(D) + key * (D / 8));
+          if ((first + j) * KVT_N + key >= ctx) {                // behind the sequence: whatever the page holds there is no number
 #pragma unroll
-            for (int g = 0; g < NG; ++g) stat[g] = 0u;
+            for (int g = 0; g < NG; ++g) stat[i][g] = 0u;
           }
-          const uint32_t row = smem_u32(part ? sV : sK) + tr.s * TILE + key * 128;
+        }
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const float2 sl = unpack_bf16x2(stat[g]);
+        for (int g = 0; g < NG; ++g) {
+          uint32_t v[2][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 sl = unpack_bf16x2(stat[i][g]);
             const uint32_t scale2 = kvt_f16x2(sl.x, sl.x), lo2 = kvt_f16x2(sl.y, sl.y);
             // values: 16-bit unit g of two chunks, the even elements and the odd ones
-            const uint32_t word = part ? kvt_prmt(code[g / 2], code[NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[g];
-            const int c = 4 * g + u;                             // 16-byte chunk of the row: 64-element block c / 8
-            kv4_sts(row + (c >> 3) * (KVT_N * 128) + (((c & 7) ^ (key & 7)) << 4), kvt_value(word, 0, scale2, lo2), kvt_value(word, 4, scale2, lo2), kvt_value(word, 8, scale2, lo2), kvt_value(word, 12, scale2, lo2));
+            const uint32_t word = part ? kvt_prmt(code[i][g / 2], code[i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[i][g];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = kvt_value(word, 4 * k, scale2, lo2);
+          }
+          const int c = 4 * g + u;                               // 16-byte chunk of the row: 64-element block c / 8
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = key0 + 32 * i;
+            kv4_sts(smem_u32(part ? sV : sK) + tr.s * TILE + key * 128 + (c >> 3) * (KVT_N * 128) + (((c & 7) ^ (key & 7)) << 4), v[i][0], v[i][1], v[i][2], v[i][3]);
           }
         }
         fence_proxy_async_smem();
@@ -179,32 +189,26 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       }
       if (bad) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
     }
-  } else if (warp == KVT_SOFT + KVT_FILL) {
-    // ================================ products ================================
-    if (elect_one() && tiles > 0) {
+  } else if (warp >= KVT_SOFT + KVT_FILL) {
+    // ================================ products: a warp for each tile ================================
+    const int i = warp == KVT_SOFT + KVT_FILL ? 0 : 1;
+    if (i < two && tiles > 0 && elect_one()) {
       const uint32_t idesc_s = umma_idesc(0, 0, 0, 0, KVT_M, KVT_N), idesc_o = umma_idesc(0, 0, 0, 1, KVT_M, D);
       // descriptors differ by byte offsets / 16 in their low bits
-      const uint64_t qd = umma_desc_sw128(smem_u32(sQ), 16, 1024), kd = umma_desc_sw128(smem_u32(sK), 16, 1024), vd = umma_desc_sw128(smem_u32(sV), KVT_N * 128, 1024);
-      bool ok = true;
-      for (int i = 0; i < two && ok; ++i) ok = mbar_wait(&bars.q_full[i], 0, abort_flag, status, KID_ATTN_PREFILL, 43);
+      const uint64_t qd = umma_desc_sw128(smem_u32(sQ) + i * QTILE, 16, 1024), kd = umma_desc_sw128(smem_u32(sK), 16, 1024), vd = umma_desc_sw128(smem_u32(sV), KVT_N * 128, 1024);
+      const uint32_t s_at = tmem + 128 * i, o_at = tmem + 256 + 128 * i;
+      bool ok = mbar_wait(&bars.q_full[i], 0, abort_flag, status, KID_ATTN_PREFILL, 43);
       RingPos kr, vr;
       auto issue_s = [&](int j) -> bool {
         if (!mbar_wait(&bars.k_full[kr.s], kr.ph, abort_flag, status, KID_ATTN_PREFILL, 44)) return false;
+        // the buffer holds the P of page j - 2
+        if (j >= 2 && !mbar_wait(&bars.pv_done[i][j & 1], ((j >> 1) & 1) ^ 1, abort_flag, status, KID_ATTN_PREFILL, 50)) return false;
+        tc_fence_after();
         const uint64_t d = kd + (uint32_t)(kr.s * (TILE >> 4));
-        const uint32_t s0 = tmem + 64 * (j & 1), before = ((j >> 1) & 1) ^ 1;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i < two) {
-            // the buffer holds the P of page j - 2
-            if (j >= 2 && !mbar_wait(&bars.pv_done[i][j & 1], before, abort_flag, status, KID_ATTN_PREFILL, 50)) return false;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              umma_f16(s0 + 128 * i, qd + (uint32_t)((i * QTILE + (k >> 2) * (KVT_M * 128) + (k & 3) * 32) >> 4), d + (uint32_t)(((k >> 2) * (KVT_N * 128) + (k & 3) * 32) >> 4),
-                       idesc_s, k != 0);
-            umma_commit(&bars.s_full[i][j & 1]);
-          }
-        }
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16(s_at + 64 * (j & 1), qd + (uint32_t)(((k >> 2) * (KVT_M * 128) + (k & 3) * 32) >> 4), d + (uint32_t)(((k >> 2) * (KVT_N * 128) + (k & 3) * 32) >> 4), idesc_s, k != 0);
+        umma_commit(&bars.s_full[i][j & 1]);
         umma_commit(&bars.k_empty[kr.s]);
         kr.next(KVT_STAGES);
         return true;
@@ -213,20 +217,14 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       for (int j = 0; j < tiles && ok; ++j) {
         if (j + 1 < tiles && !issue_s(j + 1)) { ok = false; break; }
         if (!mbar_wait(&bars.v_full[vr.s], vr.ph, abort_flag, status, KID_ATTN_PREFILL, 45)) { ok = false; break; }
+        if (!mbar_wait(&bars.p_full[i][j & 1], (j >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 46)) { ok = false; break; }
+        tc_fence_after();
         const uint64_t d = vd + (uint32_t)(vr.s * (TILE >> 4));
-        const uint32_t p0 = tmem + 64 * (j & 1), mine = (j >> 1) & 1;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i < two && ok) {
-            if (!mbar_wait(&bars.p_full[i][j & 1], mine, abort_flag, status, KID_ATTN_PREFILL, 46)) { ok = false; break; }
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < KVT_N / 16; ++k)
-              umma_f16_ts(tmem + 256 + 128 * i, p0 + 128 * i + k * 8, d + (uint32_t)((k * 2048) >> 4), idesc_o, (j > 0) || (k != 0));
-            umma_commit(&bars.pv_done[i][j & 1]);
-          }
-        }
-        if (ok) umma_commit(&bars.v_empty[vr.s]);
+        for (int k = 0; k < KVT_N / 16; ++k)
+          umma_f16_ts(o_at, s_at + 64 * (j & 1) + k * 8, d + (uint32_t)((k * 2048) >> 4), idesc_o, (j > 0) || (k != 0));
+        umma_commit(&bars.pv_done[i][j & 1]);
+        umma_commit(&bars.v_empty[vr.s]);
         vr.next(KVT_STAGES);
       }
     }
