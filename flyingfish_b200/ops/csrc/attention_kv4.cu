@@ -78,7 +78,7 @@ template <int D, int NT>
 __global__ void __launch_bounds__(32 * KV4_WARPS, NT == 1 ? 4 : 2)
 kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ block_table,
                 const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out,
-                float* __restrict__ part_o, float2* __restrict__ part_ml, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks,
+                float* __restrict__ part_o, float2* __restrict__ part_ml, int rows, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks,
                 int nsplit, uint32_t per_group, float scale_log2, int* status) {
   constexpr int NG = D / 32, PB = kv4_page_bytes(D), ROW = D / 2, STAT = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -98,6 +98,10 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   int ctx = ctx_lens[b];
   const int columns = n * G - ct * NT * 8;                      // of this CTA and behind it
   if (columns <= 0) return;
+  if (row0 < 0 || n > rows - row0) {                            // rows that the call does not have
+    if (threadIdx.x == 0) set_status(status, KID_ATTN_DECODE, FF_ERR_BOUNDS, b, row0);
+    return;
+  }
   // queries of this thread's column of B fragments (column g of every 8): 8 elements of each group
   uint4 qv[NT][NG];
 #pragma unroll
@@ -463,15 +467,15 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
 template <int D>
 __global__ void __launch_bounds__(128)
 kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int* __restrict__ q_start, const int* __restrict__ q_lens,
-                 __nv_bfloat16* __restrict__ out, int nq, int hq, long long ldo, int nsplit) {
+                 __nv_bfloat16* __restrict__ out, int rows, int nq, int hq, long long ldo, int nsplit) {
   constexpr int E = D / 32;
   __shared__ float sacc[4][D];
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.y, qi = blockIdx.x / hq, head = blockIdx.x - qi * hq;
-  if (q_lens != nullptr && qi >= q_lens[b]) return;
-  const int row = (q_start ? q_start[b] : b * nq) + qi;
+  const int n = q_lens ? q_lens[b] : nq, row0 = q_start ? q_start[b] : b * nq, row = row0 + qi;
+  if (qi >= n || row0 < 0 || n > rows - row0) return;
   const size_t pr = ((size_t)row * hq + head) * nsplit;
   float2 ml[4];                                                 // of splits lane, lane + 32, ... (at most 128)
   float M = KV4_NONE, L = 0.f;
@@ -530,19 +534,19 @@ FF_EXPORT int ff_kv4_attn_plan(int batch, int hq, int hkv, int nq, int dim, int 
   return (int)nsplit;
 }
 
-int kv4_merge(const float* part_o, const float2* part_ml, const int* q_start, const int* q_lens, void* out, int batch, int nq, int hq, int dim, long long ldo,
-              int nsplit, cudaStream_t s) {
+int kv4_merge(const float* part_o, const float2* part_ml, const int* q_start, const int* q_lens, void* out, int batch, int rows, int nq, int hq, int dim,
+              long long ldo, int nsplit, cudaStream_t s) {
   if ((long long)nq * hq > 0x7fffffffll) return FF_HOST_TOO_LARGE;
   return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(nq * hq), batch), dim3(128), 0, s, 0, part_o, part_ml, q_start, q_lens,
-                    (__nv_bfloat16*)out, nq, hq, ldo, nsplit);
+                    (__nv_bfloat16*)out, rows, nq, hq, ldo, nsplit);
 }
 
-// q rows [.., ldq] with head h at column h dim; sequence b has rows q_start[b] .. + q_lens[b], or nq rows from b nq on where those are null (only then may
+// q rows [rows, ldq] with head h at column h dim; sequence b has rows q_start[b] .. + q_lens[b], or nq rows from b nq on where those are null (only then may
 // there be more than eight splits); ctx_lens[b] keys are seen by the last of them. Rows of no keys are zero.
 FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vpages, const int* block_table, const int* q_start, const int* q_lens,
-                               const int* ctx_lens, void* out, float* scratch, int batch, int nq, int hq, int hkv, int dim, long long ldq, long long ldo,
-                               int max_blocks, int num_blocks, int nsplit, float scale, int* status, cudaStream_t s) {
-  if (batch <= 0 || batch > 65535 || nq <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0) return FF_HOST_BAD_SHAPE;
+                               const int* ctx_lens, void* out, float* scratch, int batch, int rows, int nq, int hq, int hkv, int dim, long long ldq,
+                               long long ldo, int max_blocks, int num_blocks, int nsplit, float scale, int* status, cudaStream_t s) {
+  if (batch <= 0 || batch > 65535 || rows <= 0 || nq <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0) return FF_HOST_BAD_SHAPE;
   if (!(scale > 0.f) || nsplit < 1 || nsplit > 128 || (q_start == nullptr) != (q_lens == nullptr) || (nsplit > 8 && (scratch == nullptr || q_start != nullptr))) return FF_HOST_BAD_SHAPE;
   if (ldq % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages)) & 15)) return FF_HOST_BAD_ALIGN;
   const int columns = nq * (hq / hkv);
@@ -552,11 +556,11 @@ FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vp
   auto kern = dim == 128 ? (wide ? kv4_rows_kernel<128, 2> : kv4_rows_kernel<128, 1>) : (wide ? kv4_rows_kernel<64, 2> : kv4_rows_kernel<64, 1>);
   const int bytes = dim == 128 ? (wide ? kv4_smem<128, 2>() : kv4_smem<128, 1>()) : (wide ? kv4_smem<64, 2>() : kv4_smem<64, 1>());
   if (int r = opt_in_smem(kern, bytes)) return r;
-  const long long rows = (long long)batch * nq;                 // with splits
-  float2* ml = nsplit > 8 ? reinterpret_cast<float2*>(scratch + rows * hq * nsplit * dim) : nullptr;
+  if (q_start == nullptr && (long long)batch * nq != rows) return FF_HOST_BAD_SHAPE;
+  float2* ml = nsplit > 8 ? reinterpret_cast<float2*>(scratch + (long long)rows * hq * nsplit * dim) : nullptr;
   if (int r = launch_pdl(kern, dim3(nsplit, (unsigned)tiles, batch), dim3(32 * KV4_WARPS), bytes, s, nsplit <= 8 ? nsplit : 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
-                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, nsplit > 8 ? scratch : (float*)nullptr, ml, nq, hq, hkv, ldq, ldo, max_blocks,
+                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, nsplit > 8 ? scratch : (float*)nullptr, ml, rows, nq, hq, hkv, ldq, ldo, max_blocks,
                          num_blocks, nsplit, hq == hkv ? 0u : (uint32_t)((0x100000000ull + hq / hkv - 1) / (hq / hkv)), scale * 1.4426950408889634f, status)) return r;
   if (nsplit <= 8) return FF_HOST_OK;
-  return kv4_merge(scratch, ml, nullptr, nullptr, out, batch, nq, hq, dim, ldo, nsplit, s);
+  return kv4_merge(scratch, ml, nullptr, nullptr, out, batch, rows, nq, hq, dim, ldo, nsplit, s);
 }

@@ -67,7 +67,7 @@ template <int D>
 __global__ void __launch_bounds__(32 * KVT_WARPS, 1)
 kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ block_table,
                  const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out,
-                 float* __restrict__ part_o, float2* __restrict__ part_ml, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks, int nsplit,
+                 float* __restrict__ part_o, float2* __restrict__ part_ml, int all_rows, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks, int nsplit,
                  float scale_log2, int* status) {
   constexpr int NG = D / 32, PB = kv4_page_bytes(D), TILE = KVT_N * D * 2, QTILE = KVT_M * D * 2;
   pdl_trigger();
@@ -78,6 +78,10 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
   const int c0 = (int)((gridDim.x - 1 - blockIdx.x) / nsplit) * 2 * KVT_M;          // late rows see the most keys: they start first
   const int rows = n * G - c0;                                            // of this CTA and behind it
   if (rows <= 0) return;
+  if (q_start != nullptr && (q_start[b] < 0 || n > all_rows - q_start[b])) {       // rows that the call does not have
+    if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, q_start[b]);
+    return;
+  }
   extern __shared__ uint8_t smem_raw[];
   __shared__ KvtBars bars;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -401,6 +405,7 @@ FF_EXPORT int ff_kv4_attn_tiles(const void* q, const void* kpages, const void* v
                                 int max_blocks, int num_blocks, int nsplit, float scale, int* status, cudaStream_t s) {
   if (batch <= 0 || batch > 65535 || rows <= 0 || max_q_len <= 0 || hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0)
     return FF_HOST_BAD_SHAPE;
+  if (q_start == nullptr && (long long)batch * max_q_len != rows) return FF_HOST_BAD_SHAPE;
   if (!(scale > 0.f) || (q_start == nullptr) != (q_lens == nullptr) || !ctx_lens || nsplit < 1 || nsplit > 128 || (nsplit > 1 && scratch == nullptr)) return FF_HOST_BAD_SHAPE;
   if (ldq % 8 || ldo % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages) | reinterpret_cast<uintptr_t>(out) |
                               reinterpret_cast<uintptr_t>(scratch)) & 15))
@@ -412,7 +417,7 @@ FF_EXPORT int ff_kv4_attn_tiles(const void* q, const void* kpages, const void* v
   if (int r = opt_in_smem(kern, bytes)) return r;
   float2* ml = nsplit > 1 ? reinterpret_cast<float2*>(scratch + (long long)rows * hq * nsplit * dim) : nullptr;
   if (int r = launch_pdl(kern, dim3((unsigned)grid, hkv, batch), dim3(32 * KVT_WARPS), bytes, s, 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
-                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, scratch, ml, max_q_len, hq, hkv, ldq, ldo, max_blocks,
+                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, scratch, ml, rows, max_q_len, hq, hkv, ldq, ldo, max_blocks,
                          num_blocks, nsplit, scale * 1.4426950408889634f, status)) return r;
-  return nsplit == 1 ? FF_HOST_OK : kv4_merge(scratch, ml, q_start, q_lens, out, batch, max_q_len, hq, dim, ldo, nsplit, s);
+  return nsplit == 1 ? FF_HOST_OK : kv4_merge(scratch, ml, q_start, q_lens, out, batch, rows, max_q_len, hq, dim, ldo, nsplit, s);
 }

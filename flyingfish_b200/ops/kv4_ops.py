@@ -142,7 +142,7 @@ def _lib() -> ctypes.CDLL:
         p, i, n, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
         raw.ff_kv4_write.argtypes = [p, p, p, p, p, i, p, p, f, p, i, i, i, i, n, i, p, p]
         raw.ff_kv4_read.argtypes = [p, p, p, p, p, i, i, i, i, p, p]
-        raw.ff_kv4_attn_rows.argtypes = [p, p, p, p, p, p, p, p, p, i, i, i, i, i, n, n, i, i, i, f, p, p]
+        raw.ff_kv4_attn_rows.argtypes = [p, p, p, p, p, p, p, p, p, i, i, i, i, i, i, n, n, i, i, i, f, p, p]
         raw.ff_kv4_attn_tiles.argtypes = [p, p, p, p, p, p, p, p, p, i, i, i, i, i, i, n, n, i, i, i, f, p, p]
         raw.ff_copy_pages.argtypes = [p, p, i, p, p, i, p]
         _bound = lib
@@ -263,6 +263,7 @@ def _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq
         n, at, ctx = int(q_lens[b]), int(q_start[b]), int(ctx_lens[b])
         if n == 0:
             continue
+        _require(0 <= at <= q.shape[0] - n, "attention over 4-bit pages: rows that the call does not have")
         _require(ctx <= block_table.shape[1] * PAGE, "attention over 4-bit pages: more keys than the block table has pages")
         res[at: at + n] = 0.0
         if ctx <= 0:
@@ -306,11 +307,11 @@ def _attention(q, ldq, kpages, vpages, blocks, block_table, q_start, q_lens, ctx
     scratch = torch.empty(floats.value, dtype=torch.float32, device=q.device) if floats.value else None
     tail = (hq, hkv, dim, ldq, out.stride(0), width, blocks, nsplit, scale, status_tensor(q.device).data_ptr(), _stream())
     head = (q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), block_table.data_ptr(), None if q_start is None else q_start.data_ptr(),
-            None if q_lens is None else q_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), None if scratch is None else scratch.data_ptr(), batch)
+            None if q_lens is None else q_lens.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), None if scratch is None else scratch.data_ptr(), batch, rows, nq)
     if tiles:
-        check(lib.ff_kv4_attn_tiles(*head, rows, nq, *tail), "ff_kv4_attn_tiles")
+        check(lib.ff_kv4_attn_tiles(*head, *tail), "ff_kv4_attn_tiles")
     else:
-        check(lib.ff_kv4_attn_rows(*head, nq, *tail), "ff_kv4_attn_rows")
+        check(lib.ff_kv4_attn_rows(*head, *tail), "ff_kv4_attn_rows")
     _count(1 if scratch is None else 2)
     return out
 

@@ -155,6 +155,11 @@ def test_what_the_operators_refuse():
                dict(ctx_lens=ctx.long()), dict(q=q.float()), dict(out=torch.empty(3, hq * dim)), dict(dim=128)):
         with pytest.raises(KernelError):
             decode(**kw)
+    prefill = lambda start, n: kv4_ops.attn_prefill_kv4(q, kp, vp, table[:1], torch.tensor([start], dtype=torch.int32), torch.tensor([n], dtype=torch.int32), ctx[:1], 3, hq, hkv, dim, 0.1)
+    prefill(0, 3)
+    for start, n in ((1, 3), (-1, 2), (3, 1)):
+        with pytest.raises(KernelError):
+            prefill(start, n)
     one = torch.tensor([0], dtype=torch.int32)
     with pytest.raises(KernelError):
         kv4_ops.attn_prefill_kv4(q, kp, vp, table, one, one, ctx, 3, hq, hkv, dim, 0.1)
@@ -273,6 +278,43 @@ def test_slots_and_pages_outside_the_cache_raise_the_status():
     for table, ctx in ((2, 5), (-1, 5), (0, 65)):
         assert _status_of(lambda: kv4_ops.attn_decode_kv4(qkv, *pages, i32(table).view(1, 1), i32(ctx), hq, hkv, dim, 0.1)) == 3
         assert _status_of(lambda: kv4_ops.attn_prefill_kv4(qkv, *pages, i32(table).view(1, 1), i32(0), i32(1), i32(ctx), 1, hq, hkv, dim, 0.1)) == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start,n,most", [(30, 11, 11), (-1, 5, 5), (41, 1, 1), (1 << 30, 3, 3)])
+def test_rows_that_a_call_does_not_have_raise_the_status(start, n, most):
+    dim, hq, hkv = 64, 16, 2
+    kp, vp, table = _cache([100], hkv, dim, 4, "cuda")
+    q, i32 = _rows(40, hq * dim, 3).cuda(), lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")
+    for more in (most, 40):                                                 # either kernel
+        out = torch.full((40, hq * dim), 3.0, dtype=BF16, device="cuda")
+        assert _status_of(lambda: kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(start), i32(n), i32(100), more, hq, hkv, dim, 0.1, out=out)) == 3
+        assert bool((out == 3).all())
+
+
+@pytest.mark.gpu
+def test_pages_behind_4_gib():
+    """Pages whose offsets pass 32 bits: written, attended to by both kernels, read back and copied."""
+    dim, hq, hkv, blocks = 128, 32, 4, 230000
+    pages = [torch.empty(blocks, hkv, kv4_ops.page_bytes(dim), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    assert pages[0].nbytes > 1 << 32
+    small, table = _cache([150], hkv, dim, 5, "cuda")[:2], torch.tensor([[blocks - 1, 3, blocks - 7]], dtype=torch.int32, device="cuda")
+    kp, vp, near = _cache([150], hkv, dim, 5, "cuda")
+    for big, little in zip(pages, small):
+        big[table[0].long()] = little[near[0].long()]
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    q = _rows(20, (hq + 2 * hkv) * dim, 3).cuda()
+    for n in (1, 20):
+        args = (i32(0), i32(n), i32(150), n, hq, hkv, dim, 0.1)
+        assert torch.equal(kv4_ops.attn_prefill_kv4(q[:n], *pages, table, *args), kv4_ops.attn_prefill_kv4(q[:n], kp, vp, near, *args))
+    slot = i32((blocks - 1) * PAGE + 5)
+    kv4_ops.write_kv4(q[:1], slot, *pages, hq, hkv, dim)
+    kv4_ops.copy_pages(pages, [blocks - 1], [blocks - 2])
+    a, b = (kv4_ops.read_kv4(*pages, slot - d, dim) for d in (0, PAGE))
+    code, scale, lo = kv4_ops.quantise(q[:1, hq * dim: (hq + hkv) * dim].cpu().view(1, hkv, dim))
+    want = code.double() * scale.double().repeat_interleave(32, -1) + lo.double().repeat_interleave(32, -1)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and bool(((a[0].cpu().double() - want).abs() <= want.abs() * E).all())
+    assert ops.read_status()[0] == 0
 
 
 def _close(got, want, mag, off, tot, rounded=False):
