@@ -96,12 +96,12 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   auto group_of = [&](int c) -> int { return per_group ? (int)__umulhi((uint32_t)c, per_group) : c; };      // c / G
   const int n = q_lens ? q_lens[b] : nq, row0 = q_start ? q_start[b] : b * nq;
   int ctx = ctx_lens[b];
-  const int columns = n * G - ct * NT * 8;                      // of this CTA and behind it
-  if (columns <= 0) return;
-  if (row0 < 0 || n > rows - row0) {                            // rows that the call does not have
+  if (n > 0 && (n > nq || row0 < 0 || n > rows - row0)) {       // rows that the call does not have
     if (threadIdx.x == 0) set_status(status, KID_ATTN_DECODE, FF_ERR_BOUNDS, b, row0);
     return;
   }
+  const int columns = n * G - ct * NT * 8;                      // of this CTA and behind it
+  if (columns <= 0) return;
   // queries of this thread's column of B fragments (column g of every 8): 8 elements of each group
   uint4 qv[NT][NG];
 #pragma unroll
@@ -180,7 +180,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       sq[nt][j][lane] = make_uint4(f[0], f[1], f[2], f[3]);
       if (t == 0) ssum[nt][j][g] = s * 5.9604644775390625e-8f;                       // 2^-24
     }
-    const float f = scale_log2 * back;
+    const float f = fmaxf(scale_log2 * back, 1.1754944e-38f);   // (times minus infinity it has to be that)
     cf[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);             // column 2 t is held by lanes of g = 2 t
     cf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
@@ -429,7 +429,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     }
     const int c = ct * NT * 8 + col, qi = group_of(c), head = kvh * G + c - qi * G;
     if (nsplit == 1) {
-      out[(size_t)(row0 + qi) * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+      out[(size_t)(row0 + qi) * ldo + (size_t)head * D + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
     } else if (cluster) {
       mo[i] = acc;
       if (d == 0) { mml[2 * col] = M; mml[2 * col + 1] = L; }
@@ -456,7 +456,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
           acc = fmaf(kv4_peer(mo + i, r), sc, acc);
         }
       const int c = ct * NT * 8 + col, qi = group_of(c), head = kvh * G + c - qi * G;
-      out[(size_t)(row0 + qi) * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? acc / L : 0.f);
+      out[(size_t)(row0 + qi) * ldo + (size_t)head * D + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
     }
     cluster_sync_all();                                         // no CTA leaves while its shared memory is read
   }
@@ -475,7 +475,7 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.y, qi = blockIdx.x / hq, head = blockIdx.x - qi * hq;
   const int n = q_lens ? q_lens[b] : nq, row0 = q_start ? q_start[b] : b * nq, row = row0 + qi;
-  if (qi >= n || row0 < 0 || n > rows - row0) return;
+  if (qi >= n || n > nq || row0 < 0 || n > rows - row0) return;
   const size_t pr = ((size_t)row * hq + head) * nsplit;
   float2 ml[4];                                                 // of splits lane, lane + 32, ... (at most 128)
   float M = KV4_NONE, L = 0.f;
@@ -501,7 +501,7 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
         sc[u] = __shfl_sync(0xffffffffu, ml[i].x, at & 31);
         if (at >= min(nsplit, 32 * i + 32)) sc[u] = 0.f;
 #pragma unroll
-        for (int k = 0; k < E; ++k) v[u][k] = sc[u] > 0.f ? part_o[(pr + at) * D + lane + 32 * k] : 0.f;
+        for (int k = 0; k < E; ++k) v[u][k] = sc[u] != 0.f ? part_o[(pr + at) * D + lane + 32 * k] : 0.f;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
@@ -514,7 +514,7 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
   const int d = threadIdx.x;
   if (d < D) {
     const float o = (sacc[0][d] + sacc[1][d]) + (sacc[2][d] + sacc[3][d]);
-    out[(size_t)row * ldo + (size_t)head * D + d] = __float2bfloat16(L > 0.f ? o / L : 0.f);
+    out[(size_t)row * ldo + (size_t)head * D + d] = __float2bfloat16(L == 0.f ? 0.f : o / L);
   }
 }
 

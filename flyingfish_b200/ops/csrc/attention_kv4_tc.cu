@@ -76,12 +76,13 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
   const int n = q_lens ? q_lens[b] : nq;
   const int split = blockIdx.x % nsplit;
   const int c0 = (int)((gridDim.x - 1 - blockIdx.x) / nsplit) * 2 * KVT_M;          // late rows see the most keys: they start first
-  const int rows = n * G - c0;                                            // of this CTA and behind it
-  if (rows <= 0) return;
-  if (q_start != nullptr && (q_start[b] < 0 || n > all_rows - q_start[b])) {       // rows that the call does not have
-    if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, q_start[b]);
+  const int row0 = q_start ? q_start[b] : b * nq;
+  if (n > 0 && (n > nq || row0 < 0 || n > all_rows - row0)) {             // rows that the call does not have
+    if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, row0);
     return;
   }
+  const int rows = n * G - c0;                                            // of this CTA and behind it
+  if (rows <= 0) return;
   extern __shared__ uint8_t smem_raw[];
   __shared__ KvtBars bars;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -96,7 +97,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
     if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, ctx);
     ctx = max_blocks * KV4_PAGE;
   }
-  const int past = ctx - n, row0 = q_start ? q_start[b] : b * nq;
+  const int past = ctx - n;
   const int seen = past + (c0 + min(rows, 2 * KVT_M) - 1) / G + 1;        // keys that the last row sees
   const int pages = (max(seen, 0) + KVT_N - 1) / KVT_N, per = max((pages + nsplit - 1) / nsplit, 4);
   const int first = split * per, tiles = max(0, min(pages, first + per) - first);    // pages of this split
@@ -254,7 +255,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         for (int k = 0; k < D / 2; ++k) { const float2 v = unpack_bf16x2(w[k]); most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))); }
         const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);          // 2^(e - 127), and its inverse
         const float up = __uint_as_float(e << 23), down = __uint_as_float((254u - e) << 23);
-        row_scale *= up;
+        row_scale = fmaxf(row_scale * up, 1.1754944e-38f);       // (times minus infinity it has to be that)
         const uint32_t dst = smem_u32(sQ) + i * QTILE + row * 128;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) {
@@ -347,7 +348,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        const float l = l0 + l1, inv = l > 0.f ? 1.f / l : 0.f;
+        const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l;
         __nv_bfloat16* dst = out + (size_t)(row0 + qi) * ldo + (size_t)head * D;
         const size_t pr = ((size_t)(row0 + qi) * hq + head) * nsplit + split;
         if (nsplit > 1 && live) part_ml[pr] = make_float2(m_ref == -INFINITY ? -3.0e38f : m_ref, l);
@@ -357,7 +358,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           if (tiles > 0) { tmem_ld_x16(tmem_o + k, r); tmem_ld_wait(); }
           if (!live) continue;
           if (nsplit > 1) {
-            if (l > 0.f) {                                       // (the merge does not read what has no weight)
+            if (l != 0.f) {                                      // (the merge does not read what has no weight)
 #pragma unroll
               for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part_o + pr * D + k + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
             }
@@ -365,7 +366,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           }
           uint32_t o[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = l > 0.f ? pack_bf16x2(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv) : 0u;
+          for (int e = 0; e < 8; ++e) o[e] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv);
           reinterpret_cast<uint4*>(dst + k)[0] = make_uint4(o[0], o[1], o[2], o[3]);
           reinterpret_cast<uint4*>(dst + k)[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }

@@ -6,7 +6,7 @@ group's least element, ``scale`` its span / 15 rounded to BF16, a code is 0 .. 1
 element stands for is off by half a scale at most, and by the rounding of the scale (2^-8 of it for each step up to 15). That is 160 bytes a token and
 head of 128 where BF16 pages take 512. Every token is quantised by itself, so rows may be taken back and written again, and pages may be copied.
 
-CUDA: ``csrc/kv4.cu`` and ``csrc/attention_kv4.cu``; the byte layout is in ``csrc/kv4.cuh``. CPU: the oracles below. Slots, block tables and lengths are
+CUDA: ``csrc/kv4.cu``, ``csrc/attention_kv4.cu`` and ``csrc/attention_kv4_tc.cu``; the byte layout is in ``csrc/kv4.cuh``. CPU: the oracles below. Slots, block tables and lengths are
 those of the BF16 cache (``ops.rope_kv_paged``, ``ops.attn_decode``, ``ops.attn_prefill``). Calls keep no state of their own and share no scratch: any stream may
 be current, also one that is captured, as long as the tensors are on the current device."""
 from __future__ import annotations
@@ -274,7 +274,7 @@ def _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq
         x = q[at: at + n, : hq * dim].float().view(n, hkv, hq // hkv, dim)
         score = torch.einsum("nhgd,hkd->hgnk", x, k) * scale
         hidden = torch.arange(ctx)[None, :] > torch.arange(ctx - n, ctx)[:, None]
-        p = torch.softmax(score.masked_fill(hidden, float("-inf")), dim=-1).nan_to_num(0.0)
+        p = torch.softmax(score.masked_fill(hidden, float("-inf")), dim=-1).masked_fill(hidden.all(-1, keepdim=True), 0.0)
         res[at: at + n] = torch.einsum("hgnk,hkd->nhgd", p, v).reshape(n, hq, dim)
     res = res.view(q.shape[0], hq * dim).to(BF16)
     if out is None:
@@ -334,7 +334,7 @@ def attn_prefill_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
                      ctx_lens: torch.Tensor, max_q_len: int, hq: int, hkv: int, dim: int, scale: float, max_ctx: int | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed rows over 4-bit pages: sequence b has the ``q_lens[b]`` rows from ``q_start[b]`` on (at most ``max_q_len``), the last of which
-    sees ``ctx_lens[b]`` keys. Rows that belong to no sequence stay as they are in ``out`` (undefined without one). ``max_ctx`` as in :func:`attn_decode_kv4`.
+    sees ``ctx_lens[b]`` keys. A sequence with more rows than ``max_q_len``, or with rows that ``q`` does not have, raises the device status and gets nothing. Rows that belong to no sequence stay as they are in ``out`` (undefined without one). ``max_ctx`` as in :func:`attn_decode_kv4`.
     Returns ``[rows, hq * dim]``."""
     ldq, blocks = _check_attention("attn_prefill_kv4", q, kpages, vpages, block_table, ctx_lens, hq, hkv, dim, scale, out)
     _check_ints("attn_prefill_kv4", block_table.shape[0], q_start, q_lens)
@@ -342,6 +342,7 @@ def attn_prefill_kv4(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor
     if max_q_len <= 0:
         raise KernelError("attn_prefill_kv4: at least one row")
     if not q.is_cuda:
+        _require(bool((q_lens <= max_q_len).all()), "attn_prefill_kv4: more rows of a sequence than max_q_len")
         return _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq, hkv, dim, scale, out)
     return _attention(q, ldq, kpages, vpages, blocks, block_table, q_start, q_lens, ctx_lens, max_q_len, hq, hkv, dim, scale, max_ctx, out)
 

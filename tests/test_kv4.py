@@ -157,7 +157,7 @@ def test_what_the_operators_refuse():
             decode(**kw)
     prefill = lambda start, n: kv4_ops.attn_prefill_kv4(q, kp, vp, table[:1], torch.tensor([start], dtype=torch.int32), torch.tensor([n], dtype=torch.int32), ctx[:1], 3, hq, hkv, dim, 0.1)
     prefill(0, 3)
-    for start, n in ((1, 3), (-1, 2), (3, 1)):
+    for start, n in ((1, 3), (-1, 2), (3, 1), (0, 4)):
         with pytest.raises(KernelError):
             prefill(start, n)
     one = torch.tensor([0], dtype=torch.int32)
@@ -230,9 +230,6 @@ def test_head_norms_before_the_turn():
     w = [torch.rand(dim, generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i in (6, 7)]
     pages = [kv4_ops.new_pages(1, hkv, dim, "cuda") for _ in range(2)]
     got = kv4_ops.write_kv4(qkv, slots, *pages, hq, hkv, dim, turn, *w, 1e-6)
-    # the BF16 cache's kernel, normed and turned the same way
-    cache = [torch.zeros(1, hkv, PAGE, dim, dtype=BF16, device="cuda") for _ in range(2)]
-    packed = qkv.clone()
     cpu = [t.cpu() for t in (qkv, slots, *w)]
     x = cpu[0].view(rows, -1, dim).double()
     rms = lambda t, g: t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-6) * g.double()
@@ -248,7 +245,6 @@ def test_head_norms_before_the_turn():
     step = ((span.amax(-1) - span.amin(-1)) / 15).repeat_interleave(32, -1)
     wide = tol[:, hq:].unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1)       # the group's ends move too
     assert bool(((k.cpu().double() - exact[:, hq:]).abs() <= step * 0.55 + 4 * wide).all())
-    del cache, packed
 
 
 @pytest.mark.gpu
@@ -281,12 +277,12 @@ def test_slots_and_pages_outside_the_cache_raise_the_status():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("start,n,most", [(30, 11, 11), (-1, 5, 5), (41, 1, 1), (1 << 30, 3, 3)])
+@pytest.mark.parametrize("start,n,most", [(30, 11, 11), (-1, 5, 5), (41, 1, 1), (1 << 30, 3, 3), (0, 4, 3), (0, 0x7ffffff0, 3)])
 def test_rows_that_a_call_does_not_have_raise_the_status(start, n, most):
     dim, hq, hkv = 64, 16, 2
     kp, vp, table = _cache([100], hkv, dim, 4, "cuda")
     q, i32 = _rows(40, hq * dim, 3).cuda(), lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")
-    for more in (most, 40):                                                 # either kernel
+    for more in (most, 40 if n <= most else most):                          # either kernel
         out = torch.full((40, hq * dim), 3.0, dtype=BF16, device="cuda")
         assert _status_of(lambda: kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(start), i32(n), i32(100), more, hq, hkv, dim, 0.1, out=out)) == 3
         assert bool((out == 3).all())
@@ -314,6 +310,39 @@ def test_pages_behind_4_gib():
     code, scale, lo = kv4_ops.quantise(q[:1, hq * dim: (hq + hkv) * dim].cpu().view(1, hkv, dim))
     want = code.double() * scale.double().repeat_interleave(32, -1) + lo.double().repeat_interleave(32, -1)
     assert all(torch.equal(x, y) for x, y in zip(a, b)) and bool(((a[0].cpu().double() - want).abs() <= want.abs() * E).all())
+    assert ops.read_status()[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [41, 0x7ffffff0])
+def test_more_rows_than_a_tile_kernels_call_has_raise_the_status(n):
+    dim, hq, hkv = 128, 8, 2
+    kp, vp, table = _cache([100], hkv, dim, 4, "cuda")
+    q, i32 = _rows(60, hq * dim, 3).cuda(), lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")
+    out = torch.full((60, hq * dim), 3.0, dtype=BF16, device="cuda")
+    assert _status_of(lambda: kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(0), i32(n), i32(100), 40, hq, hkv, dim, 0.1, out=out)) == 3
+    assert bool((out == 3).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,hq,hkv,nq,ctx", [(128, 8, 2, 3, 900), (64, 2, 2, 2, 300), (128, 8, 1, 1, 9000), (128, 8, 2, 70, 900), (64, 4, 4, 300, 320)])
+def test_queries_of_no_number_and_of_no_size(dim, hq, hkv, nq, ctx):
+    """A NaN among the queries makes its head's output NaN and no other's; queries of zero and of 2^-110, also with a scale near the least, attend evenly."""
+    kp, vp, table = _cache([ctx], hkv, dim, 6, "cuda")
+    q, lens = _rows(nq, hq * dim, 13).cuda(), torch.tensor([ctx], dtype=torch.int32, device="cuda")
+    run = lambda x, scale: kv4_ops.attn_decode_kv4(x, kp, vp, table, lens, hq, hkv, dim, scale, nq=nq).view(nq, hq, dim)
+    plain, bad = run(q, 0.1), q.clone()
+    bad.view(nq, hq, dim)[nq - 1, 1, 7] = float("nan")
+    got = run(bad, 0.1)
+    assert bool(got[nq - 1, 1].isnan().all())
+    got[nq - 1, 1] = plain[nq - 1, 1]
+    assert torch.equal(got, plain)
+    q.view(nq, hq, dim)[:, 0] = 0
+    q.view(nq, hq, dim)[:, 1] = 2.0 ** -110
+    tiles = kv4_ops.in_tiles(nq, hq, hkv)
+    for scale in (0.1, 1e-30):
+        want = _definition(q, kp, vp, table, [(0, nq, ctx)], hq, hkv, dim, scale, rounded=tiles)
+        _close(run(q, scale).reshape(nq, hq * dim), *want, rounded=tiles)
     assert ops.read_status()[0] == 0
 
 
