@@ -153,6 +153,26 @@ def test_samples_of_one_prompt_are_those_of_separate_requests_cpu():
     assert m.generate_samples(ids, [], 4) == []
 
 
+@pytest.mark.parametrize("kv_format", ["bf16", "affine4"])
+def test_forks_keep_their_adapter_cpu(kv_format):
+    g = torch.Generator().manual_seed(1)
+    new = lambda n, k: (torch.randn(n, k, generator=g) * 0.1).to(torch.bfloat16)
+    poet = {(l, p): (new(8, 512), new(n, 8), 2.0) for l in (0, 1) for p, n in (("q_proj", 512), ("v_proj", 128), ("o_proj", 512))}
+    m = Model.load("tiny-llama", Settings(capacity=256, max_batch=4, graph=False, kv_format=kv_format), device="cpu", seed=0, adapters={"poet": poet})
+    eng, ids = m.engine, _prompt(70)
+    want = eng.generate([ids], 7, adapter="poet")[0]
+    assert want != eng.generate([ids], 7)[0]
+    a = eng.add_sequence(ids, adapter="poet")
+    eng.prefill([a]); eng.decode([a])
+    b, again = eng.fork(a), eng.fork(a, again=True)
+    eng.prefill([again])
+    for _ in range(5):
+        eng.decode([b, again])
+    eng.decode([again])
+    assert b.output == want and again.output[:7] == want
+    assert m.generate_samples(ids, [Sampling(temperature=0)] * 2, 7, adapter="poet") == [want] * 2
+
+
 def test_stored_prefixes_are_the_pages(tmp_path):
     m = _load("cpu")
     ids = _prompt(100)
@@ -182,10 +202,10 @@ def test_cli_generates_over_4_bit_pages(capsys):
 # on the device
 # ------------------------------------------------------------------------------------------
 @pytest.mark.gpu
-@pytest.mark.parametrize("graph", [False, True])
-def test_a_model_goes_on_over_4_bit_pages(graph):
+@pytest.mark.parametrize("graph,shape", [(False, "tiny-llama"), (True, "tiny-llama"), (True, "qwen3-moe-tiny")])
+def test_a_model_goes_on_over_4_bit_pages(graph, shape):
     """Against the same model on the CPU: logits of a prompt within the two paths' roundings, and the same pages but for codes next to a border."""
-    m, c = _load("cuda", graph=graph, capacity=1024), _load("cpu", capacity=1024)
+    m, c = _load("cuda", graph=graph, capacity=1024, shape=shape), _load("cpu", capacity=1024, shape=shape)
     prompts = [_prompt(300), _prompt(5, 12), _prompt(64, 13)]
     seqs = [m.engine.add_sequence(p) for p in prompts]
     m.engine.prefill(seqs)
