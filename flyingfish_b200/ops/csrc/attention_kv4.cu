@@ -466,16 +466,13 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
 // other, 74 splits of a single sequence took as long as the attention itself).
 template <int D>
 __global__ void __launch_bounds__(128)
-kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int* __restrict__ q_start, const int* __restrict__ q_lens,
-                 __nv_bfloat16* __restrict__ out, int rows, int nq, int hq, long long ldo, int nsplit) {
+kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, __nv_bfloat16* __restrict__ out, int hq, long long ldo, int nsplit) {
   constexpr int E = D / 32;
   __shared__ float sacc[4][D];
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.y, qi = blockIdx.x / hq, head = blockIdx.x - qi * hq;
-  const int n = q_lens ? q_lens[b] : nq, row0 = q_start ? q_start[b] : b * nq, row = row0 + qi;
-  if (qi >= n || n > nq || row0 < 0 || n > rows - row0) return;
+  const int row = blockIdx.x / hq, head = blockIdx.x - row * hq;
   const size_t pr = ((size_t)row * hq + head) * nsplit;
   float2 ml[4];                                                 // of splits lane, lane + 32, ... (at most 128)
   float M = KV4_NONE, L = 0.f;
@@ -534,13 +531,6 @@ FF_EXPORT int ff_kv4_attn_plan(int batch, int hq, int hkv, int nq, int dim, int 
   return (int)nsplit;
 }
 
-int kv4_merge(const float* part_o, const float2* part_ml, const int* q_start, const int* q_lens, void* out, int batch, int rows, int nq, int hq, int dim,
-              long long ldo, int nsplit, cudaStream_t s) {
-  if ((long long)nq * hq > 0x7fffffffll) return FF_HOST_TOO_LARGE;
-  return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(nq * hq), batch), dim3(128), 0, s, 0, part_o, part_ml, q_start, q_lens,
-                    (__nv_bfloat16*)out, rows, nq, hq, ldo, nsplit);
-}
-
 // q rows [rows, ldq] with head h at column h dim; sequence b has rows q_start[b] .. + q_lens[b], or nq rows from b nq on where those are null (only then may
 // there be more than eight splits); ctx_lens[b] keys are seen by the last of them. Rows of no keys are zero.
 FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vpages, const int* block_table, const int* q_start, const int* q_lens,
@@ -562,5 +552,7 @@ FF_EXPORT int ff_kv4_attn_rows(const void* q, const void* kpages, const void* vp
                          (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, nsplit > 8 ? scratch : (float*)nullptr, ml, rows, nq, hq, hkv, ldq, ldo, max_blocks,
                          num_blocks, nsplit, hq == hkv ? 0u : (uint32_t)((0x100000000ull + hq / hkv - 1) / (hq / hkv)), scale * 1.4426950408889634f, status)) return r;
   if (nsplit <= 8) return FF_HOST_OK;
-  return kv4_merge(scratch, ml, nullptr, nullptr, out, batch, rows, nq, hq, dim, ldo, nsplit, s);
+  if ((long long)rows * hq > 0x7fffffffll) return FF_HOST_TOO_LARGE;
+  return launch_pdl(dim == 128 ? kv4_merge_kernel<128> : kv4_merge_kernel<64>, dim3((unsigned)(rows * hq)), dim3(128), 0, s, 0, (const float*)scratch, (const float2*)ml,
+                    (__nv_bfloat16*)out, hq, ldo, nsplit);
 }

@@ -63,19 +63,145 @@ __device__ __forceinline__ void kvt_bulk_load(void* dst, const void* src, uint32
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
+// Several sequences of long contexts, which differ: one CTA makes a list of what there is to do, long tile pairs cut into pieces of equal size, the largest first (the
+// next SM that is free takes the next one). Each is a CTA of the kernel below for every kv head. Two tile pairs of 470 pages beside sixty of 90 and less: 530 us as they
+// lie, 365 so.
+struct KvtPlan {
+  int* count;             // pieces; tile pairs of more than one
+  int4* item;             // piece: sequence, first flattened row, first page, pages
+  int4* join;             // tile pair of more than one: sequence, first flattened row, pieces, slot of the first
+  int* slot;              // where a piece leaves its part of the result, -1: it is the only one
+  int items, joins, slots;
+};
+// A piece is at most as large as the longest tile pair, or as an SM's share of all pages over 1, 1.5 or 2 (KVT_SHARE): whichever should end first.
+constexpr int KVT_PLAN_WARPS = 16, KVT_CLASSES = 32, KVT_CUTS = 4, KVT_SHARE = 2;
+constexpr int KVT_EXTRA = 6, KVT_PART = 4;                                // pages' time that a CTA takes beside its pages, and for a part's way out and in again
+constexpr int KVT_SEQS = 2048;                                            // sequences of a list at most
+constexpr int KVT_LIST = 32;                                              // pages of a context from which a list is made (it takes 6 us)
+
+__device__ __forceinline__ int kvt_pages(int past, int c0, int rows, int G) { return (max(past + (c0 + min(rows, 2 * KVT_M) - 1) / G + 1, 0) + KVT_N - 1) / KVT_N; }
+
+__global__ void __launch_bounds__(32 * KVT_PLAN_WARPS)
+kv4_plan_kernel(const KvtPlan plan, const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, int batch, int all_rows, int nq, int G,
+                int hkv, int max_blocks, int sms, int* status) {
+  __shared__ int s_n[KVT_SEQS], s_past[KVT_SEQS];
+  __shared__ unsigned long long s_all;
+  __shared__ int s_most, s_class[KVT_CUTS][KVT_CLASSES], s_slots, s_joins;
+  __shared__ float s_end[KVT_CUTS];
+  __shared__ int s_pieces[KVT_CUTS];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < KVT_CUTS * KVT_CLASSES) s_class[threadIdx.x / KVT_CLASSES][threadIdx.x % KVT_CLASSES] = 0;
+  if (threadIdx.x == 0) { s_all = 0; s_most = 1; s_slots = 0; s_joins = 0; }
+  pdl_wait();
+  for (int b = threadIdx.x; b < batch; b += 32 * KVT_PLAN_WARPS) {
+    int n = q_lens ? q_lens[b] : nq;
+    const int row0 = q_start ? q_start[b] : b * nq, ctx = ctx_lens[b];
+    if (n > 0 && (n > nq || row0 < 0 || n > all_rows - row0)) {   // rows that the call does not have
+      set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, row0);
+      n = 0;
+    }
+    s_n[b] = max(n, 0);
+    s_past[b] = min(max(ctx, 0), max_blocks * KV4_PAGE) - n;
+  }
+  __syncthreads();
+  auto each = [&](auto&& f) {                                    // f(sequence, first row, pages) for every tile pair: a warp has a sequence, a lane a tile pair
+    for (int b = warp; b < batch; b += KVT_PLAN_WARPS) {
+      const int n = s_n[b], past = s_past[b];
+      for (int c0 = lane * 2 * KVT_M; c0 < n * G; c0 += 32 * 2 * KVT_M) f(b, c0, kvt_pages(past, c0, n * G - c0, G));
+    }
+  };
+  unsigned long long all = 0;
+  int most = 1;
+  each([&](int, int, int pages) { all += pages + KVT_EXTRA; most = max(most, pages); });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { all += __shfl_xor_sync(0xffffffffu, all, o); most = max(most, __shfl_xor_sync(0xffffffffu, most, o)); }
+  if (lane == 0) { atomicAdd(&s_all, all); atomicMax(&s_most, most); }
+  __syncthreads();
+  most = s_most;
+  // sizes to choose from (at most 128 pieces of a tile pair), and how many pieces of which size each gives (size classes, the largest first)
+  const float share = (float)s_all * hkv / sms;
+  auto size_of = [&](int j) { return j == 0 ? most : min(most, max((int)min(share / (0.5f + 0.5f * j) + 1.f, 1.0e9f), max(4, (most + 127) / 128))); };
+  auto cut = [&](int pages, int size, int& ns, int& per) { ns = max((pages + size - 1) / size, 1); per = (pages + ns - 1) / ns; };
+  auto size_class = [&](int per) { return KVT_CLASSES - 1 - (int)((long long)per * (KVT_CLASSES - 1) / most); };
+  int sizes[KVT_CUTS];
+#pragma unroll
+  for (int j = 0; j < KVT_CUTS; ++j) sizes[j] = size_of(j);
+  each([&](int, int, int pages) {
+#pragma unroll
+    for (int j = 0; j < KVT_CUTS; ++j) { int ns, per; cut(pages, sizes[j], ns, per); atomicAdd(&s_class[j][size_class(per)], ns); }
+  });
+  __syncthreads();
+  if (warp < KVT_CUTS) {
+    // When the last piece should end: not before an SM's share of them all, nor before i + 1 times the (i sms + 1)-th largest, as one SM has i + 1 of these
+    const int own = s_class[warp][lane];
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
+    const float pages = (float)(KVT_CLASSES - 1 - lane) * most / (KVT_CLASSES - 1) + KVT_EXTRA + (warp > 0 ? KVT_PART : 0);
+    float end = own > 0 ? (float)(((long long)sum * hkv - 1) / sms + 1) * pages : 0.f, work = own * pages;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { end = fmaxf(end, __shfl_xor_sync(0xffffffffu, end, o)); work += __shfl_xor_sync(0xffffffffu, work, o); }
+    if (lane == 0) s_end[warp] = fmaxf(end, work * hkv / sms);
+    __syncwarp();
+    s_class[warp][lane] = sum - own;
+    if (lane == 31) s_pieces[warp] = sum;
+  }
+  __syncthreads();
+  int best = 0;
+#pragma unroll
+  for (int j = 1; j < KVT_CUTS; ++j)
+    if (s_end[j] < s_end[best] * 0.97f) best = j;
+  const int size = size_of(best);
+  if (threadIdx.x == 0) plan.count[0] = min(s_pieces[best], plan.items);
+  each([&](int b, int c0, int pages) {
+    int ns, per;
+    cut(pages, size, ns, per);
+    const int at = atomicAdd(&s_class[best][size_class(per)], ns);
+    int slot = -1, j = 0;
+    if (ns > 1) {
+      slot = atomicAdd(&s_slots, ns);
+      j = atomicAdd(&s_joins, 1);
+    }
+    if (at + ns > plan.items || (ns > 1 && (slot + ns > plan.slots || j >= plan.joins))) {      // (sequences that overlap have more rows than there is room for)
+      set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
+      for (int s = at; s < min(at + ns, plan.items); ++s) { plan.item[s] = make_int4(-1, 0, 0, 0); plan.slot[s] = -1; }
+      if (ns > 1 && j < plan.joins) plan.join[j] = make_int4(b, c0, 0, 0);
+      return;
+    }
+    for (int s = 0; s < ns; ++s) {
+      plan.item[at + s] = make_int4(b, c0, s * per, max(0, min(pages - s * per, per)));
+      plan.slot[at + s] = ns > 1 ? slot + s : -1;
+    }
+    if (ns > 1) plan.join[j] = make_int4(b, c0, ns, slot);
+  });
+  __syncthreads();
+  if (threadIdx.x == 0) plan.count[1] = min(s_joins, plan.joins);
+}
+
 template <int D>
 __global__ void __launch_bounds__(32 * KVT_WARPS, 1)
 kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ block_table,
                  const int* __restrict__ q_start, const int* __restrict__ q_lens, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out,
-                 float* __restrict__ part_o, float2* __restrict__ part_ml, int all_rows, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks, int nsplit,
+                 float* __restrict__ part_o, float2* __restrict__ part_ml, const KvtPlan plan, int all_rows, int nq, int hq, int hkv, long long ldq, long long ldo, int max_blocks, int num_blocks, int nsplit,
                  float scale_log2, int* status) {
   constexpr int NG = D / 32, PB = kv4_page_bytes(D), TILE = KVT_N * D * 2, QTILE = KVT_M * D * 2;
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.z, kvh = blockIdx.y, G = hq / hkv;
+  const int G = hq / hkv;
+  int b = blockIdx.z, kvh = blockIdx.y, c0 = 0, first = 0, tiles = 0, slot = -1;
+  if (plan.count != nullptr) {
+    const int at = blockIdx.x / hkv;
+    kvh = blockIdx.x - at * hkv;
+    if (at >= plan.count[0]) return;
+    const int4 v = plan.item[at];
+    b = v.x; c0 = v.y; first = v.z; tiles = v.w;
+    slot = plan.slot[at];
+    if (b < 0) return;
+  } else {
+    c0 = (int)((gridDim.x - 1 - blockIdx.x) / nsplit) * 2 * KVT_M;        // late rows see the most keys: they start first
+  }
   const int n = q_lens ? q_lens[b] : nq;
-  const int split = blockIdx.x % nsplit;
-  const int c0 = (int)((gridDim.x - 1 - blockIdx.x) / nsplit) * 2 * KVT_M;          // late rows see the most keys: they start first
   const int row0 = q_start ? q_start[b] : b * nq;
   if (n > 0 && (n > nq || row0 < 0 || n > all_rows - row0)) {             // rows that the call does not have
     if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, row0);
@@ -92,15 +218,18 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
   uint8_t* const sP = sV + KVT_STAGES * TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int two = rows > KVT_M ? 2 : 1;                                   // tiles of this CTA
-  int ctx = ctx_lens[b];
+  int ctx = max(ctx_lens[b], 0);
   if (ctx > max_blocks * KV4_PAGE) {
     if (threadIdx.x == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, ctx);
     ctx = max_blocks * KV4_PAGE;
   }
   const int past = ctx - n;
-  const int seen = past + (c0 + min(rows, 2 * KVT_M) - 1) / G + 1;        // keys that the last row sees
-  const int pages = (max(seen, 0) + KVT_N - 1) / KVT_N, per = max((pages + nsplit - 1) / nsplit, 4);
-  const int first = split * per, tiles = max(0, min(pages, first + per) - first);    // pages of this split
+  if (plan.count == nullptr) {
+    const int pages = kvt_pages(past, c0, rows, G), per = max((pages + nsplit - 1) / nsplit, 4), split = blockIdx.x % nsplit;
+    first = split * per;
+    tiles = max(0, min(pages, first + per) - first);
+    if (nsplit > 1) slot = (int)(b * (gridDim.x / nsplit) + c0 / (2 * KVT_M)) * nsplit + split;
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -350,14 +479,14 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         tc_fence_after();
         const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l;
         __nv_bfloat16* dst = out + (size_t)(row0 + qi) * ldo + (size_t)head * D;
-        const size_t pr = ((size_t)(row0 + qi) * hq + head) * nsplit + split;
-        if (nsplit > 1 && live) part_ml[pr] = make_float2(m_ref == -INFINITY ? -3.0e38f : m_ref, l);
+        const size_t pr = ((size_t)slot * hkv + kvh) * (2 * KVT_M) + i * KVT_M + row;
+        if (slot >= 0 && live) part_ml[pr] = make_float2(m_ref == -INFINITY ? -3.0e38f : m_ref, l);
 #pragma unroll
         for (int k = 0; k < D; k += 16) {
           uint32_t r[16];
           if (tiles > 0) { tmem_ld_x16(tmem_o + k, r); tmem_ld_wait(); }
           if (!live) continue;
-          if (nsplit > 1) {
+          if (slot >= 0) {
             if (l != 0.f) {                                      // (the merge does not read what has no weight)
 #pragma unroll
               for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part_o + pr * D + k + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
@@ -382,21 +511,103 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
   if (warp == KVT_SOFT + KVT_FILL) { __syncwarp(); tc_fence_after(); tmem_dealloc(bars.tmem_base, 512); }
 }
 
+// The pieces of a tile pair joined: a warp per row, a lane D / 32 elements, four pieces on their way at once.
+constexpr int KVT_JOIN = 8;                                               // rows of a CTA
+template <int D>
+__global__ void __launch_bounds__(256)
+kv4_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const KvtPlan plan, const int* __restrict__ q_start, const int* __restrict__ q_lens,
+                __nv_bfloat16* __restrict__ out, int batch, int tiles, int all_rows, int nq, int hq, int hkv, long long ldo, int nsplit) {
+  constexpr int E = D / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = hq / hkv, count = plan.count != nullptr ? plan.count[1] : tiles * batch;
+  const int chunks = (min(nq * G, 2 * KVT_M) + KVT_JOIN - 1) / KVT_JOIN;                                          // of a tile pair
+  for (long long w = blockIdx.x; w < (long long)count * hkv * chunks; w += gridDim.x) {
+    const int th = (int)(w / chunks), t = th / hkv, kvh = th - t * hkv, r0 = (int)(w - (long long)th * chunks) * KVT_JOIN;
+    const int4 v = plan.count != nullptr ? plan.join[t] : make_int4(t / tiles, t % tiles * 2 * KVT_M, nsplit, t * nsplit);
+    const int b = v.x, c0 = v.y, ns = v.z, n = q_lens ? q_lens[b] : nq, row0 = q_start ? q_start[b] : b * nq;
+    if (n > nq || row0 < 0 || n > all_rows - row0) continue;
+    for (int r = r0 + warp; r < min(r0 + KVT_JOIN, n * G - c0); r += 8) {
+      const int qi = (c0 + r) / G, head = kvh * G + c0 + r - qi * G;
+      const size_t first = ((size_t)v.w * hkv + kvh) * (2 * KVT_M) + r, step = (size_t)hkv * (2 * KVT_M);
+      float2 ml[4];                                                         // of pieces lane, lane + 32, ... (at most 128)
+      float M = -3.0e38f, L = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ml[i] = lane + 32 * i < ns ? part_ml[first + (lane + 32 * i) * step] : make_float2(-3.0e38f, 0.f);
+        M = fmaxf(M, ml[i].x);
+      }
+      M = warp_max(M);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ml[i].x = ml[i].y == 0.f ? 0.f : kvt_ex2(ml[i].x - M);              // (a piece of no weight has left nothing)
+        L = fmaf(ml[i].y, ml[i].x, L);
+      }
+      L = warp_sum(L);
+      float acc[E];
+#pragma unroll
+      for (int k = 0; k < E; ++k) acc[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        for (int s = 32 * i; s < min(ns, 32 * i + 32); s += 4) {
+          float v4[4][E], sc[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            sc[u] = __shfl_sync(0xffffffffu, ml[i].x, (s + u) & 31);        // (0 behind the last piece)
+#pragma unroll
+            for (int k = 0; k < E; ++k) v4[u][k] = 0.f;
+            if (sc[u] != 0.f) {
+              const float* src = part_o + (first + (s + u) * step) * D + lane * E;
+              if constexpr (E == 4) { const float4 x = *reinterpret_cast<const float4*>(src); v4[u][0] = x.x; v4[u][1] = x.y; v4[u][2] = x.z; v4[u][3] = x.w; }
+              else { const float2 x = *reinterpret_cast<const float2*>(src); v4[u][0] = x.x; v4[u][1] = x.y; }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int k = 0; k < E; ++k) acc[k] = fmaf(v4[u][k], sc[u], acc[k]);
+        }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(out + (size_t)(row0 + qi) * ldo + (size_t)head * D) + lane * (E / 2);
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) dst[k] = pack_bf16x2(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+    }
+  }
+}
+
+// What a call's scratch has room for. List (nsplit 0): pieces are KVT_SHARE times the SMs at most and one for every tile pair; a tile pair that is cut has no more than
+// twice as many as it is sizes large.
+struct KvtRoom { long long tiles, items, joins, slots, ints; };
+static KvtRoom kvt_room(int batch, int rows, int max_q_len, int hq, int hkv, int nsplit) {
+  const long long G = hq / hkv, each = ((long long)max_q_len * G + 2 * KVT_M - 1) / (2 * KVT_M), some = ((long long)rows * G + 2 * KVT_M - 1) / (2 * KVT_M);
+  KvtRoom r{};
+  r.tiles = batch * each < batch + some ? batch * each : batch + some;
+  if (nsplit == 0) {
+    r.joins = KVT_SHARE * sm_count() / hkv + 1;
+    r.items = r.tiles + r.joins;
+    r.slots = 2 * r.joins;
+    r.ints = (4 + 5 * r.items + 4 * r.joins + 3) / 4 * 4;
+  } else if (nsplit > 1) {
+    r.slots = batch * each * nsplit;
+  }
+  return r;
+}
+
 }  // namespace ff
 using namespace ff;
 
-// Splits of ff_kv4_attn_tiles, and the floats of scratch it needs for them. rows: of the whole call, at most max_q_len per sequence. One CTA stands on an SM;
-// where there are fewer than SMs the keys are split, down to four pages each: for one round of CTAs, or three where half of the SMs would do without (their
-// contexts differ: 96 CTAs of up to 62 pages 66 us, in three splits 61).
+// Splits of ff_kv4_attn_tiles (0: by a list), and the floats of scratch it needs. rows: of the whole call, at most max_q_len per sequence. One CTA stands on an SM. One
+// sequence, or contexts of few pages: where there are fewer CTAs than SMs the keys are split, down to four pages each: for one round of CTAs, or three where more than
+// half of the SMs have one (96 CTAs of up to 62 pages 66 us, in three splits 61).
 FF_EXPORT int ff_kv4_tiles_plan(int batch, int rows, int max_q_len, int hq, int hkv, int dim, int max_ctx, long long* floats) {
-  const long long G = hq / hkv, each = ((long long)max_q_len * G + 2 * KVT_M - 1) / (2 * KVT_M), some = ((long long)rows * G + 2 * KVT_M - 1) / (2 * KVT_M);
-  const long long ctas = hkv * (batch * each < batch + some ? batch * each : batch + some);
-  const long long most = (max_ctx + 4 * KVT_N - 1) / (4 * KVT_N);
+  const long long ctas = hkv * kvt_room(batch, rows, max_q_len, hq, hkv, 1).tiles, most = (max_ctx + 4 * KVT_N - 1) / (4 * KVT_N);
   long long nsplit = ctas <= 0 ? 1 : 2 * ctas <= sm_count() ? sm_count() / ctas : ctas < sm_count() ? 3 : 1;
   if (nsplit > most) nsplit = most;
   if (nsplit > 128) nsplit = 128;
   if (nsplit < 1) nsplit = 1;
-  if (floats) *floats = nsplit > 1 ? (long long)rows * hq * nsplit * (dim + 2) : 0;
+  if (batch > 1 && batch <= KVT_SEQS && max_ctx >= KVT_LIST * KVT_N) nsplit = 0;
+  const KvtRoom r = kvt_room(batch, rows, max_q_len, hq, hkv, (int)nsplit);
+  if (floats) *floats = r.ints + r.slots * hkv * 2 * KVT_M * (dim + 2);
   return (int)nsplit;
 }
 
@@ -407,18 +618,34 @@ FF_EXPORT int ff_kv4_attn_tiles(const void* q, const void* kpages, const void* v
   if (batch <= 0 || batch > 65535 || rows <= 0 || max_q_len <= 0 || hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv || (dim != 64 && dim != 128) || max_blocks <= 0 || num_blocks <= 0)
     return FF_HOST_BAD_SHAPE;
   if (q_start == nullptr && (long long)batch * max_q_len != rows) return FF_HOST_BAD_SHAPE;
-  if (!(scale > 0.f) || (q_start == nullptr) != (q_lens == nullptr) || !ctx_lens || nsplit < 1 || nsplit > 128 || (nsplit > 1 && scratch == nullptr)) return FF_HOST_BAD_SHAPE;
+  if (!(scale > 0.f) || (q_start == nullptr) != (q_lens == nullptr) || !ctx_lens || nsplit < 0 || nsplit > 128 || (nsplit == 0 && batch > KVT_SEQS) || (nsplit != 1 && scratch == nullptr)) return FF_HOST_BAD_SHAPE;
   if (ldq % 8 || ldo % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpages) | reinterpret_cast<uintptr_t>(vpages) | reinterpret_cast<uintptr_t>(out) |
                               reinterpret_cast<uintptr_t>(scratch)) & 15))
     return FF_HOST_BAD_ALIGN;
-  const long long columns = (long long)max_q_len * (hq / hkv), grid = (columns + 2 * KVT_M - 1) / (2 * KVT_M) * nsplit;
-  if (columns > 0x7fffff00ll || grid > 0x7fffffffll) return FF_HOST_TOO_LARGE;
+  const KvtRoom room = kvt_room(batch, rows, max_q_len, hq, hkv, nsplit);
+  const long long columns = (long long)max_q_len * (hq / hkv), each = (columns + 2 * KVT_M - 1) / (2 * KVT_M), grid = nsplit ? each * nsplit : room.items * hkv;
+  if (columns > 0x7fffff00ll || grid > 0x7fffffffll || room.slots > 0x7fffffffll) return FF_HOST_TOO_LARGE;
   auto kern = dim == 128 ? kv4_tiles_kernel<128> : kv4_tiles_kernel<64>;
   const int bytes = dim == 128 ? kvt_smem<128>() : kvt_smem<64>();
   if (int r = opt_in_smem(kern, bytes)) return r;
-  float2* ml = nsplit > 1 ? reinterpret_cast<float2*>(scratch + (long long)rows * hq * nsplit * dim) : nullptr;
-  if (int r = launch_pdl(kern, dim3((unsigned)grid, hkv, batch), dim3(32 * KVT_WARPS), bytes, s, 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
-                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, scratch, ml, rows, max_q_len, hq, hkv, ldq, ldo, max_blocks,
+  float* const part = scratch + room.ints;
+  float2* const ml = reinterpret_cast<float2*>(part + room.slots * hkv * 2 * KVT_M * dim);
+  KvtPlan plan{};
+  if (nsplit == 0) {
+    int* at = reinterpret_cast<int*>(scratch);
+    plan.count = at; at += 4;
+    plan.item = reinterpret_cast<int4*>(at); at += 4 * room.items;
+    plan.join = reinterpret_cast<int4*>(at); at += 4 * room.joins;
+    plan.slot = at;
+    plan.items = (int)room.items; plan.joins = (int)room.joins; plan.slots = (int)room.slots;
+    if (int r = launch_pdl(kv4_plan_kernel, dim3(1), dim3(32 * KVT_PLAN_WARPS), 0, s, 0, plan, q_start, q_lens, ctx_lens, batch, rows, max_q_len, hq / hkv, hkv, max_blocks,
+                           sm_count(), status)) return r;
+  }
+  if (int r = launch_pdl(kern, nsplit ? dim3((unsigned)grid, hkv, batch) : dim3((unsigned)grid), dim3(32 * KVT_WARPS), bytes, s, 0, (const __nv_bfloat16*)q, (const uint8_t*)kpages,
+                         (const uint8_t*)vpages, block_table, q_start, q_lens, ctx_lens, (__nv_bfloat16*)out, part, ml, plan, rows, max_q_len, hq, hkv, ldq, ldo, max_blocks,
                          num_blocks, nsplit, scale * 1.4426950408889634f, status)) return r;
-  return nsplit == 1 ? FF_HOST_OK : kv4_merge(scratch, ml, q_start, q_lens, out, batch, rows, max_q_len, hq, dim, ldo, nsplit, s);
+  if (nsplit == 1) return FF_HOST_OK;
+  const long long joins = (nsplit ? batch * each : room.joins) * hkv * (((columns < 2 * KVT_M ? columns : 2 * KVT_M) + KVT_JOIN - 1) / KVT_JOIN);
+  return launch_pdl(dim == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, dim3((unsigned)(joins < 8 * sm_count() ? joins : 8 * sm_count())), dim3(256),
+                    0, s, 0, (const float*)part, (const float2*)ml, plan, q_start, q_lens, (__nv_bfloat16*)out, batch, (int)each, rows, max_q_len, hq, hkv, ldo, nsplit);
 }

@@ -43,7 +43,3 @@ FF_EXPORT int ff_attn_prefill_tc(const void* q, const void* kcache, const void* 
 // norm_embed.cu
 FF_EXPORT int ff_add_rmsnorm(const void* x, void* res, const void* w, void* out, void* capture, int capture_stride, int rows, int hidden, int ldx, float eps,
                              int unit_offset, int* status, cudaStream_t s);
-
-// attention_kv4.cu: splits [row][head][nsplit][dim] with their (maximum, sum) joined, for the rows of sequences as in ff_kv4_attn_rows
-int kv4_merge(const float* part_o, const float2* part_ml, const int* q_start, const int* q_lens, void* out, int batch, int rows, int nq, int hq, int dim,
-              long long ldo, int nsplit, cudaStream_t s);

@@ -312,7 +312,7 @@ def _attention(q, ldq, kpages, vpages, blocks, block_table, q_start, q_lens, ctx
         check(lib.ff_kv4_attn_tiles(*head, *tail), "ff_kv4_attn_tiles")
     else:
         check(lib.ff_kv4_attn_rows(*head, *tail), "ff_kv4_attn_rows")
-    _count(1 if scratch is None else 2)
+    _count(1 if scratch is None else 3 if nsplit == 0 else 2)             # (a list of the work first, parts joined last)
     return out
 
 

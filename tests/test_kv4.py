@@ -403,6 +403,66 @@ def test_prompts_over_4_bit_pages(dim, hq, hkv, spans):
     _close(got[2: at], *(t[2: at] for t in want), rounded=tiles)
 
 
+MANY = [(128, 8, 2, [(40, 3000), (0, 0), (3, 5000), (200, 0), (70, 2500), (1, 40), (300, 100)]), (64, 28, 4, [(30, 9000), (2, 0), (64, 1)]), (128, 16, 1, [(16, 20000), (5, 2)]),
+        (128, 4, 4, [(n % 37, 100 * n % 2300) for n in range(40)])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,hq,hkv,spans", MANY)
+def test_prompts_whose_contexts_differ(dim, hq, hkv, spans):
+    """Sequences with contexts from none to thousands: long ones are cut into pieces, the largest pieces come first."""
+    lens = [n + past for n, past in spans]
+    kp, vp, table = _cache(lens, hkv, dim, 3 + len(spans), "cuda")
+    rows = sum(n for n, _ in spans) + 5
+    q = _rows(rows, hq * dim, 12).cuda()
+    starts, at = [], 2
+    for n, _ in spans:
+        starts.append(at)
+        at += n
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    out = torch.full((rows, hq * dim), 3.0, dtype=BF16, device="cuda")
+    scale, most = 1 / math.sqrt(dim), max(n for n, _ in spans)
+    assert kv4_ops.in_tiles(most, hq, hkv)
+    run = lambda **kw: kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(starts), i32([n for n, _ in spans]), i32(lens), most, hq, hkv, dim, scale, **kw)
+    got = run(out=out)
+    assert bool((out[:2] == 3).all()) and bool((out[at:] == 3).all()) and ops.read_status()[0] == 0
+    assert torch.equal(got[2: at], run()[2: at])                            # the pieces' places in the scratch change nothing
+    want = _definition(q, kp, vp, table, [(s, n, c) for s, (n, _), c in zip(starts, spans, lens)], hq, hkv, dim, scale, rounded=True)
+    _close(got[2: at], *(t[2: at] for t in want), rounded=True)
+    got = run(max_ctx=64)                                                    # (said to be short: as they lie)
+    _close(got[2: at], *(t[2: at] for t in want), rounded=True)
+
+
+@pytest.mark.gpu
+def test_lists_of_work_in_two_graphs():
+    """Two captured calls whose lists lie in scratch of their own, replayed at the same time over contexts that have changed since."""
+    dim, hq, hkv, nq = 128, 16, 2, 9
+    runs = []
+    for seed in (1, 2):
+        kp, vp, table = _cache([5000, 700, 64, 2600], hkv, dim, seed, "cuda")
+        runs.append((_rows(4 * nq, hq * dim, seed).cuda(), kp, vp, table, torch.tensor([9, 9, 9, 9], dtype=torch.int32, device="cuda")))
+    step = lambda r: kv4_ops.attn_decode_kv4(*r, hq, hkv, dim, 0.09, nq=nq)
+    graphs, outs, sides = [], [], [torch.cuda.Stream() for _ in runs]
+    for r in runs:
+        step(r)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(r))
+    for lens in ([5000, 0, 64, 2600], [10, 700, 33, 2000]):
+        for r in runs:
+            r[4].copy_(torch.tensor(lens, dtype=torch.int32))
+        want = [step(r) for r in runs]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, sides):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    assert ops.read_status()[0] == 0
+
+
 @pytest.mark.gpu
 def test_copied_pages_of_many_tensors():
     gen = torch.Generator(device="cuda").manual_seed(3)
