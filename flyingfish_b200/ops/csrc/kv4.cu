@@ -45,21 +45,22 @@ __device__ __forceinline__ uint32_t kv4_quantise(const uint32_t (&w)[4], uint32_
   // codes: q + 3 2^22 has the integer next to q in its last bits, of which those of a word are summed; what the upper bits add is known
   const float inv = __frcp_rn(scale);
   uint32_t word = 0u - (0x4b400000u + 0xb4000000u + 0x40000000u);
-  bool doubt = false;
+  uint32_t doubt = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float x = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
     const float q = __fmul_rn(__fsub_rn(x, lo), inv), r = __fadd_rn(q, 12582912.f);
-    doubt = doubt || fabsf(__fsub_rn(q, __fsub_rn(r, 12582912.f))) > 0.4999f;
+    if (fabsf(__fsub_rn(q, __fsub_rn(r, 12582912.f))) > 0.4999f) doubt |= 1u << e;
     word += __float_as_uint(r) << (4 * (e / 2 + 4 * (e & 1)));
   }
   if (doubt) {
-    word = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-      word |= (uint32_t)min(15, __double2int_rn(((double)x - (double)lo) / (double)scale)) << (4 * (e / 2 + 4 * (e & 1)));
-    }
+    for (int e = 0; e < 8; ++e)
+      if (doubt >> e & 1u) {
+        const float x = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        const int at = 4 * (e / 2 + 4 * (e & 1));
+        word = (word & ~(15u << at)) | ((uint32_t)min(15, __double2int_rn(((double)x - (double)lo) / (double)scale)) << at);
+      }
   }
   return word;
 }
@@ -68,7 +69,9 @@ __device__ __forceinline__ uint32_t kv4_quantise(const uint32_t (&w)[4], uint32_
 // qout, keys and values into the pages of the row's slot. A head is D / 8 lanes with 8 elements each, so a turn's partner is half a head's lanes
 // away and a group of 32 elements is 4 lanes; such a set of lanes walks heads of a row with the row's cosines and sines in registers, five heads on their way at
 // once. Norm and turn round as the BF16 cache's kernel does: every product and sum to BF16 (packed instructions; a sum of two BF16 numbers that FP32 does not
-// hold has a term too small to matter). Bound by DRAM; few rows are spread over CTAs by heads.
+// hold has a term too small to matter). Few rows are spread over CTAs by heads. 8191 rows of 64 + 2 x 8 heads of 128: 78 us, 4.2 TB/s, where the bytes alone take 50: issue
+// slots are 63 % taken, warps wait for their loads in between. With FP64 for all codes of a lane that has one in doubt (a third of the warps have) 82, with three
+// heads at once 102, with 80 registers and three CTAs 90.
 constexpr int WRITE_THREADS = 256, WRITE_HEADS = 5;
 template <int D, bool NORM>
 __global__ void __launch_bounds__(WRITE_THREADS, 4)
@@ -84,7 +87,7 @@ kv4_write_kernel(const __nv_bfloat16* __restrict__ qkv, const int* __restrict__ 
     const int slot = slots[row];
     const int block = slot / KV4_PAGE, k = slot - block * KV4_PAGE;
     if (slot >= 0 && block >= num_blocks && threadIdx.x == 0) set_status(status, KID_KV, FF_ERR_BOUNDS, row, slot);
-    const bool store = slot >= 0 && block < num_blocks, upper = c >= LANES / 2, turn = cos_sin != nullptr;
+    const bool store = slot >= 0 && block < num_blocks, upper = c >= LANES / 2, turn = cos_sin != nullptr, whole = 2 * rhalf == D;
     uint32_t cs[4], sn[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { cs[i] = 0x3f803f80u; sn[i] = 0u; }
@@ -151,8 +154,12 @@ kv4_write_kernel(const __nv_bfloat16* __restrict__ qkv, const int* __restrict__ 
           for (int i = 0; i < 4; ++i) {
             const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], LANES / 2);
             const uint32_t t = kv4_add2(kv4_mul2(w[i], cs[i]), kv4_mul2(other, sn[i]));
-            const uint32_t keep = 2 * i >= stays ? 0xffffffffu : 2 * i + 1 >= stays ? 0xffff0000u : 0u;
-            if (part < 2) w[i] = (t & ~keep) | (w[i] & keep);
+            if (whole) {
+              if (part < 2) w[i] = t;
+            } else {
+              const uint32_t keep = 2 * i >= stays ? 0xffffffffu : 2 * i + 1 >= stays ? 0xffff0000u : 0u;
+              if (part < 2) w[i] = (t & ~keep) | (w[i] & keep);
+            }
           }
         }
         if (part == 0 && live && qout != nullptr) *reinterpret_cast<uint4*>(qo + head * D) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -180,7 +187,8 @@ kv4_write_kernel(const __nv_bfloat16* __restrict__ qkv, const int* __restrict__ 
   }
 }
 
-// What the pages hold for given slots, rounded to BF16; rows of a slot below 0 are zero. D / 8 lanes a head, 8 elements each.
+// What the pages hold for given slots, rounded to BF16; rows of a slot below 0 are zero. D / 8 lanes a head, 8 elements each. The 8191 rows above, 34 MB of
+// results from 21 MB of pages: 22 us with its launch, where the bytes take 8.
 template <int D>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ slots, __nv_bfloat16* __restrict__ kout,
@@ -213,7 +221,8 @@ kv4_read_kernel(const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ 
 }
 
 // Pages copied inside every tensor of a list: one launch for all layers' keys and values. Addresses and page numbers are arguments of the launch,
-// so nothing has to be sent to the device first and a captured launch keeps its own. Bound by DRAM (bytes of the pages, read and written).
+// so nothing has to be sent to the device first and a captured launch keeps its own. Bound by DRAM: 150 BF16 blocks in 32 layers, 2.5 GB read and written, 396 us where a
+// plain copy's rate gives 383. A single page of 32 layers is bound by its 64 tensors' addresses on the host, 47 us.
 constexpr int COPY_TENSORS = 160, COPY_PAIRS = 256;
 struct CopyPages {
   unsigned long long base[COPY_TENSORS];
