@@ -13,8 +13,9 @@
 // 2^-25, an element by 2^-20 then. Queries are divided by a power of two per row, which the soft-max's scale takes back.
 // S(j + 1) of a tile waits for its P V (j - 1), whose P it overwrites; the other tile's products run meanwhile.
 // 8191 rows of 32 / 8 heads of 128 from the beginning: 567 us, 970 TFLOP/s (626 in a row, at the clock that power leaves then). The products alone take 403 (S = Q K^T has 64
-// columns, for which shared memory feeds the tensor cores at two thirds of their rate), the tiles of keys and values alone 475, both without the soft-max 500: what
-// bounds it is that four warps write a page's tiles in 1700 cycles, for which more warps would need registers that the soft-max has.
+// columns, for which shared memory feeds the tensor cores at two thirds of their rate), the tiles of keys and values alone 475, both without the soft-max 500. They share
+// shared memory (128 KB of operands a page, 42 for the tiles, some 1350 of 2050 cycles) and issue slots (54 % taken): eight warps for the tiles, with registers that the
+// others give up, take 617.
 // Every wait is bounded; a time-out records FF_ERR_TIMEOUT, and all roles leave through the abort flag.
 #include "kv4.cuh"
 #include "host_util.h"
@@ -580,10 +581,11 @@ kv4_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ par
 
 // What a call's scratch has room for. List (nsplit 0): pieces are KVT_SHARE times the SMs at most and one for every tile pair; a tile pair that is cut has no more than
 // twice as many as it is sizes large.
-struct KvtRoom { long long tiles, items, joins, slots, ints; };
+struct KvtRoom { long long each, tiles, items, joins, slots, ints; };        // each: tile pairs of a sequence at most, tiles: of all
 static KvtRoom kvt_room(int batch, int rows, int max_q_len, int hq, int hkv, int nsplit) {
-  const long long G = hq / hkv, each = ((long long)max_q_len * G + 2 * KVT_M - 1) / (2 * KVT_M), some = ((long long)rows * G + 2 * KVT_M - 1) / (2 * KVT_M);
+  const long long G = hq / hkv, each = ((long long)(max_q_len < rows ? max_q_len : rows) * G + 2 * KVT_M - 1) / (2 * KVT_M), some = ((long long)rows * G + 2 * KVT_M - 1) / (2 * KVT_M);
   KvtRoom r{};
+  r.each = each;
   r.tiles = batch * each < batch + some ? batch * each : batch + some;
   if (nsplit == 0) {
     r.joins = KVT_SHARE * sm_count() / hkv + 1;
@@ -601,9 +603,10 @@ using namespace ff;
 
 // Splits of ff_kv4_attn_tiles (0: by a list), and the floats of scratch it needs. rows: of the whole call, at most max_q_len per sequence. One CTA stands on an SM. One
 // sequence, or contexts of few pages: where there are fewer CTAs than SMs the keys are split, down to four pages each: for one round of CTAs, or three where more than
-// half of the SMs have one (96 CTAs of up to 62 pages 66 us, in three splits 61).
+// half of the SMs have one (96 CTAs of up to 62 pages 66 us, in three splits 61). That counts as many tile pairs for every sequence as the longest has, which is also what
+// their parts' room is made for.
 FF_EXPORT int ff_kv4_tiles_plan(int batch, int rows, int max_q_len, int hq, int hkv, int dim, int max_ctx, long long* floats) {
-  const long long ctas = hkv * kvt_room(batch, rows, max_q_len, hq, hkv, 1).tiles, most = (max_ctx + 4 * KVT_N - 1) / (4 * KVT_N);
+  const long long ctas = kvt_room(batch, rows, max_q_len, hq, hkv, 1).each * hkv * batch, most = (max_ctx + 4 * KVT_N - 1) / (4 * KVT_N);
   long long nsplit = ctas <= 0 ? 1 : 2 * ctas <= sm_count() ? sm_count() / ctas : ctas < sm_count() ? 3 : 1;
   if (nsplit > most) nsplit = most;
   if (nsplit > 128) nsplit = 128;
@@ -626,7 +629,8 @@ FF_EXPORT int ff_kv4_attn_tiles(const void* q, const void* kpages, const void* v
                               reinterpret_cast<uintptr_t>(scratch)) & 15))
     return FF_HOST_BAD_ALIGN;
   const KvtRoom room = kvt_room(batch, rows, max_q_len, hq, hkv, nsplit);
-  const long long columns = (long long)max_q_len * (hq / hkv), each = (columns + 2 * KVT_M - 1) / (2 * KVT_M), grid = nsplit ? each * nsplit : room.items * hkv;
+  if (max_q_len > rows) max_q_len = rows;
+  const long long columns = (long long)max_q_len * (hq / hkv), each = room.each, grid = nsplit ? each * nsplit : room.items * hkv;
   if (columns > 0x7fffff00ll || grid > 0x7fffffffll || room.slots > 0x7fffffffll) return FF_HOST_TOO_LARGE;
   auto kern = dim == 128 ? kv4_tiles_kernel<128> : kv4_tiles_kernel<64>;
   const int bytes = dim == 128 ? kvt_smem<128>() : kvt_smem<64>();

@@ -423,14 +423,16 @@ def test_prompts_whose_contexts_differ(dim, hq, hkv, spans):
     out = torch.full((rows, hq * dim), 3.0, dtype=BF16, device="cuda")
     scale, most = 1 / math.sqrt(dim), max(n for n, _ in spans)
     assert kv4_ops.in_tiles(most, hq, hkv)
-    run = lambda **kw: kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(starts), i32([n for n, _ in spans]), i32(lens), most, hq, hkv, dim, scale, **kw)
+    run = lambda most=most, **kw: kv4_ops.attn_prefill_kv4(q, kp, vp, table, i32(starts), i32([n for n, _ in spans]), i32(lens), most, hq, hkv, dim, scale, **kw)
     got = run(out=out)
     assert bool((out[:2] == 3).all()) and bool((out[at:] == 3).all()) and ops.read_status()[0] == 0
     assert torch.equal(got[2: at], run()[2: at])                            # the pieces' places in the scratch change nothing
     want = _definition(q, kp, vp, table, [(s, n, c) for s, (n, _), c in zip(starts, spans, lens)], hq, hkv, dim, scale, rounded=True)
     _close(got[2: at], *(t[2: at] for t in want), rounded=True)
-    got = run(max_ctx=64)                                                    # (said to be short: as they lie)
-    _close(got[2: at], *(t[2: at] for t in want), rounded=True)
+    for kw in (dict(max_ctx=64), dict(max_ctx=1000), dict(max_ctx=1000, most=100000), dict(most=100000)):        # (contexts said to be short, rows said to be many)
+        got = run(**kw)
+        _close(got[2: at], *(t[2: at] for t in want), rounded=True)
+    assert ops.read_status()[0] == 0
 
 
 @pytest.mark.gpu
