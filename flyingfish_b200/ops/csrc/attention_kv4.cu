@@ -39,6 +39,17 @@ __device__ __forceinline__ void kv4_bulk_load(void* dst, const void* src, uint32
 }
 __device__ __forceinline__ float kv4_low(uint32_t w) { return __uint_as_float(w << 16); }              // BF16 in the lower / upper half
 __device__ __forceinline__ float kv4_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t kv4_mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t kv4_max2u(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t kv4_warp_max(uint32_t a) { return __reduce_max_sync(0xffffffffu, a); }
 __device__ __forceinline__ float kv4_peer(const float* p, int rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(dsmem_addr(smem_u32(p), (uint32_t)rank)) : "memory");
@@ -61,9 +72,13 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 //   S = sum_j scale_j (q_j . n_j) + lo_j sum(q_j)          O_j = sum_k (p_k scale_kj) n_kj + sum_k p_k lo_kj
 // for groups j of 32 elements. A code at bits 0 .. 3 of a 16-bit half is the FP16 number n 2^-24, at bits 4 .. 7 n 2^-20 (both subnormal, so exact and linear):
 // four pairs of codes are four masks and one shift, and nothing has to be subtracted. The powers of two go into the queries (every other pair of elements, and
-// a power per column that brings its greatest element to 2^14) and out of the results. Rounded to FP16 is p scale, 11 bits; sums, maxima, scale and lo are FP32,
-// and sum(q_j) is three BF16 parts of a product of its own, whose A operand is lo as it is. The sums of p lo are a product too, with both rounded to FP16
-// (lo, a BF16 number of at most 2^15, is one unless it is below 2^-14).
+// a power per column that brings its greatest element to 2^14) and out of the results. Sums, maxima, the keys' scale and lo are FP32,
+// and sum(q_j) is three BF16 parts of a product of its own, whose A operand is lo as it is. The sums of p lo are a product too.
+// Rounded to FP16 are p, p scale and lo, 11 bits each, whatever size the values are: a warp divides scale and lo by a power of two that the greatest of the page
+// lies at most KV4_KEPT binades below (and never above), its O is held over the same power and follows where that moves. Multiplied by 2^7, as p is, they fill
+// FP16's range: p scale has 11 bits down to 2^-28 of what it can be, p and lo down to 2^-21; what is smaller is off by 2^-39 or 2^-32 of the page's
+// greatest. BF16 would need no power, but has 8 bits of p scale, and code times scale is some three times a value. Values as they are, without the power: those of 2^-20 off by 8 %
+// and more, a long tail of small weights behind a single great one by 1 to 10 % for values of 2^-10.
 // A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, fetched by bulk copies into its two slots (keys, values),
 // with its own running maximum, sum and O. The warps' results meet in shared memory, those of up to eight CTAs (splits) in that of
 // their cluster, those of more in kv4_merge_kernel.
@@ -71,9 +86,11 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 // reaches), 1195 instructions a page and warp, 60 % of the slots taken, the integer pipe 54 % busy. Columns by 8 keep 128 registers and four CTAs on an SM, by 16 (more
 // than 8 columns) they share a page's unpacking. Codes turned into BF16 operands first took 204 us, as subnormal ones 136, sums of p lo as a product 109.
 constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;      // (a warp for every group of a head at least)
+constexpr int KV4_KEPT = 4;                      // binades that a page's values may lie below the power of two that a warp has for them
+constexpr int KV4_LEAST = 17, KV4_SPAN = 60;     // exponent field (2^-110) that such a power has at least, and how far it may fall
 template <int D, int NT>
 constexpr int kv4_smem() {
-  const int ring = KV4_WARPS * KV4_SLOTS * kv4_page_bytes(D), merge = (KV4_WARPS * (D + D / 32 + 2) + D + 2) * NT * 8 * 4;
+  const int ring = KV4_WARPS * (KV4_SLOTS * kv4_page_bytes(D) + KV4_PAGE * D / 8), merge = (KV4_WARPS * (D + D / 32 + 2) + D + 2) * NT * 8 * 4;
   return ring > merge ? ring : merge;
 }
 
@@ -210,6 +227,9 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     }
   }
 
+  // exponent field of the power of two that this warp's values are divided by (what O holds is divided by it too), and its greatest so far
+  int ref = KV4_LEAST, top = KV4_LEAST;
+  const uint32_t stats_at = smem_u32(smem + KV4_WARPS * KV4_SLOTS * PB) + warp * (KV4_PAGE * STAT);
   // row r of a 16-key tile is key 4 (r / 2) + r % 2, two more from r = 8 on: a thread's four columns of P^T are then its keys 4 t .. 4 t + 3
   const int kg = 4 * (g >> 1) + (g & 1);
   const uint32_t ring_at = smem_u32(ring);
@@ -289,7 +309,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
             if (p * KV4_PAGE + mt * 16 + kg + 2 * (r >> 1) > lim[nt][r & 1]) s[mt][nt][r] = -INFINITY;
       __syncwarp();                                             // (a branch of its own: the selects are not worth their place in every other page)
     }
-    // running maxima of columns 2 t and 2 t + 1, weights times 8 (their sum has the factor too)
+    // running maxima of columns 2 t and 2 t + 1, weights times 2^7 (their sum has the factor too)
     float alpha[NT][2];
     bool moved = false;
 #pragma unroll
@@ -307,7 +327,7 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
         alpha[nt][e] = kv4_ex2(m[nt][e] - mn);
         moved = moved || mn != m[nt][e];
         m[nt][e] = mn;
-        const float off = 3.0f - mn;
+        const float off = 7.0f - mn;
         float sum = 0.f;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
@@ -334,10 +354,38 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
     }
     if (!mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 42)) { ok = false; break; }
     const uint32_t sv = ring_at + pos.s * PB;
-    if (p * KV4_PAGE + KV4_PAGE > ctx) {
-      // tokens behind the sequence: whatever the page holds there is no number, and 0 times it would not be 0 (this is the warp's last page)
-      for (int i = max(0, ctx - p * KV4_PAGE) * NG + lane; i < KV4_PAGE * NG; i += 32)
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(sv + kv4_code_bytes(D) + 4 * i), "r"(0u) : "memory");
+    {
+      // (scale, lo) of the page times 2^7 over the power of two: exact in BF16, and 2^8 at most
+      uint32_t st[NG / 2][4], most = 0u;
+#pragma unroll
+      for (int i = 0; i < NG / 2; ++i) {
+        kv4_lds(sv + kv4_code_bytes(D) + 16 * (lane + 32 * i), st[i][0], st[i][1], st[i][2], st[i][3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // tokens behind the sequence: whatever the page holds there is no number, and 0 times it would not be 0
+          if (p * KV4_PAGE + KV4_PAGE > ctx && p * KV4_PAGE + (4 * (lane + 32 * i) + k) / NG >= ctx) st[i][k] = 0u;
+          most = kv4_max2u(most, st[i][k] & 0x7fff7fffu);
+        }
+      }
+      const int ex = max((int)(kv4_warp_max(max(most & 0xffffu, most >> 16)) >> 7), KV4_LEAST);
+      if (ex > ref || ex + KV4_KEPT < ref) {                    // (for all lanes)
+        top = max(top, ex);
+        const int next = max(ex, top - KV4_SPAN);
+        const float f = __uint_as_float((uint32_t)(127 + ref - next) << 23);
+        ref = next;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            ol[nt][e] *= f;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) { o[nt][j][0][e] *= f; o[nt][j][1][e] *= f; }
+          }
+      }
+      const uint32_t by = (uint32_t)(261 - ref) * 0x00800080u;
+#pragma unroll
+      for (int i = 0; i < NG / 2; ++i)
+        kv4_sts(stats_at + 16 * (lane + 32 * i), kv4_mul2(st[i][0], by), kv4_mul2(st[i][1], by), kv4_mul2(st[i][2], by), kv4_mul2(st[i][3], by));
       __syncwarp();
     }
 #pragma unroll
@@ -346,14 +394,14 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int key = mt * 16 + kg + 2 * r;
-        kv4_words<NG>(vs[r], sv + kv4_code_bytes(D) + key * STAT);
+        kv4_words<NG>(vs[r], stats_at + key * STAT);
       }
       {
         // rows of A: lo of group g % NG (rows 8 .. 15: nothing)
         uint32_t st[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(st[i]) : "r"(sv + kv4_code_bytes(D) + (mt * 16 + 4 * t + i) * STAT + 4 * (g & (NG - 1))) : "memory");
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(st[i]) : "r"(stats_at + (mt * 16 + 4 * t + i) * STAT + 4 * (g & (NG - 1))) : "memory");
         const uint32_t a[4] = {kv4_f16x2(kv4_high(st[0]), kv4_high(st[1])), 0u, kv4_f16x2(kv4_high(st[2]), kv4_high(st[3])), 0u};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -403,6 +451,8 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   float* const mo = sol + KV4_WARPS * NT * 8 * NG;
   float* const mml = mo + NT * 8 * D;
   const bool cluster = nsplit > 1 && part_o == nullptr;         // the splits are a cluster and join in shared memory
+  // the powers of two out of O: of the values, and of the codes at bits 0 .. 3 and 4 .. 7
+  const float of_lo = __uint_as_float((uint32_t)(ref - 7) << 23), of_even = __uint_as_float((uint32_t)(ref + 17) << 23), of_odd = __uint_as_float((uint32_t)(ref + 13) << 23);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -411,12 +461,12 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4); l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
       if (g == 0) { sml[(warp * NT * 8 + col) * 2] = m[nt][e]; sml[(warp * NT * 8 + col) * 2 + 1] = l[nt][e]; }
-      if (g < NG) sol[(warp * NT * 8 + col) * NG + g] = ol[nt][e];
+      if (g < NG) sol[(warp * NT * 8 + col) * NG + g] = ol[nt][e] * of_lo;
 #pragma unroll
       for (int j = 0; j < NG; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i)                             // nibble i of lane g's unit: element 32 j + 8 (g / 2) + 2 i + g % 2
-          so[(warp * NT * 8 + col) * D + 32 * j + 8 * (g >> 1) + 2 * i + (g & 1)] = o[nt][j][i >> 1][2 * (i & 1) + e] * ((i & 1) ? 1048576.f : 16777216.f);
+          so[(warp * NT * 8 + col) * D + 32 * j + 8 * (g >> 1) + 2 * i + (g & 1)] = o[nt][j][i >> 1][2 * (i & 1) + e] * ((i & 1) ? of_odd : of_even);
     }
   __syncthreads();
   for (int i = threadIdx.x; i < min(columns, NT * 8) * D; i += 32 * KV4_WARPS) {
