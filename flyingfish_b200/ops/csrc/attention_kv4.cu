@@ -238,7 +238,8 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
   for (int w = 0; w < mine; ++w) {
     const int p = p0 + w * KV4_WARPS;
     const bool whole = p * KV4_PAGE + KV4_PAGE - 1 <= all;
-    if (!mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 41)) { ok = false; break; }
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 41));      // (lanes give up together: those that went on would wait for the others)
+    if (!ok) break;
     float s[4][NT][4];
     {
       const uint32_t sk = ring_at + pos.s * PB;
@@ -352,7 +353,8 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
             for (int a = 0; a < 2; ++a) { o[nt][j][a][e] *= alpha[nt][e]; o[nt][j][a][2 + e] *= alpha[nt][e]; }
         }
     }
-    if (!mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 42)) { ok = false; break; }
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][pos.s], pos.ph, nullptr, status, KID_ATTN_DECODE, 42));
+    if (!ok) break;
     const uint32_t sv = ring_at + pos.s * PB;
     {
       // (scale, lo) of the page times 2^7 over the power of two: exact in BF16, and 2^8 at most

@@ -128,3 +128,10 @@ def test_pages_whose_values_differ(dim, hq, hkv, nq, lens, powers):
             if p % 7 == 5:                                          # a page of zeros
                 vp[int(table[i, p])] = 0
     _run(q, kp, vp, table, lens, hq, hkv, dim, scale, nq)
+
+
+def test_lanes_that_wait_give_up_together():
+    """In the kernel of few rows every warp waits as a whole: each wait that may run out is voted on, or lanes that go on would wait for those that gave up."""
+    from pathlib import Path
+    source = (Path(kv4_ops.__file__).parent / "csrc" / "attention_kv4.cu").read_text()
+    assert source.count("mbar_wait(") == source.count("__all_sync(0xffffffffu, mbar_wait(") == 2
