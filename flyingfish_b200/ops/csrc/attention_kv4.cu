@@ -44,12 +44,6 @@ __device__ __forceinline__ uint32_t kv4_mul2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t kv4_max2u(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t kv4_warp_max(uint32_t a) { return __reduce_max_sync(0xffffffffu, a); }
 __device__ __forceinline__ float kv4_peer(const float* p, int rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(dsmem_addr(smem_u32(p), (uint32_t)rank)) : "memory");
@@ -87,7 +81,6 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 // than 8 columns) they share a page's unpacking. Codes turned into BF16 operands first took 204 us, as subnormal ones 136, sums of p lo as a product 109.
 constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;      // (a warp for every group of a head at least)
 constexpr int KV4_KEPT = 4;                      // binades that a page's values may lie below the power of two that a warp has for them
-constexpr int KV4_LEAST = 17, KV4_SPAN = 60;     // exponent field (2^-110) that such a power has at least, and how far it may fall
 template <int D, int NT>
 constexpr int kv4_smem() {
   const int ring = KV4_WARPS * (KV4_SLOTS * kv4_page_bytes(D) + KV4_PAGE * D / 8), merge = (KV4_WARPS * (D + D / 32 + 2) + D + 2) * NT * 8 * 4;

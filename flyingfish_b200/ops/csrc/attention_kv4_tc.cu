@@ -24,13 +24,16 @@
 namespace ff {
 
 constexpr int KVT_M = 128, KVT_N = KV4_PAGE, KVT_STAGES = 3;
-constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 3;      // warps 0-7 soft-max, 8-11 tiles, 12 and 14 products, 13 pages
+constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 4;      // warps 0-7 soft-max, 8-11 tiles, 12 and 14 products, 13 pages, 15 sizes
 constexpr int KVT_PAGES = 3;                                                         // pages on their way or being turned into tiles
-constexpr float KVT_MOVED = 8.0f;                                                    // log2 units
+constexpr int KVT_SIZES = 8;                                                         // pages whose sizes are known: more than are between warp 15 and the soft-max
+constexpr int KVT_KEPT = 6;                                                          // binades that a page's values may lie below the power of two that they are divided by
+constexpr float KVT_MOVED = 8.0f, KVT_GAIN = 7.0f;                                   // log2 units: how far a maximum may lie behind, and what weights are multiplied by
 template <int D> constexpr int kvt_smem() { return 2 * KVT_M * D * 2 + 2 * KVT_STAGES * KVT_N * D * 2 + KVT_PAGES * 2 * kv4_page_bytes(D) + 1024; }
 
 struct alignas(8) KvtBars {
-  uint64_t q_full[2], k_full[KVT_STAGES], k_empty[KVT_STAGES], v_full[KVT_STAGES], v_empty[KVT_STAGES], s_full[2][2], p_full[2][2], pv_done[2][2], p_in[KVT_PAGES], p_out[KVT_PAGES];
+  uint64_t q_full[2], k_full[KVT_STAGES], k_empty[KVT_STAGES], v_full[KVT_STAGES], v_empty[KVT_STAGES], s_full[2][2], p_full[2][2], pv_done[2][2], p_in[KVT_PAGES], p_out[KVT_PAGES], e_ready[KVT_SIZES];
+  int2 size[KVT_SIZES];                                                                // exponent fields of the powers of two that keys and values are divided by
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -245,6 +248,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       mbar_init(&bars.k_full[i], KVT_FILL); mbar_init(&bars.k_empty[i], two); mbar_init(&bars.v_full[i], KVT_FILL); mbar_init(&bars.v_empty[i], two);
     }
     for (int i = 0; i < KVT_PAGES; ++i) { mbar_init(&bars.p_in[i], 1); mbar_init(&bars.p_out[i], KVT_FILL); }
+    for (int i = 0; i < KVT_SIZES; ++i) mbar_init(&bars.e_ready[i], 1);
     bars.abort_flag = 0;
     mbar_fence_init();
   }
@@ -264,6 +268,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       if (!mbar_wait(&bars.p_in[pr.s], pr.ph, abort_flag, status, KID_ATTN_PREFILL, 40)) ok = false;
+      if (!mbar_wait(&bars.e_ready[j % KVT_SIZES], (j / KVT_SIZES) & 1, abort_flag, status, KID_ATTN_PREFILL, 51)) ok = false;
       const uint32_t page = smem_u32(sP) + pr.s * 2 * PB;
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
@@ -276,18 +281,13 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           const int key = key0 + 32 * i;
           kvt_load<D>(code[i], page + part * PB + (part ? kv4_value_at<D>(key, 2 * u, 0) : key * (D / 2) + u * (D / 8)));
           kvt_load<D>(stat[i], page + part * PB + kv4_code_bytes(D) + key * (D / 8));
-          if ((first + j) * KVT_N + key >= ctx) {                // behind the sequence: whatever the page holds there is no number
-#pragma unroll
-            for (int g = 0; g < NG; ++g) stat[i][g] = 0u;
-          }
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           uint32_t v[2][4];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float2 sl = unpack_bf16x2(stat[i][g]);
-            const uint32_t scale2 = kvt_f16x2(sl.x, sl.x), lo2 = kvt_f16x2(sl.y, sl.y);
+            const uint32_t scale2 = kvt_prmt(stat[i][g], stat[i][g], 0x1010u), lo2 = kvt_prmt(stat[i][g], stat[i][g], 0x3232u);
             // values: 16-bit unit g of two chunks, the even elements and the odd ones
             const uint32_t word = part ? kvt_prmt(code[i][g / 2], code[i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[i][g];
 #pragma unroll
@@ -327,6 +327,51 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         blk = next;
       }
       if (bad) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
+    }
+  } else if (warp == KVT_SOFT + KVT_FILL + 3) {
+    // ================================ sizes ================================
+    // (scale, lo) of a page, in place, as FP16 numbers: times 2^13 over a power of two that the greatest of |lo| and 16 scale lies in, so that elements are below 2^15
+    RingPos pr;
+    int ref = 0, top = 0;
+    for (int j = 0; j < tiles; ++j) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars.p_in[pr.s], pr.ph, abort_flag, status, KID_ATTN_PREFILL, 38))) break;
+      int size[2];
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const uint32_t at = smem_u32(sP) + pr.s * 2 * PB + part * PB + kv4_code_bytes(D) + 16 * lane;
+        uint32_t st[NG / 2][4], most = 0u;
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) {
+          kv4_lds(at + 512 * i, st[i][0], st[i][1], st[i][2], st[i][3]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // behind the sequence: whatever the page holds there is no number
+            if ((first + j) * KVT_N + (4 * (lane + 32 * i) + k) / NG >= ctx) st[i][k] = 0u;
+            most = kv4_max2u(most, (st[i][k] & 0x7fff7fffu) + 0x0200u);
+          }
+        }
+        int ex = max((int)(kv4_warp_max(max(most & 0xffffu, most >> 16)) >> 7), KV4_LEAST);
+        if (part) {
+          // O is held over the values' power: it rises with a binade to spare, and falls only behind much smaller pages
+          if (ex > ref) ref = ex + 1;
+          else if (ex + KVT_KEPT < ref) ref = max(ex + 1, top - KV4_SPAN);
+          top = max(top, ref);
+          ex = ref;
+        }
+        size[part] = ex;
+        const float by = __uint_as_float((uint32_t)(267 - ex) << 23);
+#pragma unroll
+        for (int i = 0; i < NG / 2; ++i) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { const float2 v = unpack_bf16x2(st[i][k]); st[i][k] = kvt_f16x2(v.x * by, v.y * by); }
+          kv4_sts(at + 512 * i, st[i][0], st[i][1], st[i][2], st[i][3]);
+        }
+      }
+      fence_proxy_async_smem();                                  // (a bulk copy writes the place next)
+      if (lane == 0) bars.size[j % KVT_SIZES] = make_int2(size[0], size[1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.e_ready[j % KVT_SIZES]);
+      pr.next(KVT_PAGES);
     }
   } else if (warp >= KVT_SOFT + KVT_FILL) {
     // ================================ products: a warp for each tile ================================
@@ -389,7 +434,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         for (int k = 0; k < D / 2; ++k) { const float2 v = unpack_bf16x2(w[k]); most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))); }
         const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);          // 2^(e - 127), and its inverse
         const float up = __uint_as_float(e << 23), down = __uint_as_float((254u - e) << 23);
-        row_scale = fmaxf(row_scale * up, 1.1754944e-38f);       // (times minus infinity it has to be that)
+        row_scale *= up;
         const uint32_t dst = smem_u32(sQ) + i * QTILE + row * 128;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) {
@@ -408,13 +453,17 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       const uint32_t tmem_o = tmem + 256 + 128 * i + lanes;
       float m_ref = -INFINITY;
       float l0 = 0.f, l1 = 0.f;
+      int over = KV4_LEAST;                                              // exponent field of the power of two that O is held over
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
         const uint32_t s_addr = tmem + 128 * i + 64 * (j & 1) + lanes;
         if (!mbar_wait(&bars.s_full[i][j & 1], (j >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 47)) ok = false;
+        if (!mbar_wait(&bars.e_ready[j % KVT_SIZES], (j / KVT_SIZES) & 1, abort_flag, status, KID_ATTN_PREFILL, 52)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
+        const int2 size = bars.size[j % KVT_SIZES];
+        const float page_scale = fmaxf(row_scale * __uint_as_float((uint32_t)(size.x - 13) << 23), 1.1754944e-38f);      // (times minus infinity it has to be that)
         float s[KVT_N];
         {
           uint32_t r[KVT_N];
@@ -431,7 +480,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int k = 0; k < KVT_N; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * row_scale;
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * page_scale;
         float alpha = 1.f;
         bool need = false;
         if (mx > m_ref + KVT_MOVED || (m_ref == -INFINITY && mx > -INFINITY)) {
@@ -439,6 +488,12 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           m_ref = mx;
           need = j > 0;
         }
+        float by = alpha;
+        if (size.y != over) {
+          by *= __uint_as_float((uint32_t)(127 + over - size.y) << 23);
+          need = j > 0;
+        }
+        over = size.y;
         if (__any_sync(0xffffffffu, need)) {
           // O is rescaled in place: the P V before has to be complete (the rare path)
           if (!mbar_wait(&bars.pv_done[i][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 48)) ok = false;
@@ -451,13 +506,13 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
             tmem_ld_x16(tmem_o + k, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * by);
             tmem_st_x16(tmem_o + k, r);
           }
           tmem_st_wait();
         }
         const float mr = m_ref == -INFINITY ? 0.f : m_ref;
-        const uint64_t scale2 = f2_pack(row_scale, row_scale), off2 = f2_pack(-mr, -mr);
+        const uint64_t scale2 = f2_pack(page_scale, page_scale), off2 = f2_pack(KVT_GAIN - mr, KVT_GAIN - mr);
         uint64_t sum = f2_pack(l0 * alpha, l1 * alpha);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -482,7 +537,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l;
+        const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l, back = __uint_as_float((uint32_t)(over - 13) << 23);
         __nv_bfloat16* dst = out + (size_t)(row0 + qi) * ldo + (size_t)head * D;
         const size_t pr = ((size_t)slot * hkv + kvh) * (2 * KVT_M) + i * KVT_M + row;
         if (slot >= 0 && live) part_ml[pr] = make_float2(m_ref == -INFINITY ? -3.0e38f : m_ref, l);
@@ -494,13 +549,14 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           if (slot >= 0) {
             if (l != 0.f) {                                      // (the merge does not read what has no weight)
 #pragma unroll
-              for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part_o + pr * D + k + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+              for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(part_o + pr * D + k + e) =
+                  make_float4(__uint_as_float(r[e]) * back, __uint_as_float(r[e + 1]) * back, __uint_as_float(r[e + 2]) * back, __uint_as_float(r[e + 3]) * back);
             }
             continue;
           }
           uint32_t o[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv);
+          for (int e = 0; e < 8; ++e) o[e] = l == 0.f ? 0u : pack_bf16x2(__uint_as_float(r[2 * e]) * inv * back, __uint_as_float(r[2 * e + 1]) * inv * back);
           reinterpret_cast<uint4*>(dst + k)[0] = make_uint4(o[0], o[1], o[2], o[3]);
           reinterpret_cast<uint4*>(dst + k)[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }

@@ -20,6 +20,10 @@ constexpr int KV4_PAGE = 64;
 __host__ __device__ constexpr int kv4_code_bytes(int dim) { return KV4_PAGE * dim / 2; }
 __host__ __device__ constexpr int kv4_page_bytes(int dim) { return KV4_PAGE * (dim / 2 + dim / 8); }
 
+// Attention divides a page's (scale, lo) by a power of two of their size, so that FP16 holds them: the exponent field (2^-110) that it has at least, and how
+// far below the greatest so far it may fall where sums are held over it.
+constexpr int KV4_LEAST = 17, KV4_SPAN = 60;
+
 // byte of 16-bit unit j of chunk c of token k's values
 template <int D>
 __device__ __forceinline__ int kv4_value_at(int k, int c, int j) {
@@ -37,5 +41,13 @@ __device__ __forceinline__ void kv4_lds(uint32_t addr, uint32_t& a, uint32_t& b,
 __device__ __forceinline__ void kv4_lds(uint32_t addr, uint32_t& a, uint32_t& b) {
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
+
+// by halves, and over the warp
+__device__ __forceinline__ uint32_t kv4_max2u(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t kv4_warp_max(uint32_t a) { return __reduce_max_sync(0xffffffffu, a); }
 
 }  // namespace ff

@@ -4,10 +4,13 @@ Bounds are relative to the terms themselves, so they shrink with the values. Wit
 magnitude of a scale or lo in key k's page:
 * the result's rounding to BF16, half a step: 2^-8 of it;
 * few rows: p scale, p and lo rounded to FP16, 2^-11 each: of p (v - lo), and twice of p |lo|, which is at most p (v - lo) + p |v|;
+* prompts in tiles: p and v rounded to FP16, 2^-11 of p |v| each, of keys that are rounded to 11 bits;
 * FP32 arithmetic (sums in other orders, exponentials of FP32 scores): 2^-14 of p |v| and of p (v - lo);
 * what is too small for FP16 beside the greatest of its page, M(k). Few rows: p, lo and p scale are held to 2^-25 where p is multiplied by 2^7, scale and lo by 2^7 over a
   power of two that is at most 2^5 M(k) (the power of an earlier page is kept while it is less than five binades above this one's): a weight is off by 2^-32 beside the greatest weight, times |lo|, a lo
   by 2^-32 x 2^5 M(k), times p, and a product p scale by 2^-39 x 2^5 M(k), times a code of 15. Together less than 2^-27 M(k) (p + 2^-3 of the greatest weight);
+* in tiles p is multiplied by 2^7 and the values by 2^13 over a power of two that is at most 2^11 M(k) (16 scale counts there, a binade is to spare, seven are kept): a scale or lo off by
+  2^-25 makes an element of code 15 off by less than 2^-20, that is 2^-22 M(k), times p; a weight is off by 2^-32 of the greatest, times |v|, at most 16 M(k);
 * a power of two is kept within 2^60 of the greatest so far, which no page here needs."""
 import math
 
@@ -59,7 +62,7 @@ def _terms(q, kpages, vpages, table, spans, hq, hkv, dim, scale, key_bits):
 
 
 def _check(got, res, mag, off, small, tiles):
-    tol = res.abs() * E + (2 * mag if tiles else 2 * off + 2 * mag) * 2.0 ** -11 + (mag + off) * 2.0 ** -14 + small * 2.0 ** -27
+    tol = res.abs() * E + (2 * mag if tiles else 2 * off + 2 * mag) * 2.0 ** -11 + (mag + off) * 2.0 ** -14 + small * (2.0 ** -22 if tiles else 2.0 ** -27)
     err = (got.cpu().double() - res).abs()
     worst = float((err / tol.clamp_min(1e-300)).max())
     assert worst <= 1, f"{worst} of the tolerance; off by {float(err.norm() / res.norm())} of the result"
@@ -75,6 +78,7 @@ def _run(q, kp, vp, table, lens, hq, hkv, dim, scale, nq=1):
 
 
 FEW = [(128, 8, 2, 1, [900, 70]), (64, 7, 1, 3, [2000, 3]), (128, 16, 1, 2, [5000]), (64, 4, 4, 1, [20000])]
+MANY = [(128, 16, 1, 9, [300, 2500]), (64, 4, 4, 70, [700]), (128, 8, 2, 40, [1500, 64, 5000]), (64, 28, 4, 9, [64, 12000])]
 
 
 def _dominant(q, kp, vp, table, hq, hkv, dim, scale, nq, blocks, nats):
@@ -93,7 +97,7 @@ def _made(dim, hq, hkv, nq, lens, seed=3):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("power", [7, 0, -10, -14, -20, -40, -100])
-@pytest.mark.parametrize("dim,hq,hkv,nq,lens", FEW)
+@pytest.mark.parametrize("dim,hq,hkv,nq,lens", FEW + MANY)
 def test_values_of_any_size(dim, hq, hkv, nq, lens, power):
     kp, vp, table, q, scale = _made(dim, hq, hkv, nq, lens)
     _resize(vp, dim, power)
@@ -103,7 +107,7 @@ def test_values_of_any_size(dim, hq, hkv, nq, lens, power):
 @pytest.mark.gpu
 @pytest.mark.parametrize("power", [0, -10, -14, -20])
 @pytest.mark.parametrize("nats", [8, 13])
-@pytest.mark.parametrize("dim,hq,hkv,nq,lens", FEW)
+@pytest.mark.parametrize("dim,hq,hkv,nq,lens", FEW + MANY)
 def test_a_key_far_above_the_others(dim, hq, hkv, nq, lens, nats, power):
     kp, vp, table, q, scale = _made(dim, hq, hkv, nq, lens)
     first = [int(table[i, 0]) for i in range(len(lens))]
@@ -119,7 +123,7 @@ def test_a_key_far_above_the_others(dim, hq, hkv, nq, lens, nats, power):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("powers", [(0, 7, -8, 3), (-20, 4, -3, -30), (-30, -6, 0, 7), (7, -2, -12, -30)])
-@pytest.mark.parametrize("dim,hq,hkv,nq,lens", FEW)
+@pytest.mark.parametrize("dim,hq,hkv,nq,lens", FEW + MANY)
 def test_pages_whose_values_differ(dim, hq, hkv, nq, lens, powers):
     kp, vp, table, q, scale = _made(dim, hq, hkv, nq, lens)
     for i, c in enumerate(lens):
@@ -127,6 +131,20 @@ def test_pages_whose_values_differ(dim, hq, hkv, nq, lens, powers):
             _resize(vp, dim, powers[p % len(powers)], int(table[i, p]))
             if p % 7 == 5:                                          # a page of zeros
                 vp[int(table[i, p])] = 0
+    _run(q, kp, vp, table, lens, hq, hkv, dim, scale, nq)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [7, -10, -20, -60])
+@pytest.mark.parametrize("dim,hq,hkv,nq,lens", FEW + MANY)
+def test_keys_of_any_size(dim, hq, hkv, nq, lens, power):
+    """Queries that make up for it; pages of keys differ by 2^6."""
+    kp, vp, table, q, scale = _made(dim, hq, hkv, nq, lens)
+    q.copy_(torch.ldexp(q.float(), torch.tensor(-power, device="cuda")).to(BF16))
+    _resize(kp, dim, power)
+    for i, c in enumerate(lens):
+        for p in range(1, -(-c // PAGE), 3):
+            _resize(kp, dim, -6, int(table[i, p]))
     _run(q, kp, vp, table, lens, hq, hkv, dim, scale, nq)
 
 
