@@ -39,11 +39,6 @@ __device__ __forceinline__ void kv4_bulk_load(void* dst, const void* src, uint32
 }
 __device__ __forceinline__ float kv4_low(uint32_t w) { return __uint_as_float(w << 16); }              // BF16 in the lower / upper half
 __device__ __forceinline__ float kv4_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ uint32_t kv4_mul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ float kv4_peer(const float* p, int rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(dsmem_addr(smem_u32(p), (uint32_t)rank)) : "memory");
@@ -77,7 +72,7 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 // with its own running maximum, sum and O. The warps' results meet in shared memory, those of up to eight CTAs (splits) in that of
 // their cluster, those of more in kv4_merge_kernel.
 // Bound by issue slots, not by the 5 bits an element of traffic: three sequences of up to 131071 tokens, 64 / 8 heads: 97 us for 474 MB (4.9 TB/s of the 6.5 a copy
-// reaches), 1195 instructions a page and warp, 60 % of the slots taken, the integer pipe 54 % busy. Columns by 8 keep 128 registers and four CTAs on an SM, by 16 (more
+// reaches) before the power of two, which adds 1 to 2 % (50 instructions to 1195 a page and warp; 60 % of the slots taken, the integer pipe 54 % busy). Columns by 8 keep 128 registers and four CTAs on an SM, by 16 (more
 // than 8 columns) they share a page's unpacking. Codes turned into BF16 operands first took 204 us, as subnormal ones 136, sums of p lo as a product 109.
 constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;      // (a warp for every group of a head at least)
 constexpr int KV4_KEPT = 4;                      // binades that a page's values may lie below the power of two that a warp has for them
@@ -359,10 +354,10 @@ kv4_rows_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__
         for (int k = 0; k < 4; ++k) {
           // tokens behind the sequence: whatever the page holds there is no number, and 0 times it would not be 0
           if (p * KV4_PAGE + KV4_PAGE > ctx && p * KV4_PAGE + (4 * (lane + 32 * i) + k) / NG >= ctx) st[i][k] = 0u;
-          most = kv4_max2u(most, st[i][k] & 0x7fff7fffu);
+          most = kv4_maxabs2(most, st[i][k]);
         }
       }
-      const int ex = max((int)(kv4_warp_max(max(most & 0xffffu, most >> 16)) >> 7), KV4_LEAST);
+      const int ex = max((int)(kv4_warp_max(max(most & 0x7fffu, most >> 16 & 0x7fffu)) >> 7), KV4_LEAST);
       if (ex > ref || ex + KV4_KEPT < ref) {                    // (for all lanes)
         top = max(top, ex);
         const int next = max(ex, top - KV4_SPAN);

@@ -2,20 +2,25 @@
 //
 // The rows of a sequence times the query heads of one kv head are flattened (row c: query c / G, head c % G of the group), and a CTA has two tiles of 128 of
 // them over one kv head: both read the same keys and values, so a page is turned into FP16 once for 256 rows. Per page j of 64 tokens:
-//   one thread    fetches the page by bulk copies, three pages ahead
+//   one warp      fetches the page by bulk copies, three pages ahead, and finds its powers of two
 //   four warps    write keys and values code * scale + lo, rounded once, as 128-byte-swizzled tiles
 //   two threads   one for a tile i: S_i(j + 1) = Q_i K^T, then O_i += P_i V; S, P and O live in tensor memory (P over the S that it came from). (One thread for both
 //                 spends 1400 cycles a page on issuing and on barriers, as long as the products take.)
 //   two x 4 warps soft-max of a tile, a thread per row: running maximum and sum in FP32 in the base-2 domain; O is rescaled only when the maximum has moved
 //                 by more than 2^8 (the stale one stays exact: P and the sum share it)
 // All operands are FP16, this kernel's choice of a rounding: keys, values and weights keep 11 bits where BF16 has 8 (outputs 0.0017 off in the root mean square,
-// as a single rounding of the result is; 0.0035 with BF16 operands). The cache's elements are at most 2^15, so they fit; a scale or lo below 2^-14 is off by
-// 2^-25, an element by 2^-20 then. Queries are divided by a power of two per row, which the soft-max's scale takes back.
+// as a single rounding of the result is; 0.0035 with BF16 operands). Whatever size they are: the warp that fetches pages finds a page's greatest |lo| and 16 scale, and its keys and
+// its values are divided by a power of two of that and multiplied by 2^13 (elements stay below 2^15; what lies 2^-28 below is off by 2^-38 of the greatest). The soft-max takes the keys'
+// back page by page; O is held over the values', which rises with a binade to spare and falls behind pages 2^KVT_KEPT smaller, by the path that rescales O. Weights are
+// multiplied by 2^7, so that they have 11 bits down to 2^-21. Operands as they are take 584 us where this takes 599, but elements of 2^-20 were off by 8 % and more. Queries are divided by a power
+// of two per row, which the soft-max's scale takes back.
 // S(j + 1) of a tile waits for its P V (j - 1), whose P it overwrites; the other tile's products run meanwhile.
-// 8191 rows of 32 / 8 heads of 128 from the beginning: 567 us, 970 TFLOP/s (626 in a row, at the clock that power leaves then). The products alone take 403 (S = Q K^T has 64
+// 8191 rows of 32 / 8 heads of 128 from the beginning: 599 us, 918 TFLOP/s (641 in a row, at the clock that power leaves then). What the parts take was measured when operands were as they are and
+// the whole took 567: the products alone 403 (S = Q K^T has 64
 // columns, for which shared memory feeds the tensor cores at two thirds of their rate), the tiles of keys and values alone 475, both without the soft-max 500. They share
 // shared memory (128 KB of operands a page, 42 for the tiles, some 1350 of 2050 cycles) and issue slots (54 % taken): eight warps for the tiles, with registers that the
-// others give up, take 617.
+// others give up, take 617. The warps that write the tiles wait for loads and barriers rather than for issue slots: a page read at once, one wait and one fence for
+// keys and values gave 3 % back of the 6 that the powers of two took, another wait costs 7.
 // Every wait is bounded; a time-out records FF_ERR_TIMEOUT, and all roles leave through the abort flag.
 #include "kv4.cuh"
 #include "host_util.h"
@@ -24,16 +29,18 @@
 namespace ff {
 
 constexpr int KVT_M = 128, KVT_N = KV4_PAGE, KVT_STAGES = 3;
-constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 4;      // warps 0-7 soft-max, 8-11 tiles, 12 and 14 products, 13 pages, 15 sizes
-constexpr int KVT_PAGES = 3;                                                         // pages on their way or being turned into tiles
-constexpr int KVT_SIZES = 8;                                                         // pages whose sizes are known: more than are between warp 15 and the soft-max
+constexpr int KVT_SOFT = 8, KVT_FILL = 4, KVT_WARPS = KVT_SOFT + KVT_FILL + 3;      // warps 0-7 soft-max, 8-11 tiles, 12 and 14 products, 13 pages
+constexpr int KVT_PAGES = 3;                                                         // pages on their way or being turned into tiles (four: 627 us where three took 619)
+constexpr int KVT_SIZES = 8;                                                         // pages whose sizes are known: more than are between warp 13 and the soft-max
 constexpr int KVT_KEPT = 6;                                                          // binades that a page's values may lie below the power of two that they are divided by
 constexpr float KVT_MOVED = 8.0f, KVT_GAIN = 7.0f;                                   // log2 units: how far a maximum may lie behind, and what weights are multiplied by
 template <int D> constexpr int kvt_smem() { return 2 * KVT_M * D * 2 + 2 * KVT_STAGES * KVT_N * D * 2 + KVT_PAGES * 2 * kv4_page_bytes(D) + 1024; }
 
 struct alignas(8) KvtBars {
-  uint64_t q_full[2], k_full[KVT_STAGES], k_empty[KVT_STAGES], v_full[KVT_STAGES], v_empty[KVT_STAGES], s_full[2][2], p_full[2][2], pv_done[2][2], p_in[KVT_PAGES], p_out[KVT_PAGES], e_ready[KVT_SIZES];
-  int2 size[KVT_SIZES];                                                                // exponent fields of the powers of two that keys and values are divided by
+  uint64_t q_full[2], k_full[KVT_STAGES], v_full[KVT_STAGES], v_empty[KVT_STAGES], s_full[2][2], p_full[2][2], pv_done[2][2], p_in[KVT_PAGES], p_out[KVT_PAGES], e_ready[KVT_SIZES];
+  float2 size[KVT_SIZES];                                                              // what a page's scores are multiplied by, and O in front of it
+  uint2 by[KVT_SIZES];                                                                 // its keys' and values' scale and lo, twice in BF16
+  float back;                                                                          // what O is multiplied by in the end
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -43,10 +50,11 @@ __device__ __forceinline__ float kvt_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// nibbles at bits s and s + 16 times scale plus lo as FP16, one rounding (1024 + n is an FP16 number, the difference is exact)
-__device__ __forceinline__ uint32_t kvt_value(uint32_t w, int s, uint32_t scale2, uint32_t lo2) {
-  uint32_t n = ((w >> s) & 0x000f000fu) | 0x64006400u, r;
-  asm("{\n\t.reg .b32 t;\n\tadd.rn.f16x2 t, %1, %2;\n\tfma.rn.f16x2 %0, t, %3, %4;\n\t}" : "=r"(r) : "r"(n), "r"(0xe400e400u), "r"(scale2), "r"(lo2));
+// nibbles at bits 0 and 16 (HIGH: 4 and 20) times scale plus lo as FP16, one rounding (1024 + n, 64 + n are FP16 numbers, the difference is exact)
+template <bool HIGH>
+__device__ __forceinline__ uint32_t kvt_value(uint32_t w, uint32_t scale2, uint32_t lo2) {
+  uint32_t n = HIGH ? (w & 0x00f000f0u) | 0x54005400u : (w & 0x000f000fu) | 0x64006400u, r;
+  asm("{\n\t.reg .b32 t;\n\tadd.rn.f16x2 t, %1, %2;\n\tfma.rn.f16x2 %0, t, %3, %4;\n\t}" : "=r"(r) : "r"(n), "r"(HIGH ? 0xd400d400u : 0xe400e400u), "r"(scale2), "r"(lo2));
   return r;
 }
 __device__ __forceinline__ uint32_t kvt_f16x2(float lo, float hi) {
@@ -245,7 +253,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       for (int k = 0; k < 2; ++k) { mbar_init(&bars.s_full[i][k], 1); mbar_init(&bars.p_full[i][k], 4); mbar_init(&bars.pv_done[i][k], 1); }
     }
     for (int i = 0; i < KVT_STAGES; ++i) {
-      mbar_init(&bars.k_full[i], KVT_FILL); mbar_init(&bars.k_empty[i], two); mbar_init(&bars.v_full[i], KVT_FILL); mbar_init(&bars.v_empty[i], two);
+      mbar_init(&bars.k_full[i], KVT_FILL); mbar_init(&bars.v_full[i], KVT_FILL); mbar_init(&bars.v_empty[i], two);
     }
     for (int i = 0; i < KVT_PAGES; ++i) { mbar_init(&bars.p_in[i], 1); mbar_init(&bars.p_out[i], KVT_FILL); }
     for (int i = 0; i < KVT_SIZES; ++i) mbar_init(&bars.e_ready[i], 1);
@@ -267,31 +275,42 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
     RingPos pr, tr;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      if (!mbar_wait(&bars.p_in[pr.s], pr.ph, abort_flag, status, KID_ATTN_PREFILL, 40)) ok = false;
-      if (!mbar_wait(&bars.e_ready[j % KVT_SIZES], (j / KVT_SIZES) & 1, abort_flag, status, KID_ATTN_PREFILL, 51)) ok = false;
+      if (!mbar_wait(&bars.e_ready[j % KVT_SIZES], (j / KVT_SIZES) & 1, abort_flag, status, KID_ATTN_PREFILL, 40)) ok = false;
+      // (its values multiplied, the keys of a stage are too)
+      if (!mbar_wait(&bars.v_empty[tr.s], tr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 41)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       const uint32_t page = smem_u32(sP) + pr.s * 2 * PB;
+      const uint2 by = bars.by[j % KVT_SIZES];
+      uint32_t code[2][2][NG], stat[2][2][NG];
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        if (!mbar_wait(part ? &bars.v_empty[tr.s] : &bars.k_empty[tr.s], tr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 41 + part)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        uint32_t code[2][NG], stat[2][NG];
+      for (int part = 0; part < 2; ++part)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int key = key0 + 32 * i;
-          kvt_load<D>(code[i], page + part * PB + (part ? kv4_value_at<D>(key, 2 * u, 0) : key * (D / 2) + u * (D / 8)));
-          kvt_load<D>(stat[i], page + part * PB + kv4_code_bytes(D) + key * (D / 8));
+          kvt_load<D>(code[part][i], page + part * PB + (part ? kv4_value_at<D>(key, 2 * u, 0) : key * (D / 2) + u * (D / 8)));
+          kvt_load<D>(stat[part][i], page + part * PB + kv4_code_bytes(D) + key * (D / 8));
         }
+      if ((first + j) * KVT_N + KVT_N > ctx) {                   // behind the sequence
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+            if ((first + j) * KVT_N + key0 + 32 * i >= ctx) stat[0][i][g] = stat[1][i][g] = 0u;
+      }
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           uint32_t v[2][4];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t scale2 = kvt_prmt(stat[i][g], stat[i][g], 0x1010u), lo2 = kvt_prmt(stat[i][g], stat[i][g], 0x3232u);
+            const float2 sl = unpack_bf16x2(kv4_mul2(stat[part][i][g], part ? by.y : by.x));
+            const uint32_t scale2 = kvt_f16x2(sl.x, sl.x), lo2 = kvt_f16x2(sl.y, sl.y);
             // values: 16-bit unit g of two chunks, the even elements and the odd ones
-            const uint32_t word = part ? kvt_prmt(code[i][g / 2], code[i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[i][g];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = kvt_value(word, 4 * k, scale2, lo2);
+            const uint32_t word = part ? kvt_prmt(code[1][i][g / 2], code[1][i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[0][i][g];
+            v[i][0] = kvt_value<false>(word, scale2, lo2); v[i][1] = kvt_value<true>(word, scale2, lo2);
+            v[i][2] = kvt_value<false>(word >> 8, scale2, lo2); v[i][3] = kvt_value<true>(word >> 8, scale2, lo2);
           }
           const int c = 4 * g + u;                               // 16-byte chunk of the row: 64-element block c / 8
 #pragma unroll
@@ -300,79 +319,72 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
             kv4_sts(smem_u32(part ? sV : sK) + tr.s * TILE + key * 128 + (c >> 3) * (KVT_N * 128) + (((c & 7) ^ (key & 7)) << 4), v[i][0], v[i][1], v[i][2], v[i][3]);
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(part ? &bars.v_full[tr.s] : &bars.k_full[tr.s]);
       }
-      if (!ok) break;
-      if (lane == 0) mbar_arrive(&bars.p_out[pr.s]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&bars.k_full[tr.s]); mbar_arrive(&bars.v_full[tr.s]); mbar_arrive(&bars.p_out[pr.s]); }
       pr.next(KVT_PAGES);
       tr.next(KVT_STAGES);
     }
   } else if (warp == KVT_SOFT + KVT_FILL + 1) {
     // ================================ pages ================================
-    if (elect_one()) {
-      bool bad = false;
-      RingPos pr;
-      int blk = tiles > 0 ? block_table[(size_t)b * max_blocks + first] : 0;
-      for (int j = 0; j < tiles; ++j) {
-        const int next = j + 1 < tiles ? block_table[(size_t)b * max_blocks + first + j + 1] : 0;
+    // A page is fetched, and the one before it gets its powers of two: 2^13 over the one that the greatest of |lo| and 16 scale lies in, so that elements are below 2^15
+    bool bad = false;
+    RingPos pr, sr;
+    int ref = 0, top = 0;
+    int blk = tiles > 0 ? block_table[(size_t)b * max_blocks + first] : 0;
+    for (int i = 0; i <= tiles && tiles > 0; ++i) {
+      if (i < tiles) {
+        const int next = i + 1 < tiles ? block_table[(size_t)b * max_blocks + first + i + 1] : 0;
         if (blk < 0 || blk >= num_blocks) { bad = true; blk = 0; }
-        const size_t at = ((size_t)blk * hkv + kvh) * PB;
-        if (!mbar_wait(&bars.p_out[pr.s], pr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 39)) break;
-        mbar_expect_tx(&bars.p_in[pr.s], 2 * PB);
-        kvt_bulk_load(sP + pr.s * 2 * PB, kpages + at, PB, &bars.p_in[pr.s]);
-        kvt_bulk_load(sP + pr.s * 2 * PB + PB, vpages + at, PB, &bars.p_in[pr.s]);
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.p_out[pr.s], pr.ph ^ 1, abort_flag, status, KID_ATTN_PREFILL, 39))) break;
+        if (lane == 0) {
+          const size_t at = ((size_t)blk * hkv + kvh) * PB;
+          mbar_expect_tx(&bars.p_in[pr.s], 2 * PB);
+          kvt_bulk_load(sP + pr.s * 2 * PB, kpages + at, PB, &bars.p_in[pr.s]);
+          kvt_bulk_load(sP + pr.s * 2 * PB + PB, vpages + at, PB, &bars.p_in[pr.s]);
+        }
+        __syncwarp();
         pr.next(KVT_PAGES);
         blk = next;
       }
-      if (bad) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
-    }
-  } else if (warp == KVT_SOFT + KVT_FILL + 3) {
-    // ================================ sizes ================================
-    // (scale, lo) of a page, in place, as FP16 numbers: times 2^13 over a power of two that the greatest of |lo| and 16 scale lies in, so that elements are below 2^15
-    RingPos pr;
-    int ref = 0, top = 0;
-    for (int j = 0; j < tiles; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars.p_in[pr.s], pr.ph, abort_flag, status, KID_ATTN_PREFILL, 38))) break;
-      int size[2];
+      if (i == 0) continue;
+      const int j = i - 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars.p_in[sr.s], sr.ph, abort_flag, status, KID_ATTN_PREFILL, 38))) break;
+      int ex[2];
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        const uint32_t at = smem_u32(sP) + pr.s * 2 * PB + part * PB + kv4_code_bytes(D) + 16 * lane;
+        const uint32_t at = smem_u32(sP) + sr.s * 2 * PB + part * PB + kv4_code_bytes(D) + 16 * lane;
         uint32_t st[NG / 2][4], most = 0u;
 #pragma unroll
-        for (int i = 0; i < NG / 2; ++i) {
-          kv4_lds(at + 512 * i, st[i][0], st[i][1], st[i][2], st[i][3]);
+        for (int h = 0; h < NG / 2; ++h) kv4_lds(at + 512 * h, st[h][0], st[h][1], st[h][2], st[h][3]);
+        if ((first + j) * KVT_N + KVT_N > ctx) {                 // behind the sequence: whatever the page holds there is no number
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // behind the sequence: whatever the page holds there is no number
-            if ((first + j) * KVT_N + (4 * (lane + 32 * i) + k) / NG >= ctx) st[i][k] = 0u;
-            most = kv4_max2u(most, (st[i][k] & 0x7fff7fffu) + 0x0200u);
-          }
-        }
-        int ex = max((int)(kv4_warp_max(max(most & 0xffffu, most >> 16)) >> 7), KV4_LEAST);
-        if (part) {
-          // O is held over the values' power: it rises with a binade to spare, and falls only behind much smaller pages
-          if (ex > ref) ref = ex + 1;
-          else if (ex + KVT_KEPT < ref) ref = max(ex + 1, top - KV4_SPAN);
-          top = max(top, ref);
-          ex = ref;
-        }
-        size[part] = ex;
-        const float by = __uint_as_float((uint32_t)(267 - ex) << 23);
+          for (int h = 0; h < NG / 2; ++h)
 #pragma unroll
-        for (int i = 0; i < NG / 2; ++i) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) { const float2 v = unpack_bf16x2(st[i][k]); st[i][k] = kvt_f16x2(v.x * by, v.y * by); }
-          kv4_sts(at + 512 * i, st[i][0], st[i][1], st[i][2], st[i][3]);
+            for (int k = 0; k < 4; ++k)
+              if ((first + j) * KVT_N + (4 * (lane + 32 * h) + k) / NG >= ctx) st[h][k] = 0u;
         }
+#pragma unroll
+        for (int h = 0; h < NG / 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) most = kv4_maxabs2(most, st[h][k]);
+        ex[part] = max((int)(kv4_warp_max(max((most & 0x7fffu) + 0x0200u, most >> 16 & 0x7fffu)) >> 7), KV4_LEAST);
       }
-      fence_proxy_async_smem();                                  // (a bulk copy writes the place next)
-      if (lane == 0) bars.size[j % KVT_SIZES] = make_int2(size[0], size[1]);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.e_ready[j % KVT_SIZES]);
-      pr.next(KVT_PAGES);
+      // O is held over the values' power: it rises with a binade to spare, and falls only behind much smaller pages
+      const int before = j > 0 ? ref : ex[1] + 1;
+      if (ex[1] > ref) ref = ex[1] + 1;
+      else if (ex[1] + KVT_KEPT < ref) ref = max(ex[1] + 1, top - KV4_SPAN);
+      top = max(top, ref);
+      if (lane == 0) {
+        bars.size[j % KVT_SIZES] = make_float2(__uint_as_float((uint32_t)(ex[0] - 13) << 23), __uint_as_float((uint32_t)(127 + before - ref) << 23));
+        bars.by[j % KVT_SIZES] = make_uint2((uint32_t)(267 - ex[0]) * 0x00800080u, (uint32_t)(267 - ref) * 0x00800080u);
+        if (j == tiles - 1) bars.back = __uint_as_float((uint32_t)(ref - 13) << 23);
+        mbar_arrive(&bars.e_ready[j % KVT_SIZES]);
+      }
+      sr.next(KVT_PAGES);
     }
+    if (bad && lane == 0) set_status(status, KID_ATTN_PREFILL, FF_ERR_BOUNDS, b, c0);
   } else if (warp >= KVT_SOFT + KVT_FILL) {
     // ================================ products: a warp for each tile ================================
     const int i = warp == KVT_SOFT + KVT_FILL ? 0 : 1;
@@ -393,7 +405,6 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         for (int k = 0; k < D / 16; ++k)
           umma_f16(s_at + 64 * (j & 1), qd + (uint32_t)(((k >> 2) * (KVT_M * 128) + (k & 3) * 32) >> 4), d + (uint32_t)(((k >> 2) * (KVT_N * 128) + (k & 3) * 32) >> 4), idesc_s, k != 0);
         umma_commit(&bars.s_full[i][j & 1]);
-        umma_commit(&bars.k_empty[kr.s]);
         kr.next(KVT_STAGES);
         return true;
       };
@@ -453,17 +464,19 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       const uint32_t tmem_o = tmem + 256 + 128 * i + lanes;
       float m_ref = -INFINITY;
       float l0 = 0.f, l1 = 0.f;
-      int over = KV4_LEAST;                                              // exponent field of the power of two that O is held over
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
         const uint32_t s_addr = tmem + 128 * i + 64 * (j & 1) + lanes;
-        if (!mbar_wait(&bars.s_full[i][j & 1], (j >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 47)) ok = false;
-        if (!mbar_wait(&bars.e_ready[j % KVT_SIZES], (j / KVT_SIZES) & 1, abort_flag, status, KID_ATTN_PREFILL, 52)) ok = false;
+        {
+          const bool sized = mbar_try_wait(&bars.e_ready[j % KVT_SIZES], (j / KVT_SIZES) & 1), there = mbar_try_wait(&bars.s_full[i][j & 1], (j >> 1) & 1);
+          if (!sized && !mbar_wait(&bars.e_ready[j % KVT_SIZES], (j / KVT_SIZES) & 1, abort_flag, status, KID_ATTN_PREFILL, 51)) ok = false;
+          if (!there && !mbar_wait(&bars.s_full[i][j & 1], (j >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 47)) ok = false;
+        }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const int2 size = bars.size[j % KVT_SIZES];
-        const float page_scale = fmaxf(row_scale * __uint_as_float((uint32_t)(size.x - 13) << 23), 1.1754944e-38f);      // (times minus infinity it has to be that)
+        const float2 size = bars.size[j % KVT_SIZES];
+        const float page_scale = fmaxf(row_scale * size.x, 1.1754944e-38f);      // (times minus infinity it has to be that)
         float s[KVT_N];
         {
           uint32_t r[KVT_N];
@@ -488,18 +501,14 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           m_ref = mx;
           need = j > 0;
         }
-        float by = alpha;
-        if (size.y != over) {
-          by *= __uint_as_float((uint32_t)(127 + over - size.y) << 23);
-          need = j > 0;
-        }
-        over = size.y;
+        need = need || size.y != 1.f;                                    // (1 for the first page)
         if (__any_sync(0xffffffffu, need)) {
           // O is rescaled in place: the P V before has to be complete (the rare path)
           if (!mbar_wait(&bars.pv_done[i][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, status, KID_ATTN_PREFILL, 48)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
+          const float by = alpha * size.y;
 #pragma unroll
           for (int k = 0; k < D; k += 16) {
             uint32_t r[16];
@@ -537,7 +546,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l, back = __uint_as_float((uint32_t)(over - 13) << 23);
+        const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l, back = tiles > 0 ? bars.back : 1.f;
         __nv_bfloat16* dst = out + (size_t)(row0 + qi) * ldo + (size_t)head * D;
         const size_t pr = ((size_t)slot * hkv + kvh) * (2 * KVT_M) + i * KVT_M + row;
         if (slot >= 0 && live) part_ml[pr] = make_float2(m_ref == -INFINITY ? -3.0e38f : m_ref, l);

@@ -42,12 +42,11 @@ __device__ __forceinline__ void kv4_lds(uint32_t addr, uint32_t& a, uint32_t& b)
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
 
-// by halves, and over the warp
-__device__ __forceinline__ uint32_t kv4_max2u(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
+// by halves
+__device__ __forceinline__ uint32_t kv4_mul2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+// the one of greater magnitude, with either's sign
+__device__ __forceinline__ uint32_t kv4_maxabs2(uint32_t a, uint32_t b) { uint32_t r; asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+// over the warp
 __device__ __forceinline__ uint32_t kv4_warp_max(uint32_t a) { return __reduce_max_sync(0xffffffffu, a); }
 
 }  // namespace ff
