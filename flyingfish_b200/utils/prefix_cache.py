@@ -185,7 +185,7 @@ class PrefixStore:
         digest = identity_for(model).digest()
         if n == 0 or any(e["token_hash"] == th and e["identity"] == digest for e in index):
             return None
-        name = f"{th[:16]}-{n}"
+        name = f"{digest[:8]}-{th[:16]}-{n}"       # (models and cache formats share the directory)
         d = save_prefix(model, seq, self.root / name)
         index.append({"dir": name, "length": n, "token_hash": th, "identity": digest})
         (self.root / "index.json").write_text(json.dumps(index))
