@@ -71,6 +71,13 @@ def page_values(pages: torch.Tensor, dim: int, keys: bool) -> torch.Tensor:
     return torch.addcmul(stats[..., 1], code.float(), stats[..., 0])
 
 
+def token_bytes(dim: int, keys: bool) -> torch.Tensor:
+    """Which bytes of a page each token has: int64 [64, page_bytes(dim) / 64], codes first (a byte's two codes belong to one token)."""
+    codes = _places(dim, keys)[0].sort(dim=1).values[:, ::2]
+    width = dim // GROUP * 4
+    return torch.cat([codes, PAGE * dim // 2 + torch.arange(PAGE * width).view(PAGE, width)], dim=1)
+
+
 def _write_rows(pages: torch.Tensor, rows: torch.Tensor, slots: torch.Tensor, dim: int, keys: bool) -> None:
     byte, shift = _places(dim, keys)
     code, scale, lo = quantise(rows)

@@ -19,6 +19,7 @@ from pathlib import Path
 import torch
 
 from ..loaders.safetensors_io import SafetensorsFile, save_safetensors
+from ..ops import kv4_ops
 
 FORMAT = "flyingfish-prefix-1"
 
@@ -71,8 +72,11 @@ def save_prefix(model, seq, directory: str | Path) -> Path:
         for tag, cache in (("k", eng.kv.k[l]), ("v", eng.kv.v[l])):
             if cache is None:
                 continue
-            if eng.kv.kv_format == "affine4":          # whole pages as they are; what lies behind the prefix is never read
-                tensors[f"layer.{l}.{tag}"] = cache[blocks].cpu()
+            if eng.kv.kv_format == "affine4":          # whole pages; behind the prefix a used block holds another request's tokens
+                pages = cache[blocks].cpu()
+                if n % bs:
+                    pages[-1][:, kv4_ops.token_bytes(eng.kv.geometry[l][1], tag == "k")[n % bs:].flatten()] = 0
+                tensors[f"layer.{l}.{tag}"] = pages
                 continue
             rows = cache[blocks].permute(1, 0, 2, 3).reshape(cache.shape[1], -1, cache.shape[3])[:, :n]
             tensors[f"layer.{l}.{tag}"] = rows.contiguous().cpu()
@@ -122,8 +126,11 @@ def restore_prefix(model, directory: str | Path, limit: int | None = None):
                 if cache is None:
                     continue
                 if eng.kv.kv_format == "affine4":
-                    at = torch.tensor(kvs.blocks[: (n + bs - 1) // bs], device=eng.device)
-                    cache[at] = f.tensor(f"layer.{l}.{tag}")[: at.numel()].to(eng.device)
+                    pages, whole = f.tensor(f"layer.{l}.{tag}"), n // bs
+                    cache[torch.tensor(kvs.blocks[:whole], dtype=torch.int64, device=eng.device)] = pages[:whole].to(eng.device)
+                    if n % bs:
+                        at = kv4_ops.token_bytes(eng.kv.geometry[l][1], tag == "k")[: n % bs].flatten()
+                        cache[kvs.blocks[whole]][:, at.to(eng.device)] = pages[whole][:, at].to(eng.device)
                     continue
                 rows = f.tensor(f"layer.{l}.{tag}")[:, :n].to(eng.device)   # [heads, n, dim]
                 cache[blk, :, off, :] = rows.permute(1, 0, 2).to(cache.dtype)

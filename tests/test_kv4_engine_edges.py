@@ -2,6 +2,9 @@
 import pytest
 import torch
 
+from flyingfish_b200.loaders.safetensors_io import SafetensorsFile
+from flyingfish_b200.ops import kv4_ops
+from flyingfish_b200.utils.prefix_cache import restore_prefix, save_prefix
 from test_kv4_engine import _load, _prompt
 
 
@@ -16,3 +19,50 @@ def test_one_store_holds_a_prompt_in_both_formats(tmp_path, order):
         assert (store.stored, store.hits) == ((0, 1) if again else (1, 0))
         got = [first] + [m.decode() for _ in range(3)]
         assert got == want.setdefault(kv_format, got)
+
+
+@pytest.mark.parametrize("n", [64, 66, 127])
+def test_stored_pages_hold_nothing_of_other_requests(tmp_path, n):
+    """A block that was used before still holds another request's keys and values behind a prefix: they are not stored with it."""
+    m = _load("cpu", capacity=256)
+    kv = m.engine.kv
+    for t in kv.k + kv.v:
+        t.fill_(0x5A)
+    seq = m.engine.add_sequence(_prompt(n))
+    m.engine.prefill([seq])
+    m.engine.decode([seq])
+    kv.truncate(seq.seq_id, n)
+    held = kv.seqs[seq.seq_id].blocks
+    before = [t[held].clone() for t in kv.k + kv.v]
+    pkg = save_prefix(m, seq, tmp_path / "pfx")
+    assert all(torch.equal(t[held], w) for t, w in zip(kv.k + kv.v, before))
+    f = SafetensorsFile(pkg / "kv.safetensors")
+    try:
+        for layer in range(kv.layers):
+            for tag, cache, keys in (("k", kv.k[layer], True), ("v", kv.v[layer], False)):
+                pages = f.tensor(f"layer.{layer}.{tag}")
+                values = kv4_ops.page_values(pages, m.engine.model.d, keys).transpose(0, 1).flatten(1, 2)
+                want = kv4_ops.page_values(cache[held], m.engine.model.d, keys).transpose(0, 1).flatten(1, 2)
+                assert torch.equal(values[:, :n], want[:, :n]) and not values[:, n:].any()
+                assert int((pages[-1] == 0x5A).sum()) <= pages[-1].numel() // 64       # (a code may be that by chance)
+    finally:
+        f.close()
+    # and restored into a used block, tokens behind them stay
+    m.reset()
+    for t in kv.k + kv.v:
+        t.fill_(0xA5)
+    seq = restore_prefix(m, pkg)
+    assert kv.seqs[seq.seq_id].length == n
+    for cache, was, keys in zip(kv.k + kv.v, before, [True] * kv.layers + [False] * kv.layers):
+        got, want = (kv4_ops.page_values(t, m.engine.model.d, keys).transpose(0, 1).flatten(1, 2)[:, :n] for t in (cache[kv.seqs[seq.seq_id].blocks], was))
+        assert torch.equal(got, want)
+        if n % 64:
+            assert bool((cache[kv.seqs[seq.seq_id].blocks[-1]][:, kv4_ops.token_bytes(m.engine.model.d, keys)[n % 64:].flatten()] == 0xA5).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("keys", [True, False])
+def test_every_byte_of_a_page_is_a_tokens(dim, keys):
+    at = kv4_ops.token_bytes(dim, keys)
+    assert torch.equal(at.flatten().sort().values, torch.arange(kv4_ops.page_bytes(dim)))
+    assert all(set(at[k, : dim // 2].tolist()) == set(kv4_ops._places(dim, keys)[0][k].tolist()) for k in range(64))
