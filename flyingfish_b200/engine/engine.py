@@ -335,7 +335,7 @@ class Engine:
     def _need_blocks(self, items: list[tuple[int, int]]) -> None:
         """Refuse a step before it reserves anything when the (sequence, new tokens) pairs do not all fit: a step
         either reserves for every sequence or for none."""
-        need = sum(self.kv.blocks_needed(sid, n) for sid, n in items)
+        need = self.kv.blocks_wanted(items)
         if need > self.kv.alloc.free_blocks:
             raise OutOfBlocks(f"step needs {need} KV blocks, {self.kv.alloc.free_blocks} free")
 

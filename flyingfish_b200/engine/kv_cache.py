@@ -127,6 +127,18 @@ class PagedKVCache:
         need = (total + self.block_size - 1) // self.block_size
         return max(0, need - len(s.blocks)) + (1 if new_tokens > 0 and self.alloc.shared and self._inside_shared(s) else 0)
 
+    def blocks_wanted(self, items: list[tuple[int, int]]) -> int:
+        """Free blocks that a step takes which reserves (sequence, new tokens) for all of them, one after the other: where they are all the owners of a block that they stand
+        inside of, the last one keeps it."""
+        total, inside = 0, {}
+        for i, n in items:
+            s = self.seqs[i]
+            total += max(0, (s.length + n + self.block_size - 1) // self.block_size - len(s.blocks))
+            if n > 0 and self.alloc.shared and self._inside_shared(s):
+                block = s.blocks[s.length // self.block_size]
+                inside[block] = inside.get(block, 0) + 1
+        return total + sum(min(n, self.alloc.refcount(block) - 1) for block, n in inside.items())
+
     def _inside_shared(self, s: SequenceKV) -> bool:
         """Whether the sequence's next row would go into a block that is not its own alone."""
         at = s.length // self.block_size
@@ -181,7 +193,7 @@ class PagedKVCache:
         held, bs = [self.seqs[i] for i in seq_ids], self.block_size
         short = [s for s in held if s.length >= len(s.blocks) * bs]
         inside = [s for s in held if self._inside_shared(s)] if self.alloc.shared else []
-        need = sum(self.blocks_needed(s.seq_id, 1) for s in short) + len(inside)
+        need = self.blocks_wanted([(s.seq_id, 1) for s in short + inside])
         if need > self.alloc.free_blocks:
             raise OutOfBlocks(f"step needs {need} KV blocks, {self.alloc.free_blocks} free")
         if inside:

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from flyingfish_b200.engine.kv_cache import PagedKVCache
 from flyingfish_b200.loaders.safetensors_io import SafetensorsFile
 from flyingfish_b200.ops import kv4_ops
 from flyingfish_b200.utils.prefix_cache import restore_prefix, save_prefix
@@ -66,3 +67,40 @@ def test_every_byte_of_a_page_is_a_tokens(dim, keys):
     at = kv4_ops.token_bytes(dim, keys)
     assert torch.equal(at.flatten().sort().values, torch.arange(kv4_ops.page_bytes(dim)))
     assert all(set(at[k, : dim // 2].tolist()) == set(kv4_ops._places(dim, keys)[0][k].tolist()) for k in range(64))
+
+
+@pytest.mark.parametrize("kv_format", ["bf16", "affine4"])
+def test_the_last_owner_of_a_shared_block_keeps_it_cpu(kv_format):
+    """Sequences that were all taken back into a block that nobody else has: one of them needs no copy, and no free block for it."""
+    kv = PagedKVCache(1, 1, 64, 4, kv_format=kv_format)
+    kv.add_sequence(0)
+    kv.reserve(0, 64)
+    kv.commit(0, 64)
+    kv.fork(0, 1)
+    kv.fork(0, 2)
+    for i in (0, 1, 2):
+        kv.truncate(i, 30 + i)
+    kv.add_sequence(3)
+    kv.reserve(3, 64)
+    assert kv.alloc.free_blocks == 2 and kv.blocks_wanted([(0, 1), (1, 1), (2, 1)]) == 2 == kv.blocks_wanted([(0, 1), (2, 20)]) and kv.blocks_wanted([(1, 60)]) == 2
+    held, at, slots = kv.reserve_step([0, 1, 2])
+    assert kv.alloc.shared == 0 == kv.alloc.free_blocks and len({int(s) // 64 for s in slots}) == 3 and [int(s) % 64 for s in slots] == [30, 31, 32]
+    for i in range(4):
+        kv.free_sequence(i)
+    assert kv.alloc.free_blocks == 4
+
+
+def test_a_step_over_forks_taken_back_needs_the_copies_that_are_made_cpu():
+    m = _load("cpu")
+    eng, ids = m.engine, _prompt(64)
+    a = eng.add_sequence(ids)
+    eng.prefill([a])
+    b = eng.fork(a)
+    for s in (a, b):
+        eng.kv.truncate(s.seq_id, 30)
+    eng.kv.add_sequence(99)
+    eng.kv.reserve(99, 64 * (eng.kv.alloc.free_blocks - 1))
+    assert eng.kv.alloc.free_blocks == 1
+    eng._need_blocks([(a.seq_id, 1), (b.seq_id, 1)])
+    eng.decode([a, b])
+    assert eng.kv.alloc.free_blocks == 0 and a.output == b.output
