@@ -951,7 +951,8 @@ class Engine:
                 live = [s for s in live if len(s.output) < max_new_tokens and (eos is None or s.output[-1] != eos)]
                 if not live:
                     return [list(s.output) for s in seqs]
-                self.decode(live)
+                for at in range(0, len(live), DECODE_BUCKETS[-1]):
+                    self.decode(live[at: at + DECODE_BUCKETS[-1]])
         finally:
             for s in seqs:
                 self.free_sequence(s.seq_id)

@@ -2,7 +2,9 @@
 import pytest
 import torch
 
+from flyingfish_b200.engine.engine import DECODE_BUCKETS
 from flyingfish_b200.engine.kv_cache import PagedKVCache
+from flyingfish_b200.engine.sampling import Sampling
 from flyingfish_b200.loaders.safetensors_io import SafetensorsFile
 from flyingfish_b200.ops import kv4_ops
 from flyingfish_b200.utils.prefix_cache import restore_prefix, save_prefix
@@ -104,3 +106,16 @@ def test_a_step_over_forks_taken_back_needs_the_copies_that_are_made_cpu():
     eng._need_blocks([(a.seq_id, 1), (b.seq_id, 1)])
     eng.decode([a, b])
     assert eng.kv.alloc.free_blocks == 0 and a.output == b.output
+
+
+def test_more_samples_than_a_decode_step_takes_cpu():
+    """Samples are decoded in groups of what a step takes; the engine goes on afterwards."""
+    m = _load("cpu")
+    ids = _prompt(20)
+    how = [Sampling(temperature=0.9, seed=s) for s in range(DECODE_BUCKETS[-1] + 3)]
+    m.engine.kv = PagedKVCache(m.spec.layers, m.engine.kv.kv_heads, m.engine.kv.head_dim, 300, kv_format="affine4")
+    got = m.generate_samples(ids, how, 3)
+    assert [len(g) for g in got] == [3] * len(how) and not m.engine.poisoned
+    for i in (0, 100, len(how) - 1):
+        assert got[i] == m.engine.generate([ids], 3, sampling=how[i])[0]
+    assert m.engine.kv.alloc.free_blocks == 300
