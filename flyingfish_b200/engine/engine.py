@@ -936,15 +936,17 @@ class Engine:
     # -- convenience ---------------------------------------------------------------------------
     def sample(self, prompt: list[int], settings: list[Sampling], max_new_tokens: int, eos: int | None = None, adapter: str | None = None) -> list[list[int]]:
         """Continuations of one prompt, one per entry of ``settings``, drawn side by side: the prompt is computed once and its cache blocks are shared. A
-        continuation ends after ``eos`` or ``max_new_tokens``."""
+        continuation ends after ``eos`` or ``max_new_tokens``. Any number of settings, as far as the cache has blocks (``OutOfBlocks``, after which the engine goes on)."""
         if not settings:
             return []
         seqs = [self.add_sequence(prompt, sampling=settings[0], adapter=adapter)]
         try:
+            self._need_blocks([(seqs[0].seq_id, len(prompt))])
             self.prefill(seqs)
             for h in settings[1:]:
                 seqs.append(self.fork(seqs[0], h, again=True))
             if len(seqs) > 1:
+                self._need_blocks([(s.seq_id, 1) for s in seqs[1:]])
                 self.prefill(seqs[1:])
             live = seqs
             while True:

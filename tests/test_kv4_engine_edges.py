@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from flyingfish_b200.engine.engine import DECODE_BUCKETS
-from flyingfish_b200.engine.kv_cache import PagedKVCache
+from flyingfish_b200.engine.kv_cache import OutOfBlocks, PagedKVCache
 from flyingfish_b200.engine.sampling import Sampling
 from flyingfish_b200.loaders.safetensors_io import SafetensorsFile
 from flyingfish_b200.ops import kv4_ops
@@ -119,3 +119,13 @@ def test_more_samples_than_a_decode_step_takes_cpu():
     for i in (0, 100, len(how) - 1):
         assert got[i] == m.engine.generate([ids], 3, sampling=how[i])[0]
     assert m.engine.kv.alloc.free_blocks == 300
+
+
+def test_samples_that_the_cache_does_not_hold_leave_the_engine_usable_cpu():
+    m = _load("cpu")
+    ids, blocks = _prompt(65), m.engine.kv.num_blocks
+    how = [Sampling(temperature=0.9, seed=s) for s in range(blocks + 2)]
+    with pytest.raises(OutOfBlocks):
+        m.generate_samples(ids, how, 3)
+    assert not m.engine.poisoned and m.engine.kv.alloc.free_blocks == blocks and not m.engine.seqs
+    assert len(m.generate_samples(ids, how[:3], 3)) == 3
