@@ -1,6 +1,14 @@
-"""Stored prefixes, forks and samples over 4-bit pages, where they meet other formats, full caches and many settings."""
+"""Stored prefixes, forks and samples over 4-bit pages, where they meet other formats, full caches and many settings; two ranks; logits on the device."""
+import json
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
+
+from _oracle import assert_tokens_equal_up_to_ties
 
 from flyingfish_b200.engine.engine import DECODE_BUCKETS
 from flyingfish_b200.engine.kv_cache import OutOfBlocks, PagedKVCache
@@ -129,3 +137,17 @@ def test_samples_that_the_cache_does_not_hold_leave_the_engine_usable_cpu():
         m.generate_samples(ids, how, 3)
     assert not m.engine.poisoned and m.engine.kv.alloc.free_blocks == blocks and not m.engine.seqs
     assert len(m.generate_samples(ids, how[:3], 3)) == 3
+
+
+def test_two_ranks_over_4_bit_pages_cpu(tmp_path):
+    """Each rank's pages hold its share of the heads (one at least); tokens are those of one rank, up to ties (the ranks' sums are added in another order)."""
+    prompts, out = [_prompt(100), _prompt(9, 12)], tmp_path / "out.json"
+    (tmp_path / "in.json").write_text(json.dumps(prompts))
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1", "--master-port", "29541",
+           str(Path(__file__).resolve().parent / "kv4_tp_worker.py"), str(tmp_path / "in.json"), str(out)]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=600, env=dict(os.environ, OMP_NUM_THREADS="2"))
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-4000:]
+    got, m = json.loads(out.read_text()), _load("cpu", capacity=256)
+    assert got["page"][1:] == [max(1, m.engine.kv.kv_heads // 2), kv4_ops.page_bytes(m.engine.model.d)]
+    for p, want, tokens in zip(prompts, m.generate_batch(prompts, 8), got["tokens"]):
+        assert_tokens_equal_up_to_ties(m, p, want, tokens)
