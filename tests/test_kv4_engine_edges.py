@@ -3,6 +3,7 @@ import json
 import os
 import subprocess
 import sys
+from dataclasses import replace
 from pathlib import Path
 
 import pytest
@@ -151,3 +152,67 @@ def test_two_ranks_over_4_bit_pages_cpu(tmp_path):
     assert got["page"][1:] == [max(1, m.engine.kv.kv_heads // 2), kv4_ops.page_bytes(m.engine.model.d)]
     for p, want, tokens in zip(prompts, m.generate_batch(prompts, 8), got["tokens"]):
         assert_tokens_equal_up_to_ties(m, p, want, tokens)
+
+
+def _plain(seq):
+    """The sequence without its settings, which a forward over given tokens refuses."""
+    return replace(seq, draws=None)
+
+
+# ------------------------------------------------------------------------------------------
+# on the device
+# ------------------------------------------------------------------------------------------
+# Two computations of the same model quantise keys and values whose last bits differ: a code next to a border falls on either side of it. Were all codes so, an element
+# would be off by two independent errors of half a step (1 / 15 of a group's span, some four standard deviations, over sqrt(12): 0.08 of a standard deviation each), 0.11 in
+# the root mean square, and what is made of them as much at most where attention's average takes nothing off it. Attention over the wrong pages moves these logits by 1 and more.
+APART = 0.11
+
+
+def _off(x, y):
+    return float((x.float().cpu() - y.float().cpu()).norm() / y.float().norm().cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 64, 300])
+def test_logits_are_those_of_the_host(n):
+    """Of a prompt in portions, of rows behind it and of a decode step in a captured graph, and the pages of the last layer, whose keys depend on every attention before."""
+    got, want, kept = [], [], []
+    for device, out in (("cuda", got), ("cpu", want)):
+        m = _load(device, graph=device == "cuda", capacity=512)
+        eng = m.engine
+        other, seq = eng.add_sequence(_prompt(90, 5)), eng.add_sequence(_prompt(n))
+        eng.prefill([other, seq], chunk=70)
+        out.append(eng.forward_rows(seq, _prompt(40, 3)).clone())                    # prompt rows, in tiles on the device
+        out.append(eng.forward_rows(seq, _prompt(3, 4)).clone())                     # a few
+        for token in _prompt(66, 6):                                                 # given tokens, so that both sides see the same ones
+            other.pending, seq.pending = 7, token
+            _, logits, _ = eng._launch_decode([other, seq])
+            logits = logits[1:2].cpu()                                               # (the next step writes this one's host buffer)
+            for s in (other, seq):
+                eng.kv.commit(s.seq_id, 1)
+        out.append(logits)
+        kv, layer = eng.kv, m.spec.layers - 1
+        slots = torch.tensor([kv.seqs[seq.seq_id].blocks[p // 64] * 64 + p % 64 for p in range(n + 66)], dtype=torch.int32, device=device)
+        out += list(kv4_ops.read_kv4(kv.k[layer], kv.v[layer], slots, eng.model.d))
+        kept.append(m)
+    assert kept[0].engine.stats["graph_replays"] == 66
+    for x, y in zip(got, want):
+        assert x.shape == y.shape and bool(torch.isfinite(x).all()) and _off(x, y) < APART
+    assert _off(got[0][1:], want[0][:-1]) > 3 * APART                                # rows of neighbouring places differ by far more
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_format", ["bf16", "affine4"])
+def test_each_sample_starts_from_a_separate_requests_logits(kv_format):
+    m = _load("cuda", kv_format=kv_format, graph=True, capacity=512)
+    eng, ids = m.engine, _prompt(200)
+    alone = eng.add_sequence(ids)
+    eng.prefill([alone])
+    eng.kv.truncate(alone.seq_id, len(ids) - 1)
+    want = eng.forward_rows(alone, ids[-1:]).clone()
+    whole = eng.add_sequence(ids)
+    eng.prefill([whole])
+    forks = [eng.fork(whole, Sampling(temperature=0.9, seed=s), again=True) for s in (3, 4, 5)]
+    for f in forks:
+        assert _off(eng.forward_rows(_plain(f), ids[-1:]), want) < APART
+    assert len(eng.prefill(forks)) == 3
