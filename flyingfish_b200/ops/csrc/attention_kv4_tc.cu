@@ -24,7 +24,6 @@
 // Every wait is bounded; a time-out records FF_ERR_TIMEOUT, and all roles leave through the abort flag.
 #include "kv4.cuh"
 #include "host_util.h"
-#include "launchers.h"
 
 namespace ff {
 
@@ -45,11 +44,6 @@ struct alignas(8) KvtBars {
   int abort_flag;
 };
 
-__device__ __forceinline__ float kvt_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // nibbles at bits 0 and 16 (HIGH: 4 and 20) times scale plus lo as FP16, one rounding (1024 + n, 64 + n are FP16 numbers, the difference is exact)
 template <bool HIGH>
 __device__ __forceinline__ uint32_t kvt_value(uint32_t w, uint32_t scale2, uint32_t lo2) {
@@ -57,25 +51,11 @@ __device__ __forceinline__ uint32_t kvt_value(uint32_t w, uint32_t scale2, uint3
   asm("{\n\t.reg .b32 t;\n\tadd.rn.f16x2 t, %1, %2;\n\tfma.rn.f16x2 %0, t, %3, %4;\n\t}" : "=r"(r) : "r"(n), "r"(HIGH ? 0xd400d400u : 0xe400e400u), "r"(scale2), "r"(lo2));
   return r;
 }
-__device__ __forceinline__ uint32_t kvt_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t kvt_prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-  return r;
-}
 
 template <int D>
 __device__ __forceinline__ void kvt_load(uint32_t (&dst)[D / 32], uint32_t src) {
   if (D == 128) kv4_lds(src, dst[0], dst[1], dst[D / 32 - 2], dst[D / 32 - 1]);
   else kv4_lds(src, dst[0], dst[1]);
-}
-__device__ __forceinline__ void kvt_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
 // Several sequences of long contexts, which differ: one CTA makes a list of what there is to do, long tile pairs cut into pieces of equal size, the largest first (the
@@ -306,9 +286,9 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float2 sl = unpack_bf16x2(kv4_mul2(stat[part][i][g], part ? by.y : by.x));
-            const uint32_t scale2 = kvt_f16x2(sl.x, sl.x), lo2 = kvt_f16x2(sl.y, sl.y);
+            const uint32_t scale2 = kv4_f16x2(sl.x, sl.x), lo2 = kv4_f16x2(sl.y, sl.y);
             // values: 16-bit unit g of two chunks, the even elements and the odd ones
-            const uint32_t word = part ? kvt_prmt(code[1][i][g / 2], code[1][i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[0][i][g];
+            const uint32_t word = part ? kv4_prmt(code[1][i][g / 2], code[1][i][NG / 2 + g / 2], (g & 1) ? 0x7632u : 0x5410u) : code[0][i][g];
             v[i][0] = kvt_value<false>(word, scale2, lo2); v[i][1] = kvt_value<true>(word, scale2, lo2);
             v[i][2] = kvt_value<false>(word >> 8, scale2, lo2); v[i][3] = kvt_value<true>(word >> 8, scale2, lo2);
           }
@@ -341,8 +321,8 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         if (lane == 0) {
           const size_t at = ((size_t)blk * hkv + kvh) * PB;
           mbar_expect_tx(&bars.p_in[pr.s], 2 * PB);
-          kvt_bulk_load(sP + pr.s * 2 * PB, kpages + at, PB, &bars.p_in[pr.s]);
-          kvt_bulk_load(sP + pr.s * 2 * PB + PB, vpages + at, PB, &bars.p_in[pr.s]);
+          kv4_bulk_load(sP + pr.s * 2 * PB, kpages + at, PB, &bars.p_in[pr.s]);
+          kv4_bulk_load(sP + pr.s * 2 * PB + PB, vpages + at, PB, &bars.p_in[pr.s]);
         }
         __syncwarp();
         pr.next(KVT_PAGES);
@@ -451,7 +431,7 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
         for (int k = 0; k < D / 8; ++k) {
           uint32_t x[4];
 #pragma unroll
-          for (int z = 0; z < 4; ++z) { const float2 v = unpack_bf16x2(w[4 * k + z]); x[z] = kvt_f16x2(v.x * down, v.y * down); }
+          for (int z = 0; z < 4; ++z) { const float2 v = unpack_bf16x2(w[4 * k + z]); x[z] = kv4_f16x2(v.x * down, v.y * down); }
           kv4_sts(dst + (k >> 3) * (KVT_M * 128) + (((k & 7) ^ (row & 7)) << 4), x[0], x[1], x[2], x[3]);
         }
         fence_proxy_async_smem();
@@ -530,8 +510,8 @@ kv4_tiles_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict_
           for (int k = 0; k < 16; ++k) {
             float a, e;
             f2_unpack(f2_fma(f2_pack(s[32 * h + 2 * k], s[32 * h + 2 * k + 1]), scale2, off2), a, e);
-            a = kvt_ex2(a); e = kvt_ex2(e);
-            pk[k] = kvt_f16x2(a, e);
+            a = kv4_ex2(a); e = kv4_ex2(e);
+            pk[k] = kv4_f16x2(a, e);
             sum = f2_add(sum, f2_pack(a, e));
           }
           tmem_st_x16(s_addr + 16 * h, pk);
@@ -610,7 +590,7 @@ kv4_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ par
       M = warp_max(M);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ml[i].x = ml[i].y == 0.f ? 0.f : kvt_ex2(ml[i].x - M);              // (a piece of no weight has left nothing)
+        ml[i].x = ml[i].y == 0.f ? 0.f : kv4_ex2(ml[i].x - M);              // (a piece of no weight has left nothing)
         L = fmaf(ml[i].y, ml[i].x, L);
       }
       L = warp_sum(L);
