@@ -3,9 +3,9 @@
 operators; mirrors src/kv.rs:5-133 and kernels/kv_cache.cuh of the reference (format identities, sealed
 boundary, ring slots, compact block sizes).
 
-The attention kernels of this engine read BF16 pages; ``Affine8Store`` is the compact store behind them:
+With the first two formats the attention kernels read BF16 pages; ``Affine8Store`` is the compact store behind them:
 ``seal`` packs every group that has left the recent window, ``materialise`` rebuilds BF16 rows for a token
-range (used when a sequence is paged back in or handed to another rank). ``affine4`` is a format of the paged cache's blocks themselves (``ops.kv4_ops``)."""
+range (used when a sequence is paged back in or handed to another rank). ``affine4`` is a format of the paged cache's blocks themselves, which kernels of its own read (``ops.kv4_ops``)."""
 from __future__ import annotations
 
 from dataclasses import dataclass

@@ -51,8 +51,8 @@ __device__ __forceinline__ void kv4_words(uint32_t (&dst)[NG], uint32_t src) {
 // A CTA has NT x 8 columns and a range of pages; every warp takes pages of its own, fetched by bulk copies into its two slots (keys, values),
 // with its own running maximum, sum and O. The warps' results meet in shared memory, those of up to eight CTAs (splits) in that of
 // their cluster, those of more in kv4_merge_kernel.
-// Bound by issue slots, not by the 5 bits an element of traffic: three sequences of up to 131071 tokens, 64 / 8 heads: 97 us for 474 MB (4.9 TB/s of the 6.5 a copy
-// reaches) before the power of two, which adds 1 to 2 % (50 instructions to 1195 a page and warp; 60 % of the slots taken, the integer pipe 54 % busy). Columns by 8 keep 128 registers and four CTAs on an SM, by 16 (more
+// Bound by issue slots, not by the 5 bits an element of traffic: three sequences of up to 131071 tokens, 64 / 8 heads: 102 us for 474 MB (4.6 TB/s of the 6.5 a copy
+// reaches), 1267 instructions a page and warp, 72 of them for the power of two (1 to 2 % of the time); 61 % of the slots taken, the integer pipe 55 % busy. Columns by 8 keep 128 registers and four CTAs on an SM, by 16 (more
 // than 8 columns) they share a page's unpacking. Codes turned into BF16 operands first took 204 us, as subnormal ones 136, sums of p lo as a product 109.
 constexpr int KV4_WARPS = 4, KV4_SLOTS = 2;      // (a warp for every group of a head at least)
 constexpr int KV4_KEPT = 4;                      // binades that a page's values may lie below the power of two that a warp has for them

@@ -72,7 +72,8 @@ struct KvtPlan {
 constexpr int KVT_PLAN_WARPS = 16, KVT_CLASSES = 32, KVT_CUTS = 4, KVT_SHARE = 2;
 constexpr int KVT_EXTRA = 6, KVT_PART = 4;                                // pages' time that a CTA takes beside its pages, and for a part's way out and in again
 constexpr int KVT_SEQS = 2048;                                            // sequences of a list at most
-// Pages of a context from which a list is made. It takes 6 us: 100 x 5 rows behind up to 2000 tokens 76 us as they lie and 89 by a list, 8 x 64 behind up to 4000 75 and 58.
+// Pages of a context from which a list is made. It takes 6 us and more where it cuts: 100 x 5 rows behind up to 2000 tokens 80 us as they lie and 93 by a list, 8 x 64 behind up to 4000 67 and 63, 500
+// of 4 behind 60000 374 and 116. It is not right for every call: 4 x 5 rows (64 / 4 heads) behind up to 30000 take 73 and 83, 10 x 16 behind 10000 124 and 132, 24 x 5 behind up to 4000 61 and 65.
 constexpr int KVT_LIST = 32;
 
 __device__ __forceinline__ int kvt_pages(int past, int c0, int rows, int G) { return (max(past + (c0 + min(rows, 2 * KVT_M) - 1) / G + 1, 0) + KVT_N - 1) / KVT_N; }

@@ -70,7 +70,8 @@ __device__ __forceinline__ uint32_t kv4_quantise(const uint32_t (&w)[4], uint32_
 // once. Norm and turn round as the BF16 cache's kernel does: every product and sum to BF16 (packed instructions; a sum of two BF16 numbers that FP32 does not
 // hold has a term too small to matter). Few rows are spread over CTAs by heads. 8191 rows of 64 + 2 x 8 heads of 128: 78 us, 4.2 TB/s, where the bytes alone take 50: issue
 // slots are 63 % taken, warps wait for their loads in between. With FP64 for all codes of a lane that has one in doubt (a third of the warps have) 82, with three
-// heads at once 102, with 80 registers and three CTAs 90.
+// heads at once 102, with 80 registers and three CTAs 90. Five heads at once are 80 heads in one round of 16 sets of lanes; other numbers lose up to 7 % by it: 48 heads 65 us where three at
+// once take 62, 10 heads 43 and 40, 36 of 64 elements 45 and 44, 96 heads 138 and 132.
 constexpr int WRITE_THREADS = 256, WRITE_HEADS = 5;
 template <int D, bool NORM>
 __global__ void __launch_bounds__(WRITE_THREADS, 4)
@@ -187,7 +188,7 @@ kv4_write_kernel(const __nv_bfloat16* __restrict__ qkv, const int* __restrict__ 
 }
 
 // What the pages hold for given slots, rounded to BF16; rows of a slot below 0 are zero. D / 8 lanes a head, 8 elements each. The 8191 rows above, 34 MB of
-// results from 21 MB of pages: 22 us with its launch, where the bytes take 8.
+// results from 21 MB of pages: 23 us with its launch, where the bytes take 8: a thread makes one 16-byte result and has nothing else in flight, and values come as two 16-bit loads.
 template <int D>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const uint8_t* __restrict__ kpages, const uint8_t* __restrict__ vpages, const int* __restrict__ slots, __nv_bfloat16* __restrict__ kout,

@@ -4,7 +4,8 @@ A page holds 64 tokens of one head of 64 or 128 elements (``uint8 [num_blocks, k
 values). Groups of 32 neighbouring elements of a token share two BF16 numbers, and an element stands for ``code * scale + lo``: ``lo`` is the
 group's least element, ``scale`` its span / 15 rounded to BF16, a code is 0 .. 15, rounded to the nearest with ties to even. What an
 element stands for is off by half a scale at most, and by the rounding of the scale (2^-8 of it for each step up to 15). That is 160 bytes a token and
-head of 128 where BF16 pages take 512. Every token is quantised by itself, so rows may be taken back and written again, and pages may be copied.
+head of 128 where BF16 pages take 512. Every token is quantised by itself, so rows may be taken back and written again, and pages may be copied. Elements are
+2^15 at most; there is no least size, attention is as exact for small values as for others.
 
 CUDA: ``csrc/kv4.cu``, ``csrc/attention_kv4.cu`` and ``csrc/attention_kv4_tc.cu``; the byte layout is in ``csrc/kv4.cuh``. CPU: the oracles below. Slots, block tables and lengths are
 those of the BF16 cache (``ops.rope_kv_paged``, ``ops.attn_decode``, ``ops.attn_prefill``). Calls keep no state of their own and share no scratch: any stream may
@@ -22,7 +23,7 @@ from .lib import KernelError, check, kernels, status_tensor
 PAGE = 64
 GROUP = 32
 DIMS = (64, 128)
-MOST = 2.0 ** 15                  # greatest magnitude of an element: FP16 holds it
+MOST = 2.0 ** 15                  # greatest magnitude of an element
 
 
 def page_bytes(dim: int) -> int:
@@ -293,7 +294,8 @@ def _attention_ref(q, kpages, vpages, block_table, q_start, q_lens, ctx_lens, hq
 def in_tiles(max_q_len: int, hq: int, hkv: int) -> bool:
     """Whether attention of so many rows per sequence takes the kernel for prompts: FP16 tiles in shared memory for tcgen05 products of 128 rows, where
     the other one multiplies 8 or 16 rows by codes as they are. A sequence's rows times the query heads of a kv head are what counts: 24 sequences of up to 4000 tokens
-    over 4 kv heads take 48 us with 32 such rows (57 in tiles), 63 in tiles with 80 (83); one of 30000 over 8 takes 31 with 32 (39), 40 in tiles with 64 (52)."""
+    over 4 kv heads take 57 us with 32 such rows (58 in tiles), 65 in tiles with 80 (86); one of 30000 over 8 takes 38 with 32 (46), 46 in tiles with 64 (56). Contexts count too, and the
+    rule leaves them out: a prompt of 37 rows with 4 heads each takes 14 either way, behind 1000 tokens 24 in tiles (20 as rows), behind 10000 34 (55); one of 100 rows alone 16 (14)."""
     return max_q_len * (hq // hkv) > 32
 
 
